@@ -540,6 +540,45 @@ int b200_peer_allreduce_apply_f32(float* data, int64_t n, const void* bufs_dev, 
                                   const int64_t* offsets, float* const* param, float* const* s1, float* const* s2, float lr,
                                   void* stream);
 
+/* ------------------------------------------------------------------------------
+ * Rotary positions of attention heads, and the RMS norm of queries and keys per head with
+ * that rotation in the same pass. No counterpart in the reference: its graphs add learned
+ * positions (the transformer workload) and norm whole rows (LayerNorm).
+ *
+ * Pair j < rotary_dim / 2 of a head is (j, j + rotary_dim / 2), or (2j, 2j + 1) when
+ * interleaved; it turns by position * turns[j] / 2^64 of a full turn and is scaled by
+ * factor. Elements from rotary_dim on are not rotated.
+ *   rotary_heads:         y = R(x), or the gradient R^T(x) with inverse != 0
+ *   qk_norm_rotary:       y = R(x rsqrt(mean(x^2) + eps) gamma) of the queries and the keys
+ *   qk_norm_rotary_grad:  dq, dk from the gradients of both results; dgamma_q / dgamma_k
+ *                         (fp32 [head_dim], may be NULL) summed over tokens and heads in a
+ *                         fixed order
+ * Tensors are [batch, seq, heads, head_dim] of dtype F32 or BF16, the head's elements
+ * adjacent, element strides of the other axes given (x_b, x_s, x_h and so on; for the
+ * gradient 2 x 9: input, upstream gradient, result of the queries, then of the keys). A
+ * result may be written over its input (same strides), over no other tensor. gamma: [head_dim] F32 or BF16, NULL: ones. positions (I64 or
+ * I32, any sign) have element strides pos_b, pos_s; NULL: offset + index in the sequence. */
+#define B200_ROTARY_MAX_DIM 512
+typedef struct b200_rotary {
+  int32_t head_dim, rotary_dim, interleaved;
+  float factor;
+  uint64_t turns[B200_ROTARY_MAX_DIM / 2]; /* fraction of a turn per position, times 2^64 */
+} b200_rotary;
+int b200_rotary_heads(const b200_rotary* r, int dtype, const void* x, void* y, int64_t batch, int64_t seq, int64_t heads,
+                      int64_t x_b, int64_t x_s, int64_t x_h, int64_t y_b, int64_t y_s, int64_t y_h, const void* positions,
+                      int pos_dtype, int64_t pos_b, int64_t pos_s, int64_t offset, int inverse, void* stream);
+int b200_qk_norm_rotary(const b200_rotary* r, int dtype, const void* q, const void* k, void* yq, void* yk, int64_t batch, int64_t seq,
+                        int64_t heads_q, int64_t heads_k, int64_t q_b, int64_t q_s, int64_t q_h, int64_t k_b, int64_t k_s,
+                        int64_t k_h, int64_t yq_b, int64_t yq_s, int64_t yq_h, int64_t yk_b, int64_t yk_s, int64_t yk_h,
+                        const void* gamma_q, const void* gamma_k, int gamma_dtype, float eps, const void* positions, int pos_dtype,
+                        int64_t pos_b, int64_t pos_s, int64_t offset, void* stream);
+size_t b200_qk_norm_rotary_grad_workspace_bytes(int64_t head_dim);
+int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, const void* dyk, const void* q, const void* k, void* dq,
+                             void* dk, int64_t batch, int64_t seq, int64_t heads_q, int64_t heads_k, const int64_t* strides,
+                             const void* gamma_q, const void* gamma_k, int gamma_dtype, float eps, const void* positions, int pos_dtype,
+                             int64_t pos_b, int64_t pos_s, int64_t offset, float* dgamma_q, float* dgamma_k, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -61,6 +61,21 @@ class EwProgram(C.Structure):
     ]
 
 
+ROTARY_MAX_DIM = 512
+
+
+class Rotary(C.Structure):
+    _fields_ = [
+        ("head_dim", C.c_int32),
+        ("rotary_dim", C.c_int32),
+        ("interleaved", C.c_int32),
+        ("factor", C.c_float),
+        ("turns", C.c_uint64 * (ROTARY_MAX_DIM // 2)),
+    ]
+
+
+I64x18 = C.c_int64 * 18
+
 _P, _I64, _I32, _F32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
 
 SIGNATURES = {
@@ -129,6 +144,17 @@ SIGNATURES = {
     "b200_gemm_batched2_residual": ([_P, _P, _P] + [_I64] * 16 + [_P, _P, _P], C.c_int),
     "b200_conv2d_dgrad_igemm": ([_P, _P, _P, _P, _P, _I64, _P, _P] + [_I64] * 13 + [_P, C.c_size_t, _P], C.c_int),
     "b200_conv2d_wgrad_igemm": ([_P, _P, _P, _P, _P] + [_I64] * 13 + [_P, C.c_size_t, _P], C.c_int),
+    "b200_rotary_heads": ([C.POINTER(Rotary), _I32, _P, _P] + [_I64] * 9 + [_P, _I32, _I64, _I64, _I64, _I32, _P], C.c_int),
+    "b200_qk_norm_rotary": (
+        [C.POINTER(Rotary), _I32, _P, _P, _P, _P] + [_I64] * 16 + [_P, _P, _I32, _F32, _P, _I32, _I64, _I64, _I64, _P],
+        C.c_int,
+    ),
+    "b200_qk_norm_rotary_grad_workspace_bytes": ([_I64], C.c_size_t),
+    "b200_qk_norm_rotary_grad": (
+        [C.POINTER(Rotary), _I32] + [_P] * 6 + [_I64] * 4 + [C.POINTER(_I64), _P, _P, _I32, _F32, _P, _I32, _I64, _I64, _I64, _P, _P,
+                                                             _P, C.c_size_t, _P],
+        C.c_int,
+    ),
     "b200_conv2d_fwd": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_dgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_wgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),

@@ -1,0 +1,274 @@
+"""Language-model operators: rotary positions, query / key norms, the vocabulary loss and
+the orthogonalised update.
+
+They have no counterpart in the reference's op vocabulary. They follow the conventions of
+``ops``: values are ``torch.Tensor`` on the current CUDA device, results are fresh tensors,
+all arithmetic runs in libb200.so, gradients are separate operators (as the reference's
+``LayerNormInputGrad``), ``execute_op`` reaches them by name.
+"""
+
+from __future__ import annotations
+
+import functools
+import math
+from typing import Any, Mapping
+
+import torch
+
+from . import _lib as L
+from . import ops
+from .errors import BackendNotSupportedError
+
+_FLOATS = (torch.float32, torch.bfloat16)
+
+
+def _on_device(name: str, *tensors: torch.Tensor | None) -> None:
+    """The kernels run on the current device's stream: operands elsewhere are refused."""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != dev):
+            raise ValueError(f"{name}: operand on {t.device}, the current device is cuda:{dev}")
+
+
+# ----------------------------------------------------------------------------------
+# rotary positions
+# ----------------------------------------------------------------------------------
+
+_SCALING_KEYS = {
+    "linear": ({"factor"}, set()),
+    "ntk": ({"factor"}, set()),
+    "yarn": ({"factor", "original_length"}, {"beta_fast", "beta_slow", "attention_factor"}),
+    "wavelength": ({"factor", "original_length", "low_factor", "high_factor"}, set()),
+}
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: Mapping[str, Any] | None = None) -> tuple[list[float], float]:
+    """Angle per position (radians) of each of the rotary_dim / 2 pairs, and the factor on
+    cosine and sine.
+
+    Pair j turns by ``base ** (-2 j / rotary_dim)`` per position. ``scaling`` stretches
+    that to contexts ``factor`` times as long as the angles were made for:
+
+    * ``{"kind": "linear", "factor": f}``: every angle divided by f;
+    * ``{"kind": "ntk", "factor": f}``: base times f ** (d / (d - 2)), so the slowest pair
+      is divided by f and the fastest keeps its angle;
+    * ``{"kind": "yarn", "factor": f, "original_length": n}`` (``beta_fast`` 32,
+      ``beta_slow`` 1, ``attention_factor`` 0.1 ln f + 1): pairs that turn less than
+      beta_slow times over n positions are divided by f, pairs that turn more than
+      beta_fast times are kept, a linear ramp over the pair index between; cosine and sine
+      are multiplied by the attention factor;
+    * ``{"kind": "wavelength", "factor": f, "original_length": n, "low_factor": a,
+      "high_factor": b}``: the same by the turns over n positions themselves, a ramp from a
+      (divided) to b (kept).
+    """
+    inv = [base ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)]
+    if scaling is None:
+        return inv, 1.0
+    kind = scaling.get("kind")
+    if kind not in _SCALING_KEYS:
+        raise ValueError(f"rotary scaling kind {kind!r} is not one of {sorted(_SCALING_KEYS)}")
+    need, may = _SCALING_KEYS[kind]
+    given = set(scaling) - {"kind"}
+    if not need <= given or not given <= need | may:
+        raise ValueError(f"rotary scaling {kind!r} takes {sorted(need)} and optionally {sorted(may)}, got {sorted(given)}")
+    f = float(scaling["factor"])
+    if not (f >= 1.0 and math.isfinite(f)):
+        raise ValueError(f"rotary scaling factor {f} is not a finite number >= 1")
+    if kind == "linear":
+        return [w / f for w in inv], 1.0
+    if kind == "ntk":
+        b = base * f ** (rotary_dim / (rotary_dim - 2.0)) if rotary_dim > 2 else base
+        return [b ** (-2.0 * j / rotary_dim) for j in range(rotary_dim // 2)], 1.0
+    n = float(scaling["original_length"])
+    if not (n > 0 and math.isfinite(n)):
+        raise ValueError(f"rotary scaling original_length {n} is not a positive number")
+    if kind == "yarn":
+        fast, slow = float(scaling.get("beta_fast", 32.0)), float(scaling.get("beta_slow", 1.0))
+        if not (fast >= slow > 0):
+            raise ValueError(f"rotary scaling needs beta_fast >= beta_slow > 0, got {fast} and {slow}")
+        pair = [rotary_dim * math.log(n / (b * 2 * math.pi)) / (2 * math.log(base)) for b in (fast, slow)]
+        low, high = max(math.floor(pair[0]), 0), min(math.ceil(pair[1]), rotary_dim - 1)
+        ramp = [min(1.0, max(0.0, (j - low) / max(high - low, 0.001))) for j in range(rotary_dim // 2)]
+        factor = float(scaling.get("attention_factor", 0.1 * math.log(f) + 1.0))
+        return [w * (1 - t) + w / f * t for w, t in zip(inv, ramp)], factor
+    low, high = float(scaling["low_factor"]), float(scaling["high_factor"])
+    if not high > low > 0:
+        raise ValueError(f"rotary scaling needs high_factor > low_factor > 0, got {high} and {low}")
+    keep = [min(1.0, max(0.0, (n * w / (2 * math.pi) - low) / (high - low))) for w in inv]
+    return [w * t + w / f * (1 - t) for w, t in zip(inv, keep)], 1.0
+
+
+@functools.lru_cache(maxsize=256)
+def _rotary_table(head_dim: int, rotary_dim: int, base: float, interleaved: bool, scaling: tuple | None) -> L.Rotary:
+    """The kernels' description of a rotation: each pair's fraction of a turn per position in
+    64-bit fixed point, so that position * turns is exact modulo one turn."""
+    if not 1 <= head_dim <= L.ROTARY_MAX_DIM:
+        raise ValueError(f"rotary: head_dim {head_dim} not in [1, {L.ROTARY_MAX_DIM}]")
+    if rotary_dim % 2 or not 0 <= rotary_dim <= head_dim:
+        raise ValueError(f"rotary: rotary_dim {rotary_dim} must be even and in [0, head_dim = {head_dim}]")
+    if not (base > 1.0 and math.isfinite(base)):
+        raise ValueError(f"rotary: base {base} is not a finite number > 1")
+    inv, factor = rotary_frequencies(rotary_dim, base, None if scaling is None else dict(scaling))
+    r = L.Rotary()
+    r.head_dim, r.rotary_dim, r.interleaved, r.factor = head_dim, rotary_dim, int(interleaved), factor
+    for j, w in enumerate(inv):
+        r.turns[j] = round(w / (2 * math.pi) * 2.0**64) % 2**64
+    return r
+
+
+def _rotary(head_dim: int, rotary_dim, base, interleaved, scaling) -> L.Rotary:
+    key = None if scaling is None else tuple(sorted(scaling.items()))
+    return _rotary_table(head_dim, head_dim if rotary_dim is None else int(rotary_dim), float(base), bool(interleaved), key)
+
+
+def _heads(name: str, x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, tuple[int, int, int]]:
+    """x [batch, seq, heads, dim] or [seq, heads, dim] -> x with adjacent head elements, its
+    batch, seq, heads and their element strides."""
+    if x.dtype not in _FLOATS:
+        raise BackendNotSupportedError(f"{name}: {x.dtype} heads have no b200 kernel (fp32 and bf16)")
+    if x.dim() not in (3, 4):
+        raise ValueError(f"{name}: heads must be [batch, seq, heads, dim] or [seq, heads, dim], got {tuple(x.shape)}")
+    if x.stride(-1) != 1 and x.shape[-1] > 1:
+        x = ops.contiguous(x)
+    if x.dim() == 3:
+        return x, 1, x.shape[0], x.shape[1], (0, x.stride(0), x.stride(1))
+    return x, x.shape[0], x.shape[1], x.shape[2], (x.stride(0), x.stride(1), x.stride(2))
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    """A fresh result for x: dense, its axes in x's storage order, adjacent head elements."""
+    y = torch.empty_like(x)
+    return y if y.stride(-1) == 1 or y.shape[-1] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _strides(x: torch.Tensor) -> tuple[int, int, int]:
+    return (0, x.stride(0), x.stride(1)) if x.dim() == 3 else (x.stride(0), x.stride(1), x.stride(2))
+
+
+def _positions(name: str, positions: Any, offset: int, batch: int, seq: int) -> tuple[torch.Tensor | None, tuple]:
+    """positions [seq], [1, seq] or [batch, seq] of int32 / int64 -> (tensor kept alive,
+    the entry points' position arguments)."""
+    if positions is None:
+        return None, (None, L.I64, 0, 0, int(offset))
+    t = positions if isinstance(positions, torch.Tensor) and positions.is_cuda else ops.to_device(positions)
+    if t.dtype not in (torch.int64, torch.int32):
+        t = ops._int_indices(t)
+    if offset:
+        raise ValueError(f"{name}: give positions or an offset, not both")
+    if t.dim() == 0 or t.dim() > 2 or t.shape[-1] != seq or (t.dim() == 2 and t.shape[0] not in (1, batch)):
+        raise ValueError(f"{name}: positions {tuple(t.shape)} do not match {batch} sequences of {seq} tokens")
+    pb = t.stride(0) if t.dim() == 2 and t.shape[0] == batch and batch > 1 else 0
+    return t, (t.data_ptr(), ops.code(t), pb, t.stride(-1), 0)
+
+
+def _rotate(name: str, x: torch.Tensor, positions, base, rotary_dim, interleaved, scaling, offset, inverse: int) -> torch.Tensor:
+    x, batch, seq, heads, xs = _heads(name, x)
+    r = _rotary(x.shape[-1], rotary_dim, base, interleaved, scaling)
+    pos, pa = _positions(name, positions, offset, batch, seq)
+    _on_device(name, x, pos)
+    y = _like(x)
+    L.call("b200_rotary_heads", r, ops.code(x), x.data_ptr(), y.data_ptr(), batch, seq, heads, *xs, *_strides(y), *pa, inverse,
+           ops.stream_ptr())
+    return y
+
+
+def op_rotary_embedding(x, positions=None, base=10000.0, rotary_dim=None, interleaved=False, scaling=None, offset=0, **_):
+    """Rotary positions: each pair of a head's first ``rotary_dim`` elements (all by default)
+    turned by its angle (``rotary_frequencies``) times the token's position.
+
+    x: [batch, seq, heads, dim] or [seq, heads, dim], fp32 or bf16, any strides (a
+    head-major tensor is passed as its transposed view); head_dim <= 512. Pairs are (j, j +
+    rotary_dim / 2), or neighbours with ``interleaved``. positions: integers [seq], [1, seq]
+    or [batch, seq]; None: ``offset`` + 0 .. seq - 1. Computed in fp32, rounded once."""
+    return _rotate("RotaryEmbedding", x, positions, base, rotary_dim, interleaved, scaling, offset, 0)
+
+
+def op_rotary_embedding_grad(dy, positions=None, base=10000.0, rotary_dim=None, interleaved=False, scaling=None, offset=0, **_):
+    """The gradient of RotaryEmbedding's input: the rotation turned back."""
+    return _rotate("RotaryEmbeddingGrad", dy, positions, base, rotary_dim, interleaved, scaling, offset, 1)
+
+
+def _pair(name: str, q: torch.Tensor, k: torch.Tensor):
+    q, batch, seq, hq, qs = _heads(name, q)
+    k, kbatch, kseq, hk, ks = _heads(name, k)
+    if q.dim() != k.dim() or (kbatch, kseq, k.shape[-1]) != (batch, seq, q.shape[-1]):
+        raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)} differ in more than their heads")
+    if q.dtype != k.dtype:
+        raise BackendNotSupportedError(f"{name}: queries of {q.dtype} with keys of {k.dtype}")
+    return q, k, batch, seq, hq, hk, qs, ks
+
+
+def _gammas(name: str, dim: int, gq: torch.Tensor | None, gk: torch.Tensor | None):
+    """The norm weights as [dim] tensors of one dtype (fp32 if they differ)."""
+    out = []
+    for g in (gq, gk):
+        if g is not None:
+            if tuple(g.shape) != (dim,):
+                raise ValueError(f"{name}: norm weight {tuple(g.shape)}, want [{dim}]")
+            if g.dtype not in _FLOATS:
+                raise BackendNotSupportedError(f"{name}: norm weights of {g.dtype} (fp32 and bf16)")
+            g = ops.contiguous(g)
+        out.append(g)
+    if gq is not None and gk is not None and gq.dtype != gk.dtype:
+        out = [ops.cast(g, torch.float32) for g in out]
+    dt = next((ops.code(g) for g in out if g is not None), L.F32)
+    return out[0], out[1], dt
+
+
+def op_qk_norm_rotary(q, k, gamma_q=None, gamma_k=None, positions=None, eps=1e-6, base=10000.0, rotary_dim=None, interleaved=False,
+                      scaling=None, offset=0, **_):
+    """RMS norm of each query and key head, times gamma, and the rotary positions of both, in
+    one pass: returns (q', k').
+
+    q [batch, seq, heads, dim], k [batch, seq, kv_heads, dim] (or both without the batch) of
+    one dtype, any strides, so slices of one projection's result are read in place; gamma_q /
+    gamma_k [dim], None: ones. The rest as RotaryEmbedding; ``rotary_dim=0`` norms alone.
+    The norm's sum and the rotation are in fp32, rounded once."""
+    name = "QKNormRotary"
+    q, k, batch, seq, hq, hk, qs, ks = _pair(name, q, k)
+    r = _rotary(q.shape[-1], rotary_dim, base, interleaved, scaling)
+    gq, gk, gdt = _gammas(name, q.shape[-1], gamma_q, gamma_k)
+    pos, pa = _positions(name, positions, offset, batch, seq)
+    _on_device(name, q, k, gq, gk, pos)
+    yq, yk = _like(q), _like(k)
+    L.call("b200_qk_norm_rotary", r, ops.code(q), q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), batch, seq, hq, hk, *qs,
+           *ks, *_strides(yq), *_strides(yk), ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, ops.stream_ptr())
+    return yq, yk
+
+
+def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions=None, eps=1e-6, base=10000.0, rotary_dim=None,
+                           interleaved=False, scaling=None, offset=0, **_):
+    """The gradients of QKNormRotary from those of its results and its inputs:
+    (dq, dk, dgamma_q, dgamma_k), the weights' in fp32 [dim] (also where a gamma is None),
+    summed over tokens and heads in a fixed order."""
+    name = "QKNormRotaryGrad"
+    q, k, batch, seq, hq, hk, qs, ks = _pair(name, q, k)
+    if tuple(dyq.shape) != tuple(q.shape) or tuple(dyk.shape) != tuple(k.shape):
+        raise ValueError(f"{name}: gradients {tuple(dyq.shape)}, {tuple(dyk.shape)} of queries {tuple(q.shape)}, keys {tuple(k.shape)}")
+    if dyq.dtype != q.dtype or dyk.dtype != q.dtype:
+        raise BackendNotSupportedError(f"{name}: gradients of {dyq.dtype}, {dyk.dtype} for {q.dtype} heads")
+    dyq, _, _, _, dqs = _heads(name, dyq)
+    dyk, _, _, _, dks = _heads(name, dyk)
+    dim = q.shape[-1]
+    r = _rotary(dim, rotary_dim, base, interleaved, scaling)
+    gq, gk, gdt = _gammas(name, dim, gamma_q, gamma_k)
+    pos, pa = _positions(name, positions, offset, batch, seq)
+    _on_device(name, q, k, dyq, dyk, gq, gk, pos)
+    dq, dk = _like(q), _like(k)
+    dgamma = torch.empty(2, dim, dtype=torch.float32, device=q.device)
+    wn = int(L.lib().b200_qk_norm_rotary_grad_workspace_bytes(dim))
+    ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
+    st = L.I64x18(*qs, *dqs, *_strides(dq), *ks, *dks, *_strides(dk))
+    L.call("b200_qk_norm_rotary_grad", r, ops.code(q), dyq.data_ptr(), dyk.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(),
+           dk.data_ptr(), batch, seq, hq, hk, st, ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, dgamma[0].data_ptr(),
+           dgamma[1].data_ptr(), ws.data_ptr(), wn, ops.stream_ptr())
+    return dq, dk, dgamma[0], dgamma[1]
+
+
+def register(table: dict) -> None:
+    table.update({
+        "RotaryEmbedding": op_rotary_embedding,
+        "RotaryEmbeddingGrad": op_rotary_embedding_grad,
+        "QKNormRotary": op_qk_norm_rotary,
+        "QKNormRotaryGrad": op_qk_norm_rotary_grad,
+    })

@@ -1474,6 +1474,10 @@ from . import fused_nodes as _fused_nodes  # noqa: E402  (fusion-pass node types
 
 _fused_nodes.register(OPS)
 
+from . import lm_ops as _lm_ops  # noqa: E402  (rotary positions, query / key norms, vocabulary loss, orthogonalised update)
+
+_lm_ops.register(OPS)
+
 # reference aliases (interpreter/evaluator.py:771-791)
 ALIASES = {"Sub": "Subtract", "Mul": "Multiply", "Div": "TrueDivide", "Neg": "Negative", "Pow": "Power", "MatMul": "Matmul",
            "Expand": "BroadcastTo", "Permute": "Transpose"}

@@ -1,0 +1,531 @@
+// Rotary positions of heads, and the RMS norm of queries and keys per head with the same
+// rotation in one pass; both directions.
+//
+//   forward          y  = R(u gamma),  u = x rsqrt(mean(x^2) + eps)      (norm)
+//                    y  = R(x)                                           (rotation alone)
+//   backward (norm)  g  = R^-1(dy), h = g gamma, dx = rstd (h - u mean(h u)), dgamma = sum g u
+//   R rotates pair j of a head by t_j = position * w_j and scales it by `factor`:
+//                    (a, b) -> factor (a cos t - b sin t, b cos t + a sin t)
+// The pairs are (j, j + rotary_dim / 2) or, interleaved, (2j, 2j + 1); elements from
+// rotary_dim on pass through (normed, not rotated).
+//
+// Angles. w_j comes as a fraction of a turn per position in 64-bit fixed point, so
+// position * w_j modulo one turn is one wrapping integer product: exact for any position
+// (an fp32 product would be off by 0.06 rad at position 10^6). Its top 32 bits go through
+// sincospif. The table travels in the kernel's parameters: nothing is uploaded or kept.
+//
+// Layout of the work. A lane owns one unit of a head: two 16-byte vectors that hold whole
+// pairs (the two halves of V pairs, or 2V neighbours), so a rotation needs no shuffle; the
+// units of a head take L lanes (a power of two), and a warp holds R = 32 / L heads. A warp
+// takes a token and walks its heads, R at a time, with the next heads' loads in flight:
+// the lane's angles are the same for every head, so cosines and sines are made once per
+// token. Few tokens (a decoding batch) are split over head groups, so that the heads of
+// one token run on many warps; each then makes the angles again.
+// Bound by HBM: x (and dy) are read once, y (dx) written once.
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace b200 {
+namespace rot {
+
+constexpr int WARPS = 8, THREADS = 32 * WARPS;
+constexpr int ROTATE = 0, NORM = 1, NORM_GRAD = 2;
+
+struct Seg {  // one tensor of heads; element strides over batch, sequence, head (the head's elements are adjacent)
+  const void* x;
+  const void* dy;
+  void* y;
+  int64_t x_b, x_s, x_h, d_b, d_s, d_h, y_b, y_s, y_h;
+  const void* gamma;
+  int heads;
+  int groups;  // ceil(heads / R)
+};
+
+struct Args {
+  Seg seg[2];
+  const void* pos;  // NULL: offset + index in the sequence
+  int64_t pos_b, pos_s, offset;
+  int pos_i32, gamma_bf16;
+  int tokens, seq, dim, part;
+  int L, chunks, per_chunk;  // lanes per head; head groups per token are cut into chunks of per_chunk
+  int n_rot, n_units;        // units that rotate, units in all
+  float eps, factor, sign;
+  float* partial;  // [grid, 2, dim] sums of g u (NORM_GRAD)
+  uint64_t freq[B200_ROTARY_MAX_DIM / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ float to_f(T v);
+template <>
+__device__ __forceinline__ float to_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f(float v);
+template <>
+__device__ __forceinline__ float from_f<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+template <typename T, int V>
+struct alignas(sizeof(T) * V) Vec {
+  T v[V];
+};
+
+// V values at p: one vector access when FAST (n is 0 or V then), else element by element
+template <typename T, int V, bool FAST>
+__device__ __forceinline__ Vec<T, V> load_vec(const T* p, int n) {
+  Vec<T, V> r;
+  if constexpr (FAST) {
+    if (n) return *reinterpret_cast<const Vec<T, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(0.f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : from_f<T>(0.f);
+  }
+  return r;
+}
+template <typename T, int V, bool FAST>
+__device__ __forceinline__ void store_vec(T* p, const float (&x)[V], int n) {
+  if constexpr (FAST) {
+    if (!n) return;
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(x[i]);
+    *reinterpret_cast<Vec<T, V>*>(p) = r;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) p[i] = from_f<T>(x[i]);
+  }
+}
+
+template <typename T, int V, int NU>
+struct Row {
+  Vec<T, V> a[NU], b[NU];
+};
+
+// rotate the V pairs of a unit; s carries the direction's sign
+template <int V, bool INTER>
+__device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
+  if constexpr (INTER) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      float x = a[2 * i], y = a[2 * i + 1];
+      a[2 * i] = x * c[i] - y * s[i];
+      a[2 * i + 1] = y * c[i] + x * s[i];
+      x = b[2 * i], y = b[2 * i + 1];
+      b[2 * i] = x * c[V / 2 + i] - y * s[V / 2 + i];
+      b[2 * i + 1] = y * c[V / 2 + i] + x * s[V / 2 + i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = x * c[i] - y * s[i];
+      b[i] = y * c[i] + x * s[i];
+    }
+  }
+}
+
+template <typename T, int V, int NU, bool FAST, bool INTER, int MODE>
+__global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kernel(const __grid_constant__ Args A) {
+  __shared__ uint64_t freq[B200_ROTARY_MAX_DIM / 2];
+  const int half = A.part / 2;
+  for (int i = threadIdx.x; i < half; i += THREADS) freq[i] = A.freq[i];
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int L = A.L, sub = lane / L, u0 = lane % L, R = 32 / L;
+  // this lane's units: element offsets, how many elements of each vector exist, first pair
+  int o0[NU], o1[NU], n0[NU], n1[NU], f0[NU];
+  bool rot[NU];
+#pragma unroll
+  for (int k = 0; k < NU; ++k) {
+    const int u = u0 + L * k;
+    rot[k] = u < A.n_rot;
+    f0[k] = u * V;
+    if (rot[k] && !INTER) {
+      o0[k] = u * V;
+      o1[k] = half + u * V;
+      n0[k] = n1[k] = min(V, half - u * V);
+    } else {
+      const int end = rot[k] ? A.part : A.dim;
+      o0[k] = rot[k] ? 2 * u * V : A.part + 2 * (u - A.n_rot) * V;
+      o1[k] = o0[k] + V;
+      n0[k] = u < A.n_units ? max(0, min(V, end - o0[k])) : 0;
+      n1[k] = u < A.n_units ? max(0, min(V, end - o1[k])) : 0;
+    }
+  }
+  float acc[2][2][NU][V];  // [tensor][vector][unit][element] sums of g u
+  if constexpr (MODE == NORM_GRAD) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[t][0][k][i] = acc[t][1][k][i] = 0.f;
+  }
+  const float inv_dim = 1.f / (float)A.dim;
+  const int total_groups = A.seg[0].groups + A.seg[1].groups;
+  const int64_t items = (int64_t)A.tokens * A.chunks;
+  for (int64_t item = (int64_t)blockIdx.x * WARPS + warp; item < items; item += (int64_t)gridDim.x * WARPS) {
+    const int token = (int)(item / A.chunks), chunk = (int)(item % A.chunks);
+    const int bt = token / A.seq, st = token % A.seq;
+    int64_t p = A.offset + st;
+    if (A.pos) {
+      const int64_t i = bt * A.pos_b + st * A.pos_s;
+      p = A.pos_i32 ? (int64_t) reinterpret_cast<const int*>(A.pos)[i] : reinterpret_cast<const long long*>(A.pos)[i];
+    }
+    float c[NU][V], s[NU][V];
+#pragma unroll
+    for (int k = 0; k < NU; ++k)
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[k][i] = 1.f;
+        s[k][i] = 0.f;
+        if (rot[k] && f0[k] + i < half) {
+          const uint64_t phase = (uint64_t)p * freq[f0[k] + i];
+          sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f /* 2^-31 */, &s[k][i], &c[k][i]);
+          c[k][i] *= A.factor;
+          s[k][i] *= A.factor * A.sign;
+        }
+      }
+    const int g_begin = chunk * A.per_chunk, g_end = min(total_groups, g_begin + A.per_chunk);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Seg& S = A.seg[t];
+      const int first = t == 0 ? 0 : A.seg[0].groups;
+      const int lo = max(0, g_begin - first), hi = min(S.groups, g_end - first);
+      if (lo >= hi) continue;
+      float gam[2][NU][V];
+      if constexpr (MODE != ROTATE) {
+#pragma unroll
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            gam[0][k][i] = gam[1][k][i] = 1.f;
+            if (S.gamma) {
+              const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
+              if (i < n0[k]) gam[0][k][i] = load_as_f32(S.gamma, o0[k] + i, dt);
+              if (i < n1[k]) gam[1][k][i] = load_as_f32(S.gamma, o1[k] + i, dt);
+            }
+          }
+      }
+      const T* xb = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s;
+      const T* db = MODE == NORM_GRAD ? reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s : nullptr;
+      T* yb = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s;
+      auto fetch = [&](Row<T, V, NU>& r, const T* base, int64_t stride, int h) {
+        const T* q = base + h * stride;
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+          r.a[k] = load_vec<T, V, FAST>(q + o0[k], h < S.heads ? n0[k] : 0);
+          r.b[k] = load_vec<T, V, FAST>(q + o1[k], h < S.heads ? n1[k] : 0);
+        }
+      };
+      Row<T, V, NU> x_next, d_next;
+      fetch(x_next, xb, S.x_h, lo * R + sub);
+      if constexpr (MODE == NORM_GRAD) fetch(d_next, db, S.d_h, lo * R + sub);
+      for (int g = lo; g < hi; ++g) {
+        const Row<T, V, NU> xr = x_next, dr = d_next;
+        const int h = g * R + sub;
+        if (g + 1 < hi) {
+          fetch(x_next, xb, S.x_h, h + R);
+          if constexpr (MODE == NORM_GRAD) fetch(d_next, db, S.d_h, h + R);
+        }
+        float a[NU][V], b[NU][V];
+#pragma unroll
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            a[k][i] = to_f(xr.a[k].v[i]);
+            b[k][i] = to_f(xr.b[k].v[i]);
+          }
+        if constexpr (MODE == NORM) {
+          float ss = 0.f;
+#pragma unroll
+          for (int k = 0; k < NU; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
+          for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          const float rstd = rsqrtf(ss * inv_dim + A.eps);
+#pragma unroll
+          for (int k = 0; k < NU; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              a[k][i] *= rstd * gam[0][k][i];
+              b[k][i] *= rstd * gam[1][k][i];
+            }
+        }
+        if constexpr (MODE != NORM_GRAD) {
+#pragma unroll
+          for (int k = 0; k < NU; ++k)
+            if (rot[k]) turn<V, INTER>(a[k], b[k], c[k], s[k]);
+        } else {
+          float ga[NU][V], gb[NU][V];
+          float ss = 0.f, hx = 0.f;
+#pragma unroll
+          for (int k = 0; k < NU; ++k) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              ga[k][i] = to_f(dr.a[k].v[i]);
+              gb[k][i] = to_f(dr.b[k].v[i]);
+            }
+            if (rot[k]) turn<V, INTER>(ga[k], gb[k], c[k], s[k]);
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
+              hx = fmaf(ga[k][i] * gam[0][k][i], a[k][i], fmaf(gb[k][i] * gam[1][k][i], b[k][i], hx));
+            }
+          }
+          for (int o = L >> 1; o > 0; o >>= 1) {
+            ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            hx += __shfl_xor_sync(0xffffffffu, hx, o);
+          }
+          const float rstd = rsqrtf(ss * inv_dim + A.eps);
+          const float m = hx * inv_dim * rstd * rstd;  // mean(h u) / (u / x)
+#pragma unroll
+          for (int k = 0; k < NU; ++k)
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              acc[t][0][k][i] = fmaf(ga[k][i], a[k][i] * rstd, acc[t][0][k][i]);
+              acc[t][1][k][i] = fmaf(gb[k][i], b[k][i] * rstd, acc[t][1][k][i]);
+              a[k][i] = rstd * (ga[k][i] * gam[0][k][i] - a[k][i] * m);
+              b[k][i] = rstd * (gb[k][i] * gam[1][k][i] - b[k][i] * m);
+            }
+        }
+        if (h < S.heads) {
+          T* q = yb + h * S.y_h;
+#pragma unroll
+          for (int k = 0; k < NU; ++k) {
+            store_vec<T, V, FAST>(q + o0[k], a[k], n0[k]);
+            store_vec<T, V, FAST>(q + o1[k], b[k], n1[k]);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (MODE == NORM_GRAD) {
+    // the block's sums: over the warp's R heads by shuffles, over its warps in order
+    __shared__ float sums[WARPS][B200_ROTARY_MAX_DIM];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      __syncthreads();
+#pragma unroll
+      for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          float a = acc[t][0][k][i], b = acc[t][1][k][i];
+          for (int o = L; o < 32; o <<= 1) {
+            a += __shfl_xor_sync(0xffffffffu, a, o);
+            b += __shfl_xor_sync(0xffffffffu, b, o);
+          }
+          if (sub == 0) {
+            if (i < n0[k]) sums[warp][o0[k] + i] = a;
+            if (i < n1[k]) sums[warp][o1[k] + i] = b;
+          }
+        }
+      __syncthreads();
+      for (int d = threadIdx.x; d < A.dim; d += THREADS) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) v += sums[w][d];
+        A.partial[((int64_t)blockIdx.x * 2 + t) * A.dim + d] = v;
+      }
+    }
+  }
+}
+
+// dgamma of both tensors from the blocks' partials, added in block order by 8 threads per
+// column and a fixed tree
+__global__ void __launch_bounds__(256) gamma_sum_kernel(const float* __restrict__ partial, float* dgq, float* dgk, int dim, int blocks) {
+  __shared__ float red[8][33];
+  const int col = blockIdx.x * 32 + (threadIdx.x & 31), part = threadIdx.x >> 5;
+  float v = 0.f;
+  if (col < 2 * dim)
+    for (int b = part; b < blocks; b += 8) v += partial[(int64_t)b * 2 * dim + col];
+  red[part][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (part == 0 && col < 2 * dim) {
+#pragma unroll
+    for (int i = 1; i < 8; ++i) v += red[i][threadIdx.x];
+    float* out = col < dim ? dgq : dgk;
+    if (out) out[col < dim ? col : col - dim] = v;
+  }
+}
+
+template <typename T, int V, int NU, bool FAST, int MODE>
+static int launch(const Args& a, bool inter, int grid, cudaStream_t s) {
+  if (inter) heads_kernel<T, V, NU, FAST, true, MODE><<<grid, THREADS, 0, s>>>(a);
+  else heads_kernel<T, V, NU, FAST, false, MODE><<<grid, THREADS, 0, s>>>(a);
+  return check_launch(MODE == ROTATE ? "rotary" : (MODE == NORM ? "qk_norm_rotary" : "qk_norm_rotary_grad"));
+}
+
+static int grad_blocks() { return 2 * num_sms(); }
+
+template <int MODE>
+static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* blocks_out = nullptr) {
+  const int size = dtype == B200_F32 ? 4 : 2;
+  const int wide = 16 / size;
+  const int half = r->rotary_dim / 2, rest = r->head_dim - r->rotary_dim;
+  // 16-byte units when they tile the head's parts and every row starts on 16 bytes;
+  // otherwise units of 2 elements, loaded one by one
+  bool fast = rest % wide == 0 && (r->interleaved ? r->rotary_dim : half) % wide == 0;
+  for (const Seg& g : a.seg) {
+    if (!g.heads) continue;
+    uint64_t bits = reinterpret_cast<uintptr_t>(g.x) | reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.dy);
+    bits |= (uint64_t)(g.x_b | g.x_s | g.x_h | g.y_b | g.y_s | g.y_h | g.d_b | g.d_s | g.d_h) * (uint64_t)size;
+    if (bits & 15) fast = false;
+  }
+  const int V = fast ? wide : 2;
+  a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
+  a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
+  a.L = 1;
+  while (a.L < a.n_units && a.L < 32) a.L *= 2;
+  const int nu = (int)ceil_div(a.n_units, a.L);
+  const int R = 32 / a.L;
+  for (Seg& g : a.seg) g.groups = (int)ceil_div(g.heads, R);
+  const int groups = a.seg[0].groups + a.seg[1].groups;
+  // one warp per token while the tokens fill the SMs (32 warps each); below that a token's
+  // head groups are spread over as many warps as it takes
+  const int64_t want = ceil_div((int64_t)num_sms() * 32, a.tokens);
+  a.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(groups, want));
+  a.per_chunk = (int)ceil_div(groups, a.chunks);
+  a.chunks = (int)ceil_div(groups, a.per_chunk);
+  const int64_t blocks = ceil_div((int64_t)a.tokens * a.chunks, WARPS);
+  const int grid = (int)std::min<int64_t>(blocks, MODE == NORM_GRAD ? grad_blocks() : 16 * num_sms());
+  if (blocks_out) *blocks_out = grid;
+  const bool in = r->interleaved != 0;
+  if (dtype == B200_F32) {
+    if (fast) return nu == 1 ? launch<float, 4, 1, true, MODE>(a, in, grid, s) : launch<float, 4, 2, true, MODE>(a, in, grid, s);
+    return nu == 1 ? launch<float, 2, 1, false, MODE>(a, in, grid, s) : launch<float, 2, 4, false, MODE>(a, in, grid, s);
+  }
+  if (fast) return launch<__nv_bfloat16, 8, 1, true, MODE>(a, in, grid, s);
+  return nu == 1 ? launch<__nv_bfloat16, 2, 1, false, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 2, 4, false, MODE>(a, in, grid, s);
+}
+
+static int check_rotary(const char* what, const b200_rotary* r, int dtype, int64_t batch, int64_t seq, const void* pos, int pos_dtype) {
+  B200_REQUIRE(r, "%s: null rotary description", what);
+  B200_REQUIRE(r->head_dim >= 1 && r->head_dim <= B200_ROTARY_MAX_DIM, "%s: head_dim %d not in [1, %d]", what, r->head_dim,
+               B200_ROTARY_MAX_DIM);
+  B200_REQUIRE(r->rotary_dim >= 0 && r->rotary_dim <= r->head_dim && r->rotary_dim % 2 == 0,
+               "%s: rotary_dim %d must be even and in [0, head_dim = %d]", what, r->rotary_dim, r->head_dim);
+  B200_REQUIRE(batch >= 0 && seq >= 0, "%s: negative size", what);
+  B200_REQUIRE(batch == 0 || seq <= INT32_MAX / batch, "%s: more than 2^31 - 1 tokens", what);
+  if (dtype != B200_F32 && dtype != B200_BF16) {
+    set_error("%s: dtype %d (fp32 and bf16 heads)", what, dtype);
+    return B200_ERR_DTYPE;
+  }
+  if (pos && pos_dtype != B200_I64 && pos_dtype != B200_I32) {
+    set_error("%s: positions of dtype %d (int32 and int64)", what, pos_dtype);
+    return B200_ERR_DTYPE;
+  }
+  return B200_OK;
+}
+
+static int check_norm(const char* what, int64_t heads_q, int64_t heads_k, bool gamma, int gamma_dtype, float eps) {
+  B200_REQUIRE(heads_q >= 0 && heads_k >= 0 && heads_q <= 65535 && heads_k <= 65535, "%s: %lld and %lld heads not in [0, 65535]", what,
+               (long long)heads_q, (long long)heads_k);
+  B200_REQUIRE(eps >= 0.f, "%s: eps %g is negative", what, (double)eps);
+  if (gamma && gamma_dtype != B200_F32 && gamma_dtype != B200_BF16) {
+    set_error("%s: weights of dtype %d (fp32 and bf16)", what, gamma_dtype);
+    return B200_ERR_DTYPE;
+  }
+  return B200_OK;
+}
+
+static void fill(Args& a, const b200_rotary* r, int64_t batch, int64_t seq, const void* pos, int pos_dtype, int64_t pos_b,
+                 int64_t pos_s, int64_t offset) {
+  a.pos = pos;
+  a.pos_i32 = pos_dtype == B200_I32;
+  a.pos_b = pos_b;
+  a.pos_s = pos_s;
+  a.offset = offset;
+  a.tokens = (int)(batch * seq);
+  a.seq = (int)seq;
+  a.dim = r->head_dim;
+  a.part = r->rotary_dim;
+  a.factor = r->factor;
+  a.sign = 1.f;
+  for (int i = 0; i < r->rotary_dim / 2; ++i) a.freq[i] = r->turns[i];
+}
+
+}  // namespace rot
+}  // namespace b200
+
+using namespace b200;
+
+extern "C" int b200_rotary_heads(const b200_rotary* r, int dtype, const void* x, void* y, int64_t batch, int64_t seq, int64_t heads,
+                                 int64_t x_b, int64_t x_s, int64_t x_h, int64_t y_b, int64_t y_s, int64_t y_h, const void* positions,
+                                 int pos_dtype, int64_t pos_b, int64_t pos_s, int64_t offset, int inverse, void* stream) {
+  const int rc = rot::check_rotary("rotary", r, dtype, batch, seq, positions, pos_dtype);
+  if (rc) return rc;
+  B200_REQUIRE(heads >= 0 && heads <= 65535, "rotary: %lld heads not in [0, 65535]", (long long)heads);
+  if (batch == 0 || seq == 0 || heads == 0) return B200_OK;
+  B200_REQUIRE(x && y, "rotary: null tensor");
+  rot::Args a = {};
+  rot::fill(a, r, batch, seq, positions, pos_dtype, pos_b, pos_s, offset);
+  if (inverse) a.sign = -1.f;
+  a.seg[0] = {x, nullptr, y, x_b, x_s, x_h, 0, 0, 0, y_b, y_s, y_h, nullptr, (int)heads, 0};
+  return rot::run<rot::ROTATE>(r, dtype, a, as_stream(stream));
+}
+
+extern "C" int b200_qk_norm_rotary(const b200_rotary* r, int dtype, const void* q, const void* k, void* yq, void* yk, int64_t batch,
+                                   int64_t seq, int64_t heads_q, int64_t heads_k, int64_t q_b, int64_t q_s, int64_t q_h, int64_t k_b,
+                                   int64_t k_s, int64_t k_h, int64_t yq_b, int64_t yq_s, int64_t yq_h, int64_t yk_b, int64_t yk_s,
+                                   int64_t yk_h, const void* gamma_q, const void* gamma_k, int gamma_dtype, float eps,
+                                   const void* positions, int pos_dtype, int64_t pos_b, int64_t pos_s, int64_t offset, void* stream) {
+  int rc = rot::check_rotary("qk_norm_rotary", r, dtype, batch, seq, positions, pos_dtype);
+  if (!rc) rc = rot::check_norm("qk_norm_rotary", heads_q, heads_k, gamma_q || gamma_k, gamma_dtype, eps);
+  if (rc) return rc;
+  if (batch == 0 || seq == 0 || heads_q + heads_k == 0) return B200_OK;
+  B200_REQUIRE((!heads_q || (q && yq)) && (!heads_k || (k && yk)), "qk_norm_rotary: null tensor");
+  rot::Args a = {};
+  rot::fill(a, r, batch, seq, positions, pos_dtype, pos_b, pos_s, offset);
+  a.eps = eps;
+  a.gamma_bf16 = gamma_dtype == B200_BF16;
+  a.seg[0] = {q, nullptr, yq, q_b, q_s, q_h, 0, 0, 0, yq_b, yq_s, yq_h, gamma_q, (int)heads_q, 0};
+  a.seg[1] = {k, nullptr, yk, k_b, k_s, k_h, 0, 0, 0, yk_b, yk_s, yk_h, gamma_k, (int)heads_k, 0};
+  return rot::run<rot::NORM>(r, dtype, a, as_stream(stream));
+}
+
+extern "C" size_t b200_qk_norm_rotary_grad_workspace_bytes(int64_t head_dim) {
+  return head_dim > 0 ? (size_t)rot::grad_blocks() * 2 * (size_t)head_dim * sizeof(float) : 0;
+}
+
+extern "C" int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, const void* dyk, const void* q, const void* k,
+                                        void* dq, void* dk, int64_t batch, int64_t seq, int64_t heads_q, int64_t heads_k,
+                                        const int64_t* strides, const void* gamma_q, const void* gamma_k, int gamma_dtype, float eps,
+                                        const void* positions, int pos_dtype, int64_t pos_b, int64_t pos_s, int64_t offset,
+                                        float* dgamma_q, float* dgamma_k, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = rot::check_rotary("qk_norm_rotary_grad", r, dtype, batch, seq, positions, pos_dtype);
+  if (!rc) rc = rot::check_norm("qk_norm_rotary_grad", heads_q, heads_k, gamma_q || gamma_k, gamma_dtype, eps);
+  if (rc) return rc;
+  B200_REQUIRE(strides, "qk_norm_rotary_grad: null strides");
+  cudaStream_t s = as_stream(stream);
+  if (batch == 0 || seq == 0 || heads_q + heads_k == 0) {
+    for (float* g : {dgamma_q, dgamma_k})
+      if (g && cudaMemsetAsync(g, 0, (size_t)r->head_dim * sizeof(float), s) != cudaSuccess) return check_launch("qk_norm_rotary_grad");
+    return B200_OK;
+  }
+  B200_REQUIRE((!heads_q || (q && dyq && dq)) && (!heads_k || (k && dyk && dk)), "qk_norm_rotary_grad: null tensor");
+  B200_REQUIRE(workspace && workspace_bytes >= b200_qk_norm_rotary_grad_workspace_bytes(r->head_dim),
+               "qk_norm_rotary_grad: workspace of %zu bytes, %zu needed", workspace_bytes,
+               b200_qk_norm_rotary_grad_workspace_bytes(r->head_dim));
+  rot::Args a = {};
+  rot::fill(a, r, batch, seq, positions, pos_dtype, pos_b, pos_s, offset);
+  a.sign = -1.f;
+  a.eps = eps;
+  a.gamma_bf16 = gamma_dtype == B200_BF16;
+  a.partial = reinterpret_cast<float*>(workspace);
+  const int64_t* t = strides;
+  a.seg[0] = {q, dyq, dq, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], gamma_q, (int)heads_q, 0};
+  t += 9;
+  a.seg[1] = {k, dyk, dk, t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7], t[8], gamma_k, (int)heads_k, 0};
+  int blocks = 0;
+  rc = rot::run<rot::NORM_GRAD>(r, dtype, a, s, &blocks);
+  if (rc || (!dgamma_q && !dgamma_k)) return rc;
+  rot::gamma_sum_kernel<<<(unsigned)ceil_div(2 * a.dim, 32), 256, 0, s>>>(a.partial, dgamma_q, dgamma_k, a.dim, blocks);
+  return check_launch("qk_norm_rotary_grad sums");
+}
