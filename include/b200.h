@@ -579,6 +579,52 @@ int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, c
                              int64_t pos_b, int64_t pos_s, int64_t offset, float* dgamma_q, float* dgamma_k, void* workspace,
                              size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * The output head and its softmax cross entropy without the logits in memory:
+ *   z = x w, lse[t] = log sum_v exp z[t, v], loss[t] = lse[t] - z[t, label[t]]
+ *   grad: d = dloss[t] (softmax(z) - onehot), dx = d w^T, dw = x^T d
+ * the Matmul (eager/core_math_ops/math_matrix.py:21-64) -> LogSoftmax
+ * (numpy/eager/math_advanced/math_log_exp.py:87-104) -> TakeAlongAxis
+ * (numpy/eager/advanced_indexing.py:163-177) chain of the transformer workload's head and
+ * its VJPs, with z made tile by tile on chip (again in the gradient, piece by piece of the
+ * vocabulary). x [N, D], w of one dtype: BF16 (tensor cores, fp32 sums; d rounded to bf16)
+ * or F32 (both as two bf16 planes, three products: 16 bits of each operand). x has row
+ * stride ldx; w is stored [D, V] with row stride ldw (w_dn != 0) or [V, D] (w_dn == 0).
+ * labels I64 / I32 [N]; rows of ignore_index get loss 0 and no gradient (and add nothing to
+ * dw, whatever x holds there); another label outside [0, V) sets the device error flag,
+ * with loss 0 and no gradient. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
+ * dense) in the operands' dtype; either may be NULL. The workspace's size depends on the
+ * pointers' alignment too: give the same ones. Results do not depend on the run. */
+size_t b200_linear_xent_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, int64_t N,
+                                        int64_t D, int64_t V);
+int b200_linear_xent(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, const void* labels, int label_dtype,
+                     int64_t ignore_index, float* loss, float* lse, int64_t N, int64_t D, int64_t V, void* workspace,
+                     size_t workspace_bytes, void* stream);
+size_t b200_linear_xent_grad_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, int64_t N,
+                                             int64_t D, int64_t V);
+int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn,
+                          const void* labels, int label_dtype, int64_t ignore_index, const float* lse, void* dx, void* dw, int64_t N,
+                          int64_t D, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * Orthogonalising matrices by Newton-Schulz products, and the optimizer step that uses it
+ * (no counterpart in the reference, whose optimizer steps are elementwise:
+ * numpy/eager/optimizers_ops.py:11-103). For each of `batch` dense matrices [rows, cols]:
+ *   X = G / (|G| + eps) (Frobenius norm); `steps` times, with (a, b, c) =
+ *   coefficients[3 i ..]: S = X X^T, X = a X + (b S + c S S) X
+ *   newton_schulz: out = X, of g's dtype (F32 or BF16)
+ *   apply_muon:    m' = mu m + g; G = g + mu m' (nesterov) or m'; p' = p (1 - lr weight_decay)
+ *                  - lr sqrt(max(1, rows / cols)) X. Outputs may alias param and momentum.
+ * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums; the
+ * coefficients have to keep X's entries below 250. Results do not depend on the run. */
+size_t b200_newton_schulz_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
+int b200_newton_schulz(int dtype, const void* g, void* out, int64_t batch, int64_t rows, int64_t cols, const float* coefficients,
+                       int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
+/* workspace >= b200_newton_schulz_workspace_bytes(B200_F32, ...) */
+int b200_apply_muon_f32(const float* param, const float* momentum, const float* grad, float* param_out, float* momentum_out,
+                        int64_t batch, int64_t rows, int64_t cols, float lr, float mu, int nesterov, float weight_decay,
+                        const float* coefficients, int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

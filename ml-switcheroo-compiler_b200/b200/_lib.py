@@ -155,6 +155,19 @@ SIGNATURES = {
                                                              _P, C.c_size_t, _P],
         C.c_int,
     ),
+    "b200_linear_xent_workspace_bytes": ([_I32, _P, _I64, _P, _I64, _I32, _I64, _I64, _I64], C.c_size_t),
+    "b200_linear_xent_grad_workspace_bytes": ([_I32, _P, _I64, _P, _I64, _I32, _I64, _I64, _I64], C.c_size_t),
+    "b200_linear_xent": ([_I32, _P, _I64, _P, _I64, _I32, _P, _I32, _I64, _P, _P, _I64, _I64, _I64, _P, C.c_size_t, _P], C.c_int),
+    "b200_linear_xent_grad": (
+        [_I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32, _I64, _P, _P, _P, _I64, _I64, _I64, _P, C.c_size_t, _P],
+        C.c_int,
+    ),
+    "b200_newton_schulz_workspace_bytes": ([_I32, _I64, _I64, _I64], C.c_size_t),
+    "b200_newton_schulz": ([_I32, _P, _P, _I64, _I64, _I64, C.POINTER(_F32), _I32, _F32, _P, C.c_size_t, _P], C.c_int),
+    "b200_apply_muon_f32": (
+        [_P] * 5 + [_I64] * 3 + [_F32, _F32, _I32, _F32, C.POINTER(_F32), _I32, _F32, _P, C.c_size_t, _P],
+        C.c_int,
+    ),
     "b200_conv2d_fwd": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_dgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_wgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),

@@ -9,6 +9,7 @@ all arithmetic runs in libb200.so, gradients are separate operators (as the refe
 
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import Any, Mapping
@@ -265,10 +266,173 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
     return dq, dk, dgamma[0], dgamma[1]
 
 
+# ----------------------------------------------------------------------------------
+# output head and cross entropy
+# ----------------------------------------------------------------------------------
+
+
+def _head(name: str, x: torch.Tensor, w: torch.Tensor, labels: Any):
+    """The operands as the entry points take them: (x [N, D], w, labels [N], row strides,
+    whether w is stored [D, V], sizes)."""
+    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[0]:
+        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} not aligned")
+    if not isinstance(labels, torch.Tensor) or not labels.is_cuda or labels.dtype not in (torch.int64, torch.int32):
+        labels = ops._int_indices(labels)
+    if labels.numel() != math.prod(x.shape[:-1]) or tuple(labels.shape) not in (tuple(x.shape[:-1]), (*x.shape[:-1], 1)):
+        raise ValueError(f"{name}: labels {tuple(labels.shape)} of x {tuple(x.shape)}")
+    if x.dtype not in _FLOATS or w.dtype not in _FLOATS:
+        raise BackendNotSupportedError(f"{name}: x of {x.dtype} and w of {w.dtype} (fp32 and bf16)")
+    D, V = w.shape
+    if D < 1 or V < 1:
+        raise ValueError(f"{name}: w {tuple(w.shape)} has no features or no words")
+    _on_device(name, x, w, labels)
+    if x.dtype != w.dtype or (x.dtype == torch.float32 and ops.Config.matmul_dtype == "bf16"):
+        # the contraction policy of Matmul: bf16 operands, or fp32 where either is
+        dt = torch.bfloat16 if ops.Config.matmul_dtype == "bf16" else torch.float32
+        x, w = ops.cast_operand(x, dt), ops.cast_operand(w, dt)
+    x2 = x.reshape(-1, D) if x.dim() == 1 or x.is_contiguous() else (x if x.dim() == 2 else ops.contiguous(x).reshape(-1, D))
+    if x2.stride(1) != 1 and D > 1 or x2.stride(0) < D:
+        x2 = ops.contiguous(x2)
+    N = x2.shape[0]
+    dn = w.stride(1) == 1 and w.stride(0) >= V
+    if not dn and not (w.stride(0) == 1 and w.stride(1) >= D):
+        w, dn = ops.contiguous(w), True
+    labels = ops.contiguous(labels).view(-1)
+    return x2, w, labels, max(x2.stride(0), D), w.stride(0) if dn else w.stride(1), int(dn), N, D, V
+
+
+def op_linear_cross_entropy(x, w, labels, ignore_index=-100, **_):
+    """The head's product and its softmax cross entropy, the logits never in memory:
+    (loss, lse) of z = x.w, lse = log sum exp z, loss = lse - z[label], fp32 in x's leading shape.
+
+    x [..., D] and w [D, V], fp32 or bf16 (a tied embedding [V, D] is passed as its
+    transposed view), labels integers in x's leading shape (or with a trailing 1). Rows
+    labelled ``ignore_index`` have loss 0; another label outside [0, V) sets the device
+    error flag. bf16 operands multiply on the tensor cores with fp32 sums; fp32 operands as
+    two bf16 planes each (16 bits), or rounded to bf16 where ``Config.matmul_dtype`` is
+    "bf16". Keep ``lse`` for LinearCrossEntropyGrad."""
+    name = "LinearCrossEntropy"
+    shape = tuple(x.shape[:-1])
+    x, w, labels, ldx, ldw, dn, N, D, V = _head(name, x, w, labels)
+    out = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    if N:
+        args = (ops.code(x), x.data_ptr(), ldx, w.data_ptr(), ldw, dn)
+        wn = int(L.lib().b200_linear_xent_workspace_bytes(*args, N, D, V))
+        ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=x.device)
+        L.call("b200_linear_xent", *args, labels.data_ptr(), ops.code(labels), int(ignore_index), out[0].data_ptr(), out[1].data_ptr(), N,
+               D, V, ws.data_ptr(), wn, ops.stream_ptr())
+    return out[0].view(shape), out[1].view(shape)
+
+
+def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **_):
+    """(dx, dw) of LinearCrossEntropy for the losses' gradient ``dloss`` (1 / N for a mean),
+    in x's and w's dtype; dw is stored as w is. ``lse`` as the forward returned it. Ignored
+    rows give no gradient, whatever x holds there. The logits are made again, one piece of
+    the vocabulary at a time (at most 512 MiB of their gradient at once)."""
+    name = "LinearCrossEntropyGrad"
+    x0, w0 = x, w
+    x, w, labels, ldx, ldw, dn, N, D, V = _head(name, x, w, labels)
+    lead = tuple(x0.shape[:-1])
+    for t, what in ((dloss, "dloss"), (lse, "lse")):
+        if t.numel() != N or tuple(t.shape) not in (lead, (*lead, 1)):
+            raise ValueError(f"{name}: {what} {tuple(t.shape)} of x {tuple(x0.shape)}")
+    _on_device(name, dloss, lse)
+    dloss, lse = (ops.contiguous(ops.cast(t, torch.float32)) for t in (dloss, lse))
+    dx = torch.empty(*lead, D, dtype=x.dtype, device=x.device)
+    dw = torch.empty((D, V) if dn else (V, D), dtype=w.dtype, device=w.device)
+    args = (x.data_ptr(), ldx, w.data_ptr(), ldw, dn)
+    wn = int(L.lib().b200_linear_xent_grad_workspace_bytes(ops.code(x), *args, N, D, V))
+    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=x.device)
+    L.call("b200_linear_xent_grad", ops.code(x), dloss.data_ptr(), *args, labels.data_ptr(), ops.code(labels), int(ignore_index),
+           lse.data_ptr(), dx.data_ptr(), dw.data_ptr(), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
+    return ops.cast(dx, x0.dtype), ops.cast(dw if dn else dw.t(), w0.dtype)
+
+
+# ----------------------------------------------------------------------------------
+# orthogonalised updates
+# ----------------------------------------------------------------------------------
+
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # steep at zero: 5 steps bring singular values from 0.01 into 0.7 .. 1.2
+
+
+@functools.lru_cache(maxsize=64)
+def _coefficients(steps: int, coefficients: tuple) -> Any:
+    """The steps' (a, b, c) as the entry points take them: one triple for all, or one each."""
+    rows = (coefficients,) * steps if not isinstance(coefficients[0], tuple) else coefficients
+    if not 1 <= steps <= 100 or len(rows) != steps or any(len(r) != 3 for r in rows):
+        raise ValueError(f"Newton-Schulz: {steps} steps (1 to 100) with coefficients {coefficients}: one (a, b, c), or one per step")
+    return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
+
+
+def _coef(steps: int, coefficients: Any) -> Any:
+    c = tuple(tuple(r) if isinstance(r, (list, tuple)) else r for r in coefficients)
+    return _coefficients(int(steps), c)
+
+
+def _matrices(name: str, t: torch.Tensor) -> tuple[int, int, int]:
+    if t.dim() < 2:
+        raise ValueError(f"{name}: a matrix or a stack of matrices is wanted, got {tuple(t.shape)}")
+    return math.prod(t.shape[:-2]), t.shape[-2], t.shape[-1]
+
+
+def op_newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, **_):
+    """The nearest (semi-)orthogonal matrix of each g [..., rows, cols], approximately:
+    X = g / (|g| + eps), then ``steps`` times X = a X + (b S + c S S) X with S = X X^T.
+
+    fp32 or bf16 in and out. ``coefficients``: one (a, b, c) or one per step. Sums are fp32;
+    the iterates carry 22 bits for fp32 matrices and 11 for bf16."""
+    name = "NewtonSchulz"
+    if g.dtype not in _FLOATS:
+        raise BackendNotSupportedError(f"{name}: matrices of {g.dtype} (fp32 and bf16)")
+    batch, rows, cols = _matrices(name, g)
+    coef = _coef(steps, coefficients)
+    _on_device(name, g)
+    gc = ops.contiguous(g)
+    out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    wn = int(L.lib().b200_newton_schulz_workspace_bytes(ops.code(g), batch, rows, cols))
+    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=g.device)
+    L.call("b200_newton_schulz", ops.code(g), gc.data_ptr(), out.data_ptr(), batch, rows, cols, coef, int(steps), float(eps),
+           ws.data_ptr(), wn, ops.stream_ptr())
+    return out
+
+
+def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
+                  coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, **_):
+    """One step of the orthogonalised momentum update for a matrix or a stack of matrices
+    [..., rows, cols], beside ApplyAdam and the others: returns (param', momentum').
+
+    momentum' = momentum * buffer + grad; G = grad + momentum * momentum' (nesterov) or
+    momentum'; param' = param (1 - lr weight_decay) - lr sqrt(max(1, rows / cols))
+    NewtonSchulz(G). fp32; lr 0.02 unless given. ``out``: the tensors to write (dense; the
+    inputs themselves for a step in place)."""
+    name = "ApplyMuon"
+    lr = 0.02 if lr is None else float(lr)
+    p, m, g = (ops.contiguous(ops.cast(t, torch.float32)) for t in (param, momentum_buffer, grad))
+    batch, rows, cols = _matrices(name, p)
+    if m.shape != p.shape or g.shape != p.shape:
+        raise ValueError(f"{name}: param, momentum and grad must have one shape, got {tuple(p.shape)}, {tuple(m.shape)}, {tuple(g.shape)}")
+    coef = _coef(steps, coefficients)
+    if out is None:
+        out = (torch.empty_like(p), torch.empty_like(m))
+    for t in out:
+        if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous():
+            raise ValueError(f"{name}: results must be dense fp32 {tuple(p.shape)}")
+    _on_device(name, p, m, g, *out)
+    wn = int(L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols))
+    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=p.device)
+    L.call("b200_apply_muon_f32", p.data_ptr(), m.data_ptr(), g.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), batch, rows, cols, lr,
+           float(momentum), int(bool(nesterov)), float(weight_decay), coef, int(steps), float(eps), ws.data_ptr(), wn, ops.stream_ptr())
+    return tuple(out)
+
+
 def register(table: dict) -> None:
     table.update({
         "RotaryEmbedding": op_rotary_embedding,
         "RotaryEmbeddingGrad": op_rotary_embedding_grad,
         "QKNormRotary": op_qk_norm_rotary,
         "QKNormRotaryGrad": op_qk_norm_rotary_grad,
+        "LinearCrossEntropy": op_linear_cross_entropy,
+        "LinearCrossEntropyGrad": op_linear_cross_entropy_grad,
+        "NewtonSchulz": op_newton_schulz,
+        "ApplyMuon": op_apply_muon,
     })

@@ -14,14 +14,16 @@
 // (an fp32 product would be off by 0.06 rad at position 10^6). Its top 32 bits go through
 // sincospif. The table travels in the kernel's parameters: nothing is uploaded or kept.
 //
-// Layout of the work. A lane owns one unit of a head: two 16-byte vectors that hold whole
-// pairs (the two halves of V pairs, or 2V neighbours), so a rotation needs no shuffle; the
-// units of a head take L lanes (a power of two), and a warp holds R = 32 / L heads. A warp
-// takes a token and walks its heads, R at a time, with the next heads' loads in flight:
-// the lane's angles are the same for every head, so cosines and sines are made once per
-// token. Few tokens (a decoding batch) are split over head groups, so that the heads of
-// one token run on many warps; each then makes the angles again.
-// Bound by HBM: x (and dy) are read once, y (dx) written once.
+// Layout of the work. A lane owns one unit of a head: two vectors of V = 4 elements that
+// hold whole pairs (the two halves of V pairs, or 2V neighbours), so a rotation needs no
+// shuffle; the units of a head take L lanes (a power of two), and a warp holds R = 32 / L
+// heads. A warp takes a token and walks its heads, R at a time: the lane's angles are the
+// same for every head, so cosines and sines are made once per token, while the first heads'
+// loads are under way. Few tokens (a decoding batch) are split over head groups, so that the
+// heads of one token run on many warps; each then makes the angles again.
+// Bound by HBM: x (and dy) are read once, y (dx) written once. BATCH groups of heads are
+// loaded before any is worked on: with 8 to 16 bytes a lane and vector the SM's warps have
+// to have 50 KB or more under way.
 #include <algorithm>
 
 #include "common.cuh"
@@ -55,56 +57,58 @@ struct Args {
   uint64_t freq[B200_ROTARY_MAX_DIM / 2];
 };
 
-template <typename T>
-__device__ __forceinline__ float to_f(T v);
-template <>
-__device__ __forceinline__ float to_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <typename T>
-__device__ __forceinline__ T from_f(float v);
-template <>
-__device__ __forceinline__ float from_f<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+// V elements as loaded: 32-bit words of one vector access (FAST; n is 0 or V), or one by one
+template <typename T, int V, bool FAST>
+struct Vec {
+  static constexpr int WORDS = FAST ? V * (int)sizeof(T) / 4 : V;
+  uint32_t w[WORDS];
 
-template <typename T, int V>
-struct alignas(sizeof(T) * V) Vec {
-  T v[V];
+  __device__ __forceinline__ void load(const T* p, int n) {
+    if constexpr (FAST) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+      if (n) {
+        if constexpr (WORDS == 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(p);
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        } else {
+          const uint2 u = *reinterpret_cast<const uint2*>(p);
+          w[0] = u.x, w[1] = u.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = i < n ? __float_as_uint((float)p[i]) : 0u;
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (FAST && sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    else return __uint_as_float(w[i]);
+  }
 };
 
-// V values at p: one vector access when FAST (n is 0 or V then), else element by element
-template <typename T, int V, bool FAST>
-__device__ __forceinline__ Vec<T, V> load_vec(const T* p, int n) {
-  Vec<T, V> r;
-  if constexpr (FAST) {
-    if (n) return *reinterpret_cast<const Vec<T, V>*>(p);
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(0.f);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = i < n ? p[i] : from_f<T>(0.f);
-  }
-  return r;
-}
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
 template <typename T, int V, bool FAST>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[V], int n) {
-  if constexpr (FAST) {
-    if (!n) return;
-    Vec<T, V> r;
-#pragma unroll
-    for (int i = 0; i < V; ++i) r.v[i] = from_f<T>(x[i]);
-    *reinterpret_cast<Vec<T, V>*>(p) = r;
-  } else {
+  if constexpr (!FAST) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) p[i] = from_f<T>(x[i]);
+      if (i < n) put(p + i, x[i]);
+  } else if (n) {
+    if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+    } else {
+      const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+    }
   }
 }
 
-template <typename T, int V, int NU>
+template <typename T, int V, int NU, bool FAST>
 struct Row {
-  Vec<T, V> a[NU], b[NU];
+  Vec<T, V, FAST> a[NU], b[NU];
 };
 
 // rotate the V pairs of a unit; s carries the direction's sign
@@ -132,6 +136,7 @@ __device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (
 
 template <typename T, int V, int NU, bool FAST, bool INTER, int MODE>
 __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kernel(const __grid_constant__ Args A) {
+  constexpr int BATCH = NU > 1 ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
   __shared__ uint64_t freq[B200_ROTARY_MAX_DIM / 2];
   const int half = A.part / 2;
   for (int i = threadIdx.x; i < half; i += THREADS) freq[i] = A.freq[i];
@@ -158,21 +163,55 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
       n1[k] = u < A.n_units ? max(0, min(V, end - o1[k])) : 0;
     }
   }
-  float acc[2][2][NU][V];  // [tensor][vector][unit][element] sums of g u
-  if constexpr (MODE == NORM_GRAD) {
+  float gam[2][2][NU][V];  // [tensor][vector][unit][element]
+  float acc[2][2][NU][V];  // sums of g u
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+  for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int k = 0; k < NU; ++k)
+    for (int k = 0; k < NU; ++k)
 #pragma unroll
-        for (int i = 0; i < V; ++i) acc[t][0][k][i] = acc[t][1][k][i] = 0.f;
-  }
+      for (int i = 0; i < V; ++i) {
+        acc[t][0][k][i] = acc[t][1][k][i] = 0.f;
+        gam[t][0][k][i] = gam[t][1][k][i] = 1.f;
+        if (MODE != ROTATE && A.seg[t].gamma) {
+          const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
+          if (i < n0[k]) gam[t][0][k][i] = load_as_f32(A.seg[t].gamma, o0[k] + i, dt);
+          if (i < n1[k]) gam[t][1][k][i] = load_as_f32(A.seg[t].gamma, o1[k] + i, dt);
+        }
+      }
   const float inv_dim = 1.f / (float)A.dim;
   const int total_groups = A.seg[0].groups + A.seg[1].groups;
   const int64_t items = (int64_t)A.tokens * A.chunks;
   for (int64_t item = (int64_t)blockIdx.x * WARPS + warp; item < items; item += (int64_t)gridDim.x * WARPS) {
     const int token = (int)(item / A.chunks), chunk = (int)(item % A.chunks);
     const int bt = token / A.seq, st = token % A.seq;
+    const int g_begin = chunk * A.per_chunk, g_end = min(total_groups, g_begin + A.per_chunk);
+    Row<T, V, NU, FAST> xr[BATCH], dr[BATCH];
+    // BATCH groups of heads of one tensor, from group g on
+    auto fetch = [&](const Seg& S, int g, int hi) {
+      const T* xb = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s;
+      const T* db = reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s;
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int h = (g + j) * R + sub;
+        const bool in = g + j < hi && h < S.heads;
+#pragma unroll
+        for (int k = 0; k < NU; ++k) {
+          xr[j].a[k].load(xb + h * S.x_h + o0[k], in ? n0[k] : 0);
+          xr[j].b[k].load(xb + h * S.x_h + o1[k], in ? n1[k] : 0);
+          if constexpr (MODE == NORM_GRAD) {
+            dr[j].a[k].load(db + h * S.d_h + o0[k], in ? n0[k] : 0);
+            dr[j].b[k].load(db + h * S.d_h + o1[k], in ? n1[k] : 0);
+          }
+        }
+      }
+    };
+    const int t_first = g_begin < A.seg[0].groups ? 0 : 1;
+    {
+      const Seg& S = A.seg[t_first];
+      const int first = t_first ? A.seg[0].groups : 0;
+      fetch(S, g_begin - first, min(S.groups, g_end - first));
+    }
     int64_t p = A.offset + st;
     if (A.pos) {
       const int64_t i = bt * A.pos_b + st * A.pos_s;
@@ -192,115 +231,86 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
           s[k][i] *= A.factor * A.sign;
         }
       }
-    const int g_begin = chunk * A.per_chunk, g_end = min(total_groups, g_begin + A.per_chunk);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const Seg& S = A.seg[t];
       const int first = t == 0 ? 0 : A.seg[0].groups;
       const int lo = max(0, g_begin - first), hi = min(S.groups, g_end - first);
-      if (lo >= hi) continue;
-      float gam[2][NU][V];
-      if constexpr (MODE != ROTATE) {
-#pragma unroll
-        for (int k = 0; k < NU; ++k)
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            gam[0][k][i] = gam[1][k][i] = 1.f;
-            if (S.gamma) {
-              const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
-              if (i < n0[k]) gam[0][k][i] = load_as_f32(S.gamma, o0[k] + i, dt);
-              if (i < n1[k]) gam[1][k][i] = load_as_f32(S.gamma, o1[k] + i, dt);
-            }
-          }
-      }
-      const T* xb = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s;
-      const T* db = MODE == NORM_GRAD ? reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s : nullptr;
       T* yb = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s;
-      auto fetch = [&](Row<T, V, NU>& r, const T* base, int64_t stride, int h) {
-        const T* q = base + h * stride;
+      for (int g = lo; g < hi; g += BATCH) {
+        if (t != t_first || g != lo) fetch(S, g, hi);
 #pragma unroll
-        for (int k = 0; k < NU; ++k) {
-          r.a[k] = load_vec<T, V, FAST>(q + o0[k], h < S.heads ? n0[k] : 0);
-          r.b[k] = load_vec<T, V, FAST>(q + o1[k], h < S.heads ? n1[k] : 0);
-        }
-      };
-      Row<T, V, NU> x_next, d_next;
-      fetch(x_next, xb, S.x_h, lo * R + sub);
-      if constexpr (MODE == NORM_GRAD) fetch(d_next, db, S.d_h, lo * R + sub);
-      for (int g = lo; g < hi; ++g) {
-        const Row<T, V, NU> xr = x_next, dr = d_next;
-        const int h = g * R + sub;
-        if (g + 1 < hi) {
-          fetch(x_next, xb, S.x_h, h + R);
-          if constexpr (MODE == NORM_GRAD) fetch(d_next, db, S.d_h, h + R);
-        }
-        float a[NU][V], b[NU][V];
+        for (int j = 0; j < BATCH; ++j) {
+          if (g + j >= hi) break;  // warp-uniform
+          const int h = (g + j) * R + sub;
+          float a[NU][V], b[NU][V];
 #pragma unroll
-        for (int k = 0; k < NU; ++k)
+          for (int k = 0; k < NU; ++k)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            a[k][i] = to_f(xr.a[k].v[i]);
-            b[k][i] = to_f(xr.b[k].v[i]);
+            for (int i = 0; i < V; ++i) {
+              a[k][i] = xr[j].a[k].get(i);
+              b[k][i] = xr[j].b[k].get(i);
+            }
+          if constexpr (MODE == NORM) {
+            float ss = 0.f;
+#pragma unroll
+            for (int k = 0; k < NU; ++k)
+#pragma unroll
+              for (int i = 0; i < V; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
+            for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const float rstd = rsqrtf(ss * inv_dim + A.eps);
+#pragma unroll
+            for (int k = 0; k < NU; ++k)
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                a[k][i] *= rstd * gam[t][0][k][i];
+                b[k][i] *= rstd * gam[t][1][k][i];
+              }
           }
-        if constexpr (MODE == NORM) {
-          float ss = 0.f;
+          if constexpr (MODE != NORM_GRAD) {
 #pragma unroll
-          for (int k = 0; k < NU; ++k)
+            for (int k = 0; k < NU; ++k)
+              if (rot[k]) turn<V, INTER>(a[k], b[k], c[k], s[k]);
+          } else {
+            float ga[NU][V], gb[NU][V];
+            float ss = 0.f, hx = 0.f;
 #pragma unroll
-            for (int i = 0; i < V; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
-          for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float rstd = rsqrtf(ss * inv_dim + A.eps);
+            for (int k = 0; k < NU; ++k) {
 #pragma unroll
-          for (int k = 0; k < NU; ++k)
+              for (int i = 0; i < V; ++i) {
+                ga[k][i] = dr[j].a[k].get(i);
+                gb[k][i] = dr[j].b[k].get(i);
+              }
+              if (rot[k]) turn<V, INTER>(ga[k], gb[k], c[k], s[k]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              a[k][i] *= rstd * gam[0][k][i];
-              b[k][i] *= rstd * gam[1][k][i];
+              for (int i = 0; i < V; ++i) {
+                ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
+                hx = fmaf(ga[k][i] * gam[t][0][k][i], a[k][i], fmaf(gb[k][i] * gam[t][1][k][i], b[k][i], hx));
+              }
             }
-        }
-        if constexpr (MODE != NORM_GRAD) {
-#pragma unroll
-          for (int k = 0; k < NU; ++k)
-            if (rot[k]) turn<V, INTER>(a[k], b[k], c[k], s[k]);
-        } else {
-          float ga[NU][V], gb[NU][V];
-          float ss = 0.f, hx = 0.f;
-#pragma unroll
-          for (int k = 0; k < NU; ++k) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              ga[k][i] = to_f(dr.a[k].v[i]);
-              gb[k][i] = to_f(dr.b[k].v[i]);
+            for (int o = L >> 1; o > 0; o >>= 1) {
+              ss += __shfl_xor_sync(0xffffffffu, ss, o);
+              hx += __shfl_xor_sync(0xffffffffu, hx, o);
             }
-            if (rot[k]) turn<V, INTER>(ga[k], gb[k], c[k], s[k]);
+            const float rstd = rsqrtf(ss * inv_dim + A.eps);
+            const float m = hx * inv_dim * rstd * rstd;  // mean(h u) / (u / x)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-              ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
-              hx = fmaf(ga[k][i] * gam[0][k][i], a[k][i], fmaf(gb[k][i] * gam[1][k][i], b[k][i], hx));
-            }
+            for (int k = 0; k < NU; ++k)
+#pragma unroll
+              for (int i = 0; i < V; ++i) {
+                acc[t][0][k][i] = fmaf(ga[k][i], a[k][i] * rstd, acc[t][0][k][i]);
+                acc[t][1][k][i] = fmaf(gb[k][i], b[k][i] * rstd, acc[t][1][k][i]);
+                a[k][i] = rstd * (ga[k][i] * gam[t][0][k][i] - a[k][i] * m);
+                b[k][i] = rstd * (gb[k][i] * gam[t][1][k][i] - b[k][i] * m);
+              }
           }
-          for (int o = L >> 1; o > 0; o >>= 1) {
-            ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            hx += __shfl_xor_sync(0xffffffffu, hx, o);
-          }
-          const float rstd = rsqrtf(ss * inv_dim + A.eps);
-          const float m = hx * inv_dim * rstd * rstd;  // mean(h u) / (u / x)
+          if (h < S.heads) {
+            T* q = yb + h * S.y_h;
 #pragma unroll
-          for (int k = 0; k < NU; ++k)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              acc[t][0][k][i] = fmaf(ga[k][i], a[k][i] * rstd, acc[t][0][k][i]);
-              acc[t][1][k][i] = fmaf(gb[k][i], b[k][i] * rstd, acc[t][1][k][i]);
-              a[k][i] = rstd * (ga[k][i] * gam[0][k][i] - a[k][i] * m);
-              b[k][i] = rstd * (gb[k][i] * gam[1][k][i] - b[k][i] * m);
+            for (int k = 0; k < NU; ++k) {
+              store_vec<T, V, FAST>(q + o0[k], a[k], n0[k]);
+              store_vec<T, V, FAST>(q + o1[k], b[k], n1[k]);
             }
-        }
-        if (h < S.heads) {
-          T* q = yb + h * S.y_h;
-#pragma unroll
-          for (int k = 0; k < NU; ++k) {
-            store_vec<T, V, FAST>(q + o0[k], a[k], n0[k]);
-            store_vec<T, V, FAST>(q + o1[k], b[k], n1[k]);
           }
         }
       }
@@ -367,16 +377,16 @@ static int grad_blocks() { return 2 * num_sms(); }
 template <int MODE>
 static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* blocks_out = nullptr) {
   const int size = dtype == B200_F32 ? 4 : 2;
-  const int wide = 16 / size;
+  const int wide = 4;
   const int half = r->rotary_dim / 2, rest = r->head_dim - r->rotary_dim;
-  // 16-byte units when they tile the head's parts and every row starts on 16 bytes;
-  // otherwise units of 2 elements, loaded one by one
+  // vectors of 4 elements when they tile the head's parts and every row starts on one's
+  // boundary; otherwise units of 2 elements, loaded one by one
   bool fast = rest % wide == 0 && (r->interleaved ? r->rotary_dim : half) % wide == 0;
   for (const Seg& g : a.seg) {
     if (!g.heads) continue;
     uint64_t bits = reinterpret_cast<uintptr_t>(g.x) | reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.dy);
     bits |= (uint64_t)(g.x_b | g.x_s | g.x_h | g.y_b | g.y_s | g.y_h | g.d_b | g.d_s | g.d_h) * (uint64_t)size;
-    if (bits & 15) fast = false;
+    if (bits & (uint64_t)(wide * size - 1)) fast = false;
   }
   const int V = fast ? wide : 2;
   a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
@@ -401,7 +411,7 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
     if (fast) return nu == 1 ? launch<float, 4, 1, true, MODE>(a, in, grid, s) : launch<float, 4, 2, true, MODE>(a, in, grid, s);
     return nu == 1 ? launch<float, 2, 1, false, MODE>(a, in, grid, s) : launch<float, 2, 4, false, MODE>(a, in, grid, s);
   }
-  if (fast) return launch<__nv_bfloat16, 8, 1, true, MODE>(a, in, grid, s);
+  if (fast) return nu == 1 ? launch<__nv_bfloat16, 4, 1, true, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 4, 2, true, MODE>(a, in, grid, s);
   return nu == 1 ? launch<__nv_bfloat16, 2, 1, false, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 2, 4, false, MODE>(a, in, grid, s);
 }
 

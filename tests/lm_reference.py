@@ -54,3 +54,29 @@ def rotate(x, positions, rotary_dim, base=10000.0, scaling=None, interleaved=Fal
 def rms_unit(x, eps):
     rstd = 1.0 / torch.sqrt((x * x).mean(-1, keepdim=True) + eps)
     return x * rstd, rstd
+
+
+def linear_xent(x, w, labels, ignore=-100, dloss=None):
+    """Losses, lse and (with dloss) dx, dw of the head x [N, D] . w [D, V] in float64, and the
+    logits' gradient itself."""
+    z = x @ w
+    lse = torch.logsumexp(z, -1)
+    kept = labels != ignore
+    at = (torch.arange(len(x), device=x.device), labels.clamp(min=0))
+    loss = torch.where(kept, lse - z[at], torch.zeros_like(lse))
+    if dloss is None:
+        return loss, lse
+    d = torch.softmax(z, -1)
+    d[at] -= 1
+    d = d * torch.where(kept, dloss, torch.zeros_like(dloss))[:, None]
+    return loss, lse, d @ w.t(), x.t() @ d, d
+
+
+def newton_schulz(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    x = g / (torch.linalg.vector_norm(g, dim=(-2, -1), keepdim=True) + eps)
+    for i in range(steps):
+        a, b, c = coefficients[i] if isinstance(coefficients[0], (list, tuple)) else coefficients
+        s = x @ x.mT if x.shape[-2] <= x.shape[-1] else x.mT @ x
+        p = b * s + c * (s @ s)
+        x = a * x + (p @ x if x.shape[-2] <= x.shape[-1] else x @ p)
+    return x
