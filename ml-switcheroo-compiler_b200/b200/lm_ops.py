@@ -27,7 +27,7 @@ def _on_device(name: str, *tensors: torch.Tensor | None) -> None:
     """The kernels run on the current device's stream: operands elsewhere are refused."""
     dev = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != dev):
+        if t is not None and t.get_device() != dev:
             raise ValueError(f"{name}: operand on {t.device}, the current device is cuda:{dev}")
 
 
@@ -122,28 +122,29 @@ def _rotary(head_dim: int, rotary_dim, base, interleaved, scaling) -> L.Rotary:
     return _rotary_table(head_dim, head_dim if rotary_dim is None else int(rotary_dim), float(base), bool(interleaved), key)
 
 
-def _heads(name: str, x: torch.Tensor) -> tuple[torch.Tensor, int, int, int, tuple[int, int, int]]:
-    """x [batch, seq, heads, dim] or [seq, heads, dim] -> x with adjacent head elements, its
-    batch, seq, heads and their element strides."""
+def _heads(name: str, x: torch.Tensor) -> tuple[torch.Tensor, tuple, tuple[int, int, int]]:
+    """x [batch, seq, heads, dim] or [seq, heads, dim] -> (x with adjacent head elements,
+    (batch, seq, heads, dim), element strides of the first three)."""
     if x.dtype not in _FLOATS:
         raise BackendNotSupportedError(f"{name}: {x.dtype} heads have no b200 kernel (fp32 and bf16)")
-    if x.dim() not in (3, 4):
-        raise ValueError(f"{name}: heads must be [batch, seq, heads, dim] or [seq, heads, dim], got {tuple(x.shape)}")
-    if x.stride(-1) != 1 and x.shape[-1] > 1:
+    shape, st = tuple(x.shape), x.stride()
+    if len(shape) not in (3, 4):
+        raise ValueError(f"{name}: heads must be [batch, seq, heads, dim] or [seq, heads, dim], got {shape}")
+    if st[-1] != 1 and shape[-1] > 1:
         x = ops.contiguous(x)
-    if x.dim() == 3:
-        return x, 1, x.shape[0], x.shape[1], (0, x.stride(0), x.stride(1))
-    return x, x.shape[0], x.shape[1], x.shape[2], (x.stride(0), x.stride(1), x.stride(2))
+        st = x.stride()
+    return (x, shape, st[:3]) if len(shape) == 4 else (x, (1, *shape), (0, *st[:2]))
 
 
-def _like(x: torch.Tensor) -> torch.Tensor:
-    """A fresh result for x: dense, its axes in x's storage order, adjacent head elements."""
+def _like(x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """A fresh result for x: dense, its axes in x's storage order, adjacent head elements;
+    and its strides."""
     y = torch.empty_like(x)
-    return y if y.stride(-1) == 1 or y.shape[-1] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-
-
-def _strides(x: torch.Tensor) -> tuple[int, int, int]:
-    return (0, x.stride(0), x.stride(1)) if x.dim() == 3 else (x.stride(0), x.stride(1), x.stride(2))
+    st = y.stride()
+    if st[-1] != 1 and y.shape[-1] > 1:
+        y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        st = y.stride()
+    return y, (st[:3] if len(st) == 4 else (0, *st[:2]))
 
 
 def _positions(name: str, positions: Any, offset: int, batch: int, seq: int) -> tuple[torch.Tensor | None, tuple]:
@@ -151,25 +152,25 @@ def _positions(name: str, positions: Any, offset: int, batch: int, seq: int) -> 
     the entry points' position arguments)."""
     if positions is None:
         return None, (None, L.I64, 0, 0, int(offset))
-    t = positions if isinstance(positions, torch.Tensor) and positions.is_cuda else ops.to_device(positions)
-    if t.dtype not in (torch.int64, torch.int32):
-        t = ops._int_indices(t)
     if offset:
         raise ValueError(f"{name}: give positions or an offset, not both")
-    if t.dim() == 0 or t.dim() > 2 or t.shape[-1] != seq or (t.dim() == 2 and t.shape[0] not in (1, batch)):
-        raise ValueError(f"{name}: positions {tuple(t.shape)} do not match {batch} sequences of {seq} tokens")
-    pb = t.stride(0) if t.dim() == 2 and t.shape[0] == batch and batch > 1 else 0
-    return t, (t.data_ptr(), ops.code(t), pb, t.stride(-1), 0)
+    t = positions if isinstance(positions, torch.Tensor) else torch.as_tensor(positions)
+    shape = tuple(t.shape)
+    if shape not in ((seq,), (1, seq), (batch, seq)):
+        raise ValueError(f"{name}: positions {shape} do not match {batch} sequences of {seq} tokens")
+    if not t.is_cuda or (t.dtype != torch.int64 and t.dtype != torch.int32):
+        t = ops._int_indices(ops.to_device(t))
+    st = t.stride()
+    return t, (t.data_ptr(), L.I64 if t.dtype == torch.int64 else L.I32, st[0] if len(shape) == 2 and shape[0] > 1 else 0, st[-1], 0)
 
 
 def _rotate(name: str, x: torch.Tensor, positions, base, rotary_dim, interleaved, scaling, offset, inverse: int) -> torch.Tensor:
-    x, batch, seq, heads, xs = _heads(name, x)
-    r = _rotary(x.shape[-1], rotary_dim, base, interleaved, scaling)
+    x, (batch, seq, heads, dim), xs = _heads(name, x)
+    r = _rotary(dim, rotary_dim, base, interleaved, scaling)
     pos, pa = _positions(name, positions, offset, batch, seq)
     _on_device(name, x, pos)
-    y = _like(x)
-    L.call("b200_rotary_heads", r, ops.code(x), x.data_ptr(), y.data_ptr(), batch, seq, heads, *xs, *_strides(y), *pa, inverse,
-           ops.stream_ptr())
+    y, ys = _like(x)
+    L.call("b200_rotary_heads", r, ops.code(x), x.data_ptr(), y.data_ptr(), batch, seq, heads, *xs, *ys, *pa, inverse, ops.stream_ptr())
     return y
 
 
@@ -190,13 +191,13 @@ def op_rotary_embedding_grad(dy, positions=None, base=10000.0, rotary_dim=None, 
 
 
 def _pair(name: str, q: torch.Tensor, k: torch.Tensor):
-    q, batch, seq, hq, qs = _heads(name, q)
-    k, kbatch, kseq, hk, ks = _heads(name, k)
-    if q.dim() != k.dim() or (kbatch, kseq, k.shape[-1]) != (batch, seq, q.shape[-1]):
+    q, (batch, seq, hq, dim), qs = _heads(name, q)
+    k, (kbatch, kseq, hk, kdim), ks = _heads(name, k)
+    if q.dim() != k.dim() or (kbatch, kseq, kdim) != (batch, seq, dim):
         raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)} differ in more than their heads")
     if q.dtype != k.dtype:
         raise BackendNotSupportedError(f"{name}: queries of {q.dtype} with keys of {k.dtype}")
-    return q, k, batch, seq, hq, hk, qs, ks
+    return q, k, batch, seq, hq, hk, dim, qs, ks
 
 
 def _gammas(name: str, dim: int, gq: torch.Tensor | None, gk: torch.Tensor | None):
@@ -226,14 +227,14 @@ def op_qk_norm_rotary(q, k, gamma_q=None, gamma_k=None, positions=None, eps=1e-6
     gamma_k [dim], None: ones. The rest as RotaryEmbedding; ``rotary_dim=0`` norms alone.
     The norm's sum and the rotation are in fp32, rounded once."""
     name = "QKNormRotary"
-    q, k, batch, seq, hq, hk, qs, ks = _pair(name, q, k)
-    r = _rotary(q.shape[-1], rotary_dim, base, interleaved, scaling)
-    gq, gk, gdt = _gammas(name, q.shape[-1], gamma_q, gamma_k)
+    q, k, batch, seq, hq, hk, dim, qs, ks = _pair(name, q, k)
+    r = _rotary(dim, rotary_dim, base, interleaved, scaling)
+    gq, gk, gdt = _gammas(name, dim, gamma_q, gamma_k)
     pos, pa = _positions(name, positions, offset, batch, seq)
     _on_device(name, q, k, gq, gk, pos)
-    yq, yk = _like(q), _like(k)
+    (yq, yqs), (yk, yks) = _like(q), _like(k)
     L.call("b200_qk_norm_rotary", r, ops.code(q), q.data_ptr(), k.data_ptr(), yq.data_ptr(), yk.data_ptr(), batch, seq, hq, hk, *qs,
-           *ks, *_strides(yq), *_strides(yk), ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, ops.stream_ptr())
+           *ks, *yqs, *yks, ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, ops.stream_ptr())
     return yq, yk
 
 
@@ -243,23 +244,22 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
     (dq, dk, dgamma_q, dgamma_k), the weights' in fp32 [dim] (also where a gamma is None),
     summed over tokens and heads in a fixed order."""
     name = "QKNormRotaryGrad"
-    q, k, batch, seq, hq, hk, qs, ks = _pair(name, q, k)
+    q, k, batch, seq, hq, hk, dim, qs, ks = _pair(name, q, k)
     if tuple(dyq.shape) != tuple(q.shape) or tuple(dyk.shape) != tuple(k.shape):
         raise ValueError(f"{name}: gradients {tuple(dyq.shape)}, {tuple(dyk.shape)} of queries {tuple(q.shape)}, keys {tuple(k.shape)}")
     if dyq.dtype != q.dtype or dyk.dtype != q.dtype:
         raise BackendNotSupportedError(f"{name}: gradients of {dyq.dtype}, {dyk.dtype} for {q.dtype} heads")
-    dyq, _, _, _, dqs = _heads(name, dyq)
-    dyk, _, _, _, dks = _heads(name, dyk)
-    dim = q.shape[-1]
+    dyq, _, dqs = _heads(name, dyq)
+    dyk, _, dks = _heads(name, dyk)
     r = _rotary(dim, rotary_dim, base, interleaved, scaling)
     gq, gk, gdt = _gammas(name, dim, gamma_q, gamma_k)
     pos, pa = _positions(name, positions, offset, batch, seq)
     _on_device(name, q, k, dyq, dyk, gq, gk, pos)
-    dq, dk = _like(q), _like(k)
+    (dq, rqs), (dk, rks) = _like(q), _like(k)
     dgamma = torch.empty(2, dim, dtype=torch.float32, device=q.device)
     wn = int(L.lib().b200_qk_norm_rotary_grad_workspace_bytes(dim))
     ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
-    st = L.I64x18(*qs, *dqs, *_strides(dq), *ks, *dks, *_strides(dk))
+    st = L.I64x18(*qs, *dqs, *rqs, *ks, *dks, *rks)
     L.call("b200_qk_norm_rotary_grad", r, ops.code(q), dyq.data_ptr(), dyk.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(),
            dk.data_ptr(), batch, seq, hq, hk, st, ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, dgamma[0].data_ptr(),
            dgamma[1].data_ptr(), ws.data_ptr(), wn, ops.stream_ptr())

@@ -45,7 +45,8 @@ def device() -> torch.device:
 
 
 def stream_ptr() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    # the raw handle: building a Stream object costs several microseconds per launch
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def code(t: torch.Tensor) -> int:

@@ -4,10 +4,10 @@
 //   z = x w  [N, V],  lse_t = log sum_v exp z_tv,  loss_t = lse_t - z_t,label(t)
 //   d_tv = dloss_t (exp(z_tv - lse_t) - [v = label(t)]),  dx = d w^T,  dw = x^T d
 //
-// Forward: one tcgen05 product whose epilogue keeps, per row and 128-column half tile, the
+// Forward: one tcgen05 product whose epilogue keeps, per row and half tile, the
 // running maximum and the sum of exponentials of the accumulator (fp32, base 2), and the
 // label's logit; a second kernel joins a row's halves. z is never written: 8 bytes leave the
-// SM for 128 logits.
+// SM for a half tile's 128 logits (64 with fp32 operands).
 // Backward: the vocabulary is walked in pieces. A piece's logits are made again (a fourth
 // product: the price of not keeping 4 bytes per token and word), its epilogue turns them
 // into d, written in the operands' precision to a workspace that one piece fills; the
@@ -42,12 +42,14 @@ __device__ __forceinline__ int64_t label_at(const void* labels, int i32, int64_t
 // ---- forward epilogue: maxima, sums and the label's logit ----
 struct LseEpi {
   struct Args {
-    float2* part;  // [2 tiles_n][N]: (maximum, sum of exp2((z - maximum) log2 e)) of a half tile's columns
+    float2* part;  // [parts][N]: (maximum, sum of exp2((z - maximum) log2 e)) of a half tile's columns
+    int width;     // columns of a half tile
     float* picked;
     const void* labels;
     int labels_i32;
     int64_t N, V;
   };
+  static constexpr bool SINGLE_WIDE = true, SINGLE_NARROW = false, TEAMS = false, INIT = false;
   const Args& a;
   float m, s, at_label;
   int64_t label;
@@ -85,11 +87,12 @@ struct LseEpi {
     for (int i = 0; i < 32; ++i) sum[i & 3] += ex2(fmaf(v[i], LOG2E, -shift));
     s += (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
+  __device__ __forceinline__ void finish(int) {}
   __device__ __forceinline__ void end(const Spot& sp) {
     if (sp.row >= a.N) return;
     a.part[(int64_t)(sp.nt * 2 + sp.half) * a.N + sp.row] = make_float2(m, s);
-    const int64_t k = label - ((int64_t)sp.nt * 256 + sp.half * 128);
-    if (k >= 0 && k < 128 && label < a.V) a.picked[sp.row] = at_label;
+    const int64_t k = label - sp.col0;
+    if (k >= 0 && k < a.width && label < a.V) a.picked[sp.row] = at_label;
   }
 };
 
@@ -131,50 +134,57 @@ __global__ void __launch_bounds__(256) lse_join_kernel(const float2* __restrict_
 // ---- backward: the gradient of the logits of one piece of the vocabulary ----
 struct GradEpi {
   struct Args {
-    __nv_bfloat16* d;  // [planes][N][ld]
-    int64_t ld, plane;
+    CUtensorMap map;  // d [planes][N][ld], stored 32 x 32 at a time
     int planes;
     const float *dloss, *lse;
     const void* labels;
     int labels_i32;
-    int64_t ignore, N, V, first, width;  // the piece's columns [first, first + width)
+    int64_t ignore, N, V, first;  // first: the piece's first column of w
   };
+  static constexpr bool SINGLE_WIDE = true, SINGLE_NARROW = false, TEAMS = false, INIT = false;
   const Args& a;
   float g, shift;
   int64_t label;  // relative to the piece
-  bool kept;
-  __device__ explicit GradEpi(const Args& args) : a(args) {}
+  uint32_t kept;  // all ones, or zero for an ignored row
+  uint32_t turn;
+  __device__ explicit GradEpi(const Args& args) : a(args), turn(0) {}
 
   __device__ __forceinline__ void begin(const Spot& sp) {
     g = shift = 0.f;
     label = -1;
-    kept = false;
+    kept = 0u;
     if (sp.row >= a.N) return;
     const int64_t l = label_at(a.labels, a.labels_i32, sp.row);
     if (l == a.ignore || l < 0 || l >= a.V) return;
     label = l - a.first;
-    kept = true;
+    kept = ~0u;
     g = a.dloss[sp.row];
     shift = a.lse[sp.row] * LOG2E;
   }
   __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
-    const int64_t k = label - col;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) {
-      float p = ex2(fmaf(v[i], LOG2E, -shift));
-      if (k == i) p -= 1.f;
-      v[i] = kept ? g * p : 0.f;
+    for (int i = 0; i < 32; ++i) v[i] = g * ex2(fmaf(v[i], LOG2E, -shift));
+    const int64_t k = label - col;
+    if (k >= 0 && k < 32) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (k == i) v[i] -= g;
     }
-    const int rows = (int)min((int64_t)32, a.N - sp.row0);
-    const int64_t cols = min((int64_t)32, a.width - col);
     for (int plane = 0; plane < a.planes; ++plane) {
       uint32_t w[16];
 #pragma unroll
-      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
+      for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]) & kept;
+      // two 2 KB buffers: the bulk store before the last one has been read
+      const uint32_t buf = sp.buf + (turn++ & 1) * 2048;
+      if (sp.lane == 0) bulk_wait_read1();
       __syncwarp();
-      stage_chunk<2>(sp.buf, sp.lane, w);
+      stage_chunk<2>(buf, sp.lane, w);
+      fence_proxy_async_smem();
       __syncwarp();
-      write_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(a.d + plane * a.plane + sp.row0 * a.ld + col), a.ld, rows, cols);
+      if (sp.lane == 0) {
+        tma_store_4d(&a.map, buf, (int)col, (int)sp.row0, plane, 0);
+        bulk_commit();
+      }
       if (plane + 1 < a.planes) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
@@ -186,6 +196,9 @@ struct GradEpi {
     }
   }
   __device__ __forceinline__ void end(const Spot&) {}
+  __device__ __forceinline__ void finish(int lane) {
+    if (lane == 0) bulk_wait0();
+  }
 };
 
 // ---- plain result: C = acc (+ an fp32 addend), fp32 or bf16; K splits write partials ----
@@ -196,25 +209,30 @@ struct StoreEpi {
     int64_t ld, ld_add, split_stride, M, N;
     int bf16;
   };
+  static constexpr bool SINGLE_WIDE = true, SINGLE_NARROW = true, TEAMS = false, INIT = true;
+  static constexpr float scale = 1.f;
   const Args& a;
   __device__ explicit StoreEpi(const Args& args) : a(args) {}
   __device__ __forceinline__ void begin(const Spot&) {}
   __device__ __forceinline__ void end(const Spot&) {}
-  __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
+  __device__ __forceinline__ void finish(int) {}
+  __device__ __forceinline__ void init(const Spot& sp, int64_t col, float (&v)[32]) {
     if (a.add && sp.row < a.M) {
       const float* p = a.add + sp.row * a.ld_add + col;
       if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
           const float4 t = *reinterpret_cast<const float4*>(p + i);
-          v[i] += t.x, v[i + 1] += t.y, v[i + 2] += t.z, v[i + 3] += t.w;
+          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
         }
       } else {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (col + i < a.N) v[i] += p[i];
+          if (col + i < a.N) v[i] = p[i];
       }
     }
+  }
+  __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
     const int rows = (int)min((int64_t)32, a.M - sp.row0);
     const int64_t cols = min((int64_t)32, a.N - col);
     const int64_t at = sp.split * a.split_stride + sp.row0 * a.ld + col;
@@ -372,7 +390,7 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
   if (needs_pack(dtype, x, ldx)) p.x = take(xb);
   if (needs_pack(dtype, w, ldw)) p.w = take((size_t)p.planes * p.w_rows * up8(p.w_cols) * 2);
   if (!grad) {
-    p.part = take((size_t)ceil_div(V, 256) * 2 * N * sizeof(float2));
+    p.part = take((size_t)ceil_div(V, p.planes > 1 ? 128 : 256) * 2 * N * sizeof(float2));
     p.picked = take((size_t)N * 4);
   } else {
     p.width = piece_width(N, D, V, p.planes);
@@ -399,9 +417,7 @@ static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int
   const int splits = lp.splits;
   if (splits > 1) a = {split_ws, nullptr, N, N, M * N, M, N, 0};
   int rc;
-  if (M > 128 && N > 128) rc = launch<256, true, StoreEpi>(A, B, M, N, K, 1, planes, lp, a, s, what);
-  else if (N > 128) rc = launch<256, false, StoreEpi>(A, B, M, N, K, 1, planes, lp, a, s, what);
-  else rc = launch<128, false, StoreEpi>(A, B, M, N, K, 1, planes, lp, a, s, what);
+  rc = launch<StoreEpi>(A, B, M, N, K, 1, planes, M > 128 && (N > 128 || planes > 1), lp, a, s, what);
   if (rc || splits == 1) return rc;
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(M * N, 256), (int64_t)num_sms() * 16);
   join_splits_kernel<<<grid, 256, 0, s>>>(split_ws, splits, M * N, N, add, C, bf16, ldc);
@@ -488,12 +504,12 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
   tile::Loop lp = {};
   lp.bf16 = 1;
   lp.group_m = 16;
-  const lx::LseEpi::Args a = {part, picked, labels, i32, N, V};
+  const int width = p.planes > 1 ? 64 : 128;
+  const lx::LseEpi::Args a = {part, width, picked, labels, i32, N, V};
   // a pair's 256 rows; one CTA's 128 when there are no more tokens than that
-  rc = N > 128 ? tile::launch<256, true, lx::LseEpi>(A, B, N, V, D, 1, p.planes, lp, a, s, what)
-               : tile::launch<256, false, lx::LseEpi>(A, B, N, V, D, 1, p.planes, lp, a, s, what);
+  rc = tile::launch<lx::LseEpi>(A, B, N, V, D, 1, p.planes, N > 128, lp, a, s, what);
   if (rc) return rc;
-  lx::lse_join_kernel<<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(part, (int)(ceil_div(V, 256) * 2), picked, labels, i32, ignore_index, loss,
+  lx::lse_join_kernel<<<(unsigned)ceil_div(N, 32), 256, 0, s>>>(part, (int)(ceil_div(V, 2 * width) * 2), picked, labels, i32, ignore_index, loss,
                                                                 lse, N, V);
   return check_launch(what);
 }
@@ -542,9 +558,12 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
     tile::Loop lp = {};
     lp.bf16 = 1;
     lp.group_m = 16;
-    const lx::GradEpi::Args a = {d, p.width, N * p.width, p.planes, dloss, lse, labels, i32, ignore_index, N, V, first, width};
-    rc = N > 128 ? tile::launch<256, true, lx::GradEpi>(X, W, N, width, D, 1, p.planes, lp, a, s, what)
-                 : tile::launch<256, false, lx::GradEpi>(X, W, N, width, D, 1, p.planes, lp, a, s, what);
+    lx::GradEpi::Args a = {{}, p.planes, dloss, lse, labels, i32, ignore_index, N, V, first};
+    if (!tc::make_store_map(&a.map, d, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, width, N, p.planes, 1, p.width, N * p.width, 0)) {
+      set_error("%s: no tensor map for the logits' gradient (%lld x %lld)", what, (long long)N, (long long)width);
+      return B200_ERR_CUDA;
+    }
+    rc = tile::launch<lx::GradEpi>(X, W, N, width, D, 1, p.planes, N > 128, lp, a, s, what);
     if (rc) return rc;
     tile::Operand Dk, Dm;  // d as [N, width] with the tokens, or the columns, as its major axis
     Dk.base = Dm.base = d, Dk.ld = Dm.ld = p.width, Dk.plane_stride = Dm.plane_stride = N * p.width;

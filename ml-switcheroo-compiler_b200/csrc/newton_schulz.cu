@@ -1,8 +1,8 @@
 // Orthogonalising a matrix by Newton-Schulz products, and the optimizer step that uses it.
 //
-//   X0 = G / (|G|_F + eps);  each step: S = X X^T, P = b S + c S S, X <- a X + P X
-// (X X^T for rows <= cols, X^T X and X <- a X + X P otherwise: the Gram matrix of the
-// shorter side, without a transpose). Step update: m' = mu m + g, G = g + mu m' (Nesterov)
+//   X0 = G / (|G|_F + eps);  each step: S = X X^T, P = a I + b S + c S S, X <- P X
+// (X X^T for rows <= cols, X^T X and X <- X P otherwise: the Gram matrix of the shorter
+// side, without a transpose; a on P's diagonal, so that only P's epilogue reads a matrix). Step update: m' = mu m + g, G = g + mu m' (Nesterov)
 // or m', p' = p (1 - lr wd) - lr sqrt(max(1, rows / cols)) X.
 //
 // Per step 3 products on the tensor cores (tc_tile.cuh). S and P are symmetric: only the
@@ -41,51 +41,52 @@ __device__ __forceinline__ void unpack_f16(uint32_t u, float& a, float& b) {
   a = f.x, b = f.y;
 }
 
-constexpr int GRAM = 0, POLY = 1, NEXT = 2;
+constexpr int GRAM = 0, POLY = 1, NEXT = 2, LAST = 3;
 
-// result = cc acc + ca source, as fp16 planes (and mirrored), or out = fa add + fb result
+// result = cc product + ca source + diag I (POLY), as fp16 planes, mirrored where symmetric;
+// LAST: out = cc product + fa add
 struct NsEpi {
   struct Args {
     const __half* src;  // planes at the result's offsets, or NULL
     __half* dst;        // planes, or NULL: the last product
     int64_t ld, plane, batch;
-    float ca, cc;
+    float ca, cc, diag;
     int planes, mirror;
     void* out;
     const float* add;  // fp32, dense as out
     int64_t M, N;
-    float fa, fb;
+    float fa;
     int bf16;
     const int* e0;               // [batch]: the exponent of t at the start
-    int e_down, e_down_next;     // how far it has shrunk, and will have after this product
-    int which;                   // GRAM, POLY, NEXT
+    int e_down, e_down_next;     // how far it has shrunk, and will have after this step
+    int which;                   // GRAM, POLY, NEXT, LAST
   };
+  static constexpr bool SINGLE_WIDE = false, SINGLE_NARROW = true, TEAMS = true, INIT = true;
   const Args& a;
-  float ca, cc, fb;
+  float scale, ca, diag;
   __device__ explicit NsEpi(const Args& args) : a(args) {}
   __device__ __forceinline__ void begin(const Spot& sp) {
-    ca = a.ca, cc = a.cc, fb = a.fb;
+    scale = a.cc, ca = a.ca, diag = a.diag;
     const int e0 = a.e0[sp.z];
-    if (e0 == 0) return;
-    const int e = max(0, e0 - a.e_down), next = a.dst ? max(0, e0 - a.e_down_next) : 0;
-    if (a.which == POLY) {
-      ca = ldexpf(ca, -2 * e);
-      cc = ldexpf(cc, -4 * e);
-    } else if (a.which == NEXT && a.dst) {
-      ca = ldexpf(ca, next - e);
-      cc = ldexpf(cc, next - e);
-    } else if (a.which == NEXT) {
-      fb = ldexpf(fb, -e);
+    if (e0 != 0) {
+      const int e = max(0, e0 - a.e_down), shrink = max(0, e0 - a.e_down_next) - e;
+      if (a.which == POLY) {
+        ca = ldexpf(ca, shrink - 2 * e);
+        scale = ldexpf(scale, shrink - 4 * e);
+        diag = ldexpf(diag, shrink);
+      } else if (a.which == LAST) {
+        scale = ldexpf(scale, -e);
+      }
     }
   }
   __device__ __forceinline__ void end(const Spot&) {}
+  __device__ __forceinline__ void finish(int) {}
 
-  __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
-    const int rows = (int)min((int64_t)32, a.M - sp.row0);
+  // what the product is added to: ca source + diag I, or fa add
+  __device__ __forceinline__ void init(const Spot& sp, int64_t col, float (&v)[32]) {
     const int64_t cols = min((int64_t)32, a.N - col);
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] *= cc;
-    if (a.src && sp.row < a.M) {
+    if (sp.row >= a.M) return;
+    if (a.which == POLY) {
       const __half* p = a.src + sp.z * a.batch + sp.row * a.ld + col;
       for (int k = 0; k < a.planes; ++k)
 #pragma unroll
@@ -101,17 +102,33 @@ struct NsEpi {
               v[8 * j + 2 * i + 1] = fmaf(ca, y, v[8 * j + 2 * i + 1]);
             }
           }
-    }
-    if (!a.dst) {
-      const int64_t at = (sp.z * a.M + sp.row0) * a.N + col;
-      if (a.add) {
-        const float* p = a.add + at + sp.lane * a.N;
+      const int64_t k = sp.row - col;
+      if (k >= 0 && k < 32) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] = (sp.lane < rows && i < cols ? p[i] * a.fa : 0.f) + fb * v[i];
+        for (int i = 0; i < 32; ++i)
+          if (k == i) v[i] += diag;
+      }
+    } else if (a.which == LAST && a.add) {
+      const float* p = a.add + (sp.z * a.M + sp.row) * a.N + col;
+      if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 4) {
+          const float4 t = *reinterpret_cast<const float4*>(p + i);
+          v[i] = a.fa * t.x, v[i + 1] = a.fa * t.y, v[i + 2] = a.fa * t.z, v[i + 3] = a.fa * t.w;
+        }
       } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) v[i] *= fb;
+        for (int i = 0; i < 32; ++i)
+          if (i < cols) v[i] = a.fa * p[i];
       }
+    }
+  }
+
+  __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
+    const int rows = (int)min((int64_t)32, a.M - sp.row0);
+    const int64_t cols = min((int64_t)32, a.N - col);
+    if (a.which == LAST) {
+      const int64_t at = (sp.z * a.M + sp.row0) * a.N + col;
       __syncwarp();
       if (a.bf16) {
         uint32_t w[16];
@@ -130,23 +147,44 @@ struct NsEpi {
       }
       return;
     }
+    // The chunk goes through shared memory, 64-byte rows whose four 16-byte pieces are swizzled by
+    // (row / 2) ^ (row / 8): rows written and read, and 8 x 8 blocks read transposed, are then free
+    // of bank conflicts. Rows leave as 64 adjacent bytes each way.
+    const int lane = sp.lane;
+    const bool mirror = a.mirror && sp.above;
     for (int k = 0; k < a.planes; ++k) {
       __half* d = a.dst + sp.z * a.batch + k * a.plane;
+      const uint32_t buf = sp.buf + (uint32_t)(k & 1) * 2048u;
       uint32_t w[16];
 #pragma unroll
       for (int i = 0; i < 16; ++i) w[i] = pack_f16(v[2 * i], v[2 * i + 1]);
       __syncwarp();
-      stage_chunk<2>(sp.buf, sp.lane, w);
-      __syncwarp();
-      write_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(d + sp.row0 * a.ld + col), a.ld, rows, cols);
-      if (a.mirror && sp.mt != sp.nt && sp.lane < rows) {
-        // the transposed tile: 32 lanes store 32 adjacent elements of each of its rows
-        __half* m = d + col * a.ld + sp.row;
+      const uint32_t f = (uint32_t)((lane >> 1) ^ (lane >> 3)) & 3u;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const __half2 h = *reinterpret_cast<const __half2*>(&w[i]);
-          if (2 * i < cols) m[(2 * i) * a.ld] = __low2half(h);
-          if (2 * i + 1 < cols) m[(2 * i + 1) * a.ld] = __high2half(h);
+      for (int j = 0; j < 4; ++j)
+        st_shared_v4(buf + (uint32_t)lane * 64u + (((uint32_t)j ^ f) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+      __syncwarp();
+      // 8 rows of 4 pieces at a time (rows are padded to 8 elements: whole pieces)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = 8 * i + (lane >> 2), j = lane & 3;
+        const uint4 u = ld_shared_v4(buf + (uint32_t)r * 64u + (((uint32_t)j ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4));
+        if (r < rows && 8 * j < cols) *reinterpret_cast<uint4*>(d + (sp.row0 + r) * a.ld + col + 8 * j) = u;
+      }
+      if (mirror) {
+        // four 8 x 8 blocks transposed: block m's rows are 8 c/2 + 2 m + c%2 (c = 0..7), so that
+        // thread l ends up with rows 8 (l % 4) .. + 7 of source column 8 g + l / 4
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int c = lane & 7, r = 8 * (c >> 1) + 2 * (lane >> 3) + (c & 1);
+          uint4 u;
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                       : "r"(buf + (uint32_t)r * 64u + (((uint32_t)g ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4))
+                       : "memory");
+          const int cc = 8 * g + (lane >> 2), j = lane & 3;
+          // the mirrored rows are as long as the result: whole pieces up to the padding
+          if (cc < cols && 8 * j < rows) *reinterpret_cast<uint4*>(d + (col + cc) * a.ld + sp.row0 + 8 * j) = u;
         }
       }
       if (k + 1 < a.planes) {
@@ -162,8 +200,33 @@ struct NsEpi {
   }
 };
 
-__device__ __forceinline__ float value_at(const void* g, int bf16, int64_t i) {
-  return bf16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(g)[i]) : reinterpret_cast<const float*>(g)[i];
+// 8 values from element i on (the first n of them; the rest zeros): 16-byte loads where all 8
+// are there and aligned
+__device__ __forceinline__ void load8(const void* g, int bf16, int64_t i, int64_t n, float (&v)[8]) {
+  if (bf16) {
+    const __nv_bfloat16* p = reinterpret_cast<const __nv_bfloat16*>(g) + i;
+    if (n >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[2 * j] = __uint_as_float(w[j] << 16);
+        v[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? __bfloat162float(p[j]) : 0.f;
+    }
+  } else {
+    const float* p = reinterpret_cast<const float*>(g) + i;
+    if (n >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? p[j] : 0.f;
+    }
+  }
 }
 
 // Sums of squares of each matrix, a part per block. With a momentum: m' = mu m + g is
@@ -173,14 +236,30 @@ __global__ void __launch_bounds__(NT) square_kernel(const void* g, int bf16, con
   __shared__ double red[NT / 32];
   const int64_t base = (int64_t)blockIdx.y * n;
   double s = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
-    float v = value_at(g, bf16, base + i);
+  for (int64_t i = ((int64_t)blockIdx.x * NT + threadIdx.x) * 8; i < n; i += (int64_t)gridDim.x * NT * 8) {
+    const int64_t left = n - i;
+    float v[8];
+    load8(g, bf16, base + i, left, v);
     if (mom) {
-      const float m = mu * mom[base + i] + v;
-      mom_out[base + i] = m;
-      v = nesterov ? v + mu * m : m;
+      float m[8];
+      load8(mom, 0, base + i, left, m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        m[j] = mu * m[j] + v[j];
+        v[j] = nesterov ? v[j] + mu * m[j] : m[j];
+      }
+      float* p = mom_out + base + i;
+      if (left >= 8 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+        *reinterpret_cast<float4*>(p) = make_float4(m[0], m[1], m[2], m[3]);
+        *reinterpret_cast<float4*>(p + 4) = make_float4(m[4], m[5], m[6], m[7]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (j < left) p[j] = m[j];
+      }
     }
-    s += (double)v * (double)v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (double)v[j] * (double)v[j];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
@@ -192,10 +271,10 @@ __global__ void __launch_bounds__(NT) square_kernel(const void* g, int bf16, con
   }
 }
 
-// X0 = 2^8 G / (|G| + eps) as fp16 planes with rows padded to 8 elements
+// X0 = 2^8 t G / (|G| + eps) as fp16 planes with rows padded to 8 elements; t's exponent
 __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, const float* mom, float mu, int nesterov, const double* part,
-                                                   int parts, float eps, int* e0, __half* x, int64_t ld, int64_t plane, int64_t batch, int planes,
-                                                   int64_t rows, int64_t cols) {
+                                                   int parts, float eps, int* e0, __half* x, int64_t ld, int64_t plane, int64_t batch,
+                                                   int planes, int64_t rows, int64_t cols) {
   __shared__ double red[NT / 32];
   double s = 0.0;
   for (int i = threadIdx.x; i < parts; i += NT) s += part[(int64_t)blockIdx.y * parts + i];
@@ -211,20 +290,18 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
   const float scale = (float)(ldexp((double)SCALE, e) / (norm + (double)eps));
   const int64_t base = (int64_t)blockIdx.y * rows * cols, per = ld / 8;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * NT) {
-    const int64_t r = i / per, c = i % per * 8;
+    const int64_t r = i / per, c = i % per * 8, at = base + r * cols + c;
     float v[8];
-    for (int j = 0; j < 8; ++j) {
-      v[j] = 0.f;
-      if (c + j < cols) {
-        const int64_t at = base + r * cols + c + j;
-        float t = value_at(g, bf16, at);
-        if (mom) t = nesterov ? t + mu * mom[at] : mom[at];  // mom: the new momentum
-        v[j] = t * scale;
-      }
+    if (!mom || nesterov) load8(g, bf16, at, cols - c, v);
+    if (mom) {  // the new momentum
+      float m[8];
+      load8(mom, 0, at, cols - c, m);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = nesterov ? v[j] + mu * m[j] : m[j];
     }
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j], v[2 * j + 1]);
+    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j] * scale, v[2 * j + 1] * scale);
     __half* d = x + (int64_t)blockIdx.y * batch + r * ld + c;
     *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
     if (planes > 1) {
@@ -232,7 +309,7 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
       for (int j = 0; j < 4; ++j) {
         float a, b;
         unpack_f16(w[j], a, b);
-        w[j] = pack_f16(v[2 * j] - a, v[2 * j + 1] - b);
+        w[j] = pack_f16(v[2 * j] * scale - a, v[2 * j + 1] * scale - b);
       }
       *reinterpret_cast<uint4*>(d + plane) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -270,18 +347,18 @@ static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
   return q;
 }
 
-// One product, on CTA pairs (256 x 256 tiles) when those alone fill two thirds of them, else
-// on 128 x 128 tiles of single CTAs: a 1024 x 1024 product has 16 of the former (10 above
-// the diagonal) for 74 pairs, 64 (36) of the latter.
+// One product, on CTA pairs when their tiles (256 x 256, or 256 x 128 of split operands) fill
+// two thirds of them, else on 128 x 128 tiles of single CTAs: a 1024 x 1024 product has 16 of
+// 256 x 256 (10 reach the diagonal) for 74 pairs, 64 (36) of 128 x 128 for 148 CTAs.
 static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, bool triangle,
                    const NsEpi::Args& a, cudaStream_t s, const char* what) {
   Loop lp = {};
   lp.group_m = 16;
   lp.walk = triangle ? WALK_TRIANGLE : WALK_GROUPED;
-  const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, 256);
-  const int64_t tiles = (triangle ? tn * (tn + 1) / 2 : tm * tn) * batch;
-  if (M > 128 && N > 128 && tiles * 3 >= num_sms()) return launch<256, true, NsEpi>(A, B, M, N, K, batch, planes, lp, a, s, what);
-  return launch<128, false, NsEpi>(A, B, M, N, K, batch, planes, lp, a, s, what);
+  const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, planes > 1 ? 128 : 256);
+  const int64_t tiles = (triangle ? tm * (tn + planes) / 2 : tm * tn) * batch;
+  const bool pair = M > 128 && N > 128 && tiles * 3 >= num_sms();
+  return launch<NsEpi>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
 }
 
 struct Finish {  // out = fa add + fb X
@@ -314,14 +391,15 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
   double grown = 0.0;  // log2 of how far a has made the smallest X grow
   for (int i = 0; i < steps; ++i) {
     const float a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
+    const bool last = i + 1 == steps;
     Operand X, Gm;
     X.base = x[i & 1], X.ld = q.ldx, X.plane_stride = q.xn, X.batch_stride = xb, X.mn = tall;
     Gm.ld = q.ldg, Gm.plane_stride = q.gn, Gm.batch_stride = gb;
     NsEpi::Args e = {};
     e.e0 = e0;
-    e.e_down = (int)std::floor(grown);
+    e.e_down = e.e_down_next = (int)std::floor(grown);
     grown += std::max(0.0, std::log2((double)std::fabs(a)));
-    e.e_down_next = (int)std::floor(grown);
+    if (!last) e.e_down_next = (int)std::floor(grown);
     e.which = GRAM;
     e.planes = q.planes;
     e.M = e.N = q.side;
@@ -332,20 +410,19 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
     rc = product(X, X, q.side, q.side, tall ? rows : cols, batch, q.planes, true, e, s, what);
     if (rc) return rc;
     e.which = POLY;
-    e.src = S, e.dst = P, e.ca = b, e.cc = c / SCALE;
+    e.src = S, e.dst = P, e.ca = b, e.cc = c / SCALE, e.diag = a * SCALE;
     Gm.base = S;
     rc = product(Gm, Gm, q.side, q.side, q.side, batch, q.planes, true, e, s, what);
     if (rc) return rc;
     Gm.base = P;
-    const bool last = i + 1 == steps;
     NsEpi::Args r = {};
-    r.e0 = e0, r.e_down = e.e_down, r.e_down_next = e.e_down_next, r.which = NEXT;
+    r.e0 = e0, r.e_down = r.e_down_next = e.e_down, r.which = last ? LAST : NEXT;
     r.planes = q.planes;
     r.M = rows, r.N = cols;
     r.ld = q.ldx, r.plane = q.xn, r.batch = xb;
-    r.src = x[i & 1], r.ca = a, r.cc = 1.f / SCALE;
+    r.cc = last ? f.fb / (SCALE * SCALE) : 1.f / SCALE;
     r.dst = last ? nullptr : x[(i + 1) & 1];
-    r.out = f.out, r.add = f.add, r.fa = f.fa, r.fb = f.fb / SCALE, r.bf16 = f.bf16;
+    r.out = f.out, r.add = f.add, r.fa = f.fa, r.bf16 = f.bf16;
     // P X (wide: X's columns are the result's) or X P (tall); P's rows serve as its columns
     Operand Xo = X;
     Xo.mn = tall ? 0 : 1;

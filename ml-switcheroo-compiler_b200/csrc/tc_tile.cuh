@@ -3,21 +3,29 @@
 // and an epilogue object that gets each accumulator 32 columns at a time.
 //
 // Two things are wider than in the graph GEMM (gemm_tc.cu):
-//  * an operand may come as two 16-bit planes, hi + lo of fp32 values (16 or 22 bits). The
-//    loop then runs three segments into the same accumulator, hi.lo + lo.hi + hi.hi, which
-//    is the fp32 product up to lo.lo: a third of the tensor rate instead of the CUDA cores'.
-//    The tensor cores cut (not round) each sum to fp32: 2^-24 of it per 16 products, all
-//    towards zero, which over K = 50000 is 1e-4. So the accumulator is drained every 512 of
-//    K and added up in registers with rounding (SPLIT), the small segments first: at most
-//    32 cuts at full size;
+//  * an operand may come as two 16-bit planes, hi + lo of fp32 values (SPLIT; 16 or 22
+//    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is the fp32 product up to lo.lo: a third of the tensor rate
+//    instead of the CUDA cores'. The tensor cores cut (not round) each sum to fp32: up to
+//    2^-23 of it per 16 products, all towards zero, which over K = 50000 was 1e-4. So the
+//    hi.hi accumulator is drained every CHUNK K blocks (16 cuts) and added up in registers
+//    with rounding; the other two products are 2^-8 to 2^-11 of it and have an accumulator of
+//    their own for the whole tile;
 //  * the tiles are walked in groups of M tiles (their A rows stay in L2 while B streams
 //    past once per group), over the upper triangle of a symmetric result, or over splits of
 //    the K axis, each with its own partial result.
 //
 // Roles as in gemm_tc.cu: warp 0 issues TMA loads, warp 1 owns TMEM and issues the MMAs,
-// eight epilogue warps (two per TMEM lane quarter) drain the double-buffered accumulator
-// while the next tile's MMAs run. PAIR: two CTAs of a cluster share a 256 x BN tile
-// (cta_group::2), each loading its 128 rows of A and half of B.
+// warps 2 to 9 (two per TMEM lane quarter) drain the double-buffered accumulator while the
+// next MMAs run. PAIR: two CTAs of a cluster share a 256 x BN tile (cta_group::2), each
+// loading its 128 rows of A and half of B: a single CTA's 128 x 128 tile reads and writes
+// 64 KB of shared memory per K block, twice the time of its MMAs; a pair's 256 x 256 tile
+// half its MMAs' time.
+// Split operands take tiles 128 wide: a drained tile is 64 registers a thread (128 of the
+// 168 there are would spill), and 120 KB of shared-memory traffic per K block cost 940
+// clocks beside 786 of MMAs.
+// TEAM: where single tiles would leave most SMs idle, a cluster of 2 or 4 CTAs shares one
+// tile's K axis; each then sends its partial sums of the columns that another one owns
+// through shared memory (in place of the operands, all read by then) and finishes its own.
 // Every wait is bounded (tc_common.cuh); on expiry the device error flag is set and the
 // block winds down.
 #pragma once
@@ -30,31 +38,35 @@ namespace tile {
 
 using namespace tc;
 
-constexpr int BM = 128, BK = 64, EPI_WARPS = 8, THREADS = 64 + 32 * EPI_WARPS;
+constexpr int BM = 128, BK = 64, EPI_WARPS = 8, EPI_FIRST = 2, THREADS = 32 * (EPI_FIRST + EPI_WARPS);
 constexpr uint32_t EPI_BUF = 4096;  // staging bytes per epilogue warp
 constexpr uint32_t LEADER = 0xFEFFFFFFu;  // shared-memory address mask of a pair's CTA 0
 
-template <int BN, bool PAIR>
+template <int BN, bool PAIR, bool SPLIT>
 struct Geo {
-  static constexpr int STAGES = BN == 256 ? (PAIR ? 6 : 4) : 6;
+  static constexpr int PLANES = SPLIT ? 2 : 1;
+  static_assert(!SPLIT || BN == 128, "split operands: 128-wide tiles");
+  static constexpr int STAGES = SPLIT ? (PAIR ? 4 : 3) : (BN == 256 && !PAIR ? 4 : 6);
   static constexpr int TM = PAIR ? 2 * BM : BM;
   static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
-  static constexpr size_t SMEM = (size_t)STAGES * (A_BYTES + B_BYTES) + EPI_WARPS * EPI_BUF + 1024 + 256;
+  static constexpr uint32_t TMEM = (SPLIT ? 4 : 2) * BN;  // columns: two accumulators, and two for the small products
+  static constexpr uint32_t STAGE = PLANES * (A_BYTES + B_BYTES);
+  static constexpr size_t SMEM = (size_t)STAGES * STAGE + EPI_WARPS * EPI_BUF + 1024 + 256;
   static_assert(SMEM <= 232448, "operand ring and staging must fit 227 KB");
 };
 
-constexpr int CHUNK = 8;  // K blocks per accumulator of split operands
+constexpr int CHUNK = 4;  // K blocks per accumulator of split operands
 constexpr int WALK_GROUPED = 0, WALK_TRIANGLE = 1;
 
 struct Loop {
   int nk;        // K blocks in all
   int nk_split;  // K blocks per split (= nk without splits)
-  int nseg;      // 1, or 3 for hi.lo + lo.hi + hi.hi
   int chunk;     // K blocks that one accumulator takes before it is drained
   int a_mn, b_mn, bf16;
-  int tiles_m, tiles_n, group_m, walk;
+  int tiles_m, tiles_n, group_m, walk, wide;
   int per_batch, total;  // tiles of one batch entry (splits included), of all
   int splits;
+  int team;      // CTAs of a cluster that share a tile's K axis (TEAM)
 };
 
 struct Tile {
@@ -69,12 +81,15 @@ __device__ __forceinline__ Tile tile_at(const Loop& lp, int t) {
   r.split = i / per_split;
   i %= per_split;
   if (lp.walk == WALK_TRIANGLE) {
-    // i = nt (nt + 1) / 2 + mt, mt <= nt
-    int nt = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
-    while ((nt + 1) * (nt + 2) / 2 <= i) ++nt;
-    while (nt * (nt + 1) / 2 > i) --nt;
-    r.nt = nt;
-    r.mt = i - nt * (nt + 1) / 2;
+    // tiles that reach the diagonal or lie above it, column by column: with `wide` tile
+    // columns to a tile row, columns wide p .. wide p + wide - 1 have rows 0 .. p
+    const int w = lp.wide;
+    int p = (int)((sqrtf(8.f * (float)i / (float)w + 1.f) - 1.f) * 0.5f);
+    while (w * (p + 1) * (p + 2) / 2 <= i) ++p;
+    while (w * p * (p + 1) / 2 > i) --p;
+    i -= w * p * (p + 1) / 2;
+    r.nt = w * p + i / (p + 1);
+    r.mt = i % (p + 1);
     return r;
   }
   const int per_group = lp.group_m * lp.tiles_n;
@@ -132,23 +147,23 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 // What an epilogue warp knows about its chunk: `row` is this lane's output row, `row0` the
 // warp's first one, `buf` its staging buffer
 struct Spot {
-  int64_t row, row0;
+  int64_t row, row0, col0;  // col0: first of this warp's columns
   int z, split, mt, nt, half, lane;
+  bool above;  // the whole tile lies above the diagonal
   uint32_t buf;
 };
 
-// Epi: begin(spot) once per tile, chunk(spot, column, values[32]) for each 32 columns
-// inside the result, end(spot).
-template <int BN, bool PAIR, bool SPLIT, typename Epi>
+// Epi: begin(spot) once per tile, init(spot, column, values[32]) where INIT, ahead of the
+// product (result = values + scale * product), chunk(spot, column, values[32]) for each 32 columns
+// inside the result, end(spot); finish(lane) at the end of the kernel.
+template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtensorMap& map_b, const Loop& lp, int64_t M, int64_t N,
                                           Epi& epi) {
-  using G = Geo<BN, PAIR>;
+  using G = Geo<BN, PAIR, SPLIT>;
   constexpr int STG = G::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_a = smem;
-  uint8_t* s_b = smem + STG * G::A_BYTES;
-  uint8_t* s_epi = s_b + STG * G::B_BYTES;
+  uint8_t* s_epi = smem + STG * G::STAGE;  // a stage: A's planes, then B's
   uint64_t* full_bar = reinterpret_cast<uint64_t*>(s_epi + EPI_WARPS * EPI_BUF);
   uint64_t* empty_bar = full_bar + STG;
   uint64_t* acc_full = empty_bar + STG;
@@ -157,8 +172,9 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
-  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
-  const int units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
+  const int member = TEAM ? (int)cluster_rank() : 0;
+  const int per_unit = PAIR ? 2 : (TEAM ? lp.team : 1);
+  const int unit = (int)blockIdx.x / per_unit, units = (int)gridDim.x / per_unit;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STG; ++s) {
@@ -173,10 +189,10 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
   }
   if (warp == 1) {
     if constexpr (PAIR) {
-      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN));
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(G::TMEM));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
     } else {
-      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(2 * BN));
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(G::TMEM));
       asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
   }
@@ -186,42 +202,39 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
-    if (lane == 0) {
+  if (warp < EPI_FIRST) {
+    if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
       for (int t = unit; t < lp.total && ok; t += units) {
         const Tile at = tile_at(lp, t);
         const int m0 = at.mt * G::TM + (int)rank * BM;
         const int n0 = at.nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
-        const int kb0 = at.split * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
-        for (int c0 = kb0; c0 < kb1 && ok; c0 += lp.chunk) {
-          const int c1 = min(kb1, c0 + lp.chunk);
-          for (int seg = 0; seg < lp.nseg && ok; ++seg) {
-            const int pa = lp.nseg == 3 && seg == 1, pb = lp.nseg == 3 && seg == 0;  // planes: hi.lo, lo.hi, hi.hi
-            for (int kb = c0; kb < c1; ++kb, ++it) {
-              const int s = it % STG;
-              if (!mbar_wait(&empty_bar[s], ((it / STG) & 1) ^ 1)) {
-                ok = false;
-                break;
-              }
-              if (rank == 0) mbar_expect_tx(&full_bar[s], (PAIR ? 2u : 1u) * (G::A_BYTES + G::B_BYTES));
-              const int k0 = kb * BK;
-              uint8_t* a_dst = s_a + s * G::A_BYTES;
-              uint8_t* b_dst = s_b + s * G::B_BYTES;
-              if (!lp.a_mn) {
-                load4<PAIR>(a_dst, &map_a, &full_bar[s], k0, m0, pa, at.z);
-              } else {
-                load4<PAIR>(a_dst, &map_a, &full_bar[s], m0, k0, pa, at.z);
-                load4<PAIR>(a_dst + 8192, &map_a, &full_bar[s], m0 + 64, k0, pa, at.z);
-              }
-              if (!lp.b_mn) {
-                load4<PAIR>(b_dst, &map_b, &full_bar[s], k0, n0, pb, at.z);
-              } else {
+        const int kb0 = (TEAM ? member : at.split) * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
+        for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          const int s = it % STG;
+          if (!mbar_wait(&empty_bar[s], ((it / STG) & 1) ^ 1)) {
+            ok = false;
+            break;
+          }
+          if (rank == 0) mbar_expect_tx(&full_bar[s], (PAIR ? 2u : 1u) * G::STAGE);
+          const int k0 = kb * BK;
 #pragma unroll
-                for (int j = 0; j < (PAIR ? BN / 2 : BN) / 64; ++j)
-                  load4<PAIR>(b_dst + j * 8192, &map_b, &full_bar[s], n0 + 64 * j, k0, pb, at.z);
-              }
+          for (int p = 0; p < G::PLANES; ++p) {
+            uint8_t* a_dst = smem + s * G::STAGE + p * G::A_BYTES;
+            uint8_t* b_dst = smem + s * G::STAGE + G::PLANES * G::A_BYTES + p * G::B_BYTES;
+            if (!lp.a_mn) {
+              load4<PAIR>(a_dst, &map_a, &full_bar[s], k0, m0, p, at.z);
+            } else {
+              load4<PAIR>(a_dst, &map_a, &full_bar[s], m0, k0, p, at.z);
+              load4<PAIR>(a_dst + 8192, &map_a, &full_bar[s], m0 + 64, k0, p, at.z);
+            }
+            if (!lp.b_mn) {
+              load4<PAIR>(b_dst, &map_b, &full_bar[s], k0, n0, p, at.z);
+            } else {
+#pragma unroll
+              for (int j = 0; j < (PAIR ? BN / 2 : BN) / 64; ++j)
+                load4<PAIR>(b_dst + j * 8192, &map_b, &full_bar[s], n0 + 64 * j, k0, p, at.z);
             }
           }
         }
@@ -232,15 +245,15 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
         for (int i = 0; i < STG && ok; ++i, ++it) ok = mbar_wait(&empty_bar[it % STG], ((it / STG) & 1) ^ 1, 64);
       }
     }
-  } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
+    if (warp == 1 && lane == 0 && rank == 0) {
       const uint32_t fmt = lp.bf16 ? (1u << 7) | (1u << 10) : 0u;
       const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)lp.a_mn << 15) | ((uint32_t)lp.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
                              ((uint32_t)(G::TM >> 4) << 24);
       uint32_t it = 0, local = 0;
       bool ok = true;
-      for (int t = unit; t < lp.total && ok; t += units) {
-        const int split = t % lp.per_batch / (lp.per_batch / lp.splits);
+      uint32_t tiles = 0;
+      for (int t = unit; t < lp.total && ok; t += units, ++tiles) {
+        const int split = TEAM ? member : t % lp.per_batch / (lp.per_batch / lp.splits);
         const int kb0 = split * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
         for (int c0 = kb0; c0 < kb1 && ok; c0 += lp.chunk, ++local) {
           const int b = local & 1;
@@ -250,20 +263,27 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           }
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(b * BN);
-          const int steps = lp.nseg * (min(kb1, c0 + lp.chunk) - c0);
-          for (int i = 0; i < steps; ++i, ++it) {
+          const int c1 = min(kb1, c0 + lp.chunk);
+          for (int kb = c0; kb < c1; ++kb, ++it) {
             const int s = it % STG;
             if (!mbar_wait(&full_bar[s], (it / STG) & 1)) {
               ok = false;
               break;
             }
             tc_fence_after();
-            const uint32_t a0 = smem_u32(s_a + s * G::A_BYTES), b0 = smem_u32(s_b + s * G::B_BYTES);
+            const uint32_t a0 = smem_u32(smem + s * G::STAGE), b0 = a0 + G::PLANES * G::A_BYTES;
 #pragma unroll
-            for (int k = 0; k < BK / 16; ++k) {
-              const uint64_t ad = lp.a_mn ? smem_desc(a0 + k * 2048, 8192, 1024) : smem_desc(a0 + k * 32, 16, 1024);
-              const uint64_t bd = lp.b_mn ? smem_desc(b0 + k * 2048, 8192, 1024) : smem_desc(b0 + k * 32, 16, 1024);
-              mma<PAIR>(d, ad, bd, idesc, (i > 0 || k > 0) ? 1u : 0u);
+            for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
+              // hi.lo and lo.hi into the tile's accumulator of small products, hi.hi into the chunk's
+              const uint32_t as = a0 + (SPLIT && seg == 1 ? G::A_BYTES : 0u), bs = b0 + (SPLIT && seg == 0 ? G::B_BYTES : 0u);
+              const uint32_t to = seg < 2 ? tmem + (uint32_t)((2 + (tiles & 1)) * BN) : d;
+              const bool fresh = seg == 0 ? kb == kb0 : (seg == 2 && kb == c0);
+#pragma unroll
+              for (int k = 0; k < BK / 16; ++k) {
+                const uint64_t ad = lp.a_mn ? smem_desc(as + k * 2048, 8192, 1024) : smem_desc(as + k * 32, 16, 1024);
+                const uint64_t bd = lp.b_mn ? smem_desc(bs + k * 2048, 8192, 1024) : smem_desc(bs + k * 32, 16, 1024);
+                mma<PAIR>(to, ad, bd, idesc, (!fresh || k > 0) ? 1u : 0u);
+              }
             }
             commit<PAIR>(&empty_bar[s]);
           }
@@ -271,14 +291,18 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
         }
       }
     }
+    if constexpr (TEAM) {  // the epilogue's two meetings
+      cluster_sync_all();
+      cluster_sync_all();
+    }
   } else {
     Spot sp;
     const int q = warp & 3;
-    sp.half = (warp - 2) >> 2;
+    sp.half = (warp - EPI_FIRST) >> 2;
     sp.lane = lane;
-    sp.buf = smem_u32(s_epi) + (uint32_t)(warp - 2) * EPI_BUF;
+    sp.buf = smem_u32(s_epi) + (uint32_t)(warp - EPI_FIRST) * EPI_BUF;
     constexpr int CH = BN / 64;  // chunks of 32 columns per warp
-    uint32_t local = 0;
+    uint32_t local = 0, tiles = 0;
     bool ok = true;
     // the accumulator may be overwritten once every epilogue warp has read it
     auto release = [&](int b) {
@@ -298,12 +322,32 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       sp.nt = at.nt;
       sp.row0 = (int64_t)at.mt * G::TM + (int64_t)rank * BM + q * 32;
       sp.row = sp.row0 + lane;
-      const int64_t col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
+      const int64_t col0 = sp.col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
+      sp.above = (int64_t)at.nt * BN >= (int64_t)(at.mt + 1) * G::TM;
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
       epi.begin(sp);
-      if constexpr (SPLIT) {
+      // the member that finishes chunk c of this warp
+      auto owner = [&](int c) { return TEAM ? (sp.half * CH + c) * lp.team / (2 * CH) : 0; };
+      if constexpr (SPLIT || TEAM) {
         float acc[CH][32];
-        const int kb0 = at.split * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
+          if constexpr (Epi::INIT)
+            if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.init(sp, col0 + c * 32, acc[c]);
+        }
+        auto add = [&](uint32_t at_col, float (&to)[32]) {
+          uint32_t cur[32];
+          tmem_ld32_issue(base + at_col, cur);
+          tmem_wait(cur);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if constexpr (Epi::INIT) to[i] = fmaf(epi.scale, __uint_as_float(cur[i]), to[i]);
+            else to[i] += __uint_as_float(cur[i]);
+          }
+        };
+        const int kb0 = (TEAM ? member : at.split) * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
         for (int c0 = kb0; c0 < kb1; c0 += lp.chunk, ++local) {
           const int b = local & 1;
           if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) {
@@ -313,56 +357,102 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
-            uint32_t cur[32];
-            tmem_ld32_issue(base + (uint32_t)(b * BN + c * 32), cur);
-            tmem_wait(cur);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) acc[c][i] = c0 == kb0 ? __uint_as_float(cur[i]) : acc[c][i] + __uint_as_float(cur[i]);
+            add((uint32_t)(b * BN + c * 32), acc[c]);
+            if (SPLIT && c0 + lp.chunk >= kb1) add((uint32_t)((2 + (tiles & 1)) * BN + c * 32), acc[c]);
           }
           release(b);
+        }
+        ++tiles;
+        if constexpr (TEAM) {
+          // every member's MMAs are done: the operand ring takes the partial sums, 16 KB (128 rows
+          // of 32, 16-byte pieces swizzled by row) per chunk and sender
+          cluster_sync_all();
+          const int each = 2 * CH / lp.team;
+          const uint32_t line = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 128u;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            const int to = owner(c);
+            if (to == member) continue;
+            const int slot = (member < to ? member : member - 1) * each + (sp.half * CH + c) % each;
+            uint32_t far;
+            asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(line + (uint32_t)slot * 16384u), "r"(to));
+#pragma unroll
+            for (int p = 0; p < 8; ++p)
+              asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(far + (uint32_t)((p ^ (lane & 7)) << 4)),
+                           "f"(acc[c][4 * p]), "f"(acc[c][4 * p + 1]), "f"(acc[c][4 * p + 2]), "f"(acc[c][4 * p + 3])
+                           : "memory");
+          }
+          cluster_sync_all();
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            if (owner(c) != member) continue;
+            for (int from = 0; from < lp.team - 1; ++from) {
+              const uint32_t at_line = line + (uint32_t)(from * each + (sp.half * CH + c) % each) * 16384u;
+#pragma unroll
+              for (int p = 0; p < 8; ++p) {
+                const uint4 u = ld_shared_v4(at_line + (uint32_t)((p ^ (lane & 7)) << 4));
+                acc[c][4 * p] += __uint_as_float(u.x);
+                acc[c][4 * p + 1] += __uint_as_float(u.y);
+                acc[c][4 * p + 2] += __uint_as_float(u.z);
+                acc[c][4 * p + 3] += __uint_as_float(u.w);
+              }
+            }
+          }
         }
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < CH; ++c)
-          if (col0 + c * 32 < N && sp.row0 < M) epi.chunk(sp, col0 + c * 32, acc[c]);  // warp-uniform
+          if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.chunk(sp, col0 + c * 32, acc[c]);  // warp-uniform
       } else {
         const int b = local & 1;
         if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) break;
         tc_fence_after();
+        uint32_t cur[32];
+        tmem_ld32_issue(base + (uint32_t)(b * BN), cur);
 #pragma unroll 1
         for (int c = 0; c < CH; ++c) {
           const int64_t col = col0 + c * 32;
-          if (col >= N || sp.row0 >= M) break;  // warp-uniform
-          uint32_t cur[32];
-          tmem_ld32_issue(base + (uint32_t)(b * BN + c * 32), cur);
-          tmem_wait(cur);
+          const bool inside = col < N && sp.row0 < M;  // warp-uniform
           float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(cur[i]);
+          for (int i = 0; i < 32; ++i) v[i] = 0.f;
+          if constexpr (Epi::INIT)
+            if (inside) epi.init(sp, col, v);
+          tmem_wait(cur);
+          if (!inside) break;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if constexpr (Epi::INIT) v[i] = fmaf(epi.scale, __uint_as_float(cur[i]), v[i]);
+            else v[i] = __uint_as_float(cur[i]);
+          }
+          // the next chunk's load is under way while this one is worked on
+          if (c + 1 < CH) tmem_ld32_issue(base + (uint32_t)(b * BN + (c + 1) * 32), cur);
           epi.chunk(sp, col, v);
         }
+        tmem_wait(cur);
         release(b);
         ++local;
       }
       epi.end(sp);
     }
+    epi.finish(lane);
   }
   tc_fence_before();
   if constexpr (PAIR) cluster_sync_all();
   else __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
-    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * BN));
+    if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TMEM));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TMEM));
   }
 }
 
-template <int BN, bool PAIR, bool SPLIT, typename Epi>
+template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                                                           const __grid_constant__ Loop lp, const int64_t M, const int64_t N,
                                                           const __grid_constant__ typename Epi::Args args) {
   Epi epi(args);
-  run_tiles<BN, PAIR, SPLIT>(map_a, map_b, lp, M, N, epi);
+  run_tiles<BN, PAIR, SPLIT, TEAM>(map_a, map_b, lp, M, N, epi);
 }
 
 // ---------------------------------------------------------------------------------
@@ -377,26 +467,25 @@ struct Operand {
   int mn = 0;
 };
 
-// CTAs (pairs count twice) that can be resident at once, per kernel and device
-template <int BN, bool PAIR, bool SPLIT, typename Epi>
-static int resident_units() {
-  static int units[64] = {0};
+// Clusters (of `size` CTAs; 1: none) that can be resident at once, per kernel, size and device
+template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
+static int resident(int size) {
+  static int units[64][5] = {{0}};
   int dev = 0;
   cudaGetDevice(&dev);
-  const int slot = dev >= 0 && dev < 64 ? dev : 0;
-  if (units[slot] && slot == dev) return units[slot];
-  auto* fn = tile_kernel<BN, PAIR, SPLIT, Epi>;
-  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<BN, PAIR>::SMEM);
-  int n = num_sms();
-  if constexpr (PAIR) {
-    n = num_sms() / 2;
+  const bool known = dev >= 0 && dev < 64;
+  if (known && units[dev][size]) return units[dev][size];
+  auto* fn = tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>;
+  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<BN, PAIR, SPLIT>::SMEM);
+  int n = num_sms() / size;
+  if (size > 1) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * n), 1, 1);
+    cfg.gridDim = dim3((unsigned)(size * n), 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = Geo<BN, PAIR>::SMEM;
+    cfg.dynamicSmemBytes = Geo<BN, PAIR, SPLIT>::SMEM;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.x = (unsigned)size;
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cfg.attrs = &attr;
@@ -405,16 +494,16 @@ static int resident_units() {
     if (cudaOccupancyMaxActiveClusters(&k, fn, &cfg) == cudaSuccess && k > 0) n = std::min(n, k);
     else cudaGetLastError();
   }
-  units[slot] = n;
+  if (known) units[dev][size] = n;
   return n;
 }
 
 // C [batch][M, N] = A . B with operands of one 16-bit plane, or of two (SPLIT). Fills in the loop's tile counts and launches as many CTAs (or
 // pairs) as are resident, each walking its share of the tiles.
-template <int BN, bool PAIR, bool SPLIT, typename Epi>
+template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, Loop lp,
                      const typename Epi::Args& args, cudaStream_t s, const char* what) {
-  using G = Geo<BN, PAIR>;
+  using G = Geo<BN, PAIR, SPLIT>;
   constexpr int planes = SPLIT ? 2 : 1;
   CUtensorMap ma, mb;
   auto map = [&](CUtensorMap* m, const Operand& o, int64_t major, int box) {
@@ -428,7 +517,6 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   if (rc) return rc;
   lp.a_mn = A.mn;
   lp.b_mn = B.mn;
-  lp.nseg = planes > 1 ? 3 : 1;
   lp.nk = (int)ceil_div(K, BK);
   if (lp.splits < 1) lp.splits = 1;
   lp.nk_split = (int)ceil_div(lp.nk, lp.splits);
@@ -436,36 +524,64 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   lp.chunk = SPLIT ? CHUNK : lp.nk_split;
   lp.tiles_m = (int)ceil_div(M, G::TM);
   lp.tiles_n = (int)ceil_div(N, BN);
-  const int64_t per = lp.walk == WALK_TRIANGLE ? (int64_t)lp.tiles_n * (lp.tiles_n + 1) / 2 : (int64_t)lp.tiles_m * lp.tiles_n;
+  lp.wide = std::max(1, G::TM / BN);
+  const int64_t p = lp.tiles_n / lp.wide;  // whole groups of tile columns; a last one may be short
+  const int64_t per = lp.walk == WALK_TRIANGLE ? lp.wide * p * (p + 1) / 2 + lp.tiles_n % lp.wide * (p + 1)
+                                               : (int64_t)lp.tiles_m * lp.tiles_n;
   B200_REQUIRE(per * lp.splits * batch < (1ll << 30), "%s: too many tiles", what);
   lp.per_batch = (int)(per * lp.splits);
   lp.total = (int)(per * lp.splits * batch);
-  const int units = std::min(resident_units<BN, PAIR, SPLIT, Epi>(), lp.total);
-  if constexpr (PAIR) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(2 * units), 1, 1);
-    cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = G::SMEM;
-    cfg.stream = s;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = 2;
-    attr.val.clusterDim.y = 1;
-    attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    cudaLaunchKernelEx(&cfg, tile_kernel<BN, PAIR, SPLIT, Epi>, ma, mb, lp, M, N, args);
+  int size = PAIR ? 2 : 1, units;
+  if constexpr (TEAM) {
+    // one tile per team; 4 or 2 members where that many teams fit and each has 2 K blocks or more
+    size = 4;
+    while (size > 1 && (lp.nk < 2 * size || resident<BN, PAIR, SPLIT, TEAM, Epi>(size) < lp.total)) size /= 2;
+    if (size == 1) return -1;
+    lp.team = size;
+    lp.nk_split = (int)ceil_div(lp.nk, size);
+    if (!SPLIT) lp.chunk = lp.nk_split;
+    units = lp.total;
   } else {
-    tile_kernel<BN, PAIR, SPLIT, Epi><<<(unsigned)units, THREADS, G::SMEM, s>>>(ma, mb, lp, M, N, args);
+    units = std::min(resident<BN, PAIR, SPLIT, TEAM, Epi>(size), lp.total);
   }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(size * units), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = G::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)size;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = size > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&cfg, tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>, ma, mb, lp, M, N, args);
   return check_launch(what);
 }
 
-template <int BN, bool PAIR, typename Epi>
-static int launch(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, const Loop& lp,
+// Split operands: 256 x 128 tiles on pairs, 128 x 128 otherwise. Plain ones: 256 x 256 on
+// pairs, else 128 x 256 for more than 128 columns or 128 x 128, as far as the epilogue has
+// them; 128 x 128 tiles on teams where it has those and they fit.
+template <typename Epi>
+static int launch(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, bool pair, const Loop& lp,
                   const typename Epi::Args& args, cudaStream_t s, const char* what) {
-  return planes > 1 ? launch_as<BN, PAIR, true, Epi>(A, B, M, N, K, batch, lp, args, s, what)
-                    : launch_as<BN, PAIR, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+  if constexpr (Epi::TEAMS) {
+    if (!pair) {
+      const int rc = planes > 1 ? launch_as<128, false, true, true, Epi>(A, B, M, N, K, batch, lp, args, s, what)
+                                : launch_as<128, false, false, true, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+      if (rc >= 0) return rc;
+    }
+  }
+  if (planes > 1)
+    return pair ? launch_as<128, true, true, false, Epi>(A, B, M, N, K, batch, lp, args, s, what)
+                : launch_as<128, false, true, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+  if (pair) return launch_as<256, true, false, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+  if constexpr (Epi::SINGLE_WIDE) {
+    if (!Epi::SINGLE_NARROW || N > 128) return launch_as<256, false, false, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+  }
+  if constexpr (Epi::SINGLE_NARROW) return launch_as<128, false, false, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
+  return B200_ERR_UNSUPPORTED;
 }
 
 }  // namespace tile
