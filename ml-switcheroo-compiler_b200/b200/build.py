@@ -22,7 +22,11 @@ BUILD = os.path.join(ROOT, "_build")
 LIB = os.path.join(PKG, "libb200.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-rdc=true", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE, "-I", CSRC]
+FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC", "--expt-relaxed-constexpr", "-I", INCLUDE, "-I", CSRC]
+RDC = ["-rdc=true"]  # the device error flag of capi.cu is shared across files
+# compiled as whole programs, with an error flag of their own: ptxas ignores setmaxnreg under -rdc
+WHOLE = {"linear_xent.cu", "newton_schulz.cu"}
+WHOLE_FLAGS = ["-DB200_OWN_ERROR_FLAG"]
 
 
 def _nvcc() -> str:
@@ -42,7 +46,7 @@ def _digest() -> str:
         with open(p, "rb") as f:
             h.update(os.path.basename(p).encode())
             h.update(f.read())
-    h.update(" ".join(ARCH + FLAGS).encode())
+    h.update(" ".join(ARCH + FLAGS + RDC + sorted(WHOLE) + WHOLE_FLAGS).encode())
     return h.hexdigest()
 
 
@@ -57,7 +61,8 @@ def build(force: bool = False, verbose: bool = False) -> str:
 
     def compile_one(src: str) -> str:
         obj = os.path.join(BUILD, os.path.basename(src)[:-3] + ".o")
-        cmd = [nvcc, *ARCH, *FLAGS, "-c", src, "-o", obj]
+        mode = WHOLE_FLAGS if os.path.basename(src) in WHOLE else RDC
+        cmd = [nvcc, *ARCH, *FLAGS, *mode, "-c", src, "-o", obj]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
         r = subprocess.run(cmd, capture_output=True, text=True)

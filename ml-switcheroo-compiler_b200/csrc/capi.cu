@@ -2,6 +2,7 @@
 #include <stdarg.h>
 #include <atomic>
 #include <mutex>
+#include <vector>
 
 #include "common.cuh"
 
@@ -19,6 +20,16 @@ void set_error(const char* fmt, ...) {
 }
 
 void count_launch(uint64_t n) { g_launches.fetch_add(n, std::memory_order_relaxed); }
+
+// the device error flags of this file and of those compiled without -rdc
+static std::vector<const void*>& error_flags() {
+  static std::vector<const void*> flags = {&g_device_error};
+  return flags;
+}
+bool register_error_flag(const void* symbol) {
+  error_flags().push_back(symbol);
+  return true;
+}
 
 int check_launch(const char* what) {
   cudaError_t e = cudaGetLastError();
@@ -60,14 +71,19 @@ int b200_check_device_error(void* stream) {
     return B200_ERR_CUDA;
   }
   int code = 0;
-  e = cudaMemcpyFromSymbol(&code, b200::g_device_error, sizeof(int));
-  if (e != cudaSuccess) {
-    b200::set_error("read device error flag: %s", cudaGetErrorString(e));
-    return B200_ERR_CUDA;
+  for (const void* flag : b200::error_flags()) {
+    int here = 0;
+    e = cudaMemcpyFromSymbol(&here, flag, sizeof(int));
+    if (e != cudaSuccess) {
+      b200::set_error("read device error flag: %s", cudaGetErrorString(e));
+      return B200_ERR_CUDA;
+    }
+    if (here == 0) continue;
+    const int zero = 0;
+    cudaMemcpyToSymbol(flag, &zero, sizeof(int));
+    if (code == 0) code = here;
   }
   if (code != 0) {
-    int zero = 0;
-    cudaMemcpyToSymbol(b200::g_device_error, &zero, sizeof(int));
     b200::set_error("device-side check failed (code %d)", code);
     return code;
   }

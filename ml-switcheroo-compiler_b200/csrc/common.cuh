@@ -23,7 +23,15 @@ int check_launch(const char* what);
 
 // Device-side error flag (index out of range, bounded wait gave up). Written with
 // atomicCAS so the first error code wins; read and cleared by b200_check_device_error.
+// Files compiled as a whole program (without -rdc, see build.py) cannot share the variable:
+// each has its own, which register_error_flag adds to what b200_check_device_error reads.
+#ifdef B200_OWN_ERROR_FLAG
+static __device__ int g_device_error;
+bool register_error_flag(const void* symbol);
+static const bool g_error_flag_registered = register_error_flag(&g_device_error);
+#else
 extern __device__ int g_device_error;
+#endif
 __device__ __forceinline__ void raise_device_error(int code) { atomicCAS(&g_device_error, 0, code); }
 
 __device__ __forceinline__ float bf16_to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -7,7 +7,7 @@
 // Forward: one tcgen05 product whose epilogue keeps, per row and half tile, the
 // running maximum and the sum of exponentials of the accumulator (fp32, base 2), and the
 // label's logit; a second kernel joins a row's halves. z is never written: 8 bytes leave the
-// SM for a half tile's 128 logits (64 with fp32 operands).
+// SM for a half tile's 128 logits.
 // Backward: the vocabulary is walked in pieces. A piece's logits are made again (a fourth
 // product: the price of not keeping 4 bytes per token and word), its epilogue turns them
 // into d, written in the operands' precision to a workspace that one piece fills; the
@@ -390,7 +390,7 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
   if (needs_pack(dtype, x, ldx)) p.x = take(xb);
   if (needs_pack(dtype, w, ldw)) p.w = take((size_t)p.planes * p.w_rows * up8(p.w_cols) * 2);
   if (!grad) {
-    p.part = take((size_t)ceil_div(V, p.planes > 1 ? 128 : 256) * 2 * N * sizeof(float2));
+    p.part = take((size_t)ceil_div(V, p.planes > 1 && N <= 128 ? 128 : 256) * 2 * N * sizeof(float2));
     p.picked = take((size_t)N * 4);
   } else {
     p.width = piece_width(N, D, V, p.planes);
@@ -417,7 +417,7 @@ static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int
   const int splits = lp.splits;
   if (splits > 1) a = {split_ws, nullptr, N, N, M * N, M, N, 0};
   int rc;
-  rc = launch<StoreEpi>(A, B, M, N, K, 1, planes, M > 128 && (N > 128 || planes > 1), lp, a, s, what);
+  rc = launch<StoreEpi>(A, B, M, N, K, 1, planes, M > 128 && N > 128, lp, a, s, what);
   if (rc || splits == 1) return rc;
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(M * N, 256), (int64_t)num_sms() * 16);
   join_splits_kernel<<<grid, 256, 0, s>>>(split_ws, splits, M * N, N, add, C, bf16, ldc);
@@ -504,7 +504,7 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
   tile::Loop lp = {};
   lp.bf16 = 1;
   lp.group_m = 16;
-  const int width = p.planes > 1 ? 64 : 128;
+  const int width = p.planes > 1 && N <= 128 ? 64 : 128;  // fp32 operands on single CTAs: 128-wide tiles
   const lx::LseEpi::Args a = {part, width, picked, labels, i32, N, V};
   // a pair's 256 rows; one CTA's 128 when there are no more tokens than that
   rc = tile::launch<lx::LseEpi>(A, B, N, V, D, 1, p.planes, N > 128, lp, a, s, what);

@@ -151,7 +151,7 @@ struct NsEpi {
     // (row / 2) ^ (row / 8): rows written and read, and 8 x 8 blocks read transposed, are then free
     // of bank conflicts. Rows leave as 64 adjacent bytes each way.
     const int lane = sp.lane;
-    const bool mirror = a.mirror && sp.above;
+    const bool mirror = a.mirror && sp.mt != sp.nt;
     for (int k = 0; k < a.planes; ++k) {
       __half* d = a.dst + sp.z * a.batch + k * a.plane;
       const uint32_t buf = sp.buf + (uint32_t)(k & 1) * 2048u;
@@ -165,27 +165,32 @@ struct NsEpi {
         st_shared_v4(buf + (uint32_t)lane * 64u + (((uint32_t)j ^ f) << 4), w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
       __syncwarp();
       // 8 rows of 4 pieces at a time (rows are padded to 8 elements: whole pieces)
+      const int piece = lane & 3;
+      uint4 u[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int r = 8 * i + (lane >> 2), j = lane & 3;
-        const uint4 u = ld_shared_v4(buf + (uint32_t)r * 64u + (((uint32_t)j ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4));
-        if (r < rows && 8 * j < cols) *reinterpret_cast<uint4*>(d + (sp.row0 + r) * a.ld + col + 8 * j) = u;
+        const int r = 8 * i + (lane >> 2);
+        u[i] = ld_shared_v4(buf + (uint32_t)r * 64u + (((uint32_t)piece ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4));
       }
+      __half* row = d + (sp.row0 + (lane >> 2)) * a.ld + col + 8 * piece;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (8 * i + (lane >> 2) < rows && 8 * piece < cols) *reinterpret_cast<uint4*>(row + 8 * i * a.ld) = u[i];
       if (mirror) {
         // four 8 x 8 blocks transposed: block m's rows are 8 c/2 + 2 m + c%2 (c = 0..7), so that
         // thread l ends up with rows 8 (l % 4) .. + 7 of source column 8 g + l / 4
+        const int c = lane & 7, r = 8 * (c >> 1) + 2 * (lane >> 3) + (c & 1);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const int c = lane & 7, r = 8 * (c >> 1) + 2 * (lane >> 3) + (c & 1);
-          uint4 u;
+        for (int g = 0; g < 4; ++g)
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
-                       : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+                       : "=r"(u[g].x), "=r"(u[g].y), "=r"(u[g].z), "=r"(u[g].w)
                        : "r"(buf + (uint32_t)r * 64u + (((uint32_t)g ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4))
                        : "memory");
-          const int cc = 8 * g + (lane >> 2), j = lane & 3;
-          // the mirrored rows are as long as the result: whole pieces up to the padding
-          if (cc < cols && 8 * j < rows) *reinterpret_cast<uint4*>(d + (col + cc) * a.ld + sp.row0 + 8 * j) = u;
-        }
+        // the mirrored rows are as long as the result: whole pieces up to the padding
+        row = d + (col + (lane >> 2)) * a.ld + sp.row0 + 8 * piece;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          if (8 * g + (lane >> 2) < cols && 8 * piece < rows) *reinterpret_cast<uint4*>(row + 8 * g * a.ld) = u[g];
       }
       if (k + 1 < a.planes) {
 #pragma unroll
@@ -347,16 +352,16 @@ static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
   return q;
 }
 
-// One product, on CTA pairs when their tiles (256 x 256, or 256 x 128 of split operands) fill
-// two thirds of them, else on 128 x 128 tiles of single CTAs: a 1024 x 1024 product has 16 of
-// 256 x 256 (10 reach the diagonal) for 74 pairs, 64 (36) of 128 x 128 for 148 CTAs.
+// One product, on CTA pairs (256 x 256 tiles) when those fill two thirds of them, else on
+// 128 x 128 tiles of single CTAs or teams: a 1024 x 1024 product has 16 of the former (10 reach
+// the diagonal) for 74 pairs, 64 (36) of the latter for 148 CTAs.
 static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, bool triangle,
                    const NsEpi::Args& a, cudaStream_t s, const char* what) {
   Loop lp = {};
   lp.group_m = 16;
   lp.walk = triangle ? WALK_TRIANGLE : WALK_GROUPED;
-  const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, planes > 1 ? 128 : 256);
-  const int64_t tiles = (triangle ? tm * (tn + planes) / 2 : tm * tn) * batch;
+  const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, 256);
+  const int64_t tiles = (triangle ? tn * (tn + 1) / 2 : tm * tn) * batch;
   const bool pair = M > 128 && N > 128 && tiles * 3 >= num_sms();
   return launch<NsEpi>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
 }

@@ -7,22 +7,23 @@
 //    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is the fp32 product up to lo.lo: a third of the tensor rate
 //    instead of the CUDA cores'. The tensor cores cut (not round) each sum to fp32: up to
 //    2^-23 of it per 16 products, all towards zero, which over K = 50000 was 1e-4. So the
-//    hi.hi accumulator is drained every CHUNK K blocks (16 cuts) and added up in registers
-//    with rounding; the other two products are 2^-8 to 2^-11 of it and have an accumulator of
-//    their own for the whole tile;
+//    accumulator is drained every CHUNK K blocks and added up in registers with rounding (48
+//    cuts; 16 in the 128-wide tiles, where hi.lo + lo.hi, 2^-8 to 2^-11 of the whole, have an
+//    accumulator of their own);
 //  * the tiles are walked in groups of M tiles (their A rows stay in L2 while B streams
 //    past once per group), over the upper triangle of a symmetric result, or over splits of
 //    the K axis, each with its own partial result.
 //
 // Roles as in gemm_tc.cu: warp 0 issues TMA loads, warp 1 owns TMEM and issues the MMAs,
-// warps 2 to 9 (two per TMEM lane quarter) drain the double-buffered accumulator while the
+// warps 4 to 11 (two per TMEM lane quarter) drain the double-buffered accumulator while the
 // next MMAs run. PAIR: two CTAs of a cluster share a 256 x BN tile (cta_group::2), each
 // loading its 128 rows of A and half of B: a single CTA's 128 x 128 tile reads and writes
 // 64 KB of shared memory per K block, twice the time of its MMAs; a pair's 256 x 256 tile
 // half its MMAs' time.
-// Split operands take tiles 128 wide: a drained tile is 64 registers a thread (128 of the
-// 168 there are would spill), and 120 KB of shared-memory traffic per K block cost 940
-// clocks beside 786 of MMAs.
+// What bounds split operands is the L2 (9 to 11 TB/s): a 256 x 128 tile reads 98 KB a K block
+// for 786 clocks of MMAs and took 1480, a 256 x 256 tile 131 KB for 1572. Its drained
+// accumulator is 128 registers a thread of the epilogue, so the two warpgroups there take over
+// most of the first one's (setmaxnreg; ptxas honours it only in files compiled without -rdc).
 // TEAM: where single tiles would leave most SMs idle, a cluster of 2 or 4 CTAs shares one
 // tile's K axis; each then sends its partial sums of the columns that another one owns
 // through shared memory (in place of the operands, all read by then) and finishes its own.
@@ -38,18 +39,24 @@ namespace tile {
 
 using namespace tc;
 
-constexpr int BM = 128, BK = 64, EPI_WARPS = 8, EPI_FIRST = 2, THREADS = 32 * (EPI_FIRST + EPI_WARPS);
+constexpr int BM = 128, BK = 64, EPI_WARPS = 8, EPI_FIRST = 4, THREADS = 32 * (EPI_FIRST + EPI_WARPS);
+// registers a thread: at launch, then in the first warpgroup and in the epilogue's two; a sum
+// beyond what the launch gave would wait forever (checked here and before the launch)
+constexpr int REGS = 168, REGS_ISSUE = 56, REGS_EPI = 224, REGS_SUM = 128 * REGS_ISSUE + 256 * REGS_EPI;
+static_assert(REGS_SUM <= THREADS * REGS, "setmaxnreg beyond the launch's registers");
 constexpr uint32_t EPI_BUF = 4096;  // staging bytes per epilogue warp
 constexpr uint32_t LEADER = 0xFEFFFFFFu;  // shared-memory address mask of a pair's CTA 0
 
 template <int BN, bool PAIR, bool SPLIT>
 struct Geo {
   static constexpr int PLANES = SPLIT ? 2 : 1;
-  static_assert(!SPLIT || BN == 128, "split operands: 128-wide tiles");
-  static constexpr int STAGES = SPLIT ? (PAIR ? 4 : 3) : (BN == 256 && !PAIR ? 4 : 6);
+  static constexpr bool LEND = SPLIT && BN == 256;   // the epilogue needs the first warpgroup's registers
+  static constexpr bool APART = SPLIT && BN == 128;  // the small products' accumulators fit beside the others
+  static_assert(!LEND || PAIR, "256-wide split tiles are for pairs");
+  static constexpr int STAGES = SPLIT ? 3 : (BN == 256 && !PAIR ? 4 : 6);
   static constexpr int TM = PAIR ? 2 * BM : BM;
   static constexpr uint32_t A_BYTES = BM * BK * 2, B_BYTES = (PAIR ? BN / 2 : BN) * BK * 2;
-  static constexpr uint32_t TMEM = (SPLIT ? 4 : 2) * BN;  // columns: two accumulators, and two for the small products
+  static constexpr uint32_t TMEM = (APART ? 4 : 2) * BN;  // columns
   static constexpr uint32_t STAGE = PLANES * (A_BYTES + B_BYTES);
   static constexpr size_t SMEM = (size_t)STAGES * STAGE + EPI_WARPS * EPI_BUF + 1024 + 256;
   static_assert(SMEM <= 232448, "operand ring and staging must fit 227 KB");
@@ -63,7 +70,7 @@ struct Loop {
   int nk_split;  // K blocks per split (= nk without splits)
   int chunk;     // K blocks that one accumulator takes before it is drained
   int a_mn, b_mn, bf16;
-  int tiles_m, tiles_n, group_m, walk, wide;
+  int tiles_m, tiles_n, group_m, walk;
   int per_batch, total;  // tiles of one batch entry (splits included), of all
   int splits;
   int team;      // CTAs of a cluster that share a tile's K axis (TEAM)
@@ -81,15 +88,12 @@ __device__ __forceinline__ Tile tile_at(const Loop& lp, int t) {
   r.split = i / per_split;
   i %= per_split;
   if (lp.walk == WALK_TRIANGLE) {
-    // tiles that reach the diagonal or lie above it, column by column: with `wide` tile
-    // columns to a tile row, columns wide p .. wide p + wide - 1 have rows 0 .. p
-    const int w = lp.wide;
-    int p = (int)((sqrtf(8.f * (float)i / (float)w + 1.f) - 1.f) * 0.5f);
-    while (w * (p + 1) * (p + 2) / 2 <= i) ++p;
-    while (w * p * (p + 1) / 2 > i) --p;
-    i -= w * p * (p + 1) / 2;
-    r.nt = w * p + i / (p + 1);
-    r.mt = i % (p + 1);
+    // square tiles on and above the diagonal: i = nt (nt + 1) / 2 + mt, mt <= nt
+    int nt = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
+    while ((nt + 1) * (nt + 2) / 2 <= i) ++nt;
+    while (nt * (nt + 1) / 2 > i) --nt;
+    r.nt = nt;
+    r.mt = i - nt * (nt + 1) / 2;
     return r;
   }
   const int per_group = lp.group_m * lp.tiles_n;
@@ -149,7 +153,6 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
 struct Spot {
   int64_t row, row0, col0;  // col0: first of this warp's columns
   int z, split, mt, nt, half, lane;
-  bool above;  // the whole tile lies above the diagonal
   uint32_t buf;
 };
 
@@ -177,6 +180,8 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
   const int unit = (int)blockIdx.x / per_unit, units = (int)gridDim.x / per_unit;
 
   if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
     for (int s = 0; s < STG; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
@@ -201,8 +206,13 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
   else __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // The next kernel of the stream may start its own set-up now; this one has waited for the
+  // kernels before it from here on (it reads and writes no global memory earlier).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   if (warp < EPI_FIRST) {
+    if constexpr (G::LEND) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
@@ -274,10 +284,10 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
             const uint32_t a0 = smem_u32(smem + s * G::STAGE), b0 = a0 + G::PLANES * G::A_BYTES;
 #pragma unroll
             for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
-              // hi.lo and lo.hi into the tile's accumulator of small products, hi.hi into the chunk's
+              // hi.lo and lo.hi into the tile's accumulator of small products (APART), hi.hi into the chunk's
               const uint32_t as = a0 + (SPLIT && seg == 1 ? G::A_BYTES : 0u), bs = b0 + (SPLIT && seg == 0 ? G::B_BYTES : 0u);
-              const uint32_t to = seg < 2 ? tmem + (uint32_t)((2 + (tiles & 1)) * BN) : d;
-              const bool fresh = seg == 0 ? kb == kb0 : (seg == 2 && kb == c0);
+              const uint32_t to = G::APART && seg < 2 ? tmem + (uint32_t)((2 + (tiles & 1)) * BN) : d;
+              const bool fresh = G::APART ? (seg == 0 ? kb == kb0 : (seg == 2 && kb == c0)) : (seg == (SPLIT ? 0 : 2) && kb == c0);
 #pragma unroll
               for (int k = 0; k < BK / 16; ++k) {
                 const uint64_t ad = lp.a_mn ? smem_desc(as + k * 2048, 8192, 1024) : smem_desc(as + k * 32, 16, 1024);
@@ -296,6 +306,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       cluster_sync_all();
     }
   } else {
+    if constexpr (G::LEND) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_EPI));
     Spot sp;
     const int q = warp & 3;
     sp.half = (warp - EPI_FIRST) >> 2;
@@ -323,7 +334,6 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       sp.row0 = (int64_t)at.mt * G::TM + (int64_t)rank * BM + q * 32;
       sp.row = sp.row0 + lane;
       const int64_t col0 = sp.col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
-      sp.above = (int64_t)at.nt * BN >= (int64_t)(at.mt + 1) * G::TM;
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
       epi.begin(sp);
       // the member that finishes chunk c of this warp
@@ -358,7 +368,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             add((uint32_t)(b * BN + c * 32), acc[c]);
-            if (SPLIT && c0 + lp.chunk >= kb1) add((uint32_t)((2 + (tiles & 1)) * BN + c * 32), acc[c]);
+            if (G::APART && c0 + lp.chunk >= kb1) add((uint32_t)((2 + (tiles & 1)) * BN + c * 32), acc[c]);
           }
           release(b);
         }
@@ -401,8 +411,10 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c) {
           if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.chunk(sp, col0 + c * 32, acc[c]);  // warp-uniform
+          asm volatile("" ::: "memory");  // one chunk at a time: the others wait in registers
+        }
       } else {
         const int b = local & 1;
         if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) break;
@@ -467,7 +479,8 @@ struct Operand {
   int mn = 0;
 };
 
-// Clusters (of `size` CTAs; 1: none) that can be resident at once, per kernel, size and device
+// Clusters (of `size` CTAs; 1: none) that can be resident at once, per kernel, size and device;
+// 0 where the kernel was compiled to fewer registers than its warpgroups trade
 template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 static int resident(int size) {
   static int units[64][5] = {{0}};
@@ -476,6 +489,10 @@ static int resident(int size) {
   const bool known = dev >= 0 && dev < 64;
   if (known && units[dev][size]) return units[dev][size];
   auto* fn = tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>;
+  if constexpr (Geo<BN, PAIR, SPLIT>::LEND) {
+    cudaFuncAttributes at;
+    if (cudaFuncGetAttributes(&at, fn) != cudaSuccess || at.numRegs * THREADS < REGS_SUM) return 0;
+  }
   cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<BN, PAIR, SPLIT>::SMEM);
   int n = num_sms() / size;
   if (size > 1) {
@@ -524,10 +541,7 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   lp.chunk = SPLIT ? CHUNK : lp.nk_split;
   lp.tiles_m = (int)ceil_div(M, G::TM);
   lp.tiles_n = (int)ceil_div(N, BN);
-  lp.wide = std::max(1, G::TM / BN);
-  const int64_t p = lp.tiles_n / lp.wide;  // whole groups of tile columns; a last one may be short
-  const int64_t per = lp.walk == WALK_TRIANGLE ? lp.wide * p * (p + 1) / 2 + lp.tiles_n % lp.wide * (p + 1)
-                                               : (int64_t)lp.tiles_m * lp.tiles_n;
+  const int64_t per = lp.walk == WALK_TRIANGLE ? (int64_t)lp.tiles_n * (lp.tiles_n + 1) / 2 : (int64_t)lp.tiles_m * lp.tiles_n;
   B200_REQUIRE(per * lp.splits * batch < (1ll << 30), "%s: too many tiles", what);
   lp.per_batch = (int)(per * lp.splits);
   lp.total = (int)(per * lp.splits * batch);
@@ -544,25 +558,31 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   } else {
     units = std::min(resident<BN, PAIR, SPLIT, TEAM, Epi>(size), lp.total);
   }
+  if (units < 1) {
+    set_error("%s: the kernel cannot be resident (registers)", what);
+    return B200_ERR_CUDA;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(size * units), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = G::SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)size;
-  attr.val.clusterDim.y = 1;
-  attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = size > 1 ? 1 : 0;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)size;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = size > 1 ? 2 : 1;
   cudaLaunchKernelEx(&cfg, tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>, ma, mb, lp, M, N, args);
   return check_launch(what);
 }
 
-// Split operands: 256 x 128 tiles on pairs, 128 x 128 otherwise. Plain ones: 256 x 256 on
-// pairs, else 128 x 256 for more than 128 columns or 128 x 128, as far as the epilogue has
-// them; 128 x 128 tiles on teams where it has those and they fit.
+// 256 x 256 tiles on pairs; else 128 x 128 of split operands, and of plain ones 128 x 256 for
+// more than 128 columns or 128 x 128, as far as the epilogue has them; 128 x 128 tiles on teams
+// where it has those and they fit.
 template <typename Epi>
 static int launch(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, bool pair, const Loop& lp,
                   const typename Epi::Args& args, cudaStream_t s, const char* what) {
@@ -574,7 +594,7 @@ static int launch(const Operand& A, const Operand& B, int64_t M, int64_t N, int6
     }
   }
   if (planes > 1)
-    return pair ? launch_as<128, true, true, false, Epi>(A, B, M, N, K, batch, lp, args, s, what)
+    return pair ? launch_as<256, true, true, false, Epi>(A, B, M, N, K, batch, lp, args, s, what)
                 : launch_as<128, false, true, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
   if (pair) return launch_as<256, true, false, false, Epi>(A, B, M, N, K, batch, lp, args, s, what);
   if constexpr (Epi::SINGLE_WIDE) {
