@@ -11,8 +11,10 @@
 //
 // Angles. w_j comes as a fraction of a turn per position in 64-bit fixed point, so
 // position * w_j modulo one turn is one wrapping integer product: exact for any position
-// (an fp32 product would be off by 0.06 rad at position 10^6). Its top 32 bits go through
-// sincospif. The table travels in the kernel's parameters: nothing is uploaded or kept.
+// (an fp32 product would be off by 0.06 rad at position 10^6). The nearest quarter turn is
+// taken off in integers, what is left (within pi / 4) goes through the Taylor polynomials of
+// sine (to x^9) and cosine (to x^10), off by less than 2^-28 there. The table travels in the
+// kernel's parameters: nothing is uploaded or kept.
 //
 // Layout of the work. A lane owns one unit of a head: two vectors of V = 4 elements that
 // hold whole pairs (the two halves of V pairs, or 2V neighbours), so a rotation needs no
@@ -23,7 +25,9 @@
 // heads of one token run on many warps; each then makes the angles again.
 // Bound by HBM: x (and dy) are read once, y (dx) written once. BATCH groups of heads are
 // loaded before any is worked on: with 8 to 16 bytes a lane and vector the SM's warps have
-// to have 50 KB or more under way.
+// to have 50 KB or more under way. The issue slots come next: elements are worked on two at a
+// time (f32x2 products), the weights are folded into the rotation's coefficients
+// (y = rstd (x k1 + partner k2)), and row pointers advance by additions.
 #include <algorithm>
 
 #include "common.cuh"
@@ -57,33 +61,81 @@ struct Args {
   uint64_t freq[B200_ROTARY_MAX_DIM / 2];
 };
 
-// V elements as loaded: 32-bit words of one vector access (FAST; n is 0 or V), or one by one
+// ---- two fp32 values in a 64-bit register pair ----
+typedef uint64_t f2;
+__device__ __forceinline__ f2 pair(float a, float b) {
+  f2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void halves(f2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f2 swapped(f2 v) {
+  float a, b;
+  halves(v, a, b);
+  return pair(b, a);
+}
+__device__ __forceinline__ f2 mul2(f2 a, f2 b) {
+  f2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f2 fma2(f2 a, f2 b, f2 c) {
+  f2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float sum2(f2 v) {
+  float a, b;
+  halves(v, a, b);
+  return a + b;
+}
+
+// cosine and sine of phase / 2^64 of a turn
+__device__ __forceinline__ void cos_sin(uint64_t phase, float& c, float& s) {
+  const uint32_t top = (uint32_t)(phase >> 32);
+  const uint32_t quarter = (top + 0x20000000u) >> 30;        // the nearest quarter turn
+  const float x = (float)(int32_t)(top - (quarter << 30)) * 1.4629180792671596e-9f;  // 2 pi 2^-32: within pi / 4
+  const float q = x * x;
+  float sn = fmaf(q, 2.7557319223985893e-6f, -1.984126984126984e-4f);
+  sn = fmaf(q, sn, 8.333333333333333e-3f);
+  sn = fmaf(q, sn, -1.6666666666666666e-1f);
+  sn = fmaf(q * sn, x, x);
+  float cs = fmaf(q, -2.755731922398589e-7f, 2.48015873015873e-5f);
+  cs = fmaf(q, cs, -1.388888888888889e-3f);
+  cs = fmaf(q, cs, 4.1666666666666664e-2f);
+  cs = fmaf(q, cs, -0.5f);
+  cs = fmaf(q, cs, 1.f);
+  const float u = quarter & 1 ? sn : cs, v = quarter & 1 ? cs : sn;
+  c = __uint_as_float(__float_as_uint(u) ^ (((quarter + 1) & 2) << 30));
+  s = __uint_as_float(__float_as_uint(v) ^ ((quarter & 2) << 30));
+}
+
+// V elements as loaded: the words of one vector access (FAST; all there or none), or floats
 template <typename T, int V, bool FAST>
 struct Vec {
   static constexpr int WORDS = FAST ? V * (int)sizeof(T) / 4 : V;
   uint32_t w[WORDS];
 
   __device__ __forceinline__ void load(const T* p, int n) {
-    if constexpr (FAST) {
 #pragma unroll
-      for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-      if (n) {
-        if constexpr (WORDS == 4) {
-          const uint4 u = *reinterpret_cast<const uint4*>(p);
-          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-        } else {
-          const uint2 u = *reinterpret_cast<const uint2*>(p);
-          w[0] = u.x, w[1] = u.y;
-        }
+    for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+    if constexpr (!FAST) {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < n) w[i] = __float_as_uint((float)p[i]);
+    } else if (n) {
+      if constexpr (WORDS == 4) {
+        const uint4 u = *reinterpret_cast<const uint4*>(p);
+        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+      } else {
+        const uint2 u = *reinterpret_cast<const uint2*>(p);
+        w[0] = u.x, w[1] = u.y;
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = i < n ? __float_as_uint((float)p[i]) : 0u;
     }
   }
-  __device__ __forceinline__ float get(int i) const {
-    if constexpr (FAST && sizeof(T) == 2) return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-    else return __uint_as_float(w[i]);
+  __device__ __forceinline__ f2 get(int i) const {  // elements 2 i and 2 i + 1
+    if constexpr (FAST && sizeof(T) == 2) return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    else return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   }
 };
 
@@ -91,16 +143,19 @@ __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 template <typename T, int V, bool FAST>
-__device__ __forceinline__ void store_vec(T* p, const float (&x)[V], int n) {
+__device__ __forceinline__ void store_vec(T* p, const f2 (&x)[V / 2], int n) {
+  float v[V];
+#pragma unroll
+  for (int i = 0; i < V / 2; ++i) halves(x[i], v[2 * i], v[2 * i + 1]);
   if constexpr (!FAST) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) put(p + i, x[i]);
+      if (i < n) put(p + i, v[i]);
   } else if (n) {
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
     } else {
-      const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
       *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
     }
   }
@@ -111,35 +166,21 @@ struct Row {
   Vec<T, V, FAST> a[NU], b[NU];
 };
 
-// rotate the V pairs of a unit; s carries the direction's sign
-template <int V, bool INTER>
-__device__ __forceinline__ void turn(float (&a)[V], float (&b)[V], const float (&c)[V], const float (&s)[V]) {
-  if constexpr (INTER) {
-#pragma unroll
-    for (int i = 0; i < V / 2; ++i) {
-      float x = a[2 * i], y = a[2 * i + 1];
-      a[2 * i] = x * c[i] - y * s[i];
-      a[2 * i + 1] = y * c[i] + x * s[i];
-      x = b[2 * i], y = b[2 * i + 1];
-      b[2 * i] = x * c[V / 2 + i] - y * s[V / 2 + i];
-      b[2 * i + 1] = y * c[V / 2 + i] + x * s[V / 2 + i];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float x = a[i], y = b[i];
-      a[i] = x * c[i] - y * s[i];
-      b[i] = y * c[i] + x * s[i];
-    }
-  }
-}
-
 template <typename T, int V, int NU, bool FAST, bool INTER, int MODE>
 __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kernel(const __grid_constant__ Args A) {
   constexpr int BATCH = NU > 1 ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
+  constexpr int P = V / 2;  // f32x2 values per vector
   __shared__ uint64_t freq[B200_ROTARY_MAX_DIM / 2];
   const int half = A.part / 2;
+  __shared__ float gamma[MODE == ROTATE ? 1 : 2][MODE == ROTATE ? 1 : B200_ROTARY_MAX_DIM];
   for (int i = threadIdx.x; i < half; i += THREADS) freq[i] = A.freq[i];
+  if constexpr (MODE != ROTATE) {
+    const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
+    for (int i = threadIdx.x; i < 2 * A.dim; i += THREADS) {
+      const int t = i >= A.dim, d = i - t * A.dim;
+      gamma[t][d] = A.seg[t].gamma ? load_as_f32(A.seg[t].gamma, d, dt) : 1.f;
+    }
+  }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int L = A.L, sub = lane / L, u0 = lane % L, R = 32 / L;
@@ -163,155 +204,209 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
       n1[k] = u < A.n_units ? max(0, min(V, end - o1[k])) : 0;
     }
   }
-  float gam[2][2][NU][V];  // [tensor][vector][unit][element]
-  float acc[2][2][NU][V];  // sums of g u
+  f2 acc[2][2][NU][P];  // [tensor][vector][unit][elements]: sums of g u
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int k = 0; k < NU; ++k)
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        acc[t][0][k][i] = acc[t][1][k][i] = 0.f;
-        gam[t][0][k][i] = gam[t][1][k][i] = 1.f;
-        if (MODE != ROTATE && A.seg[t].gamma) {
-          const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
-          if (i < n0[k]) gam[t][0][k][i] = load_as_f32(A.seg[t].gamma, o0[k] + i, dt);
-          if (i < n1[k]) gam[t][1][k][i] = load_as_f32(A.seg[t].gamma, o1[k] + i, dt);
-        }
-      }
+      for (int i = 0; i < P; ++i) acc[t][0][k][i] = acc[t][1][k][i] = 0;
   const float inv_dim = 1.f / (float)A.dim;
   const int total_groups = A.seg[0].groups + A.seg[1].groups;
   const int64_t items = (int64_t)A.tokens * A.chunks;
   for (int64_t item = (int64_t)blockIdx.x * WARPS + warp; item < items; item += (int64_t)gridDim.x * WARPS) {
-    const int token = (int)(item / A.chunks), chunk = (int)(item % A.chunks);
-    const int bt = token / A.seq, st = token % A.seq;
+    const int token = A.chunks == 1 ? (int)item : (int)(item / A.chunks), chunk = (int)(item - (int64_t)token * A.chunks);
+    const int bt = token / A.seq, st = token - bt * A.seq;
     const int g_begin = chunk * A.per_chunk, g_end = min(total_groups, g_begin + A.per_chunk);
     Row<T, V, NU, FAST> xr[BATCH], dr[BATCH];
-    // BATCH groups of heads of one tensor, from group g on
-    auto fetch = [&](const Seg& S, int g, int hi) {
-      const T* xb = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s;
-      const T* db = reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s;
+    const T *xp = nullptr, *dp = nullptr;  // this lane's head of the next group to load
+    int head = 0;
+    // the pointers of one tensor from group g on
+    auto point = [&](const Seg& S, int g) {
+      head = g * R + sub;
+      xp = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s + head * S.x_h;
+      if constexpr (MODE == NORM_GRAD) dp = reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s + head * S.d_h;
+    };
+    // BATCH groups of heads; `end`: the heads that this warp has to do end before it
+    auto fetch = [&](const Seg& S, int end) {
 #pragma unroll
       for (int j = 0; j < BATCH; ++j) {
-        const int h = (g + j) * R + sub;
-        const bool in = g + j < hi && h < S.heads;
+        const bool in = head < end;
 #pragma unroll
         for (int k = 0; k < NU; ++k) {
-          xr[j].a[k].load(xb + h * S.x_h + o0[k], in ? n0[k] : 0);
-          xr[j].b[k].load(xb + h * S.x_h + o1[k], in ? n1[k] : 0);
+          xr[j].a[k].load(xp + o0[k], in ? n0[k] : 0);
+          xr[j].b[k].load(xp + o1[k], in ? n1[k] : 0);
           if constexpr (MODE == NORM_GRAD) {
-            dr[j].a[k].load(db + h * S.d_h + o0[k], in ? n0[k] : 0);
-            dr[j].b[k].load(db + h * S.d_h + o1[k], in ? n1[k] : 0);
+            dr[j].a[k].load(dp + o0[k], in ? n0[k] : 0);
+            dr[j].b[k].load(dp + o1[k], in ? n1[k] : 0);
           }
         }
+        head += R;
+        xp += R * S.x_h;
+        if constexpr (MODE == NORM_GRAD) dp += R * S.d_h;
       }
     };
     const int t_first = g_begin < A.seg[0].groups ? 0 : 1;
     {
       const Seg& S = A.seg[t_first];
       const int first = t_first ? A.seg[0].groups : 0;
-      fetch(S, g_begin - first, min(S.groups, g_end - first));
+      point(S, g_begin - first);
+      fetch(S, min(S.heads, (g_end - first) * R));
     }
     int64_t p = A.offset + st;
     if (A.pos) {
       const int64_t i = bt * A.pos_b + st * A.pos_s;
       p = A.pos_i32 ? (int64_t) reinterpret_cast<const int*>(A.pos)[i] : reinterpret_cast<const long long*>(A.pos)[i];
     }
-    float c[NU][V], s[NU][V];
+    // y = x k1 + partner k2, the partner being the other vector, or each pair's other element
+    f2 k1[2][NU][P], k2[2][NU][P];
 #pragma unroll
-    for (int k = 0; k < NU; ++k)
+    for (int k = 0; k < NU; ++k) {
+      float c[V], s[V];
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        c[k][i] = 1.f;
-        s[k][i] = 0.f;
+        c[i] = 1.f;
+        s[i] = 0.f;
         if (rot[k] && f0[k] + i < half) {
-          const uint64_t phase = (uint64_t)p * freq[f0[k] + i];
-          sincospif((float)(int)(phase >> 32) * 4.656612873077393e-10f /* 2^-31 */, &s[k][i], &c[k][i]);
-          c[k][i] *= A.factor;
-          s[k][i] *= A.factor * A.sign;
+          cos_sin((uint64_t)p * freq[f0[k] + i], c[i], s[i]);
+          c[i] *= A.factor;
+          s[i] *= A.factor * A.sign;
         }
       }
+#pragma unroll
+      for (int i = 0; i < P; ++i) {
+        if constexpr (INTER) {
+          k1[0][k][i] = pair(c[i], c[i]);
+          k2[0][k][i] = pair(-s[i], s[i]);
+          k1[1][k][i] = pair(c[P + i], c[P + i]);
+          k2[1][k][i] = pair(-s[P + i], s[P + i]);
+        } else {
+          k1[0][k][i] = k1[1][k][i] = pair(c[2 * i], c[2 * i + 1]);
+          k2[0][k][i] = pair(-s[2 * i], -s[2 * i + 1]);
+          k2[1][k][i] = pair(s[2 * i], s[2 * i + 1]);
+        }
+      }
+    }
+    auto turn = [&](f2 (&a)[NU][P], f2 (&b)[NU][P], const f2 (&m1)[2][NU][P], const f2 (&m2)[2][NU][P]) {
+#pragma unroll
+      for (int k = 0; k < NU; ++k)
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+          const f2 x = a[k][i], y = b[k][i];
+          a[k][i] = mul2(x, m1[0][k][i]);
+          b[k][i] = mul2(y, m1[1][k][i]);
+          if (rot[k]) {  // elements that only pass see nothing of a partner
+            a[k][i] = fma2(INTER ? swapped(x) : y, m2[0][k][i], a[k][i]);
+            b[k][i] = fma2(INTER ? swapped(y) : x, m2[1][k][i], b[k][i]);
+          }
+        }
+    };
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const Seg& S = A.seg[t];
       const int first = t == 0 ? 0 : A.seg[0].groups;
       const int lo = max(0, g_begin - first), hi = min(S.groups, g_end - first);
-      T* yb = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s;
+      if (lo >= hi) continue;
+      const int end = min(S.heads, hi * R);
+      f2 gam[2][NU][P], w1[2][NU][P], w2[2][NU][P];  // the weights; the coefficients with them
+      if constexpr (MODE != ROTATE) {
+#pragma unroll
+        for (int k = 0; k < NU; ++k)
+#pragma unroll
+          for (int i = 0; i < P; ++i) {
+            float g[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              g[e] = 2 * i + e < n0[k] ? gamma[t][o0[k] + 2 * i + e] : 1.f;
+              g[2 + e] = 2 * i + e < n1[k] ? gamma[t][o1[k] + 2 * i + e] : 1.f;
+            }
+            const f2 ga = gam[0][k][i] = pair(g[0], g[1]), gb = gam[1][k][i] = pair(g[2], g[3]);
+            if constexpr (MODE == NORM) {
+              w1[0][k][i] = mul2(k1[0][k][i], ga);
+              w1[1][k][i] = mul2(k1[1][k][i], gb);
+              w2[0][k][i] = mul2(k2[0][k][i], INTER ? swapped(ga) : gb);
+              w2[1][k][i] = mul2(k2[1][k][i], INTER ? swapped(gb) : ga);
+            }
+          }
+      }
+      if (t != t_first) point(S, lo);
+      int out = lo * R + sub;
+      T* yp = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s + out * S.y_h;
       for (int g = lo; g < hi; g += BATCH) {
-        if (t != t_first || g != lo) fetch(S, g, hi);
+        if (t != t_first || g != lo) fetch(S, end);
 #pragma unroll
         for (int j = 0; j < BATCH; ++j) {
           if (g + j >= hi) break;  // warp-uniform
-          const int h = (g + j) * R + sub;
-          float a[NU][V], b[NU][V];
+          f2 a[NU][P], b[NU][P];
+          f2 ss = 0;
 #pragma unroll
           for (int k = 0; k < NU; ++k)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
+            for (int i = 0; i < P; ++i) {
               a[k][i] = xr[j].a[k].get(i);
               b[k][i] = xr[j].b[k].get(i);
+              if constexpr (MODE != ROTATE) ss = fma2(a[k][i], a[k][i], fma2(b[k][i], b[k][i], ss));
             }
-          if constexpr (MODE == NORM) {
-            float ss = 0.f;
+          if constexpr (MODE == ROTATE) {
+            turn(a, b, k1, k2);
+          } else if constexpr (MODE == NORM) {
+            float sq = sum2(ss);
+            for (int o = L >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+            const float rstd = rsqrtf(sq * inv_dim + A.eps);
+            const f2 r2 = pair(rstd, rstd);
+            turn(a, b, w1, w2);
 #pragma unroll
             for (int k = 0; k < NU; ++k)
 #pragma unroll
-              for (int i = 0; i < V; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
-            for (int o = L >> 1; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float rstd = rsqrtf(ss * inv_dim + A.eps);
-#pragma unroll
-            for (int k = 0; k < NU; ++k)
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                a[k][i] *= rstd * gam[t][0][k][i];
-                b[k][i] *= rstd * gam[t][1][k][i];
+              for (int i = 0; i < P; ++i) {
+                a[k][i] = mul2(a[k][i], r2);
+                b[k][i] = mul2(b[k][i], r2);
               }
-          }
-          if constexpr (MODE != NORM_GRAD) {
+          } else {
+            f2 ga[NU][P], gb[NU][P];
 #pragma unroll
             for (int k = 0; k < NU; ++k)
-              if (rot[k]) turn<V, INTER>(a[k], b[k], c[k], s[k]);
-          } else {
-            float ga[NU][V], gb[NU][V];
-            float ss = 0.f, hx = 0.f;
 #pragma unroll
-            for (int k = 0; k < NU; ++k) {
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
+              for (int i = 0; i < P; ++i) {
                 ga[k][i] = dr[j].a[k].get(i);
                 gb[k][i] = dr[j].b[k].get(i);
               }
-              if (rot[k]) turn<V, INTER>(ga[k], gb[k], c[k], s[k]);
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
-                hx = fmaf(ga[k][i] * gam[t][0][k][i], a[k][i], fmaf(gb[k][i] * gam[t][1][k][i], b[k][i], hx));
-              }
-            }
-            for (int o = L >> 1; o > 0; o >>= 1) {
-              ss += __shfl_xor_sync(0xffffffffu, ss, o);
-              hx += __shfl_xor_sync(0xffffffffu, hx, o);
-            }
-            const float rstd = rsqrtf(ss * inv_dim + A.eps);
-            const float m = hx * inv_dim * rstd * rstd;  // mean(h u) / (u / x)
+            turn(ga, gb, k1, k2);
+            f2 hh = 0;
 #pragma unroll
             for (int k = 0; k < NU; ++k)
 #pragma unroll
-              for (int i = 0; i < V; ++i) {
-                acc[t][0][k][i] = fmaf(ga[k][i], a[k][i] * rstd, acc[t][0][k][i]);
-                acc[t][1][k][i] = fmaf(gb[k][i], b[k][i] * rstd, acc[t][1][k][i]);
-                a[k][i] = rstd * (ga[k][i] * gam[t][0][k][i] - a[k][i] * m);
-                b[k][i] = rstd * (gb[k][i] * gam[t][1][k][i] - b[k][i] * m);
+              for (int i = 0; i < P; ++i)
+                hh = fma2(mul2(ga[k][i], gam[0][k][i]), a[k][i], fma2(mul2(gb[k][i], gam[1][k][i]), b[k][i], hh));
+            float sq = sum2(ss), hx = sum2(hh);
+            for (int o = L >> 1; o > 0; o >>= 1) {
+              sq += __shfl_xor_sync(0xffffffffu, sq, o);
+              hx += __shfl_xor_sync(0xffffffffu, hx, o);
+            }
+            const float rstd = rsqrtf(sq * inv_dim + A.eps);
+            const float m = -hx * inv_dim * rstd * rstd * rstd;  // -rstd mean(h u) / (u / x)
+            const f2 r2 = pair(rstd, rstd), m2 = pair(m, m);
+#pragma unroll
+            for (int k = 0; k < NU; ++k)
+#pragma unroll
+              for (int i = 0; i < P; ++i) {
+                ga[k][i] = mul2(ga[k][i], r2);  // rstd g
+                gb[k][i] = mul2(gb[k][i], r2);
+                acc[t][0][k][i] = fma2(ga[k][i], a[k][i], acc[t][0][k][i]);
+                acc[t][1][k][i] = fma2(gb[k][i], b[k][i], acc[t][1][k][i]);
+                a[k][i] = fma2(ga[k][i], gam[0][k][i], mul2(a[k][i], m2));
+                b[k][i] = fma2(gb[k][i], gam[1][k][i], mul2(b[k][i], m2));
               }
           }
-          if (h < S.heads) {
-            T* q = yb + h * S.y_h;
+          if (out < end) {
 #pragma unroll
             for (int k = 0; k < NU; ++k) {
-              store_vec<T, V, FAST>(q + o0[k], a[k], n0[k]);
-              store_vec<T, V, FAST>(q + o1[k], b[k], n1[k]);
+              store_vec<T, V, FAST>(yp + o0[k], a[k], n0[k]);
+              store_vec<T, V, FAST>(yp + o1[k], b[k], n1[k]);
             }
           }
+          out += R;
+          yp += R * S.y_h;
         }
       }
     }
@@ -326,7 +421,11 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
       for (int k = 0; k < NU; ++k)
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          float a = acc[t][0][k][i], b = acc[t][1][k][i];
+          float a, b, x0, x1, y0, y1;
+          halves(acc[t][0][k][i / 2], x0, x1);
+          halves(acc[t][1][k][i / 2], y0, y1);
+          a = i & 1 ? x1 : x0;
+          b = i & 1 ? y1 : y0;
           for (int o = L; o < 32; o <<= 1) {
             a += __shfl_xor_sync(0xffffffffu, a, o);
             b += __shfl_xor_sync(0xffffffffu, b, o);
