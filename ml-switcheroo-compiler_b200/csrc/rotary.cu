@@ -123,14 +123,18 @@ struct Vec {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (i < n) w[i] = __float_as_uint((float)p[i]);
-    } else if (n) {
-      if constexpr (WORDS == 4) {
-        const uint4 u = *reinterpret_cast<const uint4*>(p);
-        w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(p);
-        w[0] = u.x, w[1] = u.y;
-      }
+    } else if constexpr (WORDS == 4) {
+      // predicated, where `if` would branch around every load (17 % of all instructions); volatile
+      // keeps loads and stores in order for a result written over its input
+      asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %5, 0;\n @p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n}\n"
+                   : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])
+                   : "l"(p), "r"(n)
+                   : "memory");
+    } else {
+      asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n @p ld.global.v2.u32 {%0, %1}, [%2];\n}\n"
+                   : "+r"(w[0]), "+r"(w[1])
+                   : "l"(p), "r"(n)
+                   : "memory");
     }
   }
   __device__ __forceinline__ f2 get(int i) const {  // elements 2 i and 2 i + 1
@@ -151,13 +155,16 @@ __device__ __forceinline__ void store_vec(T* p, const f2 (&x)[V / 2], int n) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) put(p + i, v[i]);
-  } else if (n) {
-    if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-    } else {
-      const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
-      *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
-    }
+  } else if constexpr (sizeof(T) == 4) {
+    asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %5, 0;\n @p st.global.v4.f32 [%4], {%0, %1, %2, %3};\n}\n" ::"f"(v[0]), "f"(v[1]),
+                 "f"(v[2]), "f"(v[3]), "l"(p), "r"(n)
+                 : "memory");
+  } else {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    asm volatile("{\n .reg .pred p;\n setp.ne.s32 p, %3, 0;\n @p st.global.v2.u32 [%2], {%0, %1};\n}\n" ::"r"(
+                     *reinterpret_cast<const uint32_t*>(&a)),
+                 "r"(*reinterpret_cast<const uint32_t*>(&b)), "l"(p), "r"(n)
+                 : "memory");
   }
 }
 
@@ -167,7 +174,7 @@ struct Row {
 };
 
 template <typename T, int V, int NU, bool FAST, bool INTER, int MODE>
-__global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kernel(const __grid_constant__ Args A) {
+__global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 3 : 2)) heads_kernel(const __grid_constant__ Args A) {
   constexpr int BATCH = NU > 1 ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
   constexpr int P = V / 2;  // f32x2 values per vector
   __shared__ uint64_t freq[B200_ROTARY_MAX_DIM / 2];
@@ -176,9 +183,9 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
   for (int i = threadIdx.x; i < half; i += THREADS) freq[i] = A.freq[i];
   if constexpr (MODE != ROTATE) {
     const int dt = A.gamma_bf16 ? B200_BF16 : B200_F32;
-    for (int i = threadIdx.x; i < 2 * A.dim; i += THREADS) {
-      const int t = i >= A.dim, d = i - t * A.dim;
-      gamma[t][d] = A.seg[t].gamma ? load_as_f32(A.seg[t].gamma, d, dt) : 1.f;
+    for (int i = threadIdx.x; i < 2 * B200_ROTARY_MAX_DIM; i += THREADS) {
+      const int t = i / B200_ROTARY_MAX_DIM, d = i % B200_ROTARY_MAX_DIM;
+      gamma[t][d] = A.seg[t].gamma && d < A.dim ? load_as_f32(A.seg[t].gamma, d, dt) : 1.f;
     }
   }
   __syncthreads();
@@ -314,13 +321,10 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
         for (int k = 0; k < NU; ++k)
 #pragma unroll
           for (int i = 0; i < P; ++i) {
-            float g[4];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              g[e] = 2 * i + e < n0[k] ? gamma[t][o0[k] + 2 * i + e] : 1.f;
-              g[2 + e] = 2 * i + e < n1[k] ? gamma[t][o1[k] + 2 * i + e] : 1.f;
-            }
-            const f2 ga = gam[0][k][i] = pair(g[0], g[1]), gb = gam[1][k][i] = pair(g[2], g[3]);
+            // beyond the head: any weight will do, the elements are zeros and are not stored
+            const int ia = min(o0[k] + 2 * i, B200_ROTARY_MAX_DIM - 2), ib = min(o1[k] + 2 * i, B200_ROTARY_MAX_DIM - 2);
+            const f2 ga = gam[0][k][i] = pair(gamma[t][ia], gamma[t][ia + 1]);
+            const f2 gb = gam[1][k][i] = pair(gamma[t][ib], gamma[t][ib + 1]);
             if constexpr (MODE == NORM) {
               w1[0][k][i] = mul2(k1[0][k][i], ga);
               w1[1][k][i] = mul2(k1[1][k][i], gb);
@@ -334,9 +338,7 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
       T* yp = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s + out * S.y_h;
       for (int g = lo; g < hi; g += BATCH) {
         if (t != t_first || g != lo) fetch(S, end);
-#pragma unroll
-        for (int j = 0; j < BATCH; ++j) {
-          if (g + j >= hi) break;  // warp-uniform
+        auto work = [&](int j) {
           f2 a[NU][P], b[NU][P];
           f2 ss = 0;
 #pragma unroll
@@ -398,15 +400,24 @@ __global__ void __launch_bounds__(THREADS, MODE == NORM_GRAD ? 2 : 3) heads_kern
                 b[k][i] = fma2(gb[k][i], gam[1][k][i], mul2(b[k][i], m2));
               }
           }
-          if (out < end) {
 #pragma unroll
-            for (int k = 0; k < NU; ++k) {
-              store_vec<T, V, FAST>(yp + o0[k], a[k], n0[k]);
-              store_vec<T, V, FAST>(yp + o1[k], b[k], n1[k]);
-            }
+          for (int k = 0; k < NU; ++k) {
+            store_vec<T, V, FAST>(yp + o0[k], a[k], out < end ? n0[k] : 0);
+            store_vec<T, V, FAST>(yp + o1[k], b[k], out < end ? n1[k] : 0);
           }
           out += R;
           yp += R * S.y_h;
+        };
+        // whole batches without a branch between their rows, so that one's shuffles hide another's
+        if (g + BATCH <= hi) {
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j) work(j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < BATCH; ++j) {
+            if (g + j >= hi) break;  // warp-uniform
+            work(j);
+          }
         }
       }
     }
