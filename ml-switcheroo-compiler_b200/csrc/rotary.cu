@@ -173,7 +173,7 @@ struct Row {
   Vec<T, V, FAST> a[NU], b[NU];
 };
 
-template <typename T, int V, int NU, bool FAST, bool INTER, int MODE>
+template <typename T, int V, int NU, bool FAST, bool INTER, int MODE, int LANES>
 __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 3 : 2)) heads_kernel(const __grid_constant__ Args A) {
   constexpr int BATCH = NU > 1 ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
   constexpr int P = V / 2;  // f32x2 values per vector
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
   }
   __syncthreads();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int L = A.L, sub = lane / L, u0 = lane % L, R = 32 / L;
+  const int L = LANES ? LANES : A.L, sub = lane / L, u0 = lane % L, R = 32 / L;
   // this lane's units: element offsets, how many elements of each vector exist, first pair
   int o0[NU], o1[NU], n0[NU], n1[NU], f0[NU];
   bool rot[NU];
@@ -336,8 +336,19 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
       if (t != t_first) point(S, lo);
       int out = lo * R + sub;
       T* yp = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s + out * S.y_h;
+      // The gradient's few warps keep the next batch's loads in flight; the other modes load
+      // a batch and work on it (more warps, and more rows a batch, do as well there).
+      constexpr bool AHEAD = MODE == NORM_GRAD && NU == 1;
+      if (AHEAD && t != t_first) fetch(S, end);
       for (int g = lo; g < hi; g += BATCH) {
-        if (t != t_first || g != lo) fetch(S, end);
+        Row<T, V, NU, FAST> xc[BATCH], dc[BATCH];
+        if (!AHEAD && (t != t_first || g != lo)) fetch(S, end);
+#pragma unroll
+        for (int j = 0; j < BATCH; ++j) {
+          xc[j] = xr[j];
+          if constexpr (MODE == NORM_GRAD) dc[j] = dr[j];
+        }
+        if (AHEAD && g + BATCH < hi) fetch(S, end);
         auto work = [&](int j) {
           f2 a[NU][P], b[NU][P];
           f2 ss = 0;
@@ -345,14 +356,15 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
           for (int k = 0; k < NU; ++k)
 #pragma unroll
             for (int i = 0; i < P; ++i) {
-              a[k][i] = xr[j].a[k].get(i);
-              b[k][i] = xr[j].b[k].get(i);
+              a[k][i] = xc[j].a[k].get(i);
+              b[k][i] = xc[j].b[k].get(i);
               if constexpr (MODE != ROTATE) ss = fma2(a[k][i], a[k][i], fma2(b[k][i], b[k][i], ss));
             }
           if constexpr (MODE == ROTATE) {
             turn(a, b, k1, k2);
           } else if constexpr (MODE == NORM) {
             float sq = sum2(ss);
+            #pragma unroll
             for (int o = L >> 1; o > 0; o >>= 1) sq += __shfl_xor_sync(0xffffffffu, sq, o);
             const float rstd = rsqrtf(sq * inv_dim + A.eps);
             const f2 r2 = pair(rstd, rstd);
@@ -370,8 +382,8 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
             for (int k = 0; k < NU; ++k)
 #pragma unroll
               for (int i = 0; i < P; ++i) {
-                ga[k][i] = dr[j].a[k].get(i);
-                gb[k][i] = dr[j].b[k].get(i);
+                ga[k][i] = dc[j].a[k].get(i);
+                gb[k][i] = dc[j].b[k].get(i);
               }
             turn(ga, gb, k1, k2);
             f2 hh = 0;
@@ -381,6 +393,7 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
               for (int i = 0; i < P; ++i)
                 hh = fma2(mul2(ga[k][i], gam[0][k][i]), a[k][i], fma2(mul2(gb[k][i], gam[1][k][i]), b[k][i], hh));
             float sq = sum2(ss), hx = sum2(hh);
+#pragma unroll
             for (int o = L >> 1; o > 0; o >>= 1) {
               sq += __shfl_xor_sync(0xffffffffu, sq, o);
               hx += __shfl_xor_sync(0xffffffffu, hx, o);
@@ -475,11 +488,22 @@ __global__ void __launch_bounds__(256) gamma_sum_kernel(const float* __restrict_
   }
 }
 
-template <typename T, int V, int NU, bool FAST, int MODE>
+template <typename T, int V, int NU, bool FAST, int MODE, int LANES = 0>
 static int launch(const Args& a, bool inter, int grid, cudaStream_t s) {
-  if (inter) heads_kernel<T, V, NU, FAST, true, MODE><<<grid, THREADS, 0, s>>>(a);
-  else heads_kernel<T, V, NU, FAST, false, MODE><<<grid, THREADS, 0, s>>>(a);
+  if (inter) heads_kernel<T, V, NU, FAST, true, MODE, LANES><<<grid, THREADS, 0, s>>>(a);
+  else heads_kernel<T, V, NU, FAST, false, MODE, LANES><<<grid, THREADS, 0, s>>>(a);
   return check_launch(MODE == ROTATE ? "rotary" : (MODE == NORM ? "qk_norm_rotary" : "qk_norm_rotary_grad"));
+}
+
+// heads of up to 256 elements in whole vectors; the norms' reductions over 8 or 16 lanes (heads
+// of 64 or 128) are unrolled
+template <typename T, int MODE>
+static int launch_fast(const Args& a, bool inter, int grid, cudaStream_t s) {
+  if constexpr (MODE != ROTATE) {
+    if (a.L == 8) return launch<T, 4, 1, true, MODE, 8>(a, inter, grid, s);
+    if (a.L == 16) return launch<T, 4, 1, true, MODE, 16>(a, inter, grid, s);
+  }
+  return launch<T, 4, 1, true, MODE>(a, inter, grid, s);
 }
 
 static int grad_blocks() { return 2 * num_sms(); }
@@ -518,10 +542,10 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
   if (blocks_out) *blocks_out = grid;
   const bool in = r->interleaved != 0;
   if (dtype == B200_F32) {
-    if (fast) return nu == 1 ? launch<float, 4, 1, true, MODE>(a, in, grid, s) : launch<float, 4, 2, true, MODE>(a, in, grid, s);
+    if (fast) return nu == 1 ? launch_fast<float, MODE>(a, in, grid, s) : launch<float, 4, 2, true, MODE>(a, in, grid, s);
     return nu == 1 ? launch<float, 2, 1, false, MODE>(a, in, grid, s) : launch<float, 2, 4, false, MODE>(a, in, grid, s);
   }
-  if (fast) return nu == 1 ? launch<__nv_bfloat16, 4, 1, true, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 4, 2, true, MODE>(a, in, grid, s);
+  if (fast) return nu == 1 ? launch_fast<__nv_bfloat16, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 4, 2, true, MODE>(a, in, grid, s);
   return nu == 1 ? launch<__nv_bfloat16, 2, 1, false, MODE>(a, in, grid, s) : launch<__nv_bfloat16, 2, 4, false, MODE>(a, in, grid, s);
 }
 
