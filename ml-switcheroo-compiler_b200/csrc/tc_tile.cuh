@@ -313,6 +313,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
     sp.lane = lane;
     sp.buf = smem_u32(s_epi) + (uint32_t)(warp - EPI_FIRST) * EPI_BUF;
     constexpr int CH = BN / 64;  // chunks of 32 columns per warp
+    static_assert(!TEAM || CH == 2, "teams share 128-wide tiles");
     uint32_t local = 0, tiles = 0;
     bool ok = true;
     // the accumulator may be overwritten once every epilogue warp has read it
@@ -336,8 +337,8 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       const int64_t col0 = sp.col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
       epi.begin(sp);
-      // the member that finishes chunk c of this warp
-      auto owner = [&](int c) { return TEAM ? (sp.half * CH + c) * lp.team / (2 * CH) : 0; };
+      // the member that finishes chunk c of this warp: of two, each takes a chunk of every warp
+      auto owner = [&](int c) { return !TEAM ? 0 : (lp.team == 2 ? c : sp.half * CH + c); };
       if constexpr (SPLIT || TEAM) {
         float acc[CH][32];
 #pragma unroll
@@ -377,13 +378,13 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           // every member's MMAs are done: the operand ring takes the partial sums, 16 KB (128 rows
           // of 32, 16-byte pieces swizzled by row) per chunk and sender
           cluster_sync_all();
-          const int each = 2 * CH / lp.team;
+          const int each = 2 * CH / lp.team, mine = lp.team == 2 ? sp.half : 0;
           const uint32_t line = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 128u;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             const int to = owner(c);
             if (to == member) continue;
-            const int slot = (member < to ? member : member - 1) * each + (sp.half * CH + c) % each;
+            const int slot = (member < to ? member : member - 1) * each + mine;
             uint32_t far;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(line + (uint32_t)slot * 16384u), "r"(to));
 #pragma unroll
@@ -397,7 +398,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           for (int c = 0; c < CH; ++c) {
             if (owner(c) != member) continue;
             for (int from = 0; from < lp.team - 1; ++from) {
-              const uint32_t at_line = line + (uint32_t)(from * each + (sp.half * CH + c) % each) * 16384u;
+              const uint32_t at_line = line + (uint32_t)(from * each + mine) * 16384u;
 #pragma unroll
               for (int p = 0; p < 8; ++p) {
                 const uint4 u = ld_shared_v4(at_line + (uint32_t)((p ^ (lane & 7)) << 4));
