@@ -256,14 +256,14 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
     pos, pa = _positions(name, positions, offset, batch, seq)
     _on_device(name, q, k, dyq, dyk, gq, gk, pos)
     (dq, rqs), (dk, rks) = _like(q), _like(k)
-    dgamma = torch.empty(2, dim, dtype=torch.float32, device=q.device)
-    wn = int(L.lib().b200_qk_norm_rotary_grad_workspace_bytes(dim))
+    dgq, dgk = torch.empty(2, dim, dtype=torch.float32, device=q.device).unbind(0)
+    wn = L.lib().b200_qk_norm_rotary_grad_workspace_bytes(dim)
     ws = torch.empty(wn, dtype=torch.uint8, device=q.device)
     st = L.I64x18(*qs, *dqs, *rqs, *ks, *dks, *rks)
     L.call("b200_qk_norm_rotary_grad", r, ops.code(q), dyq.data_ptr(), dyk.data_ptr(), q.data_ptr(), k.data_ptr(), dq.data_ptr(),
-           dk.data_ptr(), batch, seq, hq, hk, st, ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, dgamma[0].data_ptr(),
-           dgamma[1].data_ptr(), ws.data_ptr(), wn, ops.stream_ptr())
-    return dq, dk, dgamma[0], dgamma[1]
+           dk.data_ptr(), batch, seq, hq, hk, st, ops._ptr(gq), ops._ptr(gk), gdt, float(eps), *pa, dgq.data_ptr(),
+           dgk.data_ptr(), ws.data_ptr(), wn, ops.stream_ptr())
+    return dq, dk, dgq, dgk
 
 
 # ----------------------------------------------------------------------------------
@@ -271,34 +271,46 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
 # ----------------------------------------------------------------------------------
 
 
+def _cast(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A fresh cast (of a transposed matrix in its storage order)."""
+    return ops.cast(t.t(), dtype).t() if t.dim() == 2 and t.stride(0) == 1 else ops.cast(t, dtype)
+
+
 def _head(name: str, x: torch.Tensor, w: torch.Tensor, labels: Any):
     """The operands as the entry points take them: (x [N, D], w, labels [N], row strides,
     whether w is stored [D, V], sizes)."""
-    if w.dim() != 2 or x.dim() < 1 or x.shape[-1] != w.shape[0]:
-        raise ValueError(f"{name}: x {tuple(x.shape)} and w {tuple(w.shape)} not aligned")
-    if not isinstance(labels, torch.Tensor) or not labels.is_cuda or labels.dtype not in (torch.int64, torch.int32):
-        labels = ops._int_indices(labels)
-    if labels.numel() != math.prod(x.shape[:-1]) or tuple(labels.shape) not in (tuple(x.shape[:-1]), (*x.shape[:-1], 1)):
-        raise ValueError(f"{name}: labels {tuple(labels.shape)} of x {tuple(x.shape)}")
+    xs, ws = tuple(x.shape), tuple(w.shape)
+    if len(ws) != 2 or not xs or xs[-1] != ws[0]:
+        raise ValueError(f"{name}: x {xs} and w {ws} not aligned")
     if x.dtype not in _FLOATS or w.dtype not in _FLOATS:
         raise BackendNotSupportedError(f"{name}: x of {x.dtype} and w of {w.dtype} (fp32 and bf16)")
-    D, V = w.shape
+    D, V = ws
     if D < 1 or V < 1:
-        raise ValueError(f"{name}: w {tuple(w.shape)} has no features or no words")
+        raise ValueError(f"{name}: w {ws} has no features or no words")
+    if not isinstance(labels, torch.Tensor) or not labels.is_cuda or labels.dtype not in (torch.int64, torch.int32):
+        labels = ops._int_indices(labels)
+    if tuple(labels.shape) not in (xs[:-1], (*xs[:-1], 1)):
+        raise ValueError(f"{name}: labels {tuple(labels.shape)} of x {xs}")
     _on_device(name, x, w, labels)
-    if x.dtype != w.dtype or (x.dtype == torch.float32 and ops.Config.matmul_dtype == "bf16"):
+    policy = ops.Config.matmul_dtype
+    if x.dtype != w.dtype or (policy == "bf16" and x.dtype == torch.float32):
         # the contraction policy of Matmul: bf16 operands, or fp32 where either is
-        dt = torch.bfloat16 if ops.Config.matmul_dtype == "bf16" else torch.float32
-        x, w = ops.cast_operand(x, dt), ops.cast_operand(w, dt)
-    x2 = x.reshape(-1, D) if x.dim() == 1 or x.is_contiguous() else (x if x.dim() == 2 else ops.contiguous(x).reshape(-1, D))
-    if x2.stride(1) != 1 and D > 1 or x2.stride(0) < D:
-        x2 = ops.contiguous(x2)
-    N = x2.shape[0]
-    dn = w.stride(1) == 1 and w.stride(0) >= V
-    if not dn and not (w.stride(0) == 1 and w.stride(1) >= D):
+        dt = torch.bfloat16 if policy == "bf16" else torch.float32
+        x, w = _cast(x, dt), _cast(w, dt)
+    if len(xs) != 2:
+        x = ops.contiguous(x).view(-1, D)
+    sn, sd = x.stride()
+    if (sd != 1 and D > 1) or sn < D:
+        x = ops.contiguous(x)
+        sn = D
+    N = x.shape[0]
+    wr, wc = w.stride()
+    dn = wc == 1 and wr >= V
+    if not dn and not (wr == 1 and wc >= D):
         w, dn = ops.contiguous(w), True
-    labels = ops.contiguous(labels).view(-1)
-    return x2, w, labels, max(x2.stride(0), D), w.stride(0) if dn else w.stride(1), int(dn), N, D, V
+        wr = V
+    labels = ops.contiguous(labels)
+    return x, w, labels, max(sn, D), wr if dn else wc, int(dn), N, D, V
 
 
 def op_linear_cross_entropy(x, w, labels, ignore_index=-100, **_):
@@ -312,16 +324,16 @@ def op_linear_cross_entropy(x, w, labels, ignore_index=-100, **_):
     two bf16 planes each (16 bits), or rounded to bf16 where ``Config.matmul_dtype`` is
     "bf16". Keep ``lse`` for LinearCrossEntropyGrad."""
     name = "LinearCrossEntropy"
-    shape = tuple(x.shape[:-1])
+    shape = x.shape[:-1]
     x, w, labels, ldx, ldw, dn, N, D, V = _head(name, x, w, labels)
-    out = torch.empty(2, N, dtype=torch.float32, device=x.device)
+    loss, lse = torch.empty(2, *shape, dtype=torch.float32, device=x.device).unbind(0)
     if N:
-        args = (ops.code(x), x.data_ptr(), ldx, w.data_ptr(), ldw, dn)
-        wn = int(L.lib().b200_linear_xent_workspace_bytes(*args, N, D, V))
-        ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=x.device)
-        L.call("b200_linear_xent", *args, labels.data_ptr(), ops.code(labels), int(ignore_index), out[0].data_ptr(), out[1].data_ptr(), N,
-               D, V, ws.data_ptr(), wn, ops.stream_ptr())
-    return out[0].view(shape), out[1].view(shape)
+        dt, xp, wp = ops.code(x), x.data_ptr(), w.data_ptr()
+        wn = L.lib().b200_linear_xent_workspace_bytes(dt, xp, ldx, wp, ldw, dn, N, D, V)
+        ws = torch.empty(wn, dtype=torch.uint8, device=x.device)
+        L.call("b200_linear_xent", dt, xp, ldx, wp, ldw, dn, labels.data_ptr(), ops.code(labels), int(ignore_index), loss.data_ptr(),
+               lse.data_ptr(), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
+    return loss, lse
 
 
 def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **_):
@@ -340,10 +352,10 @@ def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **
     dloss, lse = (ops.contiguous(ops.cast(t, torch.float32)) for t in (dloss, lse))
     dx = torch.empty(*lead, D, dtype=x.dtype, device=x.device)
     dw = torch.empty((D, V) if dn else (V, D), dtype=w.dtype, device=w.device)
-    args = (x.data_ptr(), ldx, w.data_ptr(), ldw, dn)
-    wn = int(L.lib().b200_linear_xent_grad_workspace_bytes(ops.code(x), *args, N, D, V))
-    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=x.device)
-    L.call("b200_linear_xent_grad", ops.code(x), dloss.data_ptr(), *args, labels.data_ptr(), ops.code(labels), int(ignore_index),
+    dt, xp, wp = ops.code(x), x.data_ptr(), w.data_ptr()
+    wn = L.lib().b200_linear_xent_grad_workspace_bytes(dt, xp, ldx, wp, ldw, dn, N, D, V)
+    ws = torch.empty(wn, dtype=torch.uint8, device=x.device)
+    L.call("b200_linear_xent_grad", dt, dloss.data_ptr(), xp, ldx, wp, ldw, dn, labels.data_ptr(), ops.code(labels), int(ignore_index),
            lse.data_ptr(), dx.data_ptr(), dw.data_ptr(), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
     return ops.cast(dx, x0.dtype), ops.cast(dw if dn else dw.t(), w0.dtype)
 
@@ -389,8 +401,8 @@ def op_newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, **_):
     _on_device(name, g)
     gc = ops.contiguous(g)
     out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
-    wn = int(L.lib().b200_newton_schulz_workspace_bytes(ops.code(g), batch, rows, cols))
-    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=g.device)
+    wn = L.lib().b200_newton_schulz_workspace_bytes(ops.code(g), batch, rows, cols)
+    ws = torch.empty(wn, dtype=torch.uint8, device=g.device)
     L.call("b200_newton_schulz", ops.code(g), gc.data_ptr(), out.data_ptr(), batch, rows, cols, coef, int(steps), float(eps),
            ws.data_ptr(), wn, ops.stream_ptr())
     return out
@@ -418,8 +430,8 @@ def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov
         if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name}: results must be dense fp32 {tuple(p.shape)}")
     _on_device(name, p, m, g, *out)
-    wn = int(L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols))
-    ws = torch.empty(max(wn, 1), dtype=torch.uint8, device=p.device)
+    wn = L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols)
+    ws = torch.empty(wn, dtype=torch.uint8, device=p.device)
     L.call("b200_apply_muon_f32", p.data_ptr(), m.data_ptr(), g.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), batch, rows, cols, lr,
            float(momentum), int(bool(nesterov)), float(weight_decay), coef, int(steps), float(eps), ws.data_ptr(), wn, ops.stream_ptr())
     return tuple(out)
