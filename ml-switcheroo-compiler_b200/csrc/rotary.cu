@@ -18,7 +18,7 @@
 //
 // Layout of the work. A lane owns one unit of a head: two vectors of V = 4 elements that
 // hold whole pairs (the two halves of V pairs, or 2V neighbours), so a rotation needs no
-// shuffle; the units of a head take L lanes (a power of two), and a warp holds R = 32 / L
+// shuffle; the units of a head take L lanes (a power of two for the norms), a warp holds R = 32 / L
 // heads. A warp takes a token and walks its heads, R at a time: the lane's angles are the
 // same for every head, so cosines and sines are made once per token, while the first heads'
 // loads are under way. Few tokens (a decoding batch) are split over head groups, so that the
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
   bool rot[NU];
 #pragma unroll
   for (int k = 0; k < NU; ++k) {
-    const int u = u0 + L * k;
+    const int u = sub < R ? u0 + L * k : A.n_units;  // lanes beyond the last whole head have none
     rot[k] = u < A.n_rot;
     f0[k] = u * V;
     if (rot[k] && !INTER) {
@@ -527,6 +527,9 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
   a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
   a.L = 1;
   while (a.L < a.n_units && a.L < 32) a.L *= 2;
+  // without a reduction the lanes of a head need be no power of two: three heads of 10 units
+  // share a warp instead of two
+  if (MODE == ROTATE && a.n_units <= 32) a.L = std::max(1, a.n_units);
   const int nu = (int)ceil_div(a.n_units, a.L);
   const int R = 32 / a.L;
   for (Seg& g : a.seg) g.groups = (int)ceil_div(g.heads, R);
