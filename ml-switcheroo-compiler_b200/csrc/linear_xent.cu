@@ -67,8 +67,9 @@ struct LseEpi {
       for (int i = 0; i < 32; ++i)
         if (col + i >= a.V) v[i] = -INFINITY;
     }
-    const int64_t k = label - col;
-    if (k >= 0 && k < 32) {
+    const int64_t at = label - col;
+    if (at >= 0 && at < 32) {
+      const int k = (int)at;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (k == i) at_label = v[i];
@@ -175,8 +176,9 @@ struct GradEpi {
   __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = g * ex2(fmaf(v[i], LOG2E, -shift));
-    const int64_t k = label - col;
-    if (k >= 0 && k < 32) {
+    const int64_t at = label - col;
+    if (at >= 0 && at < 32) {
+      const int k = (int)at;
 #pragma unroll
       for (int i = 0; i < 32; ++i)
         if (k == i) v[i] -= g;
@@ -254,14 +256,14 @@ struct StoreEpi {
       for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
       stage_chunk<2>(sp.buf, sp.lane, w);
       __syncwarp();
-      write_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a.C) + at), a.ld, rows, cols);
+      put_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a.C) + at), a.ld, rows, (int)cols);
     } else {
       uint32_t w[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
       stage_chunk<4>(sp.buf, sp.lane, w);
       __syncwarp();
-      write_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a.C) + at), a.ld, rows, cols);
+      put_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a.C) + at), a.ld, rows, (int)cols);
     }
   }
 };

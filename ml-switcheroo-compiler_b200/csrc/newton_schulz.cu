@@ -102,7 +102,7 @@ struct NsEpi {
               v[8 * j + 2 * i + 1] = fmaf(ca, y, v[8 * j + 2 * i + 1]);
             }
           }
-      const int64_t k = sp.row - col;
+      const int k = (int)(sp.row - col);
       if (k >= 0 && k < 32) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
@@ -136,14 +136,14 @@ struct NsEpi {
         for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
         stage_chunk<2>(sp.buf, sp.lane, w);
         __syncwarp();
-        write_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at), a.N, rows, cols);
+        put_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at), a.N, rows, (int)cols);
       } else {
         uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
         stage_chunk<4>(sp.buf, sp.lane, w);
         __syncwarp();
-        write_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a.out) + at), a.N, rows, cols);
+        put_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a.out) + at), a.N, rows, (int)cols);
       }
       return;
     }

@@ -148,6 +148,40 @@ __device__ __forceinline__ void commit(uint64_t* bar) {
   }
 }
 
+// A chunk staged by stage_chunk<ESZ> to rows of an output whose rows start anywhere: 16 bytes a
+// lane where every row allows it, else an element a lane. The loops stay small: an epilogue's
+// chunks are unrolled, and code beyond the instruction caches cost the first tile of a launch
+// three times the others.
+template <int ESZ>
+__device__ __forceinline__ void put_chunk(uint32_t buf, int lane, uint8_t* base, int64_t ld, int rows, int cols) {
+  constexpr int PIECES = 2 * ESZ;
+  auto word_at = [&](int r, int byte) {
+    const uint32_t sw = ESZ == 4 ? (uint32_t)(r & 7) : (uint32_t)((r >> 1) & 3);
+    return buf + (uint32_t)r * (32u * ESZ) + ((((uint32_t)byte >> 4) ^ sw) << 4) + ((uint32_t)byte & 15u);
+  };
+  if (cols == 32 && ((reinterpret_cast<uintptr_t>(base) | (uint64_t)ld * ESZ) & 15) == 0) {
+    const int j = lane % PIECES;
+#pragma unroll 2
+    for (int r = lane / PIECES; r < rows; r += 32 / PIECES)
+      *reinterpret_cast<uint4*>(base + (int64_t)r * ld * ESZ + 16 * j) = ld_shared_v4(word_at(r, 16 * j));
+    return;
+  }
+#pragma unroll 1
+  for (int r = 0; r < rows; ++r)
+    if (lane < cols) {
+      uint8_t* d = base + ((int64_t)r * ld + lane) * ESZ;
+      if constexpr (ESZ == 4) {
+        uint32_t v;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(word_at(r, 4 * lane)) : "memory");
+        *reinterpret_cast<uint32_t*>(d) = v;
+      } else {
+        uint16_t v;
+        asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(word_at(r, 2 * lane)) : "memory");
+        *reinterpret_cast<uint16_t*>(d) = v;
+      }
+    }
+}
+
 // What an epilogue warp knows about its chunk: `row` is this lane's output row, `row0` the
 // warp's first one, `buf` its staging buffer
 struct Spot {

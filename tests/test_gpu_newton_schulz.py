@@ -99,6 +99,16 @@ def test_scale_layout_steps_and_coefficients():
     assert float((q @ q.mT - torch.eye(32, device="cuda")).abs().max()) <= 1e-5
 
 
+@pytest.mark.parametrize("coef", [(2.0, -1.2, 0.01), (1.9, -1.0, 0.1), (1.2, 0.0, -0.2), (3.0, -3.2, 1.2), (1.0, 0.0, 0.0), (2.0, -1.5, 0.5)])
+@pytest.mark.parametrize("shape", [(96, 150), (260, 200), (4, 520, 700)])
+def test_small_missing_and_negative_coefficients(shape, coef):
+    g = grads(*shape)
+    got = op("NewtonSchulz", g, coefficients=coef)
+    assert off(got, R.newton_schulz(g.double(), 5, coef)) <= BOUND[F32]
+    tiny = (g * 2.0**-40).contiguous()
+    assert off(op("NewtonSchulz", tiny, coefficients=coef), R.newton_schulz(tiny.double(), 5, coef)) <= BOUND[F32]
+
+
 def test_extreme_spectra_stay_finite_and_near():
     """One direction far above the rest, equal directions, a rank of one."""
     u, v = torch.linalg.qr(torch.randn(64, 64, device="cuda"))[0], torch.linalg.qr(torch.randn(160, 64, device="cuda"))[0]
