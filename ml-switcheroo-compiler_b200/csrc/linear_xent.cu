@@ -18,6 +18,7 @@
 // (x = hi + lo, 16 bits), three products each (tc_tile.cuh); d likewise.
 // Bound by the tensor cores: 2 N D V flop forward, 6 N D V backward.
 //
+// Up to 8 tokens of fp32, or one of bf16, take kernels of their own (below): reading w bounds them.
 // Rows whose label is ignore_index: loss 0, no gradient, and the row of x they hold is
 // replaced by zeros where dw is made, so whatever it contains stays out.
 #include "tc_tile.cuh"
@@ -325,6 +326,420 @@ __global__ void __launch_bounds__(256) pack_kernel(const void* __restrict__ src,
   }
 }
 
+// ---- few tokens: up to 8 rows of fp32 x, or one of bf16, on the CUDA cores ----
+// With N rows a weight is worth 2 N flop forward and 6 N backward: below about a dozen rows
+// reading w (and writing dw) bounds the call, a 128-row tile is mostly padding, and splitting
+// fp32 weights into planes triples the bytes. x (fp32) stays in shared memory, w is read
+// once forward, twice backward (the second time for dx, from the L2 where it fits). Products
+// and sums are fp32 throughout.
+namespace few {
+
+constexpr int MOST = 8, WARPS = 8, T = 32 * WARPS, X_FLOATS = 12288;
+
+struct Args {
+  const void *x, *w, *labels;
+  const float *dloss, *lse;
+  int64_t ldx, ldw, ignore;
+  int labels_i32, N, D, V;
+  float2* part;    // forward: [blocks][N]
+  float* picked;
+  float* d;        // backward: [N][V]
+  void* dw;
+};
+
+template <typename E>
+__device__ __forceinline__ float value(E v);
+template <>
+__device__ __forceinline__ float value<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ float value<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+
+// W adjacent elements (one 8- or 16-byte access where W > 1)
+template <typename E, int W>
+__device__ __forceinline__ void get(const E* p, float (&v)[W]) {
+  if constexpr (W == 1) {
+    v[0] = value(*p);
+  } else if constexpr (sizeof(E) == 4) {
+    const float4 u = *reinterpret_cast<const float4*>(p);
+    v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+  } else {
+    const uint2 u = *reinterpret_cast<const uint2*>(p);
+    v[0] = __uint_as_float(u.x << 16), v[1] = __uint_as_float(u.x & 0xffff0000u);
+    v[2] = __uint_as_float(u.y << 16), v[3] = __uint_as_float(u.y & 0xffff0000u);
+  }
+}
+template <typename E, int W>
+__device__ __forceinline__ void set(E* p, const float (&v)[W]) {
+  if constexpr (sizeof(E) == 4) {
+    if constexpr (W == 1) *p = v[0];
+    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+    if constexpr (W == 1) *p = __float2bfloat16_rn(v[0]);
+    else *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+  }
+}
+
+// x as fp32 [NT][D] (rows that do not exist, and with `masked` those of ignored tokens, zeros)
+template <typename E, int NT>
+__device__ __forceinline__ void load_x(const Args& a, float* xs, bool masked) {
+  for (int t = 0; t < NT; ++t) {
+    const bool in = t < a.N && !(masked && label_at(a.labels, a.labels_i32, t) == a.ignore);
+    for (int k = threadIdx.x; k < a.D; k += T) xs[t * a.D + k] = in ? value(reinterpret_cast<const E*>(a.x)[t * a.ldx + k]) : 0.f;
+  }
+}
+
+// gradient of a logit z of token t at word v
+struct Row {
+  float g, shift;
+  int64_t label;
+  bool kept;
+  __device__ __forceinline__ void load(const Args& a, int t) {
+    kept = false, g = shift = 0.f, label = -1;
+    if (t >= a.N) return;
+    const int64_t l = label_at(a.labels, a.labels_i32, t);
+    if (l == a.ignore || l < 0 || l >= a.V) return;
+    kept = true, label = l, g = a.dloss[t], shift = a.lse[t] * LOG2E;
+  }
+  __device__ __forceinline__ float grad(float z, int64_t v) const {
+    return kept ? g * ex2(fmaf(z, LOG2E, -shift)) - (v == label ? g : 0.f) : 0.f;
+  }
+};
+
+__device__ __forceinline__ void online(float& m, float& s, float z) {
+  const float M = fmaxf(m, z);
+  if (M != -INFINITY || isnan(z)) {
+    s = s * ex2((m - M) * LOG2E) + ex2((z - M) * LOG2E);
+    m = M;
+  }
+}
+
+// w stored [V, D]: a warp takes P words at a time (each element of x read from shared memory
+// serves P products), lanes along D
+template <typename E, int NT, int W, bool GRAD>
+__global__ void __launch_bounds__(T) words_kernel(const __grid_constant__ Args a) {
+  constexpr int P = NT >= 4 ? 4 : 2;
+  extern __shared__ float xs[];
+  __shared__ float2 red[WARPS][NT];
+  load_x<E, NT>(a, xs, GRAD);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  Row row[NT];
+  int64_t label[NT];
+  float m[NT], s[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    if (GRAD) row[t].load(a, t);
+    label[t] = t < a.N ? label_at(a.labels, a.labels_i32, t) : -1;
+    m[t] = -INFINITY, s[t] = 0.f;
+  }
+  __syncthreads();
+  const E* w = reinterpret_cast<const E*>(a.w);
+  for (int64_t v0 = ((int64_t)blockIdx.x * WARPS + warp) * P; v0 < a.V; v0 += (int64_t)gridDim.x * WARPS * P) {
+    float z[P][NT] = {};
+    const E* p[P];
+#pragma unroll
+    for (int j = 0; j < P; ++j) p[j] = w + min(v0 + j, (int64_t)a.V - 1) * a.ldw;
+#pragma unroll(P == 2 ? 4 : 2)
+    for (int k = lane * W; k < a.D; k += 32 * W) {
+      float u[P][W];
+#pragma unroll
+      for (int j = 0; j < P; ++j) get<E, W>(p[j] + k, u[j]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float xv[W];
+        get<float, W>(xs + t * a.D + k, xv);
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int j = 0; j < P; ++j) z[j][t] = fmaf(u[j][i], xv[i], z[j][t]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) z[j][t] = warp_sum(z[j][t]);
+#pragma unroll
+    for (int j = 0; j < P; ++j) {
+      if (v0 + j >= a.V) break;
+      if constexpr (!GRAD) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          online(m[t], s[t], z[j][t]);
+          if (lane == 0 && label[t] == v0 + j) a.picked[t] = z[j][t];
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          z[j][t] = row[t].grad(z[j][t], v0 + j);
+          if (lane == 0 && t < a.N) a.d[(int64_t)t * a.V + v0 + j] = z[j][t];
+        }
+      }
+    }
+    if constexpr (GRAD) {
+      if (!a.dw) continue;
+      for (int k = lane * W; k < a.D; k += 32 * W) {
+        float o[P][W] = {};
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          float xv[W];
+          get<float, W>(xs + t * a.D + k, xv);
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < P; ++j) o[j][i] = fmaf(z[j][t], xv[i], o[j][i]);
+        }
+#pragma unroll
+        for (int j = 0; j < P; ++j)
+          if (v0 + j < a.V) set<E, W>(reinterpret_cast<E*>(a.dw) + (v0 + j) * a.D + k, o[j]);
+      }
+    }
+  }
+  if constexpr (!GRAD) {
+    if (lane == 0)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) red[warp][t] = make_float2(m[t], s[t]);
+    __syncthreads();
+    if (threadIdx.x < NT && (int)threadIdx.x < a.N) {
+      const int t = threadIdx.x;
+      float M = -INFINITY, S = 0.f;
+      for (int i = 0; i < WARPS; ++i) M = fmaxf(M, red[i][t].x);
+      for (int i = 0; i < WARPS; ++i)
+        if (red[i][t].x != -INFINITY || isnan(red[i][t].y)) S += red[i][t].y * ex2((red[i][t].x - M) * LOG2E);
+      a.part[(int64_t)blockIdx.x * a.N + t] = make_float2(M, S);
+    }
+  }
+}
+
+// w stored [D, V]: a block takes 32 W columns, its warps share out D
+template <typename E, int NT, int W, bool GRAD>
+__global__ void __launch_bounds__(T) columns_kernel(const __grid_constant__ Args a) {
+  extern __shared__ float xs[];
+  float* red = xs + NT * a.D;  // [WARPS][NT][32 W]; then d in [0][..]
+  load_x<E, NT>(a, xs, GRAD);
+  __syncthreads();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c0 = (int64_t)blockIdx.x * 32 * W, c = c0 + lane * W;
+  const E* w = reinterpret_cast<const E*>(a.w) + c;
+  float z[NT][W] = {};
+  if (c < a.V) {  // W divides V where W > 1
+#pragma unroll 4
+    for (int k = warp; k < a.D; k += WARPS) {
+      float u[W];
+      get<E, W>(w + (int64_t)k * a.ldw, u);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < W; ++i) z[t][i] = fmaf(u[i], xs[t * a.D + k], z[t][i]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int i = 0; i < W; ++i) red[(warp * NT + t) * 32 * W + lane * W + i] = z[t][i];
+  __syncthreads();
+  // warp t finishes token t (NT <= WARPS): 32 W columns
+  if (warp < NT && warp < a.N) {
+    const int t = warp;
+    Row row;
+    if (GRAD) row.load(a, t);
+    const int64_t label = label_at(a.labels, a.labels_i32, t);
+    float m = -INFINITY, s = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const int at = i * 32 + lane;
+      if (c0 + at >= a.V) continue;
+      float v = 0.f;
+#pragma unroll
+      for (int j = 0; j < WARPS; ++j) v += red[(j * NT + t) * 32 * W + at];
+      if constexpr (GRAD) {
+        v = row.grad(v, c0 + at);
+        a.d[(int64_t)t * a.V + c0 + at] = v;
+        red[t * 32 * W + at] = v;  // this token's first slot: read above by this lane alone
+      } else {
+        online(m, s, v);
+        if (label == c0 + at) a.picked[t] = v;
+      }
+    }
+    if constexpr (!GRAD) {
+      const bool nan = isnan(s);
+      const float M = warp_max(m);
+      s = warp_sum(nan ? NAN : (m == -INFINITY ? 0.f : s * ex2((m - M) * LOG2E)));
+      if (lane == 0) a.part[(int64_t)blockIdx.x * a.N + t] = make_float2(M, s);
+    }
+  }
+  if constexpr (GRAD) {
+    __syncthreads();
+    if (!a.dw || c >= a.V) return;
+    float d[NT][W];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < W; ++i) d[t][i] = t < a.N ? red[t * 32 * W + lane * W + i] : 0.f;
+    E* out = reinterpret_cast<E*>(a.dw) + c;
+#pragma unroll 2
+    for (int k = warp; k < a.D; k += WARPS) {
+      float o[W] = {};
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = fmaf(d[t][i], xs[t * a.D + k], o[i]);
+      set<E, W>(out + (int64_t)k * a.V, o);
+    }
+  }
+}
+
+// dx = d w^T over one slice of the words (blockIdx.y): part [slices][N][D]
+template <typename E, int NT, int W>
+__global__ void __launch_bounds__(T) dx_words_kernel(const __grid_constant__ Args a, float* part, int64_t per) {
+  __shared__ float ds[NT][64];
+  const int k = (blockIdx.x * T + threadIdx.x) * W;
+  const int64_t lo = blockIdx.y * per, hi = min((int64_t)a.V, lo + per);
+  const E* w = reinterpret_cast<const E*>(a.w) + k;
+  float o[NT][W] = {};
+  for (int64_t v0 = lo; v0 < hi; v0 += 64) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 64; i += T)
+      ds[i / 64][i % 64] = i / 64 < a.N && v0 + i % 64 < hi ? a.d[(int64_t)(i / 64) * a.V + v0 + i % 64] : 0.f;
+    __syncthreads();
+    if (k >= a.D) continue;
+    const int n = (int)min((int64_t)64, hi - v0);
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) {
+      float u[W];
+      get<E, W>(w + (v0 + j) * a.ldw, u);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[t][i] = fmaf(ds[t][j], u[i], o[t][i]);
+    }
+  }
+  if (k < a.D)
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      if (t < a.N)
+#pragma unroll
+        for (int i = 0; i < W; ++i) part[((int64_t)blockIdx.y * a.N + t) * a.D + k + i] = o[t][i];
+}
+
+// the same for w stored [D, V]: a warp takes 4 features, lanes along the slice's words, 256 of
+// d at a time in shared memory
+template <typename E, int NT, int W>
+__global__ void __launch_bounds__(T) dx_columns_kernel(const __grid_constant__ Args a, float* part, int64_t per) {
+  __shared__ __align__(16) float ds[NT][256];
+  const int lane = threadIdx.x & 31, k0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 4;
+  const int64_t lo = blockIdx.y * per, hi = min((int64_t)a.V, lo + per);
+  const E* w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = reinterpret_cast<const E*>(a.w) + (int64_t)min(k0 + j, a.D - 1) * a.ldw;
+  float o[4][NT] = {};
+  for (int64_t v0 = lo; v0 < hi; v0 += 256) {
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 256; i += T)
+      ds[i / 256][i % 256] = i / 256 < a.N && v0 + i % 256 < hi ? a.d[(int64_t)(i / 256) * a.V + v0 + i % 256] : 0.f;
+    __syncthreads();
+    const int n = (int)min((int64_t)256, hi - v0);
+#pragma unroll(256 / (32 * W) < 4 ? 256 / (32 * W) : 4)
+    for (int c = lane * W; c < n; c += 32 * W) {
+      float u[4][W];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) get<E, W>(w[j] + v0 + c, u[j]);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float d[W];
+        get<float, W>(&ds[t][c], d);
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[j][t] = fmaf(d[i], u[j][i], o[j][t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const float v = warp_sum(o[j][t]);
+      if (lane == 0 && t < a.N && k0 + j < a.D) part[((int64_t)blockIdx.y * a.N + t) * a.D + k0 + j] = v;
+    }
+}
+
+// the slices' parts [slices][n], 32 threads a value, added in a fixed order, rounded once
+__global__ void __launch_bounds__(1024) join_slices_kernel(const float* __restrict__ part, int slices, int64_t n, void* out, int bf16) {
+  __shared__ float red[32][33];
+  const int lane = threadIdx.x & 31, at = threadIdx.x >> 5;
+  const int64_t i = (int64_t)blockIdx.x * 32 + lane;
+  float v = 0.f;
+  if (i < n)
+#pragma unroll 4
+    for (int k = at; k < slices; k += 32) v += part[(int64_t)k * n + i];
+  red[at][lane] = v;
+  __syncthreads();
+  if (at || i >= n) return;
+  for (int k = 1; k < 32; ++k) v += red[k][lane];
+  if (bf16) reinterpret_cast<__nv_bfloat16*>(out)[i] = __float2bfloat16_rn(v);
+  else reinterpret_cast<float*>(out)[i] = v;
+}
+
+// tokens rounded up to a kernel's 1, 2, 4 or 8
+static int rounded(int64_t N) { return N <= 1 ? 1 : (N <= 2 ? 2 : (N <= 4 ? 4 : 8)); }
+// Where these kernels are the faster ones (1024 x 32000, us forward / gradient, w stored [V, D]
+// and [D, V]): fp32 up to 8 tokens (1: 29 / 71 and 44 / 90, 8: 52 / 143 and 54 / 154, the tiles
+// 94 / 147 at 9), bf16 for one (15 / 51 and 19 / 60; two take 18 / 58 and 31 / 77, the tiles
+// 19 / 63 and 20 / 63). x has to fit shared memory.
+static bool fits(int dtype, int64_t N, int64_t D) { return N <= (dtype == B200_F32 ? MOST : 1) && rounded(N) * D <= X_FLOATS; }
+// blocks of the first kernel: word rows by the SMs, or one per 32 W columns
+static int64_t blocks(int w_dn, int wide, int64_t V) {
+  return w_dn ? ceil_div(V, wide ? 128 : 32) : std::min<int64_t>(ceil_div(V, 4 * WARPS), 4 * num_sms());
+}
+// whole vectors of 4 words (or features) at every row
+static int vectors(int dtype, const void* w, int64_t ldw, int64_t row) {
+  const uint64_t unit = dtype == B200_F32 ? 16 : 8;
+  return row % 4 == 0 && ldw % 4 == 0 && reinterpret_cast<uintptr_t>(w) % unit == 0;
+}
+// slices of the words for dx: 4 blocks an SM, as far as a slice keeps 64 words
+static int64_t slices(int w_dn, int wide, int64_t D, int64_t V) {
+  const int64_t across = w_dn ? ceil_div(D, 4 * WARPS) : ceil_div(D, (int64_t)T * (wide ? 4 : 1));
+  return std::max<int64_t>(1, std::min(ceil_div(4 * (int64_t)num_sms(), across), ceil_div(V, w_dn ? 256 : 64)));
+}
+
+template <typename E, int NT, int W>
+static int launch(const Args& a, int w_dn, bool grad, float* dx_part, int64_t n_slices, cudaStream_t s, const char* what) {
+  const size_t x_bytes = (size_t)NT * a.D * 4, red = (size_t)WARPS * NT * 32 * W * 4;
+  const unsigned grid = (unsigned)blocks(w_dn, W > 1, a.V);
+  if (w_dn) {
+    auto* fn = grad ? columns_kernel<E, NT, W, true> : columns_kernel<E, NT, W, false>;
+    if (x_bytes + red > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(x_bytes + red));
+    fn<<<grid, T, x_bytes + red, s>>>(a);
+  } else {
+    auto* fn = grad ? words_kernel<E, NT, W, true> : words_kernel<E, NT, W, false>;
+    if (x_bytes + 1024 > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_bytes);
+    fn<<<grid, T, x_bytes, s>>>(a);
+  }
+  int rc = check_launch(what);
+  if (rc || !dx_part) return rc;
+  const int64_t per = ceil_div(ceil_div(a.V, n_slices), 4) * 4;
+  if (w_dn) dx_columns_kernel<E, NT, W><<<dim3((unsigned)ceil_div(a.D, 4 * WARPS), (unsigned)n_slices), T, 0, s>>>(a, dx_part, per);
+  else dx_words_kernel<E, NT, W><<<dim3((unsigned)ceil_div(a.D, (int64_t)T * W), (unsigned)n_slices), T, 0, s>>>(a, dx_part, per);
+  return check_launch(what);
+}
+
+static int run(int dtype, const Args& a, int w_dn, int wide, bool grad, float* dx_part, int64_t n_slices, cudaStream_t s, const char* what) {
+  if (dtype == B200_BF16)
+    return wide ? launch<__nv_bfloat16, 1, 4>(a, w_dn, grad, dx_part, n_slices, s, what)
+                : launch<__nv_bfloat16, 1, 1>(a, w_dn, grad, dx_part, n_slices, s, what);
+  switch (rounded(a.N) * 2 + wide) {
+    case 2: return launch<float, 1, 1>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 3: return launch<float, 1, 4>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 4: return launch<float, 2, 1>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 5: return launch<float, 2, 4>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 8: return launch<float, 4, 1>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 9: return launch<float, 4, 4>(a, w_dn, grad, dx_part, n_slices, s, what);
+    case 16: return launch<float, 8, 1>(a, w_dn, grad, dx_part, n_slices, s, what);
+    default: return launch<float, 8, 4>(a, w_dn, grad, dx_part, n_slices, s, what);
+  }
+}
+
+}  // namespace few
+
 // ---------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------
@@ -356,6 +771,9 @@ struct Plan {
   int64_t w_rows, w_cols; // of the stored matrix
   size_t x, w, part, picked, d, xg, acc, split, bytes;
   int64_t width;          // columns of one piece
+  bool few;               // the kernels for up to 8 tokens
+  int wide;               // their vectors of 4
+  int64_t parts, slices;
 };
 
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
@@ -398,9 +816,24 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
     at = align256(at + bytes);
     return here;
   };
+  p.few = few::fits(dtype, N, D);
+  if (p.few) {
+    p.wide = few::vectors(dtype, w, ldw, w_dn ? V : D);
+    p.parts = few::blocks(w_dn, p.wide, V);
+    p.slices = few::slices(w_dn, p.wide, D, V);
+    if (!grad) {
+      p.part = take((size_t)p.parts * N * sizeof(float2));
+      p.picked = take((size_t)N * 4);
+    } else {
+      p.d = take((size_t)N * V * 4);
+      p.split = take((size_t)p.slices * N * D * 4);
+    }
+    p.bytes = at;
+    return p;
+  }
   const size_t xb = (size_t)p.planes * N * up8(D) * 2;
-  // the forward product reads x as it is where it can; dw's operand has the ignored rows zeroed
-  if (needs_pack(dtype, x, ldx)) p.x = take(xb);
+  // forward x is read as it is where it can be; the gradient's copy has the ignored rows zeroed
+  if (!grad && needs_pack(dtype, x, ldx)) p.x = take(xb);
   if (needs_pack(dtype, w, ldw)) p.w = take((size_t)p.planes * p.w_rows * up8(p.w_cols) * 2);
   if (!grad) {
     p.part = take((size_t)ceil_div(V, p.planes > 1 && N <= 128 ? 128 : 256) * 2 * N * sizeof(float2));
@@ -500,6 +933,13 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
   cudaStream_t s = as_stream(stream);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   const int i32 = label_dtype == B200_I32;
+  if (p.few) {
+    lx::few::Args f = {x, w, labels, nullptr, nullptr, ldx, ldw, ignore_index, i32, (int)N, (int)D, (int)V,
+                       reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.picked), nullptr, nullptr};
+    if ((rc = lx::few::run(dtype, f, p.w_dn, p.wide, false, nullptr, 0, s, what))) return rc;
+    lx::lse_join_kernel<<<1, 32 * lx::JOIN, 0, s>>>(f.part, (int)p.parts, f.picked, labels, i32, ignore_index, loss, lse, N, V);
+    return check_launch(what);
+  }
   if (lx::needs_pack(dtype, x, ldx)) {
     auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.x);
     if ((rc = lx::pack(dtype, x, ldx, out, N, D, nullptr, 0, 0, s))) return rc;
@@ -547,14 +987,20 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
   B200_REQUIRE(dx || dw, "%s: no result asked for", what);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   const int i32 = label_dtype == B200_I32, bf16 = dtype == B200_BF16;
+  if (p.few) {
+    lx::few::Args f = {x, w, labels, dloss, lse, ldx, ldw, ignore_index, i32, (int)N, (int)D, (int)V,
+                       nullptr, nullptr, reinterpret_cast<float*>(ws + p.d), dw};
+    // dw is written dense: its rows too have to take vectors
+    const int wide = p.wide && reinterpret_cast<uintptr_t>(dw) % (bf16 ? 8 : 16) == 0;
+    float* part = dx ? reinterpret_cast<float*>(ws + p.split) : nullptr;
+    if ((rc = lx::few::run(dtype, f, w_dn, wide, true, part, p.slices, s, what)) || !dx) return rc;
+    lx::few::join_slices_kernel<<<(unsigned)ceil_div(N * D, 32), 1024, 0, s>>>(part, (int)p.slices, N * D, dx, bf16);
+    return check_launch(what);
+  }
   auto* xg = reinterpret_cast<__nv_bfloat16*>(ws + p.xg);
   const int64_t ldg = lx::up8(D);
-  if (dw && (rc = lx::pack(dtype, x, ldx, xg, N, D, labels, i32, ignore_index, s))) return rc;
-  if (lx::needs_pack(dtype, x, ldx)) {
-    auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.x);
-    if ((rc = lx::pack(dtype, x, ldx, out, N, D, nullptr, 0, 0, s))) return rc;
-    x = out, ldx = ldg;
-  }
+  // (their logits come out as zeros, which gives no gradient either)
+  if ((rc = lx::pack(dtype, x, ldx, xg, N, D, labels, i32, ignore_index, s))) return rc;
   if (lx::needs_pack(dtype, w, ldw)) {
     auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.w);
     if ((rc = lx::pack(dtype, w, ldw, out, p.w_rows, p.w_cols, nullptr, 0, 0, s))) return rc;
@@ -564,7 +1010,7 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
   float* acc = reinterpret_cast<float*>(ws + p.acc);
   float* split = reinterpret_cast<float*>(ws + p.split);
   tile::Operand X;
-  X.base = x, X.ld = ldx, X.plane_stride = N * ldx;
+  X.base = xg, X.ld = ldg, X.plane_stride = N * ldg;
   for (int64_t first = 0; first < V; first += p.width) {
     const int64_t width = std::min(p.width, V - first);
     const tile::Operand W = lx::w_columns(p, w, ldw, first);
@@ -590,8 +1036,8 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
       if (rc) return rc;
     }
     if (dw) {
-      tile::Operand Xm;
-      Xm.base = xg, Xm.ld = ldg, Xm.plane_stride = N * ldg, Xm.mn = 1;
+      tile::Operand Xm = X;
+      Xm.mn = 1;
       uint8_t* out = reinterpret_cast<uint8_t*>(dw) + (w_dn ? first : first * D) * size;
       rc = w_dn ? lx::product(Xm, Dm, D, width, N, p.planes, out, V, bf16, nullptr, split, s, what)
                 : lx::product(Dm, Xm, width, D, N, p.planes, out, D, bf16, nullptr, split, s, what);

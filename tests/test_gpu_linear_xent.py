@@ -1,8 +1,9 @@
 """The head's cross entropy without logits against its definition in 64 bits.
 
 Tolerances, from T = |x| |w| per logit (and the like for the gradients' sums):
-* a logit: the tensor cores add 16 products at a time to an fp32 accumulator, each addition
-  off by at most 2^-23 of the terms so far: (D / 16 + 2) 2^-23 T. fp32 operands come as
+* a logit: few tokens' logits are K / 8 + 8 fp32 additions at most, each off by 2^-24 of the
+  terms so far. Above, the tensor cores add 16 products at a time to an fp32 accumulator, each addition
+  off by at most 2^-23 of the terms so far: (D / 16 + 2) 2^-23 T (so (D / 16 + 4) 2^-23 T covers both). fp32 operands come as
   hi + lo in bf16 (each rounding at most 2^-8 of its value): lo is off by 2^-16, lo . lo is
   left out: 3 * 2^-16 T more, and three times the additions.
 * lse and loss: at most the largest logit's error (twice for the loss), plus 2^-21 for the
@@ -55,7 +56,7 @@ def inputs(n, d, v, dtype, seed=0, scale=1.5):
 
 
 def additions(k, dtype):
-    return ((k / 16 + 2) * (3 if dtype == F32 else 1)) * 2.0**-23
+    return ((k / 16 + 4) * (3 if dtype == F32 else 1)) * 2.0**-23
 
 
 def check(x, w, labels, dloss, got, ignore=-100):
@@ -81,13 +82,16 @@ def check(x, w, labels, dloss, got, ignore=-100):
     assert ((dw.double() - rdw).abs() <= tw + R.HALF_STEP[dtype] * rdw.abs()).all(), "dw"
 
 
+# up to 8 tokens of fp32 (one of bf16) in kernels of their own, fp32 products and sums, and just beyond them
+FEW = [(8, 1536, 333), (8, 1537, 77), (1, 12288, 40), (1, 12289, 40), (7, 100, 4001), (2, 173, 5000), (3, 64, 129), (4, 96, 128), (9, 96, 128),
+       (6, 40, 31), (1, 1024, 32000), (1, 172, 4097), (1, 7, 64), (1, 12292, 36)]
 SIZES = [(1, 8, 1), (1, 1, 5), (3, 16, 7), (5, 64, 300), (2, 1000, 129), (130, 72, 513), (257, 40, 1000), (128, 128, 256), (129, 33, 257),
          (600, 256, 3001), (4, 64, 20000)]
 
 
 @pytest.mark.parametrize("tied", [False, True])
 @pytest.mark.parametrize("dtype", [BF, F32])
-@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("size", SIZES + FEW)
 def test_loss_and_gradients(size, dtype, tied):
     x, w, labels, dloss = inputs(*size, dtype)
     if tied:
@@ -180,6 +184,30 @@ def test_labels_outside_set_the_device_error():
     assert not no_device_error() and loss[4] == 0 and no_device_error()
     dx, dw = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
     assert not dx[4].any() and dx[3].any() and no_device_error()
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_few_tokens_ignored_invalid_and_not_finite(dtype, tied):
+    x, w, labels, dloss = inputs(6, 72, 300, dtype)
+    w = w.t().contiguous().t() if tied else w
+    labels[:] = torch.tensor([3, -100, 299, 300, -100, 0], device="cuda")
+    x[1], x[4, 0] = float("nan"), float("inf")
+    loss, lse = op("LinearCrossEntropy", x, w, labels)
+    assert not no_device_error() and loss[1] == loss[3] == loss[4] == 0
+    dx, dw = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert no_device_error() and not dx[1].any() and not dx[3].any() and not dx[4].any()
+    kept = [0, 2, 5]
+    l2, e2 = op("LinearCrossEntropy", x[kept], w, labels[kept])
+    g2 = op("LinearCrossEntropyGrad", dloss[kept], x[kept], w, labels[kept], e2)
+    check(x[kept], w, labels[kept], dloss[kept], (l2, e2, *g2))
+    # alone or among others: the same tokens, in sums of other lengths
+    torch.testing.assert_close(loss[kept], l2, rtol=1e-5, atol=1e-5)
+    torch.testing.assert_close(dx[kept].float(), g2[0].float(), rtol=2e-2, atol=1e-6)
+    torch.testing.assert_close(dw.float(), g2[1].float(), rtol=2e-2, atol=1e-6)
+    x[0, 5] = float("nan")
+    loss, lse = op("LinearCrossEntropy", x[kept], w, labels[kept])
+    assert torch.isnan(lse[0]) and torch.isfinite(lse[1:]).all() and torch.isnan(loss[0])
 
 
 def test_large_logits_and_nan_rows():
