@@ -57,6 +57,7 @@ def close(got, ref, mag, what=""):
 @pytest.mark.parametrize("shape,part", [
     ((1, 1, 1, 2), 2), ((1, 1, 32, 128), 128), ((2, 37, 3, 64), 64), ((2, 5, 7, 80), 32), ((3, 33, 16, 96), 46),
     ((1, 17, 5, 512), 512), ((2, 9, 2, 256), 62), ((1, 300, 1, 33), 8), ((2, 4, 3, 48), 0), ((5, 1, 9, 81), 34),
+    ((2, 70, 11, 128), 62), ((1, 9, 5, 32), 14), ((1, 6, 3, 511), 510), ((2, 3, 4, 512), 254), ((1, 5, 2, 4), 2), ((1, 4, 2, 512), 510), ((1, 3, 2, 512), 506),
 ])
 def test_rotary_shapes(shape, part, dtype, interleaved, inverse):
     x = rand(*shape, dtype=dtype)
@@ -126,6 +127,7 @@ def test_rotary_empty():
 QK = [  # batch, seq, heads, kv_heads, dim, rotary_dim
     (1, 1, 1, 1, 64, 64), (32, 1, 32, 8, 128, 128), (2, 65, 4, 1, 128, 64), (3, 7, 5, 2, 80, 32), (1, 19, 3, 3, 46, 46),
     (2, 11, 2, 2, 512, 512), (4, 3, 6, 2, 33, 0), (1, 700, 8, 2, 64, 64), (2, 5, 3, 1, 256, 130),
+    (2, 30, 11, 3, 96, 46), (1, 9, 7, 2, 128, 62), (3, 5, 4, 4, 32, 14), (1, 4, 9, 2, 512, 254), (1, 3, 2, 1, 511, 510), (1, 4, 2, 1, 512, 510), (1, 2, 3, 2, 509, 508),
 ]
 
 
