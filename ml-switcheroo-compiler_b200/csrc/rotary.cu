@@ -110,21 +110,16 @@ __device__ __forceinline__ void cos_sin(uint64_t phase, float& c, float& s) {
   s = __uint_as_float(__float_as_uint(v) ^ ((quarter & 2) << 30));
 }
 
-// How a head's elements reach the lanes: one by one; in vectors of 4 that the units consist of;
-// or in vectors through shared memory, where the units (half a head of 62 elements, say) are
-// not made of them
-constexpr int ELEMENTS = 0, VECTORS = 1, STAGED = 2;
-
-// V elements as loaded: the words of one vector access (VECTORS; all there or none), or floats
-template <typename T, int V, int ACCESS>
+// V elements as loaded: the words of one vector access (FAST; all there or none), or floats
+template <typename T, int V, bool FAST>
 struct Vec {
-  static constexpr int WORDS = ACCESS == VECTORS ? V * (int)sizeof(T) / 4 : V;
+  static constexpr int WORDS = FAST ? V * (int)sizeof(T) / 4 : V;
   uint32_t w[WORDS];
 
   __device__ __forceinline__ void load(const T* p, int n) {
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) w[i] = 0u;
-    if constexpr (ACCESS != VECTORS) {
+    if constexpr (!FAST) {
 #pragma unroll
       for (int i = 0; i < V; ++i)
         if (i < n) w[i] = __float_as_uint((float)p[i]);
@@ -143,7 +138,7 @@ struct Vec {
     }
   }
   __device__ __forceinline__ f2 get(int i) const {  // elements 2 i and 2 i + 1
-    if constexpr (ACCESS == VECTORS && sizeof(T) == 2) return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    if constexpr (FAST && sizeof(T) == 2) return pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     else return pair(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
   }
 };
@@ -151,12 +146,12 @@ struct Vec {
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-template <typename T, int V, int ACCESS>
+template <typename T, int V, bool FAST>
 __device__ __forceinline__ void store_vec(T* p, const f2 (&x)[V / 2], int n) {
   float v[V];
 #pragma unroll
   for (int i = 0; i < V / 2; ++i) halves(x[i], v[2 * i], v[2 * i + 1]);
-  if constexpr (ACCESS != VECTORS) {
+  if constexpr (!FAST) {
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) put(p + i, v[i]);
@@ -173,22 +168,14 @@ __device__ __forceinline__ void store_vec(T* p, const f2 (&x)[V / 2], int n) {
   }
 }
 
-template <typename T, int V, int NU, int ACCESS>
+template <typename T, int V, int NU, bool FAST>
 struct Row {
-  Vec<T, V, ACCESS> a[NU], b[NU];
+  Vec<T, V, FAST> a[NU], b[NU];
 };
 
-// 4 elements to shared memory, asynchronously
-template <typename T>
-__device__ __forceinline__ void copy4(T* dst, const T* src) {
-  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
-  if constexpr (sizeof(T) == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(d), "l"(src) : "memory");
-}
-
-template <typename T, int V, int NU, int ACCESS, bool INTER, int MODE, int LANES>
+template <typename T, int V, int NU, bool FAST, bool INTER, int MODE, int LANES>
 __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 3 : 2)) heads_kernel(const __grid_constant__ Args A) {
-  constexpr int BATCH = NU > 1 || ACCESS == STAGED ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
+  constexpr int BATCH = NU > 1 ? 1 : (MODE == NORM_GRAD || sizeof(T) == 4 ? 2 : 4);
   constexpr int P = V / 2;  // f32x2 values per vector
   __shared__ uint64_t freq[B200_ROTARY_MAX_DIM / 2];
   const int half = A.part / 2;
@@ -238,7 +225,7 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
     const int token = A.chunks == 1 ? (int)item : (int)(item / A.chunks), chunk = (int)(item - (int64_t)token * A.chunks);
     const int bt = token / A.seq, st = token - bt * A.seq;
     const int g_begin = chunk * A.per_chunk, g_end = min(total_groups, g_begin + A.per_chunk);
-    Row<T, V, NU, ACCESS> xr[BATCH], dr[BATCH];
+    Row<T, V, NU, FAST> xr[BATCH], dr[BATCH];
     const T *xp = nullptr, *dp = nullptr;  // this lane's head of the next group to load
     int head = 0;
     // the pointers of one tensor from group g on
@@ -266,33 +253,12 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
         if constexpr (MODE == NORM_GRAD) dp += R * S.d_h;
       }
     };
-    // STAGED: group g of heads into one of the warp's two buffers, as vectors of its whole rows
-    extern __shared__ __align__(16) uint8_t staged_raw[];
-    constexpr int TENSORS = MODE == NORM_GRAD ? 2 : 1;
-    T* const staged = reinterpret_cast<T*>(staged_raw) + (int64_t)warp * 2 * TENSORS * R * A.dim;
-    const int quads = A.dim / 4;
-    auto send = [&](const Seg& S, int g, int end, int which) {
-      T* to = staged + which * TENSORS * R * A.dim;
-      const T* x = reinterpret_cast<const T*>(S.x) + bt * S.x_b + st * S.x_s + (int64_t)g * R * S.x_h;
-      const T* d = reinterpret_cast<const T*>(S.dy) + bt * S.d_b + st * S.d_s + (int64_t)g * R * S.d_h;
-      const int n = min(R, end - g * R) * quads;
-      for (int i = lane; i < n; i += 32) {
-        const int h = i / quads, e = 4 * (i - h * quads);
-        copy4(to + h * A.dim + e, x + h * S.x_h + e);
-        if constexpr (MODE == NORM_GRAD) copy4(to + (R + h) * A.dim + e, d + h * S.d_h + e);
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     const int t_first = g_begin < A.seg[0].groups ? 0 : 1;
     {
       const Seg& S = A.seg[t_first];
-      const int first = t_first ? A.seg[0].groups : 0, end = min(S.heads, (g_end - first) * R);
-      if constexpr (ACCESS == STAGED) {
-        send(S, g_begin - first, end, 0);
-      } else {
-        point(S, g_begin - first);
-        fetch(S, end);
-      }
+      const int first = t_first ? A.seg[0].groups : 0;
+      point(S, g_begin - first);
+      fetch(S, min(S.heads, (g_end - first) * R));
     }
     int64_t p = A.offset + st;
     if (A.pos) {
@@ -367,46 +333,20 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
             }
           }
       }
-      int which = 0;
-      if (t != t_first) {
-        if constexpr (ACCESS == STAGED) send(S, lo, end, 0);
-        else point(S, lo);
-      }
+      if (t != t_first) point(S, lo);
       int out = lo * R + sub;
       T* yp = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s + out * S.y_h;
       // The gradient's few warps keep the next batch's loads in flight; the other modes load
       // a batch and work on it (more warps, and more rows a batch, do as well there).
-      constexpr bool AHEAD = MODE == NORM_GRAD && NU == 1 && ACCESS != STAGED;
+      constexpr bool AHEAD = MODE == NORM_GRAD && NU == 1;
       if (AHEAD && t != t_first) fetch(S, end);
       for (int g = lo; g < hi; g += BATCH) {
-        Row<T, V, NU, ACCESS> xc[BATCH], dc[BATCH];
-        T* const rows = staged + which * TENSORS * R * A.dim;
-        T* const mine = rows + min(sub, R - 1) * A.dim;
-        if constexpr (ACCESS == STAGED) {
-          if (g + 1 < hi) {
-            send(S, g + 1, end, which ^ 1);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-          } else {
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-          }
-          __syncwarp();
+        Row<T, V, NU, FAST> xc[BATCH], dc[BATCH];
+        if (!AHEAD && (t != t_first || g != lo)) fetch(S, end);
 #pragma unroll
-          for (int k = 0; k < NU; ++k) {
-            const int n = out < end ? n0[k] : 0, m = out < end ? n1[k] : 0;
-            xc[0].a[k].load(mine + o0[k], n);
-            xc[0].b[k].load(mine + o1[k], m);
-            if constexpr (MODE == NORM_GRAD) {
-              dc[0].a[k].load(mine + R * A.dim + o0[k], n);
-              dc[0].b[k].load(mine + R * A.dim + o1[k], m);
-            }
-          }
-        } else {
-          if (!AHEAD && (t != t_first || g != lo)) fetch(S, end);
-#pragma unroll
-          for (int j = 0; j < BATCH; ++j) {
-            xc[j] = xr[j];
-            if constexpr (MODE == NORM_GRAD) dc[j] = dr[j];
-          }
+        for (int j = 0; j < BATCH; ++j) {
+          xc[j] = xr[j];
+          if constexpr (MODE == NORM_GRAD) dc[j] = dr[j];
         }
         if (AHEAD && g + BATCH < hi) fetch(S, end);
         auto work = [&](int j) {
@@ -473,11 +413,10 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
                 b[k][i] = fma2(gb[k][i], gam[1][k][i], mul2(b[k][i], m2));
               }
           }
-          T* const to = ACCESS == STAGED ? mine : yp;  // staged: over the elements that this lane alone read
 #pragma unroll
           for (int k = 0; k < NU; ++k) {
-            store_vec<T, V, ACCESS>(to + o0[k], a[k], out < end ? n0[k] : 0);
-            store_vec<T, V, ACCESS>(to + o1[k], b[k], out < end ? n1[k] : 0);
+            store_vec<T, V, FAST>(yp + o0[k], a[k], out < end ? n0[k] : 0);
+            store_vec<T, V, FAST>(yp + o1[k], b[k], out < end ? n1[k] : 0);
           }
           out += R;
           yp += R * S.y_h;
@@ -492,20 +431,6 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
             if (g + j >= hi) break;  // warp-uniform
             work(j);
           }
-        }
-        if constexpr (ACCESS == STAGED) {
-          __syncwarp();
-          T* y = reinterpret_cast<T*>(S.y) + bt * S.y_b + st * S.y_s + (int64_t)g * R * S.y_h;
-          const int n = min(R, end - g * R) * quads;
-          for (int i = lane; i < n; i += 32) {
-            const int h = i / quads, e = 4 * (i - h * quads);
-            if constexpr (sizeof(T) == 4)
-              *reinterpret_cast<uint4*>(y + h * S.y_h + e) = *reinterpret_cast<const uint4*>(rows + h * A.dim + e);
-            else
-              *reinterpret_cast<uint2*>(y + h * S.y_h + e) = *reinterpret_cast<const uint2*>(rows + h * A.dim + e);
-          }
-          __syncwarp();  // the buffer takes the group after the next one
-          which ^= 1;
         }
       }
     }
@@ -563,15 +488,10 @@ __global__ void __launch_bounds__(256) gamma_sum_kernel(const float* __restrict_
   }
 }
 
-template <typename T, int V, int NU, int ACCESS, int MODE, int LANES = 0>
+template <typename T, int V, int NU, bool FAST, int MODE, int LANES = 0>
 static int launch(const Args& a, bool inter, int grid, cudaStream_t s) {
-  auto* fn = inter ? heads_kernel<T, V, NU, ACCESS, true, MODE, LANES> : heads_kernel<T, V, NU, ACCESS, false, MODE, LANES>;
-  size_t smem = 0;
-  if (ACCESS == STAGED) {
-    smem = (size_t)WARPS * 2 * (MODE == NORM_GRAD ? 2 : 1) * (32 / a.L) * a.dim * sizeof(T);
-    if (smem > 24 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  }
-  fn<<<grid, THREADS, smem, s>>>(a);
+  if (inter) heads_kernel<T, V, NU, FAST, true, MODE, LANES><<<grid, THREADS, 0, s>>>(a);
+  else heads_kernel<T, V, NU, FAST, false, MODE, LANES><<<grid, THREADS, 0, s>>>(a);
   return check_launch(MODE == ROTATE ? "rotary" : (MODE == NORM ? "qk_norm_rotary" : "qk_norm_rotary_grad"));
 }
 
@@ -580,20 +500,20 @@ static int launch(const Args& a, bool inter, int grid, cudaStream_t s) {
 template <typename T, int MODE>
 static int launch_fast(const Args& a, bool inter, int grid, cudaStream_t s) {
   if constexpr (MODE != ROTATE) {
-    if (a.L == 8) return launch<T, 4, 1, VECTORS, MODE, 8>(a, inter, grid, s);
-    if (a.L == 16) return launch<T, 4, 1, VECTORS, MODE, 16>(a, inter, grid, s);
+    if (a.L == 8) return launch<T, 4, 1, true, MODE, 8>(a, inter, grid, s);
+    if (a.L == 16) return launch<T, 4, 1, true, MODE, 16>(a, inter, grid, s);
   }
-  return launch<T, 4, 1, VECTORS, MODE>(a, inter, grid, s);
+  return launch<T, 4, 1, true, MODE>(a, inter, grid, s);
 }
 
-// Units a lane: a head of 512 elements is 64 units of whole vectors, up to 65 where its parts
-// end inside one (254 pairs and a rest of 4), up to 129 of 2-element vectors.
+// Units a lane: a head of 512 elements is 64 units of whole vectors, or up to 129 of 2-element
+// vectors; an idle unit costs as much as a full one.
 template <typename T, int MODE>
-static int launch_type(const Args& a, int access, int nu, bool inter, int grid, cudaStream_t s) {
-  if (access == VECTORS) return nu == 1 ? launch_fast<T, MODE>(a, inter, grid, s) : launch<T, 4, 2, VECTORS, MODE>(a, inter, grid, s);
-  if (access == STAGED)
-    return nu == 1 ? launch<T, 4, 1, STAGED, MODE>(a, inter, grid, s) : launch<T, 4, 3, STAGED, MODE>(a, inter, grid, s);
-  return nu == 1 ? launch<T, 2, 1, ELEMENTS, MODE>(a, inter, grid, s) : launch<T, 2, 5, ELEMENTS, MODE>(a, inter, grid, s);
+static int launch_type(const Args& a, bool fast, int nu, bool inter, int grid, cudaStream_t s) {
+  if (fast) return nu == 1 ? launch_fast<T, MODE>(a, inter, grid, s) : launch<T, 4, 2, true, MODE>(a, inter, grid, s);
+  if (nu == 1) return launch<T, 2, 1, false, MODE>(a, inter, grid, s);
+  if (nu == 2) return launch<T, 2, 2, false, MODE>(a, inter, grid, s);
+  return nu == 3 ? launch<T, 2, 3, false, MODE>(a, inter, grid, s) : launch<T, 2, 5, false, MODE>(a, inter, grid, s);
 }
 
 static int grad_blocks() { return 2 * num_sms(); }
@@ -604,17 +524,16 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
   const int wide = 4;
   const int half = r->rotary_dim / 2, rest = r->head_dim - r->rotary_dim;
   // vectors of 4 elements when they tile the head's parts and every row starts on one's
-  // boundary; vectors through shared memory when they only tile the whole head; otherwise units
-  // of 2 elements, loaded one by one (16 x 1024 x 8 x 128 bf16, 62 rotated: STAGED_US, one by one ELEMENT_US)
-  bool tile = rest % wide == 0 && (r->interleaved ? r->rotary_dim : half) % wide == 0, rows = r->head_dim % wide == 0;
+  // boundary; otherwise units of 2 elements, loaded one by one (16 x 1024 x 8 x 128 bf16: 16 us
+  // with 64 rotated, 34 with 62; staging whole rows through shared memory took 40)
+  bool fast = rest % wide == 0 && (r->interleaved ? r->rotary_dim : half) % wide == 0;
   for (const Seg& g : a.seg) {
     if (!g.heads) continue;
     uint64_t bits = reinterpret_cast<uintptr_t>(g.x) | reinterpret_cast<uintptr_t>(g.y) | reinterpret_cast<uintptr_t>(g.dy);
     bits |= (uint64_t)(g.x_b | g.x_s | g.x_h | g.y_b | g.y_s | g.y_h | g.d_b | g.d_s | g.d_h) * (uint64_t)size;
-    if (bits & (uint64_t)(wide * size - 1)) rows = false;
+    if (bits & (uint64_t)(wide * size - 1)) fast = false;
   }
-  const int access = !rows ? ELEMENTS : (tile ? VECTORS : STAGED);
-  const int V = rows ? wide : 2;
+  const int V = fast ? wide : 2;
   a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
   a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
   a.L = 1;
@@ -635,8 +554,8 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
   const int64_t blocks = ceil_div((int64_t)a.tokens * a.chunks, WARPS);
   const int grid = (int)std::min<int64_t>(blocks, MODE == NORM_GRAD ? grad_blocks() : 16 * num_sms());
   if (blocks_out) *blocks_out = grid;
-  const bool in = r->interleaved != 0;
-  return dtype == B200_F32 ? launch_type<float, MODE>(a, access, nu, in, grid, s) : launch_type<__nv_bfloat16, MODE>(a, access, nu, in, grid, s);
+  return dtype == B200_F32 ? launch_type<float, MODE>(a, fast, nu, r->interleaved, grid, s)
+                           : launch_type<__nv_bfloat16, MODE>(a, fast, nu, r->interleaved, grid, s);
 }
 
 static int check_rotary(const char* what, const b200_rotary* r, int dtype, int64_t batch, int64_t seq, const void* pos, int pos_dtype) {
