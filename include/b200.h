@@ -593,8 +593,9 @@ int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, c
  * labels I64 / I32 [N]; rows of ignore_index get loss 0 and no gradient (and add nothing to
  * dw, whatever x holds there); another label outside [0, V) sets the device error flag,
  * with loss 0 and no gradient. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
- * dense) in the operands' dtype; either may be NULL. The workspace's size depends on the
- * pointers' alignment too: give the same ones. Results do not depend on the run. */
+ * dense) in the operands' dtype; either may be NULL. Results overlap no input. The workspace's
+ * size depends on the pointers' alignment too: give the same ones. Results do not depend on the
+ * run. Up to 8 tokens of F32, or one of BF16, run in fp32 on the CUDA cores. */
 size_t b200_linear_xent_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, int64_t N,
                                         int64_t D, int64_t V);
 int b200_linear_xent(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, const void* labels, int label_dtype,
@@ -614,7 +615,8 @@ int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t 
  *   coefficients[3 i ..]: S = X X^T, X = a X + (b S + c S S) X
  *   newton_schulz: out = X, of g's dtype (F32 or BF16)
  *   apply_muon:    m' = mu m + g; G = g + mu m' (nesterov) or m'; p' = p (1 - lr weight_decay)
- *                  - lr sqrt(max(1, rows / cols)) X. Outputs may alias param and momentum.
+ *                  - lr sqrt(max(1, rows / cols)) X. param_out may be param, momentum_out
+ *                  momentum; else nothing overlaps.
  * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums; the
  * coefficients have to keep X's entries below 250. Results do not depend on the run. */
 size_t b200_newton_schulz_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);

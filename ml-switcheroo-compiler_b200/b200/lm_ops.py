@@ -429,6 +429,8 @@ def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov
     for t in out:
         if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name}: results must be dense fp32 {tuple(p.shape)}")
+    if p.numel() and (out[0].data_ptr() in (m.data_ptr(), g.data_ptr()) or out[1].data_ptr() in (p.data_ptr(), g.data_ptr(), out[0].data_ptr())):
+        raise ValueError(f"{name}: a result may be written over its own input only (param', momentum')")
     _on_device(name, p, m, g, *out)
     wn = L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols)
     ws = torch.empty(wn, dtype=torch.uint8, device=p.device)

@@ -557,16 +557,6 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
                      const typename Epi::Args& args, cudaStream_t s, const char* what) {
   using G = Geo<BN, PAIR, SPLIT>;
   constexpr int planes = SPLIT ? 2 : 1;
-  CUtensorMap ma, mb;
-  auto map = [&](CUtensorMap* m, const Operand& o, int64_t major, int box) {
-    const uint64_t span = (uint64_t)o.ld * 2 * (uint64_t)(o.mn ? K : major);
-    const uint64_t ps = planes > 1 ? (uint64_t)o.plane_stride * 2 : span, bs = batch > 1 ? (uint64_t)o.batch_stride * 2 : ps * planes;
-    return o.mn ? make_map(m, o.base, major, K, planes, batch, o.ld * 2, ps, bs, 64, 64)
-                : make_map(m, o.base, K, major, planes, batch, o.ld * 2, ps, bs, 64, box);
-  };
-  int rc = map(&ma, A, M, BM);
-  if (!rc) rc = map(&mb, B, N, PAIR ? BN / 2 : BN);
-  if (rc) return rc;
   lp.a_mn = A.mn;
   lp.b_mn = B.mn;
   lp.nk = (int)ceil_div(K, BK);
@@ -597,6 +587,16 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
     set_error("%s: the kernel cannot be resident (registers)", what);
     return B200_ERR_CUDA;
   }
+  CUtensorMap ma, mb;
+  auto map = [&](CUtensorMap* m, const Operand& o, int64_t major, int box) {
+    const uint64_t span = (uint64_t)o.ld * 2 * (uint64_t)(o.mn ? K : major);
+    const uint64_t ps = planes > 1 ? (uint64_t)o.plane_stride * 2 : span, bs = batch > 1 ? (uint64_t)o.batch_stride * 2 : ps * planes;
+    return o.mn ? make_map(m, o.base, major, K, planes, batch, o.ld * 2, ps, bs, 64, 64)
+                : make_map(m, o.base, K, major, planes, batch, o.ld * 2, ps, bs, 64, box);
+  };
+  int rc = map(&ma, A, M, BM);
+  if (!rc) rc = map(&mb, B, N, PAIR ? BN / 2 : BN);
+  if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(size * units), 1, 1);
   cfg.blockDim = dim3(THREADS, 1, 1);

@@ -139,6 +139,13 @@ def test_apply_muon(shape, nesterov):
     assert torch.equal(pc, p2) and torch.equal(mc, m2)
 
 
+def test_apply_muon_refuses_results_over_other_inputs():
+    p, m, g = (grads(16, 24, seed=i) for i in range(3))
+    for out in ((m, p), (g, m), (p, g), (p, p), (p, torch.empty(24, 16, device="cuda")), (p.half(), m), (p, torch.empty(24, 16, device="cuda").t())):
+        with pytest.raises(ValueError, match="ApplyMuon"):
+            op("ApplyMuon", p, m, g, out=out)
+
+
 def test_muon_defaults_and_empty():
     p, m, g = torch.ones(8, 16, device="cuda"), torch.zeros(8, 16, device="cuda"), grads(8, 16)
     a = op("ApplyMuon", p, m, g)
