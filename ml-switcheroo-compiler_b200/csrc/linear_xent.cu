@@ -230,21 +230,23 @@ struct StoreEpi {
   __device__ __forceinline__ void begin(const Spot&) {}
   __device__ __forceinline__ void end(const Spot&) {}
   __device__ __forceinline__ void finish(int) {}
-  __device__ __forceinline__ void init(const Spot& sp, int64_t col, float (&v)[32]) {
-    if (a.add && sp.row < a.M) {
-      const float* p = a.add + sp.row * a.ld_add + col;
-      if (col + 32 <= a.N && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+  __device__ __forceinline__ bool dense(int64_t col) const {  // 16-byte rows of whole chunks
+    return col + 32 <= a.N && (a.ld_add & 3) == 0 && (reinterpret_cast<uintptr_t>(a.add) & 15) == 0;
+  }
+  __device__ __forceinline__ void fetch(const Spot& sp, int64_t col, float (&v)[32]) {
+    if (!a.add) return;
+    const int rows = (int)min((int64_t)32, a.M - sp.row0);
+    const float* p = a.add + sp.row0 * a.ld_add + col;
+    if (dense(col)) {
+      rows_load<4>(reinterpret_cast<const uint8_t*>(p), a.ld_add * 4, rows, 8, sp.lane, v, 0);
+    } else if (sp.lane < rows) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(p + i);
-          v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (col + i < a.N) v[i] = p[i];
-      }
+      for (int i = 0; i < 32; ++i)
+        if (col + i < a.N) v[i] = p[sp.lane * a.ld_add + i];
     }
+  }
+  __device__ __forceinline__ void ready(const Spot& sp, int64_t col, float (&v)[32]) {
+    if (a.add && dense(col)) rows_in<4>(sp.buf, sp.lane, v, 0);
   }
   __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
     const int rows = (int)min((int64_t)32, a.M - sp.row0);

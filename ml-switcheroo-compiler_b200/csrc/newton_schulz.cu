@@ -82,26 +82,44 @@ struct NsEpi {
   __device__ __forceinline__ void end(const Spot&) {}
   __device__ __forceinline__ void finish(int) {}
 
-  // what the product is added to: ca source + diag I, or fa add
-  __device__ __forceinline__ void init(const Spot& sp, int64_t col, float (&v)[32]) {
-    const int64_t cols = min((int64_t)32, a.N - col);
-    if (sp.row >= a.M) return;
+  // What the product is added to: ca source + diag I (POLY), fa add (LAST). The source arrives as
+  // its planes' 16 words each, in the chunk's own registers.
+  __device__ __forceinline__ bool dense(const Spot& sp, int64_t col) const {  // 16-byte rows of whole chunks
+    return col + 32 <= a.N && (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.add) & 15) == 0;
+  }
+  __device__ __forceinline__ void fetch(const Spot& sp, int64_t col, float (&v)[32]) {
+    const int rows = (int)min((int64_t)32, a.M - sp.row0), cols = (int)min((int64_t)32, a.N - col);
     if (a.which == POLY) {
-      const __half* p = a.src + sp.z * a.batch + sp.row * a.ld + col;
-      for (int k = 0; k < a.planes; ++k)
+      const __half* p = a.src + sp.z * a.batch + sp.row0 * a.ld + col;  // rows are padded to 8 elements
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (8 * j < cols) {  // rows are padded to 8 elements
-            const uint4 u = *reinterpret_cast<const uint4*>(p + k * a.plane + 8 * j);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      for (int k = 0; k < 2; ++k)
+        if (k < a.planes) rows_load<2>(reinterpret_cast<const uint8_t*>(p + k * a.plane), a.ld * 2, rows, (cols + 7) / 8, sp.lane, v, 16 * k);
+    } else if (a.which == LAST && a.add) {
+      const float* p = a.add + (sp.z * a.M + sp.row0) * a.N + col;
+      if (dense(sp, col)) {
+        rows_load<4>(reinterpret_cast<const uint8_t*>(p), a.N * 4, rows, 8, sp.lane, v, 0);
+      } else if (sp.lane < rows) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float x, y;
-              unpack_f16(w[i], x, y);
-              v[8 * j + 2 * i] = fmaf(ca, x, v[8 * j + 2 * i]);
-              v[8 * j + 2 * i + 1] = fmaf(ca, y, v[8 * j + 2 * i + 1]);
-            }
-          }
+        for (int i = 0; i < 32; ++i)
+          if (i < cols) v[i] = p[sp.lane * a.N + i];
+      }
+    }
+  }
+  __device__ __forceinline__ void ready(const Spot& sp, int64_t col, float (&v)[32]) {
+    if (a.which == POLY) {
+      rows_in<2>(sp.buf, sp.lane, v, 0);
+      if (a.planes > 1) rows_in<2>(sp.buf + 2048u, sp.lane, v, 16);
+      uint32_t w[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x, y, lx, ly;  // (one plane: its partner's words are zeros)
+        unpack_f16(w[i], x, y);
+        unpack_f16(w[16 + i], lx, ly);
+        v[2 * i] = ca * (x + lx);
+        v[2 * i + 1] = ca * (y + ly);
+      }
       const int k = (int)(sp.row - col);
       if (k >= 0 && k < 32) {
 #pragma unroll
@@ -109,18 +127,9 @@ struct NsEpi {
           if (k == i) v[i] += diag;
       }
     } else if (a.which == LAST && a.add) {
-      const float* p = a.add + (sp.z * a.M + sp.row) * a.N + col;
-      if (cols == 32 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      if (dense(sp, col)) rows_in<4>(sp.buf, sp.lane, v, 0);
 #pragma unroll
-        for (int i = 0; i < 32; i += 4) {
-          const float4 t = *reinterpret_cast<const float4*>(p + i);
-          v[i] = a.fa * t.x, v[i + 1] = a.fa * t.y, v[i + 2] = a.fa * t.z, v[i + 3] = a.fa * t.w;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-          if (i < cols) v[i] = a.fa * p[i];
-      }
+      for (int i = 0; i < 32; ++i) v[i] *= a.fa;
     }
   }
 

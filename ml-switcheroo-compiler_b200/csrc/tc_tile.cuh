@@ -182,6 +182,42 @@ __device__ __forceinline__ void put_chunk(uint32_t buf, int lane, uint8_t* base,
     }
 }
 
+// 32 rows of 32 ESZ bytes (16-byte aligned, `ld` bytes apart) as the lanes can load them together:
+// whole rows per instruction, so that a warp's load touches 8 (ESZ 2) or 4 lines, not 32, whose
+// lookups alone took as long as the tile's MMAs. A row per lane comes out of rows_in.
+template <int ESZ>
+__device__ __forceinline__ void rows_load(const uint8_t* base, int64_t ld, int rows, int pieces, int lane, float (&w)[32], int first) {
+  constexpr int PIECES = 2 * ESZ, PER = 32 / PIECES;
+  const int j = lane % PIECES;
+  base += (int64_t)(lane / PIECES) * ld + 16 * j;
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+    if (i * PER + lane / PIECES < rows && j < pieces) {
+      const float4 u = *reinterpret_cast<const float4*>(base + (int64_t)(i * PER) * ld);
+      w[first + 4 * i] = u.x, w[first + 4 * i + 1] = u.y, w[first + 4 * i + 2] = u.z, w[first + 4 * i + 3] = u.w;
+    }
+}
+template <int ESZ>
+__device__ __forceinline__ void rows_in(uint32_t buf, int lane, float (&w)[32], int first) {
+  constexpr int PIECES = 2 * ESZ, PER = 32 / PIECES;
+  auto at = [&](int r, int j) {
+    const int sw = ESZ == 4 ? r & 7 : ((r >> 1) ^ (r >> 3)) & 3;
+    return buf + (uint32_t)r * (32u * ESZ) + ((uint32_t)(j ^ sw) << 4);
+  };
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < PIECES; ++i)
+    st_shared_v4(at(i * PER + lane / PIECES, lane % PIECES), __float_as_uint(w[first + 4 * i]), __float_as_uint(w[first + 4 * i + 1]),
+                 __float_as_uint(w[first + 4 * i + 2]), __float_as_uint(w[first + 4 * i + 3]));
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < PIECES; ++j) {
+    const uint4 u = ld_shared_v4(at(lane, j));
+    w[first + 4 * j] = __uint_as_float(u.x), w[first + 4 * j + 1] = __uint_as_float(u.y);
+    w[first + 4 * j + 2] = __uint_as_float(u.z), w[first + 4 * j + 3] = __uint_as_float(u.w);
+  }
+}
+
 // What an epilogue warp knows about its chunk: `row` is this lane's output row, `row0` the
 // warp's first one, `buf` its staging buffer
 struct Spot {
@@ -190,8 +226,9 @@ struct Spot {
   uint32_t buf;
 };
 
-// Epi: begin(spot) once per tile, init(spot, column, values[32]) where INIT, ahead of the
-// product (result = values + scale * product), chunk(spot, column, values[32]) for each 32 columns
+// Epi: begin(spot) once per tile; where INIT, ahead of the product, fetch(spot, column,
+// values[32]) loads what ready(spot, column, values[32]) turns into what it is added to (result =
+// values + scale * product); chunk(spot, column, values[32]) for each 32 columns
 // inside the result, end(spot); finish(lane) at the end of the kernel.
 template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtensorMap& map_b, const Loop& lp, int64_t M, int64_t N,
@@ -379,8 +416,14 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
+          // every chunk's loads are issued before the first is waited for
           if constexpr (Epi::INIT)
-            if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.init(sp, col0 + c * 32, acc[c]);
+            if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.fetch(sp, col0 + c * 32, acc[c]);
+        }
+        if constexpr (Epi::INIT) {
+#pragma unroll
+          for (int c = 0; c < CH; ++c)
+            if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.ready(sp, col0 + c * 32, acc[c]);
         }
         auto add = [&](uint32_t at_col, float (&to)[32]) {
           uint32_t cur[32];
@@ -464,9 +507,10 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int i = 0; i < 32; ++i) v[i] = 0.f;
           if constexpr (Epi::INIT)
-            if (inside) epi.init(sp, col, v);
+            if (inside) epi.fetch(sp, col, v);
           tmem_wait(cur);
           if (!inside) break;
+          if constexpr (Epi::INIT) epi.ready(sp, col, v);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
             if constexpr (Epi::INIT) v[i] = fmaf(epi.scale, __uint_as_float(cur[i]), v[i]);
