@@ -24,7 +24,8 @@ _FLOATS = (torch.float32, torch.bfloat16)
 
 
 def _on_device(name: str, *tensors: torch.Tensor | None) -> None:
-    """The kernels run on the current device's stream: operands elsewhere are refused."""
+    """The kernels run on the current device's stream: operands elsewhere are refused, ahead
+    of the first kernel that would read them."""
     dev = torch.cuda.current_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
@@ -131,6 +132,7 @@ def _heads(name: str, x: torch.Tensor) -> tuple[torch.Tensor, tuple, tuple[int, 
     if len(shape) not in (3, 4):
         raise ValueError(f"{name}: heads must be [batch, seq, heads, dim] or [seq, heads, dim], got {shape}")
     if st[-1] != 1 and shape[-1] > 1:
+        _on_device(name, x)
         x = ops.contiguous(x)
         st = x.stride()
     return (x, shape, st[:3]) if len(shape) == 4 else (x, (1, *shape), (0, *st[:2]))
@@ -159,7 +161,9 @@ def _positions(name: str, positions: Any, offset: int, batch: int, seq: int) -> 
     if shape not in ((seq,), (1, seq), (batch, seq)):
         raise ValueError(f"{name}: positions {shape} do not match {batch} sequences of {seq} tokens")
     if not t.is_cuda or (t.dtype != torch.int64 and t.dtype != torch.int32):
-        t = ops._int_indices(ops.to_device(t))
+        t = ops.to_device(t)
+        _on_device(name, t)
+        t = ops._int_indices(t)
     st = t.stride()
     return t, (t.data_ptr(), L.I64 if t.dtype == torch.int64 else L.I32, st[0] if len(shape) == 2 and shape[0] > 1 else 0, st[-1], 0)
 
@@ -209,6 +213,7 @@ def _gammas(name: str, dim: int, gq: torch.Tensor | None, gk: torch.Tensor | Non
                 raise ValueError(f"{name}: norm weight {tuple(g.shape)}, want [{dim}]")
             if g.dtype not in _FLOATS:
                 raise BackendNotSupportedError(f"{name}: norm weights of {g.dtype} (fp32 and bf16)")
+            _on_device(name, g)
             g = ops.contiguous(g)
         out.append(g)
     if gq is not None and gk is not None and gq.dtype != gk.dtype:
@@ -287,11 +292,13 @@ def _head(name: str, x: torch.Tensor, w: torch.Tensor, labels: Any):
     D, V = ws
     if D < 1 or V < 1:
         raise ValueError(f"{name}: w {ws} has no features or no words")
-    if not isinstance(labels, torch.Tensor) or not labels.is_cuda or labels.dtype not in (torch.int64, torch.int32):
-        labels = ops._int_indices(labels)
+    if not isinstance(labels, torch.Tensor):
+        labels = ops.to_device(labels)
     if tuple(labels.shape) not in (xs[:-1], (*xs[:-1], 1)):
         raise ValueError(f"{name}: labels {tuple(labels.shape)} of x {xs}")
     _on_device(name, x, w, labels)
+    if labels.dtype != torch.int32:
+        labels = ops._int_indices(labels)
     policy = ops.Config.matmul_dtype
     if x.dtype != w.dtype or (policy == "bf16" and x.dtype == torch.float32):
         # the contraction policy of Matmul: bf16 operands, or fp32 where either is
@@ -419,24 +426,28 @@ def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov
     inputs themselves for a step in place)."""
     name = "ApplyMuon"
     lr = 0.02 if lr is None else float(lr)
-    p, m, g = (ops.contiguous(ops.cast(t, torch.float32)) for t in (param, momentum_buffer, grad))
-    batch, rows, cols = _matrices(name, p)
-    if m.shape != p.shape or g.shape != p.shape:
-        raise ValueError(f"{name}: param, momentum and grad must have one shape, got {tuple(p.shape)}, {tuple(m.shape)}, {tuple(g.shape)}")
+    batch, rows, cols = _matrices(name, param)
+    if momentum_buffer.shape != param.shape or grad.shape != param.shape:
+        raise ValueError(f"{name}: param, momentum and grad must have one shape, got {tuple(param.shape)}, "
+                         f"{tuple(momentum_buffer.shape)}, {tuple(grad.shape)}")
     coef = _coef(steps, coefficients)
+    _on_device(name, param, momentum_buffer, grad, *(out or ()))
+    p, m, g = (ops.contiguous(ops.cast(t, torch.float32)) for t in (param, momentum_buffer, grad))
     if out is None:
         out = (torch.empty_like(p), torch.empty_like(m))
+    po, mo = out
     for t in out:
         if t.shape != p.shape or t.dtype != torch.float32 or not t.is_contiguous():
             raise ValueError(f"{name}: results must be dense fp32 {tuple(p.shape)}")
-    if p.numel() and (out[0].data_ptr() in (m.data_ptr(), g.data_ptr()) or out[1].data_ptr() in (p.data_ptr(), g.data_ptr(), out[0].data_ptr())):
+    apart = [(po, t) for t in (m, g, mo)] + [(mo, t) for t in (p, g)]
+    apart += [(o, t) for o, t in ((po, p), (mo, m)) if o.data_ptr() != t.data_ptr()]
+    if any(abs(o.data_ptr() - t.data_ptr()) < 4 * p.numel() for o, t in apart):
         raise ValueError(f"{name}: a result may be written over its own input only (param', momentum')")
-    _on_device(name, p, m, g, *out)
     wn = L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols)
     ws = torch.empty(wn, dtype=torch.uint8, device=p.device)
-    L.call("b200_apply_muon_f32", p.data_ptr(), m.data_ptr(), g.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), batch, rows, cols, lr,
+    L.call("b200_apply_muon_f32", p.data_ptr(), m.data_ptr(), g.data_ptr(), po.data_ptr(), mo.data_ptr(), batch, rows, cols, lr,
            float(momentum), int(bool(nesterov)), float(weight_decay), coef, int(steps), float(eps), ws.data_ptr(), wn, ops.stream_ptr())
-    return tuple(out)
+    return po, mo
 
 
 def register(table: dict) -> None:
