@@ -594,8 +594,8 @@ int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, c
  * dw, whatever x holds there); another label outside [0, V) sets the device error flag,
  * with loss 0 and no gradient. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
  * dense) in the operands' dtype; either may be NULL. Results overlap no input. The workspace's
- * size depends on the pointers' alignment too: give the same ones. Results do not depend on the
- * run. Up to 8 tokens of F32, or one of BF16, run in fp32 on the CUDA cores. */
+ * size depends on the pointers' alignment too: give the same ones; it starts on a 256-byte
+ * boundary. Results do not depend on the run. Up to 8 tokens of F32, or one of BF16, run in fp32 on the CUDA cores. */
 size_t b200_linear_xent_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, int64_t N,
                                         int64_t D, int64_t V);
 int b200_linear_xent(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, const void* labels, int label_dtype,
@@ -622,7 +622,7 @@ int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t 
 size_t b200_newton_schulz_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
 int b200_newton_schulz(int dtype, const void* g, void* out, int64_t batch, int64_t rows, int64_t cols, const float* coefficients,
                        int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
-/* workspace >= b200_newton_schulz_workspace_bytes(B200_F32, ...) */
+/* workspace >= b200_newton_schulz_workspace_bytes(B200_F32, ...); 256-byte aligned, both */
 int b200_apply_muon_f32(const float* param, const float* momentum, const float* grad, float* param_out, float* momentum_out,
                         int64_t batch, int64_t rows, int64_t cols, float lr, float mu, int nesterov, float weight_decay,
                         const float* coefficients, int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);

@@ -881,7 +881,8 @@ static int check(const char* what, int dtype, const void* x, int64_t ldx, const 
   B200_REQUIRE(N == 0 || (x && labels), "%s: null tensor", what);
   B200_REQUIRE(w, "%s: null weight", what);
   B200_REQUIRE(ldx >= D && ldw >= (w_dn ? V : D), "%s: row stride below the row", what);
-  B200_REQUIRE(ws_bytes >= need && (need == 0 || ws), "%s: workspace of %zu bytes, %zu needed", what, ws_bytes, need);
+  B200_REQUIRE(need == 0 || (ws && ws_bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255) == 0),
+               "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, ws_bytes, need);
   return B200_OK;
 }
 

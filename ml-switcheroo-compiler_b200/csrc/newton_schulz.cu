@@ -301,7 +301,10 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
   const double norm = sqrt(s), share = norm / (norm + (double)eps);
   const int e = share > 0.0 && share < 0.5 ? min(96, -1 - ilogb(share)) : 0;  // t share in [1/2, 1)
   if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e;
-  const float scale = (float)(ldexp((double)SCALE, e) / (norm + (double)eps));
+  // the factor as two, each within fp32's normal range for any norm of fp32 values
+  const double full = ldexp((double)SCALE, e) / (norm + (double)eps);
+  const int lg = full > 0.0 && full < 1e300 ? ilogb(full) / 2 : 0;
+  const float lift = ldexpf(1.f, lg), scale = (float)ldexp(full, -lg);
   const int64_t base = (int64_t)blockIdx.y * rows * cols, per = ld / 8;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * NT) {
     const int64_t r = i / per, c = i % per * 8, at = base + r * cols + c;
@@ -315,7 +318,9 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
     }
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j] * scale, v[2 * j + 1] * scale);
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * lift * scale;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j], v[2 * j + 1]);
     __half* d = x + (int64_t)blockIdx.y * batch + r * ld + c;
     *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
     if (planes > 1) {
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
       for (int j = 0; j < 4; ++j) {
         float a, b;
         unpack_f16(w[j], a, b);
-        w[j] = pack_f16(v[2 * j] * scale - a, v[2 * j + 1] * scale - b);
+        w[j] = pack_f16(v[2 * j] - a, v[2 * j + 1] - b);
       }
       *reinterpret_cast<uint4*>(d + plane) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -454,7 +459,8 @@ static int check(const char* what, int64_t batch, int64_t rows, int64_t cols, co
                (long long)batch, (long long)rows, (long long)cols);
   B200_REQUIRE(coef && steps >= 1 && steps <= 100, "%s: %d steps not in [1, 100], or no coefficients", what, steps);
   B200_REQUIRE(eps >= 0.f, "%s: eps %g is negative", what, (double)eps);
-  B200_REQUIRE(need == 0 || (ws && bytes >= need), "%s: workspace of %zu bytes, %zu needed", what, bytes, need);
+  B200_REQUIRE(need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255) == 0),
+               "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, bytes, need);
   return B200_OK;
 }
 

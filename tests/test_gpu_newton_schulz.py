@@ -119,6 +119,15 @@ def test_extreme_spectra_stay_finite_and_near():
         assert off(op("NewtonSchulz", g.to(BF)), R.newton_schulz(g.to(BF).double())) <= 5e-2
 
 
+@pytest.mark.parametrize("dtype,power", [(F32, -140), (F32, -126), (F32, -100), (F32, 100), (F32, 124), (BF, -120), (BF, -100), (BF, 124)])
+def test_norms_beyond_fp32s_reciprocals(power, dtype):
+    """1 / |g| or |g| itself outside fp32's normal range, eps = 0: the answer is g's times a power of two."""
+    g = grads(70, 90)
+    g = (g.double() / g.abs().max() * 2.0 ** (power + 3)).to(dtype)
+    got = op("NewtonSchulz", g, eps=0.0)
+    assert off(got, R.newton_schulz(g.double(), eps=0.0)) <= BOUND[dtype]
+
+
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("shape", [(40, 24), (24, 40), (4, 256, 256), (1, 130), (1100, 300)])
 def test_apply_muon(shape, nesterov):
@@ -144,6 +153,19 @@ def test_apply_muon_refuses_results_over_other_inputs():
     for out in ((m, p), (g, m), (p, g), (p, p), (p, torch.empty(24, 16, device="cuda")), (p.half(), m), (p, torch.empty(24, 16, device="cuda").t())):
         with pytest.raises(ValueError, match="ApplyMuon"):
             op("ApplyMuon", p, m, g, out=out)
+
+
+def test_apply_muon_refuses_partial_overlaps():
+    both = torch.zeros(3, 16, 24, device="cuda")
+    flat = both.view(-1)
+    g = grads(16, 24)
+    n = 16 * 24
+    ahead = flat[24 : 24 + n].view(16, 24)
+    for out in ((ahead, both[2]), (both[0], flat[2 * n - 24 : 3 * n - 24].view(16, 24)), (both[2], ahead)):
+        with pytest.raises(ValueError, match="own input only"):
+            op("ApplyMuon", both[0], both[2], g, out=out)
+    p, m = op("ApplyMuon", both[0], both[2], g, out=(both[0], both[1]))
+    assert p.data_ptr() == both[0].data_ptr() and torch.equal(both[1], g) and m is not None
 
 
 def test_muon_defaults_and_empty():

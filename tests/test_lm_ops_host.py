@@ -110,6 +110,46 @@ def test_newton_schulz_refusals():
         lm_ops.op_apply_muon(torch.zeros(4, 4), torch.zeros(4, 4), torch.zeros(4, 5))
 
 
+def test_operands_on_another_device_reach_no_kernel(monkeypatch):
+    """Host tensors stand in for another GPU's: refused before a cast, a copy or a kernel runs."""
+    def launched(*_):
+        raise AssertionError("a kernel was launched")
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(L, "call", launched)
+    monkeypatch.setattr(lm_ops.ops.Prog, "run", launched)
+    monkeypatch.setattr(lm_ops.ops, "to_device", lambda t, *_: t)
+    q, k, b16 = torch.zeros(2, 4, 6, 64), torch.zeros(2, 4, 2, 64), torch.bfloat16
+    turned = torch.zeros(2, 4, 64, 6).transpose(2, 3)  # needs a dense copy
+    x, w, y = torch.zeros(5, 16), torch.zeros(16, 30), torch.zeros(5, dtype=torch.int64)
+    m = torch.zeros(8, 12)
+    calls = [
+        lambda: lm_ops.op_rotary_embedding(q),
+        lambda: lm_ops.op_rotary_embedding(turned),
+        lambda: lm_ops.op_rotary_embedding(q, torch.zeros(4, dtype=torch.int16)),
+        lambda: lm_ops.op_rotary_embedding(q, torch.zeros(4, dtype=torch.int32)),
+        lambda: lm_ops.op_rotary_embedding_grad(turned),
+        lambda: lm_ops.op_qk_norm_rotary(q, k),
+        lambda: lm_ops.op_qk_norm_rotary(turned, k),
+        lambda: lm_ops.op_qk_norm_rotary(q, k, torch.ones(64), torch.ones(64, dtype=b16)),
+        lambda: lm_ops.op_qk_norm_rotary(q, k, torch.ones(128)[::2]),
+        lambda: lm_ops.op_qk_norm_rotary_grad(turned, k, q, k),
+        *[lambda d=d: lm_ops.op_linear_cross_entropy(x, w, y.to(d)) for d in (torch.int64, torch.int32, torch.int16, torch.uint8)],
+        lambda: lm_ops.op_linear_cross_entropy(x.to(b16), w, y),
+        lambda: lm_ops.op_linear_cross_entropy(x[:, ::2], w[::2], y),
+        lambda: lm_ops.op_linear_cross_entropy_grad(torch.zeros(5, dtype=b16), x, w, y, torch.zeros(5)),
+        lambda: lm_ops.op_newton_schulz(m),
+        lambda: lm_ops.op_newton_schulz(m.t()),
+        lambda: lm_ops.op_apply_muon(m, m, m),
+        lambda: lm_ops.op_apply_muon(m.to(b16), m, m.to(b16)),
+        lambda: lm_ops.op_apply_muon(m, m, m.t().contiguous().t()),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match="current device"):
+            call()
+            raise AssertionError(i)
+
+
 P = 256  # a stand-in address: the calls below are refused before anything reads it
 
 
@@ -150,7 +190,7 @@ def test_c_refusals_linear_xent():
         return L.lib().b200_linear_xent_grad(L.F32, dloss, P, 64, P, 104, 1, P, L.I64, -100, P, dx, dw, 4, 64, V, P,
                                              n if bytes_ is None else bytes_, None)
 
-    for kw in ({"x": None}, {"w": None}, {"labels": None}, {"loss": None}, {"N": -1}, {"D": 0}, {"V": 0}, {"ldx": 63}, {"ldw": 99}, {"ws": None},
+    for kw in ({"x": None}, {"w": None}, {"labels": None}, {"loss": None}, {"N": -1}, {"D": 0}, {"V": 0}, {"ldx": 63}, {"ldw": 99}, {"ws": None}, {"ws": P + 16},
                {"bytes_": 8}, {"N": 1 << 30}):
         assert loss(**kw) == L.ERR_ARG, kw
     assert loss(dtype=L.I32) == L.ERR_DTYPE and loss(ldt=L.F32) == L.ERR_DTYPE
@@ -166,7 +206,7 @@ def test_c_refusals_newton_schulz():
         return L.lib().b200_newton_schulz(dtype, g, P, batch, rows, cols, coef, steps, eps, ws, n if bytes_ is None else bytes_, None)
 
     for kw in ({"g": None}, {"batch": -1}, {"batch": 1 << 16}, {"rows": 1 << 24}, {"steps": 0}, {"steps": 101}, {"eps": -1.0}, {"coef": None},
-               {"ws": None}, {"bytes_": 64}):
+               {"ws": None}, {"ws": P + 16}, {"bytes_": 64}):
         assert ns(**kw) == L.ERR_ARG, kw
     assert ns(dtype=L.I32) == L.ERR_DTYPE and ns(rows=0, g=None, ws=None) == L.OK
     assert L.lib().b200_apply_muon_f32(P, None, P, P, P, 1, 64, 64, 0.1, 0.9, 1, 0.0, c, 5, 0.0, P, 1 << 30, None) == L.ERR_ARG
