@@ -62,19 +62,23 @@ struct NsEpi {
     int which;                   // GRAM, POLY, NEXT, LAST
   };
   static constexpr bool SINGLE_WIDE = false, SINGLE_NARROW = true, TEAMS = true, INIT = true;
-  const Args& a;
+  const Args* a;
+  __half* dst;
   float scale, ca, diag;
-  __device__ explicit NsEpi(const Args& args) : a(args) {}
+  __device__ explicit NsEpi(const Args& args) : a(&args), dst(args.dst) {}
   __device__ __forceinline__ void begin(const Spot& sp) {
-    scale = a.cc, ca = a.ca, diag = a.diag;
-    const int e0 = a.e0[sp.z];
+    scale = a->cc, ca = a->ca, diag = a->diag;
+    shrunk(a->e0[sp.z], a->e_down, a->e_down_next);
+  }
+  // the coefficients where t is not 1
+  __device__ __forceinline__ void shrunk(int e0, int e_down, int e_down_next) {
     if (e0 != 0) {
-      const int e = max(0, e0 - a.e_down), shrink = max(0, e0 - a.e_down_next) - e;
-      if (a.which == POLY) {
+      const int e = max(0, e0 - e_down), shrink = max(0, e0 - e_down_next) - e;
+      if (a->which == POLY) {
         ca = ldexpf(ca, shrink - 2 * e);
         scale = ldexpf(scale, shrink - 4 * e);
         diag = ldexpf(diag, shrink);
-      } else if (a.which == LAST) {
+      } else if (a->which == LAST) {
         scale = ldexpf(scale, -e);
       }
     }
@@ -85,30 +89,30 @@ struct NsEpi {
   // What the product is added to: ca source + diag I (POLY), fa add (LAST). The source arrives as
   // its planes' 16 words each, in the chunk's own registers.
   __device__ __forceinline__ bool dense(const Spot& sp, int64_t col) const {  // 16-byte rows of whole chunks
-    return col + 32 <= a.N && (a.N & 3) == 0 && (reinterpret_cast<uintptr_t>(a.add) & 15) == 0;
+    return col + 32 <= a->N && (a->N & 3) == 0 && (reinterpret_cast<uintptr_t>(a->add) & 15) == 0;
   }
   __device__ __forceinline__ void fetch(const Spot& sp, int64_t col, float (&v)[32]) {
-    const int rows = (int)min((int64_t)32, a.M - sp.row0), cols = (int)min((int64_t)32, a.N - col);
-    if (a.which == POLY) {
-      const __half* p = a.src + sp.z * a.batch + sp.row0 * a.ld + col;  // rows are padded to 8 elements
+    const int rows = (int)min((int64_t)32, a->M - sp.row0), cols = (int)min((int64_t)32, a->N - col);
+    if (a->which == POLY) {
+      const __half* p = a->src + sp.z * a->batch + sp.row0 * a->ld + col;  // rows are padded to 8 elements
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        if (k < a.planes) rows_load<2>(reinterpret_cast<const uint8_t*>(p + k * a.plane), a.ld * 2, rows, (cols + 7) / 8, sp.lane, v, 16 * k);
-    } else if (a.which == LAST && a.add) {
-      const float* p = a.add + (sp.z * a.M + sp.row0) * a.N + col;
+        if (k < a->planes) rows_load<2>(reinterpret_cast<const uint8_t*>(p + k * a->plane), a->ld * 2, rows, (cols + 7) / 8, sp.lane, v, 16 * k);
+    } else if (a->which == LAST && a->add) {
+      const float* p = a->add + (sp.z * a->M + sp.row0) * a->N + col;
       if (dense(sp, col)) {
-        rows_load<4>(reinterpret_cast<const uint8_t*>(p), a.N * 4, rows, 8, sp.lane, v, 0);
+        rows_load<4>(reinterpret_cast<const uint8_t*>(p), a->N * 4, rows, 8, sp.lane, v, 0);
       } else if (sp.lane < rows) {
 #pragma unroll
         for (int i = 0; i < 32; ++i)
-          if (i < cols) v[i] = p[sp.lane * a.N + i];
+          if (i < cols) v[i] = p[sp.lane * a->N + i];
       }
     }
   }
   __device__ __forceinline__ void ready(const Spot& sp, int64_t col, float (&v)[32]) {
-    if (a.which == POLY) {
+    if (a->which == POLY) {
       rows_in<2>(sp.buf, sp.lane, v, 0);
-      if (a.planes > 1) rows_in<2>(sp.buf + 2048u, sp.lane, v, 16);
+      if (a->planes > 1) rows_in<2>(sp.buf + 2048u, sp.lane, v, 16);
       uint32_t w[32];
 #pragma unroll
       for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
@@ -126,33 +130,33 @@ struct NsEpi {
         for (int i = 0; i < 32; ++i)
           if (k == i) v[i] += diag;
       }
-    } else if (a.which == LAST && a.add) {
+    } else if (a->which == LAST && a->add) {
       if (dense(sp, col)) rows_in<4>(sp.buf, sp.lane, v, 0);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) v[i] *= a.fa;
+      for (int i = 0; i < 32; ++i) v[i] *= a->fa;
     }
   }
 
   __device__ __forceinline__ void chunk(const Spot& sp, int64_t col, float (&v)[32]) {
-    const int rows = (int)min((int64_t)32, a.M - sp.row0);
-    const int64_t cols = min((int64_t)32, a.N - col);
-    if (a.which == LAST) {
-      const int64_t at = (sp.z * a.M + sp.row0) * a.N + col;
+    const int rows = (int)min((int64_t)32, a->M - sp.row0);
+    const int64_t cols = min((int64_t)32, a->N - col);
+    if (a->which == LAST) {
+      const int64_t at = (sp.z * a->M + sp.row0) * a->N + col;
       __syncwarp();
-      if (a.bf16) {
+      if (a->bf16) {
         uint32_t w[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) w[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
         stage_chunk<2>(sp.buf, sp.lane, w);
         __syncwarp();
-        put_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a.out) + at), a.N, rows, (int)cols);
+        put_chunk<2>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<__nv_bfloat16*>(a->out) + at), a->N, rows, (int)cols);
       } else {
         uint32_t w[32];
 #pragma unroll
         for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i]);
         stage_chunk<4>(sp.buf, sp.lane, w);
         __syncwarp();
-        put_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a.out) + at), a.N, rows, (int)cols);
+        put_chunk<4>(sp.buf, sp.lane, reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(a->out) + at), a->N, rows, (int)cols);
       }
       return;
     }
@@ -160,9 +164,9 @@ struct NsEpi {
     // (row / 2) ^ (row / 8): rows written and read, and 8 x 8 blocks read transposed, are then free
     // of bank conflicts. Rows leave as 64 adjacent bytes each way.
     const int lane = sp.lane;
-    const bool mirror = a.mirror && sp.mt != sp.nt;
-    for (int k = 0; k < a.planes; ++k) {
-      __half* d = a.dst + sp.z * a.batch + k * a.plane;
+    const bool mirror = a->mirror && sp.mt != sp.nt;
+    for (int k = 0; k < a->planes; ++k) {
+      __half* d = dst + sp.z * a->batch + k * a->plane;
       const uint32_t buf = sp.buf + (uint32_t)(k & 1) * 2048u;
       uint32_t w[16];
 #pragma unroll
@@ -181,10 +185,10 @@ struct NsEpi {
         const int r = 8 * i + (lane >> 2);
         u[i] = ld_shared_v4(buf + (uint32_t)r * 64u + (((uint32_t)piece ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4));
       }
-      __half* row = d + (sp.row0 + (lane >> 2)) * a.ld + col + 8 * piece;
+      __half* row = d + (sp.row0 + (lane >> 2)) * a->ld + col + 8 * piece;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (8 * i + (lane >> 2) < rows && 8 * piece < cols) *reinterpret_cast<uint4*>(row + 8 * i * a.ld) = u[i];
+        if (8 * i + (lane >> 2) < rows && 8 * piece < cols) *reinterpret_cast<uint4*>(row + 8 * i * a->ld) = u[i];
       if (mirror) {
         // four 8 x 8 blocks transposed: block m's rows are 8 c/2 + 2 m + c%2 (c = 0..7), so that
         // thread l ends up with rows 8 (l % 4) .. + 7 of source column 8 g + l / 4
@@ -196,12 +200,12 @@ struct NsEpi {
                        : "r"(buf + (uint32_t)r * 64u + (((uint32_t)g ^ (((r >> 1) ^ (r >> 3)) & 3u)) << 4))
                        : "memory");
         // the mirrored rows are as long as the result: whole pieces up to the padding
-        row = d + (col + (lane >> 2)) * a.ld + sp.row0 + 8 * piece;
+        row = d + (col + (lane >> 2)) * a->ld + sp.row0 + 8 * piece;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (8 * g + (lane >> 2) < cols && 8 * piece < rows) *reinterpret_cast<uint4*>(row + 8 * g * a.ld) = u[g];
+          if (8 * g + (lane >> 2) < cols && 8 * piece < rows) *reinterpret_cast<uint4*>(row + 8 * g * a->ld) = u[g];
       }
-      if (k + 1 < a.planes) {
+      if (k + 1 < a->planes) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
           float x, y;
@@ -213,6 +217,130 @@ struct NsEpi {
     }
   }
 };
+
+// ---- all products of all steps in one launch ----
+// Where the products fill the CTA pairs, each one's last wave of tiles is partial (16 matrices of
+// 1024 x 1024: 160, 160 and 256 tiles for 74 pairs, 10 waves for 7.8) and each launch fills and
+// drains its pipeline. So all tiles of all products form one list, walked by the pairs in
+// turn. A tile waits until its matrix's previous product is complete: counters in the
+// workspace, one per matrix, of the warps that have finished a tile. Every tile depends on
+// earlier ones of the list only, and the launch is cooperative, so the first unfinished
+// tile never waits. What a matrix's buffers hold is overwritten two products after
+// their last reader at the earliest, which the same counter orders.
+constexpr int MAX_STEPS = 100, ARRIVALS = 2 * EPI_WARPS;  // of a tile
+
+struct Chain {
+  static constexpr bool CHAIN = true;
+  struct One {
+    int64_t M, N;
+    int nk, chunk, a_mn, b_mn, tiles_m, tiles_n, walk, per;  // per: tiles of one matrix
+  };
+  CUtensorMap x_gram[2], s, p, x_next[2];
+  One one[3];  // GRAM, POLY, NEXT
+  int* done;   // [batch]
+  int batch, steps, tall;
+  __device__ __forceinline__ int total() const { return steps * batch * (one[0].per + one[1].per + one[2].per); }
+  __device__ __forceinline__ Tile at(int t) const {
+    Tile r = kind(t);
+    t -= r.step * batch * (one[0].per + one[1].per + one[2].per);
+    if (r.product > 0) t -= batch * one[0].per;
+    if (r.product > 1) t -= batch * one[1].per;
+    const One& o = one[r.product];
+    r.z = t / o.per;
+    place(r, t % o.per, o.walk, o.tiles_m, o.tiles_n, 16);
+    return r;
+  }
+  __device__ __forceinline__ Tile kind(int t) const {
+    const int a = batch * one[0].per, b = batch * one[1].per, c = batch * one[2].per;
+    Tile r = {};
+    r.step = t / (a + b + c);
+    t %= a + b + c;
+    r.product = t < a ? GRAM : (t < a + b ? POLY : NEXT);
+    return r;
+  }
+  __device__ __forceinline__ int blocks(const Tile& t) const { return one[t.product].nk; }
+  __device__ __forceinline__ int blocks_each(const Tile& t) const { return one[t.product].nk; }
+  __device__ __forceinline__ int chunk(const Tile& t) const { return one[t.product].chunk; }
+  __device__ __forceinline__ int a_mn(const Tile& t) const { return one[t.product].a_mn; }
+  __device__ __forceinline__ int b_mn(const Tile& t) const { return one[t.product].b_mn; }
+  __device__ __forceinline__ int64_t rows(const Tile& t) const { return one[t.product].M; }
+  __device__ __forceinline__ int64_t cols(const Tile& t) const { return one[t.product].N; }
+  __device__ __forceinline__ const CUtensorMap* map_a(const Tile& t) const {
+    return t.product == GRAM ? &x_gram[t.step & 1] : (t.product == POLY ? &s : (tall ? &x_next[t.step & 1] : &p));
+  }
+  __device__ __forceinline__ const CUtensorMap* map_b(const Tile& t) const {
+    return t.product == GRAM ? &x_gram[t.step & 1] : (t.product == POLY ? &s : (tall ? &p : &x_next[t.step & 1]));
+  }
+  __device__ __forceinline__ void prefetch() const {
+    for (const CUtensorMap* m : {&x_gram[0], &s, &p, &x_next[0]})
+      asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+  }
+  // true once the tile's matrix has seen every product before this one (by one thread); false
+  // (and the device error flag set) if that takes too long
+  __device__ __forceinline__ bool ready(const Tile& t) const {
+    int need = t.step * (one[0].per + one[1].per + one[2].per);
+    if (t.product > 0) need += one[0].per;
+    if (t.product > 1) need += one[1].per;
+    need *= ARRIVALS;
+    unsigned long long t0 = 0;
+    while (true) {
+      int v;
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done + t.z) : "memory");
+      if (v >= need) break;
+      if (t0 == 0) t0 = globaltimer();
+      if (globaltimer() - t0 > WAIT_LIMIT_NS) {
+        raise_device_error(B200_ERR_TIMEOUT);
+        return false;
+      }
+      __nanosleep(64);
+    }
+    asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads next
+    return true;
+  }
+};
+
+struct ChainEpi : NsEpi {
+  struct Step {
+    float ca, cc, diag;
+    int e_down, e_down_next;
+  };
+  struct Args {
+    NsEpi::Args part[4];  // GRAM, POLY, NEXT, LAST
+    Step step[MAX_STEPS];
+    __half* x[2];
+    int* done;
+    int steps;
+  };
+  const Args& all;
+  __device__ explicit ChainEpi(const Args& args) : NsEpi(args.part[0]), all(args) {}
+  __device__ __forceinline__ bool enter(const Chain& work, const Tile& t, const Spot& sp) {
+    const bool last = t.product == NEXT && t.step + 1 == all.steps;
+    a = &all.part[last ? LAST : t.product];
+    dst = t.product == NEXT ? all.x[(t.step + 1) & 1] : a->dst;
+    scale = a->cc;
+    const Step& st = all.step[t.step];
+    if (t.product == POLY) ca = st.ca, scale = st.cc, diag = st.diag;
+    shrunk(a->e0[sp.z], st.e_down, st.e_down_next);
+    if (t.product != POLY) return true;
+    const bool ok = sp.lane != 0 || work.ready(t);  // S is read here
+    return __all_sync(0xffffffffu, ok);
+  }
+  __device__ __forceinline__ void end(const Spot& sp) {
+    if (a->which == LAST) return;
+    asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what was written here
+    __syncwarp();
+    if (sp.lane == 0) {
+      __threadfence();
+      asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(all.done + sp.z) : "memory");
+    }
+  }
+};
+
+template <bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1) chain_kernel(const __grid_constant__ Chain chain, const __grid_constant__ ChainEpi::Args args) {
+  ChainEpi epi(args);
+  run_tiles<256, true, SPLIT, false>(chain, 1, false, epi);
+}
 
 // 8 values from element i on (the first n of them; the rest zeros): 16-byte loads where all 8
 // are there and aligned
@@ -287,7 +415,7 @@ __global__ void __launch_bounds__(NT) square_kernel(const void* g, int bf16, con
 
 // X0 = 2^8 t G / (|G| + eps) as fp16 planes with rows padded to 8 elements; t's exponent
 __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, const float* mom, float mu, int nesterov, const double* part,
-                                                   int parts, float eps, int* e0, __half* x, int64_t ld, int64_t plane, int64_t batch,
+                                                   int parts, float eps, int* e0, int* done, __half* x, int64_t ld, int64_t plane, int64_t batch,
                                                    int planes, int64_t rows, int64_t cols) {
   __shared__ double red[NT / 32];
   double s = 0.0;
@@ -300,7 +428,7 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
   for (int i = 1; i < NT / 32; ++i) s += red[i];
   const double norm = sqrt(s), share = norm / (norm + (double)eps);
   const int e = share > 0.0 && share < 0.5 ? min(96, -1 - ilogb(share)) : 0;  // t share in [1/2, 1)
-  if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e;
+  if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e, done[blockIdx.y] = 0;
   // the factor as two, each within fp32's normal range for any norm of fp32 values
   const double full = ldexp((double)SCALE, e) / (norm + (double)eps);
   const int lg = full > 0.0 && full < 1e300 ? ilogb(full) / 2 : 0;
@@ -341,7 +469,7 @@ static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 struct Plan {
   int planes;
   int64_t side, ldx, ldg, xn, gn;  // shorter side; row strides and sizes of one X and one Gram plane
-  size_t x0, x1, s, p, part, e0, bytes;
+  size_t x0, x1, s, p, part, e0, done, bytes;
 };
 
 static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
@@ -362,6 +490,7 @@ static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
   q.x0 = take(xb), q.x1 = take(xb), q.s = take(gb), q.p = take(gb);
   q.part = take((size_t)batch * NORM_BLOCKS * 8);
   q.e0 = take((size_t)batch * 4);
+  q.done = take((size_t)batch * 4);
   q.bytes = at;
   return q;
 }
@@ -380,6 +509,64 @@ static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int
   return launch<NsEpi>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
 }
 
+// One launch where the Gram product (the one with the fewest tiles) would run on pairs
+static bool chained(int64_t batch, int64_t rows, int64_t cols, int steps) {
+  const int64_t side = std::min(rows, cols), t = ceil_div(side, 256), tri = t * (t + 1) / 2;
+  const int64_t all = (2 * tri + ceil_div(rows, 256) * ceil_div(cols, 256)) * batch * steps;
+  return side > 128 && tri * batch * 3 >= num_sms() && all < (1ll << 26);
+}
+
+template <bool SPLIT>
+static int launch_chain(const Chain& c, const ChainEpi::Args& args, cudaStream_t s, const char* what) {
+  using G = Geo<256, true, SPLIT>;
+  const int units = std::min(resident<G, chain_kernel<SPLIT>>(2), c.batch * c.one[NEXT].per);
+  if (units < 1) {
+    set_error("%s: the kernel cannot be resident (registers)", what);
+    return B200_ERR_CUDA;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * units), 1, 1);
+  cfg.blockDim = dim3(THREADS, 1, 1);
+  cfg.dynamicSmemBytes = G::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeCooperative;
+  attr[0].val.cooperative = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  cudaLaunchKernelEx(&cfg, chain_kernel<SPLIT>, c, args);
+  return check_launch(what);
+}
+
+static int run_chain(const ChainEpi::Args& args, const Operand (&X)[2], const Operand& S, const Operand& P, int64_t batch, int64_t rows,
+                     int64_t cols, int planes, cudaStream_t s, const char* what) {
+  const int64_t side = std::min(rows, cols), K = std::max(rows, cols);
+  const int tall = rows > cols;
+  Chain c = {};
+  c.done = args.done, c.batch = (int)batch, c.steps = args.steps, c.tall = tall;
+  auto fill = [&](int which, int64_t M, int64_t N, int64_t k, int a_mn, int b_mn, int walk) {
+    const int nk = (int)ceil_div(k, BK), tm = (int)ceil_div(M, 256), tn = (int)ceil_div(N, 256);
+    c.one[which] = {M, N, nk, planes > 1 ? CHUNK : nk, a_mn, b_mn, tm, tn, walk, walk == WALK_TRIANGLE ? tn * (tn + 1) / 2 : tm * tn};
+  };
+  fill(GRAM, side, side, K, tall, tall, WALK_TRIANGLE);
+  fill(POLY, side, side, side, 0, 0, WALK_TRIANGLE);
+  fill(NEXT, rows, cols, side, 0, !tall, WALK_GROUPED);
+  int rc = operand_map(&c.s, S, side, side, planes, batch, BM);
+  if (!rc) rc = operand_map(&c.p, P, side, side, planes, batch, BM);
+  for (int i = 0; i < 2 && !rc; ++i) {
+    Operand Xo = X[i];
+    Xo.mn = !tall;
+    rc = operand_map(&c.x_gram[i], X[i], side, K, planes, batch, BM);
+    if (!rc) rc = operand_map(&c.x_next[i], Xo, K, side, planes, batch, BM);
+  }
+  if (rc) return rc;
+  return planes > 1 ? launch_chain<true>(c, args, s, what) : launch_chain<false>(c, args, s, what);
+}
+
 struct Finish {  // out = fa add + fb X
   void* out;
   const float* add;
@@ -394,7 +581,7 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
   __half* x[2] = {reinterpret_cast<__half*>(ws + q.x0), reinterpret_cast<__half*>(ws + q.x1)};
   __half *S = reinterpret_cast<__half*>(ws + q.s), *P = reinterpret_cast<__half*>(ws + q.p);
   double* part = reinterpret_cast<double*>(ws + q.part);
-  int* e0 = reinterpret_cast<int*>(ws + q.e0);
+  int *e0 = reinterpret_cast<int*>(ws + q.e0), *done = reinterpret_cast<int*>(ws + q.done);
   const int64_t n = rows * cols;
   const int parts = (int)std::min<int64_t>(NORM_BLOCKS, ceil_div(n, NT * 8));
   const int bf16 = dtype == B200_BF16;
@@ -403,50 +590,54 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
   if (rc) return rc;
   const int64_t xb = q.planes * q.xn, gb = q.planes * q.gn;
   const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(rows * (q.ldx / 8), NT), 4 * num_sms());
-  start_kernel<<<dim3(gx, (unsigned)batch), NT, 0, s>>>(g, bf16, mom ? mom_out : nullptr, mu, nesterov, part, parts, eps, e0, x[0], q.ldx, q.xn,
+  start_kernel<<<dim3(gx, (unsigned)batch), NT, 0, s>>>(g, bf16, mom ? mom_out : nullptr, mu, nesterov, part, parts, eps, e0, done, x[0], q.ldx, q.xn,
                                                         xb, q.planes, rows, cols);
   if ((rc = check_launch(what))) return rc;
   const bool tall = rows > cols;
+  Operand X[2], Sm, Pm;  // by products: X as the Gram product reads it
+  X[0].ld = X[1].ld = q.ldx, X[0].plane_stride = X[1].plane_stride = q.xn, X[0].batch_stride = X[1].batch_stride = xb;
+  X[0].mn = X[1].mn = tall, X[0].base = x[0], X[1].base = x[1];
+  Sm.ld = q.ldg, Sm.plane_stride = q.gn, Sm.batch_stride = gb;
+  Pm = Sm;
+  Sm.base = S, Pm.base = P;
+  ChainEpi::Args all = {};
+  NsEpi::Args &gram = all.part[GRAM], &poly = all.part[POLY], &next = all.part[NEXT], &out = all.part[LAST];
+  gram.e0 = e0, gram.planes = q.planes, gram.M = gram.N = q.side, gram.ld = q.ldg, gram.plane = q.gn, gram.batch = gb;
+  gram.mirror = 1;
+  poly = gram;
+  gram.which = GRAM, gram.dst = S, gram.cc = 1.f / SCALE;
+  poly.which = POLY, poly.src = S, poly.dst = P;
+  next.which = NEXT, next.e0 = e0, next.planes = q.planes, next.M = rows, next.N = cols;
+  next.ld = q.ldx, next.plane = q.xn, next.batch = xb, next.cc = 1.f / SCALE;
+  out = next;
+  out.which = LAST, out.cc = f.fb / (SCALE * SCALE);
+  out.out = f.out, out.add = f.add, out.fa = f.fa, out.bf16 = f.bf16;
   double grown = 0.0;  // log2 of how far a has made the smallest X grow
   for (int i = 0; i < steps; ++i) {
     const float a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
-    const bool last = i + 1 == steps;
-    Operand X, Gm;
-    X.base = x[i & 1], X.ld = q.ldx, X.plane_stride = q.xn, X.batch_stride = xb, X.mn = tall;
-    Gm.ld = q.ldg, Gm.plane_stride = q.gn, Gm.batch_stride = gb;
-    NsEpi::Args e = {};
-    e.e0 = e0;
-    e.e_down = e.e_down_next = (int)std::floor(grown);
+    ChainEpi::Step& st = all.step[i];
+    st.ca = b, st.cc = c / SCALE, st.diag = a * SCALE;
+    st.e_down = st.e_down_next = (int)std::floor(grown);
     grown += std::max(0.0, std::log2((double)std::fabs(a)));
-    if (!last) e.e_down_next = (int)std::floor(grown);
-    e.which = GRAM;
-    e.planes = q.planes;
-    e.M = e.N = q.side;
-    e.ld = q.ldg, e.plane = q.gn, e.batch = gb;
-    e.cc = 1.f / SCALE;
-    e.mirror = 1;
-    e.dst = S;
-    rc = product(X, X, q.side, q.side, tall ? rows : cols, batch, q.planes, true, e, s, what);
-    if (rc) return rc;
-    e.which = POLY;
-    e.src = S, e.dst = P, e.ca = b, e.cc = c / SCALE, e.diag = a * SCALE;
-    Gm.base = S;
-    rc = product(Gm, Gm, q.side, q.side, q.side, batch, q.planes, true, e, s, what);
-    if (rc) return rc;
-    Gm.base = P;
-    NsEpi::Args r = {};
-    r.e0 = e0, r.e_down = r.e_down_next = e.e_down, r.which = last ? LAST : NEXT;
-    r.planes = q.planes;
-    r.M = rows, r.N = cols;
-    r.ld = q.ldx, r.plane = q.xn, r.batch = xb;
-    r.cc = last ? f.fb / (SCALE * SCALE) : 1.f / SCALE;
-    r.dst = last ? nullptr : x[(i + 1) & 1];
-    r.out = f.out, r.add = f.add, r.fa = f.fa, r.bf16 = f.bf16;
+    if (i + 1 < steps) st.e_down_next = (int)std::floor(grown);
+  }
+  all.x[0] = x[0], all.x[1] = x[1], all.done = done, all.steps = steps;
+  const int64_t K = tall ? rows : cols;  // of the Gram product
+  if (chained(batch, rows, cols, steps)) return run_chain(all, X, Sm, Pm, batch, rows, cols, q.planes, s, what);
+  for (int i = 0; i < steps; ++i) {
+    const Operand& Xi = X[i & 1];
+    if ((rc = product(Xi, Xi, q.side, q.side, K, batch, q.planes, true, gram, s, what))) return rc;
+    const ChainEpi::Step& st = all.step[i];
+    poly.ca = st.ca, poly.cc = st.cc, poly.diag = st.diag, poly.e_down = st.e_down, poly.e_down_next = st.e_down_next;
+    if ((rc = product(Sm, Sm, q.side, q.side, q.side, batch, q.planes, true, poly, s, what))) return rc;
+    NsEpi::Args& r = i + 1 < steps ? next : out;
+    r.e_down = st.e_down;
+    if (i + 1 < steps) r.dst = x[(i + 1) & 1];
     // P X (wide: X's columns are the result's) or X P (tall); P's rows serve as its columns
-    Operand Xo = X;
-    Xo.mn = tall ? 0 : 1;
-    rc = tall ? product(Xo, Gm, rows, cols, q.side, batch, q.planes, false, r, s, what)
-              : product(Gm, Xo, rows, cols, q.side, batch, q.planes, false, r, s, what);
+    Operand Xo = Xi;
+    Xo.mn = !tall;
+    rc = tall ? product(Xo, Pm, rows, cols, q.side, batch, q.planes, false, r, s, what)
+              : product(Pm, Xo, rows, cols, q.side, batch, q.planes, false, r, s, what);
     if (rc) return rc;
   }
   return B200_OK;

@@ -78,32 +78,66 @@ struct Loop {
 
 struct Tile {
   int z, split, mt, nt;
+  int product, step;  // which product of a chain, in which round
 };
 
-__device__ __forceinline__ Tile tile_at(const Loop& lp, int t) {
-  Tile r;
-  r.z = t / lp.per_batch;
-  int i = t % lp.per_batch;
-  const int per_split = lp.per_batch / lp.splits;
-  r.split = i / per_split;
-  i %= per_split;
-  if (lp.walk == WALK_TRIANGLE) {
+// the i-th tile of one product
+__device__ __forceinline__ void place(Tile& r, int i, int walk, int tiles_m, int tiles_n, int group_m) {
+  if (walk == WALK_TRIANGLE) {
     // square tiles on and above the diagonal: i = nt (nt + 1) / 2 + mt, mt <= nt
     int nt = (int)((sqrtf(8.f * (float)i + 1.f) - 1.f) * 0.5f);
     while ((nt + 1) * (nt + 2) / 2 <= i) ++nt;
     while (nt * (nt + 1) / 2 > i) --nt;
     r.nt = nt;
     r.mt = i - nt * (nt + 1) / 2;
-    return r;
+    return;
   }
-  const int per_group = lp.group_m * lp.tiles_n;
-  const int first = i / per_group * lp.group_m;
-  const int size = min(lp.group_m, lp.tiles_m - first);
+  const int per_group = group_m * tiles_n;
+  const int first = i / per_group * group_m;
+  const int size = min(group_m, tiles_m - first);
   const int j = i % per_group;
   r.mt = first + j % size;
   r.nt = j / size;
-  return r;
 }
+
+// What the tile loop walks: tile t of `total`, its K blocks, its operands' maps and whether they
+// have M (N) adjacent, the result's size. This one: one product over all of its batch.
+struct Product {
+  static constexpr bool CHAIN = false;
+  const CUtensorMap &a, &b;
+  const Loop& lp;
+  int64_t M, N;
+  __device__ __forceinline__ int total() const { return lp.total; }
+  __device__ __forceinline__ Tile at(int t) const {
+    Tile r;
+    r.product = r.step = 0;
+    r.z = t / lp.per_batch;
+    int i = t % lp.per_batch;
+    const int per_split = lp.per_batch / lp.splits;
+    r.split = i / per_split;
+    i %= per_split;
+    place(r, i, lp.walk, lp.tiles_m, lp.tiles_n, lp.group_m);
+    return r;
+  }
+  __device__ __forceinline__ Tile kind(int t) const {  // all but the place
+    Tile r = {};
+    r.split = t % lp.per_batch / (lp.per_batch / lp.splits);
+    return r;
+  }
+  __device__ __forceinline__ int blocks(const Tile&) const { return lp.nk; }
+  __device__ __forceinline__ int blocks_each(const Tile&) const { return lp.nk_split; }
+  __device__ __forceinline__ int chunk(const Tile&) const { return lp.chunk; }
+  __device__ __forceinline__ int a_mn(const Tile&) const { return lp.a_mn; }
+  __device__ __forceinline__ int b_mn(const Tile&) const { return lp.b_mn; }
+  __device__ __forceinline__ const CUtensorMap* map_a(const Tile&) const { return &a; }
+  __device__ __forceinline__ const CUtensorMap* map_b(const Tile&) const { return &b; }
+  __device__ __forceinline__ int64_t rows(const Tile&) const { return M; }
+  __device__ __forceinline__ int64_t cols(const Tile&) const { return N; }
+  __device__ __forceinline__ void prefetch() const {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&a)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&b)) : "memory");
+  }
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
   uint32_t r;
@@ -230,9 +264,10 @@ struct Spot {
 // values[32]) loads what ready(spot, column, values[32]) turns into what it is added to (result =
 // values + scale * product); chunk(spot, column, values[32]) for each 32 columns
 // inside the result, end(spot); finish(lane) at the end of the kernel.
-template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
-__device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtensorMap& map_b, const Loop& lp, int64_t M, int64_t N,
-                                          Epi& epi) {
+// Work: Product, or a chain of them (CHAIN) whose tiles wait for earlier ones: ready(tile) before
+// its first load, by one thread; the epilogue's begin does the same for what it reads.
+template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Work, typename Epi>
+__device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16, Epi& epi) {
   using G = Geo<BN, PAIR, SPLIT>;
   constexpr int STG = G::STAGES;
   extern __shared__ uint8_t smem_raw[];
@@ -247,12 +282,12 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
   const int member = TEAM ? (int)cluster_rank() : 0;
-  const int per_unit = PAIR ? 2 : (TEAM ? lp.team : 1);
+  const int per_unit = PAIR ? 2 : (TEAM ? team : 1);
+  const int total = work.total();
   const int unit = (int)blockIdx.x / per_unit, units = (int)gridDim.x / per_unit;
 
   if (threadIdx.x == 0) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_a)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_b)) : "memory");
+    work.prefetch();
     for (int s = 0; s < STG; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
@@ -287,11 +322,18 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = unit; t < lp.total && ok; t += units) {
-        const Tile at = tile_at(lp, t);
+      for (int t = unit; t < total && ok; t += units) {
+        const Tile at = work.at(t);
+        const CUtensorMap *map_a = work.map_a(at), *map_b = work.map_b(at);
+        const int a_mn = work.a_mn(at), b_mn = work.b_mn(at), each = work.blocks_each(at);
+        if constexpr (Work::CHAIN)
+          if (!work.ready(at)) {
+            ok = false;
+            break;
+          }
         const int m0 = at.mt * G::TM + (int)rank * BM;
         const int n0 = at.nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
-        const int kb0 = (TEAM ? member : at.split) * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
+        const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
           const int s = it % STG;
           if (!mbar_wait(&empty_bar[s], ((it / STG) & 1) ^ 1)) {
@@ -304,18 +346,18 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           for (int p = 0; p < G::PLANES; ++p) {
             uint8_t* a_dst = smem + s * G::STAGE + p * G::A_BYTES;
             uint8_t* b_dst = smem + s * G::STAGE + G::PLANES * G::A_BYTES + p * G::B_BYTES;
-            if (!lp.a_mn) {
-              load4<PAIR>(a_dst, &map_a, &full_bar[s], k0, m0, p, at.z);
+            if (!a_mn) {
+              load4<PAIR>(a_dst, map_a, &full_bar[s], k0, m0, p, at.z);
             } else {
-              load4<PAIR>(a_dst, &map_a, &full_bar[s], m0, k0, p, at.z);
-              load4<PAIR>(a_dst + 8192, &map_a, &full_bar[s], m0 + 64, k0, p, at.z);
+              load4<PAIR>(a_dst, map_a, &full_bar[s], m0, k0, p, at.z);
+              load4<PAIR>(a_dst + 8192, map_a, &full_bar[s], m0 + 64, k0, p, at.z);
             }
-            if (!lp.b_mn) {
-              load4<PAIR>(b_dst, &map_b, &full_bar[s], k0, n0, p, at.z);
+            if (!b_mn) {
+              load4<PAIR>(b_dst, map_b, &full_bar[s], k0, n0, p, at.z);
             } else {
 #pragma unroll
               for (int j = 0; j < (PAIR ? BN / 2 : BN) / 64; ++j)
-                load4<PAIR>(b_dst + j * 8192, &map_b, &full_bar[s], n0 + 64 * j, k0, p, at.z);
+                load4<PAIR>(b_dst + j * 8192, map_b, &full_bar[s], n0 + 64 * j, k0, p, at.z);
             }
           }
         }
@@ -327,16 +369,17 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       }
     }
     if (warp == 1 && lane == 0 && rank == 0) {
-      const uint32_t fmt = lp.bf16 ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)lp.a_mn << 15) | ((uint32_t)lp.b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
-                             ((uint32_t)(G::TM >> 4) << 24);
+      const uint32_t fmt = bf16 ? (1u << 7) | (1u << 10) : 0u;
       uint32_t it = 0, local = 0;
       bool ok = true;
       uint32_t tiles = 0;
-      for (int t = unit; t < lp.total && ok; t += units, ++tiles) {
-        const int split = TEAM ? member : t % lp.per_batch / (lp.per_batch / lp.splits);
-        const int kb0 = split * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
-        for (int c0 = kb0; c0 < kb1 && ok; c0 += lp.chunk, ++local) {
+      for (int t = unit; t < total && ok; t += units, ++tiles) {
+        const Tile at = work.kind(t);
+        const int a_mn = work.a_mn(at), b_mn = work.b_mn(at), each = work.blocks_each(at), chunk = work.chunk(at);
+        const uint32_t idesc =
+            (1u << 4) | fmt | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(G::TM >> 4) << 24);
+        const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
+        for (int c0 = kb0; c0 < kb1 && ok; c0 += chunk, ++local) {
           const int b = local & 1;
           if (!mbar_wait(&acc_empty[b], ((local >> 1) & 1) ^ 1)) {
             ok = false;
@@ -344,7 +387,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           }
           tc_fence_after();
           const uint32_t d = tmem + (uint32_t)(b * BN);
-          const int c1 = min(kb1, c0 + lp.chunk);
+          const int c1 = min(kb1, c0 + chunk);
           for (int kb = c0; kb < c1; ++kb, ++it) {
             const int s = it % STG;
             if (!mbar_wait(&full_bar[s], (it / STG) & 1)) {
@@ -361,8 +404,8 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
               const bool fresh = G::APART ? (seg == 0 ? kb == kb0 : (seg == 2 && kb == c0)) : (seg == (SPLIT ? 0 : 2) && kb == c0);
 #pragma unroll
               for (int k = 0; k < BK / 16; ++k) {
-                const uint64_t ad = lp.a_mn ? smem_desc(as + k * 2048, 8192, 1024) : smem_desc(as + k * 32, 16, 1024);
-                const uint64_t bd = lp.b_mn ? smem_desc(bs + k * 2048, 8192, 1024) : smem_desc(bs + k * 32, 16, 1024);
+                const uint64_t ad = a_mn ? smem_desc(as + k * 2048, 8192, 1024) : smem_desc(as + k * 32, 16, 1024);
+                const uint64_t bd = b_mn ? smem_desc(bs + k * 2048, 8192, 1024) : smem_desc(bs + k * 32, 16, 1024);
                 mma<PAIR>(to, ad, bd, idesc, (!fresh || k > 0) ? 1u : 0u);
               }
             }
@@ -397,8 +440,9 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
         else mbar_arrive(&acc_empty[b]);
       }
     };
-    for (int t = unit; t < lp.total && ok; t += units) {
-      const Tile at = tile_at(lp, t);
+    for (int t = unit; t < total && ok; t += units) {
+      const Tile at = work.at(t);
+      const int64_t M = work.rows(at), N = work.cols(at);
       sp.z = at.z;
       sp.split = at.split;
       sp.mt = at.mt;
@@ -407,9 +451,13 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
       sp.row = sp.row0 + lane;
       const int64_t col0 = sp.col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
-      epi.begin(sp);
+      if constexpr (Work::CHAIN) {
+        if (!epi.enter(work, at, sp)) break;
+      } else {
+        epi.begin(sp);
+      }
       // the member that finishes chunk c of this warp: of two, each takes a chunk of every warp
-      auto owner = [&](int c) { return !TEAM ? 0 : (lp.team == 2 ? c : sp.half * CH + c); };
+      auto owner = [&](int c) { return !TEAM ? 0 : (team == 2 ? c : sp.half * CH + c); };
       if constexpr (SPLIT || TEAM) {
         float acc[CH][32];
 #pragma unroll
@@ -435,8 +483,9 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
             else to[i] += __uint_as_float(cur[i]);
           }
         };
-        const int kb0 = (TEAM ? member : at.split) * lp.nk_split, kb1 = min(lp.nk, kb0 + lp.nk_split);
-        for (int c0 = kb0; c0 < kb1; c0 += lp.chunk, ++local) {
+        const int each = work.blocks_each(at), chunk = work.chunk(at);
+        const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
+        for (int c0 = kb0; c0 < kb1; c0 += chunk, ++local) {
           const int b = local & 1;
           if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) {
             ok = false;
@@ -446,7 +495,7 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             add((uint32_t)(b * BN + c * 32), acc[c]);
-            if (G::APART && c0 + lp.chunk >= kb1) add((uint32_t)((2 + (tiles & 1)) * BN + c * 32), acc[c]);
+            if (G::APART && c0 + chunk >= kb1) add((uint32_t)((2 + (tiles & 1)) * BN + c * 32), acc[c]);
           }
           release(b);
         }
@@ -455,13 +504,13 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
           // every member's MMAs are done: the operand ring takes the partial sums, 16 KB (128 rows
           // of 32, 16-byte pieces swizzled by row) per chunk and sender
           cluster_sync_all();
-          const int each = 2 * CH / lp.team, mine = lp.team == 2 ? sp.half : 0;
+          const int share = 2 * CH / team, mine = team == 2 ? sp.half : 0;
           const uint32_t line = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 128u;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             const int to = owner(c);
             if (to == member) continue;
-            const int slot = (member < to ? member : member - 1) * each + mine;
+            const int slot = (member < to ? member : member - 1) * share + mine;
             uint32_t far;
             asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(line + (uint32_t)slot * 16384u), "r"(to));
 #pragma unroll
@@ -474,8 +523,8 @@ __device__ __forceinline__ void run_tiles(const CUtensorMap& map_a, const CUtens
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             if (owner(c) != member) continue;
-            for (int from = 0; from < lp.team - 1; ++from) {
-              const uint32_t at_line = line + (uint32_t)(from * each + mine) * 16384u;
+            for (int from = 0; from < team - 1; ++from) {
+              const uint32_t at_line = line + (uint32_t)(from * share + mine) * 16384u;
 #pragma unroll
               for (int p = 0; p < 8; ++p) {
                 const uint4 u = ld_shared_v4(at_line + (uint32_t)((p ^ (lane & 7)) << 4));
@@ -543,7 +592,7 @@ __global__ void __launch_bounds__(THREADS, 1) tile_kernel(const __grid_constant_
                                                           const __grid_constant__ Loop lp, const int64_t M, const int64_t N,
                                                           const __grid_constant__ typename Epi::Args args) {
   Epi epi(args);
-  run_tiles<BN, PAIR, SPLIT, TEAM>(map_a, map_b, lp, M, N, epi);
+  run_tiles<BN, PAIR, SPLIT, TEAM>(Product{map_a, map_b, lp, M, N}, lp.team, lp.bf16 != 0, epi);
 }
 
 // ---------------------------------------------------------------------------------
@@ -558,27 +607,36 @@ struct Operand {
   int mn = 0;
 };
 
-// Clusters (of `size` CTAs; 1: none) that can be resident at once, per kernel, size and device;
-// 0 where the kernel was compiled to fewer registers than its warpgroups trade
-template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
+// The map of an operand of `major` rows and K, boxes of 64 elements of K by `box` rows (64 x 64
+// where the rows are adjacent)
+static int operand_map(CUtensorMap* m, const Operand& o, int64_t major, int64_t K, int planes, int64_t batch, int box) {
+  const uint64_t span = (uint64_t)o.ld * 2 * (uint64_t)(o.mn ? K : major);
+  const uint64_t ps = planes > 1 ? (uint64_t)o.plane_stride * 2 : span, bs = batch > 1 ? (uint64_t)o.batch_stride * 2 : ps * planes;
+  return o.mn ? make_map(m, o.base, major, K, planes, batch, o.ld * 2, ps, bs, 64, 64)
+              : make_map(m, o.base, K, major, planes, batch, o.ld * 2, ps, bs, 64, box);
+}
+
+// Clusters (of `size` CTAs; 1: none) of a kernel of geometry G that can be resident at once, per
+// kernel, size and device; 0 where it was compiled to fewer registers than its warpgroups trade
+template <typename G, auto KERNEL>
 static int resident(int size) {
   static int units[64][5] = {{0}};
   int dev = 0;
   cudaGetDevice(&dev);
   const bool known = dev >= 0 && dev < 64;
   if (known && units[dev][size]) return units[dev][size];
-  auto* fn = tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>;
-  if constexpr (Geo<BN, PAIR, SPLIT>::LEND) {
+  auto* fn = KERNEL;
+  if constexpr (G::LEND) {
     cudaFuncAttributes at;
     if (cudaFuncGetAttributes(&at, fn) != cudaSuccess || at.numRegs * THREADS < REGS_SUM) return 0;
   }
-  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Geo<BN, PAIR, SPLIT>::SMEM);
+  cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)G::SMEM);
   int n = num_sms() / size;
   if (size > 1) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(size * n), 1, 1);
     cfg.blockDim = dim3(THREADS, 1, 1);
-    cfg.dynamicSmemBytes = Geo<BN, PAIR, SPLIT>::SMEM;
+    cfg.dynamicSmemBytes = G::SMEM;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = (unsigned)size;
@@ -600,6 +658,7 @@ template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, Loop lp,
                      const typename Epi::Args& args, cudaStream_t s, const char* what) {
   using G = Geo<BN, PAIR, SPLIT>;
+  constexpr auto kernel = tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>;
   constexpr int planes = SPLIT ? 2 : 1;
   lp.a_mn = A.mn;
   lp.b_mn = B.mn;
@@ -618,28 +677,22 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   if constexpr (TEAM) {
     // one tile per team; 4 or 2 members where that many teams fit and each has 2 K blocks or more
     size = 4;
-    while (size > 1 && (lp.nk < 2 * size || resident<BN, PAIR, SPLIT, TEAM, Epi>(size) < lp.total)) size /= 2;
+    while (size > 1 && (lp.nk < 2 * size || resident<G, kernel>(size) < lp.total)) size /= 2;
     if (size == 1) return -1;
     lp.team = size;
     lp.nk_split = (int)ceil_div(lp.nk, size);
     if (!SPLIT) lp.chunk = lp.nk_split;
     units = lp.total;
   } else {
-    units = std::min(resident<BN, PAIR, SPLIT, TEAM, Epi>(size), lp.total);
+    units = std::min(resident<G, kernel>(size), lp.total);
   }
   if (units < 1) {
     set_error("%s: the kernel cannot be resident (registers)", what);
     return B200_ERR_CUDA;
   }
   CUtensorMap ma, mb;
-  auto map = [&](CUtensorMap* m, const Operand& o, int64_t major, int box) {
-    const uint64_t span = (uint64_t)o.ld * 2 * (uint64_t)(o.mn ? K : major);
-    const uint64_t ps = planes > 1 ? (uint64_t)o.plane_stride * 2 : span, bs = batch > 1 ? (uint64_t)o.batch_stride * 2 : ps * planes;
-    return o.mn ? make_map(m, o.base, major, K, planes, batch, o.ld * 2, ps, bs, 64, 64)
-                : make_map(m, o.base, K, major, planes, batch, o.ld * 2, ps, bs, 64, box);
-  };
-  int rc = map(&ma, A, M, BM);
-  if (!rc) rc = map(&mb, B, N, PAIR ? BN / 2 : BN);
+  int rc = operand_map(&ma, A, M, K, planes, batch, BM);
+  if (!rc) rc = operand_map(&mb, B, N, K, planes, batch, PAIR ? BN / 2 : BN);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(size * units), 1, 1);
@@ -655,7 +708,7 @@ static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, i
   attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = size > 1 ? 2 : 1;
-  cudaLaunchKernelEx(&cfg, tile_kernel<BN, PAIR, SPLIT, TEAM, Epi>, ma, mb, lp, M, N, args);
+  cudaLaunchKernelEx(&cfg, kernel, ma, mb, lp, M, N, args);
   return check_launch(what);
 }
 

@@ -128,8 +128,64 @@ def test_norms_beyond_fp32s_reciprocals(power, dtype):
     assert off(got, R.newton_schulz(g.double(), eps=0.0)) <= BOUND[dtype]
 
 
+STACKS = [(50, 129, 200), (50, 200, 129), (20, 300, 520), (20, 520, 300), (50, 256, 256), (17, 257, 1030), (9, 770, 600)]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("shape", STACKS)
+@pytest.mark.parametrize("steps", [1, 2, 5])
+def test_stacks_that_fill_the_gpu(shape, dtype, steps):
+    """Every matrix of a stack, each of its own scale, against 64 bits and against the call of that matrix alone."""
+    g = grads(*shape, dtype=dtype)
+    g = (g * (2.0 ** (torch.arange(shape[0]) % 7 - 3).double()).to(dtype).cuda().view(-1, 1, 1)).contiguous()
+    got = op("NewtonSchulz", g, steps=steps)
+    ref = R.newton_schulz(g.double(), steps)
+    assert max(off(got[i], ref[i]) for i in range(shape[0])) <= BOUND[dtype]
+    for i in (0, shape[0] - 1):
+        assert off(op("NewtonSchulz", g[i], steps=steps), got[i].double()) <= 2 * BOUND[dtype]
+    assert torch.equal(op("NewtonSchulz", g, steps=steps), got)
+
+
+def test_stacks_with_vanishing_matrices_and_own_coefficients():
+    g = grads(20, 300, 520)
+    g[3] *= 2.0**-60
+    g[7] = 0
+    g[11, 5, 9] = float("nan")
+    coef = [(2.0, -1.5, 0.5), (3.0, -3.2, 1.2), (1.9, -1.0, 0.1)]
+    got = op("NewtonSchulz", g, steps=3, coefficients=coef)
+    ref = g.double() / (g.double().flatten(1).norm(dim=1).view(-1, 1, 1) + 1e-7)
+    for a, b, c in coef:
+        s = ref @ ref.transpose(1, 2)
+        ref = a * ref + (b * s + c * s @ s) @ ref
+    assert not got[7].any() and got[11].isnan().any()
+    assert max(off(got[i], ref[i]) for i in range(20) if i not in (7, 11)) <= BOUND[F32]
+
+
+@pytest.mark.parametrize("shape", [(20, 300, 520), (20, 520, 300)])
+def test_stacks_on_two_streams_and_replayed(shape):
+    """Two calls at once, an eager one beside a captured one; the counters start anew each time."""
+    a, b = grads(*shape), grads(*shape, seed=4)
+    wa, wb = op("NewtonSchulz", a), op("NewtonSchulz", b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        cap = op("NewtonSchulz", a)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    outs = []
+    for _ in range(4):
+        graph.replay()
+        with torch.cuda.stream(s):
+            outs.append(op("NewtonSchulz", b))
+    torch.cuda.synchronize()
+    assert torch.equal(cap, wa) and all(torch.equal(o, wb) for o in outs)
+    p, m = grads(*shape, seed=7, scale=0.02), grads(*shape, seed=8)
+    want = op("ApplyMuon", p, m, a, lr=0.05, weight_decay=0.1)
+    op("ApplyMuon", p, m, a, lr=0.05, weight_decay=0.1, out=(p, m))
+    assert torch.equal(p, want[0]) and torch.equal(m, want[1])
+
+
 @pytest.mark.parametrize("nesterov", [True, False])
-@pytest.mark.parametrize("shape", [(40, 24), (24, 40), (4, 256, 256), (1, 130), (1100, 300)])
+@pytest.mark.parametrize("shape", [(40, 24), (24, 40), (4, 256, 256), (1, 130), (1100, 300), (20, 300, 270)])
 def test_apply_muon(shape, nesterov):
     g, m, p = grads(*shape), grads(*shape, seed=3), grads(*shape, seed=5, scale=0.02)
     kw = {"lr": 0.05, "momentum": 0.9, "nesterov": nesterov, "weight_decay": 0.1}
