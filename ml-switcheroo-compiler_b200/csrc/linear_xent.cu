@@ -233,6 +233,7 @@ struct StoreEpi {
   __device__ __forceinline__ bool dense(int64_t col) const {  // 16-byte rows of whole chunks
     return col + 32 <= a.N && (a.ld_add & 3) == 0 && (reinterpret_cast<uintptr_t>(a.add) & 15) == 0;
   }
+  __device__ __forceinline__ bool adds() const { return a.add != nullptr; }
   __device__ __forceinline__ void fetch(const Spot& sp, int64_t col, float (&v)[32]) {
     if (!a.add) return;
     const int rows = (int)min((int64_t)32, a.M - sp.row0);

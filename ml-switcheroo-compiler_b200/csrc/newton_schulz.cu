@@ -43,24 +43,27 @@ __device__ __forceinline__ void unpack_f16(uint32_t u, float& a, float& b) {
 
 constexpr int GRAM = 0, POLY = 1, NEXT = 2, LAST = 3;
 
-// result = cc product + ca source + diag I (POLY), as fp16 planes, mirrored where symmetric;
-// LAST: out = cc product + fa add
+// result = cc product + ca source + diag I (POLY), as fp16 planes; LAST: out = cc product + fa add
+struct NsArgs {
+  const __half* src;  // planes at the result's offsets, or NULL
+  __half* dst;        // planes, or NULL: the last product
+  int64_t ld, plane, batch;
+  float ca, cc, diag;
+  int planes, mirror;
+  void* out;
+  const float* add;  // fp32, dense as out
+  int64_t M, N;
+  float fa;
+  int bf16;
+  const int* e0;               // [batch]: the exponent of t at the start
+  int e_down, e_down_next;     // how far it has shrunk, and will have after this step
+  int which;                   // GRAM, POLY, NEXT, LAST
+};
+
+// MIRROR: symmetric results (`mirror`) are written on both sides of the diagonal
+template <bool MIRROR>
 struct NsEpi {
-  struct Args {
-    const __half* src;  // planes at the result's offsets, or NULL
-    __half* dst;        // planes, or NULL: the last product
-    int64_t ld, plane, batch;
-    float ca, cc, diag;
-    int planes, mirror;
-    void* out;
-    const float* add;  // fp32, dense as out
-    int64_t M, N;
-    float fa;
-    int bf16;
-    const int* e0;               // [batch]: the exponent of t at the start
-    int e_down, e_down_next;     // how far it has shrunk, and will have after this step
-    int which;                   // GRAM, POLY, NEXT, LAST
-  };
+  using Args = NsArgs;
   static constexpr bool SINGLE_WIDE = false, SINGLE_NARROW = true, TEAMS = true, INIT = true;
   const Args* a;
   __half* dst;
@@ -91,6 +94,7 @@ struct NsEpi {
   __device__ __forceinline__ bool dense(const Spot& sp, int64_t col) const {  // 16-byte rows of whole chunks
     return col + 32 <= a->N && (a->N & 3) == 0 && (reinterpret_cast<uintptr_t>(a->add) & 15) == 0;
   }
+  __device__ __forceinline__ bool adds() const { return a->which == POLY || (a->which == LAST && a->add); }
   __device__ __forceinline__ void fetch(const Spot& sp, int64_t col, float (&v)[32]) {
     const int rows = (int)min((int64_t)32, a->M - sp.row0), cols = (int)min((int64_t)32, a->N - col);
     if (a->which == POLY) {
@@ -164,7 +168,7 @@ struct NsEpi {
     // (row / 2) ^ (row / 8): rows written and read, and 8 x 8 blocks read transposed, are then free
     // of bank conflicts. Rows leave as 64 adjacent bytes each way.
     const int lane = sp.lane;
-    const bool mirror = a->mirror && sp.mt != sp.nt;
+    const bool mirror = MIRROR && a->mirror && sp.mt != sp.nt;
     for (int k = 0; k < a->planes; ++k) {
       __half* d = dst + sp.z * a->batch + k * a->plane;
       const uint32_t buf = sp.buf + (uint32_t)(k & 1) * 2048u;
@@ -223,69 +227,75 @@ struct NsEpi {
 // 1024 x 1024: 160, 160 and 256 tiles for 74 pairs, 10 waves for 7.8) and each launch fills and
 // drains its pipeline. So all tiles of all products form one list, walked by the pairs in
 // turn. A tile waits until its matrix's previous product is complete: counters in the
-// workspace, one per matrix, of the warps that have finished a tile. Every tile depends on
+// workspace, one per matrix, of the CTAs that have finished a tile. Every tile depends on
 // earlier ones of the list only, and the launch is cooperative, so the first unfinished
 // tile never waits. What a matrix's buffers hold is overwritten two products after
 // their last reader at the earliest, which the same counter orders.
-constexpr int MAX_STEPS = 100, ARRIVALS = 2 * EPI_WARPS;  // of a tile
+// S and P, symmetric, are stored on and above the diagonal's tiles only (the mirrored half
+// took 6000 clocks a tile, of 15000 for the epilogue): a K block left of the diagonal is read as the
+// transposed block above it, with the rows adjacent.
+constexpr int MAX_STEPS = 100, ARRIVALS = 2;  // of a tile
 
 struct Chain {
   static constexpr bool CHAIN = true;
   struct One {
     int64_t M, N;
-    int nk, chunk, a_mn, b_mn, tiles_m, tiles_n, walk, per;  // per: tiles of one matrix
+    int nk, chunk, tiles_m, tiles_n, walk, per;  // per: tiles of one matrix
   };
-  CUtensorMap x_gram[2], s, p, x_next[2];
-  One one[3];  // GRAM, POLY, NEXT
-  int* done;   // [batch]
+  CUtensorMap x_gram[2], x_next[2], s[2], p[2];  // s, p: [1] with the rows adjacent
+  One one[3];     // GRAM, POLY, NEXT
+  int* finished;  // [batch]
   int batch, steps, tall;
-  __device__ __forceinline__ int total() const { return steps * batch * (one[0].per + one[1].per + one[2].per); }
+  __device__ __forceinline__ int per_step() const { return one[0].per + one[1].per + one[2].per; }
+  __device__ __forceinline__ int total() const { return steps * batch * per_step(); }
   __device__ __forceinline__ Tile at(int t) const {
-    Tile r = kind(t);
-    t -= r.step * batch * (one[0].per + one[1].per + one[2].per);
-    if (r.product > 0) t -= batch * one[0].per;
-    if (r.product > 1) t -= batch * one[1].per;
+    Tile r = {};
+    r.step = t / (batch * per_step());
+    t -= r.step * batch * per_step();
+    while (r.product < NEXT && t >= batch * one[r.product].per) t -= batch * one[r.product++].per;
     const One& o = one[r.product];
     r.z = t / o.per;
     place(r, t % o.per, o.walk, o.tiles_m, o.tiles_n, 16);
     return r;
   }
-  __device__ __forceinline__ Tile kind(int t) const {
-    const int a = batch * one[0].per, b = batch * one[1].per, c = batch * one[2].per;
-    Tile r = {};
-    r.step = t / (a + b + c);
-    t %= a + b + c;
-    r.product = t < a ? GRAM : (t < a + b ? POLY : NEXT);
-    return r;
-  }
+  __device__ __forceinline__ Tile kind(int t) const { return at(t); }
   __device__ __forceinline__ int blocks(const Tile& t) const { return one[t.product].nk; }
   __device__ __forceinline__ int blocks_each(const Tile& t) const { return one[t.product].nk; }
   __device__ __forceinline__ int chunk(const Tile& t) const { return one[t.product].chunk; }
-  __device__ __forceinline__ int a_mn(const Tile& t) const { return one[t.product].a_mn; }
-  __device__ __forceinline__ int b_mn(const Tile& t) const { return one[t.product].b_mn; }
   __device__ __forceinline__ int64_t rows(const Tile& t) const { return one[t.product].M; }
   __device__ __forceinline__ int64_t cols(const Tile& t) const { return one[t.product].N; }
-  __device__ __forceinline__ const CUtensorMap* map_a(const Tile& t) const {
-    return t.product == GRAM ? &x_gram[t.step & 1] : (t.product == POLY ? &s : (tall ? &x_next[t.step & 1] : &p));
+  struct Side {  // an operand: K blocks below `until` are read with the rows adjacent
+    const CUtensorMap *adjacent, *rest;
+    int until;
+    __device__ __forceinline__ const CUtensorMap* map(int kb) const { return kb < until ? adjacent : rest; }
+    __device__ __forceinline__ int mn(int kb) const { return kb < until; }
+  };
+  // the symmetric operand's tile row i: what lies left of the diagonal, transposed
+  __device__ __forceinline__ Side symmetric(const CUtensorMap (&m)[2], int i) const { return {&m[1], &m[0], i * (256 / BK)}; }
+  __device__ __forceinline__ Side plain(const CUtensorMap& m, int adjacent) const { return {&m, &m, adjacent ? 1 << 30 : 0}; }
+  __device__ __forceinline__ Side side_a(const Tile& t) const {
+    if (t.product == GRAM) return plain(x_gram[t.step & 1], tall);
+    return t.product == POLY ? symmetric(s, t.mt) : (tall ? plain(x_next[t.step & 1], 0) : symmetric(p, t.mt));
   }
-  __device__ __forceinline__ const CUtensorMap* map_b(const Tile& t) const {
-    return t.product == GRAM ? &x_gram[t.step & 1] : (t.product == POLY ? &s : (tall ? &p : &x_next[t.step & 1]));
+  __device__ __forceinline__ Side side_b(const Tile& t) const {
+    if (t.product == GRAM) return plain(x_gram[t.step & 1], tall);
+    return t.product == POLY ? symmetric(s, t.nt) : (tall ? symmetric(p, t.nt) : plain(x_next[t.step & 1], 1));
   }
   __device__ __forceinline__ void prefetch() const {
-    for (const CUtensorMap* m : {&x_gram[0], &s, &p, &x_next[0]})
+    for (const CUtensorMap* m : {&x_gram[0], &s[0], &p[0], &x_next[0]})
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
   }
   // true once the tile's matrix has seen every product before this one (by one thread); false
   // (and the device error flag set) if that takes too long
   __device__ __forceinline__ bool ready(const Tile& t) const {
-    int need = t.step * (one[0].per + one[1].per + one[2].per);
+    int need = t.step * per_step();
     if (t.product > 0) need += one[0].per;
     if (t.product > 1) need += one[1].per;
     need *= ARRIVALS;
     unsigned long long t0 = 0;
     while (true) {
       int v;
-      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(done + t.z) : "memory");
+      asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(finished + t.z) : "memory");
       if (v >= need) break;
       if (t0 == 0) t0 = globaltimer();
       if (globaltimer() - t0 > WAIT_LIMIT_NS) {
@@ -297,23 +307,29 @@ struct Chain {
     asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads next
     return true;
   }
+  // this CTA's part of the tile is stored (by one thread that has waited for the warps which did)
+  __device__ __forceinline__ void done(const Tile& t) const {
+    if (t.product == NEXT && t.step + 1 == steps) return;
+    asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads it
+    __threadfence();
+    asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(finished + t.z) : "memory");
+  }
 };
 
-struct ChainEpi : NsEpi {
+struct ChainEpi : NsEpi<false> {
   struct Step {
     float ca, cc, diag;
     int e_down, e_down_next;
   };
   struct Args {
-    NsEpi::Args part[4];  // GRAM, POLY, NEXT, LAST
+    NsArgs part[4];  // GRAM, POLY, NEXT, LAST
     Step step[MAX_STEPS];
     __half* x[2];
-    int* done;
     int steps;
   };
   const Args& all;
-  __device__ explicit ChainEpi(const Args& args) : NsEpi(args.part[0]), all(args) {}
-  __device__ __forceinline__ bool enter(const Chain& work, const Tile& t, const Spot& sp) {
+  __device__ explicit ChainEpi(const Args& args) : NsEpi<false>(args.part[0]), all(args) {}
+  __device__ __forceinline__ void enter(const Tile& t, const Spot& sp) {
     const bool last = t.product == NEXT && t.step + 1 == all.steps;
     a = &all.part[last ? LAST : t.product];
     dst = t.product == NEXT ? all.x[(t.step + 1) & 1] : a->dst;
@@ -321,19 +337,8 @@ struct ChainEpi : NsEpi {
     const Step& st = all.step[t.step];
     if (t.product == POLY) ca = st.ca, scale = st.cc, diag = st.diag;
     shrunk(a->e0[sp.z], st.e_down, st.e_down_next);
-    if (t.product != POLY) return true;
-    const bool ok = sp.lane != 0 || work.ready(t);  // S is read here
-    return __all_sync(0xffffffffu, ok);
   }
-  __device__ __forceinline__ void end(const Spot& sp) {
-    if (a->which == LAST) return;
-    asm volatile("fence.proxy.async;" ::: "memory");  // TMA reads what was written here
-    __syncwarp();
-    if (sp.lane == 0) {
-      __threadfence();
-      asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(all.done + sp.z) : "memory");
-    }
-  }
+  __device__ __forceinline__ bool reads(const Tile& t) const { return t.product == POLY; }  // S
 };
 
 template <bool SPLIT>
@@ -499,14 +504,14 @@ static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
 // 128 x 128 tiles of single CTAs or teams: a 1024 x 1024 product has 16 of the former (10 reach
 // the diagonal) for 74 pairs, 64 (36) of the latter for 148 CTAs.
 static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, int planes, bool triangle,
-                   const NsEpi::Args& a, cudaStream_t s, const char* what) {
+                   const NsArgs& a, cudaStream_t s, const char* what) {
   Loop lp = {};
   lp.group_m = 16;
   lp.walk = triangle ? WALK_TRIANGLE : WALK_GROUPED;
   const int64_t tm = ceil_div(M, 256), tn = ceil_div(N, 256);
   const int64_t tiles = (triangle ? tn * (tn + 1) / 2 : tm * tn) * batch;
   const bool pair = M > 128 && N > 128 && tiles * 3 >= num_sms();
-  return launch<NsEpi>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
+  return launch<NsEpi<true>>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
 }
 
 // One launch where the Gram product (the one with the fewest tiles) would run on pairs
@@ -542,21 +547,26 @@ static int launch_chain(const Chain& c, const ChainEpi::Args& args, cudaStream_t
   return check_launch(what);
 }
 
-static int run_chain(const ChainEpi::Args& args, const Operand (&X)[2], const Operand& S, const Operand& P, int64_t batch, int64_t rows,
-                     int64_t cols, int planes, cudaStream_t s, const char* what) {
+static int run_chain(const ChainEpi::Args& args, int* finished, const Operand (&X)[2], const Operand& S, const Operand& P, int64_t batch,
+                     int64_t rows, int64_t cols, int planes, cudaStream_t s, const char* what) {
   const int64_t side = std::min(rows, cols), K = std::max(rows, cols);
   const int tall = rows > cols;
   Chain c = {};
-  c.done = args.done, c.batch = (int)batch, c.steps = args.steps, c.tall = tall;
-  auto fill = [&](int which, int64_t M, int64_t N, int64_t k, int a_mn, int b_mn, int walk) {
+  c.finished = finished, c.batch = (int)batch, c.steps = args.steps, c.tall = tall;
+  auto fill = [&](int which, int64_t M, int64_t N, int64_t k, int walk) {
     const int nk = (int)ceil_div(k, BK), tm = (int)ceil_div(M, 256), tn = (int)ceil_div(N, 256);
-    c.one[which] = {M, N, nk, planes > 1 ? CHUNK : nk, a_mn, b_mn, tm, tn, walk, walk == WALK_TRIANGLE ? tn * (tn + 1) / 2 : tm * tn};
+    c.one[which] = {M, N, nk, planes > 1 ? CHUNK : nk, tm, tn, walk, walk == WALK_TRIANGLE ? tn * (tn + 1) / 2 : tm * tn};
   };
-  fill(GRAM, side, side, K, tall, tall, WALK_TRIANGLE);
-  fill(POLY, side, side, side, 0, 0, WALK_TRIANGLE);
-  fill(NEXT, rows, cols, side, 0, !tall, WALK_GROUPED);
-  int rc = operand_map(&c.s, S, side, side, planes, batch, BM);
-  if (!rc) rc = operand_map(&c.p, P, side, side, planes, batch, BM);
+  fill(GRAM, side, side, K, WALK_TRIANGLE);
+  fill(POLY, side, side, side, WALK_TRIANGLE);
+  fill(NEXT, rows, cols, side, WALK_GROUPED);
+  int rc = 0;
+  for (int mn = 0; mn < 2 && !rc; ++mn) {
+    Operand So = S, Po = P;
+    So.mn = Po.mn = mn;
+    rc = operand_map(&c.s[mn], So, side, side, planes, batch, BM);
+    if (!rc) rc = operand_map(&c.p[mn], Po, side, side, planes, batch, BM);
+  }
   for (int i = 0; i < 2 && !rc; ++i) {
     Operand Xo = X[i];
     Xo.mn = !tall;
@@ -601,7 +611,7 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
   Pm = Sm;
   Sm.base = S, Pm.base = P;
   ChainEpi::Args all = {};
-  NsEpi::Args &gram = all.part[GRAM], &poly = all.part[POLY], &next = all.part[NEXT], &out = all.part[LAST];
+  NsArgs &gram = all.part[GRAM], &poly = all.part[POLY], &next = all.part[NEXT], &out = all.part[LAST];
   gram.e0 = e0, gram.planes = q.planes, gram.M = gram.N = q.side, gram.ld = q.ldg, gram.plane = q.gn, gram.batch = gb;
   gram.mirror = 1;
   poly = gram;
@@ -621,16 +631,16 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
     grown += std::max(0.0, std::log2((double)std::fabs(a)));
     if (i + 1 < steps) st.e_down_next = (int)std::floor(grown);
   }
-  all.x[0] = x[0], all.x[1] = x[1], all.done = done, all.steps = steps;
+  all.x[0] = x[0], all.x[1] = x[1], all.steps = steps;
   const int64_t K = tall ? rows : cols;  // of the Gram product
-  if (chained(batch, rows, cols, steps)) return run_chain(all, X, Sm, Pm, batch, rows, cols, q.planes, s, what);
+  if (chained(batch, rows, cols, steps)) return run_chain(all, done, X, Sm, Pm, batch, rows, cols, q.planes, s, what);
   for (int i = 0; i < steps; ++i) {
     const Operand& Xi = X[i & 1];
     if ((rc = product(Xi, Xi, q.side, q.side, K, batch, q.planes, true, gram, s, what))) return rc;
     const ChainEpi::Step& st = all.step[i];
     poly.ca = st.ca, poly.cc = st.cc, poly.diag = st.diag, poly.e_down = st.e_down, poly.e_down_next = st.e_down_next;
     if ((rc = product(Sm, Sm, q.side, q.side, q.side, batch, q.planes, true, poly, s, what))) return rc;
-    NsEpi::Args& r = i + 1 < steps ? next : out;
+    NsArgs& r = i + 1 < steps ? next : out;
     r.e_down = st.e_down;
     if (i + 1 < steps) r.dst = x[(i + 1) & 1];
     // P X (wide: X's columns are the result's) or X P (tall); P's rows serve as its columns

@@ -100,8 +100,7 @@ __device__ __forceinline__ void place(Tile& r, int i, int walk, int tiles_m, int
   r.nt = j / size;
 }
 
-// What the tile loop walks: tile t of `total`, its K blocks, its operands' maps and whether they
-// have M (N) adjacent, the result's size. This one: one product over all of its batch.
+// What the tile loop walks: tile t of `total`, its K blocks, its operands, the result's size. This one: one product over all of its batch.
 struct Product {
   static constexpr bool CHAIN = false;
   const CUtensorMap &a, &b;
@@ -119,7 +118,7 @@ struct Product {
     place(r, i, lp.walk, lp.tiles_m, lp.tiles_n, lp.group_m);
     return r;
   }
-  __device__ __forceinline__ Tile kind(int t) const {  // all but the place
+  __device__ __forceinline__ Tile kind(int t) const {  // what the MMAs need of it
     Tile r = {};
     r.split = t % lp.per_batch / (lp.per_batch / lp.splits);
     return r;
@@ -127,10 +126,14 @@ struct Product {
   __device__ __forceinline__ int blocks(const Tile&) const { return lp.nk; }
   __device__ __forceinline__ int blocks_each(const Tile&) const { return lp.nk_split; }
   __device__ __forceinline__ int chunk(const Tile&) const { return lp.chunk; }
-  __device__ __forceinline__ int a_mn(const Tile&) const { return lp.a_mn; }
-  __device__ __forceinline__ int b_mn(const Tile&) const { return lp.b_mn; }
-  __device__ __forceinline__ const CUtensorMap* map_a(const Tile&) const { return &a; }
-  __device__ __forceinline__ const CUtensorMap* map_b(const Tile&) const { return &b; }
+  struct Side {  // an operand: its map at a K block, whether it has M (N) adjacent there
+    const CUtensorMap* m;
+    int adjacent;
+    __device__ __forceinline__ const CUtensorMap* map(int) const { return m; }
+    __device__ __forceinline__ int mn(int) const { return adjacent; }
+  };
+  __device__ __forceinline__ Side side_a(const Tile&) const { return {&a, lp.a_mn}; }
+  __device__ __forceinline__ Side side_b(const Tile&) const { return {&b, lp.b_mn}; }
   __device__ __forceinline__ int64_t rows(const Tile&) const { return M; }
   __device__ __forceinline__ int64_t cols(const Tile&) const { return N; }
   __device__ __forceinline__ void prefetch() const {
@@ -260,12 +263,16 @@ struct Spot {
   uint32_t buf;
 };
 
-// Epi: begin(spot) once per tile; where INIT, ahead of the product, fetch(spot, column,
-// values[32]) loads what ready(spot, column, values[32]) turns into what it is added to (result =
+// Epi: begin(spot) once per tile; where INIT, fetch(spot, column, values[32]) loads (into zeros)
+// what ready(spot, column, values[32]) turns into what the product is added to (result =
 // values + scale * product); chunk(spot, column, values[32]) for each 32 columns
-// inside the result, end(spot); finish(lane) at the end of the kernel.
-// Work: Product, or a chain of them (CHAIN) whose tiles wait for earlier ones: ready(tile) before
-// its first load, by one thread; the epilogue's begin does the same for what it reads.
+// inside the result, end(spot); adds(): whether there is something to add; finish(lane) at the end of the kernel.
+// Work: Product, or a chain of them (CHAIN) whose tiles wait for earlier ones. Both sides of that
+// have a warp of their own, since a look at a counter in global memory takes 1200 clocks under
+// load and the fence behind a tile's stores 4000 (a tile 23000): warp 2 runs ahead, waits for
+// ready(tile) and counts up `seen` in shared memory, which the loader (and an epilogue that
+// reads(tile)) looks at; warp 3 waits for the epilogue's warps and publishes the tile by
+// done(tile).
 template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Work, typename Epi>
 __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16, Epi& epi) {
   using G = Geo<BN, PAIR, SPLIT>;
@@ -277,7 +284,10 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
   uint64_t* empty_bar = full_bar + STG;
   uint64_t* acc_full = empty_bar + STG;
   uint64_t* acc_empty = acc_full + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* fin_bar = acc_empty + 2;  // CHAIN: the epilogue's warps have stored a tile
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin_bar + 1);
+  volatile int* seen = reinterpret_cast<volatile int*>(tmem_slot + 1);  // CHAIN: tiles that may start; -1: given up
+  volatile int* passed = seen + 1;                                      // CHAIN: tiles that warp 3 has taken over
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
@@ -295,6 +305,10 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], (PAIR ? 2 : 1) * EPI_WARPS);
+    }
+    if constexpr (Work::CHAIN) {
+      mbar_init(fin_bar, EPI_WARPS);
+      *seen = *passed = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -317,6 +331,25 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
+  // a counter in shared memory at `least` or more; false if its writer gave up or takes too long
+  auto counted = [&](volatile int* count, int least) {
+    unsigned long long t0 = 0;
+    while (true) {
+      int v;
+      asm volatile("ld.acquire.cta.shared.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(const_cast<int*>(count))) : "memory");
+      if (v >= least) return true;
+      if (v < 0) return false;
+      if (t0 == 0) t0 = globaltimer();
+      if (globaltimer() - t0 > WAIT_LIMIT_NS) {
+        raise_device_error(B200_ERR_TIMEOUT);
+        return false;
+      }
+    }
+  };
+  auto count = [&](volatile int* count, int value) {
+    asm volatile("st.release.cta.shared.s32 [%0], %1;" ::"r"(smem_u32(const_cast<int*>(count))), "r"(value) : "memory");
+  };
+
   if (warp < EPI_FIRST) {
     if constexpr (G::LEND) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_ISSUE));
     if (warp == 0 && lane == 0) {
@@ -324,10 +357,11 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       bool ok = true;
       for (int t = unit; t < total && ok; t += units) {
         const Tile at = work.at(t);
-        const CUtensorMap *map_a = work.map_a(at), *map_b = work.map_b(at);
-        const int a_mn = work.a_mn(at), b_mn = work.b_mn(at), each = work.blocks_each(at);
+        const int each = work.blocks_each(at);
+        const auto a = work.side_a(at);
+        const auto b = work.side_b(at);
         if constexpr (Work::CHAIN)
-          if (!work.ready(at)) {
+          if (!counted(seen, t / units + 1)) {
             ok = false;
             break;
           }
@@ -342,6 +376,8 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
           }
           if (rank == 0) mbar_expect_tx(&full_bar[s], (PAIR ? 2u : 1u) * G::STAGE);
           const int k0 = kb * BK;
+          const CUtensorMap *map_a = a.map(kb), *map_b = b.map(kb);
+          const int a_mn = a.mn(kb), b_mn = b.mn(kb);
 #pragma unroll
           for (int p = 0; p < G::PLANES; ++p) {
             uint8_t* a_dst = smem + s * G::STAGE + p * G::A_BYTES;
@@ -375,9 +411,9 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       uint32_t tiles = 0;
       for (int t = unit; t < total && ok; t += units, ++tiles) {
         const Tile at = work.kind(t);
-        const int a_mn = work.a_mn(at), b_mn = work.b_mn(at), each = work.blocks_each(at), chunk = work.chunk(at);
-        const uint32_t idesc =
-            (1u << 4) | fmt | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(G::TM >> 4) << 24);
+        const int each = work.blocks_each(at), chunk = work.chunk(at);
+        const auto a = work.side_a(at);
+        const auto sb = work.side_b(at);
         const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
         for (int c0 = kb0; c0 < kb1 && ok; c0 += chunk, ++local) {
           const int b = local & 1;
@@ -395,6 +431,9 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
               break;
             }
             tc_fence_after();
+            const int a_mn = a.mn(kb), b_mn = sb.mn(kb);
+            const uint32_t idesc = (1u << 4) | fmt | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(BN >> 3) << 17) |
+                                   ((uint32_t)(G::TM >> 4) << 24);
             const uint32_t a0 = smem_u32(smem + s * G::STAGE), b0 = a0 + G::PLANES * G::A_BYTES;
 #pragma unroll
             for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
@@ -413,6 +452,24 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
           }
           if (ok) commit<PAIR>(&acc_full[b]);
         }
+      }
+    }
+    if constexpr (Work::CHAIN) {
+      if (warp == 2 && lane == 0) {
+        int n = 0;
+        for (int t = unit; t < total && n >= 0; t += units) {
+          n = work.ready(work.at(t)) ? n + 1 : -1;
+          count(seen, n);
+        }
+      }
+      if (warp == 3 && lane == 0) {
+        int n = 0;
+        for (int t = unit; t < total; t += units, ++n) {
+          if (!mbar_wait(fin_bar, n & 1, 64)) break;
+          count(passed, n + 1);
+          work.done(work.at(t));
+        }
+        count(passed, total);
       }
     }
     if constexpr (TEAM) {  // the epilogue's two meetings
@@ -452,23 +509,29 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       const int64_t col0 = sp.col0 = (int64_t)at.nt * BN + sp.half * (BN / 2);
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
       if constexpr (Work::CHAIN) {
-        if (!epi.enter(work, at, sp)) break;
+        epi.enter(at, sp);
+        if (epi.reads(at) && !counted(seen, t / units + 1)) break;
+        __syncwarp();
       } else {
         epi.begin(sp);
       }
       // the member that finishes chunk c of this warp: of two, each takes a chunk of every warp
       auto owner = [&](int c) { return !TEAM ? 0 : (team == 2 ? c : sp.half * CH + c); };
       if constexpr (SPLIT || TEAM) {
-        float acc[CH][32];
+        // What the product is added to comes first where registers last for it (EARLY); 256-wide
+        // tiles, whose MMAs wait as long as the accumulator is not drained, take it a
+        // chunk ahead while the chunks are stored.
+        constexpr bool EARLY = CH == 2;
+        float acc[CH][32], more[Epi::INIT && !EARLY ? 32 : 1];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) acc[c][i] = 0.f;
           // every chunk's loads are issued before the first is waited for
-          if constexpr (Epi::INIT)
+          if constexpr (Epi::INIT && EARLY)
             if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.fetch(sp, col0 + c * 32, acc[c]);
         }
-        if constexpr (Epi::INIT) {
+        if constexpr (Epi::INIT && EARLY) {
 #pragma unroll
           for (int c = 0; c < CH; ++c)
             if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.ready(sp, col0 + c * 32, acc[c]);
@@ -479,14 +542,24 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
           tmem_wait(cur);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            if constexpr (Epi::INIT) to[i] = fmaf(epi.scale, __uint_as_float(cur[i]), to[i]);
+            if constexpr (Epi::INIT && EARLY) to[i] = fmaf(epi.scale, __uint_as_float(cur[i]), to[i]);
             else to[i] += __uint_as_float(cur[i]);
+          }
+        };
+        auto ahead = [&](int c) {
+          if constexpr (Epi::INIT && !EARLY) {
+            if (!epi.adds()) return;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) more[i] = 0.f;
+            if (col0 + c * 32 < N && sp.row0 < M) epi.fetch(sp, col0 + c * 32, more);
           }
         };
         const int each = work.blocks_each(at), chunk = work.chunk(at);
         const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
         for (int c0 = kb0; c0 < kb1; c0 += chunk, ++local) {
           const int b = local & 1;
+          if constexpr (Epi::INIT && !EARLY)
+            if (c0 + chunk >= kb1) ahead(0);
           if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) {
             ok = false;
             break;
@@ -539,11 +612,33 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
         if (!ok) break;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
-          if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) epi.chunk(sp, col0 + c * 32, acc[c]);  // warp-uniform
+          if (owner(c) == member && col0 + c * 32 < N && sp.row0 < M) {  // warp-uniform
+            if constexpr (Epi::INIT && !EARLY) {
+              if (epi.adds()) {
+                epi.ready(sp, col0 + c * 32, more);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[c][i] = fmaf(epi.scale, acc[c][i], more[i]);
+                if (c + 1 < CH) ahead(c + 1);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) acc[c][i] *= epi.scale;
+              }
+            }
+            epi.chunk(sp, col0 + c * 32, acc[c]);
+          }
           asm volatile("" ::: "memory");  // one chunk at a time: the others wait in registers
         }
       } else {
         const int b = local & 1;
+        float more[Epi::INIT ? 32 : 1];
+        auto ahead = [&](int64_t col) {
+          if constexpr (Epi::INIT) {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) more[i] = 0.f;
+            if (col < N && sp.row0 < M) epi.fetch(sp, col, more);
+          }
+        };
+        ahead(col0);
         if (!mbar_wait(&acc_full[b], (local >> 1) & 1)) break;
         tc_fence_after();
         uint32_t cur[32];
@@ -551,22 +646,20 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
 #pragma unroll 1
         for (int c = 0; c < CH; ++c) {
           const int64_t col = col0 + c * 32;
-          const bool inside = col < N && sp.row0 < M;  // warp-uniform
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
-          if constexpr (Epi::INIT)
-            if (inside) epi.fetch(sp, col, v);
           tmem_wait(cur);
-          if (!inside) break;
-          if constexpr (Epi::INIT) epi.ready(sp, col, v);
+          if (!(col < N && sp.row0 < M)) break;  // warp-uniform
+          float v[32];
+          if constexpr (Epi::INIT) epi.ready(sp, col, more);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            if constexpr (Epi::INIT) v[i] = fmaf(epi.scale, __uint_as_float(cur[i]), v[i]);
+            if constexpr (Epi::INIT) v[i] = fmaf(epi.scale, __uint_as_float(cur[i]), more[i]);
             else v[i] = __uint_as_float(cur[i]);
           }
-          // the next chunk's load is under way while this one is worked on
-          if (c + 1 < CH) tmem_ld32_issue(base + (uint32_t)(b * BN + (c + 1) * 32), cur);
+          // the next chunk's loads are under way while this one is worked on
+          if (c + 1 < CH) {
+            tmem_ld32_issue(base + (uint32_t)(b * BN + (c + 1) * 32), cur);
+            ahead(col + 32);
+          }
           epi.chunk(sp, col, v);
         }
         tmem_wait(cur);
@@ -574,6 +667,11 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
         ++local;
       }
       epi.end(sp);
+      if constexpr (Work::CHAIN) {
+        __syncwarp();
+        // (an arrival two tiles ahead of warp 3 would turn the barrier's phase back)
+        if (lane == 0 && counted(passed, t / units)) mbar_arrive(fin_bar);
+      }
     }
     epi.finish(lane);
   }
