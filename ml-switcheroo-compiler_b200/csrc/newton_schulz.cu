@@ -225,11 +225,11 @@ struct NsEpi {
 // ---- all products of all steps in one launch ----
 // Where the products fill the CTA pairs, each one's last wave of tiles is partial (16 matrices of
 // 1024 x 1024: 160, 160 and 256 tiles for 74 pairs, 10 waves for 7.8) and each launch fills and
-// drains its pipeline. So all tiles of all products form one list, walked by the pairs in
-// turn. A tile waits until its matrix's previous product is complete: counters in the
+// drains its pipeline. So all tiles of all products form one list, taken by the pairs in
+// order. A tile waits until its matrix's previous product is complete: counters in the
 // workspace, one per matrix, of the CTAs that have finished a tile. Every tile depends on
-// earlier ones of the list only, and the launch is cooperative, so the first unfinished
-// tile never waits. What a matrix's buffers hold is overwritten two products after
+// earlier ones of the list only, which running pairs have taken: the first unfinished one
+// never waits, however many pairs are resident. What a matrix's buffers hold is overwritten two products after
 // their last reader at the earliest, which the same counter orders.
 // S and P, symmetric, are stored on and above the diagonal's tiles only (the mirrored half
 // took 6000 clocks a tile, of 15000 for the epilogue): a K block left of the diagonal is read as the
@@ -244,7 +244,7 @@ struct Chain {
   };
   CUtensorMap x_gram[2], x_next[2], s[2], p[2];  // s, p: [1] with the rows adjacent
   One one[3];     // GRAM, POLY, NEXT
-  int* finished;  // [batch]
+  int* finished;  // [batch], then the tickets
   int batch, steps, tall;
   __device__ __forceinline__ int per_step() const { return one[0].per + one[1].per + one[2].per; }
   __device__ __forceinline__ int total() const { return steps * batch * per_step(); }
@@ -285,6 +285,7 @@ struct Chain {
     for (const CUtensorMap* m : {&x_gram[0], &s[0], &p[0], &x_next[0]})
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
   }
+  __device__ __forceinline__ int ticket() const { return atomicAdd(finished + batch, 1); }
   // true once the tile's matrix has seen every product before this one (by one thread); false
   // (and the device error flag set) if that takes too long
   __device__ __forceinline__ bool ready(const Tile& t) const {
@@ -338,7 +339,6 @@ struct ChainEpi : NsEpi<false> {
     if (t.product == POLY) ca = st.ca, scale = st.cc, diag = st.diag;
     shrunk(a->e0[sp.z], st.e_down, st.e_down_next);
   }
-  __device__ __forceinline__ bool reads(const Tile& t) const { return t.product == POLY; }  // S
 };
 
 template <bool SPLIT>
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
   for (int i = 1; i < NT / 32; ++i) s += red[i];
   const double norm = sqrt(s), share = norm / (norm + (double)eps);
   const int e = share > 0.0 && share < 0.5 ? min(96, -1 - ilogb(share)) : 0;  // t share in [1/2, 1)
-  if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e, done[blockIdx.y] = 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e, done[blockIdx.y] = 0, done[gridDim.y] = 0;
   // the factor as two, each within fp32's normal range for any norm of fp32 values
   const double full = ldexp((double)SCALE, e) / (norm + (double)eps);
   const int lg = full > 0.0 && full < 1e300 ? ilogb(full) / 2 : 0;
@@ -495,7 +495,7 @@ static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
   q.x0 = take(xb), q.x1 = take(xb), q.s = take(gb), q.p = take(gb);
   q.part = take((size_t)batch * NORM_BLOCKS * 8);
   q.e0 = take((size_t)batch * 4);
-  q.done = take((size_t)batch * 4);
+  q.done = take((size_t)(batch + 1) * 4);
   q.bytes = at;
   return q;
 }
@@ -534,15 +534,13 @@ static int launch_chain(const Chain& c, const ChainEpi::Args& args, cudaStream_t
   cfg.blockDim = dim3(THREADS, 1, 1);
   cfg.dynamicSmemBytes = G::SMEM;
   cfg.stream = s;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeCooperative;
-  attr[0].val.cooperative = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = 2;
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2;
+  attr.val.clusterDim.y = 1;
+  attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   cudaLaunchKernelEx(&cfg, chain_kernel<SPLIT>, c, args);
   return check_launch(what);
 }

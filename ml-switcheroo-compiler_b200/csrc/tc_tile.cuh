@@ -267,12 +267,13 @@ struct Spot {
 // what ready(spot, column, values[32]) turns into what the product is added to (result =
 // values + scale * product); chunk(spot, column, values[32]) for each 32 columns
 // inside the result, end(spot); adds(): whether there is something to add; finish(lane) at the end of the kernel.
-// Work: Product, or a chain of them (CHAIN) whose tiles wait for earlier ones. Both sides of that
-// have a warp of their own, since a look at a counter in global memory takes 1200 clocks under
-// load and the fence behind a tile's stores 4000 (a tile 23000): warp 2 runs ahead, waits for
-// ready(tile) and counts up `seen` in shared memory, which the loader (and an epilogue that
-// reads(tile)) looks at; warp 3 waits for the epilogue's warps and publishes the tile by
-// done(tile).
+// Work: Product, whose tiles are dealt out in turn, or a chain of them (CHAIN) whose tiles wait
+// for earlier ones and are taken by tickets, in order, by whichever pair comes next. Two warps
+// see to that, since a look at a counter in global memory takes 1200 clocks under load and the
+// fence behind a tile's stores 4000 (a tile 23000). Warp 2 (scout) takes a ticket once the loader
+// has begun the tile before (the leader's, for both CTAs), waits for ready(tile) and shows it to
+// the other warps through a ring in shared memory; warp 3 (herald) waits for the epilogue's
+// warps and publishes the tile by done(tile).
 template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Work, typename Epi>
 __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16, Epi& epi) {
   using G = Geo<BN, PAIR, SPLIT>;
@@ -286,8 +287,10 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* fin_bar = acc_empty + 2;  // CHAIN: the epilogue's warps have stored a tile
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(fin_bar + 1);
-  volatile int* seen = reinterpret_cast<volatile int*>(tmem_slot + 1);  // CHAIN: tiles that may start; -1: given up
-  volatile int* passed = seen + 1;                                      // CHAIN: tiles that warp 3 has taken over
+  // CHAIN, counted in tiles of this CTA: shown to its warps (-1: given up), handed over by the
+  // leader's scout, begun by the loader, taken over by the herald and the peer's; tiles by number % 4
+  int *seen = reinterpret_cast<int*>(tmem_slot + 1), *given = seen + 1, *begun = seen + 2, *passed = seen + 3, *peer_passed = seen + 4;
+  int* ring = seen + 5;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_rank() : 0u;
@@ -308,7 +311,7 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
     }
     if constexpr (Work::CHAIN) {
       mbar_init(fin_bar, EPI_WARPS);
-      *seen = *passed = 0;
+      *seen = *given = *begun = *passed = *peer_passed = 0;
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -332,11 +335,11 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // a counter in shared memory at `least` or more; false if its writer gave up or takes too long
-  auto counted = [&](volatile int* count, int least) {
+  auto counted = [&](const int* count, int least) {
     unsigned long long t0 = 0;
     while (true) {
       int v;
-      asm volatile("ld.acquire.cta.shared.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(const_cast<int*>(count))) : "memory");
+      asm volatile("ld.acquire.cluster.shared::cta.s32 %0, [%1];" : "=r"(v) : "r"(smem_u32(count)) : "memory");
       if (v >= least) return true;
       if (v < 0) return false;
       if (t0 == 0) t0 = globaltimer();
@@ -346,8 +349,18 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       }
     }
   };
-  auto count = [&](volatile int* count, int value) {
-    asm volatile("st.release.cta.shared.s32 [%0], %1;" ::"r"(smem_u32(const_cast<int*>(count))), "r"(value) : "memory");
+  auto count = [&](int* count, int value) {
+    asm volatile("st.release.cta.shared::cta.s32 [%0], %1;" ::"r"(smem_u32(count)), "r"(value) : "memory");
+  };
+  auto at_peer = [&](const int* p) {
+    uint32_t far;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(smem_u32(p)), "r"(rank ^ 1u));
+    return far;
+  };
+  // the n-th tile of this CTA; `total`: no more
+  auto nth = [&](int n) {
+    if constexpr (Work::CHAIN) return counted(seen, n + 1) ? *(volatile int*)&ring[n & 3] : total;
+    else return unit + n * units;
   };
 
   if (warp < EPI_FIRST) {
@@ -355,16 +368,12 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
     if (warp == 0 && lane == 0) {
       uint32_t it = 0;
       bool ok = true;
-      for (int t = unit; t < total && ok; t += units) {
+      for (int n = 0, t; ok && (t = nth(n)) < total; ++n) {
         const Tile at = work.at(t);
+        if constexpr (Work::CHAIN) count(begun, n + 1);
         const int each = work.blocks_each(at);
         const auto a = work.side_a(at);
         const auto b = work.side_b(at);
-        if constexpr (Work::CHAIN)
-          if (!counted(seen, t / units + 1)) {
-            ok = false;
-            break;
-          }
         const int m0 = at.mt * G::TM + (int)rank * BM;
         const int n0 = at.nt * BN + (PAIR ? (int)rank * (BN / 2) : 0);
         const int kb0 = (TEAM ? member : at.split) * each, kb1 = min(work.blocks(at), kb0 + each);
@@ -409,7 +418,7 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       uint32_t it = 0, local = 0;
       bool ok = true;
       uint32_t tiles = 0;
-      for (int t = unit; t < total && ok; t += units, ++tiles) {
+      for (int t; ok && (t = nth((int)tiles)) < total; ++tiles) {
         const Tile at = work.kind(t);
         const int each = work.blocks_each(at), chunk = work.chunk(at);
         const auto a = work.side_a(at);
@@ -456,20 +465,31 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
     }
     if constexpr (Work::CHAIN) {
       if (warp == 2 && lane == 0) {
-        int n = 0;
-        for (int t = unit; t < total && n >= 0; t += units) {
-          n = work.ready(work.at(t)) ? n + 1 : -1;
-          count(seen, n);
+        bool shown = true;
+        for (int n = 0, t = 0; shown && t < total; ++n) {
+          shown = false;
+          if (rank == 0) {
+            if (!counted(begun, n) || !counted(passed, n - 3) || !counted(peer_passed, n - 3)) break;
+            t = work.ticket();
+            ring[n & 3] = t;
+            asm volatile("st.relaxed.cluster.shared::cluster.s32 [%0], %1;" ::"r"(at_peer(&ring[n & 3])), "r"(t) : "memory");
+            asm volatile("st.release.cluster.shared::cluster.s32 [%0], %1;" ::"r"(at_peer(given)), "r"(n + 1) : "memory");
+          } else {
+            if (!counted(given, n + 1)) break;
+            t = *(volatile int*)&ring[n & 3];
+          }
+          shown = t >= total || work.ready(work.at(t));
+          if (shown) count(seen, n + 1);
         }
+        if (!shown) count(seen, -1);
       }
       if (warp == 3 && lane == 0) {
-        int n = 0;
-        for (int t = unit; t < total; t += units, ++n) {
+        for (int n = 0, t; (t = nth(n)) < total; ++n) {
           if (!mbar_wait(fin_bar, n & 1, 64)) break;
           count(passed, n + 1);
+          if (rank != 0) asm volatile("st.release.cluster.shared::cluster.s32 [%0], %1;" ::"r"(at_peer(peer_passed)), "r"(n + 1) : "memory");
           work.done(work.at(t));
         }
-        count(passed, total);
       }
     }
     if constexpr (TEAM) {  // the epilogue's two meetings
@@ -497,7 +517,7 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
         else mbar_arrive(&acc_empty[b]);
       }
     };
-    for (int t = unit; t < total && ok; t += units) {
+    for (int n = 0, t; ok && (t = nth(n)) < total; ++n) {
       const Tile at = work.at(t);
       const int64_t M = work.rows(at), N = work.cols(at);
       sp.z = at.z;
@@ -510,8 +530,6 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       const uint32_t base = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(sp.half * (BN / 2));
       if constexpr (Work::CHAIN) {
         epi.enter(at, sp);
-        if (epi.reads(at) && !counted(seen, t / units + 1)) break;
-        __syncwarp();
       } else {
         epi.begin(sp);
       }
@@ -670,7 +688,7 @@ __device__ __forceinline__ void run_tiles(const Work& work, int team, bool bf16,
       if constexpr (Work::CHAIN) {
         __syncwarp();
         // (an arrival two tiles ahead of warp 3 would turn the barrier's phase back)
-        if (lane == 0 && counted(passed, t / units)) mbar_arrive(fin_bar);
+        if (lane == 0 && counted(passed, n)) mbar_arrive(fin_bar);
       }
     }
     epi.finish(lane);
