@@ -17,7 +17,11 @@
 // t = 2^e >= 1, Y = 2^8 t X is what is stored, b and c are divided by t^2 and t^4, and t
 // shrinks as a makes X grow. t is 1 for any |G| above eps.
 // The sum of squares is in 64 bits. Every sum has a fixed order.
-// Bound by the tensor cores for large matrices, by the chain of 15 launches for one small.
+// Stacks that fill the GPU run all products of all steps in one launch (below): 16 x 1024 x 1024
+// fp32 in 0.91 ms, a pair's 256 x 256 tile of 16 K blocks every 29000 clocks (37000 POLY) for
+// 22900 of MMAs, which write and read shared memory at nearly its rate while the
+// epilogue stages through it. One small matrix is bound by its chain of 15 launches (1024 x 1024
+// fp32: 222 us).
 #include <cuda_fp16.h>
 
 #include <cmath>
@@ -225,7 +229,7 @@ struct NsEpi {
 // ---- all products of all steps in one launch ----
 // Where the products fill the CTA pairs, each one's last wave of tiles is partial (16 matrices of
 // 1024 x 1024: 160, 160 and 256 tiles for 74 pairs, 10 waves for 7.8) and each launch fills and
-// drains its pipeline. So all tiles of all products form one list, taken by the pairs in
+// drains its pipeline (1.39 ms for the optimizer step, 1.08 in one launch). So all tiles of all products form one list, taken by the pairs in
 // order. A tile waits until its matrix's previous product is complete: counters in the
 // workspace, one per matrix, of the CTAs that have finished a tile. Every tile depends on
 // earlier ones of the list only, which running pairs have taken: the first unfinished one
@@ -428,42 +432,56 @@ __global__ void __launch_bounds__(NT) start_kernel(const void* g, int bf16, cons
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = s;
+  __shared__ float factors[2];
   __syncthreads();
-  s = red[0];
-  for (int i = 1; i < NT / 32; ++i) s += red[i];
-  const double norm = sqrt(s), share = norm / (norm + (double)eps);
-  const int e = share > 0.0 && share < 0.5 ? min(96, -1 - ilogb(share)) : 0;  // t share in [1/2, 1)
-  if (blockIdx.x == 0 && threadIdx.x == 0) e0[blockIdx.y] = e, done[blockIdx.y] = 0, done[gridDim.y] = 0;
-  // the factor as two, each within fp32's normal range for any norm of fp32 values
-  const double full = ldexp((double)SCALE, e) / (norm + (double)eps);
-  const int lg = full > 0.0 && full < 1e300 ? ilogb(full) / 2 : 0;
-  const float lift = ldexpf(1.f, lg), scale = (float)ldexp(full, -lg);
+  if (threadIdx.x == 0) {  // (some hundred instructions: as many as a thread's 16 elements)
+    s = red[0];
+    for (int i = 1; i < NT / 32; ++i) s += red[i];
+    const double norm = sqrt(s), share = norm / (norm + (double)eps);
+    const int e = share > 0.0 && share < 0.5 ? min(96, -1 - ilogb(share)) : 0;  // t share in [1/2, 1)
+    if (blockIdx.x == 0) e0[blockIdx.y] = e, done[blockIdx.y] = 0, done[gridDim.y] = 0;
+    // the factor as two, each within fp32's normal range for any norm of fp32 values
+    const double full = ldexp((double)SCALE, e) / (norm + (double)eps);
+    const int lg = full > 0.0 && full < 1e300 ? ilogb(full) / 2 : 0;
+    factors[0] = ldexpf(1.f, lg), factors[1] = (float)ldexp(full, -lg);
+  }
+  __syncthreads();
+  const float lift = factors[0], scale = factors[1];
   const int64_t base = (int64_t)blockIdx.y * rows * cols, per = ld / 8;
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * NT) {
-    const int64_t r = i / per, c = i % per * 8, at = base + r * cols + c;
-    float v[8];
-    if (!mom || nesterov) load8(g, bf16, at, cols - c, v);
-    if (mom) {  // the new momentum
-      float m[8];
-      load8(mom, 0, at, cols - c, m);
+  // two pieces of 8 at a time, both loaded before either is worked on
+  const int64_t total = rows * per, stride = (int64_t)gridDim.x * NT;
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < total; i += 2 * stride) {
+    float v[2][8], m[2][8];
+    __half* d[2];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = nesterov ? v[j] + mu * m[j] : m[j];
+    for (int k = 0; k < 2; ++k) {
+      const int64_t u = i + k * stride, r = u / per, c = u % per * 8, at = base + r * cols + c;
+      const int64_t n = u < total ? cols - c : 0;
+      d[k] = x + (int64_t)blockIdx.y * batch + r * ld + c;
+      if (!mom || nesterov) load8(g, bf16, at, n, v[k]);
+      if (mom) load8(mom, 0, at, n, m[k]);  // the new momentum
     }
-    uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = v[j] * lift * scale;
+    for (int k = 0; k < 2; ++k) {
+      if (i + k * stride >= total) break;
+      uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[2 * j], v[2 * j + 1]);
-    __half* d = x + (int64_t)blockIdx.y * batch + r * ld + c;
-    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-    if (planes > 1) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float a, b;
-        unpack_f16(w[j], a, b);
-        w[j] = pack_f16(v[2 * j] - a, v[2 * j + 1] - b);
+      for (int j = 0; j < 8; ++j) {
+        const float f = !mom ? v[k][j] : (nesterov ? v[k][j] + mu * m[k][j] : m[k][j]);
+        v[k][j] = f * lift * scale;
       }
-      *reinterpret_cast<uint4*>(d + plane) = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = pack_f16(v[k][2 * j], v[k][2 * j + 1]);
+      *reinterpret_cast<uint4*>(d[k]) = make_uint4(w[0], w[1], w[2], w[3]);
+      if (planes > 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float a, b;
+          unpack_f16(w[j], a, b);
+          w[j] = pack_f16(v[k][2 * j] - a, v[k][2 * j + 1] - b);
+        }
+        *reinterpret_cast<uint4*>(d[k] + plane) = make_uint4(w[0], w[1], w[2], w[3]);
+      }
     }
   }
 }
@@ -514,7 +532,11 @@ static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int
   return launch<NsEpi<true>>(A, B, M, N, K, batch, planes, pair, lp, a, s, what);
 }
 
-// One launch where the Gram product (the one with the fewest tiles) would run on pairs
+// One launch where the Gram product (the one with the fewest tiles) fills two thirds of the pairs.
+// Measured, in one launch / as launches (us): fp32 8 x 1024 x 1024 505 / 781, 80 x 256 x 256 285 /
+// 408, 8 x 768 x 3000 1004 / 1126, 17 x 512 x 2048 612 - 688 / 665, bf16 8 x 1024 x 1024 288 / 383, one
+// 4096 x 4096 1219 / 1195; below two thirds the launches' smaller tiles win: fp32 4 x 1024 x 1024
+// 422 / 380, 12 x 512 x 512 310 / 259, one 2048 x 2048 649 / 618.
 static bool chained(int64_t batch, int64_t rows, int64_t cols, int steps) {
   const int64_t side = std::min(rows, cols), t = ceil_div(side, 256), tri = t * (t + 1) / 2;
   const int64_t all = (2 * tri + ceil_div(rows, 256) * ceil_div(cols, 256)) * batch * steps;
@@ -597,7 +619,7 @@ static int run(const Plan& q, const void* g, int dtype, const float* mom, float*
   int rc = check_launch(what);
   if (rc) return rc;
   const int64_t xb = q.planes * q.xn, gb = q.planes * q.gn;
-  const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(rows * (q.ldx / 8), NT), 4 * num_sms());
+  const unsigned gx = (unsigned)std::min<int64_t>(ceil_div(rows * (q.ldx / 8), NT), ceil_div(8 * (int64_t)num_sms(), batch));
   start_kernel<<<dim3(gx, (unsigned)batch), NT, 0, s>>>(g, bf16, mom ? mom_out : nullptr, mu, nesterov, part, parts, eps, e0, done, x[0], q.ldx, q.xn,
                                                         xb, q.planes, rows, cols);
   if ((rc = check_launch(what))) return rc;

@@ -4,8 +4,8 @@
 //
 // Two things are wider than in the graph GEMM (gemm_tc.cu):
 //  * an operand may come as two 16-bit planes, hi + lo of fp32 values (SPLIT; 16 or 22
-//    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is the fp32 product up to lo.lo: a third of the tensor rate
-//    instead of the CUDA cores'. The tensor cores cut (not round) each sum to fp32: up to
+//    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is
+//    the fp32 product up to lo.lo: a third of the tensor rate instead of the CUDA cores'. The tensor cores cut (not round) each sum to fp32: up to
 //    2^-23 of it per 16 products, all towards zero, which over K = 50000 was 1e-4. So the
 //    accumulator is drained every CHUNK K blocks and added up in registers with rounding (48
 //    cuts; 16 in the 128-wide tiles, where hi.lo + lo.hi, 2^-8 to 2^-11 of the whole, have an
@@ -27,6 +27,7 @@
 // TEAM: where single tiles would leave most SMs idle, a cluster of 2 or 4 CTAs shares one
 // tile's K axis; each then sends its partial sums of the columns that another one owns
 // through shared memory (in place of the operands, all read by then) and finishes its own.
+// The loop walks one product, or a chain of them whose tiles wait for each other (run_tiles).
 // Every wait is bounded (tc_common.cuh); on expiry the device error flag is set and the
 // block winds down.
 #pragma once
