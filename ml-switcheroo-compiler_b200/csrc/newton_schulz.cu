@@ -229,12 +229,13 @@ struct NsEpi {
 // ---- all products of all steps in one launch ----
 // Where the products fill the CTA pairs, each one's last wave of tiles is partial (16 matrices of
 // 1024 x 1024: 160, 160 and 256 tiles for 74 pairs, 10 waves for 7.8) and each launch fills and
-// drains its pipeline (1.39 ms for the optimizer step, 1.08 in one launch). So all tiles of all products form one list, taken by the pairs in
-// order. A tile waits until its matrix's previous product is complete: counters in the
-// workspace, one per matrix, of the CTAs that have finished a tile. Every tile depends on
-// earlier ones of the list only, which running pairs have taken: the first unfinished one
-// never waits, however many pairs are resident. What a matrix's buffers hold is overwritten two products after
-// their last reader at the earliest, which the same counter orders.
+// drains its pipeline (the optimizer step: 1.39 ms as launches, 1.09 in one). So all tiles
+// of all products form one list, taken by the pairs in order. A tile waits until its matrix's
+// previous product is complete: counters in the workspace, one per matrix, of the CTAs that
+// have finished a tile. Every tile depends on earlier ones of the list only, which running
+// pairs have taken: the first unfinished one never waits, however many pairs are resident.
+// A matrix's buffers are overwritten two products after their last reader at the
+// earliest, which the same counter orders.
 // S and P, symmetric, are stored on and above the diagonal's tiles only (the mirrored half
 // took 6000 clocks a tile, of 15000 for the epilogue): a K block left of the diagonal is read as the
 // transposed block above it, with the rows adjacent.

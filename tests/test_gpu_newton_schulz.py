@@ -184,6 +184,25 @@ def test_stacks_on_two_streams_and_replayed(shape):
     assert torch.equal(p, want[0]) and torch.equal(m, want[1])
 
 
+def test_stacks_beside_each_other_and_a_loss():
+    """Calls on six streams at once: each list of tiles advances with whatever CTAs it gets."""
+    gs = [grads(*s) for s in ((16, 512, 700), (50, 256, 256), (7, 1024, 600), (20, 300, 520), (300, 200))]
+    x, w = torch.randn(700, 512, device="cuda").to(BF), torch.randn(512, 9000, device="cuda").to(BF)
+    labels = torch.arange(700, device="cuda") * 11
+    want = [op("NewtonSchulz", g) for g in gs] + [op("LinearCrossEntropy", x, w, labels)[0]]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(6)]
+    for turn in range(6):
+        got = []
+        for k, g in enumerate(gs):
+            with torch.cuda.stream(streams[(k + turn) % 6]):
+                got.append(op("NewtonSchulz", g))
+        with torch.cuda.stream(streams[(5 + turn) % 6]):
+            got.append(op("LinearCrossEntropy", x, w, labels)[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("nesterov", [True, False])
 @pytest.mark.parametrize("shape", [(40, 24), (24, 40), (4, 256, 256), (1, 130), (1100, 300), (20, 300, 270)])
 def test_apply_muon(shape, nesterov):
