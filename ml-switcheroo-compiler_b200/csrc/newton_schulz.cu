@@ -2,8 +2,8 @@
 //
 //   X0 = G / (|G|_F + eps);  each step: S = X X^T, P = a I + b S + c S S, X <- P X
 // (X X^T for rows <= cols, X^T X and X <- X P otherwise: the Gram matrix of the shorter
-// side, without a transpose; a on P's diagonal, so that only P's epilogue reads a matrix). Step update: m' = mu m + g, G = g + mu m' (Nesterov)
-// or m', p' = p (1 - lr wd) - lr sqrt(max(1, rows / cols)) X.
+// side, without a transpose; a on P's diagonal, so that only P's epilogue reads a matrix).
+// Step update: m' = mu m + g, G = g + mu m' (Nesterov) or m', p' = p (1 - lr wd) - lr sqrt(max(1, rows / cols)) X.
 //
 // Per step 3 products on the tensor cores (tc_tile.cuh). S and P are symmetric: only the
 // tiles on and above the diagonal are computed, each written twice, so a step costs

@@ -5,7 +5,8 @@
 // Two things are wider than in the graph GEMM (gemm_tc.cu):
 //  * an operand may come as two 16-bit planes, hi + lo of fp32 values (SPLIT; 16 or 22
 //    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is
-//    the fp32 product up to lo.lo: a third of the tensor rate instead of the CUDA cores'. The tensor cores cut (not round) each sum to fp32: up to
+//    the fp32 product up to lo.lo: a third of the tensor rate instead of the CUDA cores'. The
+//    tensor cores cut (not round) each sum to fp32: up to
 //    2^-23 of it per 16 products, all towards zero, which over K = 50000 was 1e-4. So the
 //    accumulator is drained every CHUNK K blocks and added up in registers with rounding (48
 //    cuts; 16 in the 128-wide tiles, where hi.lo + lo.hi, 2^-8 to 2^-11 of the whole, have an
@@ -267,7 +268,8 @@ struct Spot {
 // Epi: begin(spot) once per tile; where INIT, fetch(spot, column, values[32]) loads (into zeros)
 // what ready(spot, column, values[32]) turns into what the product is added to (result =
 // values + scale * product); chunk(spot, column, values[32]) for each 32 columns
-// inside the result, end(spot); adds(): whether there is something to add; finish(lane) at the end of the kernel.
+// inside the result, end(spot); adds(): whether there is something to add; finish(lane) at the
+// end of the kernel. A chain's epilogue has enter(tile, spot) in begin's place.
 // Work: Product, whose tiles are dealt out in turn, or a chain of them (CHAIN) whose tiles wait
 // for earlier ones and are taken by tickets, in order, by whichever pair comes next. Two warps
 // see to that, since a look at a counter in global memory takes 1200 clocks under load and the
@@ -769,8 +771,9 @@ static int resident(int size) {
   return n;
 }
 
-// C [batch][M, N] = A . B with operands of one 16-bit plane, or of two (SPLIT). Fills in the loop's tile counts and launches as many CTAs (or
-// pairs) as are resident, each walking its share of the tiles.
+// C [batch][M, N] = A . B with operands of one 16-bit plane, or of two (SPLIT). Fills in the
+// loop's tile counts and launches as many CTAs (or pairs) as are resident, each walking its
+// share of the tiles.
 template <int BN, bool PAIR, bool SPLIT, bool TEAM, typename Epi>
 static int launch_as(const Operand& A, const Operand& B, int64_t M, int64_t N, int64_t K, int64_t batch, Loop lp,
                      const typename Epi::Args& args, cudaStream_t s, const char* what) {
