@@ -6,7 +6,8 @@
 // Step update: m' = mu m + g, G = g + mu m' (Nesterov) or m', p' = p (1 - lr wd) - lr sqrt(max(1, rows / cols)) X.
 //
 // Per step 3 products on the tensor cores (tc_tile.cuh). S and P are symmetric: only the
-// tiles on and above the diagonal are computed, each written twice, so a step costs
+// tiles on and above the diagonal are computed (each written twice where products are
+// launches of their own), so a step costs
 // 3 m^2 n + m^3 flop (m the shorter side) instead of 4 m^2 n + 2 m^3.
 // Precision. The iterates live in fp16, scaled by 2^8: |X|_F = 1 at the start and the
 // singular values stay below about 1.3, so no entry can pass 2^9 while entries of 2^-20
