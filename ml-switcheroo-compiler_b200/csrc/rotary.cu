@@ -506,10 +506,15 @@ static int launch_fast(const Args& a, bool inter, int grid, cudaStream_t s) {
   return launch<T, 4, 1, true, MODE>(a, inter, grid, s);
 }
 
-// Units a lane: a head of 512 elements is 64 units of whole vectors, or up to 129 of 2-element
-// vectors; an idle unit costs as much as a full one.
+// Units a lane: a head of 512 elements is up to 64 units of whole vectors (FAST_UNITS), or up to
+// 129 of 2-element vectors; an idle unit costs as much as a full one.
+constexpr int FAST_UNITS = 64;
 template <typename T, int MODE>
 static int launch_type(const Args& a, bool fast, int nu, bool inter, int grid, cudaStream_t s) {
+  if (nu > (fast ? 2 : 5)) {
+    set_error("rotary: %d units a head, more than any kernel takes", a.n_units);
+    return B200_ERR_UNSUPPORTED;
+  }
   if (fast) return nu == 1 ? launch_fast<T, MODE>(a, inter, grid, s) : launch<T, 4, 2, true, MODE>(a, inter, grid, s);
   if (nu == 1) return launch<T, 2, 1, false, MODE>(a, inter, grid, s);
   if (nu == 2) return launch<T, 2, 2, false, MODE>(a, inter, grid, s);
@@ -533,9 +538,13 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
     bits |= (uint64_t)(g.x_b | g.x_s | g.x_h | g.y_b | g.y_s | g.y_h | g.d_b | g.d_s | g.d_h) * (uint64_t)size;
     if (bits & (uint64_t)(wide * size - 1)) fast = false;
   }
-  const int V = fast ? wide : 2;
-  a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
-  a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
+  auto units = [&](int V) {
+    a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
+    return a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
+  };
+  // 512 elements whose rotated part, interleaved, and whose rest both end with half a unit are 65
+  if (fast && units(wide) > FAST_UNITS) fast = false;
+  if (!fast) units(2);
   a.L = 1;
   while (a.L < a.n_units && a.L < 32) a.L *= 2;
   // without a reduction the lanes of a head need be no power of two: three heads of 10 units

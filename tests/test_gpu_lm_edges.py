@@ -1,0 +1,69 @@
+"""Edges of the language-model operators that the tests by operator leave out. Definitions in 64
+bits: ``lm_reference``."""
+
+import pytest
+import torch
+
+import lm_reference as R
+
+pytestmark = pytest.mark.gpu
+BF, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _policy(cuda):
+    from b200 import ops
+
+    ops.Config.matmul_dtype = "f32"
+    yield
+    ops.Config.matmul_dtype = "f32"
+
+
+def op(name, *args, **kw):
+    from b200.backend import B200Backend
+
+    return B200Backend.execute_op(name, *args, **kw)
+
+
+def rand(*shape, dtype=F32, seed=0):
+    g = torch.Generator().manual_seed(seed + sum(shape))
+    return torch.randn(*shape, generator=g).to(dtype)
+
+
+# ---- heads ----
+# An fp32 angle is off by its integer's rounding, 2^-25 of pi / 4, and by 2^-24 of the product;
+# the polynomials of sine and cosine by 2^-28 and their few roundings: 1.2e-7 in all. A
+# rotated element adds three roundings of 2^-24 of its terms: 3e-7 (|a| + |b|). The norm adds
+# the fp32 sum of 512 squares (16 a lane, a tree of 5: 21 roundings, halved by the root) and 5
+# roundings of its products: 1e-6. Held to 2e-6 of the terms and half a step of the result's type.
+TERMS = 2e-6
+
+
+def close(got, ref, mag):
+    got = got.cpu()
+    assert ((got.double() - ref).abs() <= R.HALF_STEP[got.dtype] * ref.abs() + TERMS * mag).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("part", [4, 12, 244, 252, 260, 500, 508])
+def test_512_wide_interleaved_heads_of_any_rotated_part(part, dtype):
+    """Both parts end inside a unit of two vectors: one unit more than 64."""
+    b, n, h, hk, d = 2, 5, 3, 1, 512
+    pos = torch.arange(n)[None] + 100 * torch.arange(b)[:, None]
+    kw = {"rotary_dim": part, "interleaved": True}
+    x, k = rand(b, n, h, d, dtype=dtype), rand(b, n, hk, d, dtype=dtype, seed=1)
+    for name, sign in (("RotaryEmbedding", 1), ("RotaryEmbeddingGrad", -1)):
+        close(op(name, x.cuda(), pos.cuda(), **kw), *R.rotate(x.double(), pos, part, interleaved=True, sign=sign))
+    gq, gk = 1 + 0.2 * rand(d, seed=2), 1 + 0.2 * rand(d, seed=3)
+    for y, t, g in zip(op("QKNormRotary", x.cuda(), k.cuda(), gq.cuda(), gk.cuda(), pos.cuda(), **kw), (x, k), (gq, gk)):
+        close(y, *R.rotate(R.rms_unit(t.double(), 1e-6)[0] * g.double(), pos, part, interleaved=True))
+    dy, dk = rand(b, n, h, d, dtype=dtype, seed=8), rand(b, n, hk, d, dtype=dtype, seed=9)
+    got = op("QKNormRotaryGrad", dy.cuda(), dk.cuda(), x.cuda(), k.cuda(), gq.cuda(), gk.cuda(), pos.cuda(), **kw)
+    for dx, dg, t, g, up in zip(got[:2], got[2:], (x, k), (gq, gk), (dy, dk)):
+        gr, mag = R.rotate(up.double(), pos, part, interleaved=True, sign=-1)
+        u, rstd = R.rms_unit(t.double(), 1e-6)
+        ref = rstd * (gr * g.double() - u * (gr * g.double() * u).mean(-1, keepdim=True))
+        m = mag * g.abs().double()
+        close(dx, ref, rstd * (m + u.abs() * (m * u.abs()).mean(-1, keepdim=True)) * 2)
+        # a sum of at most 30 terms in fp32
+        assert ((dg.cpu().double() - (gr * u).sum((0, 1, 2))).abs() <= (mag * u.abs()).sum((0, 1, 2)) * (TERMS + 30 * 2.0**-24)).all()
