@@ -398,7 +398,9 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
               sq += __shfl_xor_sync(0xffffffffu, sq, o);
               hx += __shfl_xor_sync(0xffffffffu, hx, o);
             }
-            const float rstd = rsqrtf(sq * inv_dim + A.eps);
+            // lanes beyond the last head carry zeros: without eps their rstd would be infinite, and
+            // 0 * inf would reach the sums
+            const float rstd = out < end ? rsqrtf(sq * inv_dim + A.eps) : 0.f;
             const float m = -hx * inv_dim * rstd * rstd * rstd;  // -rstd mean(h u) / (u / x)
             const f2 r2 = pair(rstd, rstd), m2 = pair(m, m);
 #pragma unroll

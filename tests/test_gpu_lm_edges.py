@@ -67,3 +67,18 @@ def test_512_wide_interleaved_heads_of_any_rotated_part(part, dtype):
         close(dx, ref, rstd * (m + u.abs() * (m * u.abs()).mean(-1, keepdim=True)) * 2)
         # a sum of at most 30 terms in fp32
         assert ((dg.cpu().double() - (gr * u).sum((0, 1, 2))).abs() <= (mag * u.abs()).sum((0, 1, 2)) * (TERMS + 30 * 2.0**-24)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("heads,dim", [((1, 1), 32), ((3, 1), 32), ((9, 2), 32), ((1, 3), 64), ((5, 1), 64), ((3, 1), 128), ((2, 1), 33)])
+def test_norm_gradient_without_eps_and_idle_lanes(heads, dim, dtype):
+    """Head counts that are no multiple of what a warp takes; eps = 0 is 1e-30 where no row is zero."""
+    q, k = rand(2, 7, heads[0], dim, dtype=dtype), rand(2, 7, heads[1], dim, dtype=dtype, seed=1)
+    dq, dk = rand(*q.shape, dtype=dtype, seed=2), rand(*k.shape, dtype=dtype, seed=3)
+    g = (1 + 0.2 * rand(dim, seed=4)).cuda()
+    args = [t.cuda() for t in (dq, dk, q, k)] + [g, g]
+    got, want = op("QKNormRotaryGrad", *args, eps=0.0, rotary_dim=0), op("QKNormRotaryGrad", *args, eps=1e-30, rotary_dim=0)
+    for a, b in zip(got, want):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    got, want = op("QKNormRotary", *args[2:], eps=0.0, rotary_dim=0), op("QKNormRotary", *args[2:], eps=1e-30, rotary_dim=0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
