@@ -706,15 +706,18 @@ static int64_t slices(int w_dn, int wide, int64_t D, int64_t V) {
 
 template <typename E, int NT, int W>
 static int launch(const Args& a, int w_dn, bool grad, float* dx_part, int64_t n_slices, cudaStream_t s, const char* what) {
-  const size_t x_bytes = (size_t)NT * a.D * 4, red = (size_t)WARPS * NT * 32 * W * 4;
+  // The limit on shared memory is the function's, for all its callers: raised to the most that
+  // any call needs, never to this call's size, below which another thread's launch may need more.
+  constexpr size_t MOST_X = (size_t)X_FLOATS * 4, RED = (size_t)WARPS * NT * 32 * W * 4;
+  const size_t x_bytes = (size_t)NT * a.D * 4;
   const unsigned grid = (unsigned)blocks(w_dn, W > 1, a.V);
   if (w_dn) {
     auto* fn = grad ? columns_kernel<E, NT, W, true> : columns_kernel<E, NT, W, false>;
-    if (x_bytes + red > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(x_bytes + red));
-    fn<<<grid, T, x_bytes + red, s>>>(a);
+    if (x_bytes + RED > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(MOST_X + RED));
+    fn<<<grid, T, x_bytes + RED, s>>>(a);
   } else {
     auto* fn = grad ? words_kernel<E, NT, W, true> : words_kernel<E, NT, W, false>;
-    if (x_bytes + 1024 > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)x_bytes);
+    if (x_bytes + 1024 > 48 * 1024) cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)MOST_X);
     fn<<<grid, T, x_bytes, s>>>(a);
   }
   int rc = check_launch(what);

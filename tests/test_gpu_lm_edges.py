@@ -1,6 +1,8 @@
 """Edges of the language-model operators that the tests by operator leave out. Definitions in 64
 bits: ``lm_reference``."""
 
+import threading
+
 import pytest
 import torch
 
@@ -82,3 +84,59 @@ def test_norm_gradient_without_eps_and_idle_lanes(heads, dim, dtype):
         assert torch.isfinite(a).all() and torch.equal(a, b)
     got, want = op("QKNormRotary", *args[2:], eps=0.0, rotary_dim=0), op("QKNormRotary", *args[2:], eps=1e-30, rotary_dim=0)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- the head's loss ----
+
+
+def inputs(n, d, v, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + n + d + v)
+    r = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    return (r(n, d).to(dtype), (r(d, v) / d**0.5).to(dtype), torch.randint(0, v, (n,), generator=g, device="cuda"),
+            (0.5 + torch.rand(n, generator=g, device="cuda")) / n)
+
+
+@pytest.mark.parametrize("tied", [False, True])
+def test_threads_with_few_tokens_of_different_widths(tied):
+    """Threads that launch the same kernels with different amounts of shared memory above 48 KB: straight
+    through the entry points, so that the calls meet."""
+    from b200 import _lib as L
+
+    lib, calls, results, keep = L.lib(), [], [], []
+    for d in (1508, 1536):
+        x, w, labels, dloss = inputs(8, d, 128, F32)
+        w = w.t().contiguous() if tied else w
+        loss, lse = op("LinearCrossEntropy", x, w.t() if tied else w, labels)
+        dx, dw = op("LinearCrossEntropyGrad", dloss, x, w.t() if tied else w, labels, lse)
+        for _ in range(2):  # two threads each, on streams, workspaces and results of their own
+            s = torch.cuda.Stream()
+            got = [torch.zeros_like(t) for t in (loss, lse, dx, w)]
+            head = (x.data_ptr(), d, w.data_ptr(), w.stride(0), int(not tied))
+            sizes = (8, d, 128)
+            nf, nb = (f(L.F32, *head, *sizes) for f in (lib.b200_linear_xent_workspace_bytes, lib.b200_linear_xent_grad_workspace_bytes))
+            wf, wb = (torch.empty(n, dtype=torch.uint8, device="cuda") for n in (nf, nb))
+            fwd = (L.F32, *head, labels.data_ptr(), L.I64, -100, got[0].data_ptr(), got[1].data_ptr(), *sizes, wf.data_ptr(), nf, s.cuda_stream)
+            bwd = (L.F32, dloss.data_ptr(), *head, labels.data_ptr(), L.I64, -100, lse.data_ptr(), got[2].data_ptr(), got[3].data_ptr(), *sizes,
+                   wb.data_ptr(), nb, s.cuda_stream)
+            calls.append((fwd, bwd))
+            results.append((got, (loss, lse, dx, dw.t() if tied else dw)))
+            keep.append((x, w, labels, dloss, lse, s, wf, wb))
+    torch.cuda.synchronize()
+    start, bad = threading.Barrier(len(calls)), []
+
+    def run(fwd, bwd):
+        start.wait()
+        for _ in range(2000):
+            rc = lib.b200_linear_xent(*fwd) or lib.b200_linear_xent_grad(*bwd)
+            if rc != L.OK:
+                bad.append(rc)
+
+    threads = [threading.Thread(target=run, args=c) for c in calls]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not bad, f"{len(bad)} calls failed, the first with status {bad[0]}"
+    assert all(torch.equal(a, b) for got, want in results for a, b in zip(got, want))
+    assert keep
