@@ -277,7 +277,8 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
 
 
 def _cast(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A fresh cast (of a transposed matrix in its storage order)."""
+    """A fresh cast (of a transposed matrix in its storage order: the layout stays); t itself if
+    it is of that type."""
     return ops.cast(t.t(), dtype).t() if t.dim() == 2 and t.stride(0) == 1 else ops.cast(t, dtype)
 
 
@@ -364,7 +365,7 @@ def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **
     ws = torch.empty(wn, dtype=torch.uint8, device=x.device)
     L.call("b200_linear_xent_grad", dt, dloss.data_ptr(), xp, ldx, wp, ldw, dn, labels.data_ptr(), ops.code(labels), int(ignore_index),
            lse.data_ptr(), dx.data_ptr(), dw.data_ptr(), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
-    return ops.cast(dx, x0.dtype), ops.cast(dw if dn else dw.t(), w0.dtype)
+    return ops.cast(dx, x0.dtype), _cast(dw if dn else dw.t(), w0.dtype)
 
 
 # ----------------------------------------------------------------------------------

@@ -140,3 +140,23 @@ def test_threads_with_few_tokens_of_different_widths(tied):
     assert not bad, f"{len(bad)} calls failed, the first with status {bad[0]}"
     assert all(torch.equal(a, b) for got, want in results for a, b in zip(got, want))
     assert keep
+
+
+@pytest.mark.parametrize("n", [3, 40])
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("policy,x_type,w_type", [("bf16", F32, F32), ("bf16", BF, F32), ("bf16", F32, BF), ("f32", F32, BF), ("f32", BF, F32)])
+def test_gradient_of_a_cast_weight_is_stored_as_the_weight(policy, x_type, w_type, tied, n):
+    from b200 import ops
+
+    ops.Config.matmul_dtype = policy
+    x, w, labels, dloss = inputs(n, 64, 200, BF)
+    x, w = x.to(x_type), w.to(w_type)
+    if tied:
+        w = w.t().contiguous().t()
+    _, lse = op("LinearCrossEntropy", x, w, labels)
+    dx, dw = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert dw.stride() == w.stride() and dw.dtype == w_type and dx.dtype == x_type and dx.is_contiguous()
+    dense = op("LinearCrossEntropyGrad", dloss, x, w.contiguous(), labels, lse)
+    for a, b in zip((dx, dw), dense):
+        # bf16 values of d and of the operands: each a half step of 2^-8 off, in sums of other orders
+        torch.testing.assert_close(a.float(), b.float(), rtol=2.0**-6, atol=2.0**-6 * float(b.float().abs().max()))
