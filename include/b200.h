@@ -591,8 +591,8 @@ int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, c
  * or F32 (both as two bf16 planes, three products: 16 bits of each operand). x has row
  * stride ldx; w is stored [D, V] with row stride ldw (w_dn != 0) or [V, D] (w_dn == 0).
  * labels I64 / I32 [N]; rows of ignore_index get loss 0 and no gradient (and add nothing to
- * dw, whatever x holds there); another label outside [0, V) sets the device error flag,
- * with loss 0 and no gradient. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
+ * dw, whatever x holds there); another label outside [0, V) does the same and sets the device
+ * error flag in the forward. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
  * dense) in the operands' dtype; either may be NULL. Results overlap no input. The workspace's
  * size depends on the pointers' alignment too: give the same ones; it starts on a 256-byte
  * boundary. Results do not depend on the run. Up to 8 tokens of F32, or one of BF16, run in fp32 on the CUDA cores. */

@@ -19,8 +19,8 @@
 // Bound by the tensor cores: 2 N D V flop forward, 6 N D V backward.
 //
 // Up to 8 tokens of fp32, or one of bf16, take kernels of their own (below): reading w bounds them.
-// Rows whose label is ignore_index: loss 0, no gradient, and the row of x they hold is
-// replaced by zeros where dw is made, so whatever it contains stays out.
+// Rows whose label is ignore_index, or outside the vocabulary: loss 0, no gradient, and the row
+// of x they hold is replaced by zeros where dw is made, so whatever it contains stays out.
 #include "tc_tile.cuh"
 
 namespace b200 {
@@ -39,6 +39,9 @@ __device__ __forceinline__ float ex2(float x) {
 __device__ __forceinline__ int64_t label_at(const void* labels, int i32, int64_t row) {
   return i32 ? (int64_t) reinterpret_cast<const int*>(labels)[row] : reinterpret_cast<const long long*>(labels)[row];
 }
+
+// whether a row of this label takes part in the gradients
+__device__ __forceinline__ bool counts(int64_t label, int64_t ignore, int64_t V) { return label != ignore && label >= 0 && label < V; }
 
 // ---- forward epilogue: maxima, sums and the label's logit ----
 struct LseEpi {
@@ -168,7 +171,7 @@ struct GradEpi {
     kept = 0u;
     if (sp.row >= a.N) return;
     const int64_t l = label_at(a.labels, a.labels_i32, sp.row);
-    if (l == a.ignore || l < 0 || l >= a.V) return;
+    if (!counts(l, a.ignore, a.V)) return;
     label = l - a.first;
     kept = ~0u;
     g = a.dloss[sp.row];
@@ -285,15 +288,15 @@ __global__ void __launch_bounds__(256) join_splits_kernel(const float* __restric
 }
 
 // A dense 16-bit operand with 16-byte rows from src [rows, cols] (row stride ld): bf16 copied,
-// fp32 split into two bf16 planes. With labels, the rows of ignored tokens become zeros.
+// fp32 split into two bf16 planes. With labels, the rows of tokens that do not count become zeros.
 template <bool F32>
 __global__ void __launch_bounds__(256) pack_kernel(const void* __restrict__ src, int64_t ld, __nv_bfloat16* __restrict__ out, int64_t ldo,
                                                    int64_t plane, int64_t rows, int64_t cols, const void* labels, int labels_i32,
-                                                   int64_t ignore) {
+                                                   int64_t ignore, int64_t V) {
   const int64_t per = ldo / 8, total = rows * per;  // 8 elements a thread
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per, c = i % per * 8;
-    const bool zero = labels && label_at(labels, labels_i32, r) == ignore;
+    const bool zero = labels && !counts(label_at(labels, labels_i32, r), ignore, V);
     float v[8];
     const int64_t at = r * ld + c;
     if constexpr (F32) {
@@ -382,11 +385,11 @@ __device__ __forceinline__ void set(E* p, const float (&v)[W]) {
   }
 }
 
-// x as fp32 [NT][D] (rows that do not exist, and with `masked` those of ignored tokens, zeros)
+// x as fp32 [NT][D] (rows that do not exist, and with `masked` those of tokens that do not count, zeros)
 template <typename E, int NT>
 __device__ __forceinline__ void load_x(const Args& a, float* xs, bool masked) {
   for (int t = 0; t < NT; ++t) {
-    const bool in = t < a.N && !(masked && label_at(a.labels, a.labels_i32, t) == a.ignore);
+    const bool in = t < a.N && !(masked && !counts(label_at(a.labels, a.labels_i32, t), a.ignore, a.V));
     for (int k = threadIdx.x; k < a.D; k += T) xs[t * a.D + k] = in ? value(reinterpret_cast<const E*>(a.x)[t * a.ldx + k]) : 0.f;
   }
 }
@@ -400,7 +403,7 @@ struct Row {
     kept = false, g = shift = 0.f, label = -1;
     if (t >= a.N) return;
     const int64_t l = label_at(a.labels, a.labels_i32, t);
-    if (l == a.ignore || l < 0 || l >= a.V) return;
+    if (!counts(l, a.ignore, a.V)) return;
     kept = true, label = l, g = a.dloss[t], shift = a.lse[t] * LOG2E;
   }
   __device__ __forceinline__ float grad(float z, int64_t v) const {
@@ -760,13 +763,13 @@ static bool needs_pack(int dtype, const void* p, int64_t ld) {
 }
 
 static int pack(int dtype, const void* src, int64_t ld, __nv_bfloat16* out, int64_t rows, int64_t cols, const void* labels, int labels_i32,
-                int64_t ignore, cudaStream_t s) {
+                int64_t ignore, int64_t V, cudaStream_t s) {
   const int64_t ldo = up8(cols), total = rows * (ldo / 8);
   const unsigned grid = (unsigned)std::min<int64_t>(ceil_div(total, 256), (int64_t)num_sms() * 16);
   if (dtype == B200_F32)
-    pack_kernel<true><<<grid, 256, 0, s>>>(src, ld, out, ldo, rows * ldo, rows, cols, labels, labels_i32, ignore);
+    pack_kernel<true><<<grid, 256, 0, s>>>(src, ld, out, ldo, rows * ldo, rows, cols, labels, labels_i32, ignore, V);
   else
-    pack_kernel<false><<<grid, 256, 0, s>>>(src, ld, out, ldo, rows * ldo, rows, cols, labels, labels_i32, ignore);
+    pack_kernel<false><<<grid, 256, 0, s>>>(src, ld, out, ldo, rows * ldo, rows, cols, labels, labels_i32, ignore, V);
   return check_launch("linear_cross_entropy pack");
 }
 
@@ -838,7 +841,7 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
     return p;
   }
   const size_t xb = (size_t)p.planes * N * up8(D) * 2;
-  // forward x is read as it is where it can be; the gradient's copy has the ignored rows zeroed
+  // forward x is read as it is where it can be; the gradient's copy has zeros for rows that do not count
   if (!grad && needs_pack(dtype, x, ldx)) p.x = take(xb);
   if (needs_pack(dtype, w, ldw)) p.w = take((size_t)p.planes * p.w_rows * up8(p.w_cols) * 2);
   if (!grad) {
@@ -949,12 +952,12 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
   }
   if (lx::needs_pack(dtype, x, ldx)) {
     auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.x);
-    if ((rc = lx::pack(dtype, x, ldx, out, N, D, nullptr, 0, 0, s))) return rc;
+    if ((rc = lx::pack(dtype, x, ldx, out, N, D, nullptr, 0, 0, 0, s))) return rc;
     x = out, ldx = lx::up8(D);
   }
   if (lx::needs_pack(dtype, w, ldw)) {
     auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.w);
-    if ((rc = lx::pack(dtype, w, ldw, out, p.w_rows, p.w_cols, nullptr, 0, 0, s))) return rc;
+    if ((rc = lx::pack(dtype, w, ldw, out, p.w_rows, p.w_cols, nullptr, 0, 0, 0, s))) return rc;
     w = out, ldw = lx::up8(p.w_cols);
   }
   auto* part = reinterpret_cast<float2*>(ws + p.part);
@@ -1007,10 +1010,10 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
   auto* xg = reinterpret_cast<__nv_bfloat16*>(ws + p.xg);
   const int64_t ldg = lx::up8(D);
   // (their logits come out as zeros, which gives no gradient either)
-  if ((rc = lx::pack(dtype, x, ldx, xg, N, D, labels, i32, ignore_index, s))) return rc;
+  if ((rc = lx::pack(dtype, x, ldx, xg, N, D, labels, i32, ignore_index, V, s))) return rc;
   if (lx::needs_pack(dtype, w, ldw)) {
     auto* out = reinterpret_cast<__nv_bfloat16*>(ws + p.w);
-    if ((rc = lx::pack(dtype, w, ldw, out, p.w_rows, p.w_cols, nullptr, 0, 0, s))) return rc;
+    if ((rc = lx::pack(dtype, w, ldw, out, p.w_rows, p.w_cols, nullptr, 0, 0, 0, s))) return rc;
     w = out, ldw = lx::up8(p.w_cols);
   }
   auto* d = reinterpret_cast<__nv_bfloat16*>(ws + p.d);

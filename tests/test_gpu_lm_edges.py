@@ -160,3 +160,24 @@ def test_gradient_of_a_cast_weight_is_stored_as_the_weight(policy, x_type, w_typ
     for a, b in zip((dx, dw), dense):
         # bf16 values of d and of the operands: each a half step of 2^-8 off, in sums of other orders
         torch.testing.assert_close(a.float(), b.float(), rtol=2.0**-6, atol=2.0**-6 * float(b.float().abs().max()))
+
+
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("n", [1, 6, 40, 300])
+def test_labels_outside_give_no_gradient_whatever_x_holds(n, dtype, tied):
+    """As rows of ignore_index do: nothing of a not finite x reaches dw."""
+    from b200 import _lib as L
+    from b200 import ops
+
+    x, w, labels, dloss = inputs(n, 72, 300, dtype)
+    w = w.t().contiguous().t() if tied else w
+    labels[0], labels[-1] = 300, -7
+    _, lse = op("LinearCrossEntropy", x, w, labels)
+    want = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    x[0], x[-1] = float("nan"), float("inf")
+    loss, lse = op("LinearCrossEntropy", x, w, labels)
+    got = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert L.lib().b200_check_device_error(ops.stream_ptr()) == L.ERR_ARG
+    assert loss[0] == 0 and loss[-1] == 0 and not got[0][0].any() and not got[0][-1].any()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
