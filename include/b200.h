@@ -617,8 +617,10 @@ int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t 
  *   apply_muon:    m' = mu m + g; G = g + mu m' (nesterov) or m'; p' = p (1 - lr weight_decay)
  *                  - lr sqrt(max(1, rows / cols)) X. param_out may be param, momentum_out
  *                  momentum; else nothing overlaps.
- * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums; the
- * coefficients have to keep X's entries below 250. Results do not depend on the run. */
+ * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums. X, S
+ * and P = a I + b S + c S S are kept in fp16 times 2^8: the coefficients (finite, |a| < 250;
+ * others are refused) have to keep the entries of all three below 250, or results are infinite
+ * or NaN. Results do not depend on the run. */
 size_t b200_newton_schulz_workspace_bytes(int dtype, int64_t batch, int64_t rows, int64_t cols);
 int b200_newton_schulz(int dtype, const void* g, void* out, int64_t batch, int64_t rows, int64_t cols, const float* coefficients,
                        int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);

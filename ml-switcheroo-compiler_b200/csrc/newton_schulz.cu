@@ -34,7 +34,7 @@ namespace ns {
 
 using namespace tile;
 
-constexpr float SCALE = 256.f;
+constexpr float SCALE = 256.f, MOST_A = 250.f;
 constexpr int NORM_BLOCKS = 296, NT = 256;
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -681,6 +681,13 @@ static int check(const char* what, int64_t batch, int64_t rows, int64_t cols, co
   B200_REQUIRE(batch <= 65535 && rows < (1 << 24) && cols < (1 << 24), "%s: %lld matrices of %lld x %lld are too many or too large", what,
                (long long)batch, (long long)rows, (long long)cols);
   B200_REQUIRE(coef && steps >= 1 && steps <= 100, "%s: %d steps not in [1, 100], or no coefficients", what, steps);
+  for (int i = 0; i < steps; ++i) {
+    // a stands on P's diagonal, in fp16 times 2^8: from 256 on it would be infinite
+    const float a = coef[3 * i], b = coef[3 * i + 1], c = coef[3 * i + 2];
+    B200_REQUIRE(std::fabs(a) < MOST_A && std::isfinite(b) && std::isfinite(c),
+                 "%s: coefficients (%g, %g, %g) of step %d: want finite numbers, the first within %g", what, (double)a, (double)b, (double)c, i,
+                 (double)MOST_A);
+  }
   B200_REQUIRE(eps >= 0.f, "%s: eps %g is negative", what, (double)eps);
   B200_REQUIRE(need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255) == 0),
                "%s: workspace of %zu bytes, %zu needed (256-byte aligned)", what, bytes, need);

@@ -1,0 +1,24 @@
+"""Refusals of the language-model operators that the tests by operator leave out (no kernel runs)."""
+
+import ctypes as C
+
+import pytest
+
+from b200 import _lib as L
+
+P = 256  # a stand-in address: the calls below are refused before anything reads it
+
+
+@pytest.mark.parametrize("step", [0, 4])
+@pytest.mark.parametrize("bad", [(250.0, 0.0, 0.0), (-300.0, 1.0, 1.0), (float("inf"), 0.0, 0.0), (float("nan"), 0.0, 0.0),
+                                 (1.0, float("inf"), 0.0), (1.0, float("nan"), 0.0), (1.0, 0.0, float("-inf")), (1.0, 0.0, float("nan"))])
+def test_coefficients_that_cannot_be_kept_are_refused(bad, step):
+    rows = [(1.0, 0.0, 0.0)] * 5
+    rows[step] = bad
+    c = (C.c_float * 15)(*[v for r in rows for v in r])
+    n = int(L.lib().b200_newton_schulz_workspace_bytes(L.F32, 1, 64, 64))
+    assert L.lib().b200_newton_schulz(L.F32, P, P, 1, 64, 64, c, 5, 0.0, P, n, None) == L.ERR_ARG
+    assert "coefficients" in L.last_error()
+    assert L.lib().b200_apply_muon_f32(P, P, P, P, P, 1, 64, 64, 0.1, 0.9, 1, 0.0, c, 5, 0.0, P, n, None) == L.ERR_ARG
+    good = (C.c_float * 15)(*[249.0, -1000.0, 1000.0] * 5)
+    assert L.lib().b200_newton_schulz(L.F32, None, None, 0, 64, 64, good, 5, 0.0, None, 0, None) == L.OK
