@@ -615,8 +615,10 @@ int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t 
  *   coefficients[3 i ..]: S = X X^T, X = a X + (b S + c S S) X
  *   newton_schulz: out = X, of g's dtype (F32 or BF16)
  *   apply_muon:    m' = mu m + g; G = g + mu m' (nesterov) or m'; p' = p (1 - lr weight_decay)
- *                  - lr sqrt(max(1, rows / cols)) X. param_out may be param, momentum_out
- *                  momentum; else nothing overlaps.
+ *                  - lr sqrt(max(1, rows / cols)) X, the scale of weights [outputs, inputs];
+ *                  for [inputs, outputs] pass lr sqrt(cols / rows) and weight_decay
+ *                  sqrt(rows / cols). param_out may be param, momentum_out momentum; else
+ *                  nothing overlaps.
  * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums. X, S
  * and P = a I + b S + c S S are kept in fp16 times 2^8: the coefficients (finite, |a| < 250;
  * others are refused) have to keep the entries of all three below 250, or results are infinite

@@ -419,17 +419,25 @@ def op_newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, **_):
 
 
 def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,
-                  coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, **_):
+                  coefficients=NEWTON_SCHULZ, eps=1e-7, out=None, output_axis=-2, **_):
     """One step of the orthogonalised momentum update for a matrix or a stack of matrices
     [..., rows, cols], beside ApplyAdam and the others: returns (param', momentum').
 
     momentum' = momentum * buffer + grad; G = grad + momentum * momentum' (nesterov) or
-    momentum'; param' = param (1 - lr weight_decay) - lr sqrt(max(1, rows / cols))
-    NewtonSchulz(G). fp32; lr 0.02 unless given. ``out``: the tensors to write (dense; the
-    inputs themselves for a step in place)."""
+    momentum'; param' = param (1 - lr weight_decay) - lr sqrt(max(1, outputs / inputs))
+    NewtonSchulz(G). ``output_axis``: the axis of the layer's outputs, -2 for matrices
+    [outputs, inputs] (so rows / cols), -1 for Matmul weights [inputs, outputs]. fp32; lr 0.02
+    unless given. ``out``: the tensors to write (dense; the inputs themselves for a step in
+    place)."""
     name = "ApplyMuon"
-    lr = 0.02 if lr is None else float(lr)
+    lr, weight_decay = 0.02 if lr is None else float(lr), float(weight_decay)
     batch, rows, cols = _matrices(name, param)
+    if output_axis not in (-2, -1, param.dim() - 2, param.dim() - 1):
+        raise ValueError(f"{name}: output_axis {output_axis} is not one of a matrix's two axes in {tuple(param.shape)}")
+    if output_axis in (-1, param.dim() - 1) and rows and cols:
+        # the entry point scales by sqrt(max(1, rows / cols)), and decays by lr weight_decay
+        turn = math.sqrt(cols / rows)
+        lr, weight_decay = lr * turn, weight_decay / turn
     if momentum_buffer.shape != param.shape or grad.shape != param.shape:
         raise ValueError(f"{name}: param, momentum and grad must have one shape, got {tuple(param.shape)}, "
                          f"{tuple(momentum_buffer.shape)}, {tuple(grad.shape)}")
@@ -449,7 +457,7 @@ def op_apply_muon(param, momentum_buffer, grad, lr=None, momentum=0.95, nesterov
     wn = L.lib().b200_newton_schulz_workspace_bytes(L.F32, batch, rows, cols)
     ws = torch.empty(wn, dtype=torch.uint8, device=p.device)
     L.call("b200_apply_muon_f32", p.data_ptr(), m.data_ptr(), g.data_ptr(), po.data_ptr(), mo.data_ptr(), batch, rows, cols, lr,
-           float(momentum), int(bool(nesterov)), float(weight_decay), coef, int(steps), float(eps), ws.data_ptr(), wn, ops.stream_ptr())
+           float(momentum), int(bool(nesterov)), weight_decay, coef, int(steps), float(eps), ws.data_ptr(), wn, ops.stream_ptr())
     return po, mo
 
 

@@ -181,3 +181,28 @@ def test_labels_outside_give_no_gradient_whatever_x_holds(n, dtype, tied):
     assert L.lib().b200_check_device_error(ops.stream_ptr()) == L.ERR_ARG
     assert loss[0] == 0 and loss[-1] == 0 and not got[0][0].any() and not got[0][-1].any()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- updates ----
+
+
+@pytest.mark.parametrize("weight_decay", [0.0, 0.1])
+@pytest.mark.parametrize("shape", [(24, 40), (40, 24), (33, 33), (3, 64, 256), (3, 256, 64), (20, 300, 270)])
+def test_apply_muon_scales_by_the_axis_of_the_outputs(shape, weight_decay):
+    """Matmul weights [inputs, outputs]: sqrt(max(1, cols / rows)), and the transpose of the default on
+    the transposed weights. Tolerance: the products' 3e-5 of the step (its derivation stands with
+    the operator's own tests), and four roundings of 2^-24 of what is added."""
+    p, m, g = (rand(*shape, seed=i).cuda() * 0.02 for i in (1, 2, 3))
+    kw = {"lr": 0.05, "momentum": 0.9, "weight_decay": weight_decay}
+    p2, m2 = op("ApplyMuon", p, m, g, output_axis=-1, **kw)
+    rm = 0.9 * m.double() + g.double()
+    step = 0.05 * max(1.0, shape[-1] / shape[-2]) ** 0.5 * R.newton_schulz(g.double() + 0.9 * rm)
+    err = p2.double() - (p.double() * (1 - 0.05 * weight_decay) - step)
+    assert float(err.norm()) <= 3e-5 * float(step.norm()) + 2.0**-22 * float(p.double().norm() + step.norm())
+    turned = op("ApplyMuon", p.mT.contiguous(), m.mT.contiguous(), g.mT.contiguous(), output_axis=len(shape) - 2, **kw)
+    assert float((turned[0].mT.double() - p2.double()).norm()) <= 6e-5 * float(step.norm()) + 2.0**-21 * float(p.double().norm() + step.norm())
+    assert torch.equal(m2, turned[1].mT) and torch.equal(m2, op("ApplyMuon", p, m, g, **kw)[1])
+    pc, mc = p.clone(), m.clone()
+    op("ApplyMuon", pc, mc, g, out=(pc, mc), output_axis=len(shape) - 1, **kw)
+    assert torch.equal(pc, p2) and torch.equal(mc, m2)
+    assert torch.equal(op("ApplyMuon", p, m, g, output_axis=-2, **kw)[0], op("ApplyMuon", p, m, g, **kw)[0])

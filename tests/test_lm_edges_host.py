@@ -3,8 +3,10 @@
 import ctypes as C
 
 import pytest
+import torch
 
 from b200 import _lib as L
+from b200 import lm_ops
 
 P = 256  # a stand-in address: the calls below are refused before anything reads it
 
@@ -22,3 +24,10 @@ def test_coefficients_that_cannot_be_kept_are_refused(bad, step):
     assert L.lib().b200_apply_muon_f32(P, P, P, P, P, 1, 64, 64, 0.1, 0.9, 1, 0.0, c, 5, 0.0, P, n, None) == L.ERR_ARG
     good = (C.c_float * 15)(*[249.0, -1000.0, 1000.0] * 5)
     assert L.lib().b200_newton_schulz(L.F32, None, None, 0, 64, 64, good, 5, 0.0, None, 0, None) == L.OK
+
+
+@pytest.mark.parametrize("axis", [0, 3, -3, None, "rows"])
+def test_apply_muon_refuses_an_axis_that_is_not_the_matrix(axis):
+    t = torch.zeros(2, 4, 5)
+    with pytest.raises(ValueError, match="output_axis"):
+        lm_ops.op_apply_muon(t, t, t, output_axis=axis)
