@@ -14,6 +14,7 @@ import functools
 import math
 from typing import Any, Mapping
 
+import numpy as np
 import torch
 
 from . import _lib as L
@@ -378,14 +379,18 @@ NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # steep at zero: 5 steps bring singul
 @functools.lru_cache(maxsize=64)
 def _coefficients(steps: int, coefficients: tuple) -> Any:
     """The steps' (a, b, c) as the entry points take them: one triple for all, or one each."""
-    rows = (coefficients,) * steps if not isinstance(coefficients[0], tuple) else coefficients
-    if not 1 <= steps <= 100 or len(rows) != steps or any(len(r) != 3 for r in rows):
+    each = any(isinstance(r, tuple) for r in coefficients)
+    rows = coefficients if each else (coefficients,) * steps
+    if not 1 <= steps <= 100 or len(rows) != steps or any(not isinstance(r, tuple) or len(r) != 3 for r in rows):
         raise ValueError(f"Newton-Schulz: {steps} steps (1 to 100) with coefficients {coefficients}: one (a, b, c), or one per step")
     return (ctypes.c_float * (3 * steps))(*[float(v) for r in rows for v in r])
 
 
 def _coef(steps: int, coefficients: Any) -> Any:
-    c = tuple(tuple(r) if isinstance(r, (list, tuple)) else r for r in coefficients)
+    def plain(v: Any) -> Any:
+        return v.tolist() if isinstance(v, (np.ndarray, torch.Tensor)) else v
+
+    c = tuple(tuple(r) if isinstance(r, (list, tuple)) else r for r in map(plain, plain(coefficients)))
     return _coefficients(int(steps), c)
 
 

@@ -2,6 +2,7 @@
 
 import ctypes as C
 
+import numpy as np
 import pytest
 import torch
 
@@ -31,3 +32,15 @@ def test_apply_muon_refuses_an_axis_that_is_not_the_matrix(axis):
     t = torch.zeros(2, 4, 5)
     with pytest.raises(ValueError, match="output_axis"):
         lm_ops.op_apply_muon(t, t, t, output_axis=axis)
+
+
+def test_coefficients_as_arrays_and_without_any():
+    rows = [[4.0, -6.9, 2.9], [3.9, -6.3, 2.6], [1.5, -0.5, 0.25]]
+    flat = [v for r in rows for v in r]
+    for c in (rows, tuple(map(tuple, rows)), np.array(rows), [np.array(r) for r in rows], torch.tensor(rows, dtype=torch.float64)):
+        assert list(lm_ops._coef(3, c)) == [np.float32(v) for v in flat]
+    for c in (rows[0], np.array(rows[0]), [np.float32(v) for v in rows[0]]):
+        assert list(lm_ops._coef(2, c)) == [np.float32(v) for v in rows[0]] * 2
+    for c in ((), [], np.zeros((0, 3)), [1.0, [1.0, 2.0, 3.0], 2.0], np.zeros((3, 2)), np.zeros((2, 3))):
+        with pytest.raises(ValueError, match="Newton-Schulz"):
+            lm_ops._coef(3, c)
