@@ -552,12 +552,13 @@ int b200_peer_allreduce_apply_f32(float* data, int64_t n, const void* bufs_dev, 
  *   qk_norm_rotary:       y = R(x rsqrt(mean(x^2) + eps) gamma) of the queries and the keys
  *   qk_norm_rotary_grad:  dq, dk from the gradients of both results; dgamma_q / dgamma_k
  *                         (fp32 [head_dim], may be NULL) summed over tokens and heads in a
- *                         fixed order
+ *                         fixed order; the workspace is 4-byte aligned
  * Tensors are [batch, seq, heads, head_dim] of dtype F32 or BF16, the head's elements
  * adjacent, element strides of the other axes given (x_b, x_s, x_h and so on; for the
  * gradient 2 x 9: input, upstream gradient, result of the queries, then of the keys). A
- * result may be written over its input (same strides), over no other tensor. gamma: [head_dim] F32 or BF16, NULL: ones. positions (I64 or
- * I32, any sign) have element strides pos_b, pos_s; NULL: offset + index in the sequence. */
+ * result may be written over its input (same strides), over no other tensor. gamma:
+ * [head_dim] F32 or BF16, NULL: ones. positions (I64 or I32, any sign) have element strides
+ * pos_b, pos_s; NULL: offset + index in the sequence. */
 #define B200_ROTARY_MAX_DIM 512
 typedef struct b200_rotary {
   int32_t head_dim, rotary_dim, interleaved;

@@ -674,8 +674,9 @@ extern "C" int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const v
     return B200_OK;
   }
   B200_REQUIRE((!heads_q || (q && dyq && dq)) && (!heads_k || (k && dyk && dk)), "qk_norm_rotary_grad: null tensor");
-  B200_REQUIRE(workspace && workspace_bytes >= b200_qk_norm_rotary_grad_workspace_bytes(r->head_dim),
-               "qk_norm_rotary_grad: workspace of %zu bytes, %zu needed", workspace_bytes,
+  B200_REQUIRE(workspace && workspace_bytes >= b200_qk_norm_rotary_grad_workspace_bytes(r->head_dim) &&
+                   reinterpret_cast<uintptr_t>(workspace) % alignof(float) == 0,
+               "qk_norm_rotary_grad: workspace of %zu bytes, %zu needed (4-byte aligned)", workspace_bytes,
                b200_qk_norm_rotary_grad_workspace_bytes(r->head_dim));
   rot::Args a = {};
   rot::fill(a, r, batch, seq, positions, pos_dtype, pos_b, pos_s, offset);

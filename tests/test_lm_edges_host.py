@@ -44,3 +44,13 @@ def test_coefficients_as_arrays_and_without_any():
     for c in ((), [], np.zeros((0, 3)), [1.0, [1.0, 2.0, 3.0], 2.0], np.zeros((3, 2)), np.zeros((2, 3))):
         with pytest.raises(ValueError, match="Newton-Schulz"):
             lm_ops._coef(3, c)
+
+
+@pytest.mark.parametrize("shift", [1, 2, 3])
+def test_norm_gradient_refuses_a_workspace_between_floats(shift):
+    r = L.Rotary()
+    r.head_dim, r.rotary_dim, r.factor = 64, 64, 1.0
+    n = int(L.lib().b200_qk_norm_rotary_grad_workspace_bytes(64))
+    rc = L.lib().b200_qk_norm_rotary_grad(r, L.BF16, P, P, P, P, P, P, 1, 1, 1, 1, L.I64x18(*[64] * 18), P, P, L.F32, 1e-6, None, L.I64,
+                                          0, 0, 0, P, P, P + shift, n, None)
+    assert rc == L.ERR_ARG and "aligned" in L.last_error()
