@@ -594,7 +594,8 @@ int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const void* dyq, c
  * labels I64 / I32 [N]; rows of ignore_index get loss 0 and no gradient (and add nothing to
  * dw, whatever x holds there); another label outside [0, V) does the same and sets the device
  * error flag in the forward. loss, lse, dloss: fp32 [N]. dx [N, D] and dw (stored as w,
- * dense) in the operands' dtype; either may be NULL. Results overlap no input. The workspace's
+ * dense) in the operands' dtype, or (mixed) each F32 or BF16, rounded once; either may be
+ * NULL. Results overlap no input. The workspace's
  * size depends on the pointers' alignment too: give the same ones; it starts on a 256-byte
  * boundary. Results do not depend on the run. Up to 8 tokens of F32, or one of BF16, run in fp32 on the CUDA cores. */
 size_t b200_linear_xent_workspace_bytes(int dtype, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn, int64_t N,
@@ -607,6 +608,10 @@ size_t b200_linear_xent_grad_workspace_bytes(int dtype, const void* x, int64_t l
 int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn,
                           const void* labels, int label_dtype, int64_t ignore_index, const float* lse, void* dx, void* dw, int64_t N,
                           int64_t D, int64_t V, void* workspace, size_t workspace_bytes, void* stream);
+int b200_linear_xent_grad_mixed(int dtype, const float* dloss, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn,
+                                const void* labels, int label_dtype, int64_t ignore_index, const float* lse, void* dx, int dx_dtype,
+                                void* dw, int dw_dtype, int64_t N, int64_t D, int64_t V, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /* ------------------------------------------------------------------------------
  * Orthogonalising matrices by Newton-Schulz products, and the optimizer step that uses it

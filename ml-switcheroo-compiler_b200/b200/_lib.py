@@ -162,6 +162,10 @@ SIGNATURES = {
         [_I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32, _I64, _P, _P, _P, _I64, _I64, _I64, _P, C.c_size_t, _P],
         C.c_int,
     ),
+    "b200_linear_xent_grad_mixed": (
+        [_I32, _P, _P, _I64, _P, _I64, _I32, _P, _I32, _I64, _P, _P, _I32, _P, _I32, _I64, _I64, _I64, _P, C.c_size_t, _P],
+        C.c_int,
+    ),
     "b200_newton_schulz_workspace_bytes": ([_I32, _I64, _I64, _I64], C.c_size_t),
     "b200_newton_schulz": ([_I32, _P, _P, _I64, _I64, _I64, C.POINTER(_F32), _I32, _F32, _P, C.c_size_t, _P], C.c_int),
     "b200_apply_muon_f32": (

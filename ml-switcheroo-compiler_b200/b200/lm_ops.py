@@ -278,8 +278,7 @@ def op_qk_norm_rotary_grad(dyq, dyk, q, k, gamma_q=None, gamma_k=None, positions
 
 
 def _cast(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """A fresh cast (of a transposed matrix in its storage order: the layout stays); t itself if
-    it is of that type."""
+    """A fresh cast (of a transposed matrix in its storage order); t itself if it is of that type."""
     return ops.cast(t.t(), dtype).t() if t.dim() == 2 and t.stride(0) == 1 else ops.cast(t, dtype)
 
 
@@ -347,7 +346,8 @@ def op_linear_cross_entropy(x, w, labels, ignore_index=-100, **_):
 
 def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **_):
     """(dx, dw) of LinearCrossEntropy for the losses' gradient ``dloss`` (1 / N for a mean),
-    in x's and w's dtype; dw is stored as w is. ``lse`` as the forward returned it. Ignored
+    in x's and w's dtype, rounded once to it whatever the operands are multiplied as; dw is
+    stored as w is. ``lse`` as the forward returned it. Ignored
     rows give no gradient, whatever x holds there. The logits are made again, one piece of
     the vocabulary at a time (at most 512 MiB of their gradient at once)."""
     name = "LinearCrossEntropyGrad"
@@ -359,14 +359,14 @@ def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **
             raise ValueError(f"{name}: {what} {tuple(t.shape)} of x {tuple(x0.shape)}")
     _on_device(name, dloss, lse)
     dloss, lse = (ops.contiguous(ops.cast(t, torch.float32)) for t in (dloss, lse))
-    dx = torch.empty(*lead, D, dtype=x.dtype, device=x.device)
-    dw = torch.empty((D, V) if dn else (V, D), dtype=w.dtype, device=w.device)
+    dx = torch.empty(*lead, D, dtype=x0.dtype, device=x.device)
+    dw = torch.empty((D, V) if dn else (V, D), dtype=w0.dtype, device=w.device)
     dt, xp, wp = ops.code(x), x.data_ptr(), w.data_ptr()
     wn = L.lib().b200_linear_xent_grad_workspace_bytes(dt, xp, ldx, wp, ldw, dn, N, D, V)
     ws = torch.empty(wn, dtype=torch.uint8, device=x.device)
-    L.call("b200_linear_xent_grad", dt, dloss.data_ptr(), xp, ldx, wp, ldw, dn, labels.data_ptr(), ops.code(labels), int(ignore_index),
-           lse.data_ptr(), dx.data_ptr(), dw.data_ptr(), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
-    return ops.cast(dx, x0.dtype), _cast(dw if dn else dw.t(), w0.dtype)
+    L.call("b200_linear_xent_grad_mixed", dt, dloss.data_ptr(), xp, ldx, wp, ldw, dn, labels.data_ptr(), ops.code(labels), int(ignore_index),
+           lse.data_ptr(), dx.data_ptr(), ops.code(dx), dw.data_ptr(), ops.code(dw), N, D, V, ws.data_ptr(), wn, ops.stream_ptr())
+    return dx, dw if dn else dw.t()
 
 
 # ----------------------------------------------------------------------------------

@@ -351,6 +351,7 @@ struct Args {
   float* picked;
   float* d;        // backward: [N][V]
   void* dw;
+  int dw_bf16;
 };
 
 template <typename E>
@@ -383,6 +384,13 @@ __device__ __forceinline__ void set(E* p, const float (&v)[W]) {
     if constexpr (W == 1) *p = __float2bfloat16_rn(v[0]);
     else *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
   }
+}
+
+// W elements of dw from the at-th on
+template <int W>
+__device__ __forceinline__ void set_dw(const Args& a, int64_t at, const float (&v)[W]) {
+  if (a.dw_bf16) set<__nv_bfloat16, W>(reinterpret_cast<__nv_bfloat16*>(a.dw) + at, v);
+  else set<float, W>(reinterpret_cast<float*>(a.dw) + at, v);
 }
 
 // x as fp32 [NT][D] (rows that do not exist, and with `masked` those of tokens that do not count, zeros)
@@ -495,7 +503,7 @@ __global__ void __launch_bounds__(T) words_kernel(const __grid_constant__ Args a
         }
 #pragma unroll
         for (int j = 0; j < P; ++j)
-          if (v0 + j < a.V) set<E, W>(reinterpret_cast<E*>(a.dw) + (v0 + j) * a.D + k, o[j]);
+          if (v0 + j < a.V) set_dw<W>(a, (v0 + j) * a.D + k, o[j]);
       }
     }
   }
@@ -580,7 +588,6 @@ __global__ void __launch_bounds__(T) columns_kernel(const __grid_constant__ Args
     for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int i = 0; i < W; ++i) d[t][i] = t < a.N ? red[t * 32 * W + lane * W + i] : 0.f;
-    E* out = reinterpret_cast<E*>(a.dw) + c;
 #pragma unroll 2
     for (int k = warp; k < a.D; k += WARPS) {
       float o[W] = {};
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(T) columns_kernel(const __grid_constant__ Args
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < W; ++i) o[i] = fmaf(d[t][i], xs[t * a.D + k], o[i]);
-      set<E, W>(out + (int64_t)k * a.V, o);
+      set_dw<W>(a, c + (int64_t)k * a.V, o);
     }
   }
 }
@@ -945,7 +952,7 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
   const int i32 = label_dtype == B200_I32;
   if (p.few) {
     lx::few::Args f = {x, w, labels, nullptr, nullptr, ldx, ldw, ignore_index, i32, (int)N, (int)D, (int)V,
-                       reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.picked), nullptr, nullptr};
+                       reinterpret_cast<float2*>(ws + p.part), reinterpret_cast<float*>(ws + p.picked), nullptr, nullptr, 0};
     if ((rc = lx::few::run(dtype, f, p.w_dn, p.wide, false, nullptr, 0, s, what))) return rc;
     lx::lse_join_kernel<<<1, 32 * lx::JOIN, 0, s>>>(f.part, (int)p.parts, f.picked, labels, i32, ignore_index, loss, lse, N, V);
     return check_launch(what);
@@ -980,15 +987,25 @@ extern "C" int b200_linear_xent(int dtype, const void* x, int64_t ldx, const voi
 extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn,
                                      const void* labels, int label_dtype, int64_t ignore_index, const float* lse, void* dx, void* dw,
                                      int64_t N, int64_t D, int64_t V, void* workspace, size_t workspace_bytes, void* stream) {
+  return b200_linear_xent_grad_mixed(dtype, dloss, x, ldx, w, ldw, w_dn, labels, label_dtype, ignore_index, lse, dx, dtype, dw, dtype, N, D,
+                                     V, workspace, workspace_bytes, stream);
+}
+
+extern "C" int b200_linear_xent_grad_mixed(int dtype, const float* dloss, const void* x, int64_t ldx, const void* w, int64_t ldw, int w_dn,
+                                           const void* labels, int label_dtype, int64_t ignore_index, const float* lse, void* dx,
+                                           int dx_dtype, void* dw, int dw_dtype, int64_t N, int64_t D, int64_t V, void* workspace,
+                                           size_t workspace_bytes, void* stream) {
   const char* what = "linear_cross_entropy_grad";
   int rc = lx::check_sizes(what, dtype, N, D, V);
+  if (!rc) rc = lx::check_sizes(what, dx_dtype, N, D, V);
+  if (!rc) rc = lx::check_sizes(what, dw_dtype, N, D, V);
   if (rc) return rc;
   w_dn = w_dn != 0;
   const lx::Plan p = lx::plan(true, dtype, x, ldx, w, ldw, w_dn, N, D, V);
   rc = lx::check(what, dtype, x, ldx, w, ldw, w_dn, labels, label_dtype, N, D, V, workspace, workspace_bytes, N ? p.bytes : 0);
   if (rc) return rc;
   cudaStream_t s = as_stream(stream);
-  const int64_t size = dtype == B200_F32 ? 4 : 2;
+  const int64_t size = dw_dtype == B200_F32 ? 4 : 2;
   if (N == 0) {
     if (dw && cudaMemsetAsync(dw, 0, (size_t)(D * V * size), s) != cudaSuccess) return check_launch(what);
     return B200_OK;
@@ -996,15 +1013,15 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
   B200_REQUIRE(dloss && lse, "%s: null tensor", what);
   B200_REQUIRE(dx || dw, "%s: no result asked for", what);
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
-  const int i32 = label_dtype == B200_I32, bf16 = dtype == B200_BF16;
+  const int i32 = label_dtype == B200_I32, dx_bf16 = dx_dtype == B200_BF16, dw_bf16 = dw_dtype == B200_BF16;
   if (p.few) {
     lx::few::Args f = {x, w, labels, dloss, lse, ldx, ldw, ignore_index, i32, (int)N, (int)D, (int)V,
-                       nullptr, nullptr, reinterpret_cast<float*>(ws + p.d), dw};
+                       nullptr, nullptr, reinterpret_cast<float*>(ws + p.d), dw, dw_bf16};
     // dw is written dense: its rows too have to take vectors
-    const int wide = p.wide && reinterpret_cast<uintptr_t>(dw) % (bf16 ? 8 : 16) == 0;
+    const int wide = p.wide && reinterpret_cast<uintptr_t>(dw) % (dw_bf16 ? 8 : 16) == 0;
     float* part = dx ? reinterpret_cast<float*>(ws + p.split) : nullptr;
     if ((rc = lx::few::run(dtype, f, w_dn, wide, true, part, p.slices, s, what)) || !dx) return rc;
-    lx::few::join_slices_kernel<<<(unsigned)ceil_div(N * D, 32), 1024, 0, s>>>(part, (int)p.slices, N * D, dx, bf16);
+    lx::few::join_slices_kernel<<<(unsigned)ceil_div(N * D, 32), 1024, 0, s>>>(part, (int)p.slices, N * D, dx, dx_bf16);
     return check_launch(what);
   }
   auto* xg = reinterpret_cast<__nv_bfloat16*>(ws + p.xg);
@@ -1042,15 +1059,15 @@ extern "C" int b200_linear_xent_grad(int dtype, const float* dloss, const void* 
       tile::Operand Wt = W;
       Wt.mn = !w_dn;
       const bool last = first + width >= V;
-      rc = lx::product(Dk, Wt, N, D, width, p.planes, last ? dx : acc, D, last ? bf16 : 0, first ? acc : nullptr, split, s, what);
+      rc = lx::product(Dk, Wt, N, D, width, p.planes, last ? dx : acc, D, last ? dx_bf16 : 0, first ? acc : nullptr, split, s, what);
       if (rc) return rc;
     }
     if (dw) {
       tile::Operand Xm = X;
       Xm.mn = 1;
       uint8_t* out = reinterpret_cast<uint8_t*>(dw) + (w_dn ? first : first * D) * size;
-      rc = w_dn ? lx::product(Xm, Dm, D, width, N, p.planes, out, V, bf16, nullptr, split, s, what)
-                : lx::product(Dm, Xm, width, D, N, p.planes, out, D, bf16, nullptr, split, s, what);
+      rc = w_dn ? lx::product(Xm, Dm, D, width, N, p.planes, out, V, dw_bf16, nullptr, split, s, what)
+                : lx::product(Dm, Xm, width, D, N, p.planes, out, D, dw_bf16, nullptr, split, s, what);
       if (rc) return rc;
     }
   }

@@ -183,6 +183,37 @@ def test_labels_outside_give_no_gradient_whatever_x_holds(n, dtype, tied):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("n,d,v", [(1, 64, 200), (1, 7, 64), (5, 64, 201), (140, 64, 333), (20000, 64, 16001)])
+def test_gradients_are_rounded_to_the_callers_types_only(n, d, v, tied):
+    """fp32 x and w under the bf16 policy: bf16 operands and fp32 gradients. Tolerance: that of bf16
+    operands (d half a step of 2^-8 off, fp32 sums cut by 2^-23 an addition of 16 products) without a
+    bf16 rounding of the result."""
+    from b200 import ops
+
+    x, w, labels, dloss = inputs(n, d, v, BF)
+    if tied:
+        w = w.t().contiguous().t()
+    ops.Config.matmul_dtype = "bf16"
+    _, lse = op("LinearCrossEntropy", x.float(), w.float(), labels)
+    dx, dw = op("LinearCrossEntropyGrad", dloss, x.float(), w.float(), labels, lse)
+    narrow = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert dx.dtype == dw.dtype == F32 and torch.equal(dx.to(BF), narrow[0]) and torch.equal(dw.to(BF), narrow[1])
+    assert float((dx != narrow[0].float()).float().mean()) > 0.5 and float((dw != narrow[1].float()).float().mean()) > 0.5
+    half = op("LinearCrossEntropyGrad", dloss, x.float(), w, labels, lse)
+    assert torch.equal(half[0], dx) and torch.equal(half[1], narrow[1]) and half[1].dtype == BF
+    if n > 1000:
+        return
+    x64, w64 = x.double(), w.double()
+    *_, rdx, rdw, dl = R.linear_xent(x64, w64, labels, dloss=dloss.double())
+    cut = lambda k: (k / 16 + 4) * 2.0**-23  # noqa: E731
+    er = (x64.abs() @ w64.abs()).max(-1).values * cut(d) + 2.0**-21
+    ed = torch.softmax(x64 @ w64, -1) * dloss.double()[:, None] * (2 * er[:, None] + 2.0**-20) + dl.abs() * 2.0**-8 + 2.0**-126
+    for got, ref, tol in ((dx, rdx, ed @ w64.abs().t() + (dl.abs() @ w64.abs().t()) * cut(v)),
+                          (dw, rdw, x64.abs().t() @ ed + (x64.abs().t() @ dl.abs()) * cut(n))):
+        assert ((got.double() - ref).abs() <= tol + R.HALF_STEP[F32] * ref.abs()).all()
+
+
 # ---- updates ----
 
 

@@ -54,3 +54,13 @@ def test_norm_gradient_refuses_a_workspace_between_floats(shift):
     rc = L.lib().b200_qk_norm_rotary_grad(r, L.BF16, P, P, P, P, P, P, 1, 1, 1, 1, L.I64x18(*[64] * 18), P, P, L.F32, 1e-6, None, L.I64,
                                           0, 0, 0, P, P, P + shift, n, None)
     assert rc == L.ERR_ARG and "aligned" in L.last_error()
+
+
+def test_loss_gradient_refuses_other_result_types():
+    n = int(L.lib().b200_linear_xent_grad_workspace_bytes(L.BF16, P, 64, P, 104, 1, 4, 64, 100))
+
+    def grad(dx_type, dw_type):
+        return L.lib().b200_linear_xent_grad_mixed(L.BF16, P, P, 64, P, 104, 1, P, L.I64, -100, P, P, dx_type, P, dw_type, 4, 64, 100, P, n, None)
+
+    for bad in (L.I32, L.F64, L.BOOL):
+        assert grad(bad, L.F32) == grad(L.BF16, bad) == L.ERR_DTYPE
