@@ -55,7 +55,7 @@ struct Args {
   int pos_i32, gamma_bf16;
   int tokens, seq, dim, part;
   int L, chunks, per_chunk;  // lanes per head; head groups per token are cut into chunks of per_chunk
-  int n_rot, n_units;        // units that rotate, units in all
+  int n_rot, n_units;        // units that rotate (by halves), units in all
   float eps, factor, sign;
   float* partial;  // [grid, 2, dim] sums of g u (NORM_GRAD)
   uint64_t freq[B200_ROTARY_MAX_DIM / 2];
@@ -193,22 +193,29 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
   const int L = LANES ? LANES : A.L, sub = lane / L, u0 = lane % L, R = 32 / L;
   // this lane's units: element offsets, how many elements of each vector exist, first pair
   int o0[NU], o1[NU], n0[NU], n1[NU], f0[NU];
-  bool rot[NU];
+  bool rot[NU], rot_b[NU];  // whether the unit's first vector turns, and its second
 #pragma unroll
   for (int k = 0; k < NU; ++k) {
     const int u = sub < R ? u0 + L * k : A.n_units;  // lanes beyond the last whole head have none
     rot[k] = u < A.n_rot;
     f0[k] = u * V;
-    if (rot[k] && !INTER) {
+    rot_b[k] = rot[k];
+    if (INTER) {
+      o0[k] = 2 * u * V;
+      o1[k] = o0[k] + V;
+      rot[k] = o0[k] < A.part;
+      rot_b[k] = o1[k] < A.part;
+      n0[k] = u < A.n_units ? max(0, min(V, A.dim - o0[k])) : 0;
+      n1[k] = u < A.n_units ? max(0, min(V, A.dim - o1[k])) : 0;
+    } else if (rot[k]) {
       o0[k] = u * V;
       o1[k] = half + u * V;
       n0[k] = n1[k] = min(V, half - u * V);
     } else {
-      const int end = rot[k] ? A.part : A.dim;
-      o0[k] = rot[k] ? 2 * u * V : A.part + 2 * (u - A.n_rot) * V;
+      o0[k] = A.part + 2 * (u - A.n_rot) * V;
       o1[k] = o0[k] + V;
-      n0[k] = u < A.n_units ? max(0, min(V, end - o0[k])) : 0;
-      n1[k] = u < A.n_units ? max(0, min(V, end - o1[k])) : 0;
+      n0[k] = u < A.n_units ? max(0, min(V, A.dim - o0[k])) : 0;
+      n1[k] = u < A.n_units ? max(0, min(V, A.dim - o1[k])) : 0;
     }
   }
   f2 acc[2][2][NU][P];  // [tensor][vector][unit][elements]: sums of g u
@@ -302,10 +309,9 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
           const f2 x = a[k][i], y = b[k][i];
           a[k][i] = mul2(x, m1[0][k][i]);
           b[k][i] = mul2(y, m1[1][k][i]);
-          if (rot[k]) {  // elements that only pass see nothing of a partner
-            a[k][i] = fma2(INTER ? swapped(x) : y, m2[0][k][i], a[k][i]);
-            b[k][i] = fma2(INTER ? swapped(y) : x, m2[1][k][i], b[k][i]);
-          }
+          // elements that only pass see nothing of a partner
+          if (rot[k]) a[k][i] = fma2(INTER ? swapped(x) : y, m2[0][k][i], a[k][i]);
+          if (INTER ? rot_b[k] : rot[k]) b[k][i] = fma2(INTER ? swapped(y) : x, m2[1][k][i], b[k][i]);
         }
     };
 #pragma unroll
@@ -508,9 +514,8 @@ static int launch_fast(const Args& a, bool inter, int grid, cudaStream_t s) {
   return launch<T, 4, 1, true, MODE>(a, inter, grid, s);
 }
 
-// Units a lane: a head of 512 elements is up to 64 units of whole vectors (FAST_UNITS), or up to
-// 129 of 2-element vectors; an idle unit costs as much as a full one.
-constexpr int FAST_UNITS = 64;
+// Units a lane: a head of 512 elements is 64 units of whole vectors, or up to 129 of 2-element
+// vectors; an idle unit costs as much as a full one.
 template <typename T, int MODE>
 static int launch_type(const Args& a, bool fast, int nu, bool inter, int grid, cudaStream_t s) {
   if (nu > (fast ? 2 : 5)) {
@@ -540,13 +545,10 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
     bits |= (uint64_t)(g.x_b | g.x_s | g.x_h | g.y_b | g.y_s | g.y_h | g.d_b | g.d_s | g.d_h) * (uint64_t)size;
     if (bits & (uint64_t)(wide * size - 1)) fast = false;
   }
-  auto units = [&](int V) {
-    a.n_rot = r->interleaved ? (int)ceil_div(r->rotary_dim, 2 * V) : (int)ceil_div(half, V);
-    return a.n_units = a.n_rot + (int)ceil_div(rest, 2 * V);
-  };
-  // 512 elements whose rotated part, interleaved, and whose rest both end with half a unit are 65
-  if (fast && units(wide) > FAST_UNITS) fast = false;
-  if (!fast) units(2);
+  const int V = fast ? wide : 2;
+  // (interleaved, a unit may hold the rotated part's last vector and the first that passes)
+  a.n_rot = (int)ceil_div(half, V);
+  a.n_units = r->interleaved ? (int)ceil_div(r->head_dim, 2 * V) : a.n_rot + (int)ceil_div(rest, 2 * V);
   a.L = 1;
   while (a.L < a.n_units && a.L < 32) a.L *= 2;
   // without a reduction the lanes of a head need be no power of two: three heads of 10 units
