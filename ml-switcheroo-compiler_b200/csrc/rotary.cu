@@ -29,6 +29,7 @@
 // time (f32x2 products), the weights are folded into the rotation's coefficients
 // (y = rstd (x k1 + partner k2)), and row pointers advance by additions.
 #include <algorithm>
+#include <limits>
 
 #include "common.cuh"
 
@@ -404,9 +405,7 @@ __global__ void __launch_bounds__(THREADS, MODE == ROTATE ? 4 : (MODE == NORM ? 
               sq += __shfl_xor_sync(0xffffffffu, sq, o);
               hx += __shfl_xor_sync(0xffffffffu, hx, o);
             }
-            // lanes beyond the last head carry zeros: without eps their rstd would be infinite, and
-            // 0 * inf would reach the sums
-            const float rstd = out < end ? rsqrtf(sq * inv_dim + A.eps) : 0.f;
+            const float rstd = rsqrtf(sq * inv_dim + A.eps);
             const float m = -hx * inv_dim * rstd * rstd * rstd;  // -rstd mean(h u) / (u / x)
             const f2 r2 = pair(rstd, rstd), m2 = pair(m, m);
 #pragma unroll
@@ -683,7 +682,10 @@ extern "C" int b200_qk_norm_rotary_grad(const b200_rotary* r, int dtype, const v
   rot::Args a = {};
   rot::fill(a, r, batch, seq, positions, pos_dtype, pos_b, pos_s, offset);
   a.sign = -1.f;
-  a.eps = eps;
+  // Lanes beyond the last head carry zeros into the sums. Without eps their rstd would be infinite,
+  // and 0 * inf NaN; the smallest number that is not zero makes it 2.7e22 and changes no mean square of
+  // 2^-124 or more. (A select per row in the kernel cost 1 % of its time.)
+  a.eps = std::max(eps, std::numeric_limits<float>::denorm_min());
   a.gamma_bf16 = gamma_dtype == B200_BF16;
   a.partial = reinterpret_cast<float*>(workspace);
   const int64_t* t = strides;
