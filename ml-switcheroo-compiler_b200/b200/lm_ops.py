@@ -349,7 +349,8 @@ def op_linear_cross_entropy_grad(dloss, x, w, labels, lse, ignore_index=-100, **
     in x's and w's dtype, rounded once to it whatever the operands are multiplied as; dw is
     stored as w is. ``lse`` as the forward returned it. Ignored
     rows give no gradient, whatever x holds there. The logits are made again, one piece of
-    the vocabulary at a time (at most 512 MiB of their gradient at once)."""
+    the vocabulary at a time: at most 512 MiB of their gradient at once up to 2^20 tokens (2^19
+    of fp32 operands), 256 words of it beyond."""
     name = "LinearCrossEntropyGrad"
     x0, w0 = x, w
     x, w, labels, ldx, ldw, dn, N, D, V = _head(name, x, w, labels)
