@@ -694,10 +694,11 @@ __global__ void __launch_bounds__(1024) join_slices_kernel(const float* __restri
 
 // tokens rounded up to a kernel's 1, 2, 4 or 8
 static int rounded(int64_t N) { return N <= 1 ? 1 : (N <= 2 ? 2 : (N <= 4 ? 4 : 8)); }
-// Where these kernels are the faster ones (1024 x 32000, us forward / gradient, w stored [V, D]
-// and [D, V]): fp32 up to 8 tokens (1: 29 / 71 and 44 / 90, 8: 52 / 143 and 54 / 154, the tiles
-// 94 / 147 at 9), bf16 for one (15 / 51 and 19 / 60; two take 18 / 58 and 31 / 77, the tiles
-// 19 / 63 and 20 / 63). x has to fit shared memory.
+// Where these kernels are the faster ones for both layouts of w (1024 x 32000, us forward / gradient,
+// w stored [V, D] and [D, V]): fp32 up to 8 tokens (1: 28 / 73 and 42 / 91, 8: 52 / 143 and
+// 53 / 147, the tiles 94 / 147 at 9), bf16 for one (15 / 47 and 19 / 56). Two bf16 tokens take 18 / 58
+// and 31 / 77 here, 19 / 63 and 20 / 63 by the tiles, which have them: [V, D] alone gains too little
+// for a rule of its own. x has to fit shared memory.
 static bool fits(int dtype, int64_t N, int64_t D) { return N <= (dtype == B200_F32 ? MOST : 1) && rounded(N) * D <= X_FLOATS; }
 // blocks of the first kernel: word rows by the SMs, or one per 32 W columns
 static int64_t blocks(int w_dn, int wide, int64_t V) {

@@ -536,9 +536,10 @@ static int product(const Operand& A, const Operand& B, int64_t M, int64_t N, int
 
 // One launch where the Gram product (the one with the fewest tiles) fills two thirds of the pairs.
 // Measured, in one launch / as launches (us): fp32 8 x 1024 x 1024 505 / 781, 80 x 256 x 256 285 /
-// 408, 8 x 768 x 3000 1004 / 1126, 17 x 512 x 2048 612 - 688 / 665, bf16 8 x 1024 x 1024 288 / 383, one
-// 4096 x 4096 1219 / 1195; below two thirds the launches' smaller tiles win: fp32 4 x 1024 x 1024
-// 422 / 380, 12 x 512 x 512 310 / 259, one 2048 x 2048 649 / 618.
+// 408, 8 x 768 x 3000 1004 / 1126, bf16 8 x 1024 x 1024 288 / 383; even, and left to the rule: fp32
+// 17 x 512 x 2048 612 - 688 / 665 (51 Gram tiles, just past two thirds), one bf16 4096 x 4096 1219 / 1195
+// (large products lose little between launches). Below two thirds the launches' smaller tiles win: fp32
+// 4 x 1024 x 1024 422 / 380, 12 x 512 x 512 310 / 259, one 2048 x 2048 649 / 618.
 static bool chained(int64_t batch, int64_t rows, int64_t cols, int steps) {
   const int64_t side = std::min(rows, cols), t = ceil_div(side, 256), tri = t * (t + 1) / 2;
   const int64_t all = (2 * tri + ceil_div(rows, 256) * ceil_div(cols, 256)) * batch * steps;

@@ -28,6 +28,9 @@
 // to have 50 KB or more under way. The issue slots come next: elements are worked on two at a
 // time (f32x2 products), the weights are folded into the rotation's coefficients
 // (y = rstd (x k1 + partner k2)), and row pointers advance by additions.
+// The launch bounds (4, 3 and 2 blocks an SM) leave some kernels short of registers: the forward norm
+// of heads up to 256 spills 8 to 88 bytes a thread, two units of vectors 40 to 360, and the five units of odd 512-element
+// heads up to 770.
 #include <algorithm>
 #include <limits>
 
@@ -535,8 +538,9 @@ static int run(const b200_rotary* r, int dtype, Args& a, cudaStream_t s, int* bl
   const int wide = 4;
   const int half = r->rotary_dim / 2, rest = r->head_dim - r->rotary_dim;
   // vectors of 4 elements when they tile the head's parts and every row starts on one's
-  // boundary; otherwise units of 2 elements, loaded one by one (16 x 1024 x 8 x 128 bf16: 16 us
-  // with 64 rotated, 34 with 62; staging whole rows through shared memory took 40)
+  // boundary; otherwise units of 2 elements, loaded one by one (16 x 1024 x 8 x 128 bf16: 15 us
+  // with 64 rotated, 33 with 62 by halves, 23 with 62 interleaved; staging whole rows through shared
+  // memory took 40)
   bool fast = rest % wide == 0 && (r->interleaved ? r->rotary_dim : half) % wide == 0;
   for (const Seg& g : a.seg) {
     if (!g.heads) continue;
