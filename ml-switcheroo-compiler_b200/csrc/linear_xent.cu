@@ -786,8 +786,9 @@ struct Plan {
   int64_t N, D, V;
   int planes, w_dn;       // w_dn: w is stored [D, V] (V adjacent), else [V, D]
   int64_t w_rows, w_cols; // of the stored matrix
-  size_t x, w, part, picked, d, xg, acc, split, bytes;
+  size_t x, w, part, picked, d, xg, acc, split, dw_acc, bytes;
   int64_t width;          // columns of one piece
+  int64_t tokens;         // of one product for dw
   bool few;               // the kernels for up to 8 tokens
   int wide;               // their vectors of 4
   int64_t parts, slices;
@@ -796,6 +797,11 @@ struct Plan {
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 constexpr size_t PIECE_BYTES = size_t(512) << 20;
+// Tokens that one accumulator of a dw product takes where operands are one plane: its additions are
+// cut towards zero (tc_tile.cuh), and sums of one sign fall short by 1.7e-4 over 32768 tokens, 3.7e-4
+// over 65536, 7.8e-4 over 131072. More tokens than this are several products, added up in fp32 with
+// rounding; the shortfall stays at a twentieth of bf16's half step.
+constexpr int64_t MOST_TOKENS = 32768;
 
 // The piece: as few as keep d (2 bytes per token, column and plane) within 512 MiB, and of
 // those counts the one whose dw tiles fill the CTA pairs best, since each piece ends with
@@ -860,6 +866,8 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
     p.d = take((size_t)p.planes * N * p.width * 2);
     p.xg = take(xb);
     if (p.width < V) p.acc = take((size_t)N * D * 4);
+    p.tokens = p.planes > 1 ? N : std::min(N, MOST_TOKENS * splits_for(D, std::min(p.width, V), N));
+    if (p.tokens < N) p.dw_acc = take((size_t)D * p.width * 4);
     // splits x tiles of 256 x 256 never exceed the pairs of SMs
     p.split = take((size_t)(num_sms() / 2) * 256 * 256 * 4);
   }
@@ -1067,9 +1075,17 @@ extern "C" int b200_linear_xent_grad_mixed(int dtype, const float* dloss, const 
       tile::Operand Xm = X;
       Xm.mn = 1;
       uint8_t* out = reinterpret_cast<uint8_t*>(dw) + (w_dn ? first : first * D) * size;
-      rc = w_dn ? lx::product(Xm, Dm, D, width, N, p.planes, out, V, dw_bf16, nullptr, split, s, what)
-                : lx::product(Dm, Xm, width, D, N, p.planes, out, D, dw_bf16, nullptr, split, s, what);
-      if (rc) return rc;
+      float* sums = reinterpret_cast<float*>(ws + p.dw_acc);
+      for (int64_t t = 0; t < N; t += p.tokens) {
+        const int64_t n = std::min(p.tokens, N - t);
+        const bool last = t + n >= N;
+        void* to = last ? static_cast<void*>(out) : sums;
+        const float* add = t ? sums : nullptr;
+        Xm.base = xg + t * ldg, Dm.base = d + t * p.width;
+        rc = w_dn ? lx::product(Xm, Dm, D, width, n, p.planes, to, last ? V : width, last ? dw_bf16 : 0, add, split, s, what)
+                  : lx::product(Dm, Xm, width, D, n, p.planes, to, D, last ? dw_bf16 : 0, add, split, s, what);
+        if (rc) return rc;
+      }
     }
   }
   return B200_OK;

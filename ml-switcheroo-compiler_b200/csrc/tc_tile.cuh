@@ -6,8 +6,8 @@
 //  * an operand may come as two 16-bit planes, hi + lo of fp32 values (SPLIT; 16 or 22
 //    bits). Each K block then brings all four planes and runs hi.lo + lo.hi + hi.hi, which is
 //    the fp32 product up to lo.lo: a third of the tensor rate instead of the CUDA cores'. The
-//    tensor cores cut (not round) each sum to fp32: up to
-//    2^-23 of it per 16 products, all towards zero, which over K = 50000 was 1e-4. So the
+//    tensor cores cut (not round) each sum to fp32, all towards zero: sums of one sign lose
+//    0.76 2^-23 of their value per 16 products, which over K = 50000 was 1e-4. So the
 //    accumulator is drained every CHUNK K blocks and added up in registers with rounding (48
 //    cuts; 16 in the 128-wide tiles, where hi.lo + lo.hi, 2^-8 to 2^-11 of the whole, have an
 //    accumulator of their own);

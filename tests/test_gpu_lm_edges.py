@@ -214,6 +214,39 @@ def test_gradients_are_rounded_to_the_callers_types_only(n, d, v, tied):
         assert ((got.double() - ref).abs() <= tol + R.HALF_STEP[F32] * ref.abs()).all()
 
 
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("n", [65537, 2**18 + 77])
+def test_weight_gradient_of_many_tokens_is_not_cut_short(n, tied):
+    """Sums over all tokens of terms of one sign, in fp32 from bf16 operands. The tensor cores cut a sum
+    towards zero by up to 2^-23 of it in each of at most two additions per 16 products, half of
+    that on average and of half the final sum: 2^-24 of it per 16. Over the 32768 tokens of one
+    accumulator that is 2048 2^-24 = 2^-13, and the same of the whole for sums of several (131072 at once:
+    2^-11). d's rounding to bf16 is to either side: 2^-9 a term, 2^-17 of such sums. A logit's
+    error, 2^-21 as in the operator's tests, moves p by as much. So the mean over the sums is held to
+    2^-12, twice the cut."""
+    from b200 import ops
+
+    d, v = 4096, 1000  # tiles enough that the tokens are not shared out for the SMs' sake
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = (0.5 + torch.rand(n, d, generator=g, device="cuda")).to(BF)
+    w = (torch.randn(d, v, generator=g, device="cuda") / d**0.5).to(BF)
+    if tied:
+        w = w.t().contiguous().t()
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")  # the other words' sums have positive terms only
+    dloss = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    ops.Config.matmul_dtype = "bf16"
+    _, lse = op("LinearCrossEntropy", x.float(), w.float(), labels)
+    dx, dw = op("LinearCrossEntropyGrad", dloss, x.float(), w.float(), labels, lse)
+    ref = torch.zeros(d, v, dtype=torch.float64, device="cuda")
+    for i in range(0, n, 2**16):
+        xc, lc = x[i : i + 2**16].double(), slice(i, i + 2**16)
+        ref += xc.t() @ (torch.softmax(xc @ w.double(), -1) * dloss[lc].double()[:, None])
+    off = ((dw.double() - ref) / ref)[:, 1:]
+    assert abs(float(off.mean())) <= 2.0**-12 and float(off.abs().max()) <= 2.0**-10
+    narrow = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert torch.equal(narrow[1], dw.to(BF)) and torch.equal(narrow[0], dx.to(BF)) and narrow[1].stride() == w.stride()
+
+
 # ---- updates ----
 
 
