@@ -788,7 +788,7 @@ struct Plan {
   int64_t w_rows, w_cols; // of the stored matrix
   size_t x, w, part, picked, d, xg, acc, split, dw_acc, bytes;
   int64_t width;          // columns of one piece
-  int64_t tokens;         // of one product for dw
+  int64_t tokens, words;  // of one product for dw, and for dx
   bool few;               // the kernels for up to 8 tokens
   int wide;               // their vectors of 4
   int64_t parts, slices;
@@ -797,11 +797,11 @@ struct Plan {
 static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 constexpr size_t PIECE_BYTES = size_t(512) << 20;
-// Tokens that one accumulator of a dw product takes where operands are one plane: its additions are
-// cut towards zero (tc_tile.cuh), and sums of one sign fall short by 1.7e-4 over 32768 tokens, 3.7e-4
-// over 65536, 7.8e-4 over 131072. More tokens than this are several products, added up in fp32 with
-// rounding; the shortfall stays at a twentieth of bf16's half step.
-constexpr int64_t MOST_TOKENS = 32768;
+// Tokens of a dw product, or words of a dx product, that one accumulator takes where operands are one
+// plane: its additions are cut towards zero (tc_tile.cuh), and sums of one sign fall short by
+// 1.7e-4 over 32768 terms, 3.7e-4 over 65536, 7.8e-4 over 131072. More terms than this are several
+// products, added up in fp32 with rounding; the shortfall stays at a twentieth of bf16's half step.
+constexpr int64_t MOST_TERMS = 32768;
 
 // The piece: as few as keep d (2 bytes per token, column and plane) within 512 MiB, and of
 // those counts the one whose dw tiles fill the CTA pairs best, since each piece ends with
@@ -865,8 +865,10 @@ static Plan plan(bool grad, int dtype, const void* x, int64_t ldx, const void* w
     p.width = piece_width(N, D, V, p.planes);
     p.d = take((size_t)p.planes * N * p.width * 2);
     p.xg = take(xb);
-    if (p.width < V) p.acc = take((size_t)N * D * 4);
-    p.tokens = p.planes > 1 ? N : std::min(N, MOST_TOKENS * splits_for(D, std::min(p.width, V), N));
+    const int64_t width = std::min(p.width, V);
+    p.words = p.planes > 1 ? width : std::min(width, MOST_TERMS * splits_for(N, D, width));
+    p.tokens = p.planes > 1 ? N : std::min(N, MOST_TERMS * splits_for(D, width, N));
+    if (p.words < V) p.acc = take((size_t)N * D * 4);
     if (p.tokens < N) p.dw_acc = take((size_t)D * p.width * 4);
     // splits x tiles of 256 x 256 never exceed the pairs of SMs
     p.split = take((size_t)(num_sms() / 2) * 256 * 256 * 4);
@@ -1065,11 +1067,15 @@ extern "C" int b200_linear_xent_grad_mixed(int dtype, const float* dloss, const 
     Dm.mn = 1;
     if (dx) {
       // dx (+)= d w^T over the piece: w's features are the result's columns
-      tile::Operand Wt = W;
-      Wt.mn = !w_dn;
-      const bool last = first + width >= V;
-      rc = lx::product(Dk, Wt, N, D, width, p.planes, last ? dx : acc, D, last ? dx_bf16 : 0, first ? acc : nullptr, split, s, what);
-      if (rc) return rc;
+      for (int64_t c = 0; c < width; c += p.words) {
+        const int64_t n = std::min(p.words, width - c);
+        tile::Operand Wt = lx::w_columns(p, w, ldw, first + c);
+        Wt.mn = !w_dn;
+        Dk.base = d + c;
+        const bool last = first + c + n >= V;
+        rc = lx::product(Dk, Wt, N, D, n, p.planes, last ? dx : acc, D, last ? dx_bf16 : 0, first + c ? acc : nullptr, split, s, what);
+        if (rc) return rc;
+      }
     }
     if (dw) {
       tile::Operand Xm = X;

@@ -247,6 +247,37 @@ def test_weight_gradient_of_many_tokens_is_not_cut_short(n, tied):
     assert torch.equal(narrow[1], dw.to(BF)) and torch.equal(narrow[0], dx.to(BF)) and narrow[1].stride() == w.stride()
 
 
+@pytest.mark.parametrize("tied", [False, True])
+@pytest.mark.parametrize("v", [33000, 2**18 + 100])
+def test_input_gradient_of_many_words_is_not_cut_short(v, tied):
+    """The same of sums over the vocabulary: positive weights, but for the label's own, which are zero. The
+    tolerance is that of the sums over tokens."""
+    from b200 import ops
+
+    n, d = 1280, 2048  # tiles enough that the words are not shared out for the SMs' sake
+    g = torch.Generator(device="cuda").manual_seed(v)
+    x = (torch.randn(n, d, generator=g, device="cuda") / d**0.5).to(BF)
+    w = (0.5 + torch.rand(d, v, generator=g, device="cuda")).to(BF)
+    w[:, 0] = 0
+    if tied:
+        w = w.t().contiguous().t()
+    labels = torch.zeros(n, dtype=torch.int64, device="cuda")
+    dloss = (0.5 + torch.rand(n, generator=g, device="cuda")) / n
+    ops.Config.matmul_dtype = "bf16"
+    _, lse = op("LinearCrossEntropy", x.float(), w, labels)
+    dx, dw = op("LinearCrossEntropyGrad", dloss, x.float(), w, labels, lse)
+    ref, all_of = torch.zeros(n, d, dtype=torch.float64, device="cuda"), []
+    for i in range(0, v, 2**15):
+        all_of.append(x.double() @ w[:, i : i + 2**15].double())
+    p = torch.softmax(torch.cat(all_of, 1), -1) * dloss.double()[:, None]
+    for i in range(0, v, 2**15):
+        ref += p[:, i : i + 2**15] @ w[:, i : i + 2**15].double().t()
+    off = (dx.double() - ref) / ref
+    assert abs(float(off.mean())) <= 2.0**-12 and float(off.abs().max()) <= 2.0**-9
+    narrow = op("LinearCrossEntropyGrad", dloss, x, w, labels, lse)
+    assert torch.equal(narrow[0], dx.to(BF)) and torch.equal(narrow[1], dw) and dw.stride() == w.stride()
+
+
 # ---- updates ----
 
 
