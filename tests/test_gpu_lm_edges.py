@@ -33,11 +33,11 @@ def rand(*shape, dtype=F32, seed=0):
 
 
 # ---- heads ----
-# An fp32 angle is off by its integer's rounding, 2^-25 of pi / 4, and by 2^-24 of the product;
-# the polynomials of sine and cosine by 2^-28 and their few roundings: 1.2e-7 in all. A
-# rotated element adds three roundings of 2^-24 of its terms: 3e-7 (|a| + |b|). The norm adds
-# the fp32 sum of 512 squares (16 a lane, a tree of 5: 21 roundings, halved by the root) and 5
-# roundings of its products: 1e-6. Held to 2e-6 of the terms and half a step of the result's type.
+# A rotated element is within 6e-7 (|a| + |b|): three roundings of an angle within pi / 4 (1.4e-7),
+# the polynomials (2^-28) and their last roundings (2^-23), then four of 2^-24 for the factor, the
+# products and the sum. The norm adds the fp32 sum of 512 squares (16 a lane, a tree of 5: 21
+# roundings, halved by the root) and 5 roundings of its products: 1e-6. Held to 2e-6 of the
+# terms and half a step of the result's type.
 TERMS = 2e-6
 
 

@@ -1,9 +1,10 @@
 """Rotary positions and query / key norms on the GPU against their definitions in 64 bits.
 
-Tolerances. An angle reaches sincospif as a 24-bit float of half turns: off by at most
-pi 2^-25, and the function by about 2 units of 2^-24, so cosine and sine are within 2.2e-7
-and a rotated element within (|a| + |b|) (2.2e-7 + 3 2^-24 for the products and the sum)
-< 5e-7 (|a| + |b|). The norm adds the fp32 sum of at most 512 squares over at most 16
+Tolerances. The angle past the nearest quarter turn is a 32-bit integer turned into a float
+and multiplied by 2 pi 2^-32: three roundings (integer, constant, product) of 2^-24 of at most
+pi / 4, 1.4e-7. The Taylor polynomials are off by less than 2^-28 there, and by 2^-23 for their
+last roundings, so cosine and sine are within 2.7e-7 and a rotated element within (|a| + |b|)
+(2.7e-7 + 4 2^-24 for the factor, the products and the sum) < 6e-7 (|a| + |b|). The norm adds the fp32 sum of at most 512 squares over at most 16
 elements a lane and a tree of 5 (21 roundings of 2^-24, halved by the root) and 5 roundings
 of rsqrt and products: 1e-6 relative in all. So fp32 values are held to 2e-6 of their
 terms' magnitude, and a result of fewer bits to half a step of its own value besides."""
