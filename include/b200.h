@@ -625,7 +625,8 @@ int b200_linear_xent_grad_mixed(int dtype, const float* dloss, const void* x, in
  *                  for [inputs, outputs] pass lr sqrt(cols / rows) and weight_decay
  *                  sqrt(rows / cols). param_out may be param, momentum_out momentum; else
  *                  nothing overlaps.
- * BF16 runs on fp16 iterates (11 bits), F32 on pairs of them (22 bits), fp32 sums. X, S
+ * BF16 runs on fp16 iterates (11 bits), F32, and
+ * BF16 of up to 16 rows or columns, on pairs of them (22 bits), fp32 sums. X, S
  * and P = a I + b S + c S S are kept in fp16 times 2^8: the coefficients (finite, |a| < 250;
  * others are refused) have to keep the entries of all three below 250, or results are infinite
  * or NaN. Results do not depend on the run. */

@@ -408,7 +408,7 @@ def op_newton_schulz(g, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, **_):
     fp32 or bf16 in and out. ``coefficients``: one (a, b, c) or one per step, finite, |a| below
     250; they have to keep the entries of X, S and a I + b S + c S S below 250 too (the default
     ones keep them below 4), or the result is infinite or NaN. Sums are fp32; the iterates carry
-    22 bits for fp32 matrices and 11 for bf16."""
+    22 bits for fp32 matrices, and for bf16 ones of up to 16 rows or columns, else 11."""
     name = "NewtonSchulz"
     if g.dtype not in _FLOATS:
         raise BackendNotSupportedError(f"{name}: matrices of {g.dtype} (fp32 and bf16)")

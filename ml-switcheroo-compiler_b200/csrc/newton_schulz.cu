@@ -13,7 +13,10 @@
 // singular values stay below about 1.3, so no entry can pass 2^9 while entries of 2^-20
 // of the largest keep their bits. bf16 matrices take one fp16 plane (11 bits: 2e-3 of the
 // result after 5 steps, below bf16's own rounding; with bf16 iterates it is 2e-2). fp32
-// matrices take two planes, hi + lo (22 bits), three products: 2e-6, as with fp32 products.
+// matrices take two planes, hi + lo (22 bits), three products: 2e-6, as with fp32 products. So do bf16
+// ones of few rows or columns, where no error averages out and a small singular value makes it
+// grow: of 1600 matrices each with one plane, 2 x 2 were off by up to 3.8e-2, 8 x 8 by 1.8e-2, 16 x 16 by 6.4e-3
+// (24 x 24: 4.3e-3), with two by 3.2e-3 at most, bf16's rounding; a call takes 12 % longer (57 -> 64 us).
 // Where eps outweighs |G| the iterates start far below 1: each matrix carries a power of two
 // t = 2^e >= 1, Y = 2^8 t X is what is stored, b and c are divided by t^2 and t^4, and t
 // shrinks as a makes X grow. t is 1 for any |G| above eps.
@@ -35,6 +38,7 @@ namespace ns {
 using namespace tile;
 
 constexpr float SCALE = 256.f, MOST_A = 250.f;
+constexpr int64_t NARROW = 16;  // bf16 matrices up to this side take two planes
 constexpr int NORM_BLOCKS = 296, NT = 256;
 
 __device__ __forceinline__ uint32_t pack_f16(float a, float b) {
@@ -499,8 +503,8 @@ struct Plan {
 
 static Plan plan(int dtype, int64_t batch, int64_t rows, int64_t cols) {
   Plan q = {};
-  q.planes = dtype == B200_F32 ? 2 : 1;
   q.side = std::min(rows, cols);
+  q.planes = dtype == B200_F32 || q.side <= NARROW ? 2 : 1;
   q.ldx = up8(cols);
   q.ldg = up8(q.side);
   q.xn = rows * q.ldx;

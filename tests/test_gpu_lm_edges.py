@@ -278,6 +278,20 @@ def test_input_gradient_of_many_words_is_not_cut_short(v, tied):
     assert torch.equal(narrow[0], dx.to(BF)) and torch.equal(narrow[1], dw) and dw.stride() == w.stride()
 
 
+# ---- orthogonalisation ----
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 9), (2, 2), (2, 3), (500, 2), (3, 3), (4, 4), (5, 5), (8, 8), (8, 64), (12, 12), (16, 16), (16, 200)])
+def test_narrow_bf16_matrices_one_by_one(rows, cols):
+    """Each of 1600 matrices: at most half a step of bf16, and the products' 3e-6 grown by a = 3.4445 in each of five
+    steps, which a small singular value may do."""
+    g = torch.Generator(device="cuda").manual_seed(rows + cols)
+    m = (torch.randn(1600, rows, cols, generator=g, device="cuda") * 1e-3).to(BF)
+    ref = R.newton_schulz(m.double())
+    off = (op("NewtonSchulz", m).double() - ref).flatten(1).norm(dim=1) / ref.flatten(1).norm(dim=1)
+    assert float(off.max()) <= R.HALF_STEP[BF] + 3e-6 * 3.4445**5
+
+
 # ---- updates ----
 
 
