@@ -13,10 +13,11 @@
 // singular values stay below about 1.3, so no entry can pass 2^9 while entries of 2^-20
 // of the largest keep their bits. bf16 matrices take one fp16 plane (11 bits: 2e-3 of the
 // result after 5 steps, below bf16's own rounding; with bf16 iterates it is 2e-2). fp32
-// matrices take two planes, hi + lo (22 bits), three products: 2e-6, as with fp32 products. So do bf16
-// ones of few rows or columns, where no error averages out and a small singular value makes it
-// grow: of 1600 matrices each with one plane, 2 x 2 were off by up to 3.8e-2, 8 x 8 by 1.8e-2, 16 x 16 by 6.4e-3
-// (24 x 24: 4.3e-3), with two by 3.2e-3 at most, bf16's rounding; a call takes 12 % longer (57 -> 64 us).
+// matrices take two planes, hi + lo (22 bits), three products: 2e-6, as with fp32 products. So
+// do bf16 ones of few rows or columns, where no error averages out and a small singular value
+// makes it grow: of 1600 matrices each with one plane, 2 x 2 were off by up to 3.8e-2, 8 x 8 by
+// 1.8e-2, 16 x 16 by 6.4e-3 (24 x 24: 4.3e-3), with two by 3.2e-3 at most, bf16's rounding; a
+// call takes 12 % longer (57 -> 64 us).
 // Where eps outweighs |G| the iterates start far below 1: each matrix carries a power of two
 // t = 2^e >= 1, Y = 2^8 t X is what is stored, b and c are divided by t^2 and t^4, and t
 // shrinks as a makes X grow. t is 1 for any |G| above eps.

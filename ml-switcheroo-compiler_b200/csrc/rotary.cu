@@ -28,9 +28,9 @@
 // to have 50 KB or more under way. The issue slots come next: elements are worked on two at a
 // time (f32x2 products), the weights are folded into the rotation's coefficients
 // (y = rstd (x k1 + partner k2)), and row pointers advance by additions.
-// The launch bounds (4, 3 and 2 blocks an SM) leave some kernels short of registers: the forward norm
-// of heads up to 256 spills 8 to 88 bytes a thread, two units of vectors 40 to 360, and the five units of odd 512-element
-// heads up to 770.
+// The launch bounds (4, 3 and 2 blocks an SM) leave some kernels short of registers: the forward
+// norm of heads up to 256 spills 8 to 88 bytes a thread, two units of vectors 40 to 360, and the
+// five units of odd 512-element heads up to 770.
 #include <algorithm>
 #include <limits>
 
