@@ -638,6 +638,100 @@ int b200_apply_muon_f32(const float* param, const float* momentum, const float* 
                         int64_t batch, int64_t rows, int64_t cols, float lr, float mu, int nesterov, float weight_decay,
                         const float* coefficients, int steps, float eps, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------
+ * A block's output f added to the residual stream x, with the norms before and after it
+ * (the LayerNorm, Multiply and Add chain of the transformer workload: numpy/eager/nn_ops.py:
+ * 219-318, numpy/eager/math_binary.py:9-51; RMS norms have no counterpart there):
+ *   p = post ? N(f; post_gamma, post_beta) : f;  sum = scale x + gate p;
+ *   normed = N(sum; gamma, beta)
+ * N over the last axis: RMS (t rsqrt(mean t^2 + eps) gamma) or layer norm (centred, plus beta;
+ * betas are for it alone). x, f, sum, normed are dense [rows, cols], cols <= 16384; x, sum, their
+ * gradients and dx are of x_dtype, f, normed, dnormed and df of f_dtype, each F32 or BF16. The
+ * weights [cols] share weight_dtype, a NULL gamma is ones, a NULL beta zeros. gate [groups, cols]
+ * of gate_dtype: rows / groups consecutive rows share each (1: one value a channel; rows: one an
+ * element); NULL and 0 groups: ones. Sums are fp32, `normed` is made of the unrounded sum, every
+ * output is rounded once. The gradient makes the sums again from x and f; the weights' gradients
+ * (in their own types, NULL where not wanted; dgate is wanted with a gate) are summed over the rows
+ * in a fixed order. `sum` may be x, `normed` f, dx dsum or x, df dnormed or f; nothing else overlaps. */
+enum b200_norm_kind { B200_NORM_RMS = 0, B200_NORM_LAYER = 1 };
+typedef struct b200_residual_norm {
+  int64_t rows, cols, groups;
+  int32_t kind, post, x_dtype, f_dtype, weight_dtype, gate_dtype;
+  float scale, eps;
+  const void *gate, *gamma, *beta, *post_gamma, *post_beta;
+} b200_residual_norm;
+typedef struct b200_residual_norm_grads {
+  void *dgamma, *dbeta, *dpost_gamma, *dpost_beta, *dgate;
+} b200_residual_norm_grads;
+int b200_residual_norm_forward(const b200_residual_norm* n, const void* x, const void* f, void* sum, void* normed, void* stream);
+size_t b200_residual_norm_grad_workspace_bytes(const b200_residual_norm* n);
+int b200_residual_norm_grad(const b200_residual_norm* n, const void* dsum, const void* dnormed, const void* x, const void* f, void* dx,
+                            void* df, const b200_residual_norm_grads* grads, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * A learned bias by relative position, one value a bucket and head: bias[h, i, j] =
+ * table[bucket(j - i - shift), h] (no counterpart in the reference). One side's buckets are given
+ * by the smallest distance of each: start[0] = 0, not decreasing, the last at most
+ * B200_RELATIVE_MAX_FAR; a distance n >= 0 has the last bucket with start <= n. With
+ * `bidirectional` keys at or before the query's position have buckets 0 .. side - 1, later ones
+ * side .. 2 side - 1; without it later keys share bucket 0. table is dense [buckets, heads] F32 or
+ * BF16, buckets = side or 2 side.
+ *   relative_bias:      out [heads, queries, keys], dense, of the table's dtype
+ *   relative_bias_grad: dtable (dtype of dbias) = sums over batch, queries and keys of the dense
+ *                       dbias [batch, heads, queries, keys], in a fixed order; fp32 sums */
+#define B200_RELATIVE_MAX_SIDE 128
+#define B200_RELATIVE_MAX_FAR 1024
+typedef struct b200_relative {
+  int32_t side, bidirectional;
+  int32_t start[B200_RELATIVE_MAX_SIDE];
+} b200_relative;
+int b200_relative_bias(const b200_relative* r, int dtype, const void* table, void* out, int64_t heads, int64_t queries, int64_t keys,
+                       int64_t shift, void* stream);
+size_t b200_relative_bias_grad_workspace_bytes(const b200_relative* r, int64_t heads, int64_t queries, int64_t keys);
+int b200_relative_bias_grad(const b200_relative* r, int dtype, const void* dbias, void* dtable, int64_t batch, int64_t heads,
+                            int64_t queries, int64_t keys, int64_t shift, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------
+ * Attention without the scores in memory: for query i of head h and the keys j that it sees
+ *   z_j = scale q_i . k_j [+ table[bucket(j - i - shift), h]], lse_i = log sum_j exp z_j,
+ *   out_i = sum_j exp(z_j - lse_i) v_j
+ *   grad: p_j = exp(z_j - lse_i) made again, dz_j = p_j (dout_i . v_j - dout_i . out_i),
+ *   dq_i = scale sum_j dz_j k_j, dk_j = scale sum_i dz_j q_i, dv_j = sum_i p_j dout_i,
+ *   dtable[bucket, h] = sums of dz over the bucket
+ * the Matmul (eager/core_math_ops/math_matrix.py:21-64) -> Multiply -> Softmax
+ * (numpy/eager/math_advanced/math_signal.py:450-467) -> Matmul chain of the transformer
+ * workload's heads and its VJPs. q, out, dout, dq are [batch, queries, heads, dim], k, v, dk, dv
+ * [batch, keys, kv_heads, dim], of one dtype, F32 or BF16; heads is a multiple of kv_heads (head h
+ * reads key head h / (heads / kv_heads)); dim <= 256. Inputs have element strides {batch, token,
+ * head} and adjacent elements in a head; results are dense. lengths / query_lengths [batch]
+ * (length_dtype I32 or I64, NULL: all) cut each sequence's keys and queries at its end; nothing
+ * behind is read; one outside [0, keys] ([0, queries]) is clamped and sets the device error flag.
+ * Query i is at position i + shift, shift = the sequence's keys - its queries: its last query at its last key.
+ * causal: keys behind that position are hidden; window > 0: so are those at `window` or more
+ * before it (and, not causal, behind it). A query that sees nothing, or behind its sequence's
+ * end, has out 0, lse -inf and no gradient. lse [batch, heads, queries] fp32. table: [buckets,
+ * heads] dense of table_dtype, NULL: none; entries are finite or -inf. Sums and probabilities are fp32. The workspace is 256-byte aligned.
+ * Results do not depend on the run. */
+typedef struct b200_attention {
+  int64_t batch, queries, keys, heads, kv_heads, dim, window;
+  int32_t dtype, causal, length_dtype, table_dtype;
+  float scale;
+  const void *lengths, *query_lengths, *table;
+  b200_relative relative;
+  const void *q, *k, *v;
+  int64_t q_stride[3], k_stride[3], v_stride[3];
+} b200_attention;
+typedef struct b200_attention_grads {
+  const void *dout, *out;
+  int64_t dout_stride[3];
+  const float* lse;
+  void *dq, *dk, *dv, *dtable; /* dtable of table_dtype, wanted with a table */
+} b200_attention_grads;
+size_t b200_attention_workspace_bytes(const b200_attention* a);
+int b200_attention_forward(const b200_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t b200_attention_grad_workspace_bytes(const b200_attention* a);
+int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -74,6 +74,41 @@ class Rotary(C.Structure):
     ]
 
 
+RELATIVE_MAX_SIDE, RELATIVE_MAX_FAR = 128, 1024
+ATTENTION_MAX_DIM = 256
+RESIDUAL_NORM_MAX_COLS = 16384
+
+
+class ResidualNorm(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("rows", "cols", "groups")]
+    _fields_ += [(n, C.c_int32) for n in ("kind", "post", "x_dtype", "f_dtype", "weight_dtype", "gate_dtype")]
+    _fields_ += [(n, C.c_float) for n in ("scale", "eps")]
+    _fields_ += [(n, C.c_void_p) for n in ("gate", "gamma", "beta", "post_gamma", "post_beta")]
+
+
+class ResidualNormGrads(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("dgamma", "dbeta", "dpost_gamma", "dpost_beta", "dgate")]
+
+
+class Relative(C.Structure):
+    _fields_ = [("side", C.c_int32), ("bidirectional", C.c_int32), ("start", C.c_int32 * RELATIVE_MAX_SIDE)]
+
+
+class Attention(C.Structure):
+    _fields_ = [(n, C.c_int64) for n in ("batch", "queries", "keys", "heads", "kv_heads", "dim", "window")]
+    _fields_ += [(n, C.c_int32) for n in ("dtype", "causal", "length_dtype", "table_dtype")]
+    _fields_ += [("scale", C.c_float)]
+    _fields_ += [(n, C.c_void_p) for n in ("lengths", "query_lengths", "table")]
+    _fields_ += [("relative", Relative)]
+    _fields_ += [(n, C.c_void_p) for n in ("q", "k", "v")]
+    _fields_ += [(n, C.c_int64 * 3) for n in ("q_stride", "k_stride", "v_stride")]
+
+
+class AttentionGrads(C.Structure):
+    _fields_ = [("dout", C.c_void_p), ("out", C.c_void_p), ("dout_stride", C.c_int64 * 3)]
+    _fields_ += [(n, C.c_void_p) for n in ("lse", "dq", "dk", "dv", "dtable")]
+
+
 I64x18 = C.c_int64 * 18
 
 _P, _I64, _I32, _F32 = C.c_void_p, C.c_int64, C.c_int, C.c_float
@@ -172,6 +207,16 @@ SIGNATURES = {
         [_P] * 5 + [_I64] * 3 + [_F32, _F32, _I32, _F32, C.POINTER(_F32), _I32, _F32, _P, C.c_size_t, _P],
         C.c_int,
     ),
+    "b200_residual_norm_forward": ([C.POINTER(ResidualNorm)] + [_P] * 5, C.c_int),
+    "b200_residual_norm_grad_workspace_bytes": ([C.POINTER(ResidualNorm)], C.c_size_t),
+    "b200_residual_norm_grad": ([C.POINTER(ResidualNorm)] + [_P] * 6 + [C.POINTER(ResidualNormGrads), _P, C.c_size_t, _P], C.c_int),
+    "b200_relative_bias": ([C.POINTER(Relative), _I32, _P, _P] + [_I64] * 4 + [_P], C.c_int),
+    "b200_relative_bias_grad_workspace_bytes": ([C.POINTER(Relative)] + [_I64] * 3, C.c_size_t),
+    "b200_relative_bias_grad": ([C.POINTER(Relative), _I32, _P, _P] + [_I64] * 5 + [_P, C.c_size_t, _P], C.c_int),
+    "b200_attention_workspace_bytes": ([C.POINTER(Attention)], C.c_size_t),
+    "b200_attention_forward": ([C.POINTER(Attention), _P, _P, _P, C.c_size_t, _P], C.c_int),
+    "b200_attention_grad_workspace_bytes": ([C.POINTER(Attention)], C.c_size_t),
+    "b200_attention_grad": ([C.POINTER(Attention), C.POINTER(AttentionGrads), _P, C.c_size_t, _P], C.c_int),
     "b200_conv2d_fwd": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_dgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_wgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),

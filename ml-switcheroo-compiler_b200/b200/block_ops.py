@@ -1,0 +1,379 @@
+"""Operators of a transformer block: attention without the scores in memory, the learned position
+bias, and the residual sum with its norms.
+
+Like ``lm_ops``: values are ``torch.Tensor`` on the current CUDA device, results are fresh tensors,
+all arithmetic runs in libb200.so, gradients are separate operators, ``execute_op`` reaches them by
+name. The chain that they replace in a graph is Matmul, Multiply, Softmax, Matmul (attention) and
+LayerNorm, Multiply, Add (the residual sum).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import Any
+
+import torch
+
+from . import _lib as L
+from . import ops
+from .errors import BackendNotSupportedError
+from .lm_ops import _FLOATS, _on_device
+
+# ----------------------------------------------------------------------------------
+# learned position bias
+# ----------------------------------------------------------------------------------
+
+
+def relative_bucket_starts(side: int, max_distance: int) -> list[int]:
+    """The smallest distance of each of one side's ``side`` buckets: half of them one distance
+    each, the others equal steps of the logarithm from there to ``max_distance``, behind which all
+    share the last. Bucket side / 2 + i starts at the first distance n with
+    floor(log(n / near) / log(max_distance / near) (side - near)) = i, near = side // 2; compared
+    in whole numbers, since the steps may end on one."""
+    near = side // 2
+    wide = side - near
+    starts, d = list(range(near)), near
+    for i in range(wide):
+        while d**wide < near ** (wide - i) * max_distance**i:
+            d += 1
+        starts.append(d)
+    return starts
+
+
+@functools.lru_cache(maxsize=64)
+def _relative(buckets: int, max_distance: int, bidirectional: bool) -> L.Relative:
+    side, odd = divmod(buckets, 2) if bidirectional else (buckets, 0)
+    if odd or not 2 <= side <= L.RELATIVE_MAX_SIDE:
+        raise ValueError(f"relative bias: {buckets} buckets; want 2 to {L.RELATIVE_MAX_SIDE} a side, as many on both")
+    if not side // 2 < max_distance <= L.RELATIVE_MAX_FAR:
+        raise ValueError(f"relative bias: max_distance {max_distance} not in ({side // 2}, {L.RELATIVE_MAX_FAR}] for {buckets} buckets")
+    r = L.Relative()
+    r.side, r.bidirectional = side, int(bidirectional)
+    for i, d in enumerate(relative_bucket_starts(side, max_distance)):
+        r.start[i] = d
+    return r
+
+
+def _count(name: str, what: str, n: Any) -> int:
+    if n is None or int(n) != n or n < 0:
+        raise ValueError(f"{name}: {what} {n!r} is not a number of tokens")
+    return int(n)
+
+
+def op_relative_position_bias(table, queries=None, keys=None, bidirectional=True, max_distance=128, shift=None, **_):
+    """The learned bias of every query and key, [heads, queries, keys] of the table's type, to
+    be added to scores: ``table[bucket(rel), head]`` for rel = key - query - shift.
+
+    table [buckets, heads], fp32 or bf16. Half of the buckets (of each side, ``bidirectional``: keys
+    behind the query use the second half; else they share the first bucket) hold one distance each,
+    the others equal steps of the logarithm up to ``max_distance`` (``relative_bucket_starts``).
+    ``shift``: keys - queries by default, the last query at the last key."""
+    name = "RelativePositionBias"
+    if table.dim() != 2:
+        raise ValueError(f"{name}: table {tuple(table.shape)}, want [buckets, heads]")
+    if table.dtype not in _FLOATS:
+        raise BackendNotSupportedError(f"{name}: table of {table.dtype} (fp32 and bf16)")
+    nq, nk = _count(name, "queries", queries), _count(name, "keys", keys)
+    r = _relative(table.shape[0], int(max_distance), bool(bidirectional))
+    _on_device(name, table)
+    table = ops.contiguous(table)
+    out = torch.empty(table.shape[1], nq, nk, dtype=table.dtype, device=table.device)
+    L.call("b200_relative_bias", r, ops.code(table), table.data_ptr(), out.data_ptr(), table.shape[1], nq, nk,
+           nk - nq if shift is None else int(shift), ops.stream_ptr())
+    return out
+
+
+def op_relative_position_bias_grad(dscores, buckets=None, bidirectional=True, max_distance=128, shift=None, **_):
+    """The gradient of RelativePositionBias's table, [buckets, heads] of the scores' type, from
+    that of the scores, [..., heads, queries, keys]: summed over each bucket and all leading axes,
+    in fp32 and a fixed order."""
+    name = "RelativePositionBiasGrad"
+    if dscores.dim() < 3:
+        raise ValueError(f"{name}: scores {tuple(dscores.shape)}, want [..., heads, queries, keys]")
+    if dscores.dtype not in _FLOATS:
+        raise BackendNotSupportedError(f"{name}: scores of {dscores.dtype} (fp32 and bf16)")
+    heads, nq, nk = dscores.shape[-3:]
+    buckets = _count(name, "buckets", buckets)
+    r = _relative(buckets, int(max_distance), bool(bidirectional))
+    _on_device(name, dscores)
+    d = ops.contiguous(dscores)
+    out = torch.empty(buckets, heads, dtype=d.dtype, device=d.device)
+    wn = L.lib().b200_relative_bias_grad_workspace_bytes(r, heads, nq, nk)
+    ws = torch.empty(wn, dtype=torch.uint8, device=d.device)
+    L.call("b200_relative_bias_grad", r, ops.code(d), d.data_ptr(), out.data_ptr(), math.prod(d.shape[:-3]), heads, nq, nk,
+           nk - nq if shift is None else int(shift), ws.data_ptr(), wn, ops.stream_ptr())
+    return out
+
+
+# ----------------------------------------------------------------------------------
+# attention
+# ----------------------------------------------------------------------------------
+
+
+def _tokens(name: str, what: str, x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
+    """x [batch, tokens, heads, dim] with adjacent head elements, and its other strides."""
+    if x.dim() != 4:
+        raise ValueError(f"{name}: {what} {tuple(x.shape)}, want [batch, tokens, heads, dim] or [tokens, heads, dim]")
+    if x.stride(3) != 1 and x.shape[3] > 1:
+        x = ops.contiguous(x)
+    return x, x.stride()[:3]
+
+
+def _lengths(name: str, what: str, n: Any, batch: int) -> torch.Tensor | None:
+    if n is None:
+        return None
+    t = n if isinstance(n, torch.Tensor) else torch.as_tensor(n)
+    if tuple(t.shape) != (batch,):
+        raise ValueError(f"{name}: {what} {tuple(t.shape)} of {batch} sequences")
+    if t.dtype.is_floating_point or t.dtype == torch.bool:
+        raise BackendNotSupportedError(f"{name}: {what} of {t.dtype} (integers)")
+    t = ops.to_device(t)
+    _on_device(name, t)
+    if t.dtype not in (torch.int32, torch.int64):
+        t = ops._int_indices(t)
+    return ops.contiguous(t)
+
+
+def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, window, max_distance, bidirectional):
+    """(description, the tensors that it points to, whether the batch axis was left out)."""
+    flat = q.dim() == 3
+    if flat:
+        q, k, v = (t.unsqueeze(0) if t.dim() == 3 else t for t in (q, k, v))
+    for t, what in ((q, "queries"), (k, "keys"), (v, "values")):
+        if t.dim() != 4:
+            raise ValueError(f"{name}: {what} {tuple(t.shape)}, want [batch, tokens, heads, dim] or [tokens, heads, dim]")
+        if t.dtype not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: {what} of {t.dtype} (fp32 and bf16)")
+    b, nq, h, d = q.shape
+    nk, hk = k.shape[1], k.shape[2]
+    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
+        raise ValueError(f"{name}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not match")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise BackendNotSupportedError(f"{name}: queries of {q.dtype} with keys of {k.dtype} and values of {v.dtype}")
+    if not 1 <= d <= L.ATTENTION_MAX_DIM:
+        raise ValueError(f"{name}: heads of {d} elements (1 to {L.ATTENTION_MAX_DIM})")
+    if h < 1 or hk < 1 or h % hk:
+        raise ValueError(f"{name}: {h} heads over {hk} key heads")
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"{name}: scale {scale} is not a positive number")
+    if window is not None and (int(window) != window or window < 1):
+        raise ValueError(f"{name}: window {window!r} is not a number of tokens")
+    a = L.Attention()
+    if table is not None:
+        if table.dim() != 2 or table.shape[1] != h:
+            raise ValueError(f"{name}: position bias {tuple(table.shape)}, want [buckets, {h} heads]")
+        if table.dtype not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: position bias of {table.dtype} (fp32 and bf16)")
+        a.relative = _relative(table.shape[0], int(max_distance), not causal if bidirectional is None else bool(bidirectional))
+    _on_device(name, q, k, v, table)
+    lengths, query_lengths = _lengths(name, "lengths", lengths, b), _lengths(name, "query_lengths", query_lengths, b)
+    if lengths is not None and query_lengths is not None and lengths.dtype != query_lengths.dtype:
+        lengths, query_lengths = (ops.cast(t, torch.int64) for t in (lengths, query_lengths))
+    q, qs = _tokens(name, "queries", q)
+    k, ks = _tokens(name, "keys", k)
+    v, vs = _tokens(name, "values", v)
+    a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim = b, nq, nk, h, hk, d
+    a.window, a.causal, a.scale, a.dtype = int(window or 0), int(bool(causal)), scale, ops.code(q)
+    for n in (lengths, query_lengths):
+        if n is not None:
+            a.length_dtype = ops.code(n)
+    if table is not None:
+        table = ops.contiguous(table)
+        a.table, a.table_dtype = table.data_ptr(), ops.code(table)
+    a.lengths, a.query_lengths = ops._ptr(lengths), ops._ptr(query_lengths)
+    a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = qs, ks, vs
+    return a, (q, k, v, lengths, query_lengths, table), flat
+
+
+def op_fused_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False, window=None,
+                       max_distance=128, bidirectional=None, **_):
+    """Attention without the scores in memory: (out, lse), out_i = sum_j softmax_j(z_i) v_j for
+    z_ij = scale q_i . k_j (+ the position bias), lse_i = log sum_j exp z_ij.
+
+    q [batch, queries, heads, dim], k and v [batch, keys, kv_heads, dim] (or all without the
+    batch), of one type, fp32 or bf16, any strides (slices of one projection are read in place;
+    head-major tensors are passed as their transposed views); dim <= 256; heads is a multiple of
+    kv_heads, neighbouring heads share a key head. ``scale``: 1 / sqrt(dim). out is dense, in q's
+    shape and type; lse fp32 [batch, heads, queries].
+
+    ``lengths`` and ``query_lengths`` (integers [batch]) end each sequence's keys and queries: a padded
+    batch, or a cache that is not full. Nothing behind them is read. The last query is at the last key's
+    position: query i at i + keys - queries of its sequence. ``causal`` hides the keys behind a
+    query's position, ``window`` w those w or more before it (and, not causal, behind it). A query that
+    sees nothing has out 0 and lse -inf. ``relative_bias`` [buckets, heads]: the table of
+    RelativePositionBias, added to the scores by the positions' difference (``bidirectional``: not
+    causal by default); entries finite or -inf.
+
+    Scores, their maxima and sums are fp32; bf16 heads round the probabilities to bf16 for their
+    product with the values. Keep ``lse`` and ``out`` for FusedAttentionGrad."""
+    name = "FusedAttention"
+    a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
+    x = kept[0]
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    lse = torch.empty(a.batch, a.heads, a.queries, dtype=torch.float32, device=x.device)
+    wn = L.lib().b200_attention_workspace_bytes(a)
+    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    L.call("b200_attention_forward", a, out.data_ptr(), lse.data_ptr(), ops._ptr(ws), wn, ops.stream_ptr())
+    return (out[0], lse[0]) if flat else (out, lse)
+
+
+def op_fused_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False,
+                            window=None, max_distance=128, bidirectional=None, **_):
+    """(dq, dk, dv, dtable) of FusedAttention for its output's gradient ``dout``; ``out`` and ``lse`` as
+    the forward returned them, the rest as it took it. The probabilities are made again from lse.
+
+    Each is dense, in the shape and type of what it is the gradient of, rounded once; the heads that
+    share a key head are summed, dtable (None without ``relative_bias``) over batch and positions.
+    Queries and keys behind their sequence's end have zeros. The same from run to run."""
+    name = "FusedAttentionGrad"
+    a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
+    x, y, table = kept[0], kept[1], kept[5]
+    if tuple(dout.shape) != tuple(q.shape) or tuple(out.shape) != tuple(q.shape):
+        raise ValueError(f"{name}: gradient {tuple(dout.shape)} and output {tuple(out.shape)} of queries {tuple(q.shape)}")
+    if dout.dtype != x.dtype or out.dtype != x.dtype:
+        raise BackendNotSupportedError(f"{name}: gradient of {dout.dtype} and output of {out.dtype} for {x.dtype} heads")
+    want = (a.heads, a.queries) if flat else (a.batch, a.heads, a.queries)
+    if tuple(lse.shape) != want or lse.dtype != torch.float32:
+        raise ValueError(f"{name}: lse {tuple(lse.shape)} of {lse.dtype}, want fp32 {want}")
+    _on_device(name, dout, out, lse)
+    dout, ds = _tokens(name, "gradient", dout.unsqueeze(0) if flat else dout)
+    out, lse = ops.contiguous(out), ops.contiguous(lse)
+    g = L.AttentionGrads()
+    dq = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dk, dv = (torch.empty(y.shape, dtype=y.dtype, device=y.device) for _ in range(2))
+    dtable = None if table is None else torch.empty(table.shape, dtype=table.dtype, device=table.device)
+    g.dout, g.out, g.lse, g.dout_stride[:] = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), ds
+    g.dq, g.dk, g.dv, g.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ops._ptr(dtable)
+    wn = L.lib().b200_attention_grad_workspace_bytes(a)
+    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    L.call("b200_attention_grad", a, g, ops._ptr(ws), wn, ops.stream_ptr())
+    return (dq[0], dk[0], dv[0], dtable) if flat else (dq, dk, dv, dtable)
+
+
+# ----------------------------------------------------------------------------------
+# residual sum and its norms
+# ----------------------------------------------------------------------------------
+
+_NORMS = {"rms": 0, "layer": 1}
+
+
+def _residual(name: str, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps):
+    """(description, x, f, the weights as the kernels take them)."""
+    if x.shape != f.shape or x.dim() < 1:
+        raise ValueError(f"{name}: residual stream {tuple(x.shape)} and block output {tuple(f.shape)} differ")
+    for t, what in ((x, "residual stream"), (f, "block output")):
+        if t.dtype not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: {what} of {t.dtype} (fp32 and bf16)")
+    if norm not in _NORMS:
+        raise ValueError(f"{name}: norm {norm!r} is not one of {sorted(_NORMS)}")
+    width = x.shape[-1]
+    if not 1 <= width <= L.RESIDUAL_NORM_MAX_COLS:
+        raise ValueError(f"{name}: rows of {width} elements (1 to {L.RESIDUAL_NORM_MAX_COLS})")
+    post = post_gamma is not None or post_beta is not None if post_norm is None else bool(post_norm)
+    if not post and (post_gamma is not None or post_beta is not None):
+        raise ValueError(f"{name}: post weights without a post norm")
+    if norm != "layer" and (beta is not None or post_beta is not None):
+        raise ValueError(f"{name}: an RMS norm has no beta")
+    if not math.isfinite(residual_scale):
+        raise ValueError(f"{name}: residual_scale {residual_scale} is not finite")
+    weights = [gamma, beta, post_gamma, post_beta]
+    for w in weights:
+        if w is not None:
+            if tuple(w.shape) != (width,):
+                raise ValueError(f"{name}: norm weight {tuple(w.shape)}, want [{width}]")
+            if w.dtype not in _FLOATS:
+                raise BackendNotSupportedError(f"{name}: norm weights of {w.dtype} (fp32 and bf16)")
+    groups = 0
+    if gate is not None:
+        if gate.dtype not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: gate of {gate.dtype} (fp32 and bf16)")
+        lead = tuple(x.shape[:-1])
+        shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
+        # leading axes in full, then axes of one: consecutive rows share a gate
+        n = next((i for i in range(len(lead)) if len(shape) == x.dim() and shape[i] != lead[i]), len(lead))
+        if len(shape) != x.dim() or shape[-1] != width or any(s != 1 for s in shape[n:-1]):
+            raise ValueError(f"{name}: gate {tuple(gate.shape)} of {tuple(x.shape)}: want leading axes in full, then ones, then {width}")
+        groups = math.prod(shape[:n])
+    _on_device(name, x, f, gate, *weights)
+    x, f = ops.contiguous(x), ops.contiguous(f)
+    given = [w for w in weights if w is not None]
+    if len({w.dtype for w in given}) > 1:
+        weights = [None if w is None else ops.cast(w, torch.float32) for w in weights]
+    weights = [None if w is None else ops.contiguous(w) for w in weights]
+    gate = None if gate is None else ops.contiguous(gate)
+    d = L.ResidualNorm()
+    d.rows, d.cols = math.prod(x.shape[:-1]), width
+    d.groups = groups if d.rows else 0
+    d.kind, d.post, d.scale, d.eps = _NORMS[norm], int(post), float(residual_scale), float(eps)
+    d.x_dtype, d.f_dtype = ops.code(x), ops.code(f)
+    d.weight_dtype = next((ops.code(w) for w in weights if w is not None), L.F32)
+    d.gamma, d.beta, d.post_gamma, d.post_beta = (ops._ptr(w) for w in weights)
+    if gate is not None:
+        d.gate_dtype, d.gate = ops.code(gate), gate.data_ptr() if d.rows else None
+    return d, x, f, weights, gate
+
+
+def op_residual_norm(x, f, gamma=None, beta=None, post_gamma=None, post_beta=None, gate=None, residual_scale=1.0, norm="rms",
+                     post_norm=None, eps=1e-6, **_):
+    """A block's output added to the residual stream, with the norms on both sides of the sum, in
+    one pass: (sum, normed), sum = residual_scale x + gate N(f; post_gamma, post_beta), normed =
+    N(sum; gamma, beta), which the next block reads.
+
+    x and f [..., width] in one shape, fp32 or bf16 each (an fp32 stream with bf16 blocks too); sum is
+    of x's type, normed of f's. ``norm``: "rms" or "layer" (with betas), over the last axis, width <=
+    16384; a gamma of None is ones. ``post_norm``: whether f is normed first (by default where it has
+    weights). ``gate``: [width], or x's leading axes and then ones ([batch, 1, width], one gate a
+    sequence), or x's shape; None: ones. Computed in fp32, rounded once each."""
+    name = "ResidualNorm"
+    d, x, f, weights, gate = _residual(name, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps)
+    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    normed = torch.empty(f.shape, dtype=f.dtype, device=f.device)
+    L.call("b200_residual_norm_forward", d, x.data_ptr(), f.data_ptr(), total.data_ptr(), normed.data_ptr(), ops.stream_ptr())
+    return total, normed
+
+
+def op_residual_norm_grad(dsum, dnormed, x, f, gamma=None, beta=None, post_gamma=None, post_beta=None, gate=None, residual_scale=1.0,
+                          norm="rms", post_norm=None, eps=1e-6, **_):
+    """The gradients of ResidualNorm from those of its results and its inputs: (dx, df, dgamma,
+    dbeta, dpost_gamma, dpost_beta, dgate), None for weights that were not given, each in the type
+    and shape of what it is the gradient of. The sum and its norms are made again; the weights' sums over
+    rows are fp32, in a fixed order."""
+    name = "ResidualNormGrad"
+    given = (gamma, beta, post_gamma, post_beta)
+    shape = None if gate is None else gate.shape
+    d, x, f, weights, gate = _residual(name, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps)
+    if dsum.shape != x.shape or dnormed.shape != x.shape:
+        raise ValueError(f"{name}: gradients {tuple(dsum.shape)}, {tuple(dnormed.shape)} of {tuple(x.shape)}")
+    if dsum.dtype != x.dtype or dnormed.dtype != f.dtype:
+        raise BackendNotSupportedError(f"{name}: gradients of {dsum.dtype}, {dnormed.dtype} for a sum of {x.dtype} and norms of {f.dtype}")
+    _on_device(name, dsum, dnormed)
+    dsum, dnormed = ops.contiguous(dsum), ops.contiguous(dnormed)
+    dx, df = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, f))
+    grads = [None if w is None else torch.empty(w.shape, dtype=w.dtype, device=w.device) for w in weights]
+    dgate = None if gate is None else torch.empty(shape, dtype=gate.dtype, device=gate.device)
+    g = L.ResidualNormGrads()
+    g.dgamma, g.dbeta, g.dpost_gamma, g.dpost_beta = (ops._ptr(t) for t in grads)
+    g.dgate = ops._ptr(dgate)
+    wn = L.lib().b200_residual_norm_grad_workspace_bytes(d)
+    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    L.call("b200_residual_norm_grad", d, dsum.data_ptr(), dnormed.data_ptr(), x.data_ptr(), f.data_ptr(), dx.data_ptr(), df.data_ptr(), g,
+           ops._ptr(ws), wn, ops.stream_ptr())
+    if dgate is not None and not d.rows:
+        dgate = ops.full(tuple(shape), 0.0, dgate.dtype) if dgate.numel() else dgate
+    grads = [t if t is None else ops.cast(t, w.dtype) for t, w in zip(grads, given)]
+    return dx, df, *grads, dgate
+
+
+def register(table: dict) -> None:
+    table.update({
+        "FusedAttention": op_fused_attention,
+        "FusedAttentionGrad": op_fused_attention_grad,
+        "RelativePositionBias": op_relative_position_bias,
+        "RelativePositionBiasGrad": op_relative_position_bias_grad,
+        "ResidualNorm": op_residual_norm,
+        "ResidualNormGrad": op_residual_norm_grad,
+    })

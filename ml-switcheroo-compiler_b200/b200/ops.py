@@ -1480,6 +1480,10 @@ from . import lm_ops as _lm_ops  # noqa: E402  (rotary positions, query / key no
 
 _lm_ops.register(OPS)
 
+from . import block_ops as _block_ops  # noqa: E402  (attention, position bias, residual norms)
+
+_block_ops.register(OPS)
+
 # reference aliases (interpreter/evaluator.py:771-791)
 ALIASES = {"Sub": "Subtract", "Mul": "Multiply", "Div": "TrueDivide", "Neg": "Negative", "Pow": "Power", "MatMul": "Matmul",
            "Expand": "BroadcastTo", "Permute": "Transpose"}

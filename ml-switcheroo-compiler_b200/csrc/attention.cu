@@ -1,0 +1,116 @@
+// The attention entry points: checks, and the choice of the kernels.
+#include "attention.cuh"
+
+namespace b200 {
+namespace attention {
+
+static int check_attention(const char* what, const b200_attention* a) {
+  B200_REQUIRE(a, "%s: no description", what);
+  B200_REQUIRE(a->batch >= 0 && a->queries >= 0 && a->keys >= 0 && a->heads >= 1 && a->kv_heads >= 1 && a->heads % a->kv_heads == 0,
+               "%s: batch %lld, %lld queries, %lld keys, %lld heads, %lld key heads", what, (long long)a->batch, (long long)a->queries,
+               (long long)a->keys, (long long)a->heads, (long long)a->kv_heads);
+  B200_REQUIRE(a->batch <= 65535 && a->heads <= 65535 && a->queries < (1 << 30) && a->keys < (1 << 30),
+               "%s: batch and heads up to 65535, queries and keys below 2^30", what);
+  B200_REQUIRE(a->queries * (a->heads / a->kv_heads) < (1ll << 30), "%s: %lld queries times %lld heads a key head reach 2^30", what,
+               (long long)a->queries, (long long)(a->heads / a->kv_heads));
+  B200_REQUIRE(a->dim >= 1 && a->dim <= 256, "%s: dim %lld (1 to 256)", what, (long long)a->dim);
+  B200_REQUIRE(a->scale > 0 && a->scale < 3e38f, "%s: scale %g is not a positive number", what, (double)a->scale);
+  B200_REQUIRE(a->window >= 0, "%s: window %lld", what, (long long)a->window);
+  if (a->dtype != B200_F32 && a->dtype != B200_BF16) {
+    set_error("%s: dtype %d (F32 and BF16)", what, a->dtype);
+    return B200_ERR_DTYPE;
+  }
+  if (a->lengths || a->query_lengths)
+    if (a->length_dtype != B200_I32 && a->length_dtype != B200_I64) {
+      set_error("%s: lengths of dtype %d (I32 and I64)", what, a->length_dtype);
+      return B200_ERR_DTYPE;
+    }
+  if (a->table) {
+    if (int rc = relative::check(what, &a->relative)) return rc;
+    if (a->table_dtype != B200_F32 && a->table_dtype != B200_BF16) {
+      set_error("%s: table of dtype %d (F32 and BF16)", what, a->table_dtype);
+      return B200_ERR_DTYPE;
+    }
+  }
+  B200_REQUIRE(a->batch == 0 || a->queries == 0 || a->q, "%s: null queries", what);
+  B200_REQUIRE(a->batch == 0 || a->keys == 0 || (a->k && a->v), "%s: null keys or values", what);
+  return B200_OK;
+}
+
+// delta = dout . out of every query: a warp each
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200_attention a, const T* dout, const T* out, int64_t sb, int64_t ss,
+                                                    int64_t sh, float* delta) {
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;  // [batch, queries, heads]
+  const int lane = threadIdx.x & 31;
+  if (row >= a.batch * a.queries * a.heads) return;
+  const int64_t h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
+  if (i >= Sequence(a, b).queries) return;  // never read
+  const T *x = dout + b * sb + i * ss + h * sh, *y = out + row * a.dim;
+  float s = 0.f;
+  for (int c = lane; c < a.dim; c += 32) s = fmaf((float)x[c], (float)y[c], s);
+  s = warp_sum(s);
+  if (lane == 0) delta[(b * a.heads + h) * a.queries + i] = s;
+}
+
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+static size_t delta_bytes(const b200_attention& a) { return up256((size_t)(a.batch * a.heads * a.queries) * sizeof(float)); }
+
+}  // namespace attention
+}  // namespace b200
+
+using namespace b200;
+using namespace b200::attention;
+
+extern "C" size_t b200_attention_workspace_bytes(const b200_attention* a) {
+  if (check_attention("attention", a) || a->batch == 0 || a->queries == 0) return 0;
+  return rows_forward_workspace(*a);
+}
+
+extern "C" int b200_attention_forward(const b200_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_attention("attention", a)) return rc;
+  if (a->batch == 0 || a->queries == 0) return B200_OK;
+  B200_REQUIRE(out && lse, "attention: null result");
+  const size_t need = b200_attention_workspace_bytes(a);
+  B200_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
+               "attention: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
+  return rows_forward(*a, out, lse, workspace, as_stream(stream));
+}
+
+extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) {
+  if (check_attention("attention_grad", a) || a->batch == 0) return 0;
+  return delta_bytes(*a) + rows_grad_workspace(*a);
+}
+
+extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
+  if (int rc = check_attention("attention_grad", a)) return rc;
+  B200_REQUIRE(g, "attention_grad: no gradients");
+  B200_REQUIRE(!a->table || g->dtable, "attention_grad: no place for the table's gradient");
+  cudaStream_t st = as_stream(stream);
+  const size_t size = a->dtype == B200_F32 ? 4 : 2;
+  if (a->batch == 0 || a->queries == 0 || a->keys == 0) {
+    if (a->batch * a->queries) cudaMemsetAsync(g->dq, 0, (size_t)(a->batch * a->queries * a->heads * a->dim) * size, st);
+    if (a->batch * a->keys) {
+      cudaMemsetAsync(g->dk, 0, (size_t)(a->batch * a->keys * a->kv_heads * a->dim) * size, st);
+      cudaMemsetAsync(g->dv, 0, (size_t)(a->batch * a->keys * a->kv_heads * a->dim) * size, st);
+    }
+    if (a->table)
+      cudaMemsetAsync(g->dtable, 0, (size_t)(relative::buckets_of(a->relative) * a->heads) * (a->table_dtype == B200_F32 ? 4 : 2), st);
+    return check_launch("attention_grad");
+  }
+  B200_REQUIRE(g->dout && g->out && g->lse && g->dq && g->dk && g->dv, "attention_grad: null operand");
+  const size_t need = b200_attention_grad_workspace_bytes(a);
+  B200_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
+               "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
+  float* delta = reinterpret_cast<float*>(workspace);
+  const unsigned grid = (unsigned)ceil_div(a->batch * a->queries * a->heads, 8);
+  B200_REQUIRE(a->batch * a->queries * a->heads < (1ll << 33), "attention_grad: too many queries");
+  const int64_t* s = g->dout_stride;
+  if (a->dtype == B200_F32)
+    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, s[0], s[1], s[2], delta);
+  else
+    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, s[0], s[1], s[2], delta);
+  if (int rc = check_launch("attention_grad")) return rc;
+  return rows_grad(*a, *g, delta, reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a), st);
+}

@@ -1,0 +1,58 @@
+// What the attention kernels share: a sequence's lengths, which keys a query sees, and the
+// launchers of the two families (attention_rows.cu on the CUDA cores, attention_tiles.cu on the
+// tensor cores), which attention.cu chooses between.
+#pragma once
+#include "relative.cuh"
+
+namespace b200 {
+namespace attention {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+// keys, queries and shift of sequence b; a length outside its range is clamped and flagged
+struct Sequence {
+  int keys, queries, shift;
+  __device__ __forceinline__ Sequence(const b200_attention& a, int64_t b) {
+    keys = one(a, a.lengths, b, (int)a.keys);
+    queries = one(a, a.query_lengths, b, (int)a.queries);
+    shift = keys - queries;
+  }
+  static __device__ __forceinline__ int one(const b200_attention& a, const void* lengths, int64_t b, int all) {
+    if (!lengths) return all;
+    const int64_t n = a.length_dtype == B200_I64 ? reinterpret_cast<const long long*>(lengths)[b] : (int64_t)reinterpret_cast<const int*>(lengths)[b];
+    if (n < 0 || n > all) raise_device_error(B200_ERR_ARG);
+    return (int)max((int64_t)0, min((int64_t)all, n));
+  }
+  // keys that query i (< queries) sees: [first, end)
+  __device__ __forceinline__ int first_key(const b200_attention& a, int i) const {
+    return a.window ? (int)max((int64_t)0, (int64_t)i + shift - a.window + 1) : 0;
+  }
+  __device__ __forceinline__ int end_key(const b200_attention& a, int i) const {
+    if (a.causal) return min(keys, i + shift + 1);
+    return a.window ? (int)min((int64_t)keys, (int64_t)i + shift + a.window) : keys;
+  }
+  // queries that see key j (< keys): [first, end)
+  __device__ __forceinline__ int first_query(const b200_attention& a, int j) const {
+    if (a.causal) return max(0, j - shift);
+    return a.window ? (int)max((int64_t)0, (int64_t)j - shift - a.window + 1) : 0;
+  }
+  __device__ __forceinline__ int end_query(const b200_attention& a, int j) const {
+    return a.window ? (int)min((int64_t)queries, max((int64_t)0, (int64_t)j - shift + a.window)) : queries;
+  }
+};
+
+// a table entry in the log2 domain; what is finite stays finite
+__device__ __forceinline__ float table_log2(const void* table, int64_t at, int dtype) {
+  const float v = dtype == B200_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(table)[at]) : reinterpret_cast<const float*>(table)[at];
+  const float w = v * LOG2E;
+  return isinf(w) && !isinf(v) ? copysignf(3.402823466e38f, w) : w;
+}
+
+// attention_rows.cu
+size_t rows_forward_workspace(const b200_attention& a);
+int rows_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st);
+size_t rows_grad_workspace(const b200_attention& a);
+int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st);
+
+}  // namespace attention
+}  // namespace b200

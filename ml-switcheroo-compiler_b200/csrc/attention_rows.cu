@@ -1,0 +1,586 @@
+// Attention on the CUDA cores: few queries against a long cache, fp32, heads of any size.
+//
+// A block holds R rows (queries of the heads that share a key head; for dk and dv, keys) and its
+// four warps stream the other side past them, KEYS = 32 / R tokens a step, each warp steps of its own.
+// The lanes of a warp lie over the head's elements (E each), so a token is one coalesced load and no
+// shared memory. A step has R x KEYS = 32 scores, one a lane in the end: every lane sums its elements
+// of all 32, then 16 + 8 + 4 + 2 + 1 exchanges leave score l in lane l, where mask, bias and exponential
+// are done once each; the probabilities go back to all lanes through 128 bytes of shared memory a warp.
+// Forward: running maximum and sum per row (exp2 in the log2 domain), the warps' results joined at the end;
+// where rows leave SMs idle the keys are split over blocks and a second launch joins the parts.
+// Backward: p = exp2(z - lse) made again; dq has rows of queries, dk and dv rows of keys, so every sum
+// stays in registers, in a fixed order. Everything is fp32.
+// What bounds it: HBM for single tokens, else the FMA pipe (2 FMAs of 32 lanes for 32 E of a score's
+// elements, 60 % of the issue slots at 128 elements a head).
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace b200 {
+namespace attention {
+namespace rows {
+
+constexpr int WARPS = 4, THREADS = 32 * WARPS;
+constexpr int FWD = 0, DQ = 1, DKV = 2;
+
+struct Io {
+  int64_t out_rows;             // blocks of rows of one (batch, head or key head)
+  int splits;                   // FWD: blocks that share a row block's keys
+  int vec;                      // vector loads: 16-byte aligned tokens, dim a multiple of the lane's elements
+  void* out;                    // FWD: out; DQ: dq; DKV: dk
+  void* out2;                   // DKV: dv
+  float* lse;                   // FWD: written; else read
+  const void* dout;
+  int64_t dout_stride[3];
+  const float* delta;
+  float* part;                  // FWD with splits: [row blocks][splits][R][dim + 2]; DQ with a table: [row blocks][buckets]
+};
+
+template <typename T, int E>
+__device__ __forceinline__ void load(float (&v)[E], const T* p, int c, int dim, int vec) {
+  if (vec) {
+    if (c < dim) {
+      if constexpr (sizeof(T) == 4) {
+        if constexpr (E == 2) {
+          const float2 u = *reinterpret_cast<const float2*>(p + c);
+          v[0] = u.x, v[1] = u.y;
+        } else {
+#pragma unroll
+          for (int i = 0; i < E; i += 4) {
+            const float4 u = *reinterpret_cast<const float4*>(p + c + i);
+            v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
+          }
+        }
+      } else {
+        uint32_t w[E / 2];
+        if constexpr (E == 2) w[0] = *reinterpret_cast<const uint32_t*>(p + c);
+        else if constexpr (E == 4) {
+          const uint2 u = *reinterpret_cast<const uint2*>(p + c);
+          w[0] = u.x, w[1] = u.y;
+        } else {
+          const uint4 u = *reinterpret_cast<const uint4*>(p + c);
+          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
+        }
+#pragma unroll
+        for (int i = 0; i < E / 2; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < E; ++i) v[i] = c + i < dim ? (float)p[c + i] : 0.f;
+  }
+}
+template <int E>
+__device__ __forceinline__ void zero(float (&v)[E]) {
+#pragma unroll
+  for (int i = 0; i < E; ++i) v[i] = 0.f;
+}
+
+// 32 values a lane -> the sum over lanes of value `lane`
+__device__ __forceinline__ float sum_to_lane(float (&v)[32], int lane) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+    for (int i = 0; i < o; ++i) {
+      const bool up = lane & o;
+      const float send = up ? v[i] : v[i + o], keep = up ? v[i + o] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+    }
+  return v[0];
+}
+
+template <typename T, int E, int R, int MODE>
+__global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
+    rows_kernel(const __grid_constant__ b200_attention a, const __grid_constant__ Io io) {
+  constexpr int KEYS = 32 / R;
+  constexpr bool KEEP = KEYS * E <= 16;  // the step's tokens stay in registers between both products
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* s_p = reinterpret_cast<float*>(smem);             // [WARPS][2][32]: p or corrections; dz
+  float* s_join = s_p + WARPS * 64;                        // [WARPS][R][32 E] (DKV: twice), then FWD's m and l [WARPS][R] each
+  constexpr int JOIN = WARPS * R * 32 * E * (MODE == DKV ? 2 : 1) + 2 * WARPS * R;
+  float* s_near = s_join + JOIN;                           // DQ with a table: [WARPS][2 far + 1] sums by rel
+  const int far = a.table ? relative::far_of(a.relative) : 0;
+  const int bins = 2 * far + 1;
+  uint8_t* s_bucket = reinterpret_cast<uint8_t*>(s_near + (MODE == DQ && a.table ? WARPS * bins : 0));  // [2 far + 1]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, c = lane * E;
+  const int group = (int)(a.heads / a.kv_heads), dim = (int)a.dim;
+  const int64_t b = blockIdx.z;
+  const int hy = blockIdx.y;  // key head (FWD, DKV) or head (DQ)
+  const int kvh = MODE == DQ ? hy / group : hy;
+  const Sequence seq(a, b);
+  const int rb = MODE == FWD ? (int)(blockIdx.x / io.splits) : (int)blockIdx.x, part = MODE == FWD ? (int)(blockIdx.x % io.splits) : 0;
+  if (a.table) {
+    for (int i = threadIdx.x; i < bins; i += THREADS) s_bucket[i] = (uint8_t)relative::bucket_of(a.relative, i - far);
+    if constexpr (MODE == DQ)
+      for (int i = threadIdx.x; i < WARPS * bins; i += THREADS) s_near[i] = 0.f;
+    __syncthreads();
+  }
+  const T *q = reinterpret_cast<const T*>(a.q) + b * a.q_stride[0], *dout = reinterpret_cast<const T*>(io.dout) + (MODE == FWD ? 0 : b * io.dout_stride[0]);
+  const T *k = reinterpret_cast<const T*>(a.k) + b * a.k_stride[0] + kvh * a.k_stride[2],
+          *v = reinterpret_cast<const T*>(a.v) + b * a.v_stride[0] + kvh * a.v_stride[2];
+  // row r of the block: its query and head, or its key
+  auto row_query = [&](int r) { return MODE == FWD ? (rb * R + r) / group : rb * R + r; };
+  auto row_head = [&](int r) { return MODE == FWD ? kvh * group + (rb * R + r) % group : hy; };
+  const int row_end = MODE == DKV ? seq.keys : seq.queries;  // rows inside the sequence
+
+  // this lane's score is row lr, token lk of a step
+  const int lr = lane / KEYS, lk = lane % KEYS;
+  const int my_row = MODE == DKV ? rb * R + lr : row_query(lr);
+  const int my_head = MODE == DKV ? 0 : row_head(lr);
+  const bool my_in = my_row < row_end;
+  int lo, hi;  // tokens that this lane's row takes part with
+  if (MODE == DKV) lo = my_in ? seq.first_query(a, my_row) : 0, hi = my_in ? seq.end_query(a, my_row) : 0;
+  else lo = my_in ? seq.first_key(a, my_row) : 0, hi = my_in ? seq.end_key(a, my_row) : 0;
+  // the block's tokens: from the smallest to the largest of its rows' (whose ranges move one way)
+  int first = __reduce_min_sync(0xffffffffu, hi > lo ? lo : 0x7fffffff), end = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
+  if (first > end) first = end;
+  if (MODE == DKV) {  // tokens are (query, head of the group)
+    first *= group, end *= group;
+  }
+  if (MODE == FWD && io.splits > 1) {
+    const int unit = io.splits * KEYS * WARPS;
+    const int each = (end - first + unit - 1) / unit * KEYS * WARPS;
+    first = min(end, first + part * each);
+    end = min(end, first + each);
+  }
+
+  float x1[R][E], x2[MODE == FWD ? 1 : R][E], acc[R][E], acc2[MODE == DKV ? R : 1][E];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    zero(acc[r]);
+    zero(x1[r]);
+    if constexpr (MODE == DKV) zero(acc2[r]);
+    if constexpr (MODE != FWD) zero(x2[r]);
+    if constexpr (MODE == DKV) {
+      const int j = rb * R + r;
+      if (j < row_end) {
+        load<T, E>(x1[r], k + j * a.k_stride[1], c, dim, io.vec);
+        load<T, E>(x2[r], v + j * a.v_stride[1], c, dim, io.vec);
+      }
+    } else {
+      const int i = row_query(r), h = row_head(r);
+      if (i < row_end) {
+        load<T, E>(x1[r], q + i * a.q_stride[1] + h * a.q_stride[2], c, dim, io.vec);
+        if constexpr (MODE == DQ) load<T, E>(x2[r], dout + i * io.dout_stride[1] + h * io.dout_stride[2], c, dim, io.vec);
+      }
+    }
+  }
+  const float sl = a.scale * LOG2E;
+  float m = -INFINITY, l = 0.f;            // FWD: this lane's row's maximum, this lane's share of its sum
+  float my_lse = INFINITY, my_delta = 0.f;  // DQ
+  float before = 0.f, after = 0.f;          // DQ with a table: sums of dz at rel <= -far, >= far
+  if (MODE == DQ && my_in) {
+    const int64_t at = (b * a.heads + my_head) * a.queries + my_row;
+    my_lse = io.lse[at] * LOG2E;
+    if (my_lse == -INFINITY) my_lse = INFINITY;  // sees nothing: p = 0
+    my_delta = io.delta[at];
+  }
+  float* sp = s_p + warp * 64;
+
+  for (int t0 = first + warp * KEYS; t0 < end; t0 += WARPS * KEYS) {
+    float z[32], y1[KEEP ? KEYS : 1][E], y2[KEEP && MODE == DKV ? KEYS : 1][E];
+    auto token1 = [&](float (&y)[E], int n) {  // K, or Q for dk and dv
+      const int t = t0 + n;
+      if (t >= end) {
+        zero(y);
+        return;
+      }
+      if constexpr (MODE == DKV) load<T, E>(y, q + (t / group) * a.q_stride[1] + (kvh * group + t % group) * a.q_stride[2], c, dim, io.vec);
+      else load<T, E>(y, k + t * a.k_stride[1], c, dim, io.vec);
+    };
+    auto token2 = [&](float (&y)[E], int n) {  // V, or dout for dk and dv
+      const int t = t0 + n;
+      if (t >= end) {
+        zero(y);
+        return;
+      }
+      if constexpr (MODE == DKV)
+        load<T, E>(y, dout + (t / group) * io.dout_stride[1] + (kvh * group + t % group) * io.dout_stride[2], c, dim, io.vec);
+      else load<T, E>(y, v + t * a.v_stride[1], c, dim, io.vec);
+    };
+#pragma unroll
+    for (int n = 0; n < KEYS; ++n) {
+      float y[E];
+      token1(y, n);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) s = fmaf(x1[r][e], y[e], s);
+        z[r * KEYS + n] = s;
+      }
+      if constexpr (KEEP && MODE != FWD)
+#pragma unroll
+        for (int e = 0; e < E; ++e) y1[n][e] = y[e];
+    }
+    const float dot = sum_to_lane(z, lane);
+    // the lane's score
+    const int t = t0 + lk;
+    const int i = MODE == DKV ? t / group : my_row, j = MODE == DKV ? my_row : t;
+    const int other = MODE == DKV ? i : j;
+    const bool seen = t < end && other >= lo && other < hi;
+    const int rel = j - i - seq.shift;
+    float s = dot * sl;
+    if (a.table && seen) {
+      const int h = MODE == DKV ? kvh * group + t % group : my_head;
+      s += table_log2(a.table, (int64_t)s_bucket[max(-far, min(far, rel)) + far] * a.heads + h, a.table_dtype);
+    }
+    if (!seen) s = -INFINITY;
+    if constexpr (MODE == FWD) {
+      float top = s;
+#pragma unroll
+      for (int o = KEYS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      top = fmaxf(m, top);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float p = exp2f(s - base), fix = exp2f(m - base);
+      const bool grown = __any_sync(0xffffffffu, top != m);
+      l = l * fix + p;
+      m = top;
+      __syncwarp();
+      sp[lane] = p;
+      if (lk == 0) sp[32 + lr] = fix;
+      __syncwarp();
+      if (grown) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float f = sp[32 + r];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[r][e] *= f;
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < KEYS; ++n) {
+        float y[E];
+        token2(y, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float f = sp[r * KEYS + n];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < KEYS; ++n) {
+        float y[E];
+        token2(y, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) d = fmaf(x2[r][e], y[e], d);
+          z[r * KEYS + n] = d;
+        }
+        if constexpr (KEEP && MODE == DKV)
+#pragma unroll
+          for (int e = 0; e < E; ++e) y2[n][e] = y[e];
+      }
+      const float dp = sum_to_lane(z, lane);
+      float lse = my_lse, delta = my_delta;
+      if constexpr (MODE == DKV) {
+        lse = INFINITY, delta = 0.f;
+        if (seen) {
+          const int64_t at = (b * a.heads + kvh * group + t % group) * a.queries + i;
+          lse = io.lse[at] * LOG2E;
+          if (lse == -INFINITY) lse = INFINITY;
+          delta = io.delta[at];
+        }
+      }
+      const float p = seen ? exp2f(s - lse) : 0.f;
+      const float dz = seen ? p * (dp - delta) : 0.f;
+      __syncwarp();
+      sp[lane] = p;
+      sp[32 + lane] = dz;
+      __syncwarp();
+      if constexpr (MODE == DQ) {
+        if (a.table) {
+          if (rel >= far) after += dz;
+          else if (rel <= -far) before += dz;
+          // the step's near diagonals rel = t0 + d - (R - 1) - first query - shift, one a lane: no lane adds to another's
+          const int d = lane - (R - 1);
+          const int at = t0 + d - rb * R - seq.shift;
+          if (lane < R + KEYS - 1 && at > -far && at < far) {
+            float sum = 0.f;
+#pragma unroll
+            for (int r = 0; r < R; ++r)
+              if (d + r >= 0 && d + r < KEYS) sum += sp[32 + r * KEYS + d + r];
+            s_near[warp * bins + at + far] += sum;
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < KEYS; ++n) {
+        float y[E];
+        if constexpr (KEEP)
+#pragma unroll
+          for (int e = 0; e < E; ++e) y[e] = y1[n][e];
+        else token1(y, n);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float f = sp[32 + r * KEYS + n];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
+        }
+        if constexpr (MODE == DKV) {
+          if constexpr (KEEP)
+#pragma unroll
+            for (int e = 0; e < E; ++e) y[e] = y2[n][e];
+          else token2(y, n);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float f = sp[r * KEYS + n];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc2[r][e] = fmaf(f, y[e], acc2[r][e]);
+          }
+        }
+      }
+    }
+  }
+
+  // the warps' results joined, in order
+  float *jm = s_join + JOIN - 2 * WARPS * R, *jl = jm + WARPS * R;
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      s_join[(warp * R + r) * 32 * E + c + e] = acc[r][e];
+      if constexpr (MODE == DKV) s_join[((WARPS + warp) * R + r) * 32 * E + c + e] = acc2[r][e];
+    }
+  if constexpr (MODE == FWD) {
+#pragma unroll
+    for (int o = KEYS / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lk == 0) jm[warp * R + lr] = m, jl[warp * R + lr] = l;
+  }
+  if constexpr (MODE == DQ) {
+    if (a.table) {
+      before = warp_sum(before), after = warp_sum(after);
+      if (lane == 0) s_near[warp * bins] = before, s_near[warp * bins + 2 * far] = after;
+    }
+  }
+  __syncthreads();
+  const int64_t row_block = ((int64_t)b * gridDim.y + hy) * io.out_rows + rb;
+  for (int at = threadIdx.x; at < R * dim; at += THREADS) {
+    const int r = at / dim, col = at % dim;
+    if constexpr (MODE == FWD) {
+      const int i = row_query(r), h = row_head(r);
+      if (i >= a.queries) continue;
+      float top = -INFINITY, sum = 0.f, o = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, jm[w * R + r]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        const float f = exp2f(jm[w * R + r] - base);
+        sum = fmaf(f, jl[w * R + r], sum);
+        o = fmaf(f, s_join[(w * R + r) * 32 * E + col], o);
+      }
+      if (io.splits > 1) {
+        float* p = io.part + ((row_block * io.splits + part) * R + r) * (dim + 2);
+        p[col] = o;
+        if (col == 0) p[dim] = top, p[dim + 1] = sum;
+      } else {
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        reinterpret_cast<T*>(io.out)[((b * a.queries + i) * a.heads + h) * dim + col] = (T)(o * inv);
+        if (col == 0) io.lse[(b * a.heads + h) * a.queries + i] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * LN2;
+      }
+    } else {
+      float o = 0.f, o2 = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        o += s_join[(w * R + r) * 32 * E + col];
+        if constexpr (MODE == DKV) o2 += s_join[((WARPS + w) * R + r) * 32 * E + col];
+      }
+      const int row = rb * R + r;
+      if (MODE == DQ) {
+        if (row < a.queries) reinterpret_cast<T*>(io.out)[((b * a.queries + row) * a.heads + hy) * dim + col] = (T)(o * a.scale);
+      } else if (row < a.keys) {
+        const int64_t to = ((b * a.keys + row) * a.kv_heads + hy) * dim + col;
+        reinterpret_cast<T*>(io.out)[to] = (T)(o * a.scale);
+        reinterpret_cast<T*>(io.out2)[to] = (T)o2;
+      }
+    }
+  }
+  if constexpr (MODE == DQ) {
+    if (a.table) {
+      const int nb = relative::buckets_of(a.relative);
+      for (int n = threadIdx.x; n < nb; n += THREADS) {
+        float s = 0.f;
+        for (int i = 0; i < bins; ++i)
+          if (s_bucket[i] == n)
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) s += s_near[w * bins + i];
+        io.part[row_block * nb + n] = s;
+      }
+    }
+  }
+}
+
+// joins the splits of a row: a warp each
+template <typename T>
+__global__ void __launch_bounds__(256)
+    join_kernel(const __grid_constant__ b200_attention a, const float* part, int splits, int64_t row_blocks, int R, T* out, float* lse) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;  // [batch][key head][query][head of the group]
+  const int lane = threadIdx.x & 31, dim = (int)a.dim;
+  const int64_t group = a.heads / a.kv_heads, per = a.queries * group;
+  if (at >= a.batch * a.kv_heads * per) return;
+  const int64_t bk = at / per, rr = at % per, b = bk / a.kv_heads, i = rr / group, h = bk % a.kv_heads * group + rr % group;
+  const float* p = part + ((bk * row_blocks + rr / R) * splits * R + rr % R) * (dim + 2);
+  const int64_t step = (int64_t)R * (dim + 2);
+  float top = -INFINITY, sum = 0.f;
+  for (int s = lane; s < splits; s += 32) top = fmaxf(top, p[s * step + dim]);
+  top = warp_max(top);
+  const float base = top == -INFINITY ? 0.f : top;
+  for (int s = lane; s < splits; s += 32) sum = fmaf(exp2f(p[s * step + dim] - base), p[s * step + dim + 1], sum);
+  sum = warp_sum(sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int c = lane; c < dim; c += 32) {
+    float o = 0.f;
+    for (int s = 0; s < splits; ++s) o = fmaf(exp2f(p[s * step + dim] - base), p[s * step + c], o);
+    out[((b * a.queries + i) * a.heads + h) * dim + c] = (T)(o * inv);
+  }
+  if (lane == 0) lse[(b * a.heads + h) * a.queries + i] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * LN2;
+}
+
+// dtable[bucket, h]: the blocks' sums, batch by batch; 32 lanes a value
+template <typename T>
+__global__ void __launch_bounds__(256) table_kernel(const float* part, T* dtable, int64_t batch, int heads, int64_t blocks, int nb) {
+  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;
+  const int lane = threadIdx.x & 31;
+  if (at >= (int64_t)heads * nb) return;
+  const int n = (int)(at / heads), h = (int)(at % heads);
+  float s = 0.f;
+  for (int64_t i = lane; i < batch * blocks; i += 32) s += part[(((i / blocks) * heads + h) * blocks + i % blocks) * nb + n];
+  s = warp_sum(s);
+  if (lane == 0) dtable[at] = (T)s;
+}
+
+static bool vectors(const b200_attention& a, int elements, const void* dout, const int64_t* ds) {
+  const int64_t size = a.dtype == B200_F32 ? 4 : 2;
+  uint64_t u = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k) | reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(dout);
+  for (int i = 0; i < 3; ++i) u |= (uint64_t)((a.q_stride[i] | a.k_stride[i] | a.v_stride[i] | (ds ? ds[i] : 0)) * size);
+  return (u & 15) == 0 && a.dim % elements == 0;
+}
+
+static int elements(const b200_attention& a) { return a.dim <= 64 ? 2 : (a.dim <= 128 ? 4 : 8); }
+
+// rows of a block: as few as there are, so that a step has more tokens
+static int rows_of(const b200_attention& a, int64_t rows) {
+  const int most = a.dim <= 128 ? 8 : 4;
+  for (int r = 1; r < most; r *= 2)
+    if (rows <= r) return r;
+  return most;
+}
+
+struct Shape {
+  int R, splits;
+  int64_t blocks;  // row blocks of a (batch, key head)
+};
+static Shape forward_shape(const b200_attention& a) {
+  Shape s;
+  const int64_t rows = a.queries * (a.heads / a.kv_heads);
+  s.R = rows_of(a, rows);
+  s.blocks = ceil_div(rows, s.R);
+  // splits that bring 4 blocks to every SM, of 256 keys at least
+  const int64_t have = s.blocks * a.batch * a.kv_heads, want = 4 * (int64_t)num_sms();
+  s.splits = (int)std::max<int64_t>(1, std::min({ceil_div(want, have), ceil_div(a.keys, 256), (int64_t)1024}));
+  if (have >= 2 * (int64_t)num_sms()) s.splits = 1;
+  return s;
+}
+
+template <int MODE>
+static size_t shared_bytes(const b200_attention& a, int R, int E) {
+  size_t n = WARPS * 64 + (size_t)WARPS * R * 32 * E * (MODE == DKV ? 2 : 1) + 2 * WARPS * R;
+  const size_t bins = a.table ? 2 * relative::far_of(a.relative) + 1 : 0;
+  if (MODE == DQ) n += WARPS * bins;
+  return n * sizeof(float) + bins;
+}
+
+template <typename T, int E, int R, int MODE>
+static int launch(const b200_attention& a, const Io& io, dim3 grid, cudaStream_t st) {
+  const size_t shared = shared_bytes<MODE>(a, R, E);
+  const auto kernel = rows_kernel<T, E, R, MODE>;
+  if (shared > 48 * 1024) {
+    // the largest that any call needs, so that calls of several threads do not lower it
+    const size_t most = sizeof(float) * (WARPS * 64 + WARPS * R * 32 * E * 2 + 2 * WARPS * R + WARPS * (2 * B200_RELATIVE_MAX_FAR + 1)) + 2 * B200_RELATIVE_MAX_FAR + 1;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return check_launch("attention");
+  }
+  kernel<<<grid, THREADS, shared, st>>>(a, io);
+  return check_launch("attention");
+}
+
+template <typename T, int E, int MODE>
+static int launch_r(const b200_attention& a, const Io& io, int R, dim3 grid, cudaStream_t st) {
+  if constexpr (E < 8)
+    if (R == 8) return launch<T, E, 8, MODE>(a, io, grid, st);
+  if constexpr (MODE == FWD) {
+    if (R == 1) return launch<T, E, 1, MODE>(a, io, grid, st);
+    if (R == 2) return launch<T, E, 2, MODE>(a, io, grid, st);
+    return launch<T, E, 4, MODE>(a, io, grid, st);
+  } else if constexpr (E == 8) {
+    return launch<T, E, 4, MODE>(a, io, grid, st);
+  }
+  return B200_ERR_UNSUPPORTED;
+}
+template <int MODE>
+static int launch_any(const b200_attention& a, const Io& io, int R, dim3 grid, cudaStream_t st) {
+  const int e = elements(a);
+  if (a.dtype == B200_F32)
+    return e == 2 ? launch_r<float, 2, MODE>(a, io, R, grid, st) : (e == 4 ? launch_r<float, 4, MODE>(a, io, R, grid, st) : launch_r<float, 8, MODE>(a, io, R, grid, st));
+  using B = __nv_bfloat16;
+  return e == 2 ? launch_r<B, 2, MODE>(a, io, R, grid, st) : (e == 4 ? launch_r<B, 4, MODE>(a, io, R, grid, st) : launch_r<B, 8, MODE>(a, io, R, grid, st));
+}
+
+}  // namespace rows
+
+size_t rows_forward_workspace(const b200_attention& a) {
+  const rows::Shape s = rows::forward_shape(a);
+  return s.splits == 1 ? 0 : (size_t)(a.batch * a.kv_heads * s.blocks * s.splits * s.R * (a.dim + 2)) * sizeof(float);
+}
+
+int rows_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st) {
+  using namespace rows;
+  const Shape s = forward_shape(a);
+  Io io = {};
+  io.out_rows = s.blocks, io.splits = s.splits, io.vec = vectors(a, elements(a), nullptr, nullptr), io.out = out, io.lse = lse;
+  io.part = reinterpret_cast<float*>(workspace);
+  B200_REQUIRE(s.blocks * s.splits < (1ll << 31), "attention: too many queries");
+  if (int rc = launch_any<FWD>(a, io, s.R, dim3((unsigned)(s.blocks * s.splits), (unsigned)a.kv_heads, (unsigned)a.batch), st)) return rc;
+  if (s.splits == 1) return B200_OK;
+  const unsigned grid = (unsigned)ceil_div(a.batch * a.heads * a.queries, 8);
+  if (a.dtype == B200_F32) join_kernel<float><<<grid, 256, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (float*)out, lse);
+  else join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (__nv_bfloat16*)out, lse);
+  return check_launch("attention");
+}
+
+size_t rows_grad_workspace(const b200_attention& a) {
+  if (!a.table) return 0;
+  const int R = a.dim <= 128 ? 8 : 4;
+  return (size_t)(a.batch * a.heads * ceil_div(a.queries, R) * relative::buckets_of(a.relative)) * sizeof(float);
+}
+
+int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st) {
+  using namespace rows;
+  const int R = a.dim <= 128 ? 8 : 4;
+  Io io = {};
+  io.splits = 1, io.vec = vectors(a, elements(a), g.dout, g.dout_stride), io.dout = g.dout, io.delta = delta;
+  for (int i = 0; i < 3; ++i) io.dout_stride[i] = g.dout_stride[i];
+  io.lse = const_cast<float*>(g.lse);
+  io.out_rows = ceil_div(a.queries, R), io.out = g.dq, io.part = reinterpret_cast<float*>(workspace);
+  if (int rc = launch_any<DQ>(a, io, R, dim3((unsigned)io.out_rows, (unsigned)a.heads, (unsigned)a.batch), st)) return rc;
+  if (a.table) {
+    const int nb = relative::buckets_of(a.relative);
+    const unsigned grid = (unsigned)ceil_div(a.heads * nb, 8);
+    if (a.table_dtype == B200_F32) table_kernel<float><<<grid, 256, 0, st>>>(io.part, (float*)g.dtable, a.batch, (int)a.heads, io.out_rows, nb);
+    else table_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(io.part, (__nv_bfloat16*)g.dtable, a.batch, (int)a.heads, io.out_rows, nb);
+    if (int rc = check_launch("attention_grad")) return rc;
+  }
+  io.out_rows = ceil_div(a.keys, R), io.out = g.dk, io.out2 = g.dv, io.part = nullptr;
+  return launch_any<DKV>(a, io, R, dim3((unsigned)io.out_rows, (unsigned)a.kv_heads, (unsigned)a.batch), st);
+}
+
+}  // namespace attention
+}  // namespace b200
