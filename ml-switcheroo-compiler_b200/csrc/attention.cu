@@ -64,7 +64,7 @@ using namespace b200::attention;
 
 extern "C" size_t b200_attention_workspace_bytes(const b200_attention* a) {
   if (check_attention("attention", a) || a->batch == 0 || a->queries == 0) return 0;
-  return rows_forward_workspace(*a);
+  return tiles_take(*a) ? tiles_forward_workspace(*a) : rows_forward_workspace(*a);
 }
 
 extern "C" int b200_attention_forward(const b200_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
@@ -74,12 +74,12 @@ extern "C" int b200_attention_forward(const b200_attention* a, void* out, float*
   const size_t need = b200_attention_workspace_bytes(a);
   B200_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
                "attention: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
-  return rows_forward(*a, out, lse, workspace, as_stream(stream));
+  return tiles_take(*a) ? tiles_forward(*a, out, lse, workspace, as_stream(stream)) : rows_forward(*a, out, lse, workspace, as_stream(stream));
 }
 
 extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) {
   if (check_attention("attention_grad", a) || a->batch == 0) return 0;
-  return delta_bytes(*a) + rows_grad_workspace(*a);
+  return delta_bytes(*a) + (tiles_take(*a) ? tiles_grad_workspace(*a, nullptr) : rows_grad_workspace(*a));
 }
 
 extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes,
@@ -112,5 +112,6 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
   else
     delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, s[0], s[1], s[2], delta);
   if (int rc = check_launch("attention_grad")) return rc;
-  return rows_grad(*a, *g, delta, reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a), st);
+  void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
+  return tiles_take(*a) ? tiles_grad(*a, *g, delta, rest, st) : rows_grad(*a, *g, delta, rest, st);
 }

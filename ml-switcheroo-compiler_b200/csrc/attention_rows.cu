@@ -556,6 +556,14 @@ int rows_forward(const b200_attention& a, void* out, float* lse, void* workspace
   return check_launch("attention");
 }
 
+int table_sum(const b200_attention& a, const float* part, int64_t blocks, void* dtable, cudaStream_t st) {
+  const int nb = relative::buckets_of(a.relative);
+  const unsigned grid = (unsigned)ceil_div(a.heads * nb, 8);
+  if (a.table_dtype == B200_F32) rows::table_kernel<float><<<grid, 256, 0, st>>>(part, (float*)dtable, a.batch, (int)a.heads, blocks, nb);
+  else rows::table_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(part, (__nv_bfloat16*)dtable, a.batch, (int)a.heads, blocks, nb);
+  return check_launch("attention_grad");
+}
+
 size_t rows_grad_workspace(const b200_attention& a) {
   if (!a.table) return 0;
   const int R = a.dim <= 128 ? 8 : 4;
@@ -571,13 +579,8 @@ int rows_grad(const b200_attention& a, const b200_attention_grads& g, const floa
   io.lse = const_cast<float*>(g.lse);
   io.out_rows = ceil_div(a.queries, R), io.out = g.dq, io.part = reinterpret_cast<float*>(workspace);
   if (int rc = launch_any<DQ>(a, io, R, dim3((unsigned)io.out_rows, (unsigned)a.heads, (unsigned)a.batch), st)) return rc;
-  if (a.table) {
-    const int nb = relative::buckets_of(a.relative);
-    const unsigned grid = (unsigned)ceil_div(a.heads * nb, 8);
-    if (a.table_dtype == B200_F32) table_kernel<float><<<grid, 256, 0, st>>>(io.part, (float*)g.dtable, a.batch, (int)a.heads, io.out_rows, nb);
-    else table_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(io.part, (__nv_bfloat16*)g.dtable, a.batch, (int)a.heads, io.out_rows, nb);
-    if (int rc = check_launch("attention_grad")) return rc;
-  }
+  if (a.table)
+    if (int rc = table_sum(a, io.part, io.out_rows, g.dtable, st)) return rc;
   io.out_rows = ceil_div(a.keys, R), io.out = g.dk, io.out2 = g.dv, io.part = nullptr;
   return launch_any<DKV>(a, io, R, dim3((unsigned)io.out_rows, (unsigned)a.kv_heads, (unsigned)a.batch), st);
 }
