@@ -37,20 +37,37 @@ static int check_attention(const char* what, const b200_attention* a) {
   return B200_OK;
 }
 
-// delta = dout . out of every query: a warp each
+// delta = dout . out of every query: 8 lanes each, two 8-element pieces of both rows in flight a lane
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200_attention a, const T* dout, const T* out, int64_t sb, int64_t ss,
-                                                    int64_t sh, float* delta) {
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;  // [batch, queries, heads]
-  const int lane = threadIdx.x & 31;
-  if (row >= a.batch * a.queries * a.heads) return;
-  const int64_t h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
-  if (i >= Sequence(a, b).queries) return;  // never read
-  const T *x = dout + b * sb + i * ss + h * sh, *y = out + row * a.dim;
+                                                    int64_t sh, float* delta, int vec) {
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;  // [batch, queries, heads]
+  const int lane = threadIdx.x & 7;
+  const bool in = row < a.batch * a.queries * a.heads;
   float s = 0.f;
-  for (int c = lane; c < a.dim; c += 32) s = fmaf((float)x[c], (float)y[c], s);
-  s = warp_sum(s);
-  if (lane == 0) delta[(b * a.heads + h) * a.queries + i] = s;
+  int64_t h = 0, i = 0, b = 0;
+  if (in) {
+    h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
+    const T *x = dout + b * sb + i * ss + h * sh, *y = out + row * a.dim;
+    if (i >= Sequence(a, b).queries) {
+    } else {
+      constexpr int V = 16 / sizeof(T);
+#pragma unroll 2
+      for (int c = lane * V; c < a.dim; c += 8 * V) {
+        if (vec) {
+          const uint4 u = *reinterpret_cast<const uint4*>(x + c), w = *reinterpret_cast<const uint4*>(y + c);
+          const T *p = reinterpret_cast<const T*>(&u), *q = reinterpret_cast<const T*>(&w);
+#pragma unroll
+          for (int k = 0; k < V; ++k) s = fmaf((float)p[k], (float)q[k], s);
+        } else {  // the same elements in the same order
+          for (int k = 0; k < V && c + k < a.dim; ++k) s = fmaf((float)x[c + k], (float)y[c + k], s);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (in && lane == 0) delta[(b * a.heads + h) * a.queries + i] = s;
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -104,13 +121,14 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
   B200_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
   float* delta = reinterpret_cast<float*>(workspace);
-  const unsigned grid = (unsigned)ceil_div(a->batch * a->queries * a->heads, 8);
-  B200_REQUIRE(a->batch * a->queries * a->heads < (1ll << 33), "attention_grad: too many queries");
+  const unsigned grid = (unsigned)ceil_div(a->batch * a->queries * a->heads, 32);
+  B200_REQUIRE(a->batch * a->queries * a->heads < (1ll << 35), "attention_grad: too many queries");
   const int64_t* s = g->dout_stride;
+  const int vec = ((reinterpret_cast<uintptr_t>(g->dout) | reinterpret_cast<uintptr_t>(g->out) | (uint64_t)((s[0] | s[1] | s[2] | a->dim) * size)) & 15) == 0;
   if (a->dtype == B200_F32)
-    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, s[0], s[1], s[2], delta);
+    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, s[0], s[1], s[2], delta, vec);
   else
-    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, s[0], s[1], s[2], delta);
+    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, s[0], s[1], s[2], delta, vec);
   if (int rc = check_launch("attention_grad")) return rc;
   void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
   return tiles_take(*a) ? tiles_grad(*a, *g, delta, rest, st) : rows_grad(*a, *g, delta, rest, st);

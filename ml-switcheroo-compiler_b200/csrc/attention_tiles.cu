@@ -35,21 +35,67 @@ using namespace tc;
 constexpr int THREADS = 384, ROWS = 128;
 constexpr uint32_t SMEM_LIMIT = 232448;
 
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int sleep_ns = 0) {
-  bool ok = true;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, sleep_ns);
-  return __shfl_sync(0xffffffffu, ok ? 1 : 0, 0) != 0;
+// Bounded wait of whoever calls it. A look at the timer takes longer than a tile's MMAs, so it comes every 256 polls. After
+// WAIT_LIMIT_NS the block gives up: every later wait ends at once, results are not valid, the error flag says so.
+__device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* gave_up) {
+  unsigned long long t0 = 0;
+  while (true) {
+#pragma unroll 1
+    for (int k = 0; k < 256; ++k)
+      if (mbar_try_wait(bar, parity)) return;
+    if (*reinterpret_cast<volatile int*>(gave_up)) return;
+    const unsigned long long now = globaltimer();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > WAIT_LIMIT_NS) {
+      raise_device_error(B200_ERR_TIMEOUT);
+      *reinterpret_cast<volatile int*>(gave_up) = 1;
+    }
+  }
+}
+// by all lanes, together again behind it
+__device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
+  wait(bar, parity, gave_up);
+  __syncwarp();
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// D += A B with A (16-bit, two K a column) in TMEM
-__device__ __forceinline__ void mma_from_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+// The warp that issues MMAs walks its code with all lanes, and only the instruction itself is the elected lane's: under a
+// branch of one lane every operand is fetched into the uniform registers anew, 95 clocks an MMA of 64. A descriptor is
+// two words, of which tiles and K steps change the low one.
+struct Desc {
+  uint32_t lo, hi;
+};
+__device__ __forceinline__ Desc desc_at(uint32_t addr, uint32_t lbo_bytes) {
+  const uint64_t d = smem_desc(addr, lbo_bytes, 1024);
+  return {(uint32_t)d, (uint32_t)(d >> 32)};
+}
+__device__ __forceinline__ int elect_one() {
+  int e;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.s32 %0, 1, 0, p;\n}\n" : "=r"(e));
+  return e;
+}
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
+__device__ __forceinline__ void mma(int elected, uint32_t d, Desc a, uint32_t a_off, Desc b, uint32_t b_off, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b),
-      "r"(idesc), "r"(acc));
+      "{\n .reg .pred p, e;\n .reg .b64 x, y;\n mov.b64 x, {%1, %2};\n mov.b64 y, {%3, %4};\n setp.ne.b32 p, %6, 0;\n setp.ne.b32 e, %7, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %5, p;\n}\n" ::"r"(d),
+      "r"(a.lo + a_off), "r"(a.hi), "r"(b.lo + b_off), "r"(b.hi), "r"(idesc), "r"(acc), "r"(elected));
+}
+// D += A B with A (16-bit, two K a column) in TMEM
+__device__ __forceinline__ void mma_from_tmem(int elected, uint32_t d, uint32_t a, Desc b, uint32_t b_off, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n .reg .b64 y;\n mov.b64 y, {%2, %3};\n setp.ne.b32 p, %5, 0;\n setp.ne.b32 e, %6, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %4, p;\n}\n" ::"r"(d),
+      "r"(a), "r"(b.lo + b_off), "r"(b.hi), "r"(idesc), "r"(acc), "r"(elected));
+}
+__device__ __forceinline__ void commit(int elected, uint64_t* bar) {
+  asm volatile(
+      "{\n .reg .pred e;\n setp.ne.b32 e, %1, 0;\n @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar)),
+      "r"(elected)
+      : "memory");
 }
 #define B200_R16(r, o)                                                                                                              \
   "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7]), "r"(r[o + 8]), \
@@ -68,15 +114,13 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ uint32_t idesc_of(int m, int n, bool b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-// a tile of R rows is DP / 64 pieces of [R][64] elements, 128-byte rows, swizzled
+// A tile of R rows is DP / 64 pieces of [R][64] elements, 128-byte rows, swizzled. K-major, elements 16 k .. 16 k + 15 of every row
+// are at off_k<R>(k) of its descriptor (in 16 bytes); with the elements as N, rows 16 k .. 16 k + 15 at off_mn(k).
 template <int R>
-__device__ __forceinline__ uint64_t desc_k(uint32_t base, int k) {  // K-major: elements 16 k .. 16 k + 15 of every row
-  return smem_desc(base + (uint32_t)(k >> 2) * (R * 128u) + (uint32_t)(k & 3) * 32u, 16, 1024);
+__device__ __forceinline__ constexpr uint32_t off_k(int k) {
+  return (uint32_t)(k >> 2) * (R * 8u) + (uint32_t)(k & 3) * 2u;
 }
-template <int R>
-__device__ __forceinline__ uint64_t desc_mn(uint32_t base, int k) {  // rows 16 k .. 16 k + 15 as K, the elements as N
-  return smem_desc(base + (uint32_t)k * 2048u, R * 128u, 1024);
-}
+__device__ __forceinline__ constexpr uint32_t off_mn(int k) { return (uint32_t)k * 128u; }
 // rows [from, R) of a tile set to zero by one warp
 template <int R, int DP>
 __device__ __forceinline__ void zero_rows(uint32_t base, int from, int lane) {
@@ -139,9 +183,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST,
            *p_full = s_full + 2, *o_full = p_full + 2, *idle = o_full + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
+  int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* lut = reinterpret_cast<float*>(smem + F::LUT);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int head = blockIdx.y, kvh = head / (int)(a.heads / a.kv_heads), dim = (int)a.dim;
   const int64_t b = blockIdx.z;
   const Sequence seq(a, b);
@@ -156,12 +201,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int lo = seq.first_key(a, i0), hi = seq.end_key(a, i1);
       if (hi > lo) t0[w] = lo / KEYS, t1[w] = (hi + KEYS - 1) / KEYS;
     }
+    t0[w] = uniform(t0[w]), t1[w] = uniform(t1[w]);
   }
   const bool any0 = t1[0] > t0[0], any1 = t1[1] > t0[1];
   const int T0 = any0 ? (any1 ? min(t0[0], t0[1]) : t0[0]) : t0[1], T1 = max(t1[0], t1[1]);
   const int far = BIAS ? relative::far_of(a.relative) : 0;
 
   if (threadIdx.x == 0) {
+    *gave_up = 0;
     for (const CUtensorMap* m : {&map_q, &map_k, &map_v}) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     mbar_init(q_full, 1);
     for (int s = 0; s < ST; ++s) {
@@ -186,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
 
   if (warp == 0) {
     if (lane == 0 && T1 > T0) {
@@ -195,55 +242,49 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (t1[w] > t0[w])
           for (int p = 0; p < DP / 64; ++p)
             tma_load_4d(smem + w * F::TILE + p * (ROWS * 128), &map_q, q_full, p * 64, (2 * pair + w) * ROWS, head, (int)b);
-      bool ok = true;
       int n = 0;
-      for (int t = T0; t < T1 && ok; ++t, ++n) {
+      for (int t = T0; t < T1; ++t, ++n) {
         const int s = n % ST;
         const uint32_t par = ((n / ST) & 1) ^ 1;
-        if (!(ok = mbar_wait(&k_empty[s], par))) break;
+        wait(&k_empty[s], par, gave_up);
         mbar_expect_tx(&k_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
           tma_load_4d(smem + 2 * F::TILE + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, t * KEYS, kvh, (int)b);
-        if (!(ok = mbar_wait(&v_empty[s], par))) {
-          mbar_wait(&k_full[s], par ^ 1);
-          break;
-        }
+        wait(&v_empty[s], par, gave_up);
         mbar_expect_tx(&v_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
           tma_load_4d(smem + (2 + ST) * F::TILE + s * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, t * KEYS, kvh, (int)b);
       }
       // every load has landed before the block may end
-      mbar_wait(q_full, 0);
+      wait(q_full, 0, gave_up);
       for (int m = max(0, n - ST); m < n; ++m) {
-        mbar_wait(&k_full[m % ST], (m / ST) & 1);
-        mbar_wait(&v_full[m % ST], (m / ST) & 1);
+        wait(&k_full[m % ST], (m / ST) & 1, gave_up);
+        wait(&v_full[m % ST], (m / ST) & 1, gave_up);
       }
     }
   } else if (warp == 1) {
-    const int ks = (dim + 15) / 16;
+    const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, KEYS, false), id_o = idesc_of(ROWS, ks * 16, true);
-    bool ok = T1 > T0 && warp_wait(q_full, 0);
-    auto product_s = [&](int w, int t) {  // S_w of tile t, whose K has landed
-      const uint32_t kb = s_k + ((t - T0) % ST) * F::TILE;
+    if (T1 > T0) warp_wait(q_full, 0, gave_up);
+    const Desc dq = desc_at(s_q, 16), dk = desc_at(s_k, 16), dv = desc_at(s_v, KEYS * 128);
+    auto product_s = [&](int w, int s) {  // S_w of the tile in stage s, whose K has landed
       tc_fence_after();
-      if (lane == 0) {
-        for (int k = 0; k < ks; ++k)
-          mma_bf16(tmem + w * KEYS, desc_k<ROWS>(s_q + w * F::TILE, k), desc_k<KEYS>(kb, k), id_s, k > 0);
-        mma_commit(&s_full[w]);
-      }
-      __syncwarp();
+      const Desc kd = {dk.lo + s * (F::TILE >> 4), dk.hi}, qd = {dq.lo + w * (F::TILE >> 4), dq.hi};
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < ks) mma(elected, tmem + w * KEYS, qd, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
+      commit(elected, &s_full[w]);
     };
     int done[2] = {0, 0};
-    if (ok && (ok = warp_wait(&k_full[0], 0))) {
+    if (T1 > T0) {
+      warp_wait(&k_full[0], 0, gave_up);
       for (int w = 0; w < 2; ++w)
-        if (t0[w] == T0 && t1[w] > t0[w]) product_s(w, T0);
-      if (lane == 0) mma_commit(&k_empty[0]);
-      __syncwarp();
+        if (t0[w] == T0 && t1[w] > t0[w]) product_s(w, 0);
+      commit(elected, &k_empty[0]);
     }
-    for (int t = T0; t < T1 && ok; ++t) {
-      const int s = (t - T0) % ST, next = (t + 1 - T0) % ST;
-      const uint32_t par = ((t - T0) / ST) & 1, next_par = ((t + 1 - T0) / ST) & 1;
-      if (!(ok = warp_wait(&v_full[s], par))) break;
+    for (int t = T0, s = 0, par = 0, next = 0, next_par = 0; t < T1; ++t, s = next, par = next_par) {
+      next = s + 1 == ST ? 0 : s + 1, next_par = s + 1 == ST ? par ^ 1 : par;
+      warp_wait(&v_full[s], par, gave_up);
       const int have = seq.keys - t * KEYS;
       if (have < KEYS && seq.keys < a.keys) {
         // what lies behind the sequence's end may be anything, and is multiplied by zeros
@@ -251,31 +292,27 @@ __global__ void __launch_bounds__(THREADS, 1)
         fence_proxy_async_smem();
         __syncwarp();
       }
-      const uint32_t vb = s_v + s * F::TILE;
-      if (t + 1 < T1 && !(ok = warp_wait(&k_full[next], next_par))) break;
-      for (int w = 0; w < 2 && ok; ++w) {
+      const Desc vd = {dv.lo + s * (F::TILE >> 4), dv.hi};
+      if (t + 1 < T1) warp_wait(&k_full[next], next_par, gave_up);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
         if (t >= t0[w] && t < t1[w]) {
-          if (!(ok = warp_wait(&p_full[w], done[w] & 1))) break;
+          warp_wait(&p_full[w], done[w] & 1, gave_up);
           tc_fence_after();
-          if (lane == 0) {
-            for (int k = 0; k < KEYS / 16; ++k)
-              mma_from_tmem(tmem + F::TMEM_O + w * DP, tmem + w * KEYS + k * 8, desc_mn<KEYS>(vb, k), id_o, done[w] > 0 || k > 0);
-            if (t + 1 == t1[w]) mma_commit(&o_full[w]);
-          }
-          __syncwarp();
+#pragma unroll
+          for (int k = 0; k < KEYS / 16; ++k)
+            mma_from_tmem(elected, tmem + F::TMEM_O + w * DP, tmem + w * KEYS + k * 8, vd, off_mn(k), id_o, done[w] > 0 || k > 0);
+          if (t + 1 == t1[w]) commit(elected, &o_full[w]);
           ++done[w];
         }
-        if (t + 1 >= t0[w] && t + 1 < t1[w]) product_s(w, t + 1);
+        if (t + 1 >= t0[w] && t + 1 < t1[w]) product_s(w, next);
       }
-      if (ok && lane == 0) {
-        mma_commit(&v_empty[s]);
-        if (t + 1 < T1) mma_commit(&k_empty[next]);
-      }
-      __syncwarp();
+      commit(elected, &v_empty[s]);
+      if (t + 1 < T1) commit(elected, &k_empty[next]);
     }
     // no MMA and no commit is on its way when the block ends
-    if (lane == 0) mma_commit(idle);
-    warp_wait(idle, 0);
+    commit(elected, idle);
+    warp_wait(idle, 0, gave_up);
   } else if (warp >= 4) {
     const int w = (warp - 4) >> 2, q = warp & 3;
     const int i0 = (2 * pair + w) * ROWS + q * 32, i = i0 + lane;
@@ -288,17 +325,15 @@ __global__ void __launch_bounds__(THREADS, 1)
     const uint32_t t_s = tmem + lanes + w * KEYS, t_o = tmem + lanes + F::TMEM_O + w * DP;
     const float sl = a.scale * LOG2E;
     float m = -INFINITY, l = 0.f;
-    bool ok = true;
     for (int t = t0[w]; t < t1[w]; ++t) {
       const int n = t - t0[w], j0 = t * KEYS;
-      if (!(ok = warp_wait(&s_full[w], n & 1))) break;
+      warp_wait(&s_full[w], n & 1, gave_up);
       tc_fence_after();
       uint32_t v[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32_issue(t_s + c * 32, v[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
-      float top = -INFINITY;
       float mul = sl;
       if constexpr (BIAS) {
         mul = 1.f;
@@ -327,11 +362,14 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (j < lo || j >= hi) v[c][k] = 0xff800000u;
           }
       }
+      float tops[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) tops[k] = -INFINITY;
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int k = 0; k < 32; ++k) top = fmaxf(top, __uint_as_float(v[c][k]));
-      top *= mul;
+        for (int k = 0; k < 32; ++k) tops[k & 7] = fmaxf(tops[k & 7], __uint_as_float(v[c][k]));
+      const float top = mul * fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
       if (__any_sync(0xffffffffu, top > m + LAZY)) {
         const float grown = fmaxf(m, top);
         const float fix = ex2(m - (grown == -INFINITY ? 0.f : grown));
@@ -368,7 +406,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&p_full[w]);
     }
-    const bool some = t1[w] > t0[w] && ok && warp_wait(&o_full[w], 0);
+    const bool some = t1[w] > t0[w];
+    if (some) warp_wait(&o_full[w], 0, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;
@@ -443,11 +482,12 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t *x_full = bars, *y_full = bars + 1, *y_empty = y_full + G::MOST, *st_full = y_empty + G::MOST, *sp_full = st_full + G::MOST, *sp_free = sp_full + 1,
            *pd_full = sp_full + 2, *pd_free = sp_full + 3, *acc_full = sp_full + 4, *idle = sp_full + 5;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
+  int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* s_stat = reinterpret_cast<float*>(bars + 32);           // DKV: [stages][lse, delta][BN]
   float* lut = s_stat + (DKV ? G::MOST * 2 * BN : 0);            // BIAS: [2 far + 1]
   float* near = lut + (BIAS ? 2 * relative::far_of(a.relative) + 1 : 0);  // dq with BIAS: [8 warps][2 far + 1]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int group = (int)(a.heads / a.kv_heads), dim = (int)a.dim;
   const int hy = blockIdx.y, kvh = DKV ? hy : hy / group;
   const int64_t b = blockIdx.z;
@@ -460,6 +500,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int lo = DKV ? seq.first_query(a, r0) : seq.first_key(a, r0), hi = DKV ? seq.end_query(a, r1) : seq.end_key(a, r1);
     if (hi > lo) first = lo / BN, per = (hi + BN - 1) / BN - first;
   }
+  first = uniform(first), per = uniform(per);
   const int total = per * (DKV ? group : 1);
   const int far = BIAS ? relative::far_of(a.relative) : 0, bins = 2 * far + 1;
   // tile n: its head and first token
@@ -467,6 +508,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   auto token_of = [&](int n) { return (first + (DKV ? n % per : n)) * BN; };
 
   if (threadIdx.x == 0) {
+    *gave_up = 0;
     for (const CUtensorMap* m : {&map_x0, &map_x1, &map_y0, &map_y1})
       asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
     mbar_init(x_full, 1);
@@ -494,7 +536,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
 
   if (warp == 0) {
     if (lane == 0 && total > 0) {
@@ -507,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       int n = 0;
       for (; n < total; ++n) {
         const int s = n % ST;
-        if (!mbar_wait(&y_empty[s], ((n / ST) & 1) ^ 1)) break;
+        wait(&y_empty[s], ((n / ST) & 1) ^ 1, gave_up);
         mbar_expect_tx(&y_full[s], 2 * G::Y);
         const int yh = DKV ? head_of(n) : kvh;
         for (int p = 0; p < DP / 64; ++p) {
@@ -517,16 +559,16 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
       }
       // every load has landed before the block may end
-      mbar_wait(x_full, 0);
-      for (int m = max(0, n - ST); m < n; ++m) mbar_wait(&y_full[m % ST], (m / ST) & 1);
+      wait(x_full, 0, gave_up);
+      for (int m = max(0, n - ST); m < n; ++m) wait(&y_full[m % ST], (m / ST) & 1, gave_up);
     }
   } else if (warp == 1) {
-    const int ks = (dim + 15) / 16;
+    const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, BN, false), id_a = idesc_of(ROWS, ks * 16, true);
-    bool ok = total > 0 && warp_wait(x_full, 0);
-    auto scores = [&](int n) {  // S and dP of tile n
-      const int s = n % ST;
-      if (!warp_wait(&y_full[s], (n / ST) & 1)) return false;
+    if (total > 0) warp_wait(x_full, 0, gave_up);
+    const Desc x0 = desc_at(s_x, 16), x1 = desc_at(s_x + G::X, 16), yk = desc_at(s_y, 16), ymn = desc_at(s_y, BN * 128);
+    auto scores = [&](int n, int s, int par) {  // S and dP of tile n, in stage s
+      warp_wait(&y_full[s], par, gave_up);
       const uint32_t y = s_y + s * 2 * G::Y;
       const int have = (DKV ? seq.queries : seq.keys) - token_of(n);
       if (have < BN && (DKV ? seq.queries < a.queries : seq.keys < a.keys)) {
@@ -537,47 +579,50 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       }
       tc_fence_after();
-      if (lane == 0) {
-        for (int k = 0; k < ks; ++k) mma_bf16(tmem, desc_k<ROWS>(s_x, k), desc_k<BN>(y, k), id_s, k > 0);
-        for (int k = 0; k < ks; ++k) mma_bf16(tmem + G::T_DP, desc_k<ROWS>(s_x + G::X, k), desc_k<BN>(y + G::Y, k), id_s, k > 0);
-        mma_commit(sp_full);
-      }
-      __syncwarp();
-      return true;
+      const Desc y0 = {yk.lo + s * (2 * G::Y >> 4), yk.hi}, y1 = {y0.lo + (G::Y >> 4), yk.hi};
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < ks) mma(elected, tmem, x0, off_k<ROWS>(k), y0, off_k<BN>(k), id_s, k > 0);
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k)
+        if (k < ks) mma(elected, tmem + G::T_DP, x1, off_k<ROWS>(k), y1, off_k<BN>(k), id_s, k > 0);
+      commit(elected, sp_full);
     };
-    if (ok) ok = scores(0);
-    for (int n = 0; n < total && ok; ++n) {
+    if (total > 0) scores(0, 0, 0);
+    for (int n = 0, s = 0, par = 0, next = 0; n < total; ++n, s = next) {
+      next = s + 1 == ST ? 0 : s + 1;
+      par ^= next == 0;
       if (n + 1 < total) {
-        if (!(ok = warp_wait(sp_free, n & 1))) break;
-        if (!(ok = scores(n + 1))) break;
+        warp_wait(sp_free, n & 1, gave_up);
+        scores(n + 1, next, par);
       }
-      if (!(ok = warp_wait(pd_full, n & 1))) break;
+      warp_wait(pd_full, n & 1, gave_up);
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t y = s_y + (n % ST) * 2 * G::Y;
-        if constexpr (DKV) {
-          for (int k = 0; k < BN / 16; ++k)  // dV += P dO
-            mma_from_tmem(tmem + G::T_ACC, tmem + G::T_P + k * 8, desc_mn<BN>(y + G::Y, k), id_a, n > 0 || k > 0);
-          for (int k = 0; k < BN / 16; ++k)  // dK += dS Q
-            mma_from_tmem(tmem + G::T_ACC + DP, tmem + G::T_DS + k * 8, desc_mn<BN>(y, k), id_a, n > 0 || k > 0);
-        } else {
-          for (int k = 0; k < BN / 16; ++k)  // dQ += dS K
-            mma_from_tmem(tmem + G::T_ACC, tmem + G::T_DS + k * 8, desc_mn<BN>(y, k), id_a, n > 0 || k > 0);
-        }
-        mma_commit(&y_empty[n % ST]);
-        mma_commit(pd_free);
-        if (n + 1 == total) mma_commit(acc_full);
+      const Desc y0 = {ymn.lo + s * (2 * G::Y >> 4), ymn.hi}, y1 = {y0.lo + (G::Y >> 4), ymn.hi};
+      if constexpr (DKV) {
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)  // dV += P dO
+          mma_from_tmem(elected, tmem + G::T_ACC, tmem + G::T_P + k * 8, y1, off_mn(k), id_a, n > 0 || k > 0);
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)  // dK += dS Q
+          mma_from_tmem(elected, tmem + G::T_ACC + DP, tmem + G::T_DS + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
+      } else {
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)  // dQ += dS K
+          mma_from_tmem(elected, tmem + G::T_ACC, tmem + G::T_DS + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
       }
-      __syncwarp();
+      commit(elected, &y_empty[s]);
+      commit(elected, pd_free);
+      if (n + 1 == total) commit(elected, acc_full);
     }
     // no MMA and no commit is on its way when the block ends
-    if (lane == 0) mma_commit(idle);
-    warp_wait(idle, 0);
+    commit(elected, idle);
+    warp_wait(idle, 0, gave_up);
   } else if (DKV && warp == 2) {
     // the queries' lse (log2; infinite where nothing is to be had) and delta
     for (int n = 0; n < total; ++n) {
       const int s = n % ST;
-      if (!warp_wait(&y_empty[s], ((n / ST) & 1) ^ 1)) break;
+      warp_wait(&y_empty[s], ((n / ST) & 1) ^ 1, gave_up);
       const int64_t at = (b * a.heads + head_of(n)) * a.queries;
       for (int c = lane; c < BN; c += 32) {
         const int i = token_of(n) + c;
@@ -611,7 +656,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       row_delta = io.delta[at];
     }
     float* my_near = near + (warp - 4) * bins;
-    bool ok = true;
     int lut_head = -1;
     for (int n = 0; n < total; ++n) {
       if constexpr (BIAS && DKV) {
@@ -624,12 +668,8 @@ __global__ void __launch_bounds__(THREADS, 1)
           asm volatile("bar.sync 1, 256;" ::: "memory");
         }
       }
-      if (ok) ok = warp_wait(sp_full, n & 1);
-      if (DKV && ok) ok = warp_wait(&st_full[n % ST], (n / ST) & 1);
-      if (!ok) {
-        if (BIAS && DKV) continue;  // the others still meet at the lookup's barrier
-        break;
-      }
+      warp_wait(sp_full, n & 1, gave_up);
+      if constexpr (DKV) warp_wait(&st_full[n % ST], (n / ST) & 1, gave_up);
       tc_fence_after();
       const float* stat = s_stat + (n % ST) * 2 * BN + g * HALF;
 #pragma unroll
@@ -663,11 +703,7 @@ __global__ void __launch_bounds__(THREADS, 1)
               x[k] = fmaf(__uint_as_float(s[k]), sl, lut[max(-far, min(far, rel)) + far]);
             }
           }
-        } else {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) x[k] = __uint_as_float(s[k]) * sl;
         }
-        const bool cut = t0 < full0 || t0 + 32 > full1;
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           float4 ls, de;
@@ -681,12 +717,18 @@ __global__ void __launch_bounds__(THREADS, 1)
           const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            float p = ex2(x[k + u] - l4[u]);
-            float z = p * (__uint_as_float(d[k + u]) - d4[u]);
-            if (cut && (t0 + k + u < lo || t0 + k + u >= hi)) p = z = 0.f;
-            x[k + u] = z;
+            const float p = ex2(BIAS ? x[k + u] - l4[u] : fmaf(__uint_as_float(s[k + u]), sl, -l4[u]));
+            x[k + u] = p * (__uint_as_float(d[k + u]) - d4[u]);
             s[k + u] = __float_as_uint(p);
           }
+        }
+        if (t0 < full0 || t0 + 32 > full1) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k)
+            if (t0 + k < lo || t0 + k >= hi) {
+              x[k] = 0.f;
+              s[k] = 0;
+            }
         }
         if constexpr (BIAS && !DKV) {
           if (!valid) {
@@ -717,7 +759,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
         if (c0 == 0 && n > 0) {
           // the sums of the tile before have read P and dS
-          if (!(ok = warp_wait(pd_free, (n - 1) & 1))) break;
+          warp_wait(pd_free, (n - 1) & 1, gave_up);
           tc_fence_after();
         }
         uint32_t p[16];
@@ -733,9 +775,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (ok && lane == 0) mbar_arrive(pd_full);
+      if (lane == 0) mbar_arrive(pd_full);
     }
-    const bool some = total > 0 && ok && warp_wait(acc_full, 0);
+    const bool some = total > 0;
+    if (some) warp_wait(acc_full, 0, gave_up);
     tc_fence_after();
     const int rows = DKV ? (int)a.keys : (int)a.queries, heads = DKV ? (int)a.kv_heads : (int)a.heads;
     // dk, dv: a warpgroup each; dq: half of the columns each
