@@ -37,20 +37,22 @@ static int check_attention(const char* what, const b200_attention* a) {
   return B200_OK;
 }
 
-// delta = dout . out of every query: 8 lanes each, two 8-element pieces of both rows in flight a lane
+// What the gradient needs of each query beside its own row: delta = dout . out, and lse in the log2 domain, infinite where the
+// query sees nothing or is none (so that p = 0). [batch x heads][padded]; 8 lanes a query, two 16-byte pieces of both rows in flight a lane.
 template <typename T>
-__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200_attention a, const T* dout, const T* out, int64_t sb, int64_t ss,
-                                                    int64_t sh, float* delta, int vec) {
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;  // [batch, queries, heads]
+__global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200_attention a, const T* dout, const T* out, const float* lse, int64_t sb,
+                                                    int64_t ss, int64_t sh, float* lse2, float* delta, int64_t padded, int vec) {
+  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;  // [batch, padded, heads]
   const int lane = threadIdx.x & 7;
-  const bool in = row < a.batch * a.queries * a.heads;
-  float s = 0.f;
+  const bool in = row < a.batch * padded * a.heads;
+  float s = 0.f, e = INFINITY;
   int64_t h = 0, i = 0, b = 0;
   if (in) {
-    h = row % a.heads, i = row / a.heads % a.queries, b = row / a.heads / a.queries;
-    const T *x = dout + b * sb + i * ss + h * sh, *y = out + row * a.dim;
-    if (i >= Sequence(a, b).queries) {
-    } else {
+    h = row % a.heads, i = row / a.heads % padded, b = row / a.heads / padded;
+    if (i < Sequence(a, b).queries) {
+      const T *x = dout + b * sb + i * ss + h * sh, *y = out + ((b * a.queries + i) * a.heads + h) * a.dim;
+      e = lse[(b * a.heads + h) * a.queries + i] * LOG2E;
+      if (e == -INFINITY) e = INFINITY;
       constexpr int V = 16 / sizeof(T);
 #pragma unroll 2
       for (int c = lane * V; c < a.dim; c += 8 * V) {
@@ -67,11 +69,15 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200
   }
 #pragma unroll
   for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (in && lane == 0) delta[(b * a.heads + h) * a.queries + i] = s;
+  if (in && lane == 0) {
+    delta[(b * a.heads + h) * padded + i] = s;
+    lse2[(b * a.heads + h) * padded + i] = e;
+  }
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
-static size_t delta_bytes(const b200_attention& a) { return up256((size_t)(a.batch * a.heads * a.queries) * sizeof(float)); }
+static int64_t padded_of(const b200_attention& a) { return ceil_div(a.queries, 128) * 128; }
+static size_t delta_bytes(const b200_attention& a) { return (size_t)(2 * a.batch * a.heads * padded_of(a)) * sizeof(float); }
 
 }  // namespace attention
 }  // namespace b200
@@ -120,16 +126,18 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
   const size_t need = b200_attention_grad_workspace_bytes(a);
   B200_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
-  float* delta = reinterpret_cast<float*>(workspace);
-  const unsigned grid = (unsigned)ceil_div(a->batch * a->queries * a->heads, 32);
-  B200_REQUIRE(a->batch * a->queries * a->heads < (1ll << 35), "attention_grad: too many queries");
+  const int64_t padded = padded_of(*a);
+  float *lse2 = reinterpret_cast<float*>(workspace), *delta = lse2 + a->batch * a->heads * padded;
+  const unsigned grid = (unsigned)ceil_div(a->batch * padded * a->heads, 32);
+  B200_REQUIRE(a->batch * padded * a->heads < (1ll << 35), "attention_grad: too many queries");
   const int64_t* s = g->dout_stride;
   const int vec = ((reinterpret_cast<uintptr_t>(g->dout) | reinterpret_cast<uintptr_t>(g->out) | (uint64_t)((s[0] | s[1] | s[2] | a->dim) * size)) & 15) == 0;
   if (a->dtype == B200_F32)
-    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, s[0], s[1], s[2], delta, vec);
+    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, g->lse, s[0], s[1], s[2], lse2, delta, padded, vec);
   else
-    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, s[0], s[1], s[2], delta, vec);
+    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, g->lse, s[0], s[1], s[2], lse2,
+                                                      delta, padded, vec);
   if (int rc = check_launch("attention_grad")) return rc;
   void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
-  return tiles_take(*a) ? tiles_grad(*a, *g, delta, rest, st) : rows_grad(*a, *g, delta, rest, st);
+  return tiles_take(*a) ? tiles_grad(*a, *g, lse2, delta, padded, rest, st) : rows_grad(*a, *g, delta, padded, rest, st);
 }

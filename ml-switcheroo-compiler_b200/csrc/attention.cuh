@@ -52,7 +52,7 @@ __device__ __forceinline__ float table_log2(const void* table, int64_t at, int d
 size_t rows_forward_workspace(const b200_attention& a);
 int rows_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t rows_grad_workspace(const b200_attention& a);
-int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st);
+int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, int64_t padded, void* workspace, cudaStream_t st);
 // dtable from [batch][heads][blocks][buckets] partial sums, in order
 int table_sum(const b200_attention& a, const float* part, int64_t blocks, void* dtable, cudaStream_t st);
 
@@ -61,7 +61,9 @@ bool tiles_take(const b200_attention& a);
 size_t tiles_forward_workspace(const b200_attention& a);
 int tiles_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads* g);
-int tiles_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st);
+// lse2 (log2, infinite where a query sees nothing) and delta: [batch x heads][padded], padded a multiple of 128
+int tiles_grad(const b200_attention& a, const b200_attention_grads& g, const float* lse2, const float* delta, int64_t padded, void* workspace,
+               cudaStream_t st);
 
 }  // namespace attention
 }  // namespace b200

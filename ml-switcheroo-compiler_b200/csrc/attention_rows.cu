@@ -32,7 +32,8 @@ struct Io {
   float* lse;                   // FWD: written; else read
   const void* dout;
   int64_t dout_stride[3];
-  const float* delta;
+  const float* delta;           // [batch x heads][padded]
+  int64_t padded;
   float* part;                  // FWD with splits: [row blocks][splits][R][dim + 2]; DQ with a table: [row blocks][buckets]
 };
 
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
     const int64_t at = (b * a.heads + my_head) * a.queries + my_row;
     my_lse = io.lse[at] * LOG2E;
     if (my_lse == -INFINITY) my_lse = INFINITY;  // sees nothing: p = 0
-    my_delta = io.delta[at];
+    my_delta = io.delta[(b * a.heads + my_head) * io.padded + my_row];
   }
   float* sp = s_p + warp * 64;
 
@@ -287,7 +288,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
           const int64_t at = (b * a.heads + kvh * group + t % group) * a.queries + i;
           lse = io.lse[at] * LOG2E;
           if (lse == -INFINITY) lse = INFINITY;
-          delta = io.delta[at];
+          delta = io.delta[(b * a.heads + kvh * group + t % group) * io.padded + i];
         }
       }
       const float p = seen ? exp2f(s - lse) : 0.f;
@@ -406,15 +407,15 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   }
   if constexpr (MODE == DQ) {
     if (a.table) {
-      const int nb = relative::buckets_of(a.relative);
-      for (int n = threadIdx.x; n < nb; n += THREADS) {
+      for (int i = threadIdx.x; i < bins; i += THREADS) {
         float s = 0.f;
-        for (int i = 0; i < bins; ++i)
-          if (s_bucket[i] == n)
 #pragma unroll
-            for (int w = 0; w < WARPS; ++w) s += s_near[w * bins + i];
-        io.part[row_block * nb + n] = s;
+        for (int w = 0; w < WARPS; ++w) s += s_near[w * bins + i];
+        s_near[i] = s;  // this thread's column alone
       }
+      __syncthreads();
+      const int nb = relative::buckets_of(a.relative);
+      for (int n = threadIdx.x; n < nb; n += THREADS) io.part[row_block * nb + n] = relative::bucket_sum(a.relative, far, s_near, n);
     }
   }
 }
@@ -570,11 +571,11 @@ size_t rows_grad_workspace(const b200_attention& a) {
   return (size_t)(a.batch * a.heads * ceil_div(a.queries, R) * relative::buckets_of(a.relative)) * sizeof(float);
 }
 
-int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st) {
+int rows_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, int64_t padded, void* workspace, cudaStream_t st) {
   using namespace rows;
   const int R = a.dim <= 128 ? 8 : 4;
   Io io = {};
-  io.splits = 1, io.vec = vectors(a, elements(a), g.dout, g.dout_stride), io.dout = g.dout, io.delta = delta;
+  io.splits = 1, io.vec = vectors(a, elements(a), g.dout, g.dout_stride), io.dout = g.dout, io.delta = delta, io.padded = padded;
   for (int i = 0; i < 3; ++i) io.dout_stride[i] = g.dout_stride[i];
   io.lse = const_cast<float*>(g.lse);
   io.out_rows = ceil_div(a.queries, R), io.out = g.dq, io.part = reinterpret_cast<float*>(workspace);

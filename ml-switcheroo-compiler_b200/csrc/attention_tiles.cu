@@ -1,27 +1,31 @@
 // Attention on the tensor cores: bf16 heads of up to 128 elements, many queries.
 //
-// Forward. A block takes two tiles of 128 queries of one head past the keys, 128 at a time:
-//   warp 0       TMA: both query tiles once, then K and V tiles into a ring;
-//   warp 1       owns TMEM, issues S_w = Q_w K^T (operands in shared memory) and O_w += P_w V (P from TMEM);
-//   warps 4-7, 8-11   softmax of tile 0, tile 1: a thread owns a query's row of S.
-// TMEM: S_0, S_1 (128 columns each; P, bf16, over its own S), O_0, O_1. While one tile's threads make their
-// exponentials, the tensor cores work for the other. S_w of the next keys is issued right behind O_w's product: MMAs
-// run in their order, so it overwrites P only when that is used up, and its completion says that O_w is at rest.
-// The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8, sums are
-// fp32), so O is hardly ever rescaled.
+// Forward. A block takes 128 queries of one head past the keys, 128 at a time; two blocks share an SM, so that one's
+// exponentials run under the other's MMAs, and its start and end under the other's middle:
+//   warp 0      TMA: the queries once, then K and V tiles into a ring;
+//   warp 1      owns 256 columns of TMEM, issues S = Q K^T (operands in shared memory) and O += P V (P from TMEM);
+//   warps 2-5   softmax: a thread owns a query's row of S.
+// Heads of up to 64: S, P and O have columns of their own (128 + 64 + 64), and the next S is made as soon as the threads hold this
+// one in registers. Wider heads: P lies over S (O has 128), whose MMAs, issued behind O's, overwrite it only when it is used up: MMAs
+// run in their order. The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8,
+// sums are fp32), so O is hardly ever rescaled. P is handed over in two halves of 64 keys.
+// The special function unit makes 16 exponentials a clock: 1024 clocks a tile, of which the MMAs take 512 (heads of 64). A part of
+// them is therefore made on the FMA pipe (exp2_pair).
 //
-// Backward, one kernel in two forms. 128 rows stay, tiles of the other side go past:
+// Backward, one kernel in two forms. 128 rows stay, tiles of 64 tokens of the other side go past:
 //   dq:      rows are queries (Q, dO), tiles are keys (K, V):     S = Q K^T, dP = dO V^T, dQ += dS K
 //   dk, dv:  rows are keys (K, V), tiles are queries (Q, dO):     S = K Q^T, dP = V dO^T, dV += P dO, dK += dS Q
-// so p and dz of a tile are made by the threads that own its rows, go back to TMEM as bf16 and are the A operand of the
-// sums from there: nothing is transposed, no sum leaves its block, every order is fixed. S and dP are made
-// twice for that (7 products instead of 5). Threads read S and dP early, so the MMAs of the next tile run
-// under their exponentials.
+// so p and dz of a tile are made by the threads that own its rows, go back to TMEM as bf16 over the S and dP that they come
+// from, and are the A operand of the sums there: nothing is transposed, no sum leaves its block, every order is fixed. S and
+// dP are made twice for that (7 products instead of 5). Heads of up to 64: one warpgroup and 256 columns of TMEM a block, two
+// blocks an SM; wider heads: two warpgroups that take tiles in turn, each with an S and dP of its own.
+// Tiles of 64 because of TMEM; an MMA of 128 x 64 from shared memory takes 48 clocks, of 128 x 128 64 (measured).
 //
 // Probabilities and dz are rounded to bf16 for the products that they are operands of; scores, maxima, sums and
 // all accumulators are fp32. Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
 // block winds down.
 #include <algorithm>
+#include <type_traits>
 
 #include "attention.cuh"
 #include "tc_common.cuh"
@@ -32,8 +36,27 @@ namespace tiles {
 
 using namespace tc;
 
-constexpr int THREADS = 384, ROWS = 128;
+constexpr int ROWS = 128;
 constexpr uint32_t SMEM_LIMIT = 232448;
+
+// Which rows and head a block has. Blocks of one group of heads come one after the other, and in it the row tiles in turn: causal
+// calls with the most tiles first and as many heads a group as have their tokens in the L2, others head by head.
+struct Order {
+  int row_tiles, heads, pairs, group, last_first;  // pairs: batch x heads
+};
+struct Place {
+  int tile, head;
+  int64_t batch;
+  __device__ __forceinline__ Place(const Order& o) {
+    const int per = o.group * o.row_tiles;
+    const int g = (int)blockIdx.x / per, r = (int)blockIdx.x % per;
+    const int size = min(o.group, o.pairs - g * o.group);
+    const int pair = g * o.group + r % size;
+    tile = r / size;
+    if (o.last_first) tile = o.row_tiles - 1 - tile;
+    head = pair % o.heads, batch = pair / o.heads;
+  }
+};
 
 // Bounded wait of whoever calls it. A look at the timer takes longer than a tile's MMAs, so it comes every 256 polls. After
 // WAIT_LIMIT_NS the block gives up: every later wait ends at once, results are not valid, the error flag says so.
@@ -109,6 +132,20 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
       "%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
       B200_R16(r, 0), B200_R16(r, 16));
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+        "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
+// `bytes` (a multiple of 16, both addresses too) of global memory, counted on the barrier
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
+               "r"(smem_u32(bar))
+               : "memory");
+}
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t idesc_of(int m, int n, bool b_mn) {
@@ -132,6 +169,47 @@ __device__ __forceinline__ void zero_rows(uint32_t base, int from, int lane) {
 __device__ __forceinline__ void fill_bias(float* lut, const b200_attention& a, int far, int head) {
   for (int i = threadIdx.x; i <= 2 * far; i += blockDim.x)
     lut[i] = table_log2(a.table, (int64_t)relative::bucket_of(a.relative, i - far) * a.heads + head, a.table_dtype);
+}
+
+// two fp32 in one instruction
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(a)), "r"(__float_as_uint(b)));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t r, float& a, float& b) {
+  uint32_t x, y;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(x), "=r"(y) : "l"(r));
+  a = __uint_as_float(x), b = __uint_as_float(y);
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// 2^x of two values on the FMA pipe, -125 < x < 127: x = n + f with n whole (adding 1.5 2^23 rounds it there and leaves n in the low bits), 2^f by
+// a polynomial of degree 4 fitted to the least relative error over [-1/2, 1/2] (2.7e-6 with fp32's rounding; a probability's
+// rounding to bf16 is 2e-3), n added to the exponent.
+__device__ __forceinline__ void exp2_pair(uint64_t x, float& a, float& b) {
+  const float big = 12582912.f;
+  const uint64_t t = add2(x, pack2(big, big));
+  const uint64_t n = add2(t, pack2(-big, -big));
+  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
+  uint64_t p = pack2(0.009570102207362652f, 0.009570102207362652f);
+  p = fma2(p, f, pack2(0.05591786280274391f, 0.05591786280274391f));
+  p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
+  p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float t0, t1;
+  unpack2(t, t0, t1);
+  unpack2(p, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
 }
 
 // 32 fp32 columns of a row, scaled, to a row of the result from column `col` on
@@ -158,53 +236,58 @@ __device__ __forceinline__ void store32(__nv_bfloat16* row, int col, int dim, bo
 // forward
 // ------------------------------------------------------------------------------------
 
-constexpr int KEYS = 128;
+constexpr int KEYS = 128, FWD_THREADS = 192;
 constexpr float LAZY = 8.f;  // log2 by which a maximum may grow before O is rescaled
+constexpr float FLOOR = -124.f;  // what exp2_pair takes
+__device__ __forceinline__ float floored(float x) {  // a score that is no number stays none
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(FLOOR));
+  return r;
+}
+// of 8 pairs of exponentials, those made on the FMA pipe
+constexpr int FMA_PAIRS = 3;
 
 template <int DP>
 struct Fwd {
-  static constexpr int STAGES = DP == 64 ? 4 : 2;
+  static constexpr bool APART = DP == 64;  // P beside S
+  static constexpr int STAGES = DP == 64 ? 2 : 1;
   static constexpr uint32_t TILE = 128 * DP * 2;
-  static constexpr uint32_t BARS = 2 * TILE + STAGES * 2 * TILE;
+  static constexpr uint32_t BARS = TILE + STAGES * 2 * TILE;
   static constexpr uint32_t LUT = BARS + 256;
-  static constexpr uint32_t TMEM_O = 256;
+  static constexpr uint32_t TMEM = 256, T_P = APART ? 128 : 0, T_O = TMEM - DP;
 };
 
 template <int DP, bool BIAS>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(FWD_THREADS, 2)
     forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                   const __grid_constant__ b200_attention a, __nv_bfloat16* out, float* lse, int vec) {
+                   const __grid_constant__ b200_attention a, const __grid_constant__ Order order, __nv_bfloat16* out, float* lse, int vec) {
   using F = Fwd<DP>;
   constexpr int ST = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t s_q = smem_u32(smem), s_k = s_q + 2 * F::TILE, s_v = s_k + ST * F::TILE;
+  const uint32_t s_q = smem_u32(smem), s_k = s_q + F::TILE, s_v = s_k + ST * F::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST,
-           *p_full = s_full + 2, *o_full = p_full + 2, *idle = o_full + 2;
+           *s_free = s_full + 1, *p_full = s_full + 2, *o_done = s_full + 4, *idle = s_full + 5;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* lut = reinterpret_cast<float*>(smem + F::LUT);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  const int head = blockIdx.y, kvh = head / (int)(a.heads / a.kv_heads), dim = (int)a.dim;
-  const int64_t b = blockIdx.z;
+  const Place at(order);
+  const int head = at.head, kvh = head / (int)(a.heads / a.kv_heads), dim = (int)a.dim;
+  const int64_t b = at.batch;
   const Sequence seq(a, b);
-  // causal blocks with the most keys start first
-  const int pair = a.causal ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
-  int t0[2], t1[2];  // key tiles of each query tile
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    const int i0 = (2 * pair + w) * ROWS, i1 = min(i0 + ROWS, seq.queries) - 1;
-    t0[w] = t1[w] = 0;
-    if (i1 >= i0) {
-      const int lo = seq.first_key(a, i0), hi = seq.end_key(a, i1);
-      if (hi > lo) t0[w] = lo / KEYS, t1[w] = (hi + KEYS - 1) / KEYS;
+  const int r0 = at.tile * ROWS;
+  int T0 = 0, n_tiles = 0;  // key tiles
+  {
+    const int r1 = min(r0 + ROWS, seq.queries) - 1;
+    if (r1 >= r0) {
+      const int lo = seq.first_key(a, r0), hi = seq.end_key(a, r1);
+      if (hi > lo) T0 = lo / KEYS, n_tiles = (hi + KEYS - 1) / KEYS - T0;
     }
-    t0[w] = uniform(t0[w]), t1[w] = uniform(t1[w]);
+    T0 = uniform(T0), n_tiles = uniform(n_tiles);
   }
-  const bool any0 = t1[0] > t0[0], any1 = t1[1] > t0[1];
-  const int T0 = any0 ? (any1 ? min(t0[0], t0[1]) : t0[0]) : t0[1], T1 = max(t1[0], t1[1]);
   const int far = BIAS ? relative::far_of(a.relative) : 0;
 
   if (threadIdx.x == 0) {
@@ -217,16 +300,16 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(&s_full[w], 1);
-      mbar_init(&p_full[w], 4);
-      mbar_init(&o_full[w], 1);
-    }
+    mbar_init(s_full, 1);
+    mbar_init(s_free, 4);
+    mbar_init(&p_full[0], 4);
+    mbar_init(&p_full[1], 4);
+    mbar_init(o_done, 1);
     mbar_init(idle, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(F::TMEM));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if constexpr (BIAS) fill_bias(lut, a, far, head);
@@ -236,28 +319,24 @@ __global__ void __launch_bounds__(THREADS, 1)
   const uint32_t tmem = (uint32_t)uniform((int)*tmem_slot);
 
   if (warp == 0) {
-    if (lane == 0 && T1 > T0) {
-      mbar_expect_tx(q_full, ((any0 ? 1 : 0) + (any1 ? 1 : 0)) * F::TILE);
-      for (int w = 0; w < 2; ++w)
-        if (t1[w] > t0[w])
-          for (int p = 0; p < DP / 64; ++p)
-            tma_load_4d(smem + w * F::TILE + p * (ROWS * 128), &map_q, q_full, p * 64, (2 * pair + w) * ROWS, head, (int)b);
-      int n = 0;
-      for (int t = T0; t < T1; ++t, ++n) {
+    if (lane == 0 && n_tiles > 0) {
+      mbar_expect_tx(q_full, F::TILE);
+      for (int p = 0; p < DP / 64; ++p) tma_load_4d(smem + p * (ROWS * 128), &map_q, q_full, p * 64, r0, head, (int)b);
+      for (int n = 0; n < n_tiles; ++n) {
         const int s = n % ST;
         const uint32_t par = ((n / ST) & 1) ^ 1;
         wait(&k_empty[s], par, gave_up);
         mbar_expect_tx(&k_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
-          tma_load_4d(smem + 2 * F::TILE + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, t * KEYS, kvh, (int)b);
+          tma_load_4d(smem + F::TILE + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
         wait(&v_empty[s], par, gave_up);
         mbar_expect_tx(&v_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
-          tma_load_4d(smem + (2 + ST) * F::TILE + s * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, t * KEYS, kvh, (int)b);
+          tma_load_4d(smem + (1 + ST) * F::TILE + s * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
       }
       // every load has landed before the block may end
       wait(q_full, 0, gave_up);
-      for (int m = max(0, n - ST); m < n; ++m) {
+      for (int m = max(0, n_tiles - ST); m < n_tiles; ++m) {
         wait(&k_full[m % ST], (m / ST) & 1, gave_up);
         wait(&v_full[m % ST], (m / ST) & 1, gave_up);
       }
@@ -265,27 +344,29 @@ __global__ void __launch_bounds__(THREADS, 1)
   } else if (warp == 1) {
     const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, KEYS, false), id_o = idesc_of(ROWS, ks * 16, true);
-    if (T1 > T0) warp_wait(q_full, 0, gave_up);
     const Desc dq = desc_at(s_q, 16), dk = desc_at(s_k, 16), dv = desc_at(s_v, KEYS * 128);
-    auto product_s = [&](int w, int s) {  // S_w of the tile in stage s, whose K has landed
+    auto scores = [&](int s, int par) {  // S of the tile in stage s
+      warp_wait(&k_full[s], par, gave_up);
       tc_fence_after();
-      const Desc kd = {dk.lo + s * (F::TILE >> 4), dk.hi}, qd = {dq.lo + w * (F::TILE >> 4), dq.hi};
+      const Desc kd = {dk.lo + s * (F::TILE >> 4), dk.hi};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        if (k < ks) mma(elected, tmem + w * KEYS, qd, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
-      commit(elected, &s_full[w]);
+        if (k < ks) mma(elected, tmem, dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
+      commit(elected, s_full);
+      commit(elected, &k_empty[s]);
     };
-    int done[2] = {0, 0};
-    if (T1 > T0) {
-      warp_wait(&k_full[0], 0, gave_up);
-      for (int w = 0; w < 2; ++w)
-        if (t0[w] == T0 && t1[w] > t0[w]) product_s(w, 0);
-      commit(elected, &k_empty[0]);
+    if (n_tiles > 0) {
+      warp_wait(q_full, 0, gave_up);
+      scores(0, 0);
     }
-    for (int t = T0, s = 0, par = 0, next = 0, next_par = 0; t < T1; ++t, s = next, par = next_par) {
+    for (int n = 0, s = 0, par = 0, next = 0, next_par = 0; n < n_tiles; ++n, s = next, par = next_par) {
       next = s + 1 == ST ? 0 : s + 1, next_par = s + 1 == ST ? par ^ 1 : par;
+      if (F::APART && n + 1 < n_tiles) {
+        warp_wait(s_free, n & 1, gave_up);
+        scores(next, next_par);
+      }
       warp_wait(&v_full[s], par, gave_up);
-      const int have = seq.keys - t * KEYS;
+      const int have = seq.keys - (T0 + n) * KEYS;
       if (have < KEYS && seq.keys < a.keys) {
         // what lies behind the sequence's end may be anything, and is multiplied by zeros
         zero_rows<KEYS, DP>(s_v + s * F::TILE, max(have, 0), lane);
@@ -293,54 +374,52 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
       }
       const Desc vd = {dv.lo + s * (F::TILE >> 4), dv.hi};
-      if (t + 1 < T1) warp_wait(&k_full[next], next_par, gave_up);
 #pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        if (t >= t0[w] && t < t1[w]) {
-          warp_wait(&p_full[w], done[w] & 1, gave_up);
-          tc_fence_after();
+      for (int h = 0; h < 2; ++h) {
+        warp_wait(&p_full[h], n & 1, gave_up);
+        tc_fence_after();
 #pragma unroll
-          for (int k = 0; k < KEYS / 16; ++k)
-            mma_from_tmem(elected, tmem + F::TMEM_O + w * DP, tmem + w * KEYS + k * 8, vd, off_mn(k), id_o, done[w] > 0 || k > 0);
-          if (t + 1 == t1[w]) commit(elected, &o_full[w]);
-          ++done[w];
-        }
-        if (t + 1 >= t0[w] && t + 1 < t1[w]) product_s(w, next);
+        for (int k = 4 * h; k < 4 * h + 4; ++k)
+          mma_from_tmem(elected, tmem + F::T_O, tmem + F::T_P + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
       }
       commit(elected, &v_empty[s]);
-      if (t + 1 < T1) commit(elected, &k_empty[next]);
+      commit(elected, o_done);
+      if (!F::APART && n + 1 < n_tiles) scores(next, next_par);
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
     warp_wait(idle, 0, gave_up);
-  } else if (warp >= 4) {
-    const int w = (warp - 4) >> 2, q = warp & 3;
-    const int i0 = (2 * pair + w) * ROWS + q * 32, i = i0 + lane;
+  } else {
+    const int q = warp & 3;
+    const int i0 = r0 + q * 32, i = i0 + lane;
     const bool valid = i < seq.queries;
     const int lo = valid ? seq.first_key(a, i) : 0, hi = valid ? seq.end_key(a, i) : 0;
     // every key of [full0, full1) is seen by all rows of the warp
-    const int last = min(i0 + 31, seq.queries - 1);
-    const int full0 = seq.first_key(a, last), full1 = seq.end_key(a, i0);
-    const uint32_t lanes = (uint32_t)(q * 32) << 16;
-    const uint32_t t_s = tmem + lanes + w * KEYS, t_o = tmem + lanes + F::TMEM_O + w * DP;
+    const int full0 = seq.first_key(a, min(i0 + 31, seq.queries - 1)), full1 = seq.end_key(a, i0);
+    const uint32_t t_s = tmem + ((uint32_t)(q * 32) << 16), t_p = t_s + F::T_P, t_o = t_s + F::T_O;
     const float sl = a.scale * LOG2E;
     float m = -INFINITY, l = 0.f;
-    for (int t = t0[w]; t < t1[w]; ++t) {
-      const int n = t - t0[w], j0 = t * KEYS;
-      warp_wait(&s_full[w], n & 1, gave_up);
+    for (int n = 0; n < n_tiles; ++n) {
+      const int j0 = (T0 + n) * KEYS;
+      warp_wait(s_full, n & 1, gave_up);
       tc_fence_after();
       uint32_t v[4][32];
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_ld32_issue(t_s + c * 32, v[c]);
 #pragma unroll
       for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
+      if constexpr (F::APART) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_free);
+      }
       float mul = sl;
       if constexpr (BIAS) {
         mul = 1.f;
-        const int r0 = j0 - i - seq.shift;  // of column 0
-        const int w0 = j0 - i0 - seq.shift;  // of lane 0
-        if (w0 - 31 >= far || w0 + KEYS - 1 <= -far) {
-          const float c0 = lut[w0 >= far ? 2 * far : 0];
+        const int rel0 = j0 - i - seq.shift;   // of column 0
+        const int w_rel = j0 - i0 - seq.shift;  // of lane 0
+        if (w_rel - 31 >= far || w_rel + KEYS - 1 <= -far) {
+          const float c0 = lut[w_rel >= far ? 2 * far : 0];
 #pragma unroll
           for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -350,10 +429,11 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int k = 0; k < 32; ++k)
-              v[c][k] = __float_as_uint(fmaf(__uint_as_float(v[c][k]), sl, lut[max(-far, min(far, r0 + c * 32 + k)) + far]));
+              v[c][k] = __float_as_uint(fmaf(__uint_as_float(v[c][k]), sl, lut[max(-far, min(far, rel0 + c * 32 + k)) + far]));
         }
       }
-      if (j0 < full0 || j0 + KEYS > full1) {
+      const bool cut = j0 < full0 || j0 + KEYS > full1;
+      if (cut) {
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
@@ -362,63 +442,82 @@ __global__ void __launch_bounds__(THREADS, 1)
             if (j < lo || j >= hi) v[c][k] = 0xff800000u;
           }
       }
-      float tops[8];
+      float tops[4];
 #pragma unroll
-      for (int k = 0; k < 8; ++k) tops[k] = -INFINITY;
+      for (int c = 0; c < 4; ++c) {
+        tops[c] = __uint_as_float(v[c][0]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int k = 0; k < 32; ++k) tops[k & 7] = fmaxf(tops[k & 7], __uint_as_float(v[c][k]));
-      const float top = mul * fmaxf(fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3])), fmaxf(fmaxf(tops[4], tops[5]), fmaxf(tops[6], tops[7])));
+        for (int k = 1; k < 31; k += 2) tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(v[c][k])), __uint_as_float(v[c][k + 1]));
+        tops[c] = fmaxf(tops[c], __uint_as_float(v[c][31]));
+      }
+      const float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      if (n > 0) warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest, P used up
       if (__any_sync(0xffffffffu, top > m + LAZY)) {
         const float grown = fmaxf(m, top);
         const float fix = ex2(m - (grown == -INFINITY ? 0.f : grown));
         l *= fix;
         m = grown;
         if (n > 0) {
+          tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 32) {
-            uint32_t o[32];
-            tmem_ld32_issue(t_o + c, o);
-            tmem_wait(o);
+          for (int c = 0; c < DP; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(t_o + c, o);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix);
-            tmem_st32(t_o + c, o);
+            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix);
+            tmem_st16(t_o + c, o);
           }
         }
       }
       const float base = m == -INFINITY ? 0.f : m;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t mul2 = pack2(mul, mul), base2 = pack2(-base, -base);
+      uint64_t sum[2] = {0, 0};  // two zeros each
+      auto probabilities = [&](auto fma_pairs) {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        uint32_t p[16];
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          const float x = ex2(fmaf(__uint_as_float(v[c][2 * k]), mul, -base)), y = ex2(fmaf(__uint_as_float(v[c][2 * k + 1]), mul, -base));
-          sum[k & 3] += x + y;
-          p[k] = pack_bf16(x, y);
+          for (int k = 0; k < 16; ++k) {
+            const uint64_t z = fma2(pack2(__uint_as_float(v[c][2 * k]), __uint_as_float(v[c][2 * k + 1])), mul2, base2);
+            float x, y;
+            unpack2(z, x, y);
+            if ((k & 7) * decltype(fma_pairs)::value % 8 + decltype(fma_pairs)::value > 7) {
+              exp2_pair(pack2(floored(x), floored(y)), x, y);
+            } else {
+              x = ex2(x), y = ex2(y);
+            }
+            sum[k & 1] = add2(sum[k & 1], pack2(x, y));
+            p[k] = pack_bf16(x, y);
+          }
+          tmem_st16(t_p + c * 16, p);
+          if (c & 1) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[c >> 1]);
+          }
         }
-        tmem_st16(t_s + c * 16, p);
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[w]);
+      };
+      // a score of -inf (masked, or by the bias) has to give zero: by the unit itself
+      if (BIAS || cut) probabilities(std::integral_constant<int, 0>());
+      else probabilities(std::integral_constant<int, FMA_PAIRS>());
+      float s0, s1, s2, s3;
+      unpack2(sum[0], s0, s1);
+      unpack2(sum[1], s2, s3);
+      l += (s0 + s1) + (s2 + s3);
     }
-    const bool some = t1[w] > t0[w];
-    if (some) warp_wait(&o_full[w], 0, gave_up);
+    if (n_tiles > 0) warp_wait(o_done, (n_tiles - 1) & 1, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;
     __nv_bfloat16* row = out + ((b * a.queries + i) * a.heads + head) * dim;
     for (int c = 0; c < DP && c < dim; c += 32) {
       uint32_t o[32];
-      if (some) {
+      if (n_tiles > 0) {
         tmem_ld32_issue(t_o + c, o);
         tmem_wait(o);
       }
-      if (!some || !live) {
+      if (n_tiles == 0 || !live) {
 #pragma unroll
         for (int k = 0; k < 32; ++k) o[k] = 0;
       }
@@ -430,7 +529,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(F::TMEM));
   }
 }
 
@@ -438,20 +537,22 @@ __global__ void __launch_bounds__(THREADS, 1)
 // backward
 // ------------------------------------------------------------------------------------
 
+constexpr int BN = 64;  // tokens of a tile
+
 template <int DP>
 struct Bwd {
-  static constexpr int BN = DP == 64 ? 128 : 64;  // tokens of a tile
+  static constexpr int GROUPS = DP == 64 ? 1 : 2;  // warpgroups, which take tiles in turn
+  static constexpr int THREADS = 64 + 128 * GROUPS, STAGES = 3;
   static constexpr uint32_t X = ROWS * DP * 2, Y = BN * DP * 2;
-  // TMEM columns: S, dP, then P and dS (bf16), then the sums
-  static constexpr uint32_t T_DP = BN, T_P = 2 * BN, T_DS = 2 * BN + BN / 2, T_ACC = 3 * BN;
-  static constexpr int MOST = 3;  // ring stages at most
+  // TMEM: each warpgroup's S and dP (P and dS over them), then the sums
+  static constexpr uint32_t TMEM = DP == 64 ? 256 : 512, T_ACC = GROUPS * 2 * BN;
 };
 
 struct BwdIo {
-  const float *lse, *delta;
+  const float *lse, *delta;  // [batch x heads][padded]: log2 (infinite where nothing is seen), and dout . out
+  int padded, stages, vec;
   __nv_bfloat16 *d0, *d1;  // dq; or dv and dk
   float* part;             // dq with a table: [batch][heads][row tiles][buckets]
-  int stages, vec;
 };
 
 // the diagonal sums of a 32 x 32 piece (lane = row, x = its columns): lane l gets the sum over column - row = l - 31, and
@@ -469,40 +570,43 @@ __device__ __forceinline__ void diagonals(const float (&x)[32], int lane, float&
 }
 
 template <int DP, bool DKV, bool BIAS>
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     backward_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CUtensorMap map_y0,
-                    const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ b200_attention a, const __grid_constant__ BwdIo io) {
+                    const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ b200_attention a, const __grid_constant__ Order order,
+                    const __grid_constant__ BwdIo io) {
   using G = Bwd<DP>;
-  constexpr int BN = G::BN, HALF = BN / 2;
+  constexpr int WG = G::GROUPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const int ST = io.stages;
   const uint32_t s_x = smem_u32(smem), s_y = s_x + 2 * G::X;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + 2 * G::X + ST * 2 * G::Y);
-  uint64_t *x_full = bars, *y_full = bars + 1, *y_empty = y_full + G::MOST, *st_full = y_empty + G::MOST, *sp_full = st_full + G::MOST, *sp_free = sp_full + 1,
-           *pd_full = sp_full + 2, *pd_free = sp_full + 3, *acc_full = sp_full + 4, *idle = sp_full + 5;
+  uint64_t *x_full = bars, *y_full = bars + 1, *y_empty = y_full + G::STAGES, *sp_full = y_empty + G::STAGES, *pd_full = sp_full + 2, *acc_full = pd_full + 2,
+           *idle = acc_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* s_stat = reinterpret_cast<float*>(bars + 32);           // DKV: [stages][lse, delta][BN]
-  float* lut = s_stat + (DKV ? G::MOST * 2 * BN : 0);            // BIAS: [2 far + 1]
-  float* near = lut + (BIAS ? 2 * relative::far_of(a.relative) + 1 : 0);  // dq with BIAS: [8 warps][2 far + 1]
+  float* lut0 = s_stat + (DKV ? G::STAGES * 2 * BN : 0);         // BIAS: [2 far + 1], for dk and dv one a warpgroup
+  const int far = BIAS ? relative::far_of(a.relative) : 0, bins = 2 * far + 1;
+  float* near = lut0 + bins;                                     // dq with BIAS: [4 warps x warpgroups][2 far + 1]
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const Place at(order);
   const int group = (int)(a.heads / a.kv_heads), dim = (int)a.dim;
-  const int hy = blockIdx.y, kvh = DKV ? hy : hy / group;
-  const int64_t b = blockIdx.z;
+  const int hy = at.head, kvh = DKV ? hy : hy / group;
+  const int64_t b = at.batch;
   const Sequence seq(a, b);
-  // causal blocks with the most tiles start first
-  const int rt = !DKV && a.causal ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
-  const int r0 = rt * ROWS, row_end = DKV ? seq.keys : seq.queries, r1 = min(r0 + ROWS, row_end) - 1;
+  const int rt = at.tile, r0 = rt * ROWS, row_end = DKV ? seq.keys : seq.queries;
   int first = 0, per = 0;  // tiles of one head
-  if (r1 >= r0) {
-    const int lo = DKV ? seq.first_query(a, r0) : seq.first_key(a, r0), hi = DKV ? seq.end_query(a, r1) : seq.end_key(a, r1);
-    if (hi > lo) first = lo / BN, per = (hi + BN - 1) / BN - first;
+  {
+    const int r1 = min(r0 + ROWS, row_end) - 1;
+    if (r1 >= r0) {
+      const int lo = DKV ? seq.first_query(a, r0) : seq.first_key(a, r0), hi = DKV ? seq.end_query(a, r1) : seq.end_key(a, r1);
+      if (hi > lo) first = lo / BN, per = (hi + BN - 1) / BN - first;
+    }
+    first = uniform(first), per = uniform(per);
   }
-  first = uniform(first), per = uniform(per);
   const int total = per * (DKV ? group : 1);
-  const int far = BIAS ? relative::far_of(a.relative) : 0, bins = 2 * far + 1;
   // tile n: its head and first token
   auto head_of = [&](int n) { return DKV ? kvh * group + n / per : hy; };
   auto token_of = [&](int n) { return (first + (DKV ? n % per : n)) * BN; };
@@ -515,23 +619,22 @@ __global__ void __launch_bounds__(THREADS, 1)
     for (int s = 0; s < ST; ++s) {
       mbar_init(&y_full[s], 1);
       mbar_init(&y_empty[s], 1);
-      mbar_init(&st_full[s], 1);
     }
-    mbar_init(sp_full, 1);
-    mbar_init(sp_free, 8);
-    mbar_init(pd_full, 8);
-    mbar_init(pd_free, 1);
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&sp_full[g], 1);
+      mbar_init(&pd_full[g], 4);
+    }
     mbar_init(acc_full, 1);
     mbar_init(idle, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512));
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(G::TMEM));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   if constexpr (BIAS && !DKV) {
-    fill_bias(lut, a, far, hy);
-    for (int i = threadIdx.x; i < 8 * bins; i += THREADS) near[i] = 0.f;
+    fill_bias(lut0, a, far, hy);
+    for (int i = threadIdx.x; i < 4 * WG * bins; i += G::THREADS) near[i] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -546,145 +649,127 @@ __global__ void __launch_bounds__(THREADS, 1)
         tma_load_4d(smem + p * (ROWS * 128), &map_x0, x_full, p * 64, r0, xh, (int)b);
         tma_load_4d(smem + G::X + p * (ROWS * 128), &map_x1, x_full, p * 64, r0, xh, (int)b);
       }
-      int n = 0;
-      for (; n < total; ++n) {
+      for (int n = 0; n < total; ++n) {
         const int s = n % ST;
         wait(&y_empty[s], ((n / ST) & 1) ^ 1, gave_up);
-        mbar_expect_tx(&y_full[s], 2 * G::Y);
+        mbar_expect_tx(&y_full[s], 2 * G::Y + (DKV ? 2 * BN * 4 : 0));
         const int yh = DKV ? head_of(n) : kvh;
         for (int p = 0; p < DP / 64; ++p) {
           uint8_t* y = smem + 2 * G::X + s * 2 * G::Y + p * (BN * 128);
           tma_load_4d(y, &map_y0, &y_full[s], p * 64, token_of(n), yh, (int)b);
           tma_load_4d(y + G::Y, &map_y1, &y_full[s], p * 64, token_of(n), yh, (int)b);
         }
+        if constexpr (DKV) {  // 256 bytes each, on 256-byte boundaries; rows are padded to whole tiles
+          const int64_t from = (b * a.heads + yh) * io.padded + token_of(n);
+          bulk_load(s_stat + s * 2 * BN, io.lse + from, BN * 4, &y_full[s]);
+          bulk_load(s_stat + s * 2 * BN + BN, io.delta + from, BN * 4, &y_full[s]);
+        }
       }
       // every load has landed before the block may end
       wait(x_full, 0, gave_up);
-      for (int m = max(0, n - ST); m < n; ++m) wait(&y_full[m % ST], (m / ST) & 1, gave_up);
+      for (int m = max(0, total - ST); m < total; ++m) wait(&y_full[m % ST], (m / ST) & 1, gave_up);
     }
   } else if (warp == 1) {
     const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, BN, false), id_a = idesc_of(ROWS, ks * 16, true);
-    if (total > 0) warp_wait(x_full, 0, gave_up);
     const Desc x0 = desc_at(s_x, 16), x1 = desc_at(s_x + G::X, 16), yk = desc_at(s_y, 16), ymn = desc_at(s_y, BN * 128);
-    auto scores = [&](int n, int s, int par) {  // S and dP of tile n, in stage s
-      warp_wait(&y_full[s], par, gave_up);
-      const uint32_t y = s_y + s * 2 * G::Y;
+    int ls = 0, lpar = 0;  // stage and parity of the next tile whose scores are made
+    auto scores = [&](int n) {  // S and dP of tile n
+      warp_wait(&y_full[ls], lpar, gave_up);
       const int have = (DKV ? seq.queries : seq.keys) - token_of(n);
       if (have < BN && (DKV ? seq.queries < a.queries : seq.keys < a.keys)) {
         // what lies behind the sequence's end may be anything, and is multiplied by zeros in the sums
+        const uint32_t y = s_y + ls * 2 * G::Y;
         zero_rows<BN, DP>(y, max(have, 0), lane);
         zero_rows<BN, DP>(y + G::Y, max(have, 0), lane);
         fence_proxy_async_smem();
         __syncwarp();
       }
       tc_fence_after();
-      const Desc y0 = {yk.lo + s * (2 * G::Y >> 4), yk.hi}, y1 = {y0.lo + (G::Y >> 4), yk.hi};
+      const uint32_t t_s = tmem + (WG == 2 ? (n & 1) * 2 * BN : 0);
+      const Desc y0 = {yk.lo + ls * (2 * G::Y >> 4), yk.hi}, y1 = {y0.lo + (G::Y >> 4), yk.hi};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        if (k < ks) mma(elected, tmem, x0, off_k<ROWS>(k), y0, off_k<BN>(k), id_s, k > 0);
+        if (k < ks) mma(elected, t_s, x0, off_k<ROWS>(k), y0, off_k<BN>(k), id_s, k > 0);
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        if (k < ks) mma(elected, tmem + G::T_DP, x1, off_k<ROWS>(k), y1, off_k<BN>(k), id_s, k > 0);
-      commit(elected, sp_full);
+        if (k < ks) mma(elected, t_s + BN, x1, off_k<ROWS>(k), y1, off_k<BN>(k), id_s, k > 0);
+      commit(elected, &sp_full[WG == 2 ? n & 1 : 0]);
+      if (++ls == ST) ls = 0, lpar ^= 1;
     };
-    if (total > 0) scores(0, 0, 0);
-    for (int n = 0, s = 0, par = 0, next = 0; n < total; ++n, s = next) {
-      next = s + 1 == ST ? 0 : s + 1;
-      par ^= next == 0;
-      if (n + 1 < total) {
-        warp_wait(sp_free, n & 1, gave_up);
-        scores(n + 1, next, par);
-      }
-      warp_wait(pd_full, n & 1, gave_up);
+    if (total > 0) {
+      warp_wait(x_full, 0, gave_up);
+      for (int n = 0; n < WG && n < total; ++n) scores(n);
+    }
+    for (int n = 0, s = 0; n < total; ++n, s = s + 1 == ST ? 0 : s + 1) {
+      const int g = WG == 2 ? n & 1 : 0;
+      warp_wait(&pd_full[g], (n / WG) & 1, gave_up);
       tc_fence_after();
+      const uint32_t t_s = tmem + g * 2 * BN;
       const Desc y0 = {ymn.lo + s * (2 * G::Y >> 4), ymn.hi}, y1 = {y0.lo + (G::Y >> 4), ymn.hi};
       if constexpr (DKV) {
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)  // dV += P dO
-          mma_from_tmem(elected, tmem + G::T_ACC, tmem + G::T_P + k * 8, y1, off_mn(k), id_a, n > 0 || k > 0);
+          mma_from_tmem(elected, tmem + G::T_ACC, t_s + k * 8, y1, off_mn(k), id_a, n > 0 || k > 0);
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)  // dK += dS Q
-          mma_from_tmem(elected, tmem + G::T_ACC + DP, tmem + G::T_DS + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
+          mma_from_tmem(elected, tmem + G::T_ACC + DP, t_s + BN + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
       } else {
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)  // dQ += dS K
-          mma_from_tmem(elected, tmem + G::T_ACC, tmem + G::T_DS + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
+          mma_from_tmem(elected, tmem + G::T_ACC, t_s + BN + k * 8, y0, off_mn(k), id_a, n > 0 || k > 0);
       }
       commit(elected, &y_empty[s]);
-      commit(elected, pd_free);
       if (n + 1 == total) commit(elected, acc_full);
+      // behind the sums in the MMAs' order: their P and dS are used up when it overwrites them
+      if (n + WG < total) scores(n + WG);
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
     warp_wait(idle, 0, gave_up);
-  } else if (DKV && warp == 2) {
-    // the queries' lse (log2; infinite where nothing is to be had) and delta
-    for (int n = 0; n < total; ++n) {
-      const int s = n % ST;
-      warp_wait(&y_empty[s], ((n / ST) & 1) ^ 1, gave_up);
-      const int64_t at = (b * a.heads + head_of(n)) * a.queries;
-      for (int c = lane; c < BN; c += 32) {
-        const int i = token_of(n) + c;
-        float x = INFINITY, d = 0.f;
-        if (i < seq.queries) {
-          x = io.lse[at + i] * LOG2E;
-          if (x == -INFINITY) x = INFINITY;
-          d = io.delta[at + i];
-        }
-        s_stat[s * 2 * BN + c] = x;
-        s_stat[s * 2 * BN + BN + c] = d;
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&st_full[s]);
-    }
-  } else if (warp >= 4) {
-    const int g = (warp - 4) >> 2, q = warp & 3;
+  } else {
+    const int g = (warp - 2) >> 2, q = warp & 3;
     const int w0 = r0 + q * 32, r = w0 + lane;
     const bool valid = r < row_end;
     const int lo = !valid ? 0 : (DKV ? seq.first_query(a, r) : seq.first_key(a, r)), hi = !valid ? 0 : (DKV ? seq.end_query(a, r) : seq.end_key(a, r));
     // every token of [full0, full1) goes with all rows of the warp
     const int last = min(w0 + 31, row_end - 1);
     const int full0 = DKV ? seq.first_query(a, last) : seq.first_key(a, last), full1 = DKV ? seq.end_query(a, w0) : seq.end_key(a, w0);
-    const uint32_t lanes = (uint32_t)(q * 32) << 16, tm = tmem + lanes;
+    const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16), t_s = tm + g * 2 * BN;
     const float sl = a.scale * LOG2E;
+    const uint64_t sl2 = pack2(sl, sl);
     float row_lse = INFINITY, row_delta = 0.f, before = 0.f, after = 0.f;
     if (!DKV && valid) {
-      const int64_t at = (b * a.heads + hy) * a.queries + r;
-      row_lse = io.lse[at] * LOG2E;
-      if (row_lse == -INFINITY) row_lse = INFINITY;
-      row_delta = io.delta[at];
+      const int64_t from = (b * a.heads + hy) * io.padded + r;
+      row_lse = io.lse[from];
+      row_delta = io.delta[from];
     }
-    float* my_near = near + (warp - 4) * bins;
+    float* lut = lut0 + (DKV ? g * bins : 0);
+    float* my_near = near + (warp - 2) * bins;
     int lut_head = -1;
-    for (int n = 0; n < total; ++n) {
+    for (int n = g; n < total; n += WG) {
       if constexpr (BIAS && DKV) {
         // the lookup of the tile's head, by the threads that read it
         if (head_of(n) != lut_head) {
           lut_head = head_of(n);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          for (int i = threadIdx.x - 128; i < bins; i += 256)
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
+          for (int i = (q << 5) + lane; i < bins; i += 128)
             lut[i] = table_log2(a.table, (int64_t)relative::bucket_of(a.relative, i - far) * a.heads + lut_head, a.table_dtype);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
         }
       }
-      warp_wait(sp_full, n & 1, gave_up);
-      if constexpr (DKV) warp_wait(&st_full[n % ST], (n / ST) & 1, gave_up);
+      if constexpr (DKV) warp_wait(&y_full[n % ST], (n / ST) & 1, gave_up);  // lse and delta
+      warp_wait(&sp_full[g], (n / WG) & 1, gave_up);
       tc_fence_after();
-      const float* stat = s_stat + (n % ST) * 2 * BN + g * HALF;
+      const float* stat = s_stat + (n % ST) * 2 * BN;
 #pragma unroll
-      for (int c0 = 0; c0 < HALF; c0 += 32) {
-        const int t0 = token_of(n) + g * HALF + c0;  // first token of these columns
+      for (int c0 = 0; c0 < BN; c0 += 32) {
+        const int t0 = token_of(n) + c0;  // first token of these columns
         uint32_t s[32], d[32];
-        tmem_ld32_issue(tm + g * HALF + c0, s);
-        tmem_ld32_issue(tm + G::T_DP + g * HALF + c0, d);
+        tmem_ld32_issue(t_s + c0, s);
+        tmem_ld32_issue(t_s + BN + c0, d);
         tmem_wait(s);
         tmem_wait(d);
-        if (c0 + 32 == HALF) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(sp_free);
-        }
         float x[32];
         int w_rel = 0;  // key - query - shift of lane 0, column 0; + 1 a column for dq, - 1 for dk and dv
         bool is_near = false;
@@ -730,6 +815,15 @@ __global__ void __launch_bounds__(THREADS, 1)
               s[k] = 0;
             }
         }
+        uint32_t p[16];
+        if constexpr (DKV) {
+#pragma unroll
+          for (int k = 0; k < 16; ++k) p[k] = pack_bf16(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
+          tmem_st16(t_s + c0 / 2, p);
+        }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) p[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
+        tmem_st16(t_s + BN + c0 / 2, p);
         if constexpr (BIAS && !DKV) {
           if (!valid) {
 #pragma unroll
@@ -757,45 +851,34 @@ __global__ void __launch_bounds__(THREADS, 1)
             else before += sum;
           }
         }
-        if (c0 == 0 && n > 0) {
-          // the sums of the tile before have read P and dS
-          warp_wait(pd_free, (n - 1) & 1, gave_up);
-          tc_fence_after();
-        }
-        uint32_t p[16];
-        if constexpr (DKV) {
-#pragma unroll
-          for (int k = 0; k < 16; ++k) p[k] = pack_bf16(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1]));
-          tmem_st16(tm + G::T_P + (g * HALF + c0) / 2, p);
-        }
-#pragma unroll
-        for (int k = 0; k < 16; ++k) p[k] = pack_bf16(x[2 * k], x[2 * k + 1]);
-        tmem_st16(tm + G::T_DS + (g * HALF + c0) / 2, p);
       }
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(pd_full);
+      if (lane == 0) mbar_arrive(&pd_full[g]);
     }
-    const bool some = total > 0;
-    if (some) warp_wait(acc_full, 0, gave_up);
+    if (total > 0) warp_wait(acc_full, 0, gave_up);
     tc_fence_after();
     const int rows = DKV ? (int)a.keys : (int)a.queries, heads = DKV ? (int)a.kv_heads : (int)a.heads;
-    // dk, dv: a warpgroup each; dq: half of the columns each
-    const int from = DKV ? 0 : g * (DP / 2), to = DKV ? DP : from + DP / 2;
-    const uint32_t acc = tm + G::T_ACC + (DKV ? g * DP : 0);
-    __nv_bfloat16* row = (DKV && g ? io.d1 : io.d0) + ((b * rows + r) * heads + hy) * dim;
-    for (int c = from; c < to && c < dim; c += 32) {
-      uint32_t o[32];
-      if (some) {
-        tmem_ld32_issue(acc + c, o);
-        tmem_wait(o);
-      }
-      if (!some || !valid) {
+    // two warpgroups: dv and dk, or half of dq's columns, each
 #pragma unroll
-        for (int k = 0; k < 32; ++k) o[k] = 0;
+    for (int o0 = 0; o0 < (DKV ? 2 : 1); ++o0) {
+      if (DKV && WG == 2 && o0 != g) continue;
+      const int from = !DKV && WG == 2 ? g * (DP / 2) : 0, to = !DKV && WG == 2 ? from + DP / 2 : DP;
+      const uint32_t acc = tm + G::T_ACC + o0 * DP;
+      __nv_bfloat16* row = (o0 ? io.d1 : io.d0) + ((b * rows + r) * heads + hy) * dim;
+      for (int c = from; c < to && c < dim; c += 32) {
+        uint32_t o[32];
+        if (total > 0) {
+          tmem_ld32_issue(acc + c, o);
+          tmem_wait(o);
+        }
+        if (total == 0 || !valid) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = 0;
+        }
+        if (r < rows) store32(row, c, dim, io.vec, o, DKV && !o0 ? 1.f : a.scale);
       }
-      if (r < rows) store32(row, c, dim, io.vec, o, DKV && !g ? 1.f : a.scale);
     }
     if constexpr (BIAS && !DKV) {
       before = warp_sum(before), after = warp_sum(after);
@@ -806,20 +889,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512));
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(G::TMEM));
   }
   if constexpr (BIAS && !DKV) {
-    // the warps' sums by rel to buckets, in order
-    const int nb = relative::buckets_of(a.relative);
-    float* part = io.part + (((int64_t)b * gridDim.y + hy) * gridDim.x + rt) * nb;
-    for (int n = threadIdx.x; n < nb; n += THREADS) {
+    // the warps' sums by rel, then to buckets, in order
+    for (int i = threadIdx.x; i < bins; i += G::THREADS) {
       float s = 0.f;
-      for (int i = 0; i < bins; ++i)
-        if (relative::bucket_of(a.relative, i - far) == n)
 #pragma unroll
-          for (int w = 0; w < 8; ++w) s += near[w * bins + i];
-      part[n] = s;
+      for (int w = 0; w < 4 * WG; ++w) s += near[w * bins + i];
+      lut0[i] = s;
     }
+    __syncthreads();
+    const int nb = relative::buckets_of(a.relative);
+    float* part = io.part + ((b * a.heads + hy) * order.row_tiles + rt) * nb;
+    for (int n = threadIdx.x; n < nb; n += G::THREADS) part[n] = relative::bucket_sum(a.relative, far, lut0, n);
   }
 }
 
@@ -888,15 +971,26 @@ static int allow(Kernel k) {
   return cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM_LIMIT) == cudaSuccess ? B200_OK : check_launch("attention");
 }
 
+// `heads` of rows, row tiles of them; `bytes`: the tokens that go past a head's rows
+static int order_of(Order* o, const b200_attention& a, int64_t heads, int64_t rows, int64_t bytes, bool last_first) {
+  const int64_t tiles = ceil_div(rows, ROWS), pairs = a.batch * heads;
+  B200_REQUIRE(tiles * pairs < (1ll << 31), "attention: %lld rows of %lld heads are too many", (long long)rows, (long long)pairs);
+  // causal: 32 MB of them at a time, a quarter of the L2
+  const int64_t group = a.causal ? std::max<int64_t>(1, (32ll << 20) / std::max<int64_t>(1, bytes)) : 1;
+  *o = {(int)tiles, (int)heads, (int)pairs, (int)std::min(group, pairs), a.causal && last_first};
+  return B200_OK;
+}
+
 template <int DP, bool BIAS>
 static int launch_forward(const b200_attention& a, const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, void* out, float* lse,
                           cudaStream_t st) {
+  Order order;
+  if (int rc = order_of(&order, a, a.heads, a.queries, a.keys * a.dim * 4 * a.kv_heads / a.heads, true)) return rc;
   const size_t shared = 1024 + Fwd<DP>::LUT + bias_bytes(a, 1);
   const auto kernel = forward_kernel<DP, BIAS>;
   if (int rc = allow(kernel)) return rc;
   const int vec = a.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  kernel<<<dim3((unsigned)ceil_div(a.queries, 2 * ROWS), (unsigned)a.heads, (unsigned)a.batch), THREADS, shared, st>>>(
-      q, k, v, a, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
+  kernel<<<(unsigned)(order.row_tiles * order.pairs), FWD_THREADS, shared, st>>>(q, k, v, a, order, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
   return check_launch("attention");
 }
 
@@ -906,17 +1000,21 @@ static int launch_backward(const b200_attention& a, const Operand (&x)[2], const
   CUtensorMap m[4];
   for (int i = 0; i < 2; ++i) {
     if (int rc = map_of(&m[i], a, x[i], ROWS)) return rc;
-    if (int rc = map_of(&m[2 + i], a, y[i], G::BN)) return rc;
+    if (int rc = map_of(&m[2 + i], a, y[i], BN)) return rc;
   }
+  Order order;
+  const int64_t token = a.dim * 4;
+  if (int rc = DKV ? order_of(&order, a, a.kv_heads, a.keys, a.queries * token * a.heads / a.kv_heads, false)
+                   : order_of(&order, a, a.heads, a.queries, a.keys * token * a.kv_heads / a.heads, true))
+    return rc;
   auto shared = [&](int stages) {
-    return 1024 + 2 * (size_t)G::X + stages * 2 * (size_t)G::Y + 256 + (DKV ? G::MOST * 2 * G::BN * 4 : 0) + bias_bytes(a, DKV ? 1 : 9);
+    return 1024 + 2 * (size_t)G::X + stages * 2 * (size_t)G::Y + 256 + (DKV ? G::STAGES * 2 * BN * 4 : 0) +
+           bias_bytes(a, DKV ? G::GROUPS : 1 + 4 * G::GROUPS);
   };
-  io.stages = shared(G::MOST) <= SMEM_LIMIT ? G::MOST : 2;
+  io.stages = shared(G::STAGES) <= SMEM_LIMIT ? G::STAGES : 2;
   const auto kernel = backward_kernel<DP, DKV, BIAS>;
   if (int rc = allow(kernel)) return rc;
-  const int64_t rows = DKV ? a.keys : a.queries;
-  kernel<<<dim3((unsigned)ceil_div(rows, ROWS), (unsigned)(DKV ? a.kv_heads : a.heads), (unsigned)a.batch), THREADS, shared(io.stages), st>>>(
-      m[0], m[1], m[2], m[3], a, io);
+  kernel<<<(unsigned)(order.row_tiles * order.pairs), G::THREADS, shared(io.stages), st>>>(m[0], m[1], m[2], m[3], a, order, io);
   return check_launch("attention_grad");
 }
 
@@ -954,11 +1052,12 @@ size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads*
   return part_bytes(a) + tiles_forward_workspace(a) + d;
 }
 
-int tiles_grad(const b200_attention& a, const b200_attention_grads& g, const float* delta, void* workspace, cudaStream_t st) {
+int tiles_grad(const b200_attention& a, const b200_attention_grads& g, const float* lse2, const float* delta, int64_t padded, void* workspace,
+               cudaStream_t st) {
   using namespace tiles;
   uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
   BwdIo io = {};
-  io.lse = g.lse, io.delta = delta, io.part = reinterpret_cast<float*>(ws);
+  io.lse = lse2, io.delta = delta, io.padded = (int)padded, io.part = reinterpret_cast<float*>(ws);
   ws += part_bytes(a);
   Operand q = queries_of(a), k = keys_of(a), v = values_of(a), d = operand(g.dout, a.queries, a.heads, g.dout_stride);
   for (Operand* x : {&q, &k, &v, &d})

@@ -24,6 +24,21 @@ __device__ __forceinline__ int bucket_of(const b200_relative& r, int rel) {
   return lo + (r.bidirectional && rel > 0 ? r.side : 0);
 }
 
+// the sum of a bucket's positions from the sums by rel (rel + far; the ends hold all beyond them): neighbours on each side, in order
+__device__ __forceinline__ float bucket_sum(const b200_relative& r, int far, const float* by_rel, int bucket) {
+  const int side = bucket % r.side;
+  const int lo = r.start[side], hi = side + 1 < r.side ? r.start[side + 1] : far + 1;  // distances lo .. hi - 1
+  float s = 0.f;
+  if (r.bidirectional && bucket >= r.side) {
+    for (int n = max(lo, 1); n < hi; ++n) s += by_rel[far + n];
+    return s;
+  }
+  for (int n = lo; n < hi; ++n) s += by_rel[far - n];
+  if (!r.bidirectional && lo == 0 && hi > 0)
+    for (int n = 1; n <= far; ++n) s += by_rel[far + n];  // later keys share the first bucket
+  return s;
+}
+
 inline int check(const char* what, const b200_relative* r) {
   B200_REQUIRE(r, "%s: no buckets", what);
   B200_REQUIRE(r->side >= 1 && r->side <= B200_RELATIVE_MAX_SIDE, "%s: %d buckets a side (1 to %d)", what, r->side, B200_RELATIVE_MAX_SIDE);

@@ -129,21 +129,9 @@ __global__ void __launch_bounds__(THREADS) bias_grad_kernel(const __grid_constan
     near[threadIdx.x ? 2 * far : 0] = s;
   }
   __syncthreads();
-  // a bucket's diagonals are neighbours on each side: its thread adds them in order
   const int nb = buckets_of(r);
-  for (int b = threadIdx.x; b < nb; b += THREADS) {
-    const int side = b % r.side;
-    const int lo = r.start[side], hi = side + 1 < r.side ? r.start[side + 1] : far + 1;  // distances lo .. hi - 1
-    float s = 0.f;
-    if (r.bidirectional) {
-      if (b < r.side) for (int n = lo; n < hi; ++n) s += near[far - n];
-      else for (int n = max(lo, 1); n < hi; ++n) s += near[far + n];
-    } else {
-      for (int n = lo; n < hi; ++n) s += near[far - n];
-      if (lo == 0 && hi > 0) for (int n = 1; n <= far; ++n) s += near[far + n];  // later keys share the first bucket
-    }
-    part[(((int64_t)h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * nb + b] = s;
-  }
+  for (int b = threadIdx.x; b < nb; b += THREADS)
+    part[(((int64_t)h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * nb + b] = bucket_sum(r, far, near, b);
 }
 
 template <typename T>
