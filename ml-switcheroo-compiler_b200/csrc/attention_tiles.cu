@@ -4,13 +4,12 @@
 // exponentials run under the other's MMAs, and its start and end under the other's middle:
 //   warp 0      TMA: the queries once, then K and V tiles into a ring;
 //   warp 1      owns 256 columns of TMEM, issues S = Q K^T (operands in shared memory) and O += P V (P from TMEM);
-//   warps 2-5   softmax: a thread owns a query's row of S.
+//   warps 2-9   softmax: two threads own a query's row of S, 64 keys each, and exchange its maximum.
 // Heads of up to 64: S, P and O have columns of their own (128 + 64 + 64), and the next S is made as soon as the threads hold this
 // one in registers. Wider heads: P lies over S (O has 128), whose MMAs, issued behind O's, overwrite it only when it is used up: MMAs
 // run in their order. The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8,
 // sums are fp32), so O is hardly ever rescaled. P is handed over in two halves of 64 keys.
-// The special function unit makes 16 exponentials a clock: 1024 clocks a tile, of which the MMAs take 512 (heads of 64). A part of
-// them is therefore made on the FMA pipe (exp2_pair).
+// Making up to 3 of 8 exponentials on the FMA pipe changed nothing (the special function unit is busy for a third of the time): not done.
 //
 // Backward, one kernel in two forms. 128 rows stay, tiles of 64 tokens of the other side go past:
 //   dq:      rows are queries (Q, dO), tiles are keys (K, V):     S = Q K^T, dP = dO V^T, dQ += dS K
@@ -25,7 +24,6 @@
 // all accumulators are fp32. Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
 // block winds down.
 #include <algorithm>
-#include <type_traits>
 
 #include "attention.cuh"
 #include "tc_common.cuh"
@@ -75,7 +73,7 @@ __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* gave_u
     }
   }
 }
-// by all lanes, together again behind it
+// by all lanes, together again behind it (61 clocks where it is satisfied; one polling lane and the others' wait for it 136)
 __device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
   wait(bar, parity, gave_up);
   __syncwarp();
@@ -192,26 +190,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-// 2^x of two values on the FMA pipe, -125 < x < 127: x = n + f with n whole (adding 1.5 2^23 rounds it there and leaves n in the low bits), 2^f by
-// a polynomial of degree 4 fitted to the least relative error over [-1/2, 1/2] (2.7e-6 with fp32's rounding; a probability's
-// rounding to bf16 is 2e-3), n added to the exponent.
-__device__ __forceinline__ void exp2_pair(uint64_t x, float& a, float& b) {
-  const float big = 12582912.f;
-  const uint64_t t = add2(x, pack2(big, big));
-  const uint64_t n = add2(t, pack2(-big, -big));
-  const uint64_t f = fma2(n, pack2(-1.f, -1.f), x);
-  uint64_t p = pack2(0.009570102207362652f, 0.009570102207362652f);
-  p = fma2(p, f, pack2(0.05591786280274391f, 0.05591786280274391f));
-  p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
-  p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  float t0, t1;
-  unpack2(t, t0, t1);
-  unpack2(p, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(t0) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(t1) << 23));
-}
-
 // 32 fp32 columns of a row, scaled, to a row of the result from column `col` on
 __device__ __forceinline__ void store32(__nv_bfloat16* row, int col, int dim, bool vec, const uint32_t (&v)[32], float f) {
   if (vec) {
@@ -236,16 +214,8 @@ __device__ __forceinline__ void store32(__nv_bfloat16* row, int col, int dim, bo
 // forward
 // ------------------------------------------------------------------------------------
 
-constexpr int KEYS = 128, FWD_THREADS = 192;
+constexpr int KEYS = 128, FWD_THREADS = 320;
 constexpr float LAZY = 8.f;  // log2 by which a maximum may grow before O is rescaled
-constexpr float FLOOR = -124.f;  // what exp2_pair takes
-__device__ __forceinline__ float floored(float x) {  // a score that is no number stays none
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(x), "f"(FLOOR));
-  return r;
-}
-// of 8 pairs of exponentials, those made on the FMA pipe
-constexpr int FMA_PAIRS = 3;
 
 template <int DP>
 struct Fwd {
@@ -253,7 +223,7 @@ struct Fwd {
   static constexpr int STAGES = DP == 64 ? 2 : 1;
   static constexpr uint32_t TILE = 128 * DP * 2;
   static constexpr uint32_t BARS = TILE + STAGES * 2 * TILE;
-  static constexpr uint32_t LUT = BARS + 256;
+  static constexpr uint32_t MAXIMA = BARS + 256, LUT = MAXIMA + 2 * 2 * ROWS * 4;
   static constexpr uint32_t TMEM = 256, T_P = APART ? 128 : 0, T_O = TMEM - DP;
 };
 
@@ -271,6 +241,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
            *s_free = s_full + 1, *p_full = s_full + 2, *o_done = s_full + 4, *idle = s_full + 5;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
+  float* maxima = reinterpret_cast<float*>(smem + F::MAXIMA);  // [parity][half][row]
   float* lut = reinterpret_cast<float*>(smem + F::LUT);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -301,7 +272,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 4);
+    mbar_init(s_free, 8);
     mbar_init(&p_full[0], 4);
     mbar_init(&p_full[1], 4);
     mbar_init(o_done, 1);
@@ -390,26 +361,33 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     commit(elected, idle);
     warp_wait(idle, 0, gave_up);
   } else {
-    const int q = warp & 3;
-    const int i0 = r0 + q * 32, i = i0 + lane;
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int i0 = r0 + q * 32, i = i0 + lane, row_at = q * 32 + lane;
     const bool valid = i < seq.queries;
     const int lo = valid ? seq.first_key(a, i) : 0, hi = valid ? seq.end_key(a, i) : 0;
     // every key of [full0, full1) is seen by all rows of the warp
     const int full0 = seq.first_key(a, min(i0 + 31, seq.queries - 1)), full1 = seq.end_key(a, i0);
-    const uint32_t t_s = tmem + ((uint32_t)(q * 32) << 16), t_p = t_s + F::T_P, t_o = t_s + F::T_O;
+    const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16), t_s = t_row + half * 64, t_p = t_row + F::T_P + half * 32, t_o = t_row + F::T_O;
     const float sl = a.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;  // the row's maximum, the sum of this thread's keys
+    // this thread's value and that of the row's other thread, which meet at a barrier of their two warps
+    auto exchange = [&](float x, int parity) {
+      float* area = maxima + parity * 2 * ROWS;
+      area[half * ROWS + row_at] = x;
+      asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
+      return area[(half ^ 1) * ROWS + row_at];
+    };
     for (int n = 0; n < n_tiles; ++n) {
-      const int j0 = (T0 + n) * KEYS;
+      const int j0 = (T0 + n) * KEYS + half * 64;
       warp_wait(s_full, n & 1, gave_up);
       tc_fence_after();
-      uint32_t v[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32_issue(t_s + c * 32, v[c]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait(v[c]);
+      uint32_t v[2][32];
+      tmem_ld32_issue(t_s, v[0]);
+      tmem_ld32_issue(t_s + 32, v[1]);
+      tmem_wait(v[0]);
+      tmem_wait(v[1]);
+      tc_fence_before();
       if constexpr (F::APART) {
-        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
       }
@@ -418,24 +396,24 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         mul = 1.f;
         const int rel0 = j0 - i - seq.shift;   // of column 0
         const int w_rel = j0 - i0 - seq.shift;  // of lane 0
-        if (w_rel - 31 >= far || w_rel + KEYS - 1 <= -far) {
+        if (w_rel - 31 >= far || w_rel + 63 <= -far) {
           const float c0 = lut[w_rel >= far ? 2 * far : 0];
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int k = 0; k < 32; ++k) v[c][k] = __float_as_uint(fmaf(__uint_as_float(v[c][k]), sl, c0));
         } else {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c)
 #pragma unroll
             for (int k = 0; k < 32; ++k)
               v[c][k] = __float_as_uint(fmaf(__uint_as_float(v[c][k]), sl, lut[max(-far, min(far, rel0 + c * 32 + k)) + far]));
         }
       }
-      const bool cut = j0 < full0 || j0 + KEYS > full1;
+      const bool cut = j0 < full0 || j0 + 64 > full1;
       if (cut) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int k = 0; k < 32; ++k) {
             const int j = j0 + c * 32 + k;
@@ -445,20 +423,40 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       float tops[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        tops[c] = __uint_as_float(v[c][0]);
+        tops[c] = __uint_as_float(v[c >> 1][16 * (c & 1)]);
 #pragma unroll
-        for (int k = 1; k < 31; k += 2) tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(v[c][k])), __uint_as_float(v[c][k + 1]));
-        tops[c] = fmaxf(tops[c], __uint_as_float(v[c][31]));
+        for (int k = 1; k < 15; k += 2)
+          tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(v[c >> 1][16 * (c & 1) + k])), __uint_as_float(v[c >> 1][16 * (c & 1) + k + 1]));
+        tops[c] = fmaxf(tops[c], __uint_as_float(v[c >> 1][16 * (c & 1) + 15]));
       }
-      const float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      if (n > 0) warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest, P used up
-      if (__any_sync(0xffffffffu, top > m + LAZY)) {
+      float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      // behind this barrier both threads hold their scores: P may be written over them
+      top = fmaxf(top, exchange(top, n & 1));
+      float fix = 1.f;
+      const bool moved = __any_sync(0xffffffffu, top > m + LAZY);  // the same in both warps
+      if (moved) {
         const float grown = fmaxf(m, top);
-        const float fix = ex2(m - (grown == -INFINITY ? 0.f : grown));
+        fix = ex2(m - (grown == -INFINITY ? 0.f : grown));
         l *= fix;
         m = grown;
-        if (n > 0) {
-          tc_fence_after();
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      const uint64_t mul2 = pack2(mul, mul), base2 = pack2(-base, -base);
+      uint64_t sum[2] = {0, 0};  // two zeros each
+      uint32_t p[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {
+        const int c = k >> 4, e = 2 * (k & 15);
+        float x, y;
+        unpack2(fma2(pack2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), mul2, base2), x, y);
+        x = ex2(x), y = ex2(y);
+        sum[k & 1] = add2(sum[k & 1], pack2(x, y));
+        p[k] = pack_bf16(x, y);
+      }
+      if (n > 0) {
+        warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest, P used up: under the exponentials
+        tc_fence_after();
+        if (moved && half == 0) {  // ahead of this half's P, so ahead of the first product
 #pragma unroll 1
           for (int c = 0; c < DP; c += 16) {
             uint32_t o[16];
@@ -469,49 +467,23 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
           }
         }
       }
-      const float base = m == -INFINITY ? 0.f : m;
-      const uint64_t mul2 = pack2(mul, mul), base2 = pack2(-base, -base);
-      uint64_t sum[2] = {0, 0};  // two zeros each
-      auto probabilities = [&](auto fma_pairs) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
-#pragma unroll
-          for (int k = 0; k < 16; ++k) {
-            const uint64_t z = fma2(pack2(__uint_as_float(v[c][2 * k]), __uint_as_float(v[c][2 * k + 1])), mul2, base2);
-            float x, y;
-            unpack2(z, x, y);
-            if ((k & 7) * decltype(fma_pairs)::value % 8 + decltype(fma_pairs)::value > 7) {
-              exp2_pair(pack2(floored(x), floored(y)), x, y);
-            } else {
-              x = ex2(x), y = ex2(y);
-            }
-            sum[k & 1] = add2(sum[k & 1], pack2(x, y));
-            p[k] = pack_bf16(x, y);
-          }
-          tmem_st16(t_p + c * 16, p);
-          if (c & 1) {
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[c >> 1]);
-          }
-        }
-      };
-      // a score of -inf (masked, or by the bias) has to give zero: by the unit itself
-      if (BIAS || cut) probabilities(std::integral_constant<int, 0>());
-      else probabilities(std::integral_constant<int, FMA_PAIRS>());
+      tmem_st32(t_p, p);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[half]);
       float s0, s1, s2, s3;
       unpack2(sum[0], s0, s1);
       unpack2(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
     }
+    l += exchange(l, n_tiles & 1);
     if (n_tiles > 0) warp_wait(o_done, (n_tiles - 1) & 1, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;
     __nv_bfloat16* row = out + ((b * a.queries + i) * a.heads + head) * dim;
-    for (int c = 0; c < DP && c < dim; c += 32) {
+    for (int c = half * (DP / 2); c < (half + 1) * (DP / 2) && c < dim; c += 32) {
       uint32_t o[32];
       if (n_tiles > 0) {
         tmem_ld32_issue(t_o + c, o);
@@ -523,7 +495,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       }
       if (i < a.queries) store32(row, c, dim, vec, o, inv);
     }
-    if (i < a.queries) lse[(b * a.heads + head) * a.queries + i] = live ? (m + log2f(l)) * LN2 : -INFINITY;
+    if (half == 0 && i < a.queries) lse[(b * a.heads + head) * a.queries + i] = live ? (m + log2f(l)) * LN2 : -INFINITY;
   }
   tc_fence_before();
   __syncthreads();
@@ -539,10 +511,12 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
 
 constexpr int BN = 64;  // tokens of a tile
 
-template <int DP>
+template <int DP, bool DKV, bool BIAS>
 struct Bwd {
-  static constexpr int GROUPS = DP == 64 ? 1 : 2;  // warpgroups, which take tiles in turn
-  static constexpr int THREADS = 64 + 128 * GROUPS, STAGES = 3;
+  // pairs of warpgroups, which take tiles in turn (32 columns of a tile a warpgroup); dq's sums by diagonal, a set a warp, leave
+  // room for one
+  static constexpr int GROUPS = DP == 64 || (BIAS && !DKV) ? 1 : 2;
+  static constexpr int THREADS = 64 + 256 * GROUPS, STAGES = 3;
   static constexpr uint32_t X = ROWS * DP * 2, Y = BN * DP * 2;
   // TMEM: each warpgroup's S and dP (P and dS over them), then the sums
   static constexpr uint32_t TMEM = DP == 64 ? 256 : 512, T_ACC = GROUPS * 2 * BN;
@@ -570,11 +544,11 @@ __device__ __forceinline__ void diagonals(const float (&x)[32], int lane, float&
 }
 
 template <int DP, bool DKV, bool BIAS>
-__global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
+__global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
     backward_kernel(const __grid_constant__ CUtensorMap map_x0, const __grid_constant__ CUtensorMap map_x1, const __grid_constant__ CUtensorMap map_y0,
                     const __grid_constant__ CUtensorMap map_y1, const __grid_constant__ b200_attention a, const __grid_constant__ Order order,
                     const __grid_constant__ BwdIo io) {
-  using G = Bwd<DP>;
+  using G = Bwd<DP, DKV, BIAS>;
   constexpr int WG = G::GROUPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -586,9 +560,9 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* s_stat = reinterpret_cast<float*>(bars + 32);           // DKV: [stages][lse, delta][BN]
-  float* lut0 = s_stat + (DKV ? G::STAGES * 2 * BN : 0);         // BIAS: [2 far + 1], for dk and dv one a warpgroup
+  float* lut0 = s_stat + (DKV ? G::STAGES * 2 * BN : 0);         // BIAS: [2 far + 1], for dk and dv one a pair of warpgroups
   const int far = BIAS ? relative::far_of(a.relative) : 0, bins = 2 * far + 1;
-  float* near = lut0 + bins;                                     // dq with BIAS: [4 warps x warpgroups][2 far + 1]
+  float* near = lut0 + bins;                                     // dq with BIAS: [warps][2 far + 1]
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const Place at(order);
@@ -607,9 +581,16 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     first = uniform(first), per = uniform(per);
   }
   const int total = per * (DKV ? group : 1);
-  // tile n: its head and first token
-  auto head_of = [&](int n) { return DKV ? kvh * group + n / per : hy; };
-  auto token_of = [&](int n) { return (first + (DKV ? n % per : n)) * BN; };
+  // a warp's way through the tiles: head and first token, ring stage and its parity, without divisions
+  struct Step {
+    int head, tile, stage, parity;
+  };
+  auto start = [&]() { return Step{DKV ? kvh * group : hy, 0, 0, 0}; };
+  auto advance = [&](Step& x) {
+    if (++x.stage == ST) x.stage = 0, x.parity ^= 1;
+    if (++x.tile == per && DKV) x.tile = 0, ++x.head;
+  };
+  auto token_of = [&](const Step& x) { return (first + x.tile) * BN; };
 
   if (threadIdx.x == 0) {
     *gave_up = 0;
@@ -622,7 +603,7 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&sp_full[g], 1);
-      mbar_init(&pd_full[g], 4);
+      mbar_init(&pd_full[g], 8);
     }
     mbar_init(acc_full, 1);
     mbar_init(idle, 1);
@@ -634,7 +615,7 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
   }
   if constexpr (BIAS && !DKV) {
     fill_bias(lut0, a, far, hy);
-    for (int i = threadIdx.x; i < 4 * WG * bins; i += G::THREADS) near[i] = 0.f;
+    for (int i = threadIdx.x; i < 8 * WG * bins; i += G::THREADS) near[i] = 0.f;
   }
   tc_fence_before();
   __syncthreads();
@@ -649,18 +630,18 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
         tma_load_4d(smem + p * (ROWS * 128), &map_x0, x_full, p * 64, r0, xh, (int)b);
         tma_load_4d(smem + G::X + p * (ROWS * 128), &map_x1, x_full, p * 64, r0, xh, (int)b);
       }
-      for (int n = 0; n < total; ++n) {
-        const int s = n % ST;
-        wait(&y_empty[s], ((n / ST) & 1) ^ 1, gave_up);
+      Step x = start();
+      for (int n = 0; n < total; ++n, advance(x)) {
+        const int s = x.stage, token = token_of(x), yh = DKV ? x.head : kvh;
+        wait(&y_empty[s], x.parity ^ 1, gave_up);
         mbar_expect_tx(&y_full[s], 2 * G::Y + (DKV ? 2 * BN * 4 : 0));
-        const int yh = DKV ? head_of(n) : kvh;
         for (int p = 0; p < DP / 64; ++p) {
           uint8_t* y = smem + 2 * G::X + s * 2 * G::Y + p * (BN * 128);
-          tma_load_4d(y, &map_y0, &y_full[s], p * 64, token_of(n), yh, (int)b);
-          tma_load_4d(y + G::Y, &map_y1, &y_full[s], p * 64, token_of(n), yh, (int)b);
+          tma_load_4d(y, &map_y0, &y_full[s], p * 64, token, yh, (int)b);
+          tma_load_4d(y + G::Y, &map_y1, &y_full[s], p * 64, token, yh, (int)b);
         }
         if constexpr (DKV) {  // 256 bytes each, on 256-byte boundaries; rows are padded to whole tiles
-          const int64_t from = (b * a.heads + yh) * io.padded + token_of(n);
+          const int64_t from = (b * a.heads + yh) * io.padded + token;
           bulk_load(s_stat + s * 2 * BN, io.lse + from, BN * 4, &y_full[s]);
           bulk_load(s_stat + s * 2 * BN + BN, io.delta + from, BN * 4, &y_full[s]);
         }
@@ -673,10 +654,11 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, BN, false), id_a = idesc_of(ROWS, ks * 16, true);
     const Desc x0 = desc_at(s_x, 16), x1 = desc_at(s_x + G::X, 16), yk = desc_at(s_y, 16), ymn = desc_at(s_y, BN * 128);
-    int ls = 0, lpar = 0;  // stage and parity of the next tile whose scores are made
-    auto scores = [&](int n) {  // S and dP of tile n
-      warp_wait(&y_full[ls], lpar, gave_up);
-      const int have = (DKV ? seq.queries : seq.keys) - token_of(n);
+    Step next = start();
+    auto scores = [&](int g) {  // S and dP of the next tile, for warpgroups g
+      const int ls = next.stage;
+      warp_wait(&y_full[ls], next.parity, gave_up);
+      const int have = (DKV ? seq.queries : seq.keys) - token_of(next);
       if (have < BN && (DKV ? seq.queries < a.queries : seq.keys < a.keys)) {
         // what lies behind the sequence's end may be anything, and is multiplied by zeros in the sums
         const uint32_t y = s_y + ls * 2 * G::Y;
@@ -686,7 +668,7 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
         __syncwarp();
       }
       tc_fence_after();
-      const uint32_t t_s = tmem + (WG == 2 ? (n & 1) * 2 * BN : 0);
+      const uint32_t t_s = tmem + g * 2 * BN;
       const Desc y0 = {yk.lo + ls * (2 * G::Y >> 4), yk.hi}, y1 = {y0.lo + (G::Y >> 4), yk.hi};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
@@ -694,16 +676,15 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
         if (k < ks) mma(elected, t_s + BN, x1, off_k<ROWS>(k), y1, off_k<BN>(k), id_s, k > 0);
-      commit(elected, &sp_full[WG == 2 ? n & 1 : 0]);
-      if (++ls == ST) ls = 0, lpar ^= 1;
+      commit(elected, &sp_full[g]);
+      advance(next);
     };
     if (total > 0) {
       warp_wait(x_full, 0, gave_up);
       for (int n = 0; n < WG && n < total; ++n) scores(n);
     }
-    for (int n = 0, s = 0; n < total; ++n, s = s + 1 == ST ? 0 : s + 1) {
-      const int g = WG == 2 ? n & 1 : 0;
-      warp_wait(&pd_full[g], (n / WG) & 1, gave_up);
+    for (int n = 0, s = 0, g = 0, par = 0; n < total; ++n, s = s + 1 == ST ? 0 : s + 1) {
+      warp_wait(&pd_full[g], par, gave_up);
       tc_fence_after();
       const uint32_t t_s = tmem + g * 2 * BN;
       const Desc y0 = {ymn.lo + s * (2 * G::Y >> 4), ymn.hi}, y1 = {y0.lo + (G::Y >> 4), ymn.hi};
@@ -722,13 +703,14 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
       commit(elected, &y_empty[s]);
       if (n + 1 == total) commit(elected, acc_full);
       // behind the sums in the MMAs' order: their P and dS are used up when it overwrites them
-      if (n + WG < total) scores(n + WG);
+      if (n + WG < total) scores(g);
+      if (++g == WG) g = 0, par ^= 1;
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
     warp_wait(idle, 0, gave_up);
   } else {
-    const int g = (warp - 2) >> 2, q = warp & 3;
+    const int g = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, q = warp & 3;
     const int w0 = r0 + q * 32, r = w0 + lane;
     const bool valid = r < row_end;
     const int lo = !valid ? 0 : (DKV ? seq.first_query(a, r) : seq.first_key(a, r)), hi = !valid ? 0 : (DKV ? seq.end_query(a, r) : seq.end_key(a, r));
@@ -746,30 +728,39 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     }
     float* lut = lut0 + (DKV ? g * bins : 0);
     float* my_near = near + (warp - 2) * bins;
-    int lut_head = -1;
-    for (int n = g; n < total; n += WG) {
+    int lut_head = -1, par = 0;
+    Step at_tile = start();
+    if (g && total > 0) advance(at_tile);
+    for (int n = g; n < total; n += WG, par ^= 1) {
+      const Step x_at = at_tile;
+      const int token = token_of(x_at);
+#pragma unroll
+      for (int k = 0; k < WG; ++k) advance(at_tile);
       if constexpr (BIAS && DKV) {
         // the lookup of the tile's head, by the threads that read it
-        if (head_of(n) != lut_head) {
-          lut_head = head_of(n);
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
-          for (int i = (q << 5) + lane; i < bins; i += 128)
+        if (x_at.head != lut_head) {
+          lut_head = x_at.head;
+          asm volatile("bar.sync %0, 256;" ::"r"(1 + g) : "memory");
+          for (int i = ((half * 4 + q) << 5) + lane; i < bins; i += 256)
             lut[i] = table_log2(a.table, (int64_t)relative::bucket_of(a.relative, i - far) * a.heads + lut_head, a.table_dtype);
-          asm volatile("bar.sync %0, 128;" ::"r"(1 + g) : "memory");
+          asm volatile("bar.sync %0, 256;" ::"r"(1 + g) : "memory");
         }
       }
-      if constexpr (DKV) warp_wait(&y_full[n % ST], (n / ST) & 1, gave_up);  // lse and delta
-      warp_wait(&sp_full[g], (n / WG) & 1, gave_up);
+      if constexpr (DKV) warp_wait(&y_full[x_at.stage], x_at.parity, gave_up);  // lse and delta
+      warp_wait(&sp_full[g], par, gave_up);
       tc_fence_after();
-      const float* stat = s_stat + (n % ST) * 2 * BN;
-#pragma unroll
-      for (int c0 = 0; c0 < BN; c0 += 32) {
-        const int t0 = token_of(n) + c0;  // first token of these columns
+      const float* stat = s_stat + x_at.stage * 2 * BN;
+      {
+        const int c0 = half * 32, t0 = token + c0;  // this warp's columns, and the first's token
         uint32_t s[32], d[32];
         tmem_ld32_issue(t_s + c0, s);
         tmem_ld32_issue(t_s + BN + c0, d);
         tmem_wait(s);
         tmem_wait(d);
+        // P and dS go over what the other half's warp of these rows may not have read yet
+        tc_fence_before();
+        asm volatile("bar.sync %0, 64;" ::"r"(3 + g * 4 + q) : "memory");
+        tc_fence_after();
         float x[32];
         int w_rel = 0;  // key - query - shift of lane 0, column 0; + 1 a column for dq, - 1 for dk and dv
         bool is_near = false;
@@ -859,26 +850,22 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     }
     if (total > 0) warp_wait(acc_full, 0, gave_up);
     tc_fence_after();
+    const int part = g * 2 + half, parts = 2 * WG;  // dv and dk: half of the warpgroups each; each a share of the columns
     const int rows = DKV ? (int)a.keys : (int)a.queries, heads = DKV ? (int)a.kv_heads : (int)a.heads;
-    // two warpgroups: dv and dk, or half of dq's columns, each
-#pragma unroll
-    for (int o0 = 0; o0 < (DKV ? 2 : 1); ++o0) {
-      if (DKV && WG == 2 && o0 != g) continue;
-      const int from = !DKV && WG == 2 ? g * (DP / 2) : 0, to = !DKV && WG == 2 ? from + DP / 2 : DP;
-      const uint32_t acc = tm + G::T_ACC + o0 * DP;
-      __nv_bfloat16* row = (o0 ? io.d1 : io.d0) + ((b * rows + r) * heads + hy) * dim;
-      for (int c = from; c < to && c < dim; c += 32) {
-        uint32_t o[32];
-        if (total > 0) {
-          tmem_ld32_issue(acc + c, o);
-          tmem_wait(o);
-        }
-        if (total == 0 || !valid) {
-#pragma unroll
-          for (int k = 0; k < 32; ++k) o[k] = 0;
-        }
-        if (r < rows) store32(row, c, dim, io.vec, o, DKV && !o0 ? 1.f : a.scale);
+    const int which = DKV ? part & 1 : 0, share = DKV ? part >> 1 : part, shares = DKV ? WG : parts;
+    const uint32_t acc = tm + G::T_ACC + which * DP;
+    __nv_bfloat16* row = (which ? io.d1 : io.d0) + ((b * rows + r) * heads + hy) * dim;
+    for (int c = share * 32; c < DP && c < dim; c += shares * 32) {
+      uint32_t o[32];
+      if (total > 0) {
+        tmem_ld32_issue(acc + c, o);
+        tmem_wait(o);
       }
+      if (total == 0 || !valid) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) o[k] = 0;
+      }
+      if (r < rows) store32(row, c, dim, io.vec, o, DKV && !which ? 1.f : a.scale);
     }
     if constexpr (BIAS && !DKV) {
       before = warp_sum(before), after = warp_sum(after);
@@ -896,7 +883,7 @@ __global__ void __launch_bounds__(Bwd<DP>::THREADS, DP == 64 ? 2 : 1)
     for (int i = threadIdx.x; i < bins; i += G::THREADS) {
       float s = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4 * WG; ++w) s += near[w * bins + i];
+      for (int w = 0; w < 8 * WG; ++w) s += near[w * bins + i];
       lut0[i] = s;
     }
     __syncthreads();
@@ -996,7 +983,7 @@ static int launch_forward(const b200_attention& a, const CUtensorMap& q, const C
 
 template <int DP, bool DKV, bool BIAS>
 static int launch_backward(const b200_attention& a, const Operand (&x)[2], const Operand (&y)[2], BwdIo io, cudaStream_t st) {
-  using G = Bwd<DP>;
+  using G = Bwd<DP, DKV, BIAS>;
   CUtensorMap m[4];
   for (int i = 0; i < 2; ++i) {
     if (int rc = map_of(&m[i], a, x[i], ROWS)) return rc;
@@ -1009,7 +996,7 @@ static int launch_backward(const b200_attention& a, const Operand (&x)[2], const
     return rc;
   auto shared = [&](int stages) {
     return 1024 + 2 * (size_t)G::X + stages * 2 * (size_t)G::Y + 256 + (DKV ? G::STAGES * 2 * BN * 4 : 0) +
-           bias_bytes(a, DKV ? G::GROUPS : 1 + 4 * G::GROUPS);
+           bias_bytes(a, DKV ? G::GROUPS : 1 + 8 * G::GROUPS);
   };
   io.stages = shared(G::STAGES) <= SMEM_LIMIT ? G::STAGES : 2;
   const auto kernel = backward_kernel<DP, DKV, BIAS>;
