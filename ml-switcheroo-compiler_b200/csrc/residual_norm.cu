@@ -44,8 +44,8 @@ __global__ void __launch_bounds__(256) fold_kernel(const __grid_constant__ Fold 
 }
 
 // threads of a block, register sets of 8 elements a thread
-static void shape(int64_t cols, bool vec, int* threads, int* nv) {
-  *nv = cols <= 256 * 8 ? 1 : (cols <= 512 * 16 && vec ? 2 : 4);
+static void shape(int64_t cols, bool vec, bool grad, int* threads, int* nv) {
+  *nv = cols <= (grad && vec ? 512 : 256 * 8) ? 1 : (cols <= 512 * 16 && vec ? 2 : 4);
   *threads = (int)(ceil_div(cols, 8 * *nv * 32) * 32);
 }
 
@@ -103,7 +103,7 @@ static Args fill_args(const b200_residual_norm* n, const void* x, const void* f)
   a.rows = n->rows, a.groups = n->groups ? n->groups : 1, a.cols = (int)n->cols;
   a.per_group = a.rows / a.groups;
   a.w_bf16 = (weights ? n->weight_dtype : n->x_dtype) == B200_BF16, a.gate_bf16 = (n->gate ? n->gate_dtype : n->x_dtype) == B200_BF16;
-  a.scale = n->scale, a.eps = n->eps;
+  a.scale = n->scale, a.eps = n->eps, a.inv_cols = (float)(1.0 / (double)n->cols);
   return a;
 }
 
@@ -119,7 +119,7 @@ static bool vectors(const b200_residual_norm* n, std::initializer_list<const voi
 // the launch's shape, and how the kernel gets its weights
 static Launch plan(const b200_residual_norm* n, Args& a, bool vec, bool grad) {
   Launch l = {};
-  shape(n->cols, vec, &l.threads, &l.nv);
+  shape(n->cols, vec, grad, &l.threads, &l.nv);
   const Split s = split(a.rows, a.groups, fill_of(l.threads, l.nv, grad));
   a.chunks = s.chunks, a.per_chunk = s.per_chunk;
   l.blocks = s.blocks, l.vec = vec, l.layer = n->kind == B200_NORM_LAYER, l.post = n->post != 0, l.gate = n->groups > 0;
@@ -162,7 +162,7 @@ extern "C" size_t b200_residual_norm_grad_workspace_bytes(const b200_residual_no
   int64_t most = 0;
   for (bool vec : {false, true}) {  // which of the two depends on the pointers
     int threads, nv;
-    shape(n->cols, vec, &threads, &nv);
+    shape(n->cols, vec, true, &threads, &nv);
     const Split s = split(n->rows, n->groups ? n->groups : 1, fill_of(threads, nv, true));
     const int64_t gate = n->groups && s.chunks > 1 ? s.blocks : 0;
     most = std::max(most, s.blocks * kept_of(n->kind, n->post) + gate);

@@ -53,7 +53,7 @@ struct Args {
   int64_t rows, groups, per_group;      // per_group = rows / groups
   int64_t chunks, per_chunk;            // a group's rows are cut into chunks
   int cols;
-  float scale, eps;
+  float scale, eps, inv_cols;
 };
 
 // Where a thread's element i (of 8 NV) of a row is: vectors of 8 neighbours, or one column in
@@ -188,17 +188,20 @@ __device__ __forceinline__ void put_any(void* base, int64_t row, int cols, int b
 // thread's four neighbours are 16 bytes; or, where they do not fit, reads again from global memory.
 template <int NV>
 struct Slot {
-  float4* at;  // [2 NV][threads], this thread's
+  uint32_t at, step;  // shared-memory address of this thread's first 16 bytes, bytes to the next
   __device__ __forceinline__ void put(const float (&o)[8 * NV]) {
 #pragma unroll
-    for (int i = 0; i < 2 * NV; ++i) at[i * blockDim.x] = make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+    for (int i = 0; i < 2 * NV; ++i)
+      asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at + i * step), "f"(o[4 * i]), "f"(o[4 * i + 1]), "f"(o[4 * i + 2]), "f"(o[4 * i + 3])
+                   : "memory");
   }
   __device__ __forceinline__ void get(float (&o)[8 * NV]) const {
 #pragma unroll
-    for (int i = 0; i < 2 * NV; ++i) {
-      const float4 u = at[i * blockDim.x];
-      o[4 * i] = u.x, o[4 * i + 1] = u.y, o[4 * i + 2] = u.z, o[4 * i + 3] = u.w;
-    }
+    for (int i = 0; i < 2 * NV; ++i)
+      asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                   : "=f"(o[4 * i]), "=f"(o[4 * i + 1]), "=f"(o[4 * i + 2]), "=f"(o[4 * i + 3])
+                   : "r"(at + i * step)
+                   : "memory");
   }
 };
 constexpr int GAMMA = 0, BETA = 1, POST_GAMMA = 2, POST_BETA = 3, GATE_SLOT = 4, SLOTS = 5;
@@ -206,15 +209,15 @@ constexpr int GAMMA = 0, BETA = 1, POST_GAMMA = 2, POST_BETA = 3, GATE_SLOT = 4,
 template <int V, int NV>
 struct Weights {
   const Args& a;
-  float4* smem;
-  int slot[SLOTS];
+  uint32_t slot[SLOTS], step;
   int64_t gate_group;  // whose gate its slot holds
 
-  __device__ __forceinline__ Weights(const Args& a_, float4* s) : a(a_), smem(s + threadIdx.x), gate_group(-1) {
+  __device__ __forceinline__ Weights(const Args& a_, float4* s) : a(a_), step(blockDim.x * 16u), gate_group(-1) {
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(s + threadIdx.x);
     const int has[SLOTS] = {a.has_gamma, a.has_beta, a.has_post_gamma, a.has_post_beta, a.has_gate && a.gate_kept};
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < SLOTS; ++i) slot[i] = has[i] ? n++ : 0;
+    for (int i = 0; i < SLOTS; ++i) slot[i] = base + (has[i] ? n++ : 0) * (2 * NV * step);
     if (!a.shared) return;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -225,7 +228,7 @@ struct Weights {
       }
   }
   __device__ __forceinline__ const void* pointer(int i) const { return i == GAMMA ? a.gamma : (i == BETA ? a.beta : (i == POST_GAMMA ? a.post_gamma : a.post_beta)); }
-  __device__ __forceinline__ Slot<NV> at(int i) const { return {smem + (size_t)slot[i] * 2 * NV * blockDim.x}; }
+  __device__ __forceinline__ Slot<NV> at(int i) const { return {slot[i], step}; }
   __device__ __forceinline__ void get(float (&o)[8 * NV], int i) const {
     if (a.shared) at(i).get(o);
     else fetch<V, NV>(o, pointer(i), 0, a.cols, a.w_bf16);
@@ -246,45 +249,57 @@ struct Weights {
 };
 
 // Sums over the block, the same on every thread: one barrier, the area alternates between two
-// halves so that the next sum may write while slow warps still read this one.
+// halves so that the next sum may write while slow warps still read this one. Places of warps that the block does not have stay zero.
 struct Sums {
   float (*area)[2][16];  // [half][value][warp]
-  int half;
+  int half, quads;       // quads: fours of warps
+  __device__ __forceinline__ Sums(float (*s)[2][16]) : area(s), half(0), quads(((int)blockDim.x + 127) >> 7) {
+    for (int i = threadIdx.x; i < 64; i += blockDim.x) (&s[0][0][0])[i] = 0.f;
+    __syncthreads();
+  }
+  __device__ __forceinline__ float read(const float* p) const {
+    const float4* v = reinterpret_cast<const float4*>(p);
+    float4 u = v[0];
+    float s = (u.x + u.y) + (u.z + u.w);
+    if (quads > 1) u = v[1], s += (u.x + u.y) + (u.z + u.w);
+    if (quads > 2) {
+      u = v[2], s += (u.x + u.y) + (u.z + u.w);
+      u = v[3], s += (u.x + u.y) + (u.z + u.w);
+    }
+    return s;
+  }
   __device__ __forceinline__ void operator()(float& a, float& b) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       a += __shfl_xor_sync(0xffffffffu, a, o);
       b += __shfl_xor_sync(0xffffffffu, b, o);
     }
-    if (warps == 1) return;
-    if (lane == 0) area[half][0][warp] = a, area[half][1][warp] = b;
+    if (blockDim.x == 32) return;
+    if ((threadIdx.x & 31) == 0) area[half][0][threadIdx.x >> 5] = a, area[half][1][threadIdx.x >> 5] = b;
     __syncthreads();
-    a = b = 0.f;
-    for (int w = 0; w < warps; ++w) a += area[half][0][w], b += area[half][1][w];
+    a = read(area[half][0]), b = read(area[half][1]);
     half ^= 1;
   }
   __device__ __forceinline__ void operator()(float& a) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
     a = warp_sum(a);
-    if (warps == 1) return;
-    if (lane == 0) area[half][0][warp] = a;
+    if (blockDim.x == 32) return;
+    if ((threadIdx.x & 31) == 0) area[half][0][threadIdx.x >> 5] = a;
     __syncthreads();
-    a = 0.f;
-    for (int w = 0; w < warps; ++w) a += area[half][0][w];
+    a = read(area[half][0]);
     half ^= 1;
   }
 };
 
 // t (zeros behind the row's end) -> the normed row u before gamma; returns rstd
 template <int V, int NV, bool LAYER>
-__device__ __forceinline__ float unit(float (&t)[8 * NV], int cols, float eps, Sums& sums) {
+__device__ __forceinline__ float unit(float (&t)[8 * NV], const Args& a, Sums& sums) {
+  const int cols = a.cols;
   if constexpr (LAYER) {
     float m = 0.f;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) m += t[i];
     sums(m);
-    m /= (float)cols;
+    m *= a.inv_cols;
 #pragma unroll
     for (int i = 0; i < 8 * NV; ++i) t[i] = column<V>(i) < cols ? t[i] - m : 0.f;
   }
@@ -292,7 +307,7 @@ __device__ __forceinline__ float unit(float (&t)[8 * NV], int cols, float eps, S
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) q = fmaf(t[i], t[i], q);
   sums(q);
-  const float rstd = 1.f / sqrtf(q / (float)cols + eps);
+  const float rstd = rsqrtf(fmaf(q, a.inv_cols, a.eps));
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) t[i] *= rstd;
   return rstd;
@@ -300,7 +315,8 @@ __device__ __forceinline__ float unit(float (&t)[8 * NV], int cols, float eps, S
 
 // d = dy gamma -> the gradient rstd (d - [mean d] - u mean(d u))
 template <int V, int NV, bool LAYER>
-__device__ __forceinline__ void unit_grad(float (&d)[8 * NV], const float (&u)[8 * NV], float rstd, int cols, Sums& sums) {
+__device__ __forceinline__ void unit_grad(float (&d)[8 * NV], const float (&u)[8 * NV], float rstd, const Args& args, Sums& sums) {
+  const int cols = args.cols;
   float a = 0.f, b = 0.f;
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) {
@@ -309,11 +325,11 @@ __device__ __forceinline__ void unit_grad(float (&d)[8 * NV], const float (&u)[8
   }
   if constexpr (LAYER) sums(a, b);
   else sums(a);
-  a /= (float)cols;
-  b /= (float)cols;
+  a *= -rstd * args.inv_cols;
+  b *= args.inv_cols;
 #pragma unroll
   for (int i = 0; i < 8 * NV; ++i) {
-    d[i] = rstd * (d[i] - b - u[i] * a);
+    d[i] = LAYER ? fmaf(a, u[i], rstd * (d[i] - b)) : fmaf(a, u[i], rstd * d[i]);
     if (LAYER && column<V>(i) >= cols) d[i] = 0.f;  // what a later mean adds up
   }
 }
@@ -357,9 +373,9 @@ __device__ __forceinline__ void plus(float (&x)[8 * NV], const float (&y)[8 * NV
 
 template <int V, int NV, bool LAYER, bool POST, typename TX, typename TF>
 __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::FORWARD) forward_kernel(const __grid_constant__ Args a) {
-  __shared__ float area[2][2][16];
+  __shared__ __align__(16) float area[2][2][16];
   extern __shared__ float4 slots[];
-  Sums sums{area, 0};
+  Sums sums(area);
   Weights<V, NV> weights(a, slots);
   constexpr int E = 8 * NV;
   for (Walk w(a); w.more(a); w.next(a)) {
@@ -373,7 +389,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::FORWARD) forw
       rx.get(s);
     }
     if constexpr (POST) {
-      unit<V, NV, LAYER>(p, a.cols, a.eps, sums);
+      unit<V, NV, LAYER>(p, a, sums);
       if (a.has_post_gamma) {
         weights.get(t, POST_GAMMA);
         times<NV>(p, t);
@@ -390,7 +406,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::FORWARD) forw
 #pragma unroll
     for (int i = 0; i < E; ++i) s[i] = fmaf(a.scale, s[i], p[i]);
     put<V, NV>(reinterpret_cast<TX*>(a.out0), w.row, a.cols, s);
-    unit<V, NV, LAYER>(s, a.cols, a.eps, sums);
+    unit<V, NV, LAYER>(s, a, sums);
     if (a.has_gamma) {
       weights.get(t, GAMMA);
       times<NV>(s, t);
@@ -413,9 +429,9 @@ struct Kept {
 template <int V, int NV, bool LAYER, bool POST, bool GATE, typename TX, typename TF>
 __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::GRADIENT) gradient_kernel(const __grid_constant__ Args a) {
   using K = Kept<LAYER, POST>;
-  __shared__ float area[2][2][16];
+  __shared__ __align__(16) float area[2][2][16];
   extern __shared__ float4 slots[];
-  Sums sums{area, 0};
+  Sums sums(area);
   Weights<V, NV> weights(a, slots);
   constexpr int E = 8 * NV;
   float kept[K::N][E], dgate[GATE ? E : 1];
@@ -467,7 +483,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::GRADIENT) gra
       }
     };
     float rstd_f = 0.f;
-    if constexpr (POST) rstd_f = unit<V, NV, LAYER>(p, a.cols, a.eps, sums);
+    if constexpr (POST) rstd_f = unit<V, NV, LAYER>(p, a, sums);
     {
       float o[E];
       block(o);
@@ -478,7 +494,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::GRADIENT) gra
 #pragma unroll
       for (int i = 0; i < E; ++i) s[i] = fmaf(a.scale, s[i], o[i]);
     }
-    const float rstd = unit<V, NV, LAYER>(s, a.cols, a.eps, sums);
+    const float rstd = unit<V, NV, LAYER>(s, a, sums);
     float d[E];
     rh.get(d);
 #pragma unroll
@@ -490,7 +506,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::GRADIENT) gra
       weights.get(t, GAMMA);
       times<NV>(d, t);
     }
-    unit_grad<V, NV, LAYER>(d, s, rstd, a.cols, sums);
+    unit_grad<V, NV, LAYER>(d, s, rstd, a, sums);
     rs.get(t);
     plus<NV>(d, t);  // the sum's whole gradient
 #pragma unroll
@@ -517,7 +533,7 @@ __global__ void __launch_bounds__(Bounds<NV>::THREADS, Bounds<NV>::GRADIENT) gra
         weights.get(t, POST_GAMMA);
         times<NV>(d, t);
       }
-      unit_grad<V, NV, LAYER>(d, p, rstd_f, a.cols, sums);
+      unit_grad<V, NV, LAYER>(d, p, rstd_f, a, sums);
     }
     put<V, NV>(reinterpret_cast<TF*>(a.out1), row, a.cols, d);
   }
