@@ -37,42 +37,58 @@ struct Io {
   float* part;                  // FWD with splits: [row blocks][splits][R][dim + 2]; DQ with a table: [row blocks][buckets]
 };
 
+// A lane's E elements of a token as they are in memory. Lanes behind the head's end read its first elements, whose factors are
+// zero, and tokens behind the last are the last again: no load waits behind a branch.
 template <typename T, int E>
-__device__ __forceinline__ void load(float (&v)[E], const T* p, int c, int dim, int vec) {
-  if (vec) {
-    if (c < dim) {
-      if constexpr (sizeof(T) == 4) {
-        if constexpr (E == 2) {
-          const float2 u = *reinterpret_cast<const float2*>(p + c);
-          v[0] = u.x, v[1] = u.y;
-        } else {
-#pragma unroll
-          for (int i = 0; i < E; i += 4) {
-            const float4 u = *reinterpret_cast<const float4*>(p + c + i);
-            v[i] = u.x, v[i + 1] = u.y, v[i + 2] = u.z, v[i + 3] = u.w;
-          }
-        }
+struct Token {
+  static constexpr int WORDS = E * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+
+  __device__ __forceinline__ void load(const T* p, int c, int dim, int vec) {
+    if (vec) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p + (c < dim ? c : 0));
+      if constexpr (WORDS == 1) {
+        w[0] = *q;
+      } else if constexpr (WORDS == 2) {
+        const uint2 u = *reinterpret_cast<const uint2*>(q);
+        w[0] = u.x, w[1] = u.y;
       } else {
-        uint32_t w[E / 2];
-        if constexpr (E == 2) w[0] = *reinterpret_cast<const uint32_t*>(p + c);
-        else if constexpr (E == 4) {
-          const uint2 u = *reinterpret_cast<const uint2*>(p + c);
-          w[0] = u.x, w[1] = u.y;
-        } else {
-          const uint4 u = *reinterpret_cast<const uint4*>(p + c);
-          w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w;
-        }
 #pragma unroll
-        for (int i = 0; i < E / 2; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        for (int i = 0; i < WORDS; i += 4) {
+          const uint4 u = *reinterpret_cast<const uint4*>(q + i);
+          w[i] = u.x, w[i + 1] = u.y, w[i + 2] = u.z, w[i + 3] = u.w;
+        }
       }
+    } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) w[i] = __float_as_uint(c + i < dim ? (float)p[c + i] : 0.f);
     } else {
 #pragma unroll
-      for (int i = 0; i < E; ++i) v[i] = 0.f;
+      for (int i = 0; i < E / 2; ++i) {
+        const __nv_bfloat162 u = __floats2bfloat162_rn(c + 2 * i < dim ? (float)p[c + 2 * i] : 0.f, c + 2 * i + 1 < dim ? (float)p[c + 2 * i + 1] : 0.f);
+        w[i] = *reinterpret_cast<const uint32_t*>(&u);
+      }
     }
-  } else {
-#pragma unroll
-    for (int i = 0; i < E; ++i) v[i] = c + i < dim ? (float)p[c + i] : 0.f;
   }
+  __device__ __forceinline__ void get(float (&v)[E]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < E; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < E / 2; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+  }
+};
+// a row that stays: zeros behind the head's end
+template <typename T, int E>
+__device__ __forceinline__ void load_row(float (&v)[E], const T* p, int c, int dim, int vec) {
+  Token<T, E> x;
+  x.load(p, c, dim, vec);
+  x.get(v);
+#pragma unroll
+  for (int i = 0; i < E; ++i)
+    if (c + i >= dim) v[i] = 0.f;
 }
 template <int E>
 __device__ __forceinline__ void zero(float (&v)[E]) {
@@ -97,7 +113,6 @@ template <typename T, int E, int R, int MODE>
 __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
     rows_kernel(const __grid_constant__ b200_attention a, const __grid_constant__ Io io) {
   constexpr int KEYS = 32 / R;
-  constexpr bool KEEP = KEYS * E <= 16;  // the step's tokens stay in registers between both products
   extern __shared__ __align__(16) uint8_t smem[];
   float* s_p = reinterpret_cast<float*>(smem);             // [WARPS][2][32]: p or corrections; dz
   float* s_join = s_p + WARPS * 64;                        // [WARPS][R][32 E] (DKV: twice), then FWD's m and l [WARPS][R] each
@@ -139,9 +154,6 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   // the block's tokens: from the smallest to the largest of its rows' (whose ranges move one way)
   int first = __reduce_min_sync(0xffffffffu, hi > lo ? lo : 0x7fffffff), end = __reduce_max_sync(0xffffffffu, hi > lo ? hi : 0);
   if (first > end) first = end;
-  if (MODE == DKV) {  // tokens are (query, head of the group)
-    first *= group, end *= group;
-  }
   if (MODE == FWD && io.splits > 1) {
     const int unit = io.splits * KEYS * WARPS;
     const int each = (end - first + unit - 1) / unit * KEYS * WARPS;
@@ -159,14 +171,14 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
     if constexpr (MODE == DKV) {
       const int j = rb * R + r;
       if (j < row_end) {
-        load<T, E>(x1[r], k + j * a.k_stride[1], c, dim, io.vec);
-        load<T, E>(x2[r], v + j * a.v_stride[1], c, dim, io.vec);
+        load_row<T, E>(x1[r], k + j * a.k_stride[1], c, dim, io.vec);
+        load_row<T, E>(x2[r], v + j * a.v_stride[1], c, dim, io.vec);
       }
     } else {
       const int i = row_query(r), h = row_head(r);
       if (i < row_end) {
-        load<T, E>(x1[r], q + i * a.q_stride[1] + h * a.q_stride[2], c, dim, io.vec);
-        if constexpr (MODE == DQ) load<T, E>(x2[r], dout + i * io.dout_stride[1] + h * io.dout_stride[2], c, dim, io.vec);
+        load_row<T, E>(x1[r], q + i * a.q_stride[1] + h * a.q_stride[2], c, dim, io.vec);
+        if constexpr (MODE == DQ) load_row<T, E>(x2[r], dout + i * io.dout_stride[1] + h * io.dout_stride[2], c, dim, io.vec);
       }
     }
   }
@@ -182,165 +194,161 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   }
   float* sp = s_p + warp * 64;
 
-  for (int t0 = first + warp * KEYS; t0 < end; t0 += WARPS * KEYS) {
-    float z[32], y1[KEEP ? KEYS : 1][E], y2[KEEP && MODE == DKV ? KEYS : 1][E];
-    auto token1 = [&](float (&y)[E], int n) {  // K, or Q for dk and dv
-      const int t = t0 + n;
-      if (t >= end) {
-        zero(y);
-        return;
-      }
-      if constexpr (MODE == DKV) load<T, E>(y, q + (t / group) * a.q_stride[1] + (kvh * group + t % group) * a.q_stride[2], c, dim, io.vec);
-      else load<T, E>(y, k + t * a.k_stride[1], c, dim, io.vec);
-    };
-    auto token2 = [&](float (&y)[E], int n) {  // V, or dout for dk and dv
-      const int t = t0 + n;
-      if (t >= end) {
-        zero(y);
-        return;
-      }
-      if constexpr (MODE == DKV)
-        load<T, E>(y, dout + (t / group) * io.dout_stride[1] + (kvh * group + t % group) * io.dout_stride[2], c, dim, io.vec);
-      else load<T, E>(y, v + t * a.v_stride[1], c, dim, io.vec);
-    };
+  // dk and dv: the tokens of one head of the group after the other
+  for (int head = MODE == DKV ? kvh * group : 0, heads = MODE == DKV ? group : 1; heads > 0; ++head, --heads)
+    for (int t0 = first + warp * KEYS; t0 < end; t0 += WARPS * KEYS) {
+      auto token1 = [&](int n) {  // K, or Q for dk and dv
+        const int t = min(t0 + n, end - 1);
+        return MODE == DKV ? q + t * a.q_stride[1] + head * a.q_stride[2] : k + t * a.k_stride[1];
+      };
+      auto token2 = [&](int n) {  // V, or dout for dk and dv
+        const int t = min(t0 + n, end - 1);
+        return MODE == DKV ? dout + t * io.dout_stride[1] + head * io.dout_stride[2] : v + t * a.v_stride[1];
+      };
+      // both sides' tokens are on their way before the first product where registers allow
+      constexpr int WORDS = Token<T, E>::WORDS;
+      constexpr bool BOTH = KEYS * WORDS <= 32;
+      Token<T, E> y1[KEYS], y2[BOTH ? KEYS : 1];
 #pragma unroll
-    for (int n = 0; n < KEYS; ++n) {
-      float y[E];
-      token1(y, n);
+      for (int n = 0; n < KEYS; ++n) y1[n].load(token1(n), c, dim, io.vec);
+      if constexpr (BOTH)
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        float s = 0.f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) s = fmaf(x1[r][e], y[e], s);
-        z[r * KEYS + n] = s;
-      }
-      if constexpr (KEEP && MODE != FWD)
-#pragma unroll
-        for (int e = 0; e < E; ++e) y1[n][e] = y[e];
-    }
-    const float dot = sum_to_lane(z, lane);
-    // the lane's score
-    const int t = t0 + lk;
-    const int i = MODE == DKV ? t / group : my_row, j = MODE == DKV ? my_row : t;
-    const int other = MODE == DKV ? i : j;
-    const bool seen = t < end && other >= lo && other < hi;
-    const int rel = j - i - seq.shift;
-    float s = dot * sl;
-    if (a.table && seen) {
-      const int h = MODE == DKV ? kvh * group + t % group : my_head;
-      s += table_log2(a.table, (int64_t)s_bucket[max(-far, min(far, rel)) + far] * a.heads + h, a.table_dtype);
-    }
-    if (!seen) s = -INFINITY;
-    if constexpr (MODE == FWD) {
-      float top = s;
-#pragma unroll
-      for (int o = KEYS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      top = fmaxf(m, top);
-      const float base = top == -INFINITY ? 0.f : top;
-      const float p = exp2f(s - base), fix = exp2f(m - base);
-      const bool grown = __any_sync(0xffffffffu, top != m);
-      l = l * fix + p;
-      m = top;
-      __syncwarp();
-      sp[lane] = p;
-      if (lk == 0) sp[32 + lr] = fix;
-      __syncwarp();
-      if (grown) {
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float f = sp[32 + r];
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[r][e] *= f;
-        }
-      }
+        for (int n = 0; n < KEYS; ++n) y2[n].load(token2(n), c, dim, io.vec);
+      float z[32];
 #pragma unroll
       for (int n = 0; n < KEYS; ++n) {
         float y[E];
-        token2(y, n);
+        y1[n].get(y);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
-          const float f = sp[r * KEYS + n];
+          float s = 0.f;
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
+          for (int e = 0; e < E; ++e) s = fmaf(x1[r][e], y[e], s);
+          z[r * KEYS + n] = s;
         }
       }
-    } else {
-#pragma unroll
-      for (int n = 0; n < KEYS; ++n) {
-        float y[E];
-        token2(y, n);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float d = 0.f;
-#pragma unroll
-          for (int e = 0; e < E; ++e) d = fmaf(x2[r][e], y[e], d);
-          z[r * KEYS + n] = d;
+      auto second = [&](float (&y)[E], int n) {
+        if constexpr (BOTH) {
+          y2[n].get(y);
+        } else {
+          Token<T, E> u;
+          u.load(token2(n), c, dim, io.vec);
+          u.get(y);
         }
-        if constexpr (KEEP && MODE == DKV)
-#pragma unroll
-          for (int e = 0; e < E; ++e) y2[n][e] = y[e];
+      };
+      const float dot = sum_to_lane(z, lane);
+      // the lane's score
+      const int t = t0 + lk;
+      const int i = MODE == DKV ? t : my_row, j = MODE == DKV ? my_row : t;
+      const int other = MODE == DKV ? i : j;
+      const bool seen = t < end && other >= lo && other < hi;
+      const int rel = j - i - seq.shift;
+      float s = dot * sl;
+      if (a.table && seen) {
+        const int h = MODE == DKV ? head : my_head;
+        s += table_log2(a.table, (int64_t)s_bucket[max(-far, min(far, rel)) + far] * a.heads + h, a.table_dtype);
       }
-      const float dp = sum_to_lane(z, lane);
-      float lse = my_lse, delta = my_delta;
-      if constexpr (MODE == DKV) {
-        lse = INFINITY, delta = 0.f;
-        if (seen) {
-          const int64_t at = (b * a.heads + kvh * group + t % group) * a.queries + i;
-          lse = io.lse[at] * LOG2E;
-          if (lse == -INFINITY) lse = INFINITY;
-          delta = io.delta[(b * a.heads + kvh * group + t % group) * io.padded + i];
-        }
-      }
-      const float p = seen ? exp2f(s - lse) : 0.f;
-      const float dz = seen ? p * (dp - delta) : 0.f;
-      __syncwarp();
-      sp[lane] = p;
-      sp[32 + lane] = dz;
-      __syncwarp();
-      if constexpr (MODE == DQ) {
-        if (a.table) {
-          if (rel >= far) after += dz;
-          else if (rel <= -far) before += dz;
-          // the step's near diagonals rel = t0 + d - (R - 1) - first query - shift, one a lane: no lane adds to another's
-          const int d = lane - (R - 1);
-          const int at = t0 + d - rb * R - seq.shift;
-          if (lane < R + KEYS - 1 && at > -far && at < far) {
-            float sum = 0.f;
+      if (!seen) s = -INFINITY;
+      if constexpr (MODE == FWD) {
+        float top = s;
 #pragma unroll
-            for (int r = 0; r < R; ++r)
-              if (d + r >= 0 && d + r < KEYS) sum += sp[32 + r * KEYS + d + r];
-            s_near[warp * bins + at + far] += sum;
+        for (int o = KEYS / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top = fmaxf(m, top);
+        const float base = top == -INFINITY ? 0.f : top;
+        const float p = exp2f(s - base), fix = exp2f(m - base);
+        const bool grown = __any_sync(0xffffffffu, top != m);
+        l = l * fix + p;
+        m = top;
+        __syncwarp();
+        sp[lane] = p;
+        if (lk == 0) sp[32 + lr] = fix;
+        __syncwarp();
+        if (grown) {
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float f = sp[32 + r];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] *= f;
           }
         }
-      }
 #pragma unroll
-      for (int n = 0; n < KEYS; ++n) {
-        float y[E];
-        if constexpr (KEEP)
-#pragma unroll
-          for (int e = 0; e < E; ++e) y[e] = y1[n][e];
-        else token1(y, n);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          const float f = sp[32 + r * KEYS + n];
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
-        }
-        if constexpr (MODE == DKV) {
-          if constexpr (KEEP)
-#pragma unroll
-            for (int e = 0; e < E; ++e) y[e] = y2[n][e];
-          else token2(y, n);
+        for (int n = 0; n < KEYS; ++n) {
+          float y[E];
+          second(y, n);
 #pragma unroll
           for (int r = 0; r < R; ++r) {
             const float f = sp[r * KEYS + n];
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc2[r][e] = fmaf(f, y[e], acc2[r][e]);
+            for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int n = 0; n < KEYS; ++n) {
+          float y[E];
+          second(y, n);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            float d = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) d = fmaf(x2[r][e], y[e], d);
+            z[r * KEYS + n] = d;
+          }
+        }
+        const float dp = sum_to_lane(z, lane);
+        float lse = my_lse, delta = my_delta;
+        if constexpr (MODE == DKV) {
+          lse = INFINITY, delta = 0.f;
+          if (seen) {
+            lse = io.lse[(b * a.heads + head) * a.queries + i] * LOG2E;
+            if (lse == -INFINITY) lse = INFINITY;
+            delta = io.delta[(b * a.heads + head) * io.padded + i];
+          }
+        }
+        const float p = seen ? exp2f(s - lse) : 0.f;
+        const float dz = seen ? p * (dp - delta) : 0.f;
+        __syncwarp();
+        sp[lane] = p;
+        sp[32 + lane] = dz;
+        __syncwarp();
+        if constexpr (MODE == DQ) {
+          if (a.table) {
+            if (rel >= far) after += dz;
+            else if (rel <= -far) before += dz;
+            // the step's near diagonals rel = t0 + d - (R - 1) - first query - shift, one a lane: no lane adds to another's
+            const int d = lane - (R - 1);
+            const int at = t0 + d - rb * R - seq.shift;
+            if (lane < R + KEYS - 1 && at > -far && at < far) {
+              float sum = 0.f;
+#pragma unroll
+              for (int r = 0; r < R; ++r)
+                if (d + r >= 0 && d + r < KEYS) sum += sp[32 + r * KEYS + d + r];
+              s_near[warp * bins + at + far] += sum;
+            }
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < KEYS; ++n) {
+          float y[E];
+          y1[n].get(y);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float f = sp[32 + r * KEYS + n];
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
+          }
+          if constexpr (MODE == DKV) {
+            second(y, n);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+              const float f = sp[r * KEYS + n];
+#pragma unroll
+              for (int e = 0; e < E; ++e) acc2[r][e] = fmaf(f, y[e], acc2[r][e]);
+            }
           }
         }
       }
     }
-  }
 
   // the warps' results joined, in order
   float *jm = s_join + JOIN - 2 * WARPS * R, *jl = jm + WARPS * R;
