@@ -194,26 +194,35 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   }
   float* sp = s_p + warp * 64;
 
+  constexpr int WORDS = Token<T, E>::WORDS;
+  // both sides' tokens are on their way before the first product where registers allow; forward, the next step's as soon as
+  // this one's are used up
+  constexpr bool BOTH = KEYS * WORDS <= 32, AHEAD = MODE == FWD && BOTH;
+  Token<T, E> y1[KEYS], y2[BOTH ? KEYS : 1];
   // dk and dv: the tokens of one head of the group after the other
-  for (int head = MODE == DKV ? kvh * group : 0, heads = MODE == DKV ? group : 1; heads > 0; ++head, --heads)
-    for (int t0 = first + warp * KEYS; t0 < end; t0 += WARPS * KEYS) {
-      auto token1 = [&](int n) {  // K, or Q for dk and dv
-        const int t = min(t0 + n, end - 1);
-        return MODE == DKV ? q + t * a.q_stride[1] + head * a.q_stride[2] : k + t * a.k_stride[1];
-      };
-      auto token2 = [&](int n) {  // V, or dout for dk and dv
-        const int t = min(t0 + n, end - 1);
-        return MODE == DKV ? dout + t * io.dout_stride[1] + head * io.dout_stride[2] : v + t * a.v_stride[1];
-      };
-      // both sides' tokens are on their way before the first product where registers allow
-      constexpr int WORDS = Token<T, E>::WORDS;
-      constexpr bool BOTH = KEYS * WORDS <= 32;
-      Token<T, E> y1[KEYS], y2[BOTH ? KEYS : 1];
+  for (int head = MODE == DKV ? kvh * group : 0, heads = MODE == DKV ? group : 1; heads > 0; ++head, --heads) {
+    auto token1 = [&](int t) {  // K, or Q for dk and dv
+      t = min(t, end - 1);
+      return MODE == DKV ? q + t * a.q_stride[1] + head * a.q_stride[2] : k + t * a.k_stride[1];
+    };
+    auto token2 = [&](int t) {  // V, or dout for dk and dv
+      t = min(t, end - 1);
+      return MODE == DKV ? dout + t * io.dout_stride[1] + head * io.dout_stride[2] : v + t * a.v_stride[1];
+    };
+    auto load1 = [&](int t) {
 #pragma unroll
-      for (int n = 0; n < KEYS; ++n) y1[n].load(token1(n), c, dim, io.vec);
+      for (int n = 0; n < KEYS; ++n) y1[n].load(token1(t + n), c, dim, io.vec);
+    };
+    auto load2 = [&](int t) {
       if constexpr (BOTH)
 #pragma unroll
-        for (int n = 0; n < KEYS; ++n) y2[n].load(token2(n), c, dim, io.vec);
+        for (int n = 0; n < KEYS; ++n) y2[n].load(token2(t + n), c, dim, io.vec);
+    };
+    int t0 = first + warp * KEYS;
+    if (AHEAD && t0 < end) load1(t0), load2(t0);
+    for (; t0 < end; t0 += WARPS * KEYS) {
+      const bool more = t0 + WARPS * KEYS < end;
+      if constexpr (!AHEAD) load1(t0), load2(t0);
       float z[32];
 #pragma unroll
       for (int n = 0; n < KEYS; ++n) {
@@ -232,10 +241,11 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
           y2[n].get(y);
         } else {
           Token<T, E> u;
-          u.load(token2(n), c, dim, io.vec);
+          u.load(token2(t0 + n), c, dim, io.vec);
           u.get(y);
         }
       };
+      if (AHEAD && more) load1(t0 + WARPS * KEYS);
       const float dot = sum_to_lane(z, lane);
       // the lane's score
       const int t = t0 + lk;
@@ -282,6 +292,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
             for (int e = 0; e < E; ++e) acc[r][e] = fmaf(f, y[e], acc[r][e]);
           }
         }
+        if (AHEAD && more) load2(t0 + WARPS * KEYS);
       } else {
 #pragma unroll
         for (int n = 0; n < KEYS; ++n) {
@@ -349,6 +360,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
         }
       }
     }
+  }
 
   // the warps' results joined, in order
   float *jm = s_join + JOIN - 2 * WARPS * R, *jl = jm + WARPS * R;
@@ -428,30 +440,46 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   }
 }
 
-// joins the splits of a row: a warp each
+// joins the splits of a row, a block each: their factors once, then a thread a column
+constexpr int MOST_SPLITS = 256;
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
     join_kernel(const __grid_constant__ b200_attention a, const float* part, int splits, int64_t row_blocks, int R, T* out, float* lse) {
-  const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5;  // [batch][key head][query][head of the group]
-  const int lane = threadIdx.x & 31, dim = (int)a.dim;
+  __shared__ float factor[MOST_SPLITS], red[32];
+  const int64_t at = blockIdx.x;  // [batch][key head][query][head of the group]
+  const int dim = (int)a.dim;
   const int64_t group = a.heads / a.kv_heads, per = a.queries * group;
-  if (at >= a.batch * a.kv_heads * per) return;
   const int64_t bk = at / per, rr = at % per, b = bk / a.kv_heads, i = rr / group, h = bk % a.kv_heads * group + rr % group;
   const float* p = part + ((bk * row_blocks + rr / R) * splits * R + rr % R) * (dim + 2);
   const int64_t step = (int64_t)R * (dim + 2);
-  float top = -INFINITY, sum = 0.f;
-  for (int s = lane; s < splits; s += 32) top = fmaxf(top, p[s * step + dim]);
-  top = warp_max(top);
-  const float base = top == -INFINITY ? 0.f : top;
-  for (int s = lane; s < splits; s += 32) sum = fmaf(exp2f(p[s * step + dim] - base), p[s * step + dim + 1], sum);
-  sum = warp_sum(sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  for (int c = lane; c < dim; c += 32) {
-    float o = 0.f;
-    for (int s = 0; s < splits; ++s) o = fmaf(exp2f(p[s * step + dim] - base), p[s * step + c], o);
-    out[((b * a.queries + i) * a.heads + h) * dim + c] = (T)(o * inv);
+  float m[MOST_SPLITS / 128], l[MOST_SPLITS / 128], top = -INFINITY, sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < MOST_SPLITS / 128; ++k) {
+    const int s = threadIdx.x + 128 * k;
+    m[k] = s < splits ? p[s * step + dim] : -INFINITY;
+    l[k] = s < splits ? p[s * step + dim + 1] : 0.f;
+    top = fmaxf(top, m[k]);
   }
-  if (lane == 0) lse[(b * a.heads + h) * a.queries + i] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * LN2;
+  top = block_max(top, red);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int k = 0; k < MOST_SPLITS / 128; ++k) {
+    const float f = exp2f(m[k] - base);
+    factor[threadIdx.x + 128 * k] = f;
+    sum = fmaf(f, l[k], sum);
+  }
+  sum = block_sum(sum, red);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int c = threadIdx.x; c < dim; c += 128) {
+    float o[4] = {0.f, 0.f, 0.f, 0.f};
+    int s = 0;
+    for (; s + 8 <= splits; s += 8)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) o[k & 3] = fmaf(factor[s + k], p[(s + k) * step + c], o[k & 3]);
+    for (; s < splits; ++s) o[0] = fmaf(factor[s], p[s * step + c], o[0]);
+    out[((b * a.queries + i) * a.heads + h) * dim + c] = (T)(((o[0] + o[1]) + (o[2] + o[3])) * inv);
+  }
+  if (threadIdx.x == 0) lse[(b * a.heads + h) * a.queries + i] = sum == 0.f ? -INFINITY : (base + log2f(sum)) * LN2;
 }
 
 // dtable[bucket, h]: the blocks' sums, batch by batch; 32 lanes a value
@@ -493,10 +521,10 @@ static Shape forward_shape(const b200_attention& a) {
   const int64_t rows = a.queries * (a.heads / a.kv_heads);
   s.R = rows_of(a, rows);
   s.blocks = ceil_div(rows, s.R);
-  // splits that bring 4 blocks to every SM, of 256 keys at least
-  const int64_t have = s.blocks * a.batch * a.kv_heads, want = 4 * (int64_t)num_sms();
-  s.splits = (int)std::max<int64_t>(1, std::min({ceil_div(want, have), ceil_div(a.keys, 256), (int64_t)1024}));
-  if (have >= 2 * (int64_t)num_sms()) s.splits = 1;
+  // splits that bring 12 blocks to every SM (four waves, so that caches of several lengths even out), of 64 keys at least;
+  // none where the rows alone fill the SMs twice
+  const int64_t have = s.blocks * a.batch * a.kv_heads, sms = num_sms();
+  s.splits = have >= 6 * sms ? 1 : (int)std::max<int64_t>(1, std::min({12 * sms / have, ceil_div(a.keys, 64), (int64_t)MOST_SPLITS}));
   return s;
 }
 
@@ -559,9 +587,9 @@ int rows_forward(const b200_attention& a, void* out, float* lse, void* workspace
   B200_REQUIRE(s.blocks * s.splits < (1ll << 31), "attention: too many queries");
   if (int rc = launch_any<FWD>(a, io, s.R, dim3((unsigned)(s.blocks * s.splits), (unsigned)a.kv_heads, (unsigned)a.batch), st)) return rc;
   if (s.splits == 1) return B200_OK;
-  const unsigned grid = (unsigned)ceil_div(a.batch * a.heads * a.queries, 8);
-  if (a.dtype == B200_F32) join_kernel<float><<<grid, 256, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (float*)out, lse);
-  else join_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (__nv_bfloat16*)out, lse);
+  const unsigned grid = (unsigned)(a.batch * a.heads * a.queries);
+  if (a.dtype == B200_F32) join_kernel<float><<<grid, 128, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (float*)out, lse);
+  else join_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(a, io.part, s.splits, s.blocks, s.R, (__nv_bfloat16*)out, lse);
   return check_launch("attention");
 }
 
