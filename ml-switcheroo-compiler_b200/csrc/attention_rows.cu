@@ -10,6 +10,8 @@
 // where rows leave SMs idle the keys are split over blocks and a second launch joins the parts.
 // Backward: p = exp2(z - lse) made again; dq has rows of queries, dk and dv rows of keys, so every sum
 // stays in registers, in a fixed order. Everything is fp32.
+// bf16 queries (rows of whole 16 bytes) make their scores by mma.sync instead, 8 tokens a step, whose operands a lane loads as
+// they are: without the sums over lanes and the conversions of K a step has half the instructions.
 // What bounds it: HBM for single tokens, else the FMA pipe (2 FMAs of 32 lanes for 32 E of a score's
 // elements, 60 % of the issue slots at 128 elements a head).
 #include <algorithm>
@@ -22,6 +24,7 @@ namespace rows {
 
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int FWD = 0, DQ = 1, DKV = 2;
+constexpr int AREA = 80;  // floats that a warp hands scores round by
 
 struct Io {
   int64_t out_rows;             // blocks of rows of one (batch, head or key head)
@@ -96,6 +99,13 @@ __device__ __forceinline__ void zero(float (&v)[E]) {
   for (int i = 0; i < E; ++i) v[i] = 0.f;
 }
 
+// D += A B for 16 rows, 8 columns and 16 elements in bf16; rows 8 to 15 of A are zeros
+__device__ __forceinline__ void mma_16x8(float& d0, float& d1, float& d2, float& d3, uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d0), "+f"(d1), "+f"(d2), "+f"(d3)
+      : "r"(a0), "r"(0), "r"(a2), "r"(0), "r"(b0), "r"(b1));
+}
+
 // 32 values a lane -> the sum over lanes of value `lane`
 __device__ __forceinline__ float sum_to_lane(float (&v)[32], int lane) {
 #pragma unroll
@@ -109,13 +119,15 @@ __device__ __forceinline__ float sum_to_lane(float (&v)[32], int lane) {
   return v[0];
 }
 
-template <typename T, int E, int R, int MODE>
-__global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
+template <typename T, int E, int R, int MODE, bool MMA>
+__global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : (MMA ? 4 : 3))
     rows_kernel(const __grid_constant__ b200_attention a, const __grid_constant__ Io io) {
-  constexpr int KEYS = 32 / R;
+  static_assert(!MMA || (MODE == FWD && sizeof(T) == 2), "queries of bf16");
+  // tokens of a step, lanes that share a row's scores
+  constexpr int KEYS = MMA ? 8 : 32 / R, LANES = MMA ? 4 : KEYS;
   extern __shared__ __align__(16) uint8_t smem[];
-  float* s_p = reinterpret_cast<float*>(smem);             // [WARPS][2][32]: p or corrections; dz
-  float* s_join = s_p + WARPS * 64;                        // [WARPS][R][32 E] (DKV: twice), then FWD's m and l [WARPS][R] each
+  float* s_p = reinterpret_cast<float*>(smem);             // [WARPS][AREA]: p; corrections or dz
+  float* s_join = s_p + WARPS * AREA;                        // [WARPS][R][32 E] (DKV: twice), then FWD's m and l [WARPS][R] each
   constexpr int JOIN = WARPS * R * 32 * E * (MODE == DKV ? 2 : 1) + 2 * WARPS * R;
   float* s_near = s_join + JOIN;                           // DQ with a table: [WARPS][2 far + 1] sums by rel
   const int far = a.table ? relative::far_of(a.relative) : 0;
@@ -143,11 +155,11 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
   auto row_head = [&](int r) { return MODE == FWD ? kvh * group + (rb * R + r) % group : hy; };
   const int row_end = MODE == DKV ? seq.keys : seq.queries;  // rows inside the sequence
 
-  // this lane's score is row lr, token lk of a step
-  const int lr = lane / KEYS, lk = lane % KEYS;
+  // this lane's score is row lr, token lk of a step (MMA: tokens 2 lk and 2 lk + 1)
+  const int lr = lane / LANES, lk = lane % LANES;
   const int my_row = MODE == DKV ? rb * R + lr : row_query(lr);
   const int my_head = MODE == DKV ? 0 : row_head(lr);
-  const bool my_in = my_row < row_end;
+  const bool my_in = my_row < row_end && lr < R;
   int lo, hi;  // tokens that this lane's row takes part with
   if (MODE == DKV) lo = my_in ? seq.first_query(a, my_row) : 0, hi = my_in ? seq.end_query(a, my_row) : 0;
   else lo = my_in ? seq.first_key(a, my_row) : 0, hi = my_in ? seq.end_key(a, my_row) : 0;
@@ -176,7 +188,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
       }
     } else {
       const int i = row_query(r), h = row_head(r);
-      if (i < row_end) {
+      if (!MMA && i < row_end) {
         load_row<T, E>(x1[r], q + i * a.q_stride[1] + h * a.q_stride[2], c, dim, io.vec);
         if constexpr (MODE == DQ) load_row<T, E>(x2[r], dout + i * io.dout_stride[1] + h * io.dout_stride[2], c, dim, io.vec);
       }
@@ -192,8 +204,101 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
     if (my_lse == -INFINITY) my_lse = INFINITY;  // sees nothing: p = 0
     my_delta = io.delta[(b * a.heads + my_head) * io.padded + my_row];
   }
-  float* sp = s_p + warp * 64;
+  float* sp = s_p + warp * AREA;
 
+  if constexpr (MMA) {
+    // S = Q K^T of 8 rows and 8 tokens by mma.m16n8k16 (rows 8 to 15 are zeros). The order of the products' elements is free: lane
+    // (g, t) = (lane / 4, lane % 4) brings 16 bytes of token g's elements 32 j + 8 t .. + 7 and has the same ones of row g, which
+    // are two K steps of 16 elements. So a token goes from its load to the tensor core as it is.
+    const int g8 = lane >> 2, t8 = lane & 3;
+    uint4 qf[E], kf[E];
+    Token<T, E> y2[KEYS];
+    auto piece = [&](const T* p, int j) {  // zeros for rows, the first elements again for tokens, behind the head's end
+      const int d = 32 * j + 8 * t8;
+      return *reinterpret_cast<const uint4*>(p + (d < dim ? d : 0));
+    };
+    {
+      const int i = row_query(min(g8, R - 1)), h = row_head(min(g8, R - 1));
+      const bool in = g8 < R && i < row_end;
+      const T* p = q + (in ? i * a.q_stride[1] + h * a.q_stride[2] : 0);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        qf[j] = make_uint4(0, 0, 0, 0);
+        if (in && 32 * j + 8 * t8 < dim) qf[j] = piece(p, j);
+      }
+    }
+    auto load1 = [&](int t) {
+      const T* p = k + min(t + g8, end - 1) * a.k_stride[1];
+#pragma unroll
+      for (int j = 0; j < E; ++j) kf[j] = piece(p, j);
+    };
+    auto load2 = [&](int t) {
+#pragma unroll
+      for (int n = 0; n < KEYS; ++n) y2[n].load(v + min(t + n, end - 1) * a.v_stride[1], c, dim, 1);
+    };
+    int t0 = first + warp * KEYS;
+    if (t0 < end) load1(t0), load2(t0);
+    for (; t0 < end; t0 += WARPS * KEYS) {
+      const bool more = t0 + WARPS * KEYS < end;
+      float d0 = 0.f, d1 = 0.f, d2 = 0.f, d3 = 0.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        mma_16x8(d0, d1, d2, d3, qf[j].x, qf[j].y, kf[j].x, kf[j].y);
+        mma_16x8(d0, d1, d2, d3, qf[j].z, qf[j].w, kf[j].z, kf[j].w);
+      }
+      if (more) load1(t0 + WARPS * KEYS);
+      float s[2] = {d0 * sl, d1 * sl};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int j = t0 + 2 * t8 + u;
+        const bool seen = j < end && j >= lo && j < hi;
+        if (a.table && seen)
+          s[u] += table_log2(a.table, (int64_t)s_bucket[max(-far, min(far, j - my_row - seq.shift)) + far] * a.heads + my_head, a.table_dtype);
+        if (!seen) s[u] = -INFINITY;
+      }
+      float top = fmaxf(s[0], s[1]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = fmaxf(m, top);
+      const float base = top == -INFINITY ? 0.f : top;
+      const float p0 = exp2f(s[0] - base), p1 = exp2f(s[1] - base), fix = exp2f(m - base);
+      const bool grown = __any_sync(0xffffffffu, top != m);
+      l = l * fix + (p0 + p1);
+      m = top;
+      __syncwarp();
+      if (g8 < R) {
+        *reinterpret_cast<float2*>(sp + g8 * KEYS + 2 * t8) = make_float2(p0, p1);
+        if (t8 == 0) sp[64 + g8] = fix;
+      }
+      __syncwarp();
+      if (grown) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float f = sp[64 + r];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[r][e] *= f;
+        }
+      }
+#pragma unroll
+      for (int n0 = 0; n0 < KEYS; n0 += 4) {
+        float4 f[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) f[r] = *reinterpret_cast<const float4*>(sp + r * KEYS + n0);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          float y[E];
+          y2[n0 + n].get(y);
+#pragma unroll
+          for (int r = 0; r < R; ++r) {
+            const float w = n == 0 ? f[r].x : (n == 1 ? f[r].y : (n == 2 ? f[r].z : f[r].w));
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[r][e] = fmaf(w, y[e], acc[r][e]);
+          }
+        }
+      }
+      if (more) load2(t0 + WARPS * KEYS);
+    }
+  } else {
   constexpr int WORDS = Token<T, E>::WORDS;
   // both sides' tokens are on their way before the first product where registers allow; forward, the next step's as soon as
   // this one's are used up
@@ -361,6 +466,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
       }
     }
   }
+  }
 
   // the warps' results joined, in order
   float *jm = s_join + JOIN - 2 * WARPS * R, *jl = jm + WARPS * R;
@@ -373,8 +479,8 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : 3)
     }
   if constexpr (MODE == FWD) {
 #pragma unroll
-    for (int o = KEYS / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    if (lk == 0) jm[warp * R + lr] = m, jl[warp * R + lr] = l;
+    for (int o = LANES / 2; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    if (lk == 0 && lr < R) jm[warp * R + lr] = m, jl[warp * R + lr] = l;
   }
   if constexpr (MODE == DQ) {
     if (a.table) {
@@ -530,19 +636,19 @@ static Shape forward_shape(const b200_attention& a) {
 
 template <int MODE>
 static size_t shared_bytes(const b200_attention& a, int R, int E) {
-  size_t n = WARPS * 64 + (size_t)WARPS * R * 32 * E * (MODE == DKV ? 2 : 1) + 2 * WARPS * R;
+  size_t n = WARPS * AREA + (size_t)WARPS * R * 32 * E * (MODE == DKV ? 2 : 1) + 2 * WARPS * R;
   const size_t bins = a.table ? 2 * relative::far_of(a.relative) + 1 : 0;
   if (MODE == DQ) n += WARPS * bins;
   return n * sizeof(float) + bins;
 }
 
-template <typename T, int E, int R, int MODE>
+template <typename T, int E, int R, int MODE, bool MMA = false>
 static int launch(const b200_attention& a, const Io& io, dim3 grid, cudaStream_t st) {
   const size_t shared = shared_bytes<MODE>(a, R, E);
-  const auto kernel = rows_kernel<T, E, R, MODE>;
+  const auto kernel = rows_kernel<T, E, R, MODE, MMA>;
   if (shared > 48 * 1024) {
     // the largest that any call needs, so that calls of several threads do not lower it
-    const size_t most = sizeof(float) * (WARPS * 64 + WARPS * R * 32 * E * 2 + 2 * WARPS * R + WARPS * (2 * B200_RELATIVE_MAX_FAR + 1)) + 2 * B200_RELATIVE_MAX_FAR + 1;
+    const size_t most = sizeof(float) * (WARPS * AREA + WARPS * R * 32 * E * 2 + 2 * WARPS * R + WARPS * (2 * B200_RELATIVE_MAX_FAR + 1)) + 2 * B200_RELATIVE_MAX_FAR + 1;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) return check_launch("attention");
   }
   kernel<<<grid, THREADS, shared, st>>>(a, io);
@@ -551,6 +657,15 @@ static int launch(const b200_attention& a, const Io& io, dim3 grid, cudaStream_t
 
 template <typename T, int E, int MODE>
 static int launch_r(const b200_attention& a, const Io& io, int R, dim3 grid, cudaStream_t st) {
+  if constexpr (MODE == FWD && sizeof(T) == 2) {
+    // whole 16-byte pieces of a head
+    if (io.vec && a.dim % 8 == 0) {
+      if (R == 1) return launch<T, E, 1, MODE, true>(a, io, grid, st);
+      if (R == 2) return launch<T, E, 2, MODE, true>(a, io, grid, st);
+      if (R == 4) return launch<T, E, 4, MODE, true>(a, io, grid, st);
+      if constexpr (E < 8) return launch<T, E, 8, MODE, true>(a, io, grid, st);
+    }
+  }
   if constexpr (E < 8)
     if (R == 8) return launch<T, E, 8, MODE>(a, io, grid, st);
   if constexpr (MODE == FWD) {
