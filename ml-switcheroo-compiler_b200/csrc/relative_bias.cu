@@ -12,16 +12,17 @@
 // workspace, and a second launch adds the blocks up in order.
 #include <algorithm>
 
+#include "ew_common.cuh"
 #include "relative.cuh"
 
 namespace b200 {
 namespace relative {
 
-constexpr int THREADS = 256, PIECE = 16384;  // elements a block writes
+constexpr int THREADS = 256, PIECE = 32768;  // elements a block writes
 
 template <typename T>
-__global__ void __launch_bounds__(THREADS)
-    bias_kernel(const __grid_constant__ b200_relative r, const T* table, T* out, int heads, int64_t plane, int keys, int shift) {
+__global__ void __launch_bounds__(THREADS) bias_kernel(const __grid_constant__ b200_relative r, const T* table, T* out, int heads, int64_t plane, int keys,
+                                                       int shift, uint32_t mul, uint32_t shr) {
   extern __shared__ __align__(16) uint8_t smem[];
   T* lut = reinterpret_cast<T*>(smem);  // by rel + far
   const int far = far_of(r), h = blockIdx.y;
@@ -32,36 +33,44 @@ __global__ void __launch_bounds__(THREADS)
   // the first element of the plane on a 16-byte boundary; pieces start there, the first one takes what is before it
   const int64_t lead = min(plane, (int64_t)((16 - (reinterpret_cast<uintptr_t>(base) & 15)) & 15) / (int64_t)sizeof(T));
   const int64_t begin = lead + (int64_t)blockIdx.x * PIECE, end = min(plane, begin + PIECE);
-  auto value = [&](int64_t i, int j) { return lut[(int)max((int64_t)-far, min((int64_t)far, j - i - shift)) + far]; };
-  if (blockIdx.x == 0 && threadIdx.x < lead) base[threadIdx.x] = value(threadIdx.x / keys, threadIdx.x % keys);
+  auto value = [&](int rel) { return lut[max(-far, min(far, rel)) + far]; };
+  if (blockIdx.x == 0 && threadIdx.x < lead) base[threadIdx.x] = value((int)(threadIdx.x % keys) - (int)(threadIdx.x / keys) - shift);
   if (begin >= end) return;
-  const int64_t row0 = begin / keys;
-  const int col0 = (int)(begin - row0 * keys);  // < keys; PIECE more fit 32 bits
-  for (int o = threadIdx.x * VEC; o < PIECE; o += THREADS * VEC) {
-    const int64_t e = begin + o;
-    if (e >= end) break;
-    const uint32_t at = (uint32_t)col0 + (uint32_t)o;
-    int64_t i = row0 + at / (uint32_t)keys;
-    int j = (int)(at % (uint32_t)keys);
-    const int64_t rel = j - i - shift;
+  const int row0 = (int)(begin / keys), col0 = (int)(begin - (int64_t)row0 * keys);
+  const int n = (int)(end - begin);
+  for (int o = threadIdx.x * VEC; o < n; o += THREADS * VEC) {
+    const uint32_t at = (uint32_t)(col0 + o);  // < keys + PIECE
+    const uint32_t down = fast_div(at, mul, shr);
+    int j = (int)(at - down * (uint32_t)keys);
+    int rel = j - (row0 + (int)down) - shift;
     union {
       uint4 v;
       T t[VEC];
     } u;
-    if (j + VEC <= keys && (rel >= far || rel + VEC - 1 <= -far)) {
-      const T c = lut[rel >= far ? 2 * far : 0];
+    if (j + VEC <= keys) {
+      if (rel >= far || rel + VEC - 1 <= -far) {
+        const T c = lut[rel >= far ? 2 * far : 0];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) u.t[k] = c;
+        for (int k = 0; k < VEC; ++k) u.t[k] = c;
+      } else {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) u.t[k] = value(rel + k);
+      }
     } else {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        u.t[k] = value(i, j);
-        if (++j == keys) j = 0, ++i;
+        u.t[k] = value(rel);
+        ++rel;
+        if (++j == keys) j = 0, rel -= keys + 1;
       }
     }
-    if (e + VEC <= end) *reinterpret_cast<uint4*>(base + e) = u.v;
-    else
-      for (int k = 0; e + k < end; ++k) base[e + k] = u.t[k];
+    if (o + VEC <= n) {
+      *reinterpret_cast<uint4*>(base + begin + o) = u.v;
+    } else {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        if (o + k < n) base[begin + o + k] = u.t[k];
+    }
   }
 }
 
@@ -97,28 +106,41 @@ __global__ void __launch_bounds__(THREADS) bias_grad_kernel(const __grid_constan
   float before = 0.f, after = 0.f;  // rel <= -far, rel >= far
   // diagonal c: column c - (n - 1) + k in row i0 + k
   const int first = blockIdx.x * WIDE, last = min(first + WIDE, keys + n - 1);
-  for (int c = first + (int)threadIdx.x; c < last; c += THREADS) {
-    const int j0 = c - (n - 1);
-    const int k0 = max(0, -j0), k1 = min(n, keys - j0);
-    float s = 0.f;
+  constexpr int WAYS = 2;  // diagonals of a thread at once
+  for (int c = first + (int)threadIdx.x; c < last; c += WAYS * THREADS) {
+    float s[WAYS] = {};
     for (int64_t b = 0; b < batch; ++b) {
-      const T* p = d + (b * heads + h) * plane + (int64_t)i0 * keys + j0;
-      float t[4] = {0.f, 0.f, 0.f, 0.f};
-      int k = k0;
-      for (; k + 8 <= k1; k += 8) {
-        float v[8];
+      const T* p = d + (b * heads + h) * plane + (int64_t)i0 * keys + (c - (n - 1));
+      for (int k = 0; k < n; k += 16) {  // 32 loads under way
+        float v[WAYS][16];
 #pragma unroll
-        for (int u = 0; u < 8; ++u) v[u] = as_float(p[(int64_t)(k + u) * (keys + 1)]);
+        for (int w = 0; w < WAYS; ++w) {
+          const int j = c + w * THREADS - (n - 1) + k;  // the column of row k
+          const bool in = c + w * THREADS < last;
+          const T* q = p + w * THREADS + (int64_t)k * (keys + 1);
 #pragma unroll
-        for (int u = 0; u < 8; ++u) t[u & 3] += v[u];
+          for (int u = 0; u < 16; ++u) {
+            v[w][u] = in && k + u < n && j + u >= 0 && j + u < keys ? as_float(*q) : 0.f;
+            q += keys + 1;
+          }
+        }
+#pragma unroll
+        for (int w = 0; w < WAYS; ++w) {
+          float t[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int u = 0; u < 16; ++u) t[u & 3] += v[w][u];
+          s[w] += (t[0] + t[1]) + (t[2] + t[3]);
+        }
       }
-      for (; k < k1; ++k) t[0] += as_float(p[(int64_t)k * (keys + 1)]);
-      s += (t[0] + t[1]) + (t[2] + t[3]);
     }
-    const int rel = j0 - i0 - shift;  // |.| < 2^31: checked on the host
-    if (rel >= far) after += s;
-    else if (rel <= -far) before += s;
-    else near[rel + far] = s;  // this thread's alone
+#pragma unroll
+    for (int w = 0; w < WAYS; ++w) {
+      if (c + w * THREADS >= last) break;
+      const int rel = c + w * THREADS - (n - 1) - i0 - shift;  // |.| < 2^31: checked on the host
+      if (rel >= far) after += s[w];
+      else if (rel <= -far) before += s[w];
+      else near[rel + far] = s[w];  // this thread's alone
+    }
   }
   before = warp_sum(before), after = warp_sum(after);
   if ((threadIdx.x & 31) == 0) edge[0][threadIdx.x >> 5] = before, edge[1][threadIdx.x >> 5] = after;
@@ -174,12 +196,14 @@ extern "C" int b200_relative_bias(const b200_relative* r, int dtype, const void*
   const int64_t plane = queries * keys;
   const dim3 grid((unsigned)std::max<int64_t>(1, ceil_div(plane, PIECE)), (unsigned)heads);
   const size_t shared = (size_t)(2 * far_of(*r) + 1) * (dtype == B200_F32 ? 4 : 2);
+  uint32_t mul, shr;
+  fastdiv_params((uint32_t)keys, mul, shr);
   if (dtype == B200_F32)
     bias_kernel<float><<<grid, relative::THREADS, shared, as_stream(stream)>>>(*r, (const float*)table, (float*)out, (int)heads, plane, (int)keys,
-                                                                     (int)shift);
+                                                                     (int)shift, mul, shr);
   else
     bias_kernel<__nv_bfloat16><<<grid, relative::THREADS, shared, as_stream(stream)>>>(*r, (const __nv_bfloat16*)table, (__nv_bfloat16*)out,
-                                                                             (int)heads, plane, (int)keys, (int)shift);
+                                                                             (int)heads, plane, (int)keys, (int)shift, mul, shr);
   return check_launch("relative_bias");
 }
 
