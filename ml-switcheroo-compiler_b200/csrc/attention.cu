@@ -37,41 +37,61 @@ static int check_attention(const char* what, const b200_attention* a) {
   return B200_OK;
 }
 
-// What the gradient needs of each query beside its own row: delta = dout . out, and lse in the log2 domain, infinite where the
-// query sees nothing or is none (so that p = 0). [batch x heads][padded]; 8 lanes a query, two 16-byte pieces of both rows in flight a lane.
+// What the gradient needs of each query beside its own row, negated: delta = dout . out, and lse in the log2 domain, infinite where
+// the query sees nothing or is none (so that p = 0). [batch x heads][padded]; 8 lanes a query, FOUR queries of theirs under way.
+constexpr int FOUR = 4;
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200_attention a, const T* dout, const T* out, const float* lse, int64_t sb,
-                                                    int64_t ss, int64_t sh, float* lse2, float* delta, int64_t padded, int vec) {
-  const int64_t row = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3;  // [batch, padded, heads]
-  const int lane = threadIdx.x & 7;
-  const bool in = row < a.batch * padded * a.heads;
-  float s = 0.f, e = INFINITY;
-  int64_t h = 0, i = 0, b = 0;
-  if (in) {
-    h = row % a.heads, i = row / a.heads % padded, b = row / a.heads / padded;
-    if (i < Sequence(a, b).queries) {
-      const T *x = dout + b * sb + i * ss + h * sh, *y = out + ((b * a.queries + i) * a.heads + h) * a.dim;
-      e = lse[(b * a.heads + h) * a.queries + i] * LOG2E;
-      if (e == -INFINITY) e = INFINITY;
-      constexpr int V = 16 / sizeof(T);
-#pragma unroll 2
-      for (int c = lane * V; c < a.dim; c += 8 * V) {
-        if (vec) {
-          const uint4 u = *reinterpret_cast<const uint4*>(x + c), w = *reinterpret_cast<const uint4*>(y + c);
-          const T *p = reinterpret_cast<const T*>(&u), *q = reinterpret_cast<const T*>(&w);
+                                                    int64_t ss, int64_t sh, float* lse2, float* delta, int padded, int vec) {
+  const int64_t b = blockIdx.y;
+  const int lane = threadIdx.x & 7, heads = (int)a.heads, dim = (int)a.dim;
+  const uint32_t rows = (uint32_t)padded * (uint32_t)heads;  // [padded, heads]
+  const uint32_t row0 = blockIdx.x * (32u * FOUR) + (threadIdx.x >> 3);
+  const int queries = Sequence(a, b).queries;
+  constexpr int V = 16 / sizeof(T);
+  float s[FOUR], e[FOUR];
+  uint32_t h[FOUR], i[FOUR];
+  const T *x[FOUR], *y[FOUR];
 #pragma unroll
-          for (int k = 0; k < V; ++k) s = fmaf((float)p[k], (float)q[k], s);
-        } else {  // the same elements in the same order
-          for (int k = 0; k < V && c + k < a.dim; ++k) s = fmaf((float)x[c + k], (float)y[c + k], s);
+  for (int n = 0; n < FOUR; ++n) {
+    const uint32_t row = row0 + 32u * n;
+    i[n] = row / (uint32_t)heads, h[n] = row - i[n] * (uint32_t)heads;
+    s[n] = 0.f, e[n] = -INFINITY;
+    // a row that is none reads the last one's: no load waits behind a branch
+    const int64_t at = min(i[n], (uint32_t)max(queries - 1, 0));
+    x[n] = dout + b * sb + at * ss + h[n] * sh, y[n] = out + ((b * a.queries + at) * heads + h[n]) * dim;
+    if (queries > 0) e[n] = lse[(b * heads + h[n]) * a.queries + at] * -LOG2E;
+  }
+  if (queries > 0) {
+    for (int c = lane * V; c < dim; c += 8 * V) {
+      if (vec) {
+        uint4 u[FOUR], w[FOUR];
+#pragma unroll
+        for (int n = 0; n < FOUR; ++n) u[n] = *reinterpret_cast<const uint4*>(x[n] + c), w[n] = *reinterpret_cast<const uint4*>(y[n] + c);
+#pragma unroll
+        for (int n = 0; n < FOUR; ++n) {
+          const T *p = reinterpret_cast<const T*>(&u[n]), *q = reinterpret_cast<const T*>(&w[n]);
+#pragma unroll
+          for (int k = 0; k < V; ++k) s[n] = fmaf((float)p[k], (float)q[k], s[n]);
         }
+      } else {  // the same elements in the same order
+        for (int n = 0; n < FOUR; ++n)
+          for (int k = 0; k < V && c + k < dim; ++k) s[n] = fmaf((float)x[n][c + k], (float)y[n][c + k], s[n]);
       }
     }
   }
 #pragma unroll
-  for (int o = 4; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if (in && lane == 0) {
-    delta[(b * a.heads + h) * padded + i] = s;
-    lse2[(b * a.heads + h) * padded + i] = e;
+  for (int n = 0; n < FOUR; ++n)
+    if (e[n] == INFINITY || (int)i[n] >= queries) e[n] = -INFINITY, s[n] = (int)i[n] >= queries ? 0.f : s[n];
+#pragma unroll
+  for (int n = 0; n < FOUR; ++n) {
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) s[n] += __shfl_xor_sync(0xffffffffu, s[n], o);
+    if (row0 + 32u * n < rows && lane == 0) {
+      const int64_t to = (b * heads + h[n]) * padded + i[n];
+      delta[to] = -s[n];
+      lse2[to] = e[n];
+    }
   }
 }
 
@@ -128,15 +148,15 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
                "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
   const int64_t padded = padded_of(*a);
   float *lse2 = reinterpret_cast<float*>(workspace), *delta = lse2 + a->batch * a->heads * padded;
-  const unsigned grid = (unsigned)ceil_div(a->batch * padded * a->heads, 32);
-  B200_REQUIRE(a->batch * padded * a->heads < (1ll << 35), "attention_grad: too many queries");
+  B200_REQUIRE(padded * a->heads < (1ll << 31), "attention_grad: %lld queries of %lld heads are too many", (long long)a->queries, (long long)a->heads);
+  const dim3 grid((unsigned)ceil_div(padded * a->heads, 32 * FOUR), (unsigned)a->batch);
   const int64_t* s = g->dout_stride;
   const int vec = ((reinterpret_cast<uintptr_t>(g->dout) | reinterpret_cast<uintptr_t>(g->out) | (uint64_t)((s[0] | s[1] | s[2] | a->dim) * size)) & 15) == 0;
   if (a->dtype == B200_F32)
-    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, g->lse, s[0], s[1], s[2], lse2, delta, padded, vec);
+    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, g->lse, s[0], s[1], s[2], lse2, delta, (int)padded, vec);
   else
     delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, g->lse, s[0], s[1], s[2], lse2,
-                                                      delta, padded, vec);
+                                                      delta, (int)padded, vec);
   if (int rc = check_launch("attention_grad")) return rc;
   void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
   return tiles_take(*a) ? tiles_grad(*a, *g, lse2, delta, padded, rest, st) : rows_grad(*a, *g, delta, padded, rest, st);

@@ -35,7 +35,7 @@ struct Io {
   float* lse;                   // FWD: written; else read
   const void* dout;
   int64_t dout_stride[3];
-  const float* delta;           // [batch x heads][padded]
+  const float* delta;           // [batch x heads][padded], negated
   int64_t padded;
   float* part;                  // FWD with splits: [row blocks][splits][R][dim + 2]; DQ with a table: [row blocks][buckets]
 };
@@ -202,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : (MMA ? 4 : 3))
     const int64_t at = (b * a.heads + my_head) * a.queries + my_row;
     my_lse = io.lse[at] * LOG2E;
     if (my_lse == -INFINITY) my_lse = INFINITY;  // sees nothing: p = 0
-    my_delta = io.delta[(b * a.heads + my_head) * io.padded + my_row];
+    my_delta = -io.delta[(b * a.heads + my_head) * io.padded + my_row];
   }
   float* sp = s_p + warp * AREA;
 
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : (MMA ? 4 : 3))
           if (seen) {
             lse = io.lse[(b * a.heads + head) * a.queries + i] * LOG2E;
             if (lse == -INFINITY) lse = INFINITY;
-            delta = io.delta[(b * a.heads + head) * io.padded + i];
+            delta = -io.delta[(b * a.heads + head) * io.padded + i];
           }
         }
         const float p = seen ? exp2f(s - lse) : 0.f;

@@ -185,6 +185,14 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// first in a block of code that few tiles run: keeps it behind a branch (as selects of every element it is a third of all
+// instructions)
+__device__ __forceinline__ void seldom() { asm volatile("" ::: "memory"); }
 __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
@@ -412,6 +420,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       }
       const bool cut = j0 < full0 || j0 + 64 > full1;
       if (cut) {
+        seldom();
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -441,14 +450,14 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         m = grown;
       }
       const float base = m == -INFINITY ? 0.f : m;
-      const uint64_t mul2 = pack2(mul, mul), base2 = pack2(-base, -base);
+      const uint64_t mul22 = pack2(mul, mul), base2 = pack2(-base, -base);
       uint64_t sum[2] = {0, 0};  // two zeros each
       uint32_t p[32];
 #pragma unroll
       for (int k = 0; k < 32; ++k) {
         const int c = k >> 4, e = 2 * (k & 15);
         float x, y;
-        unpack2(fma2(pack2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), mul2, base2), x, y);
+        unpack2(fma2(pack2(__uint_as_float(v[c][e]), __uint_as_float(v[c][e + 1])), mul22, base2), x, y);
         x = ex2(x), y = ex2(y);
         sum[k & 1] = add2(sum[k & 1], pack2(x, y));
         p[k] = pack_bf16(x, y);
@@ -523,7 +532,7 @@ struct Bwd {
 };
 
 struct BwdIo {
-  const float *lse, *delta;  // [batch x heads][padded]: log2 (infinite where nothing is seen), and dout . out
+  const float *lse, *delta;  // [batch x heads][padded], both negated: lse in the log2 domain (-inf where nothing is seen), dout . out
   int padded, stages, vec;
   __nv_bfloat16 *d0, *d1;  // dq; or dv and dk
   float* part;             // dq with a table: [batch][heads][row tiles][buckets]
@@ -720,7 +729,7 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
     const uint32_t tm = tmem + ((uint32_t)(q * 32) << 16), t_s = tm + g * 2 * BN;
     const float sl = a.scale * LOG2E;
     const uint64_t sl2 = pack2(sl, sl);
-    float row_lse = INFINITY, row_delta = 0.f, before = 0.f, after = 0.f;
+    float row_lse = -INFINITY, row_delta = 0.f, before = 0.f, after = 0.f;
     if (!DKV && valid) {
       const int64_t from = (b * a.heads + hy) * io.padded + r;
       row_lse = io.lse[from];
@@ -780,6 +789,7 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
             }
           }
         }
+        // p = 2^(x - lse), dz = p (dP - delta), two columns at a time
 #pragma unroll
         for (int k = 0; k < 32; k += 4) {
           float4 ls, de;
@@ -790,15 +800,20 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
             ls = make_float4(row_lse, row_lse, row_lse, row_lse);
             de = make_float4(row_delta, row_delta, row_delta, row_delta);
           }
-          const float l4[4] = {ls.x, ls.y, ls.z, ls.w}, d4[4] = {de.x, de.y, de.z, de.w};
+          const uint64_t l2[2] = {pack2(ls.x, ls.y), pack2(ls.z, ls.w)}, d2[2] = {pack2(de.x, de.y), pack2(de.z, de.w)};
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            const float p = ex2(BIAS ? x[k + u] - l4[u] : fmaf(__uint_as_float(s[k + u]), sl, -l4[u]));
-            x[k + u] = p * (__uint_as_float(d[k + u]) - d4[u]);
-            s[k + u] = __float_as_uint(p);
+          for (int u = 0; u < 2; ++u) {
+            const int e = k + 2 * u;
+            const uint64_t z = BIAS ? add2(pack2(x[e], x[e + 1]), l2[u]) : fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), sl2, l2[u]);
+            float p0, p1;
+            unpack2(z, p0, p1);
+            p0 = ex2(p0), p1 = ex2(p1);
+            unpack2(mul2(pack2(p0, p1), add2(pack2(__uint_as_float(d[e]), __uint_as_float(d[e + 1])), d2[u])), x[e], x[e + 1]);
+            s[e] = __float_as_uint(p0), s[e + 1] = __float_as_uint(p1);
           }
         }
         if (t0 < full0 || t0 + 32 > full1) {
+          seldom();
 #pragma unroll
           for (int k = 0; k < 32; ++k)
             if (t0 + k < lo || t0 + k >= hi) {
