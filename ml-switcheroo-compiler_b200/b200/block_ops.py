@@ -112,13 +112,11 @@ def op_relative_position_bias_grad(dscores, buckets=None, bidirectional=True, ma
 # ----------------------------------------------------------------------------------
 
 
-def _tokens(name: str, what: str, x: torch.Tensor) -> tuple[torch.Tensor, tuple[int, int, int]]:
-    """x [batch, tokens, heads, dim] with adjacent head elements, and its other strides."""
+def _tokens(name: str, what: str, x: torch.Tensor) -> torch.Tensor:
+    """x [batch, tokens, heads, dim] with adjacent head elements."""
     if x.dim() != 4:
         raise ValueError(f"{name}: {what} {tuple(x.shape)}, want [batch, tokens, heads, dim] or [tokens, heads, dim]")
-    if x.stride(3) != 1 and x.shape[3] > 1:
-        x = ops.contiguous(x)
-    return x, x.stride()[:3]
+    return ops.contiguous(x) if x.stride(3) != 1 and x.shape[3] > 1 else x
 
 
 def _lengths(name: str, what: str, n: Any, batch: int) -> torch.Tensor | None:
@@ -136,22 +134,19 @@ def _lengths(name: str, what: str, n: Any, batch: int) -> torch.Tensor | None:
     return ops.contiguous(t)
 
 
-def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, window, max_distance, bidirectional):
-    """(description, the tensors that it points to, whether the batch axis was left out)."""
-    flat = q.dim() == 3
-    if flat:
-        q, k, v = (t.unsqueeze(0) if t.dim() == 3 else t for t in (q, k, v))
-    for t, what in ((q, "queries"), (k, "keys"), (v, "values")):
-        if t.dim() != 4:
-            raise ValueError(f"{name}: {what} {tuple(t.shape)}, want [batch, tokens, heads, dim] or [tokens, heads, dim]")
-        if t.dtype not in _FLOATS:
-            raise BackendNotSupportedError(f"{name}: {what} of {t.dtype} (fp32 and bf16)")
-    b, nq, h, d = q.shape
-    nk, hk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != b or k.shape[3] != d:
-        raise ValueError(f"{name}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)} do not match")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise BackendNotSupportedError(f"{name}: queries of {q.dtype} with keys of {k.dtype} and values of {v.dtype}")
+@functools.lru_cache(maxsize=256)
+def _attention_plan(name, shapes, dtypes, table, scale, causal, window, max_distance, bidirectional) -> L.Attention:
+    """The checks of shapes and types, and what of the description they decide."""
+    for s, d, what in zip(shapes, dtypes, ("queries", "keys", "values")):
+        if len(s) != 4:
+            raise ValueError(f"{name}: {what} {tuple(s)}, want [batch, tokens, heads, dim] or [tokens, heads, dim]")
+        if d not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: {what} of {d} (fp32 and bf16)")
+    (b, nq, h, d), (kb, nk, hk, kd) = shapes[:2]
+    if shapes[1] != shapes[2] or kb != b or kd != d:
+        raise ValueError(f"{name}: queries {tuple(shapes[0])}, keys {tuple(shapes[1])} and values {tuple(shapes[2])} do not match")
+    if dtypes[1] != dtypes[0] or dtypes[2] != dtypes[0]:
+        raise BackendNotSupportedError(f"{name}: queries of {dtypes[0]} with keys of {dtypes[1]} and values of {dtypes[2]}")
     if not 1 <= d <= L.ATTENTION_MAX_DIM:
         raise ValueError(f"{name}: heads of {d} elements (1 to {L.ATTENTION_MAX_DIM})")
     if h < 1 or hk < 1 or h % hk:
@@ -163,29 +158,40 @@ def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, 
         raise ValueError(f"{name}: window {window!r} is not a number of tokens")
     a = L.Attention()
     if table is not None:
-        if table.dim() != 2 or table.shape[1] != h:
-            raise ValueError(f"{name}: position bias {tuple(table.shape)}, want [buckets, {h} heads]")
-        if table.dtype not in _FLOATS:
-            raise BackendNotSupportedError(f"{name}: position bias of {table.dtype} (fp32 and bf16)")
-        a.relative = _relative(table.shape[0], int(max_distance), not causal if bidirectional is None else bool(bidirectional))
-    _on_device(name, q, k, v, table)
-    lengths, query_lengths = _lengths(name, "lengths", lengths, b), _lengths(name, "query_lengths", query_lengths, b)
-    if lengths is not None and query_lengths is not None and lengths.dtype != query_lengths.dtype:
-        lengths, query_lengths = (ops.cast(t, torch.int64) for t in (lengths, query_lengths))
-    q, qs = _tokens(name, "queries", q)
-    k, ks = _tokens(name, "keys", k)
-    v, vs = _tokens(name, "values", v)
+        shape, dtype = table
+        if len(shape) != 2 or shape[1] != h:
+            raise ValueError(f"{name}: position bias {tuple(shape)}, want [buckets, {h} heads]")
+        if dtype not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: position bias of {dtype} (fp32 and bf16)")
+        a.relative = _relative(shape[0], int(max_distance), not causal if bidirectional is None else bool(bidirectional))
+        a.table_dtype = ops._TORCH2CODE[dtype]
     a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim = b, nq, nk, h, hk, d
-    a.window, a.causal, a.scale, a.dtype = int(window or 0), int(bool(causal)), scale, ops.code(q)
-    for n in (lengths, query_lengths):
-        if n is not None:
-            a.length_dtype = ops.code(n)
+    a.window, a.causal, a.scale, a.dtype = int(window or 0), int(bool(causal)), scale, ops._TORCH2CODE[dtypes[0]]
+    return a
+
+
+def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, window, max_distance, bidirectional):
+    """(description, the tensors that it points to, whether the batch axis was left out)."""
+    flat = q.dim() == 3
+    if flat:
+        q, k, v = (t.unsqueeze(0) if t.dim() == 3 else t for t in (q, k, v))
+    plan = _attention_plan(name, (q.shape, k.shape, v.shape), (q.dtype, k.dtype, v.dtype), None if table is None else (table.shape, table.dtype),
+                           None if scale is None else float(scale), bool(causal), None if window is None else float(window), int(max_distance),
+                           None if bidirectional is None else bool(bidirectional))
+    a = L.Attention.from_buffer_copy(plan)
+    _on_device(name, q, k, v, table)
+    q, k, v = _tokens(name, "queries", q), _tokens(name, "keys", k), _tokens(name, "values", v)
+    if lengths is not None or query_lengths is not None:
+        lengths, query_lengths = (_lengths(name, what, n, q.shape[0]) for n, what in ((lengths, "lengths"), (query_lengths, "query_lengths")))
+        if lengths is not None and query_lengths is not None and lengths.dtype != query_lengths.dtype:
+            lengths, query_lengths = (ops.cast(t, torch.int64) for t in (lengths, query_lengths))
+        a.length_dtype = ops.code(query_lengths if lengths is None else lengths)
+        a.lengths, a.query_lengths = ops._ptr(lengths), ops._ptr(query_lengths)
     if table is not None:
         table = ops.contiguous(table)
-        a.table, a.table_dtype = table.data_ptr(), ops.code(table)
-    a.lengths, a.query_lengths = ops._ptr(lengths), ops._ptr(query_lengths)
+        a.table = table.data_ptr()
     a.q, a.k, a.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    a.q_stride[:], a.k_stride[:], a.v_stride[:] = qs, ks, vs
+    a.q_stride[:], a.k_stride[:], a.v_stride[:] = q.stride()[:3], k.stride()[:3], v.stride()[:3]
     return a, (q, k, v, lengths, query_lengths, table), flat
 
 
@@ -213,10 +219,10 @@ def op_fused_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=
     name = "FusedAttention"
     a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
     x = kept[0]
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    lse = torch.empty(a.batch, a.heads, a.queries, dtype=torch.float32, device=x.device)
+    out = x.new_empty(x.shape)
+    lse = x.new_empty((a.batch, a.heads, a.queries), dtype=torch.float32)
     wn = L.lib().b200_attention_workspace_bytes(a)
-    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    ws = x.new_empty(wn, dtype=torch.uint8) if wn else None
     L.call("b200_attention_forward", a, out.data_ptr(), lse.data_ptr(), ops._ptr(ws), wn, ops.stream_ptr())
     return (out[0], lse[0]) if flat else (out, lse)
 
@@ -240,16 +246,15 @@ def op_fused_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths
     if tuple(lse.shape) != want or lse.dtype != torch.float32:
         raise ValueError(f"{name}: lse {tuple(lse.shape)} of {lse.dtype}, want fp32 {want}")
     _on_device(name, dout, out, lse)
-    dout, ds = _tokens(name, "gradient", dout.unsqueeze(0) if flat else dout)
+    dout = _tokens(name, "gradient", dout.unsqueeze(0) if flat else dout)
     out, lse = ops.contiguous(out), ops.contiguous(lse)
     g = L.AttentionGrads()
-    dq = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dk, dv = (torch.empty(y.shape, dtype=y.dtype, device=y.device) for _ in range(2))
-    dtable = None if table is None else torch.empty(table.shape, dtype=table.dtype, device=table.device)
-    g.dout, g.out, g.lse, g.dout_stride[:] = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), ds
+    dq, dk, dv = x.new_empty(x.shape), y.new_empty(y.shape), y.new_empty(y.shape)
+    dtable = None if table is None else table.new_empty(table.shape)
+    g.dout, g.out, g.lse, g.dout_stride[:] = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.stride()[:3]
     g.dq, g.dk, g.dv, g.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ops._ptr(dtable)
     wn = L.lib().b200_attention_grad_workspace_bytes(a)
-    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    ws = x.new_empty(wn, dtype=torch.uint8) if wn else None
     L.call("b200_attention_grad", a, g, ops._ptr(ws), wn, ops.stream_ptr())
     return (dq[0], dk[0], dv[0], dtable) if flat else (dq, dk, dv, dtable)
 
@@ -261,60 +266,69 @@ def op_fused_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths
 _NORMS = {"rms": 0, "layer": 1}
 
 
-def _residual(name: str, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps):
-    """(description, x, f, the weights as the kernels take them)."""
-    if x.shape != f.shape or x.dim() < 1:
-        raise ValueError(f"{name}: residual stream {tuple(x.shape)} and block output {tuple(f.shape)} differ")
-    for t, what in ((x, "residual stream"), (f, "block output")):
-        if t.dtype not in _FLOATS:
-            raise BackendNotSupportedError(f"{name}: {what} of {t.dtype} (fp32 and bf16)")
+@functools.lru_cache(maxsize=256)
+def _residual_plan(name, shape, f_shape, x_dtype, f_dtype, weights, gate, residual_scale, norm, post_norm, eps) -> L.ResidualNorm:
+    """The checks of shapes and types (weights, gate: (shape, dtype) or None), and what of the description they decide."""
+    if shape != f_shape or len(shape) < 1:
+        raise ValueError(f"{name}: residual stream {tuple(shape)} and block output {tuple(f_shape)} differ")
+    for d, what in ((x_dtype, "residual stream"), (f_dtype, "block output")):
+        if d not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: {what} of {d} (fp32 and bf16)")
     if norm not in _NORMS:
         raise ValueError(f"{name}: norm {norm!r} is not one of {sorted(_NORMS)}")
-    width = x.shape[-1]
+    width = shape[-1]
     if not 1 <= width <= L.RESIDUAL_NORM_MAX_COLS:
         raise ValueError(f"{name}: rows of {width} elements (1 to {L.RESIDUAL_NORM_MAX_COLS})")
-    post = post_gamma is not None or post_beta is not None if post_norm is None else bool(post_norm)
-    if not post and (post_gamma is not None or post_beta is not None):
+    given = weights[2] is not None or weights[3] is not None
+    post = given if post_norm is None else bool(post_norm)
+    if given and not post:
         raise ValueError(f"{name}: post weights without a post norm")
-    if norm != "layer" and (beta is not None or post_beta is not None):
+    if norm != "layer" and (weights[1] is not None or weights[3] is not None):
         raise ValueError(f"{name}: an RMS norm has no beta")
     if not math.isfinite(residual_scale):
         raise ValueError(f"{name}: residual_scale {residual_scale} is not finite")
-    weights = [gamma, beta, post_gamma, post_beta]
     for w in weights:
         if w is not None:
-            if tuple(w.shape) != (width,):
-                raise ValueError(f"{name}: norm weight {tuple(w.shape)}, want [{width}]")
-            if w.dtype not in _FLOATS:
-                raise BackendNotSupportedError(f"{name}: norm weights of {w.dtype} (fp32 and bf16)")
-    groups = 0
-    if gate is not None:
-        if gate.dtype not in _FLOATS:
-            raise BackendNotSupportedError(f"{name}: gate of {gate.dtype} (fp32 and bf16)")
-        lead = tuple(x.shape[:-1])
-        shape = (1,) * (x.dim() - gate.dim()) + tuple(gate.shape)
-        # leading axes in full, then axes of one: consecutive rows share a gate
-        n = next((i for i in range(len(lead)) if len(shape) == x.dim() and shape[i] != lead[i]), len(lead))
-        if len(shape) != x.dim() or shape[-1] != width or any(s != 1 for s in shape[n:-1]):
-            raise ValueError(f"{name}: gate {tuple(gate.shape)} of {tuple(x.shape)}: want leading axes in full, then ones, then {width}")
-        groups = math.prod(shape[:n])
-    _on_device(name, x, f, gate, *weights)
-    x, f = ops.contiguous(x), ops.contiguous(f)
-    given = [w for w in weights if w is not None]
-    if len({w.dtype for w in given}) > 1:
-        weights = [None if w is None else ops.cast(w, torch.float32) for w in weights]
-    weights = [None if w is None else ops.contiguous(w) for w in weights]
-    gate = None if gate is None else ops.contiguous(gate)
+            if tuple(w[0]) != (width,):
+                raise ValueError(f"{name}: norm weight {tuple(w[0])}, want [{width}]")
+            if w[1] not in _FLOATS:
+                raise BackendNotSupportedError(f"{name}: norm weights of {w[1]} (fp32 and bf16)")
     d = L.ResidualNorm()
-    d.rows, d.cols = math.prod(x.shape[:-1]), width
-    d.groups = groups if d.rows else 0
-    d.kind, d.post, d.scale, d.eps = _NORMS[norm], int(post), float(residual_scale), float(eps)
-    d.x_dtype, d.f_dtype = ops.code(x), ops.code(f)
-    d.weight_dtype = next((ops.code(w) for w in weights if w is not None), L.F32)
-    d.gamma, d.beta, d.post_gamma, d.post_beta = (ops._ptr(w) for w in weights)
     if gate is not None:
-        d.gate_dtype, d.gate = ops.code(gate), gate.data_ptr() if d.rows else None
-    return d, x, f, weights, gate
+        if gate[1] not in _FLOATS:
+            raise BackendNotSupportedError(f"{name}: gate of {gate[1]} (fp32 and bf16)")
+        lead = tuple(shape[:-1])
+        g = (1,) * (len(shape) - len(gate[0])) + tuple(gate[0])
+        # leading axes in full, then axes of one: consecutive rows share a gate
+        n = next((i for i in range(len(lead)) if len(g) == len(shape) and g[i] != lead[i]), len(lead))
+        if len(g) != len(shape) or g[-1] != width or any(s != 1 for s in g[n:-1]):
+            raise ValueError(f"{name}: gate {tuple(gate[0])} of {tuple(shape)}: want leading axes in full, then ones, then {width}")
+        d.groups, d.gate_dtype = math.prod(g[:n]), ops._TORCH2CODE[gate[1]]
+    d.rows, d.cols = math.prod(shape[:-1]), width
+    if not d.rows:
+        d.groups = 0
+    d.kind, d.post, d.scale, d.eps = _NORMS[norm], int(post), float(residual_scale), float(eps)
+    d.x_dtype, d.f_dtype = ops._TORCH2CODE[x_dtype], ops._TORCH2CODE[f_dtype]
+    kinds = {w[1] for w in weights if w is not None}
+    d.weight_dtype = L.BF16 if kinds == {torch.bfloat16} else L.F32  # fp32 where they differ
+    return d
+
+
+def _residual(name: str, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps):
+    """(description, x, f, the weights as the kernels take them, the gate)."""
+    weights = (gamma, beta, post_gamma, post_beta)
+    plan = _residual_plan(name, x.shape, f.shape, x.dtype, f.dtype, tuple([None if w is None else (w.shape, w.dtype) for w in weights]),
+                          None if gate is None else (gate.shape, gate.dtype), float(residual_scale), norm, None if post_norm is None else bool(post_norm),
+                          float(eps))
+    _on_device(name, x, f, gate, *weights)
+    d = L.ResidualNorm.from_buffer_copy(plan)
+    kind = torch.bfloat16 if d.weight_dtype == L.BF16 else torch.float32
+    weights = [None if w is None else ops.contiguous(ops.cast(w, kind)) for w in weights]
+    d.gamma, d.beta, d.post_gamma, d.post_beta = [None if w is None else w.data_ptr() for w in weights]
+    if gate is not None:
+        gate = ops.contiguous(gate)
+        d.gate = gate.data_ptr() if d.rows else None
+    return d, ops.contiguous(x), ops.contiguous(f), weights, gate
 
 
 def op_residual_norm(x, f, gamma=None, beta=None, post_gamma=None, post_beta=None, gate=None, residual_scale=1.0, norm="rms",
@@ -330,8 +344,7 @@ def op_residual_norm(x, f, gamma=None, beta=None, post_gamma=None, post_beta=Non
     sequence), or x's shape; None: ones. Computed in fp32, rounded once each."""
     name = "ResidualNorm"
     d, x, f, weights, gate = _residual(name, x, f, gamma, beta, post_gamma, post_beta, gate, residual_scale, norm, post_norm, eps)
-    total = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    normed = torch.empty(f.shape, dtype=f.dtype, device=f.device)
+    total, normed = torch.empty_like(x), torch.empty_like(f)
     L.call("b200_residual_norm_forward", d, x.data_ptr(), f.data_ptr(), total.data_ptr(), normed.data_ptr(), ops.stream_ptr())
     return total, normed
 
@@ -352,14 +365,14 @@ def op_residual_norm_grad(dsum, dnormed, x, f, gamma=None, beta=None, post_gamma
         raise BackendNotSupportedError(f"{name}: gradients of {dsum.dtype}, {dnormed.dtype} for a sum of {x.dtype} and norms of {f.dtype}")
     _on_device(name, dsum, dnormed)
     dsum, dnormed = ops.contiguous(dsum), ops.contiguous(dnormed)
-    dx, df = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (x, f))
-    grads = [None if w is None else torch.empty(w.shape, dtype=w.dtype, device=w.device) for w in weights]
-    dgate = None if gate is None else torch.empty(shape, dtype=gate.dtype, device=gate.device)
+    dx, df = torch.empty_like(x), torch.empty_like(f)
+    grads = [None if w is None else torch.empty_like(w) for w in weights]
+    dgate = None if gate is None else gate.new_empty(shape)
     g = L.ResidualNormGrads()
     g.dgamma, g.dbeta, g.dpost_gamma, g.dpost_beta = (ops._ptr(t) for t in grads)
     g.dgate = ops._ptr(dgate)
     wn = L.lib().b200_residual_norm_grad_workspace_bytes(d)
-    ws = torch.empty(wn, dtype=torch.uint8, device=x.device) if wn else None
+    ws = x.new_empty(wn, dtype=torch.uint8) if wn else None
     L.call("b200_residual_norm_grad", d, dsum.data_ptr(), dnormed.data_ptr(), x.data_ptr(), f.data_ptr(), dx.data_ptr(), df.data_ptr(), g,
            ops._ptr(ws), wn, ops.stream_ptr())
     if dgate is not None and not d.rows:
