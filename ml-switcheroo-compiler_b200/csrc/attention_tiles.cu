@@ -1,15 +1,16 @@
 // Attention on the tensor cores: bf16 heads of up to 128 elements, many queries.
 //
-// Forward. A block takes 128 queries of one head past the keys, 128 at a time; two blocks share an SM, so that one's
-// exponentials run under the other's MMAs, and its start and end under the other's middle:
+// Forward. A block takes 128 queries of one head past the keys; two blocks share an SM, so that one's exponentials run under
+// the other's MMAs, and its start and end under the other's middle:
 //   warp 0      TMA: the queries once, then K and V tiles into a ring;
 //   warp 1      owns 256 columns of TMEM, issues S = Q K^T (operands in shared memory) and O += P V (P from TMEM);
-//   warps 2-9   softmax: two threads own a query's row of S, 64 keys each, and exchange its maximum.
-// Heads of up to 64: S, P and O have columns of their own (128 + 64 + 64), and the next S is made as soon as the threads hold this
-// one in registers. Wider heads: P lies over S (O has 128), whose MMAs, issued behind O's, overwrite it only when it is used up: MMAs
-// run in their order. The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8,
-// sums are fp32), so O is hardly ever rescaled. P is handed over in two halves of 64 keys.
-// Making up to 3 of 8 exponentials on the FMA pipe changed nothing (the special function unit is busy for a third of the time): not done.
+//   the others  softmax, 64 scores a thread.
+// The next tile's S is made under this one's exponentials. Heads of up to 64: tiles of 128 keys, S, P and O in columns of their own (128 + 64 +
+// 64), two threads a row, which exchange its maximum. Wider heads: tiles of 64 keys, two S in turn with P over them, and O
+// (64 + 64 + 128); MMAs run in their order, so an S is overwritten only when the P over it is used up. (With one S of 128 keys and P
+// over it, whose successor had to wait for P, 2 x 4096 causal tokens of 32 heads of 128 took 314 us.) The running maximum moves only
+// when a row's has grown by 2^8 (probabilities stay below 2^8, sums are fp32), so O is hardly ever rescaled.
+// Making up to 3 of 8 exponentials on the FMA pipe changed nothing (the special function unit is busy for 60 % of the time): not done.
 //
 // Backward, one kernel in two forms. 128 rows stay, tiles of 64 tokens of the other side go past:
 //   dq:      rows are queries (Q, dO), tiles are keys (K, V):     S = Q K^T, dP = dO V^T, dQ += dS K
@@ -222,28 +223,27 @@ __device__ __forceinline__ void store32(__nv_bfloat16* row, int col, int dim, bo
 // forward
 // ------------------------------------------------------------------------------------
 
-constexpr int KEYS = 128, FWD_THREADS = 320;
 constexpr float LAZY = 8.f;  // log2 by which a maximum may grow before O is rescaled
 
 template <int DP>
 struct Fwd {
-  static constexpr bool APART = DP == 64;  // P beside S
-  static constexpr int STAGES = DP == 64 ? 2 : 1;
-  static constexpr uint32_t TILE = 128 * DP * 2;
-  static constexpr uint32_t BARS = TILE + STAGES * 2 * TILE;
+  static constexpr int HALVES = DP == 64 ? 2 : 1;  // threads of a row
+  static constexpr int KEYS = 64 * HALVES, THREADS = 64 + 128 * HALVES, STAGES = 2;
+  static constexpr uint32_t Q = ROWS * DP * 2, TILE = KEYS * DP * 2;
+  static constexpr uint32_t BARS = Q + STAGES * 2 * TILE;
   static constexpr uint32_t MAXIMA = BARS + 256, LUT = MAXIMA + 2 * 2 * ROWS * 4;
-  static constexpr uint32_t TMEM = 256, T_P = APART ? 128 : 0, T_O = TMEM - DP;
+  static constexpr uint32_t TMEM = 256, T_O = TMEM - DP;
 };
 
 template <int DP, bool BIAS>
-__global__ void __launch_bounds__(FWD_THREADS, 2)
+__global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
     forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ b200_attention a, const __grid_constant__ Order order, __nv_bfloat16* out, float* lse, int vec) {
   using F = Fwd<DP>;
-  constexpr int ST = F::STAGES;
+  constexpr int ST = F::STAGES, KEYS = F::KEYS, HALVES = F::HALVES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  const uint32_t s_q = smem_u32(smem), s_k = s_q + F::TILE, s_v = s_k + ST * F::TILE;
+  const uint32_t s_q = smem_u32(smem), s_k = s_q + F::Q, s_v = s_k + ST * F::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST,
            *s_free = s_full + 1, *p_full = s_full + 2, *o_done = s_full + 4, *idle = s_full + 5;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
 
   if (warp == 0) {
     if (lane == 0 && n_tiles > 0) {
-      mbar_expect_tx(q_full, F::TILE);
+      mbar_expect_tx(q_full, F::Q);
       for (int p = 0; p < DP / 64; ++p) tma_load_4d(smem + p * (ROWS * 128), &map_q, q_full, p * 64, r0, head, (int)b);
       for (int n = 0; n < n_tiles; ++n) {
         const int s = n % ST;
@@ -307,11 +307,11 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         wait(&k_empty[s], par, gave_up);
         mbar_expect_tx(&k_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
-          tma_load_4d(smem + F::TILE + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
+          tma_load_4d(smem + F::Q + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
         wait(&v_empty[s], par, gave_up);
         mbar_expect_tx(&v_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
-          tma_load_4d(smem + (1 + ST) * F::TILE + s * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
+          tma_load_4d(smem + F::Q + (ST + s) * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
       }
       // every load has landed before the block may end
       wait(q_full, 0, gave_up);
@@ -324,25 +324,27 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     const int ks = (dim + 15) / 16, elected = elect_one();
     const uint32_t id_s = idesc_of(ROWS, KEYS, false), id_o = idesc_of(ROWS, ks * 16, true);
     const Desc dq = desc_at(s_q, 16), dk = desc_at(s_k, 16), dv = desc_at(s_v, KEYS * 128);
-    auto scores = [&](int s, int par) {  // S of the tile in stage s
+    auto scores = [&](int s, int par, int n) {  // S of tile n, in stage s
       warp_wait(&k_full[s], par, gave_up);
       tc_fence_after();
       const Desc kd = {dk.lo + s * (F::TILE >> 4), dk.hi};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        if (k < ks) mma(elected, tmem, dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
+        if (k < ks) mma(elected, tmem + (HALVES == 1 ? (n & 1) * KEYS : 0), dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
       commit(elected, s_full);
       commit(elected, &k_empty[s]);
     };
     if (n_tiles > 0) {
       warp_wait(q_full, 0, gave_up);
-      scores(0, 0);
+      scores(0, 0, 0);
     }
     for (int n = 0, s = 0, par = 0, next = 0, next_par = 0; n < n_tiles; ++n, s = next, par = next_par) {
       next = s + 1 == ST ? 0 : s + 1, next_par = s + 1 == ST ? par ^ 1 : par;
-      if (F::APART && n + 1 < n_tiles) {
-        warp_wait(s_free, n & 1, gave_up);
-        scores(next, next_par);
+      if (n + 1 < n_tiles) {
+        // two threads a row: they hold this tile's scores in registers; else the next S has columns of its own, whose P the sums before
+        // have used up
+        if constexpr (HALVES == 2) warp_wait(s_free, n & 1, gave_up);
+        scores(next, next_par, n + 1);
       }
       warp_wait(&v_full[s], par, gave_up);
       const int have = seq.keys - (T0 + n) * KEYS;
@@ -354,16 +356,15 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       }
       const Desc vd = {dv.lo + s * (F::TILE >> 4), dv.hi};
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
+      for (int h = 0; h < HALVES; ++h) {
         warp_wait(&p_full[h], n & 1, gave_up);
         tc_fence_after();
 #pragma unroll
         for (int k = 4 * h; k < 4 * h + 4; ++k)
-          mma_from_tmem(elected, tmem + F::T_O, tmem + F::T_P + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
+          mma_from_tmem(elected, tmem + F::T_O, tmem + (HALVES == 2 ? KEYS : (n & 1) * KEYS) + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
       }
       commit(elected, &v_empty[s]);
       commit(elected, o_done);
-      if (!F::APART && n + 1 < n_tiles) scores(next, next_par);
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
@@ -375,10 +376,10 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     const int lo = valid ? seq.first_key(a, i) : 0, hi = valid ? seq.end_key(a, i) : 0;
     // every key of [full0, full1) is seen by all rows of the warp
     const int full0 = seq.first_key(a, min(i0 + 31, seq.queries - 1)), full1 = seq.end_key(a, i0);
-    const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16), t_s = t_row + half * 64, t_p = t_row + F::T_P + half * 32, t_o = t_row + F::T_O;
+    const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16), t_o = t_row + F::T_O;
     const float sl = a.scale * LOG2E;
     float m = -INFINITY, l = 0.f;  // the row's maximum, the sum of this thread's keys
-    // this thread's value and that of the row's other thread, which meet at a barrier of their two warps
+    // this thread's value for that of the row's other thread, at a barrier of their two warps
     auto exchange = [&](float x, int parity) {
       float* area = maxima + parity * 2 * ROWS;
       area[half * ROWS + row_at] = x;
@@ -387,6 +388,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     };
     for (int n = 0; n < n_tiles; ++n) {
       const int j0 = (T0 + n) * KEYS + half * 64;
+      const uint32_t t_s = t_row + (HALVES == 2 ? half : n & 1) * 64, t_p = HALVES == 2 ? t_row + KEYS + half * 32 : t_s;
       warp_wait(s_full, n & 1, gave_up);
       tc_fence_after();
       uint32_t v[2][32];
@@ -394,8 +396,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       tmem_ld32_issue(t_s + 32, v[1]);
       tmem_wait(v[0]);
       tmem_wait(v[1]);
-      tc_fence_before();
-      if constexpr (F::APART) {
+      if constexpr (HALVES == 2) {
+        tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(s_free);
       }
@@ -439,8 +441,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         tops[c] = fmaxf(tops[c], __uint_as_float(v[c >> 1][16 * (c & 1) + 15]));
       }
       float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      // behind this barrier both threads hold their scores: P may be written over them
-      top = fmaxf(top, exchange(top, n & 1));
+      if constexpr (HALVES == 2) top = fmaxf(top, exchange(top, n & 1));
       float fix = 1.f;
       const bool moved = __any_sync(0xffffffffu, top > m + LAZY);  // the same in both warps
       if (moved) {
@@ -462,7 +463,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         sum[k & 1] = add2(sum[k & 1], pack2(x, y));
         p[k] = pack_bf16(x, y);
       }
-      if (n > 0) {
+      if (n > 0 && (HALVES == 2 || moved)) {
         warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest, P used up: under the exponentials
         tc_fence_after();
         if (moved && half == 0) {  // ahead of this half's P, so ahead of the first product
@@ -486,13 +487,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       unpack2(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
     }
-    l += exchange(l, n_tiles & 1);
+    if constexpr (HALVES == 2) l += exchange(l, n_tiles & 1);
     if (n_tiles > 0) warp_wait(o_done, (n_tiles - 1) & 1, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;
     __nv_bfloat16* row = out + ((b * a.queries + i) * a.heads + head) * dim;
-    for (int c = half * (DP / 2); c < (half + 1) * (DP / 2) && c < dim; c += 32) {
+    for (int c = half * 32; c < DP && c < dim; c += HALVES * 32) {
       uint32_t o[32];
       if (n_tiles > 0) {
         tmem_ld32_issue(t_o + c, o);
@@ -992,7 +993,7 @@ static int launch_forward(const b200_attention& a, const CUtensorMap& q, const C
   const auto kernel = forward_kernel<DP, BIAS>;
   if (int rc = allow(kernel)) return rc;
   const int vec = a.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  kernel<<<(unsigned)(order.row_tiles * order.pairs), FWD_THREADS, shared, st>>>(q, k, v, a, order, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
+  kernel<<<(unsigned)(order.row_tiles * order.pairs), Fwd<DP>::THREADS, shared, st>>>(q, k, v, a, order, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
   return check_launch("attention");
 }
 
@@ -1036,7 +1037,7 @@ int tiles_forward(const b200_attention& a, void* out, float* lse, void* workspac
   CUtensorMap m[3];
   for (int i = 0; i < 3; ++i) {
     if (int rc = make_addressable(a, x[i], ws, st)) return rc;
-    if (int rc = map_of(&m[i], a, x[i], 128)) return rc;
+    if (int rc = map_of(&m[i], a, x[i], i == 0 ? ROWS : (a.dim <= 64 ? Fwd<64>::KEYS : Fwd<128>::KEYS))) return rc;
   }
   if (a.dim <= 64)
     return a.table ? launch_forward<64, true>(a, m[0], m[1], m[2], out, lse, st) : launch_forward<64, false>(a, m[0], m[1], m[2], out, lse, st);
