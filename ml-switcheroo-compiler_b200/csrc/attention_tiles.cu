@@ -4,12 +4,13 @@
 // the other's MMAs, and its start and end under the other's middle:
 //   warp 0      TMA: the queries once, then K and V tiles into a ring;
 //   warp 1      owns 256 columns of TMEM, issues S = Q K^T (operands in shared memory) and O += P V (P from TMEM);
-//   the others  softmax, 64 scores a thread.
-// The next tile's S is made under this one's exponentials. Heads of up to 64: tiles of 128 keys, S, P and O in columns of their own (128 + 64 +
-// 64), two threads a row, which exchange its maximum. Wider heads: tiles of 64 keys, two S in turn with P over them, and O
-// (64 + 64 + 128); MMAs run in their order, so an S is overwritten only when the P over it is used up. (With one S of 128 keys and P
-// over it, whose successor had to wait for P, 2 x 4096 causal tokens of 32 heads of 128 took 314 us.) The running maximum moves only
-// when a row's has grown by 2^8 (probabilities stay below 2^8, sums are fp32), so O is hardly ever rescaled.
+//   warps 2-5   softmax, a row of S a thread.
+// Tiles of 64 keys: two S take turns, P lies over its S (bf16 in the lower half), O has the rest (64 + 64 + 128 columns), so that the
+// next tile's S is made under this one's exponentials. MMAs run in their order: an S is overwritten only when the P over it is used up.
+// (One S of 128 keys with P over it, whose successor waited for P, took 314 us for 2 x 4096 causal tokens of 32 heads of 128, this 272;
+// S of 128 keys beside P, with two threads a row that exchange its maximum, 167 us for 64 x 512 tokens of 16 heads of 64, this 151.)
+// The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8, sums are fp32), so O is hardly ever
+// rescaled.
 // Making up to 3 of 8 exponentials on the FMA pipe changed nothing (the special function unit is busy for 60 % of the time): not done.
 //
 // Backward, one kernel in two forms. 128 rows stay, tiles of 64 tokens of the other side go past:
@@ -223,33 +224,31 @@ __device__ __forceinline__ void store32(__nv_bfloat16* row, int col, int dim, bo
 // forward
 // ------------------------------------------------------------------------------------
 
+constexpr int KEYS = 64, FWD_THREADS = 192;
 constexpr float LAZY = 8.f;  // log2 by which a maximum may grow before O is rescaled
 
 template <int DP>
 struct Fwd {
-  static constexpr int HALVES = DP == 64 ? 2 : 1;  // threads of a row
-  static constexpr int KEYS = 64 * HALVES, THREADS = 64 + 128 * HALVES, STAGES = 2;
+  static constexpr int STAGES = DP == 64 ? 4 : 2;
   static constexpr uint32_t Q = ROWS * DP * 2, TILE = KEYS * DP * 2;
-  static constexpr uint32_t BARS = Q + STAGES * 2 * TILE;
-  static constexpr uint32_t MAXIMA = BARS + 256, LUT = MAXIMA + 2 * 2 * ROWS * 4;
+  static constexpr uint32_t BARS = Q + STAGES * 2 * TILE, LUT = BARS + 256;
   static constexpr uint32_t TMEM = 256, T_O = TMEM - DP;
 };
 
 template <int DP, bool BIAS>
-__global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
+__global__ void __launch_bounds__(FWD_THREADS, 2)
     forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                    const __grid_constant__ b200_attention a, const __grid_constant__ Order order, __nv_bfloat16* out, float* lse, int vec) {
   using F = Fwd<DP>;
-  constexpr int ST = F::STAGES, KEYS = F::KEYS, HALVES = F::HALVES;
+  constexpr int ST = F::STAGES;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t s_q = smem_u32(smem), s_k = s_q + F::Q, s_v = s_k + ST * F::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST,
-           *s_free = s_full + 1, *p_full = s_full + 2, *o_done = s_full + 4, *idle = s_full + 5;
+           *p_full = s_full + 1, *o_done = s_full + 2, *idle = s_full + 3;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
-  float* maxima = reinterpret_cast<float*>(smem + F::MAXIMA);  // [parity][half][row]
   float* lut = reinterpret_cast<float*>(smem + F::LUT);
 
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -280,9 +279,7 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(s_full, 1);
-    mbar_init(s_free, 8);
-    mbar_init(&p_full[0], 4);
-    mbar_init(&p_full[1], 4);
+    mbar_init(p_full, 4);
     mbar_init(o_done, 1);
     mbar_init(idle, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -330,7 +327,7 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
       const Desc kd = {dk.lo + s * (F::TILE >> 4), dk.hi};
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
-        if (k < ks) mma(elected, tmem + (HALVES == 1 ? (n & 1) * KEYS : 0), dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
+        if (k < ks) mma(elected, tmem + (n & 1) * KEYS, dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
       commit(elected, s_full);
       commit(elected, &k_empty[s]);
     };
@@ -340,12 +337,7 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
     }
     for (int n = 0, s = 0, par = 0, next = 0, next_par = 0; n < n_tiles; ++n, s = next, par = next_par) {
       next = s + 1 == ST ? 0 : s + 1, next_par = s + 1 == ST ? par ^ 1 : par;
-      if (n + 1 < n_tiles) {
-        // two threads a row: they hold this tile's scores in registers; else the next S has columns of its own, whose P the sums before
-        // have used up
-        if constexpr (HALVES == 2) warp_wait(s_free, n & 1, gave_up);
-        scores(next, next_par, n + 1);
-      }
+      if (n + 1 < n_tiles) scores(next, next_par, n + 1);  // over the P before this one, which is used up
       warp_wait(&v_full[s], par, gave_up);
       const int have = seq.keys - (T0 + n) * KEYS;
       if (have < KEYS && seq.keys < a.keys) {
@@ -355,14 +347,11 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
         __syncwarp();
       }
       const Desc vd = {dv.lo + s * (F::TILE >> 4), dv.hi};
+      warp_wait(p_full, n & 1, gave_up);
+      tc_fence_after();
 #pragma unroll
-      for (int h = 0; h < HALVES; ++h) {
-        warp_wait(&p_full[h], n & 1, gave_up);
-        tc_fence_after();
-#pragma unroll
-        for (int k = 4 * h; k < 4 * h + 4; ++k)
-          mma_from_tmem(elected, tmem + F::T_O, tmem + (HALVES == 2 ? KEYS : (n & 1) * KEYS) + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
-      }
+      for (int k = 0; k < KEYS / 16; ++k)
+        mma_from_tmem(elected, tmem + F::T_O, tmem + (n & 1) * KEYS + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
       commit(elected, &v_empty[s]);
       commit(elected, o_done);
     }
@@ -370,25 +359,18 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
     commit(elected, idle);
     warp_wait(idle, 0, gave_up);
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
-    const int i0 = r0 + q * 32, i = i0 + lane, row_at = q * 32 + lane;
+    const int q = warp & 3;
+    const int i0 = r0 + q * 32, i = i0 + lane;
     const bool valid = i < seq.queries;
     const int lo = valid ? seq.first_key(a, i) : 0, hi = valid ? seq.end_key(a, i) : 0;
     // every key of [full0, full1) is seen by all rows of the warp
     const int full0 = seq.first_key(a, min(i0 + 31, seq.queries - 1)), full1 = seq.end_key(a, i0);
     const uint32_t t_row = tmem + ((uint32_t)(q * 32) << 16), t_o = t_row + F::T_O;
     const float sl = a.scale * LOG2E;
-    float m = -INFINITY, l = 0.f;  // the row's maximum, the sum of this thread's keys
-    // this thread's value for that of the row's other thread, at a barrier of their two warps
-    auto exchange = [&](float x, int parity) {
-      float* area = maxima + parity * 2 * ROWS;
-      area[half * ROWS + row_at] = x;
-      asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
-      return area[(half ^ 1) * ROWS + row_at];
-    };
+    float m = -INFINITY, l = 0.f;
     for (int n = 0; n < n_tiles; ++n) {
-      const int j0 = (T0 + n) * KEYS + half * 64;
-      const uint32_t t_s = t_row + (HALVES == 2 ? half : n & 1) * 64, t_p = HALVES == 2 ? t_row + KEYS + half * 32 : t_s;
+      const int j0 = (T0 + n) * KEYS;
+      const uint32_t t_s = t_row + (n & 1) * KEYS;
       warp_wait(s_full, n & 1, gave_up);
       tc_fence_after();
       uint32_t v[2][32];
@@ -396,11 +378,6 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
       tmem_ld32_issue(t_s + 32, v[1]);
       tmem_wait(v[0]);
       tmem_wait(v[1]);
-      if constexpr (HALVES == 2) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_free);
-      }
       float mul = sl;
       if constexpr (BIAS) {
         mul = 1.f;
@@ -440,10 +417,9 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
           tops[c] = fmaxf(fmaxf(tops[c], __uint_as_float(v[c >> 1][16 * (c & 1) + k])), __uint_as_float(v[c >> 1][16 * (c & 1) + k + 1]));
         tops[c] = fmaxf(tops[c], __uint_as_float(v[c >> 1][16 * (c & 1) + 15]));
       }
-      float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      if constexpr (HALVES == 2) top = fmaxf(top, exchange(top, n & 1));
+      const float top = mul * fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       float fix = 1.f;
-      const bool moved = __any_sync(0xffffffffu, top > m + LAZY);  // the same in both warps
+      const bool moved = __any_sync(0xffffffffu, top > m + LAZY);
       if (moved) {
         const float grown = fmaxf(m, top);
         fix = ex2(m - (grown == -INFINITY ? 0.f : grown));
@@ -463,37 +439,34 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
         sum[k & 1] = add2(sum[k & 1], pack2(x, y));
         p[k] = pack_bf16(x, y);
       }
-      if (n > 0 && (HALVES == 2 || moved)) {
-        warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest, P used up: under the exponentials
+      if (n > 0 && moved) {
+        warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest
         tc_fence_after();
-        if (moved && half == 0) {  // ahead of this half's P, so ahead of the first product
 #pragma unroll 1
-          for (int c = 0; c < DP; c += 16) {
-            uint32_t o[16];
-            tmem_ld16(t_o + c, o);
+        for (int c = 0; c < DP; c += 16) {
+          uint32_t o[16];
+          tmem_ld16(t_o + c, o);
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix);
-            tmem_st16(t_o + c, o);
-          }
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * fix);
+          tmem_st16(t_o + c, o);
         }
       }
-      tmem_st32(t_p, p);
+      tmem_st32(t_s, p);
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[half]);
+      if (lane == 0) mbar_arrive(p_full);
       float s0, s1, s2, s3;
       unpack2(sum[0], s0, s1);
       unpack2(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
     }
-    if constexpr (HALVES == 2) l += exchange(l, n_tiles & 1);
     if (n_tiles > 0) warp_wait(o_done, (n_tiles - 1) & 1, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;
     __nv_bfloat16* row = out + ((b * a.queries + i) * a.heads + head) * dim;
-    for (int c = half * 32; c < DP && c < dim; c += HALVES * 32) {
+    for (int c = 0; c < DP && c < dim; c += 32) {
       uint32_t o[32];
       if (n_tiles > 0) {
         tmem_ld32_issue(t_o + c, o);
@@ -505,7 +478,7 @@ __global__ void __launch_bounds__(Fwd<DP>::THREADS, 2)
       }
       if (i < a.queries) store32(row, c, dim, vec, o, inv);
     }
-    if (half == 0 && i < a.queries) lse[(b * a.heads + head) * a.queries + i] = live ? (m + log2f(l)) * LN2 : -INFINITY;
+    if (i < a.queries) lse[(b * a.heads + head) * a.queries + i] = live ? (m + log2f(l)) * LN2 : -INFINITY;
   }
   tc_fence_before();
   __syncthreads();
@@ -993,7 +966,7 @@ static int launch_forward(const b200_attention& a, const CUtensorMap& q, const C
   const auto kernel = forward_kernel<DP, BIAS>;
   if (int rc = allow(kernel)) return rc;
   const int vec = a.dim % 8 == 0 && (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-  kernel<<<(unsigned)(order.row_tiles * order.pairs), Fwd<DP>::THREADS, shared, st>>>(q, k, v, a, order, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
+  kernel<<<(unsigned)(order.row_tiles * order.pairs), FWD_THREADS, shared, st>>>(q, k, v, a, order, reinterpret_cast<__nv_bfloat16*>(out), lse, vec);
   return check_launch("attention");
 }
 
@@ -1037,7 +1010,7 @@ int tiles_forward(const b200_attention& a, void* out, float* lse, void* workspac
   CUtensorMap m[3];
   for (int i = 0; i < 3; ++i) {
     if (int rc = make_addressable(a, x[i], ws, st)) return rc;
-    if (int rc = map_of(&m[i], a, x[i], i == 0 ? ROWS : (a.dim <= 64 ? Fwd<64>::KEYS : Fwd<128>::KEYS))) return rc;
+    if (int rc = map_of(&m[i], a, x[i], i == 0 ? ROWS : KEYS)) return rc;
   }
   if (a.dim <= 64)
     return a.table ? launch_forward<64, true>(a, m[0], m[1], m[2], out, lse, st) : launch_forward<64, false>(a, m[0], m[1], m[2], out, lse, st);
