@@ -195,7 +195,7 @@ def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, 
     return a, (q, k, v, lengths, query_lengths, table), flat
 
 
-def op_fused_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False, window=None,
+def op_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False, window=None,
                        max_distance=128, bidirectional=None, **_):
     """Attention without the scores in memory: (out, lse), out_i = sum_j softmax_j(z_i) v_j for
     z_ij = scale q_i . k_j (+ the position bias), lse_i = log sum_j exp z_ij.
@@ -215,8 +215,8 @@ def op_fused_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=
     causal by default); entries finite or -inf.
 
     Scores, their maxima and sums are fp32; bf16 heads round the probabilities to bf16 for their
-    product with the values. Keep ``lse`` and ``out`` for FusedAttentionGrad."""
-    name = "FusedAttention"
+    product with the values. Keep ``lse`` and ``out`` for AttentionGrad."""
+    name = "Attention"
     a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
     x = kept[0]
     out = x.new_empty(x.shape)
@@ -227,15 +227,15 @@ def op_fused_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=
     return (out[0], lse[0]) if flat else (out, lse)
 
 
-def op_fused_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False,
+def op_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None, relative_bias=None, scale=None, causal=False,
                             window=None, max_distance=128, bidirectional=None, **_):
-    """(dq, dk, dv, dtable) of FusedAttention for its output's gradient ``dout``; ``out`` and ``lse`` as
+    """(dq, dk, dv, dtable) of Attention for its output's gradient ``dout``; ``out`` and ``lse`` as
     the forward returned them, the rest as it took it. The probabilities are made again from lse.
 
     Each is dense, in the shape and type of what it is the gradient of, rounded once; the heads that
     share a key head are summed, dtable (None without ``relative_bias``) over batch and positions.
     Queries and keys behind their sequence's end have zeros. The same from run to run."""
-    name = "FusedAttentionGrad"
+    name = "AttentionGrad"
     a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
     x, y, table = kept[0], kept[1], kept[5]
     if tuple(dout.shape) != tuple(q.shape) or tuple(out.shape) != tuple(q.shape):
@@ -383,8 +383,8 @@ def op_residual_norm_grad(dsum, dnormed, x, f, gamma=None, beta=None, post_gamma
 
 def register(table: dict) -> None:
     table.update({
-        "FusedAttention": op_fused_attention,
-        "FusedAttentionGrad": op_fused_attention_grad,
+        "Attention": op_attention,
+        "AttentionGrad": op_attention_grad,
         "RelativePositionBias": op_relative_position_bias,
         "RelativePositionBiasGrad": op_relative_position_bias_grad,
         "ResidualNorm": op_residual_norm,

@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
   const uint32_t s_q = smem_u32(smem), s_k = s_q + F::Q, s_v = s_k + ST * F::TILE;
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + F::BARS);
   uint64_t *q_full = bars, *k_full = bars + 1, *k_empty = k_full + ST, *v_full = k_empty + ST, *v_empty = v_full + ST, *s_full = v_empty + ST,
-           *p_full = s_full + 1, *o_done = s_full + 2, *idle = s_full + 3;
+           *p_full = s_full + 2, *o_done = s_full + 4, *idle = s_full + 6;  // s_full, p_full, o_done: one each for even and odd tiles
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(idle + 1);
   int* gave_up = reinterpret_cast<int*>(tmem_slot + 1);
   float* lut = reinterpret_cast<float*>(smem + F::LUT);
@@ -278,9 +278,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
-    mbar_init(o_done, 1);
+    for (int e = 0; e < 2; ++e) {
+      // two sets: a tile's scores are full before every warp has seen the ones before, and a warp may hand over a tile's P before
+      // another has the last one's; the next but one needs both
+      mbar_init(&s_full[e], 1);
+      mbar_init(&p_full[e], 4);
+      mbar_init(&o_done[e], 1);
+    }
     mbar_init(idle, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -328,7 +332,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
 #pragma unroll
       for (int k = 0; k < DP / 16; ++k)
         if (k < ks) mma(elected, tmem + (n & 1) * KEYS, dq, off_k<ROWS>(k), kd, off_k<KEYS>(k), id_s, k > 0);
-      commit(elected, s_full);
+      commit(elected, &s_full[n & 1]);
       commit(elected, &k_empty[s]);
     };
     if (n_tiles > 0) {
@@ -347,13 +351,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         __syncwarp();
       }
       const Desc vd = {dv.lo + s * (F::TILE >> 4), dv.hi};
-      warp_wait(p_full, n & 1, gave_up);
+      warp_wait(&p_full[n & 1], (n >> 1) & 1, gave_up);
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < KEYS / 16; ++k)
         mma_from_tmem(elected, tmem + F::T_O, tmem + (n & 1) * KEYS + k * 8, vd, off_mn(k), id_o, n > 0 || k > 0);
       commit(elected, &v_empty[s]);
-      commit(elected, o_done);
+      commit(elected, &o_done[n & 1]);
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
@@ -371,7 +375,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     for (int n = 0; n < n_tiles; ++n) {
       const int j0 = (T0 + n) * KEYS;
       const uint32_t t_s = t_row + (n & 1) * KEYS;
-      warp_wait(s_full, n & 1, gave_up);
+      warp_wait(&s_full[n & 1], (n >> 1) & 1, gave_up);
       tc_fence_after();
       uint32_t v[2][32];
       tmem_ld32_issue(t_s, v[0]);
@@ -440,7 +444,7 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
         p[k] = pack_bf16(x, y);
       }
       if (n > 0 && moved) {
-        warp_wait(o_done, (n - 1) & 1, gave_up);  // O at rest
+        warp_wait(&o_done[(n - 1) & 1], ((n - 1) >> 1) & 1, gave_up);  // O at rest
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DP; c += 16) {
@@ -455,13 +459,13 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[n & 1]);
       float s0, s1, s2, s3;
       unpack2(sum[0], s0, s1);
       unpack2(sum[1], s2, s3);
       l += (s0 + s1) + (s2 + s3);
     }
-    if (n_tiles > 0) warp_wait(o_done, (n_tiles - 1) & 1, gave_up);
+    if (n_tiles > 0) warp_wait(&o_done[(n_tiles - 1) & 1], ((n_tiles - 1) >> 1) & 1, gave_up);
     tc_fence_after();
     const bool live = valid && l != 0.f;
     const float inv = live ? 1.f / l : 0.f;

@@ -23,8 +23,15 @@ def test_bucket_starts(side, far):
 
 
 def test_names_are_registered():
-    for n in ("FusedAttention", "FusedAttentionGrad", "RelativePositionBias", "RelativePositionBiasGrad", "ResidualNorm", "ResidualNormGrad"):
-        assert n in ops.OPS
+    from b200 import fused_nodes, lm_ops
+
+    names, others = {}, {}
+    block_ops.register(names)
+    fused_nodes.register(others)
+    lm_ops.register(others)
+    assert set(names) == {"Attention", "AttentionGrad", "RelativePositionBias", "RelativePositionBiasGrad", "ResidualNorm", "ResidualNormGrad"}
+    assert not set(names) & set(others) and not set(names) & set(ops.ALIASES)
+    assert all(ops.OPS[n] is f for n, f in names.items())
 
 
 def qkv(b=2, nq=5, nk=7, h=4, hk=2, d=16, dtype=torch.float32):
@@ -33,7 +40,7 @@ def qkv(b=2, nq=5, nk=7, h=4, hk=2, d=16, dtype=torch.float32):
 
 def test_attention_refusals():
     q, k, v = qkv()
-    f = block_ops.op_fused_attention
+    f = block_ops.op_attention
     for bad in ((q, k[:1], v), (q, k, v[:, :3]), (q, k[..., :8], v[..., :8]), (q[:, :, :3], k, v), (q[0], k, v), (q[0, 0], k[0, 0], v[0, 0]),
                 (torch.zeros(1, 2, 2, 257),) * 3, (torch.zeros(1, 2, 2, 0),) * 3, (q, k[:, :, :0], v[:, :, :0])):
         with pytest.raises(ValueError):
@@ -58,7 +65,7 @@ def test_lengths_refusals():
     for bad, err in (([1, 2, 3], ValueError), (torch.zeros(2, 1, dtype=torch.int64), ValueError), (torch.zeros(2), BackendNotSupportedError),
                      (torch.zeros(2, dtype=torch.bool), BackendNotSupportedError)):
         with pytest.raises(err):
-            block_ops._lengths("FusedAttention", "lengths", bad, 2)
+            block_ops._lengths("Attention", "lengths", bad, 2)
 
 
 def test_bias_refusals():

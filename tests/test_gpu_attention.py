@@ -57,7 +57,7 @@ def close(got, ref, mag, heads, what=""):
 def check(q, k, v, dout=None, table=None, **kw):
     on = {n: t.cuda() if isinstance(t, torch.Tensor) else t for n, t in kw.items() if n not in ("scale_of",)}
     tc = None if table is None else table.cuda()
-    out, lse = op("FusedAttention", q.cuda(), k.cuda(), v.cuda(), relative_bias=tc, **on)
+    out, lse = op("Attention", q.cuda(), k.cuda(), v.cuda(), relative_bias=tc, **on)
     far = kw.get("max_distance", 128)
     ref_kw = {n: t for n, t in kw.items() if n != "max_distance"}
     ref, mag = R.attention(q, k, v, dout, table=table, far=far, **ref_kw)
@@ -66,7 +66,7 @@ def check(q, k, v, dout=None, table=None, **kw):
     close(lse, ref["lse"], mag["lse"], q.dtype, "lse")
     if dout is None:
         return out, lse
-    grads = op("FusedAttentionGrad", dout.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, relative_bias=tc, **on)
+    grads = op("AttentionGrad", dout.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, relative_bias=tc, **on)
     for got, name in zip(grads, ("dq", "dk", "dv", "dtable")):
         if name == "dtable" and table is None:
             assert got is None
@@ -118,7 +118,7 @@ def test_padded_batch(dtype, dim, causal):
         assert not out[e, queries[e]:].any() and (lse[e, :, queries[e]:] == -math.inf).all() and not dq[e, queries[e]:].any()
         assert not dk[e, lengths[e]:].any() and not dv[e, lengths[e]:].any()
     # 32-bit lengths, lengths of one side alone
-    again = op("FusedAttention", q.cuda(), k.cuda(), v.cuda(), lengths=lengths.int().cuda(), query_lengths=queries.cuda(), causal=causal)
+    again = op("Attention", q.cuda(), k.cuda(), v.cuda(), lengths=lengths.int().cuda(), query_lengths=queries.cuda(), causal=causal)
     assert torch.equal(again[0], out)
     check(*inputs(b, nq, nk, 4, 2, dim, dtype), lengths=lengths, causal=causal)
     check(*inputs(b, nq, nk, 4, 2, dim, dtype), query_lengths=queries, causal=causal)
@@ -133,8 +133,8 @@ def test_decode_from_caches():
     assert not out[4].any() and (lse[4] == -math.inf).all()
     # the same token as the last of its own prompt
     qa, ka, va, _ = inputs(1, 300, 300, 8, 2, 128, BF, seed=5)
-    whole, l0 = op("FusedAttention", qa.cuda(), ka.cuda(), va.cuda(), causal=True)
-    one, l1 = op("FusedAttention", qa[:, -1:].cuda(), ka.cuda(), va.cuda(), causal=True)
+    whole, l0 = op("Attention", qa.cuda(), ka.cuda(), va.cuda(), causal=True)
+    one, l1 = op("Attention", qa[:, -1:].cuda(), ka.cuda(), va.cuda(), causal=True)
     ref, mag = R.attention(qa, ka, va, causal=True)
     close(whole, ref["out"], mag["out"], BF, "out")
     close(one, ref["out"][:, -1:], mag["out"][:, -1:], BF, "out")
@@ -160,7 +160,7 @@ def test_position_bias_that_hides_and_padding():
     assert not out[0][:, :, 1].any() and not out[2][:, :, 1].any()
     # the type's lowest value is a number: a row of nothing else is a plain mean
     low = torch.full((16, 4), torch.finfo(BF).min, dtype=BF)
-    got, _ = op("FusedAttention", q.cuda(), k.cuda(), v.cuda(), relative_bias=low.cuda(), max_distance=30)
+    got, _ = op("Attention", q.cuda(), k.cuda(), v.cuda(), relative_bias=low.cuda(), max_distance=30)
     mean = v.double().mean(1, keepdim=True).repeat_interleave(2, 2).expand(3, 100, 4, 64)
     assert (got.cpu().double() - mean).abs().max() < 2.0**-8 * 4
 
@@ -168,8 +168,8 @@ def test_position_bias_that_hides_and_padding():
 @pytest.mark.parametrize("dtype", [BF, F32])
 def test_layouts(dtype):
     q, k, v, do = inputs(2, 70, 90, 4, 2, 64, dtype)
-    ref = op("FusedAttention", q.cuda(), k.cuda(), v.cuda(), causal=True)
-    gref = op("FusedAttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), *ref, causal=True)
+    ref = op("Attention", q.cuda(), k.cuda(), v.cuda(), causal=True)
+    gref = op("AttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), *ref, causal=True)
 
     def head_major(t):
         return t.cuda().transpose(1, 2).contiguous().transpose(1, 2)
@@ -193,17 +193,17 @@ def test_layouts(dtype):
         return t.cuda().permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0)
 
     for way in (head_major, sliced, unaligned, odd_rows, turned):
-        got = op("FusedAttention", way(q), way(k), way(v), causal=True)
+        got = op("Attention", way(q), way(k), way(v), causal=True)
         assert torch.equal(got[0], ref[0]) and torch.equal(got[1], ref[1]), way.__name__
-        grads = op("FusedAttentionGrad", way(do), way(q), way(k), way(v), *got, causal=True)
+        grads = op("AttentionGrad", way(do), way(q), way(k), way(v), *got, causal=True)
         assert all(torch.equal(x, y) for x, y in zip(grads[:3], gref[:3])), way.__name__
     # without the batch axis; one key and value for every sequence
-    one = op("FusedAttention", q[0].cuda(), k[0].cuda(), v[0].cuda(), causal=True)
+    one = op("Attention", q[0].cuda(), k[0].cuda(), v[0].cuda(), causal=True)
     assert torch.equal(one[0], ref[0][0]) and torch.equal(one[1], ref[1][0])
-    gone = op("FusedAttentionGrad", do[0].cuda(), q[0].cuda(), k[0].cuda(), v[0].cuda(), *one, causal=True)
+    gone = op("AttentionGrad", do[0].cuda(), q[0].cuda(), k[0].cuda(), v[0].cuda(), *one, causal=True)
     assert all(torch.equal(x, y[0]) for x, y in zip(gone[:3], gref[:3])) and gone[3] is None
     ks, vs = k[:1].cuda().expand(2, -1, -1, -1), v[:1].cuda().expand(2, -1, -1, -1)
-    shared = op("FusedAttention", q.cuda(), ks, vs, causal=True)
+    shared = op("Attention", q.cuda(), ks, vs, causal=True)
     assert torch.equal(shared[0][0], ref[0][0])
     close(shared[0], *(t["out"] for t in R.attention(q, k[:1].expand(2, -1, -1, -1), v[:1].expand(2, -1, -1, -1), causal=True)), dtype, "out")
 
@@ -220,18 +220,18 @@ def test_large_scores_and_scale(dtype):
 
 def test_nothing_to_do():
     q, k, v, do = inputs(2, 5, 0, 2, 1, 64, BF)
-    out, lse = op("FusedAttention", q.cuda(), k.cuda(), v.cuda())
+    out, lse = op("Attention", q.cuda(), k.cuda(), v.cuda())
     assert not out.any() and (lse == -math.inf).all()
     table = rand(8, 2, dtype=BF).cuda()
-    dq, dk, dv, dt = op("FusedAttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, relative_bias=table)
+    dq, dk, dv, dt = op("AttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse, relative_bias=table)
     assert not dq.any() and dk.numel() == 0 and dv.numel() == 0 and not dt.any() and dt.shape == table.shape
     q, k, v, do = inputs(2, 0, 5, 2, 1, 64, BF)
-    out, lse = op("FusedAttention", q.cuda(), k.cuda(), v.cuda())
-    dq, dk, dv, _ = op("FusedAttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse)
+    out, lse = op("Attention", q.cuda(), k.cuda(), v.cuda())
+    dq, dk, dv, _ = op("AttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse)
     assert out.numel() == 0 and not dk.any() and not dv.any() and dk.shape == k.shape
     q, k, v, do = inputs(0, 4, 5, 2, 1, 64, BF)
-    out, lse = op("FusedAttention", q.cuda(), k.cuda(), v.cuda())
-    assert out.numel() == 0 and all(t.numel() == 0 for t in op("FusedAttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse)[:3])
+    out, lse = op("Attention", q.cuda(), k.cuda(), v.cuda())
+    assert out.numel() == 0 and all(t.numel() == 0 for t in op("AttentionGrad", do.cuda(), q.cuda(), k.cuda(), v.cuda(), out, lse)[:3])
 
 
 def test_gradient_against_differences():
@@ -262,8 +262,8 @@ def test_same_from_run_to_run_and_in_graphs(dtype, dim):
     table = rand(32, 4, dtype=dtype).cuda()
 
     def step(x):
-        out, lse = op("FusedAttention", x, k, v, causal=True, relative_bias=table)
-        return (out, lse, *op("FusedAttentionGrad", do, x, k, v, out, lse, causal=True, relative_bias=table))
+        out, lse = op("Attention", x, k, v, causal=True, relative_bias=table)
+        return (out, lse, *op("AttentionGrad", do, x, k, v, out, lse, causal=True, relative_bias=table))
 
     first = step(q)
     assert all(torch.equal(x, y) for x, y in zip(first, step(q)))
@@ -294,10 +294,10 @@ def test_lengths_outside_are_clamped_and_flagged():
 
     q, k, v, _ = (t.cuda() for t in inputs(2, 30, 40, 2, 1, 64, BF))
     L.lib().b200_check_device_error(None)
-    want = op("FusedAttention", q, k, v)
+    want = op("Attention", q, k, v)
     assert L.lib().b200_check_device_error(None) == 0
-    got = op("FusedAttention", q, k, v, lengths=torch.tensor([41, 2**31 - 1]).cuda())
+    got = op("Attention", q, k, v, lengths=torch.tensor([41, 2**31 - 1]).cuda())
     assert torch.equal(got[0], want[0]) and L.lib().b200_check_device_error(None) != 0
-    empty = op("FusedAttention", q, k, v, lengths=torch.tensor([-1, -(2**31)]).cuda())
+    empty = op("Attention", q, k, v, lengths=torch.tensor([-1, -(2**31)]).cuda())
     assert not empty[0].any() and L.lib().b200_check_device_error(None) != 0
     assert L.lib().b200_check_device_error(None) == 0

@@ -69,7 +69,7 @@ def test_decoder_block_training_step_matches_64_bit_gradients():
     qkv = op("Matmul", y0, c["wqkv"]).view(B, S, H + 2 * HK, D)
     heads = (qkv[:, :, :H], qkv[:, :, H : H + HK], qkv[:, :, H + HK :])
     kw = {"causal": True, "lengths": lengths.cuda(), "query_lengths": lengths.cuda(), "relative_bias": c["table"], "max_distance": 20}
-    out, lse = op("FusedAttention", *heads, **kw)
+    out, lse = op("Attention", *heads, **kw)
     flat = out.flatten(2)
     f1 = op("Matmul", flat, c["wo"])
     t1, y1 = op("ResidualNorm", t0, f1, gamma=c["g1"])
@@ -79,7 +79,7 @@ def test_decoder_block_training_step_matches_64_bit_gradients():
     dt0, df1, dg1, *_ = op("ResidualNormGrad", torch.zeros_like(t1), dy1, t0, f1, gamma=c["g1"])
     dflat = op("Matmul", df1, c["wo"].t())
     dwo = op("Matmul", flat.reshape(-1, H * D).t(), df1.reshape(-1, C))
-    dq, dk, dv, dtable = op("FusedAttentionGrad", dflat.view(B, S, H, D), *heads, out, lse, **kw)
+    dq, dk, dv, dtable = op("AttentionGrad", dflat.view(B, S, H, D), *heads, out, lse, **kw)
     dqkv = torch.cat([dq, dk, dv], 2).flatten(2)
     dy0 = op("Matmul", dqkv, c["wqkv"].t())
     dwqkv = op("Matmul", y0.reshape(-1, C).t(), dqkv.reshape(-1, dqkv.shape[-1]))
@@ -100,9 +100,9 @@ def test_operators_as_graph_nodes(dtype):
 
     inputs = ["q", "k", "v", "len", "table", "do", "x", "f", "gamma"]
     nodes = [{"id": i, "op_type": "Input", "inputs": [], "attributes": {}} for i in inputs] + [
-        node("att", "FusedAttention", ["q", "k", "v", "len", "len", "table"], causal=True),
+        node("att", "Attention", ["q", "k", "v", "len", "len", "table"], causal=True),
         node("out", "TupleGetItem", ["att"], index=0), node("lse", "TupleGetItem", ["att"], index=1),
-        node("ag", "FusedAttentionGrad", ["do", "q", "k", "v", "out", "lse", "len", "len", "table"], causal=True),
+        node("ag", "AttentionGrad", ["do", "q", "k", "v", "out", "lse", "len", "len", "table"], causal=True),
         node("dk", "TupleGetItem", ["ag"], index=1), node("dt", "TupleGetItem", ["ag"], index=3),
         node("bias", "RelativePositionBias", ["table"], queries=9, keys=11),
         node("dbias", "RelativePositionBiasGrad", ["bias"], buckets=32),
@@ -122,8 +122,8 @@ def test_operators_as_graph_nodes(dtype):
 
     def calls(v):
         kw = {"lengths": v["len"], "query_lengths": v["len"], "relative_bias": v["table"], "causal": True}
-        out, lse = op("FusedAttention", v["q"], v["k"], v["v"], **kw)
-        ag = op("FusedAttentionGrad", v["do"], v["q"], v["k"], v["v"], out, lse, **kw)
+        out, lse = op("Attention", v["q"], v["k"], v["v"], **kw)
+        ag = op("AttentionGrad", v["do"], v["q"], v["k"], v["v"], out, lse, **kw)
         bias = op("RelativePositionBias", v["table"], queries=9, keys=11)
         total, normed = op("ResidualNorm", v["x"], v["f"], v["gamma"], residual_scale=0.5)
         rg = op("ResidualNormGrad", total, normed, v["x"], v["f"], v["gamma"], residual_scale=0.5)
@@ -147,7 +147,7 @@ def test_tokens_one_at_a_time_equal_the_prompt(dtype, dim):
     q, k, v = (torch.randn(3, n, h, dim, generator=g).to(dtype) for h in (H, HK, HK))
     table = torch.randn(16, H, generator=g).to(dtype)
     kw = {"causal": True, "relative_bias": table.cuda(), "max_distance": 12}
-    whole, lse = op("FusedAttention", q.cuda(), k.cuda(), v.cuda(), lengths=lengths.cuda(), query_lengths=lengths.cuda(), **kw)
+    whole, lse = op("Attention", q.cuda(), k.cuda(), v.cuda(), lengths=lengths.cuda(), query_lengths=lengths.cuda(), **kw)
     ref, mag = R.attention(q, k, v, lengths=lengths, query_lengths=lengths, causal=True, table=table, far=12)
     caches = [torch.full((3, 64, HK, dim), math.nan, dtype=dtype, device="cuda") for _ in range(2)]
     for t in range(n):
@@ -157,7 +157,7 @@ def test_tokens_one_at_a_time_equal_the_prompt(dtype, dim):
                 if now[e]:
                     cache[e, t] = x[e, t].cuda()
         have = torch.minimum(lengths, torch.tensor(t + 1))
-        one, one_lse = op("FusedAttention", q[:, t : t + 1].cuda(), *caches, lengths=have.cuda(), **kw)
+        one, one_lse = op("Attention", q[:, t : t + 1].cuda(), *caches, lengths=have.cuda(), **kw)
         for e in range(3):
             if not now[e]:
                 continue
@@ -183,8 +183,8 @@ def test_threads_call_at_once():
         res = [op("RelativePositionBias", table, queries=20, keys=70, max_distance=1024), *op("ResidualNorm", x, x, post_norm=True)]
         for q, k, v, do in sets:
             kw = {"relative_bias": table, "max_distance": 1024}
-            out, lse = op("FusedAttention", q, k, v, **kw)
-            res += [out, lse, *op("FusedAttentionGrad", do, q, k, v, out, lse, **kw)]
+            out, lse = op("Attention", q, k, v, **kw)
+            res += [out, lse, *op("AttentionGrad", do, q, k, v, out, lse, **kw)]
         return res
 
     want = work()
@@ -218,8 +218,8 @@ def test_offsets_beyond_32_bits(queries):
     k.copy_(small[0])
     v.copy_(small[1])
     q, do = (torch.randn(2, queries, 4, 64, generator=g, device="cuda").to(BF) for _ in range(2))
-    want, lse = op("FusedAttention", q, *small, causal=True)
-    got, lse2 = op("FusedAttention", q, k, v, causal=True)
+    want, lse = op("Attention", q, *small, causal=True)
+    got, lse2 = op("Attention", q, k, v, causal=True)
     assert torch.equal(got, want) and torch.equal(lse, lse2)
-    for a, b in zip(op("FusedAttentionGrad", do, q, *small, want, lse, causal=True)[:3], op("FusedAttentionGrad", do, q, k, v, got, lse, causal=True)[:3]):
+    for a, b in zip(op("AttentionGrad", do, q, *small, want, lse, causal=True)[:3], op("AttentionGrad", do, q, k, v, got, lse, causal=True)[:3]):
         assert torch.equal(a, b)
