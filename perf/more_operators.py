@@ -2,7 +2,7 @@
 
 The operators of a decoder or encoder block's training step and of its single-token serving form:
 
-* ``FusedAttention`` (and its gradient, which makes the probabilities again from the saved
+* ``Attention`` (and its gradient, which makes the probabilities again from the saved
   log-sum-exp): shared key heads, causal or not, sequences padded at their ends, a cache
   longer than what it holds, a learned bias by relative position;
 * ``RelativePositionBias`` (and its gradient): that bias on its own, for scores in memory;
@@ -195,10 +195,10 @@ def _run_own(c, s):
     op = B200Backend.execute_op
     if c["op"] == "attention":
         kw = {"causal": c["causal"], "lengths": s["lengths"], "query_lengths": s["query_lengths"], "relative_bias": s["table"]}
-        out, lse = op("FusedAttention", s["q"], s["k"], s["v"], **kw)
+        out, lse = op("Attention", s["q"], s["k"], s["v"], **kw)
         if not c["grad"]:
             return out, lse
-        grads = op("FusedAttentionGrad", s["dout"], s["q"], s["k"], s["v"], out, lse, **kw)
+        grads = op("AttentionGrad", s["dout"], s["q"], s["k"], s["v"], out, lse, **kw)
         return (out, *grads) if c["bias"] else (out, *grads[:3])
     if c["op"] == "bias":
         if c["grad"]:
