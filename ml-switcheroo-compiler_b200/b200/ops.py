@@ -10,7 +10,8 @@ Numeric policy: fp32 values are computed in fp32. numpy's float64 promotion from
 Python-float constants is not reproduced: those constants are applied as fp32.
 Contractions use ``matmul_dtype`` (``"f32"`` exact CUDA-core path, ``"bf16"`` tcgen05
 tensor cores with fp32 accumulation). The head's cross entropy (``lm_ops``) is the exception:
-beyond 8 tokens its fp32 operands multiply as pairs of bf16 values, 16 bits each.
+beyond 8 tokens its fp32 operands multiply as pairs of bf16 values, 16 bits each. Attention (``block_ops``)
+goes by its heads' type alone.
 """
 
 from __future__ import annotations

@@ -18,9 +18,13 @@
 //   dk, dv:  rows are keys (K, V), tiles are queries (Q, dO):     S = K Q^T, dP = V dO^T, dV += P dO, dK += dS Q
 // so p and dz of a tile are made by the threads that own its rows, go back to TMEM as bf16 over the S and dP that they come
 // from, and are the A operand of the sums there: nothing is transposed, no sum leaves its block, every order is fixed. S and
-// dP are made twice for that (7 products instead of 5). Heads of up to 64: one warpgroup and 256 columns of TMEM a block, two
-// blocks an SM; wider heads: two warpgroups that take tiles in turn, each with an S and dP of its own.
+// dP are made twice for that (7 products instead of 5). Two warpgroups share a tile, 32 columns each (one for all 64 took as long).
+// Heads of up to 64: 256 columns of TMEM a block and two blocks an SM; wider heads: two pairs of warpgroups that take tiles in turn,
+// each with an S and dP of its own (one pair: 739 us for 4 x 2048 tokens of 16 heads of 128, two: 542).
 // Tiles of 64 because of TMEM; an MMA of 128 x 64 from shared memory takes 48 clocks, of 128 x 128 64 (measured).
+// What bounds both directions is the chain of a tile, with two tiles under way on an SM: the tensor pipe is active for 29 to 35 % of
+// the time, the special function unit for 29 to 61 %, issue slots for 40 to 47 % (8 x 2048 tokens of 16 heads of 64: forward 217,
+// gradients 741 us).
 //
 // Probabilities and dz are rounded to bf16 for the products that they are operands of; scores, maxima, sums and
 // all accumulators are fp32. Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the

@@ -10,6 +10,8 @@
 // threads read neighbouring elements and every element is added in a register, without atomics.
 // A diagonal's sum goes to the block's own [-far, far] array, that to buckets, those to the
 // workspace, and a second launch adds the blocks up in order.
+// Measured: 16 x 1023 x 2047 bf16 in 21 us (29 with a division by the row length an element), the gradient of 4 x 16 x 777 x 1000 fp32
+// in 43 to 50 us (67 with 8 loads a thread under way instead of 32).
 #include <algorithm>
 
 #include "ew_common.cuh"
