@@ -174,7 +174,9 @@ def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, 
     """(description, the tensors that it points to, whether the batch axis was left out)."""
     flat = q.dim() == 3
     if flat:
-        q, k, v = (t.unsqueeze(0) if t.dim() == 3 else t for t in (q, k, v))
+        if k.dim() != 3 or v.dim() != 3:
+            raise ValueError(f"{name}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)}: all with the batch axis or none")
+        q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
     plan = _attention_plan(name, (q.shape, k.shape, v.shape), (q.dtype, k.dtype, v.dtype), None if table is None else (table.shape, table.dtype),
                            None if scale is None else float(scale), bool(causal), None if window is None else float(window), int(max_distance),
                            None if bidirectional is None else bool(bidirectional))

@@ -41,7 +41,8 @@ def qkv(b=2, nq=5, nk=7, h=4, hk=2, d=16, dtype=torch.float32):
 def test_attention_refusals():
     q, k, v = qkv()
     f = block_ops.op_attention
-    for bad in ((q, k[:1], v), (q, k, v[:, :3]), (q, k[..., :8], v[..., :8]), (q[:, :, :3], k, v), (q[0], k, v), (q[0, 0], k[0, 0], v[0, 0]),
+    for bad in ((q, k[:1], v), (q, k, v[:, :3]), (q, k[..., :8], v[..., :8]), (q[:, :, :3], k, v), (q[0], k, v), (q[0], k[0], v), (q[0], k, v[0]),
+                (q, k[0], v[0]), (q[0], k[:1], v[:1]), (q[0], k[0], v[:1]), (q[0, 0], k[0, 0], v[0, 0]),
                 (torch.zeros(1, 2, 2, 257),) * 3, (torch.zeros(1, 2, 2, 0),) * 3, (q, k[:, :, :0], v[:, :, :0])):
         with pytest.raises(ValueError):
             f(*bad)
