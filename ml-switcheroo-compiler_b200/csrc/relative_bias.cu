@@ -196,6 +196,7 @@ extern "C" int b200_relative_bias(const b200_relative* r, int dtype, const void*
   if (heads == 0 || queries == 0 || keys == 0) return B200_OK;
   B200_REQUIRE(table && out, "relative_bias: null operand");
   const int64_t plane = queries * keys;
+  B200_REQUIRE(plane < (1ll << 45), "relative_bias: %lld queries times %lld keys", (long long)queries, (long long)keys);
   const dim3 grid((unsigned)std::max<int64_t>(1, ceil_div(plane, PIECE)), (unsigned)heads);
   const size_t shared = (size_t)(2 * far_of(*r) + 1) * (dtype == B200_F32 ? 4 : 2);
   uint32_t mul, shr;
