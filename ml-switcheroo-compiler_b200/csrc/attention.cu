@@ -122,7 +122,7 @@ extern "C" int b200_attention_forward(const b200_attention* a, void* out, float*
 
 extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) {
   if (check_attention("attention_grad", a) || a->batch == 0) return 0;
-  return delta_bytes(*a) + (tiles_take(*a) ? tiles_grad_workspace(*a, nullptr) : rows_grad_workspace(*a));
+  return delta_bytes(*a) + (tiles_take_grad(*a) ? tiles_grad_workspace(*a, nullptr) : rows_grad_workspace(*a));
 }
 
 extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes,
@@ -159,5 +159,5 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
                                                       delta, (int)padded, vec);
   if (int rc = check_launch("attention_grad")) return rc;
   void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
-  return tiles_take(*a) ? tiles_grad(*a, *g, lse2, delta, padded, rest, st) : rows_grad(*a, *g, delta, padded, rest, st);
+  return tiles_take_grad(*a) ? tiles_grad(*a, *g, lse2, delta, padded, rest, st) : rows_grad(*a, *g, delta, padded, rest, st);
 }

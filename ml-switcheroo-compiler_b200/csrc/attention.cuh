@@ -57,7 +57,8 @@ int rows_grad(const b200_attention& a, const b200_attention_grads& g, const floa
 int table_sum(const b200_attention& a, const float* part, int64_t blocks, void* dtable, cudaStream_t st);
 
 // attention_tiles.cu
-bool tiles_take(const b200_attention& a);
+bool tiles_take(const b200_attention& a);       // whether they make the forward,
+bool tiles_take_grad(const b200_attention& a);  // and the gradient
 size_t tiles_forward_workspace(const b200_attention& a);
 int tiles_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st);
 size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads* g);

@@ -1004,7 +1004,16 @@ static int launch_backward(const b200_attention& a, const Operand (&x)[2], const
 
 }  // namespace tiles
 
-bool tiles_take(const b200_attention& a) { return a.dtype == B200_BF16 && a.dim <= 128 && a.queries >= 16 && a.keys >= 1; }
+bool tiles_take_grad(const b200_attention& a) { return a.dtype == B200_BF16 && a.dim <= 128 && a.queries >= 16 && a.keys >= 1; }
+
+// Forward, the row kernels split long keys over the SMs, which a tile's block walks alone (0.7 us for 64 keys). They take few queries
+// over 2048 keys or more, while queries x heads x elements stay below 75000. Measured, rows against tiles: 16 queries of 8 heads of
+// 64 over 2048 keys 24 and 28 us, 64 queries 29 and 27; over 16384 keys 64 queries 90 and 177 us, 128 queries 167 and 178, 256
+// queries 312 and 178; 32 + 8 heads of 128 over 16384 keys, 16 queries 142 and 213, 32 queries 264 and 207; 16 queries of 4 x 32
+// heads of 128 over 4096 keys 158 and 56.
+bool tiles_take(const b200_attention& a) {
+  return tiles_take_grad(a) && (a.keys < 2048 || a.batch * a.heads * a.queries * a.dim >= 75000);
+}
 
 size_t tiles_forward_workspace(const b200_attention& a) {
   using namespace tiles;

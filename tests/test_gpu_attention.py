@@ -84,7 +84,7 @@ SHAPES = [  # batch, queries, keys, heads, key heads, dim
     (1, 1, 1, 1, 1, 1), (1, 1, 1, 2, 1, 8), (2, 3, 5, 3, 3, 16), (1, 17, 33, 4, 2, 33), (2, 64, 64, 2, 2, 64), (1, 129, 257, 2, 1, 64),
     (1, 200, 131, 4, 1, 80), (2, 128, 128, 2, 1, 128), (1, 300, 300, 1, 1, 96), (1, 70, 190, 5, 5, 127), (1, 33, 65, 2, 1, 130),
     (1, 40, 70, 2, 2, 256), (3, 1, 700, 8, 2, 64), (1, 2, 1500, 6, 1, 128), (1, 5, 900, 3, 1, 200), (2, 1, 300, 1, 1, 40),
-    (1, 385, 513, 2, 2, 32), (1, 259, 4, 2, 1, 64),
+    (1, 385, 513, 2, 2, 32), (1, 259, 4, 2, 1, 64), (1, 40, 40, 2, 1, 1), (1, 50, 50, 2, 2, 8), (1, 33, 47, 2, 1, 65), (1, 16, 1, 1, 1, 64),
 ]
 
 
@@ -93,6 +93,30 @@ SHAPES = [  # batch, queries, keys, heads, key heads, dim
 @pytest.mark.parametrize("shape", SHAPES)
 def test_shapes(shape, dtype, causal):
     check(*inputs(*shape, dtype), causal=causal)
+
+
+@pytest.mark.parametrize("causal,window,lengths", [(True, None, None), (False, 1500, [2100, 40]), (True, 700, [0, 1999]), (False, None, None)])
+@pytest.mark.parametrize("nq,h,hk,dim", [(16, 4, 1, 128), (33, 8, 8, 64), (100, 2, 1, 40), (292, 2, 1, 64), (293, 2, 1, 64)])
+def test_few_queries_of_long_keys(nq, h, hk, dim, causal, window, lengths):
+    q, k, v, do = inputs(2, nq, 2100, h, hk, dim, BF)
+    lengths = lengths and torch.tensor(lengths)
+    check(q, k, v, do, lengths=lengths, causal=causal, window=window)
+    check(q, k, v, do, table=rand(32, h, dtype=BF, seed=9), lengths=lengths, causal=causal, window=window, max_distance=300)
+
+
+@pytest.mark.parametrize("table_type", [BF, F32])
+@pytest.mark.parametrize("dim", [64, 96, 128])
+@pytest.mark.parametrize("causal,window", [(True, None), (False, 90), (True, 33)])
+def test_everything_at_once(causal, window, dim, table_type):
+    """Bias of either type, padding of both sides, shared heads, windows; forward and gradients on the tensor cores."""
+    b, nq, nk = 6, 190, 270
+    q, k, v, do = inputs(b, nq, nk, 4, 2, dim, BF)
+    lengths, queries = torch.tensor([0, 70, 128, 270, 200, 64]), torch.tensor([190, 1, 64, 190, 0, 128])
+    for e in range(b):
+        k[e, lengths[e]:] = v[e, lengths[e]:] = math.nan
+        q[e, queries[e]:] = do[e, queries[e]:] = math.nan
+    check(q, k, v, do, table=rand(32, 4, dtype=table_type, seed=9), lengths=lengths, query_lengths=queries, causal=causal, window=window,
+          max_distance=60)
 
 
 @pytest.mark.parametrize("causal,window", [(True, 1), (True, 40), (False, 1), (False, 33), (True, 5000), (False, 5000)])
