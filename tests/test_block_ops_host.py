@@ -151,6 +151,7 @@ def test_bias_entry_points_check():
     call = lambda r, *s, dt=L.F32: lib.b200_relative_bias(r, dt, 4096, 4096, *s, None)  # noqa: E731
     assert call(None, 1, 1, 1, 0) == L.ERR_ARG
     assert call(r, -1, 1, 1, 0) == L.ERR_ARG and call(r, 1, 1 << 30, 1, 0) == L.ERR_ARG and call(r, 1, 1, 1, 1 << 40) == L.ERR_ARG
+    assert call(r, 1, 1 << 23, 1 << 22, 0) == L.ERR_ARG  # more pieces than a grid has
     assert call(r, 1, 1, 1, 0, dt=L.I64) == L.ERR_DTYPE and call(r, 0, 1, 1, 0) == L.OK
     bad = L.Relative()
     for side, starts in ((0, []), (129, []), (2, [1, 2]), (3, [0, 5, 4]), (2, [0, 1025])):
