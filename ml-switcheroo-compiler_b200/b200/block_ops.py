@@ -119,6 +119,15 @@ def _tokens(name: str, what: str, x: torch.Tensor) -> torch.Tensor:
     return ops.contiguous(x) if x.stride(3) != 1 and x.shape[3] > 1 else x
 
 
+def _window(name: str, window: Any) -> int:
+    """The window in tokens, 0 for none; what hides nothing at any length is cut to what a C int64 holds."""
+    if window is None:
+        return 0
+    if not window >= 1 or (window != math.inf and int(window) != window):
+        raise ValueError(f"{name}: window {window!r} is not a number of tokens")
+    return int(min(window, L.ATTENTION_MAX_WINDOW))
+
+
 def _lengths(name: str, what: str, n: Any, batch: int) -> torch.Tensor | None:
     if n is None:
         return None
@@ -154,8 +163,6 @@ def _attention_plan(name, shapes, dtypes, table, scale, causal, window, max_dist
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"{name}: scale {scale} is not a positive number")
-    if window is not None and (int(window) != window or window < 1):
-        raise ValueError(f"{name}: window {window!r} is not a number of tokens")
     a = L.Attention()
     if table is not None:
         shape, dtype = table
@@ -166,7 +173,7 @@ def _attention_plan(name, shapes, dtypes, table, scale, causal, window, max_dist
         a.relative = _relative(shape[0], int(max_distance), not causal if bidirectional is None else bool(bidirectional))
         a.table_dtype = ops._TORCH2CODE[dtype]
     a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim = b, nq, nk, h, hk, d
-    a.window, a.causal, a.scale, a.dtype = int(window or 0), int(bool(causal)), scale, ops._TORCH2CODE[dtypes[0]]
+    a.window, a.causal, a.scale, a.dtype = window, int(bool(causal)), scale, ops._TORCH2CODE[dtypes[0]]
     return a
 
 
@@ -178,7 +185,7 @@ def _describe(name: str, q, k, v, lengths, query_lengths, table, scale, causal, 
             raise ValueError(f"{name}: queries {tuple(q.shape)}, keys {tuple(k.shape)} and values {tuple(v.shape)}: all with the batch axis or none")
         q, k, v = q.unsqueeze(0), k.unsqueeze(0), v.unsqueeze(0)
     plan = _attention_plan(name, (q.shape, k.shape, v.shape), (q.dtype, k.dtype, v.dtype), None if table is None else (table.shape, table.dtype),
-                           None if scale is None else float(scale), bool(causal), None if window is None else float(window), int(max_distance),
+                           None if scale is None else float(scale), bool(causal), _window(name, window), int(max_distance),
                            None if bidirectional is None else bool(bidirectional))
     a = L.Attention.from_buffer_copy(plan)
     _on_device(name, q, k, v, table)

@@ -1,4 +1,6 @@
 // The attention entry points: checks, and the choice of the kernels.
+#include <algorithm>
+
 #include "attention.cuh"
 
 namespace b200 {
@@ -35,6 +37,13 @@ static int check_attention(const char* what, const b200_attention* a) {
   B200_REQUIRE(a->batch == 0 || a->queries == 0 || a->q, "%s: null queries", what);
   B200_REQUIRE(a->batch == 0 || a->keys == 0 || (a->k && a->v), "%s: null keys or values", what);
   return B200_OK;
+}
+
+// The description with a window that positions can be added to: 2^31 is more than queries and keys together and hides nothing.
+static b200_attention within(const b200_attention& a) {
+  b200_attention own = a;
+  own.window = std::min<int64_t>(a.window, 1ll << 31);
+  return own;
 }
 
 // What the gradient needs of each query beside its own row, negated: delta = dout . out, and lse in the log2 domain, infinite where
@@ -117,7 +126,8 @@ extern "C" int b200_attention_forward(const b200_attention* a, void* out, float*
   const size_t need = b200_attention_workspace_bytes(a);
   B200_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0),
                "attention: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
-  return tiles_take(*a) ? tiles_forward(*a, out, lse, workspace, as_stream(stream)) : rows_forward(*a, out, lse, workspace, as_stream(stream));
+  const b200_attention own = within(*a);
+  return tiles_take(own) ? tiles_forward(own, out, lse, workspace, as_stream(stream)) : rows_forward(own, out, lse, workspace, as_stream(stream));
 }
 
 extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) {
@@ -146,6 +156,7 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
   const size_t need = b200_attention_grad_workspace_bytes(a);
   B200_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
+  const b200_attention own = within(*a);
   const int64_t padded = padded_of(*a);
   float *lse2 = reinterpret_cast<float*>(workspace), *delta = lse2 + a->batch * a->heads * padded;
   B200_REQUIRE(padded * a->heads < (1ll << 31), "attention_grad: %lld queries of %lld heads are too many", (long long)a->queries, (long long)a->heads);
@@ -153,11 +164,11 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
   const int64_t* s = g->dout_stride;
   const int vec = ((reinterpret_cast<uintptr_t>(g->dout) | reinterpret_cast<uintptr_t>(g->out) | (uint64_t)((s[0] | s[1] | s[2] | a->dim) * size)) & 15) == 0;
   if (a->dtype == B200_F32)
-    delta_kernel<float><<<grid, 256, 0, st>>>(*a, (const float*)g->dout, (const float*)g->out, g->lse, s[0], s[1], s[2], lse2, delta, (int)padded, vec);
+    delta_kernel<float><<<grid, 256, 0, st>>>(own, (const float*)g->dout, (const float*)g->out, g->lse, s[0], s[1], s[2], lse2, delta, (int)padded, vec);
   else
-    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(*a, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, g->lse, s[0], s[1], s[2], lse2,
+    delta_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(own, (const __nv_bfloat16*)g->dout, (const __nv_bfloat16*)g->out, g->lse, s[0], s[1], s[2], lse2,
                                                       delta, (int)padded, vec);
   if (int rc = check_launch("attention_grad")) return rc;
   void* rest = reinterpret_cast<uint8_t*>(workspace) + delta_bytes(*a);
-  return tiles_take_grad(*a) ? tiles_grad(*a, *g, lse2, delta, padded, rest, st) : rows_grad(*a, *g, delta, padded, rest, st);
+  return tiles_take_grad(own) ? tiles_grad(own, *g, lse2, delta, padded, rest, st) : rows_grad(own, *g, delta, padded, rest, st);
 }

@@ -1,0 +1,26 @@
+"""Arguments of the block operators at the ends of their ranges, on the host (no kernel runs)."""
+
+import sys
+
+import pytest
+import torch
+
+from b200 import _lib as L
+from b200 import block_ops
+
+
+@pytest.mark.parametrize("window", [1, 7.0, 2**31, 2**31 + 5, sys.maxsize, 2**63, 2**64 + 2**13, 10**400, float("inf")])
+def test_a_window_reaches_the_kernels_as_itself_or_as_more_than_any_length(window):
+    got = block_ops._window("Attention", window)
+    assert got == (window if window <= 2**31 else 2**31)
+    x = torch.Size((1, 4, 2, 64))
+    plan = block_ops._attention_plan("Attention", (x,) * 3, (torch.float32,) * 3, None, None, True, got, 128, None)
+    assert plan.window == got
+    assert block_ops._window("Attention", None) == 0
+
+
+@pytest.mark.parametrize("window", [0, -1, 0.5, 1.5, float("nan"), -float("inf"), -(2**64) + 5])
+def test_no_windows(window):
+    x = torch.zeros(1, 4, 2, 64)
+    with pytest.raises(ValueError):
+        block_ops.op_attention(x, x, x, window=window)
