@@ -74,7 +74,7 @@ class Rotary(C.Structure):
     ]
 
 
-RELATIVE_MAX_SIDE, RELATIVE_MAX_FAR = 128, 1024
+RELATIVE_MAX_SIDE, RELATIVE_MAX_FAR, RELATIVE_MAX_SHIFT = 128, 1024, 1 << 29
 ATTENTION_MAX_DIM = 256
 ATTENTION_MAX_WINDOW = 1 << 31  # more than queries and keys together: hides nothing
 RESIDUAL_NORM_MAX_COLS = 16384

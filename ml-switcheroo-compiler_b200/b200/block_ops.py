@@ -62,6 +62,13 @@ def _count(name: str, what: str, n: Any) -> int:
     return int(n)
 
 
+def _shift(name: str, shift: Any, queries: int, keys: int) -> int:
+    n = keys - queries if shift is None else int(shift)
+    if abs(n) >= L.RELATIVE_MAX_SHIFT:
+        raise ValueError(f"{name}: shift {n} of {queries} queries and {keys} keys (below 2^29)")
+    return n
+
+
 def op_relative_position_bias(table, queries=None, keys=None, bidirectional=True, max_distance=128, shift=None, **_):
     """The learned bias of every query and key, [heads, queries, keys] of the table's type, to
     be added to scores: ``table[bucket(rel), head]`` for rel = key - query - shift.
@@ -76,12 +83,13 @@ def op_relative_position_bias(table, queries=None, keys=None, bidirectional=True
     if table.dtype not in _FLOATS:
         raise BackendNotSupportedError(f"{name}: table of {table.dtype} (fp32 and bf16)")
     nq, nk = _count(name, "queries", queries), _count(name, "keys", keys)
+    shift = _shift(name, shift, nq, nk)
     r = _relative(table.shape[0], int(max_distance), bool(bidirectional))
     _on_device(name, table)
     table = ops.contiguous(table)
     out = torch.empty(table.shape[1], nq, nk, dtype=table.dtype, device=table.device)
-    L.call("b200_relative_bias", r, ops.code(table), table.data_ptr(), out.data_ptr(), table.shape[1], nq, nk,
-           nk - nq if shift is None else int(shift), ops.stream_ptr())
+    L.call("b200_relative_bias", r, ops.code(table), table.data_ptr(), out.data_ptr(), table.shape[1], nq, nk, shift,
+           ops.stream_ptr())
     return out
 
 
@@ -96,14 +104,15 @@ def op_relative_position_bias_grad(dscores, buckets=None, bidirectional=True, ma
         raise BackendNotSupportedError(f"{name}: scores of {dscores.dtype} (fp32 and bf16)")
     heads, nq, nk = dscores.shape[-3:]
     buckets = _count(name, "buckets", buckets)
+    shift = _shift(name, shift, nq, nk)
     r = _relative(buckets, int(max_distance), bool(bidirectional))
     _on_device(name, dscores)
     d = ops.contiguous(dscores)
     out = torch.empty(buckets, heads, dtype=d.dtype, device=d.device)
     wn = L.lib().b200_relative_bias_grad_workspace_bytes(r, heads, nq, nk)
     ws = torch.empty(wn, dtype=torch.uint8, device=d.device)
-    L.call("b200_relative_bias_grad", r, ops.code(d), d.data_ptr(), out.data_ptr(), math.prod(d.shape[:-3]), heads, nq, nk,
-           nk - nq if shift is None else int(shift), ws.data_ptr(), wn, ops.stream_ptr())
+    L.call("b200_relative_bias_grad", r, ops.code(d), d.data_ptr(), out.data_ptr(), math.prod(d.shape[:-3]), heads, nq, nk, shift,
+           ws.data_ptr(), wn, ops.stream_ptr())
     return out
 
 

@@ -5,7 +5,6 @@ import sys
 import pytest
 import torch
 
-from b200 import _lib as L
 from b200 import block_ops
 
 
@@ -24,3 +23,13 @@ def test_no_windows(window):
     x = torch.zeros(1, 4, 2, 64)
     with pytest.raises(ValueError):
         block_ops.op_attention(x, x, x, window=window)
+
+
+@pytest.mark.parametrize("shift", [2**29, -(2**29), 2**31, 2**63, 2**64, 2**64 + 7, -(2**64) - 7])
+def test_a_shift_is_not_taken_for_another_one(shift):
+    """Numbers beyond int64 wrap on their way into C."""
+    with pytest.raises(ValueError):
+        block_ops.op_relative_position_bias(torch.zeros(32, 2), queries=3, keys=4, shift=shift)
+    with pytest.raises(ValueError):
+        block_ops.op_relative_position_bias_grad(torch.zeros(2, 3, 4), buckets=32, shift=shift)
+    assert block_ops._shift("RelativePositionBias", 2**29 - 1, 3, 4) == 2**29 - 1 and block_ops._shift("RelativePositionBias", None, 3, 4) == 1
