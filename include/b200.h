@@ -710,7 +710,10 @@ int b200_relative_bias_grad(const b200_relative* r, int dtype, const void* dbias
  * causal: keys behind that position are hidden; window > 0: so are those at `window` or more
  * before it (and, not causal, behind it). A query that sees nothing, or behind its sequence's
  * end, has out 0, lse -inf and no gradient. lse [batch, heads, queries] fp32. table: [buckets,
- * heads] dense of table_dtype, NULL: none; entries are finite or -inf. Sums and probabilities are fp32. The workspace is 256-byte aligned.
+ * heads] dense of table_dtype, NULL: none; entries are finite or -inf. Sums and probabilities are fp32. The gradient's exponent z - lse
+ * is off by the fp32 rounding of lse, its probabilities by up to 2e-7 |lse|: a query with |lse| of 2^20 or more (one that a bias of
+ * large negative entries leaves nothing else) has no gradient, and sets the device error flag if its dout is not zero. The workspace is
+ * 256-byte aligned.
  * Results do not depend on the run. */
 typedef struct b200_attention {
   int64_t batch, queries, keys, heads, kv_heads, dim, window;

@@ -252,7 +252,12 @@ def op_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None,
 
     Each is dense, in the shape and type of what it is the gradient of, rounded once; the heads that
     share a key head are summed, dtable (None without ``relative_bias``) over batch and positions.
-    Queries and keys behind their sequence's end have zeros. The same from run to run."""
+    Queries and keys behind their sequence's end have zeros. The same from run to run.
+
+    Probabilities exp(z - lse) are off by the fp32 rounding of lse, up to 2e-7 |lse| of each: hide keys by
+    lengths, ``causal``, ``window`` or table entries of -inf rather than by large negative ones. A query whose
+    visible scores are all that large (|lse| >= 2^20) gets no gradient, and sets the device error flag where
+    its row of dout is not zero; a large negative entry beside others is no harm."""
     name = "AttentionGrad"
     a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
     x, y, table = kept[0], kept[1], kept[5]

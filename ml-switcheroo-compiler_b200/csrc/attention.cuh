@@ -41,6 +41,15 @@ struct Sequence {
   }
 };
 
+// The gradient makes p = exp(z - lse) again. lse holds the scores' size and log sum exp(z - max) in 24 bits, so the exponent is off by
+// the roundings of numbers of that size: five of at most 2^-24 each (z, max + log2 sum, to lse, back, the constants), 0.02 at |lse| =
+// 2^16 (p off by 1.2 %), 0.27 at 2^20 (a fifth), hundreds at 1e9. From 2^20 on a row has no probabilities to make again: p = 0, and the
+// error flag is set unless its dout is zero.
+constexpr float LSE_LIMIT = 1048576.f;
+__device__ __forceinline__ bool lse_lost(float lse) { return fabsf(lse) >= LSE_LIMIT && !isinf(lse); }
+// lse in the log2 domain as the gradient takes it away; infinite where there are no probabilities
+__device__ __forceinline__ float exponent_of(float lse) { return lse == -INFINITY || lse_lost(lse) ? INFINITY : lse * LOG2E; }
+
 // a table entry in the log2 domain; what is finite stays finite
 __device__ __forceinline__ float table_log2(const void* table, int64_t at, int dtype) {
   const float v = dtype == B200_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(table)[at]) : reinterpret_cast<const float*>(table)[at];

@@ -201,8 +201,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : (MMA ? 4 : 3))
   float before = 0.f, after = 0.f;          // DQ with a table: sums of dz at rel <= -far, >= far
   if (MODE == DQ && my_in) {
     const int64_t at = (b * a.heads + my_head) * a.queries + my_row;
-    my_lse = io.lse[at] * LOG2E;
-    if (my_lse == -INFINITY) my_lse = INFINITY;  // sees nothing: p = 0
+    my_lse = exponent_of(io.lse[at]);
     my_delta = -io.delta[(b * a.heads + my_head) * io.padded + my_row];
   }
   float* sp = s_p + warp * AREA;
@@ -417,8 +416,7 @@ __global__ void __launch_bounds__(THREADS, MODE == DKV ? 2 : (MMA ? 4 : 3))
         if constexpr (MODE == DKV) {
           lse = INFINITY, delta = 0.f;
           if (seen) {
-            lse = io.lse[(b * a.heads + head) * a.queries + i] * LOG2E;
-            if (lse == -INFINITY) lse = INFINITY;
+            lse = exponent_of(io.lse[(b * a.heads + head) * a.queries + i]);
             delta = -io.delta[(b * a.heads + head) * io.padded + i];
           }
         }

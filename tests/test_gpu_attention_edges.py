@@ -54,3 +54,54 @@ def test_windows_that_hide_nothing(nq, nk, causal, dtype, dim, monkeypatch):
         assert all(torch.equal(a, b) for a, b in zip(got, want)), window
         again = op("AttentionGrad", do, q, k, v, *want, causal=causal, window=window)
         assert all(torch.equal(a, b) for a, b in zip(again[:3], grads[:3])), window
+
+
+@pytest.mark.parametrize("low", [-1e7, -1e9, torch.finfo(BF).min])
+@pytest.mark.parametrize("dtype,dim,nq", [(BF, 64, 70), (BF, 128, 70), (F32, 64, 70), (BF, 160, 70), (BF, 64, 9)])
+def test_rows_whose_lse_cannot_tell_their_keys_apart(dtype, dim, nq, low):
+    """A bias that leaves the first query nothing but entries of a large negative value: without a gradient of its own the step is
+    right and no flag is set; with one its row is left out and the flag says so. Rows that see other keys are not touched."""
+    from b200 import _lib as L
+
+    q, k, v, do = inputs(2, nq, nq, 4, 2, dim, dtype)
+    table = rand(16, 4, dtype=dtype, seed=9)
+    table[0] = low  # distance 0: all that the first query of a causal sequence sees
+    kw = {"relative_bias": table, "causal": True, "max_distance": 30}
+    out, lse = op("Attention", q, k, v, **kw)
+    assert (lse[:, :, 0] < -(2**20)).all() and (lse[:, :, 1:].abs() < 100).all()
+    quiet = do.clone()
+    quiet[:, 0] = 0
+    L.lib().b200_check_device_error(None)
+    want = op("AttentionGrad", quiet, q, k, v, out, lse, **kw)
+    assert L.lib().b200_check_device_error(None) == L.OK
+    wrong = check_gradients(want, (q, k, v, quiet), table)
+    assert not wrong, wrong
+    got = op("AttentionGrad", do, q, k, v, out, lse, **kw)
+    assert L.lib().b200_check_device_error(None) == L.ERR_ARG
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and not got[0][:, 0].any()
+
+
+def check_gradients(grads, operands, table):
+    import rounding_norms as N
+
+    q, k, v, do = (t.cpu() for t in operands)
+    ref, var = N.attention_noise(q, k, v, do, table=table.cpu(), causal=True, far=30)
+    off = {n: N.attention_off(n, t, ref, var) for n, t in zip(("dq", "dk", "dv", "dtable"), grads)}
+    return {n: t for n, t in off.items() if t}
+
+
+@pytest.mark.parametrize("dtype,dim,nq", [(BF, 64, 70), (F32, 64, 70)])
+def test_large_biases_below_that_have_their_gradient(dtype, dim, nq):
+    """-65536 for every key: the exponent is off by five roundings, p by 1.2 % at most, and no flag is set."""
+    from b200 import _lib as L
+
+    q, k, v, do = inputs(1, nq, nq, 2, 2, dim, dtype)
+    q = q * 0  # the scores are the bias alone, so that 64 bits have the same ones
+    table = torch.full((16, 2), -65536.0, dtype=dtype, device="cuda")
+    kw = {"relative_bias": table, "max_distance": 30}
+    L.lib().b200_check_device_error(None)
+    out, lse = op("Attention", q, k, v, **kw)
+    dv = op("AttentionGrad", do, q, k, v, out, lse, **kw)[2].cpu().double()
+    assert L.lib().b200_check_device_error(None) == L.OK
+    want = do.cpu().double().mean(1, keepdim=True).expand(-1, nq, -1, -1)
+    assert ((dv - want).norm() / want.norm()) < 0.012 + 2.0**-8
