@@ -65,10 +65,11 @@ __device__ __forceinline__ int column(int i) {
   else return i * (int)blockDim.x + (int)threadIdx.x;
 }
 
-// 16 bytes that are read once: not kept in the L1
+// 16 bytes that are read once: not kept in the L1. An ordinary load in its place among the stores: results may lie over the arrays
+// that are read here (a row's elements are read by the thread that writes them, before it does).
 __device__ __forceinline__ uint4 load_once(const void* p) {
   uint4 u;
-  asm("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p));
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "l"(p) : "memory");
   return u;
 }
 __device__ __forceinline__ void widen(const uint4& u, float* o) {
