@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200
   const int queries = Sequence(a, b).queries;
   constexpr int V = 16 / sizeof(T);
   float s[FOUR], e[FOUR];
-  uint32_t h[FOUR], i[FOUR], lost = 0;
+  uint32_t h[FOUR], i[FOUR];
   const T *x[FOUR], *y[FOUR];
 #pragma unroll
   for (int n = 0; n < FOUR; ++n) {
@@ -69,11 +69,7 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200
     // a row that is none reads the last one's: no load waits behind a branch
     const int64_t at = min(i[n], (uint32_t)max(queries - 1, 0));
     x[n] = dout + b * sb + at * ss + h[n] * sh, y[n] = out + ((b * a.queries + at) * heads + h[n]) * dim;
-    if (queries > 0) {
-      const float l = lse[(b * heads + h[n]) * a.queries + at];
-      e[n] = -exponent_of(l);
-      lost |= (uint32_t)lse_lost(l) << n;
-    }
+    if (queries > 0) e[n] = lse[(b * heads + h[n]) * a.queries + at] * -LOG2E;
   }
   if (queries > 0) {
     for (int c = lane * V; c < dim; c += 8 * V) {
@@ -93,18 +89,18 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200
       }
     }
   }
-  if (lost) {
 #pragma unroll
-    for (int n = 0; n < FOUR; ++n)
-      if ((lost >> n & 1) && (int)i[n] < queries) {
+  for (int n = 0; n < FOUR; ++n)
+    if ((int)i[n] >= queries) {
+      e[n] = -INFINITY, s[n] = 0.f;
+    } else if (fabsf(e[n]) >= LSE_LIMIT) {  // as exponent_of
+      if (!isinf(e[n])) {
         bool any = false;
         for (int c = lane; c < dim; c += 8) any |= (float)x[n][c] != 0.f;
         if (any) raise_device_error(B200_ERR_ARG);
       }
-  }
-#pragma unroll
-  for (int n = 0; n < FOUR; ++n)
-    if ((int)i[n] >= queries) e[n] = -INFINITY, s[n] = 0.f;
+      e[n] = -INFINITY;
+    }
 #pragma unroll
   for (int n = 0; n < FOUR; ++n) {
 #pragma unroll

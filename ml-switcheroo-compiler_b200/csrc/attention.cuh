@@ -45,10 +45,12 @@ struct Sequence {
 // the roundings of numbers of that size: five of at most 2^-24 each (z, max + log2 sum, to lse, back, the constants), 0.02 at |lse| =
 // 2^16 (p off by 1.2 %), 0.27 at 2^20 (a fifth), hundreds at 1e9. From 2^20 on a row has no probabilities to make again: p = 0, and the
 // error flag is set unless its dout is zero.
-constexpr float LSE_LIMIT = 1048576.f;
-__device__ __forceinline__ bool lse_lost(float lse) { return fabsf(lse) >= LSE_LIMIT && !isinf(lse); }
+constexpr float LSE_LIMIT = 1048576.f * LOG2E;  // in the log2 domain
 // lse in the log2 domain as the gradient takes it away; infinite where there are no probabilities
-__device__ __forceinline__ float exponent_of(float lse) { return lse == -INFINITY || lse_lost(lse) ? INFINITY : lse * LOG2E; }
+__device__ __forceinline__ float exponent_of(float lse) {
+  const float x = lse * LOG2E;
+  return fabsf(x) >= LSE_LIMIT ? INFINITY : x;
+}
 
 // a table entry in the log2 domain; what is finite stays finite
 __device__ __forceinline__ float table_log2(const void* table, int64_t at, int dtype) {
