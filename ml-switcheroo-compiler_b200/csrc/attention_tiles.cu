@@ -64,21 +64,28 @@ struct Place {
 
 // Bounded wait of whoever calls it. A look at the timer takes longer than a tile's MMAs, so it comes every 256 polls. After
 // WAIT_LIMIT_NS the block gives up: every later wait ends at once, results are not valid, the error flag says so.
+__device__ __forceinline__ bool given_up(const int* gave_up) { return *reinterpret_cast<const volatile int*>(gave_up) != 0; }
+template <bool EVEN_THEN = false>
 __device__ __forceinline__ void wait(uint64_t* bar, uint32_t parity, int* gave_up) {
   unsigned long long t0 = 0;
   while (true) {
 #pragma unroll 1
-    for (int k = 0; k < 256; ++k)
+    for (int k = 0; k < 256; ++k) {
       if (mbar_try_wait(bar, parity)) return;
-    if (*reinterpret_cast<volatile int*>(gave_up)) return;
+      if (!EVEN_THEN && given_up(gave_up)) return;
+    }
     const unsigned long long now = globaltimer();
     if (t0 == 0) t0 = now;
     else if (now - t0 > WAIT_LIMIT_NS) {
       raise_device_error(B200_ERR_TIMEOUT);
       *reinterpret_cast<volatile int*>(gave_up) = 1;
+      return;
     }
   }
 }
+// for what is in flight when a block ends (copies into its shared memory, its MMAs): waited for even by a block that has given up,
+// with a limit of its own
+__device__ __forceinline__ void settle(uint64_t* bar, uint32_t parity, int* gave_up) { wait<true>(bar, parity, gave_up); }
 // by all lanes, together again behind it (61 clocks where it is satisfied; one polling lane and the others' wait for it 136)
 __device__ __forceinline__ void warp_wait(uint64_t* bar, uint32_t parity, int* gave_up) {
   wait(bar, parity, gave_up);
@@ -306,24 +313,27 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     if (lane == 0 && n_tiles > 0) {
       mbar_expect_tx(q_full, F::Q);
       for (int p = 0; p < DP / 64; ++p) tma_load_4d(smem + p * (ROWS * 128), &map_q, q_full, p * 64, r0, head, (int)b);
+      int keys = 0, values = 0;  // tiles under way: none into a stage that a block which gave up may still read or fill
       for (int n = 0; n < n_tiles; ++n) {
         const int s = n % ST;
         const uint32_t par = ((n / ST) & 1) ^ 1;
         wait(&k_empty[s], par, gave_up);
+        if (given_up(gave_up)) break;
+        ++keys;
         mbar_expect_tx(&k_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
           tma_load_4d(smem + F::Q + s * F::TILE + p * (KEYS * 128), &map_k, &k_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
         wait(&v_empty[s], par, gave_up);
+        if (given_up(gave_up)) break;
+        ++values;
         mbar_expect_tx(&v_full[s], F::TILE);
         for (int p = 0; p < DP / 64; ++p)
           tma_load_4d(smem + F::Q + (ST + s) * F::TILE + p * (KEYS * 128), &map_v, &v_full[s], p * 64, (T0 + n) * KEYS, kvh, (int)b);
       }
       // every load has landed before the block may end
-      wait(q_full, 0, gave_up);
-      for (int m = max(0, n_tiles - ST); m < n_tiles; ++m) {
-        wait(&k_full[m % ST], (m / ST) & 1, gave_up);
-        wait(&v_full[m % ST], (m / ST) & 1, gave_up);
-      }
+      settle(q_full, 0, gave_up);
+      for (int m = max(0, keys - ST); m < keys; ++m) settle(&k_full[m % ST], (m / ST) & 1, gave_up);
+      for (int m = max(0, values - ST); m < values; ++m) settle(&v_full[m % ST], (m / ST) & 1, gave_up);
     }
   } else if (warp == 1) {
     const int ks = (dim + 15) / 16, elected = elect_one();
@@ -365,7 +375,8 @@ __global__ void __launch_bounds__(FWD_THREADS, 2)
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
-    warp_wait(idle, 0, gave_up);
+    settle(idle, 0, gave_up);
+    __syncwarp();
   } else {
     const int q = warp & 3;
     const int i0 = r0 + q * 32, i = i0 + lane;
@@ -622,9 +633,11 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
         tma_load_4d(smem + G::X + p * (ROWS * 128), &map_x1, x_full, p * 64, r0, xh, (int)b);
       }
       Step x = start();
-      for (int n = 0; n < total; ++n, advance(x)) {
+      int n = 0;  // tiles under way, as in the forward
+      for (; n < total; ++n, advance(x)) {
         const int s = x.stage, token = token_of(x), yh = DKV ? x.head : kvh;
         wait(&y_empty[s], x.parity ^ 1, gave_up);
+        if (given_up(gave_up)) break;
         mbar_expect_tx(&y_full[s], 2 * G::Y + (DKV ? 2 * BN * 4 : 0));
         for (int p = 0; p < DP / 64; ++p) {
           uint8_t* y = smem + 2 * G::X + s * 2 * G::Y + p * (BN * 128);
@@ -638,8 +651,8 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
         }
       }
       // every load has landed before the block may end
-      wait(x_full, 0, gave_up);
-      for (int m = max(0, total - ST); m < total; ++m) wait(&y_full[m % ST], (m / ST) & 1, gave_up);
+      settle(x_full, 0, gave_up);
+      for (int m = max(0, n - ST); m < n; ++m) settle(&y_full[m % ST], (m / ST) & 1, gave_up);
     }
   } else if (warp == 1) {
     const int ks = (dim + 15) / 16, elected = elect_one();
@@ -699,7 +712,8 @@ __global__ void __launch_bounds__(Bwd<DP, DKV, BIAS>::THREADS, DP == 64 ? 2 : 1)
     }
     // no MMA and no commit is on its way when the block ends
     commit(elected, idle);
-    warp_wait(idle, 0, gave_up);
+    settle(idle, 0, gave_up);
+    __syncwarp();
   } else {
     const int g = (warp - 2) >> 3, half = ((warp - 2) >> 2) & 1, q = warp & 3;
     const int w0 = r0 + q * 32, r = w0 + lane;
