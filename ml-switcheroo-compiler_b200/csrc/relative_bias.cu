@@ -80,7 +80,7 @@ __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 struct GradShape {
-  int rows, runs, wide, pieces;  // rows a run, runs, diagonals a piece, pieces
+  int rows, runs, pieces;  // rows a run, runs, pieces of WIDE diagonals
 };
 constexpr int WIDE = 2048;
 static GradShape grad_shape(int64_t heads, int64_t queries, int64_t keys) {
@@ -90,7 +90,6 @@ static GradShape grad_shape(int64_t heads, int64_t queries, int64_t keys) {
   while (rows < 64 && heads * ceil_div(queries, 2 * rows) >= 8 * (int64_t)num_sms()) rows *= 2;
   g.rows = (int)std::min<int64_t>(rows, queries);
   g.runs = (int)ceil_div(queries, g.rows);
-  g.wide = WIDE;
   g.pieces = (int)ceil_div(keys + g.rows - 1, WIDE);
   return g;
 }
