@@ -732,7 +732,9 @@ typedef struct b200_attention_grads {
 } b200_attention_grads;
 size_t b200_attention_workspace_bytes(const b200_attention* a);
 int b200_attention_forward(const b200_attention* a, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
-size_t b200_attention_grad_workspace_bytes(const b200_attention* a);
+size_t b200_attention_grad_workspace_bytes(const b200_attention* a); /* for any dout */
+/* for the dout (pointer and strides) of g: without room for a copy of it where none is needed */
+size_t b200_attention_grad_workspace_bytes_of(const b200_attention* a, const b200_attention_grads* g);
 int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus

@@ -217,6 +217,7 @@ SIGNATURES = {
     "b200_attention_workspace_bytes": ([C.POINTER(Attention)], C.c_size_t),
     "b200_attention_forward": ([C.POINTER(Attention), _P, _P, _P, C.c_size_t, _P], C.c_int),
     "b200_attention_grad_workspace_bytes": ([C.POINTER(Attention)], C.c_size_t),
+    "b200_attention_grad_workspace_bytes_of": ([C.POINTER(Attention), C.POINTER(AttentionGrads)], C.c_size_t),
     "b200_attention_grad": ([C.POINTER(Attention), C.POINTER(AttentionGrads), _P, C.c_size_t, _P], C.c_int),
     "b200_conv2d_fwd": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),
     "b200_conv2d_dgrad": ([_I32, _P, _P, _P] + [_I64] * 13 + [_P], C.c_int),

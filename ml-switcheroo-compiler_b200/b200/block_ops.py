@@ -276,7 +276,7 @@ def op_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None,
     dtable = None if table is None else table.new_empty(table.shape)
     g.dout, g.out, g.lse, g.dout_stride[:] = dout.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.stride()[:3]
     g.dq, g.dk, g.dv, g.dtable = dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ops._ptr(dtable)
-    wn = L.lib().b200_attention_grad_workspace_bytes(a)
+    wn = L.lib().b200_attention_grad_workspace_bytes_of(a, g)
     ws = x.new_empty(wn, dtype=torch.uint8) if wn else None
     L.call("b200_attention_grad", a, g, ops._ptr(ws), wn, ops.stream_ptr())
     return (dq[0], dk[0], dv[0], dtable) if flat else (dq, dk, dv, dtable)

@@ -113,7 +113,6 @@ __global__ void __launch_bounds__(256) delta_kernel(const __grid_constant__ b200
   }
 }
 
-static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
 static int64_t padded_of(const b200_attention& a) { return ceil_div(a.queries, 128) * 128; }
 static size_t delta_bytes(const b200_attention& a) { return (size_t)(2 * a.batch * a.heads * padded_of(a)) * sizeof(float); }
 
@@ -139,10 +138,11 @@ extern "C" int b200_attention_forward(const b200_attention* a, void* out, float*
   return tiles_take(own) ? tiles_forward(own, out, lse, workspace, as_stream(stream)) : rows_forward(own, out, lse, workspace, as_stream(stream));
 }
 
-extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) {
+extern "C" size_t b200_attention_grad_workspace_bytes_of(const b200_attention* a, const b200_attention_grads* g) {
   if (check_attention("attention_grad", a) || a->batch == 0) return 0;
-  return delta_bytes(*a) + (tiles_take_grad(*a) ? tiles_grad_workspace(*a, nullptr) : rows_grad_workspace(*a));
+  return delta_bytes(*a) + (tiles_take_grad(*a) ? tiles_grad_workspace(*a, g) : rows_grad_workspace(*a));
 }
+extern "C" size_t b200_attention_grad_workspace_bytes(const b200_attention* a) { return b200_attention_grad_workspace_bytes_of(a, nullptr); }
 
 extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention_grads* g, void* workspace, size_t workspace_bytes,
                                    void* stream) {
@@ -162,7 +162,7 @@ extern "C" int b200_attention_grad(const b200_attention* a, const b200_attention
     return check_launch("attention_grad");
   }
   B200_REQUIRE(g->dout && g->out && g->lse && g->dq && g->dk && g->dv, "attention_grad: null operand");
-  const size_t need = b200_attention_grad_workspace_bytes(a);
+  const size_t need = b200_attention_grad_workspace_bytes_of(a, g);
   B200_REQUIRE(workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0,
                "attention_grad: workspace of %zu bytes, %zu needed on a 256-byte boundary", workspace_bytes, need);
   const b200_attention own = within(*a);

@@ -72,7 +72,7 @@ bool tiles_take(const b200_attention& a);       // whether they make the forward
 bool tiles_take_grad(const b200_attention& a);  // and the gradient
 size_t tiles_forward_workspace(const b200_attention& a);
 int tiles_forward(const b200_attention& a, void* out, float* lse, void* workspace, cudaStream_t st);
-size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads* g);
+size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads* g);  // g NULL: for any dout
 // lse2 (log2) and delta: [batch x heads][padded], both negated (so that a query that sees nothing, or is none, has p = 2^-inf),
 // padded a multiple of 128
 int tiles_grad(const b200_attention& a, const b200_attention_grads& g, const float* lse2, const float* delta, int64_t padded, void* workspace,

@@ -1054,7 +1054,7 @@ static size_t part_bytes(const b200_attention& a) {
 
 size_t tiles_grad_workspace(const b200_attention& a, const b200_attention_grads* g) {
   using namespace tiles;
-  // the gradient's own strides are not known to a caller who asks for the size: room for its copy
+  // a caller who does not say where dout is gets room for its copy
   const size_t d = g ? packed_bytes(a, operand(g->dout, a.queries, a.heads, g->dout_stride)) : up256((size_t)(a.batch * a.queries * a.heads * wide_of(a)) * 2);
   return part_bytes(a) + tiles_forward_workspace(a) + d;
 }

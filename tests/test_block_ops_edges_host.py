@@ -33,3 +33,22 @@ def test_a_shift_is_not_taken_for_another_one(shift):
     with pytest.raises(ValueError):
         block_ops.op_relative_position_bias_grad(torch.zeros(2, 3, 4), buckets=32, shift=shift)
     assert block_ops._shift("RelativePositionBias", 2**29 - 1, 3, 4) == 2**29 - 1 and block_ops._shift("RelativePositionBias", None, 3, 4) == 1
+
+
+def test_the_gradients_workspace_has_a_copy_of_dout_only_where_one_is_made():
+    from b200 import _lib as L
+
+    lib, a, g = L.load(), L.Attention(), L.AttentionGrads()
+    a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim, a.scale, a.dtype = 2, 100, 120, 4, 2, 64, 1.0, L.BF16
+    a.q = a.k = a.v = 4096
+    a.q_stride[:] = 100 * 256, 256, 64
+    a.k_stride[:] = a.v_stride[:] = 120 * 128, 128, 64
+    copy = 2 * 100 * 4 * 64 * 2
+    most = lib.b200_attention_grad_workspace_bytes(a)
+    g.dout, g.dout_stride[:] = 4096, (100 * 256, 256, 64)
+    assert lib.b200_attention_grad_workspace_bytes_of(a, g) == most - copy
+    for pointer, strides in ((4098, (100 * 256, 256, 64)), (4096, (100 * 260, 260, 65)), (4096, (0, 256, 64))):
+        g.dout, g.dout_stride[:] = pointer, strides
+        assert lib.b200_attention_grad_workspace_bytes_of(a, g) == most
+    a.dim = 0
+    assert lib.b200_attention_grad_workspace_bytes_of(a, g) == 0 and lib.b200_attention_grad_workspace_bytes_of(None, g) == 0

@@ -105,3 +105,31 @@ def test_large_biases_below_that_have_their_gradient(dtype, dim, nq):
     assert L.lib().b200_check_device_error(None) == L.OK
     want = do.cpu().double().mean(1, keepdim=True).expand(-1, nq, -1, -1)
     assert ((dv - want).norm() / want.norm()) < 0.012 + 2.0**-8
+
+
+@pytest.mark.parametrize("dtype,dim", [(BF, 64), (BF, 100), (F32, 64)])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_gradient_stays_in_the_workspace_of_its_dout(dtype, dim, shift, monkeypatch):
+    """dout aligned (read in place) and not (copied): what lies behind the workspace is left as it was."""
+    from b200 import _lib as L
+
+    q, k, v, do = inputs(2, 70, 90, 4, 2, dim, dtype)
+    table = rand(32, 4, seed=9)
+    kw = {"causal": True, "relative_bias": table}
+    out, lse = op("Attention", q, k, v, **kw)
+    want = op("AttentionGrad", do, q, k, v, out, lse, **kw)
+    flat = torch.zeros(do.numel() + shift, dtype=dtype, device="cuda")
+    moved = flat[shift:].view(do.shape).copy_(do)
+    spaces, call = [], L.call
+
+    def guarded(name, *args):
+        if name == "b200_attention_grad":
+            a, g, _, n, stream = args
+            spaces.append(torch.full((n + 4096,), 0x5A, dtype=torch.uint8, device="cuda"))
+            args = (a, g, spaces[0].data_ptr(), n, stream)
+        return call(name, *args)
+
+    monkeypatch.setattr(L, "call", guarded)
+    got = op("AttentionGrad", moved, q, k, v, out, lse, **kw)
+    assert len(spaces) == 1 and (spaces[0][-4096:] == 0x5A).all()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
