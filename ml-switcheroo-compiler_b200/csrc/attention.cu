@@ -16,7 +16,8 @@ static int check_attention(const char* what, const b200_attention* a) {
   B200_REQUIRE(a->queries * (a->heads / a->kv_heads) < (1ll << 30), "%s: %lld queries times %lld heads a key head reach 2^30", what,
                (long long)a->queries, (long long)(a->heads / a->kv_heads));
   B200_REQUIRE(a->dim >= 1 && a->dim <= 256, "%s: dim %lld (1 to 256)", what, (long long)a->dim);
-  B200_REQUIRE(a->scale > 0 && a->scale < 3e38f, "%s: scale %g is not a positive number", what, (double)a->scale);
+  // the kernels multiply by scale log2 e, which has to be a number too
+  B200_REQUIRE(a->scale > 0 && a->scale < 3.402823466e38f / LOG2E, "%s: scale %g is not a positive number below 2.3e38", what, (double)a->scale);
   B200_REQUIRE(a->window >= 0, "%s: window %lld", what, (long long)a->window);
   if (a->dtype != B200_F32 && a->dtype != B200_BF16) {
     set_error("%s: dtype %d (F32 and BF16)", what, a->dtype);

@@ -52,3 +52,13 @@ def test_the_gradients_workspace_has_a_copy_of_dout_only_where_one_is_made():
         assert lib.b200_attention_grad_workspace_bytes_of(a, g) == most
     a.dim = 0
     assert lib.b200_attention_grad_workspace_bytes_of(a, g) == 0 and lib.b200_attention_grad_workspace_bytes_of(None, g) == 0
+
+
+@pytest.mark.parametrize("scale,fine", [(2.3e38, True), (2.4e38, False), (2.9e38, False), (1e-45, True)])
+def test_a_scale_stays_a_number_in_the_log2_domain(scale, fine):
+    """Above 2.35e38 scale log2 e is infinite, and a score of zero was not a number."""
+    from b200 import _lib as L
+
+    lib, a = L.load(), L.Attention()
+    a.batch, a.queries, a.keys, a.heads, a.kv_heads, a.dim, a.scale = 0, 4, 4, 2, 1, 64, scale
+    assert lib.b200_attention_forward(a, None, None, None, 0, None) == (L.OK if fine else L.ERR_ARG)
