@@ -704,8 +704,10 @@ int b200_relative_bias_grad(const b200_relative* r, int dtype, const void* dbias
  * [batch, keys, kv_heads, dim], of one dtype, F32 or BF16; heads is a multiple of kv_heads (head h
  * reads key head h / (heads / kv_heads)); dim <= 256. Inputs have element strides {batch, token,
  * head} and adjacent elements in a head; results are dense. lengths / query_lengths [batch]
- * (length_dtype I32 or I64, NULL: all) cut each sequence's keys and queries at its end; nothing
- * behind is read; one outside [0, keys] ([0, queries]) is clamped and sets the device error flag.
+ * (length_dtype I32 or I64, NULL: all) cut each sequence's keys and queries at its end; what lies behind
+ * (it has to be addressable) may be anything; one outside [0, keys] ([0, queries]) is clamped and sets the
+ * device error flag. Inside the lengths a key that a mask hides from a query is a factor of zero: what is
+ * not finite there may make that query's results NaN, as in a product.
  * Query i is at position i + shift, shift = the sequence's keys - its queries: its last query at its last key.
  * causal: keys behind that position are hidden; window > 0: so are those at `window` or more
  * before it (and, not causal, behind it). A query that sees nothing, or behind its sequence's

@@ -225,15 +225,16 @@ def op_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=None, 
     shape and type; lse fp32 [batch, heads, queries].
 
     ``lengths`` and ``query_lengths`` (integers [batch]) end each sequence's keys and queries: a padded
-    batch, or a cache that is not full. Nothing behind them is read. The last query is at the last key's
-    position: query i at i + keys - queries of its sequence. ``causal`` hides the keys behind a
+    batch, or a cache that is not full. What lies behind them may be anything, NaN too; keys and values inside
+    are finite (one that a mask hides is still a factor of zero). The last query is at the last key's position: query i at i + keys - queries of its sequence. ``causal`` hides the keys behind a
     query's position, ``window`` w those w or more before it (and, not causal, behind it). A query that
     sees nothing has out 0 and lse -inf. ``relative_bias`` [buckets, heads]: the table of
     RelativePositionBias, added to the scores by the positions' difference (``bidirectional``: not
     causal by default); entries finite or -inf.
 
     Scores, their maxima and sums are fp32; bf16 heads round the probabilities to bf16 for their
-    product with the values. Keep ``lse`` and ``out`` for AttentionGrad."""
+    product with the values, whatever ``Config.matmul_dtype`` is: cast heads to fp32 for fp32 products. Keep
+    ``lse`` and ``out`` for AttentionGrad."""
     name = "Attention"
     a, kept, flat = _describe(name, q, k, v, lengths, query_lengths, relative_bias, scale, causal, window, max_distance, bidirectional)
     x = kept[0]
@@ -252,7 +253,9 @@ def op_attention_grad(dout, q, k, v, out, lse, lengths=None, query_lengths=None,
 
     Each is dense, in the shape and type of what it is the gradient of, rounded once; the heads that
     share a key head are summed, dtable (None without ``relative_bias``) over batch and positions.
-    Queries and keys behind their sequence's end have zeros. The same from run to run.
+    Queries and keys behind their sequence's end have zeros. The same from run to run. bf16 heads round the
+    probabilities and the scores' gradients to bf16 for their products, and ``out`` is the rounded one (so is
+    dout . out of each query, of which an fp32 table's gradient is off as well).
 
     Probabilities exp(z - lse) are off by the fp32 rounding of lse, up to 2e-7 |lse| of each: hide keys by
     lengths, ``causal``, ``window`` or table entries of -inf rather than by large negative ones. A query whose

@@ -13,8 +13,10 @@
 // bf16 queries (rows of whole 16 bytes) make their scores by mma.sync instead, 8 tokens a step, whose operands a lane loads as
 // they are: without the sums over lanes and the conversions of K a step has half the instructions.
 // What bounds it: for single tokens latency and issue on the way to HBM (32 caches of 4096 places, 32 + 8 heads of 128 bf16: 96 us, 4.2
-// TB/s; 661 us with loads that waited behind branches, 132 without mma.sync), else the FMA pipe's issue slots
-// (2 x 777 tokens, 8 heads of 80 fp32: forward 190, dq 259, dk and dv 323 us).
+// TB/s; 661 us with loads that waited behind branches, 132 without mma.sync), else issue: of 2 x 777 tokens, 8 heads of 80 fp32 the
+// forward takes 190, dq 257, dk and dv 322 us, with 61, 59 and 54 % of the issue slots in use but the FMA pipe only for 34, 33 and
+// 34 %. The rest are the sums over lanes (31 exchanges and 62 selects for 32 scores, twice in the gradients), the probabilities' way
+// through shared memory, and 48 of 128 lanes' elements behind a head of 80. Heads above 128 spill: 168 to 1360 bytes a thread.
 #include <algorithm>
 
 #include "attention.cuh"

@@ -7,7 +7,7 @@
 //   warps 2-5   softmax, a row of S a thread.
 // Tiles of 64 keys: two S take turns, P lies over its S (bf16 in the lower half), O has the rest (64 + 64 + 128 columns), so that the
 // next tile's S is made under this one's exponentials. MMAs run in their order: an S is overwritten only when the P over it is used up.
-// (One S of 128 keys with P over it, whose successor waited for P, took 314 us for 2 x 4096 causal tokens of 32 heads of 128, this 272;
+// (One S of 128 keys with P over it, whose successor waited for P, took 314 us for 2 x 4096 causal tokens of 32 heads of 128, this 276;
 // S of 128 keys beside P, with two threads a row that exchange its maximum, 167 us for 64 x 512 tokens of 16 heads of 64, this 151.)
 // The running maximum moves only when a row's has grown by 2^8 (probabilities stay below 2^8, sums are fp32), so O is hardly ever
 // rescaled.
@@ -20,11 +20,13 @@
 // from, and are the A operand of the sums there: nothing is transposed, no sum leaves its block, every order is fixed. S and
 // dP are made twice for that (7 products instead of 5). Two warpgroups share a tile, 32 columns each (one for all 64 took as long).
 // Heads of up to 64: 256 columns of TMEM a block and two blocks an SM; wider heads: two pairs of warpgroups that take tiles in turn,
-// each with an S and dP of its own (one pair: 739 us for 4 x 2048 tokens of 16 heads of 128, two: 542).
+// each with an S and dP of its own (one pair: 739 us for 4 x 2048 tokens of 16 heads of 128, two: 537).
 // Tiles of 64 because of TMEM; an MMA of 128 x 64 from shared memory takes 48 clocks, of 128 x 128 64 (measured).
-// What bounds both directions is the chain of a tile, with two tiles under way on an SM: the tensor pipe is active for 29 to 35 % of
-// the time, the special function unit for 29 to 61 %, issue slots for 40 to 47 % (8 x 2048 tokens of 16 heads of 64: forward 217,
-// gradients 741 us).
+// dk and dv are capped at 96 registers (two blocks of 10 warps or one of 18: five warps to a quarter of an SM) and spill 84 to 116 bytes
+// a thread, dq of heads of 64 with a bias 56.
+// What bounds both directions is the chain of a tile, with two tiles under way on an SM: the tensor pipe is active for 29 to 36 % of
+// the time, the special function unit for 29 to 62 %, issue slots for 40 to 46 % (8 x 2048 tokens of 16 heads of 64: forward 216, dq 274,
+// dk and dv 441 us).
 //
 // Probabilities and dz are rounded to bf16 for the products that they are operands of; scores, maxima, sums and
 // all accumulators are fp32. Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
@@ -1020,11 +1022,11 @@ static int launch_backward(const b200_attention& a, const Operand (&x)[2], const
 
 bool tiles_take_grad(const b200_attention& a) { return a.dtype == B200_BF16 && a.dim <= 128 && a.queries >= 16 && a.keys >= 1; }
 
-// Forward, the row kernels split long keys over the SMs, which a tile's block walks alone (0.7 us for 64 keys). They take few queries
-// over 2048 keys or more, while queries x heads x elements stay below 75000. Measured, rows against tiles: 16 queries of 8 heads of
-// 64 over 2048 keys 24 and 28 us, 64 queries 29 and 27; over 16384 keys 64 queries 90 and 177 us, 128 queries 167 and 178, 256
-// queries 312 and 178; 32 + 8 heads of 128 over 16384 keys, 16 queries 142 and 213, 32 queries 264 and 207; 16 queries of 4 x 32
-// heads of 128 over 4096 keys 158 and 56.
+// Forward, the row kernels split long keys over the SMs, which a tile's block walks alone (0.6 us for 64 keys). They take few queries
+// over 2048 keys or more, while queries x heads x elements stay below 75000. Measured, kernels of rows (with the join) against tiles:
+// 16 queries of 8 heads of 64 over 2048 keys 12.5 and 24.9 us, 64 queries 28.7 and 25.2, 128 queries 39 and 26; calls over 16384 keys,
+// 16 queries 45 and 168 us, 64 queries 90 and 168, 128 queries 167 and 168, 256 queries 312 and 168; 32 + 8 heads of 128 over 16384
+// keys, 16 queries 143 and 218, 32 queries 264 and 210; 16 queries of 4 x 32 heads of 128 over 4096 keys 158 and 55.
 bool tiles_take(const b200_attention& a) {
   return tiles_take_grad(a) && (a.keys < 2048 || a.batch * a.heads * a.queries * a.dim >= 75000);
 }
