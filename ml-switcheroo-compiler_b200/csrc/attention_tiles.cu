@@ -28,8 +28,10 @@
 // the time, the special function unit for 29 to 62 %, issue slots for 40 to 46 % (8 x 2048 tokens of 16 heads of 64: forward 216, dq 274,
 // dk and dv 441 us).
 //
-// Probabilities and dz are rounded to bf16 for the products that they are operands of; scores, maxima, sums and
-// all accumulators are fp32. Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
+// Probabilities and dz are rounded to bf16 for the products that they are operands of: both operands of an MMA have one type, the
+// heads', and a second plane for what is lost would double those products, against an error of 2.0e-3 (outputs) to 2.9e-3 (gradients)
+// where the results' own rounding is 1.7e-3. Scores, maxima, sums and all accumulators are fp32; exponentials are ex2.approx, whose
+// error of 2^-22 is far below a bf16 operand's 2^-9 (the row kernels use exp2f, so their bits differ). Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
 // block winds down.
 #include <algorithm>
 
