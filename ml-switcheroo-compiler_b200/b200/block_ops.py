@@ -76,7 +76,7 @@ def op_relative_position_bias(table, queries=None, keys=None, bidirectional=True
     table [buckets, heads], fp32 or bf16. Half of the buckets (of each side, ``bidirectional``: keys
     behind the query use the second half; else they share the first bucket) hold one distance each,
     the others equal steps of the logarithm up to ``max_distance`` (``relative_bucket_starts``).
-    ``shift``: keys - queries by default, the last query at the last key."""
+    ``shift`` (below 2^29 either way): keys - queries by default, the last query at the last key."""
     name = "RelativePositionBias"
     if table.dim() != 2:
         raise ValueError(f"{name}: table {tuple(table.shape)}, want [buckets, heads]")
@@ -129,7 +129,7 @@ def _tokens(name: str, what: str, x: torch.Tensor) -> torch.Tensor:
 
 
 def _window(name: str, window: Any) -> int:
-    """The window in tokens, 0 for none; what hides nothing at any length is cut to what a C int64 holds."""
+    """The window in tokens, 0 for none; one longer than any sequence is cut, so that it stays itself in C."""
     if window is None:
         return 0
     if not window >= 1 or (window != math.inf and int(window) != window):
@@ -226,7 +226,8 @@ def op_attention(q, k, v, lengths=None, query_lengths=None, relative_bias=None, 
 
     ``lengths`` and ``query_lengths`` (integers [batch]) end each sequence's keys and queries: a padded
     batch, or a cache that is not full. What lies behind them may be anything, NaN too; keys and values inside
-    are finite (one that a mask hides is still a factor of zero). The last query is at the last key's position: query i at i + keys - queries of its sequence. ``causal`` hides the keys behind a
+    are finite (one that a mask hides is still a factor of zero). The last query is at the last key's
+    position: query i at i + keys - queries of its sequence. ``causal`` hides the keys behind a
     query's position, ``window`` w those w or more before it (and, not causal, behind it). A query that
     sees nothing has out 0 and lse -inf. ``relative_bias`` [buckets, heads]: the table of
     RelativePositionBias, added to the scores by the positions' difference (``bidirectional``: not

@@ -49,7 +49,8 @@ static b200_attention within(const b200_attention& a) {
 
 // What the gradient needs of each query beside its own row, negated: delta = dout . out, and lse in the log2 domain, infinite where
 // the query sees nothing, is none or has lost its probabilities (so that p = 0). out is the caller's, rounded to the heads' type: bf16
-// moves all dz of a row by p times one error, and with it an fp32 table's gradient (2.9e-3 of its norm); keeping out in fp32 would double its bytes.
+// moves all dz of a row by p times one error, and with it an fp32 table's gradient (2.9e-3 of its norm); keeping out in fp32 would
+// double its bytes.
 // [batch x heads][padded]; 8 lanes a query, FOUR queries of theirs under way.
 constexpr int FOUR = 4;
 template <typename T>

@@ -31,8 +31,8 @@
 // Probabilities and dz are rounded to bf16 for the products that they are operands of: both operands of an MMA have one type, the
 // heads', and a second plane for what is lost would double those products, against an error of 2.0e-3 (outputs) to 2.9e-3 (gradients)
 // where the results' own rounding is 1.7e-3. Scores, maxima, sums and all accumulators are fp32; exponentials are ex2.approx, whose
-// error of 2^-22 is far below a bf16 operand's 2^-9 (the row kernels use exp2f, so their bits differ). Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the
-// block winds down.
+// error of 2^-22 is far below a bf16 operand's 2^-8 (the row kernels use exp2f, so their bits differ).
+// Every wait is bounded (tc_common.cuh); on expiry the error flag is set and the block winds down.
 #include <algorithm>
 
 #include "attention.cuh"

@@ -20,8 +20,9 @@
 // forward, up to six in the gradient, a barrier each. So many blocks share an SM (registers are capped for it)
 // rather than that a block loads ahead, a thread of the gradient has 16 elements (fewer threads to a barrier, more rows under way),
 // and weights stay in shared memory. Measured: 64 x 512 x 1024 layer norm, fp32 stream, 71 us (141 with the next row loaded early
-// and types looked up at run time), the gradients of 16 x 1000 x 2048 with post norm and gate 124 to 127 us (430; 206 with 8 elements a thread). Most gradients spill: 4 to 416 bytes
-// a thread for whole vectors up to 8192 columns (152 in the measured one), up to 2154 for wider or ragged rows.
+// and types looked up at run time), the gradients of 16 x 1000 x 2048 with post norm and gate 124 to 127 us (430; 206 with 8
+// elements a thread). Most gradients spill: 4 to 416 bytes a thread for whole vectors up to 8192 columns (152 in the measured one), up
+// to 2154 for wider or ragged rows.
 // The weights' gradients are kept per thread over the block's rows (a thread owns columns), go to
 // the workspace once a block, and are added up in a fixed order by a second launch; a gate's
 // gradient whose group one block covers alone is written by that block.
